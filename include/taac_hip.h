@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define TAAC_ABI_VERSION 9
+#define TAAC_ABI_VERSION 10
 
 enum taac_status {
   TAAC_OK = 0,
@@ -108,6 +108,24 @@ int taac_rmsnorm_bwd(const void* x, const void* w, const void* dy, void* dx, voi
                      int64_t workspace_floats, int64_t rows, int32_t cols, float eps, int dtype, void* stream);
 int taac_layernorm_bwd(const void* x, const void* w, const void* dy, void* dx, void* dw, void* db, float* workspace,
                        int64_t workspace_floats, int64_t rows, int32_t cols, float eps, int dtype, void* stream);
+
+/*
+ * RMSNorm of a sum: summed = round(x + residual) in the storage type, y = summed * rsqrt(mean(summed^2) + eps) * w. All tensors
+ * [rows, cols] contiguous, w [cols]. summed may be x or residual. Any cols; whole aligned 16-byte vectors, at most 512 of them a row,
+ * take the vector kernel.
+ * taac_residual_rmsnorm_fp8_fwd: y leaves as e4m3 with a maximum per row instead: row_amax fp32 [rows] = max |y|,
+ * q [rows, cols] = e4m3(y * 448 / row_amax) (maxima below 1e-12 count as 1e-12).
+ * taac_residual_rmsnorm_bwd: dx = dsummed + the gradient of summed through the norm (it is the gradient of x and of the residual),
+ * dw [cols]; dsummed may be NULL (the sum has no gradient of its own). workspace: taac_norm_bwd_workspace_floats(rows, cols, 0)
+ * floats, as taac_rmsnorm_bwd.
+ * Replaces: `x + update` followed by RMSNorm in the reference's blocks (experiments/symbiosis/backbone.py:62-67).
+ */
+int taac_residual_rmsnorm_fwd(const void* x, const void* residual, const void* w, void* summed, void* y, int64_t rows, int32_t cols,
+                              float eps, int dtype, void* stream);
+int taac_residual_rmsnorm_fp8_fwd(const void* x, const void* residual, const void* w, void* summed, void* q, float* row_amax,
+                                  int64_t rows, int32_t cols, float eps, int dtype, void* stream);
+int taac_residual_rmsnorm_bwd(const void* summed, const void* w, const void* dy, const void* dsummed, void* dx, void* dw,
+                              float* workspace, int64_t workspace_floats, int64_t rows, int32_t cols, float eps, int dtype, void* stream);
 
 /*
  * taac_rmsnorm_bwd for callers that cannot allocate device memory (code under HIP graph capture, tight serving loops,
@@ -760,6 +778,12 @@ int taac_quantize_fp8(const void* x, int64_t n, int dtype, const float* amax, vo
 int taac_linear_fp8(const void* a, int a_is_fp8, int64_t lda, const void* w, const float* amax_a, const float* amax_w,
                     const void* bias, const void* residual, void* out, int64_t ldo, int64_t M, int32_t N, int32_t K,
                     int epilogue, int gate_first, void* stream);
+/* taac_linear_fp8 for e4m3 activations with a maximum per row (row_amax fp32 [M], taac_residual_rmsnorm_fp8_fwd): row i is
+ * dequantised with row_amax[i] / 448. */
+int taac_linear_fp8_rows(const void* a, int64_t lda, const void* w, const float* row_amax, const float* amax_w, const void* bias,
+                         const void* residual, void* out, int64_t ldo, int64_t M, int32_t N, int32_t K, int epilogue, int gate_first,
+                         void* stream);
+
 
 /*
  * Fused [RMSNorm ->] FP8 dense layer [-> + residual], the FP8 counterpart of

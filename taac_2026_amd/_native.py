@@ -6,6 +6,7 @@ The library is the only compute backend of this package: if it cannot be loaded 
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -25,7 +26,7 @@ ATTN_CAUSAL, ATTN_REGISTER_STAGING = 1, 2
 BACKBONE_DENSE_TOKENS, BACKBONE_SPLIT_OUT_FFN, BACKBONE_FP8, BACKBONE_ROW_MAJOR_QKV = 1, 2, 4, 8
 FOLDED_NORM, FOLDED_ACTIVATION = 1, 2
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 _DTYPE_CODES = {torch.float32: TAAC_F32, torch.bfloat16: TAAC_BF16, torch.float16: TAAC_F16}
 
@@ -79,6 +80,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "taac_rmsnorm_bwd_static": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float, c_int, c_void_p],
+    ),
+    "taac_residual_rmsnorm_fwd": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float, c_int, c_void_p]),
+    "taac_residual_rmsnorm_fp8_fwd": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float, c_int, c_void_p]),
+    "taac_residual_rmsnorm_bwd": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_float, c_int, c_void_p],
     ),
     "taac_flash_attn_fwd": (
         c_int,
@@ -254,6 +263,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
          c_int32, c_int32, c_int, c_int, c_void_p],
     ),
+    "taac_linear_fp8_rows": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32,
+         c_int, c_int, c_void_p],
+    ),
     "taac_embedding_bag_mean_fwd": (
         c_int,
         [c_void_p, c_int64, c_int32, c_void_p, c_int, c_int64, c_int32, c_void_p, c_void_p, c_int, c_void_p],
@@ -367,6 +381,16 @@ def check(status: int, operator_name: str) -> None:
     raise RuntimeError(f"{operator_name}: {message}")
 
 
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current GPU: a launch goes to the current one, whatever its stream."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NO_GUARD
+    return torch.cuda.device(device)
+
+
 def ptr(tensor: torch.Tensor | None) -> int | None:
     return None if tensor is None else tensor.data_ptr()
 
@@ -396,5 +420,6 @@ __all__ = [
     "dtype_code",
     "library_available",
     "load_library",
+    "on_device",
     "ptr",
 ]

@@ -1159,6 +1159,8 @@ def linear_fp8(
 
     ``x`` is bf16 (quantised on load with scale ``amax_x / 448``) or already ``float8_e4m3fn``;
     ``weight_fp8`` is ``float8_e4m3fn`` ``[out, in]`` quantised with scale ``amax_w / 448``.
+    ``amax_x`` with the shape of x without its last dimension holds one maximum per row of an x that is ``float8_e4m3fn``
+    already (:func:`residual_rms_norm_fp8`); a scalar holds the tensor's.
     ``swiglu`` selects the ``silu(gate) * value`` epilogue (output has ``out / 2`` features), ``residual`` the
     fused residual add; they are exclusive.
     """
@@ -1186,6 +1188,16 @@ def linear_fp8(
     res_rows = residual.reshape(-1, out_features).contiguous() if residual is not None else None
     epilogue = _native.EPI_SWIGLU if swiglu else (_native.EPI_RESIDUAL if res_rows is not None else _native.EPI_NONE)
     library = _native.load_library()
+    if amax_x.numel() != 1 and amax_x.shape == shape[:-1]:
+        if x.dtype != torch.float8_e4m3fn or amax_x.dtype != torch.float32:
+            raise ValueError("linear_fp8 takes one float32 amax_x per row with float8_e4m3fn activations only")
+        status = library.taac_linear_fp8_rows(
+            rows.data_ptr(), rows.stride(0), weight_fp8.data_ptr(), amax_x.contiguous().data_ptr(), amax_w.data_ptr(),
+            _native.ptr(bias), _native.ptr(res_rows), out.data_ptr(), out_features, rows.shape[0], n, weight_fp8.shape[1],
+            epilogue, int(bool(gate_first)), _native.current_stream(x.device),
+        )
+        _native.check(status, "linear_fp8")
+        return out.reshape(*shape[:-1], out_features)
     status = library.taac_linear_fp8(
         rows.data_ptr(), int(x.dtype == torch.float8_e4m3fn), rows.stride(0), weight_fp8.data_ptr(),
         amax_x.data_ptr(), amax_w.data_ptr(), _native.ptr(bias), _native.ptr(res_rows), out.data_ptr(), out_features,

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from taac_2026_amd import _native
-from taac_2026_amd.accelerators.tensor_validation import require_cuda_tensors
+from taac_2026_amd.accelerators.tensor_validation import require_cuda_tensors, require_inference, require_same_dtype
 
 RMS_NORM_BACKENDS = ("hip", "torch", "tilelang", "triton")
 LAYER_NORM_BACKENDS = ("hip", "torch", "triton")
@@ -231,6 +231,98 @@ def layer_norm(
     return hip_layer_norm_kernel(rows, normalized_weight, normalized_bias, eps).reshape(original_shape)
 
 
+def _residual_rows(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, operator: str
+                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    if x.ndim < 2:
+        raise ValueError(f"{operator} expects input with at least 2 dimensions")
+    if residual.shape != x.shape:
+        raise ValueError(f"{operator} residual shape {tuple(residual.shape)} does not match input shape {tuple(x.shape)}")
+    if weight.ndim != 1:
+        raise ValueError(f"{operator} weight must be a 1D tensor")
+    if x.shape[-1] != weight.shape[0]:
+        raise ValueError(f"last dimension {x.shape[-1]} does not match weight size {weight.shape[0]}")
+    require_cuda_tensors(f"hip {operator}", x, residual, weight)
+    require_same_dtype(operator, x, residual)
+    width = x.shape[-1]
+    return x.reshape(-1, width).contiguous(), residual.reshape(-1, width).contiguous(), weight.to(x.dtype).contiguous()
+
+
+def _residual_rms_norm_forward(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float
+                               ) -> tuple[torch.Tensor, torch.Tensor]:
+    library = _native.load_library()
+    normed, summed = torch.empty_like(x), torch.empty_like(x)
+    with _native.on_device(x.device):
+        status = library.taac_residual_rmsnorm_fwd(
+            x.data_ptr(), residual.data_ptr(), weight.data_ptr(), summed.data_ptr(), normed.data_ptr(), x.shape[0], x.shape[1],
+            float(eps), _native.dtype_code(x.dtype), _native.current_stream(x.device))
+    _native.check(status, "residual_rms_norm")
+    return normed, summed
+
+
+class _HipResidualRMSNormFunction(torch.autograd.Function):
+    """The backward recomputes the row statistic from the sum, which it keeps instead of both summands."""
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float):
+        normed, summed = _residual_rms_norm_forward(x, residual, weight, eps)
+        ctx.save_for_backward(summed, weight)
+        ctx.eps = float(eps)
+        ctx.set_materialize_grads(False)
+        return normed, summed
+
+    @staticmethod
+    def backward(ctx, grad_normed, grad_summed):
+        if grad_normed is None:  # only the sum was used
+            return grad_summed, grad_summed, None, None
+        summed, weight = ctx.saved_tensors
+        library = _native.load_library()
+        grad_normed = grad_normed.contiguous()
+        grad_summed = None if grad_summed is None else grad_summed.contiguous()
+        with _native.on_device(summed.device):
+            grad_x, grad_w = torch.empty_like(summed), torch.empty_like(weight)
+            workspace = _backward_workspace(summed, False)
+            status = library.taac_residual_rmsnorm_bwd(
+                summed.data_ptr(), weight.data_ptr(), grad_normed.data_ptr(), _native.ptr(grad_summed), grad_x.data_ptr(),
+                grad_w.data_ptr(), workspace.data_ptr(), workspace.numel(), summed.shape[0], summed.shape[1], ctx.eps,
+                _native.dtype_code(summed.dtype), _native.current_stream(summed.device))
+        _native.check(status, "residual_rms_norm backward")
+        return grad_x, grad_x, grad_w, None
+
+
+def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6
+                      ) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(rms_norm(summed, weight, eps), summed)`` with ``summed = x + residual`` in one pass: the addition of a block's update
+    to its residual stream and the norm in front of the next half. The norm is that of the sum as it is stored (rounded to
+    x's dtype), so the results are those of the addition followed by :func:`rms_norm`. Differentiable in x, residual and
+    weight; the gradient of the sum and that through the norm are added in the backward kernel."""
+    rows, residual_rows, normalized_weight = _residual_rows(x, residual, weight, "residual_rms_norm")
+    if _needs_grad(x, residual, weight):
+        normed, summed = _HipResidualRMSNormFunction.apply(rows, residual_rows, normalized_weight, eps)
+    else:
+        normed, summed = _residual_rms_norm_forward(rows, residual_rows, normalized_weight, eps)
+    return normed.reshape(x.shape), summed.reshape(x.shape)
+
+
+def residual_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6
+                          ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(values, row_amax, summed)``: :func:`residual_rms_norm` whose norm leaves as ``float8_e4m3fn`` with one float32
+    maximum per row, ``values = e4m3(normed * 448 / row_amax)``, the activations of ``linear_fp8(values, weight, row_amax,
+    amax_w)``. The norm is not rounded on its way to 8 bits. Forward only."""
+    rows, residual_rows, normalized_weight = _residual_rows(x, residual, weight, "residual_rms_norm_fp8")
+    require_inference("hip residual_rms_norm_fp8", x, residual, weight)
+    library = _native.load_library()
+    summed = torch.empty_like(rows)
+    values = torch.empty(rows.shape, dtype=torch.uint8, device=rows.device)
+    row_amax = torch.empty(rows.shape[0], dtype=torch.float32, device=rows.device)
+    with _native.on_device(rows.device):
+        status = library.taac_residual_rmsnorm_fp8_fwd(
+            rows.data_ptr(), residual_rows.data_ptr(), normalized_weight.data_ptr(), summed.data_ptr(), values.data_ptr(),
+            row_amax.data_ptr(), rows.shape[0], rows.shape[1], float(eps), _native.dtype_code(rows.dtype),
+            _native.current_stream(rows.device))
+    _native.check(status, "residual_rms_norm_fp8")
+    return values.view(torch.float8_e4m3fn).reshape(x.shape), row_amax.reshape(x.shape[:-1]), summed.reshape(x.shape)
+
+
 __all__ = [
     "LAYER_NORM_BACKENDS",
     "RMS_NORM_BACKENDS",
@@ -240,6 +332,8 @@ __all__ = [
     "hip_rms_norm_backward_static_kernel",
     "hip_rms_norm_kernel",
     "layer_norm",
+    "residual_rms_norm",
+    "residual_rms_norm_fp8",
     "resolved_layer_norm_backend",
     "resolved_rms_norm_backend",
     "rms_norm",

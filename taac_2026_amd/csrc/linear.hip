@@ -416,8 +416,10 @@ __device__ __forceinline__ u32x2 quant8(const bf16x8& v, float inv_scale) {
   return r;
 }
 
-template <int EPI, bool A_FP8>
+// ROWS: p.amax_a holds one maximum per row of a (which is e4m3 already) instead of one for the tensor.
+template <int EPI, bool A_FP8, bool ROWS = false>
 __global__ __launch_bounds__(kThreads) void linear_fp8_kernel(const LinearParams p) {
+  static_assert(A_FP8 || !ROWS, "rows with scales of their own arrive quantised");
   constexpr int BK = 128;              // bytes == elements per tile row
   constexpr int STR = BK + 16;         // LDS row stride in bytes
   constexpr int CH = BK / 16;          // 16-byte chunks per tile row (8)
@@ -439,7 +441,7 @@ __global__ __launch_bounds__(kThreads) void linear_fp8_kernel(const LinearParams
   const int wt = wave % 2;
   const int wn = wave / 2;
 
-  const float amax_a = fmaxf(*p.amax_a, 1e-12f);
+  const float amax_a = ROWS ? 448.0f : fmaxf(*p.amax_a, 1e-12f);
   const float amax_w = fmaxf(*p.amax_w, 1e-12f);
   const float inv_scale_a = 448.0f / amax_a;
   const float dq = (amax_a / 448.0f) * (amax_w / 448.0f);
@@ -544,6 +546,18 @@ __global__ __launch_bounds__(kThreads) void linear_fp8_kernel(const LinearParams
         for (int mi = 0; mi < 2; ++mi)
           acc[ni][mi] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[ni], af[mi], acc[ni][mi], 0, 0, 0, kScaleOne,
                                                                         0, kScaleOne);
+    }
+  }
+  if (ROWS) {  // a lane's accumulators belong to one token per sub-tile
+#pragma unroll
+    for (int mi = 0; mi < 2; ++mi) {
+      const int64_t row = m0 + wt * 64 + mi * 32 + l32;
+      const float amax = row < p.M ? p.amax_a[row] : 0.f;
+      const float scale = (amax < 1e-12f ? 1e-12f : amax) / 448.0f;
+#pragma unroll
+      for (int ni = 0; ni < 2; ++ni)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[ni][mi][j] *= scale;
     }
   }
   store_tile<EPI>(p, acc, dq, m0, n0, wt, wn, l32, hh);
@@ -678,11 +692,11 @@ extern "C" int taac_linear_f16(const void* a, int64_t lda, const void* w, const 
   return check_launch(name);
 }
 
-extern "C" int taac_linear_fp8(const void* a, int a_is_fp8, int64_t lda, const void* w, const float* amax_a,
-                               const float* amax_w, const void* bias, const void* residual, void* out, int64_t ldo,
-                               int64_t M, int32_t N, int32_t K, int epilogue, int gate_first, void* stream) {
-  using namespace taac;
-  const char* name = "taac_linear_fp8";
+namespace taac {
+namespace {
+int linear_fp8_entry(const char* name, const void* a, int a_is_fp8, bool row_amax, int64_t lda, const void* w, const float* amax_a,
+                     const float* amax_w, const void* bias, const void* residual, void* out, int64_t ldo, int64_t M, int32_t N,
+                     int32_t K, int epilogue, int gate_first, void* stream) {
   int rc = validate_common(name, a, w, out, residual, lda, ldo, M, N, K, epilogue, 16);
   if (rc != TAAC_OK || M == 0) return rc;
   if (!amax_a || !amax_w) return set_error(TAAC_ERR_INVALID_VALUE, "%s: null amax pointer", name);
@@ -707,6 +721,14 @@ extern "C" int taac_linear_fp8(const void* a, int a_is_fp8, int64_t lda, const v
   rc = fill_params(name, p, M, N, epilogue);
   if (rc != TAAC_OK) return rc;
   hipStream_t s = as_stream(stream);
+  if (row_amax) {
+    switch (epilogue) {
+      case TAAC_EPI_NONE: hipLaunchKernelGGL((linear_fp8_kernel<TAAC_EPI_NONE, true, true>), dim3(p.total), dim3(kThreads), 0, s, p); break;
+      case TAAC_EPI_RESIDUAL: hipLaunchKernelGGL((linear_fp8_kernel<TAAC_EPI_RESIDUAL, true, true>), dim3(p.total), dim3(kThreads), 0, s, p); break;
+      default: hipLaunchKernelGGL((linear_fp8_kernel<TAAC_EPI_SWIGLU, true, true>), dim3(p.total), dim3(kThreads), 0, s, p); break;
+    }
+    return check_launch(name);
+  }
   rc = launch_linear_fp8_ts(a, a_is_fp8, lda, w, amax_a, amax_w, bias, residual, out, ldo, M, N, K, epilogue, gate_first,
                             s, name);
   if (rc <= 0) return rc;  // launched (or failed) on the token-stationary path
@@ -722,4 +744,20 @@ extern "C" int taac_linear_fp8(const void* a, int a_is_fp8, int64_t lda, const v
   }
 #undef TAAC_FP8_LAUNCH
   return check_launch(name);
+}
+}  // namespace
+}  // namespace taac
+
+extern "C" int taac_linear_fp8(const void* a, int a_is_fp8, int64_t lda, const void* w, const float* amax_a,
+                               const float* amax_w, const void* bias, const void* residual, void* out, int64_t ldo,
+                               int64_t M, int32_t N, int32_t K, int epilogue, int gate_first, void* stream) {
+  return taac::linear_fp8_entry("taac_linear_fp8", a, a_is_fp8, false, lda, w, amax_a, amax_w, bias, residual, out, ldo, M, N, K, epilogue,
+                                gate_first, stream);
+}
+
+extern "C" int taac_linear_fp8_rows(const void* a, int64_t lda, const void* w, const float* row_amax, const float* amax_w, const void* bias,
+                                    const void* residual, void* out, int64_t ldo, int64_t M, int32_t N, int32_t K, int epilogue,
+                                    int gate_first, void* stream) {
+  return taac::linear_fp8_entry("taac_linear_fp8_rows", a, 1, true, lda, w, row_amax, amax_w, bias, residual, out, ldo, M, N, K, epilogue,
+                                gate_first, stream);
 }

@@ -11,61 +11,12 @@
 //                                                      (normalization/kernels/triton.py:224-247)
 #include <mutex>
 
-#include "common.h"
+#include "norm_rows.h"
 
 namespace taac {
 namespace {
 
-constexpr int kBlock = 256;
 constexpr int kMaxNV = 8;
-
-template <typename T>
-struct Pack;
-template <>
-struct Pack<float> {
-  static constexpr int VEC = 4;
-  typedef f32x4 vec;
-  static __device__ __forceinline__ void unpack(const vec& v, float* f) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = v[i];
-  }
-  static __device__ __forceinline__ vec pack(const float* f) {
-    vec v;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = f[i];
-    return v;
-  }
-};
-template <>
-struct Pack<bf16_t> {
-  static constexpr int VEC = 8;
-  typedef bf16x8 vec;
-  static __device__ __forceinline__ void unpack(const vec& v, float* f) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = static_cast<float>(v[i]);
-  }
-  static __device__ __forceinline__ vec pack(const float* f) {
-    vec v;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = static_cast<bf16_t>(f[i]);
-    return v;
-  }
-};
-template <>
-struct Pack<f16_t> {
-  static constexpr int VEC = 8;
-  typedef f16x8 vec;
-  static __device__ __forceinline__ void unpack(const vec& v, float* f) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = static_cast<float>(v[i]);
-  }
-  static __device__ __forceinline__ vec pack(const float* f) {
-    vec v;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = static_cast<f16_t>(f[i]);
-    return v;
-  }
-};
 
 // One block = 256 / G lane groups, each group normalises R rows per launch slot.
 template <typename T, int G, int NV, int R, bool LN>
@@ -416,56 +367,6 @@ __global__ __launch_bounds__(kBlock) void norm_bwd_rows_vec_kernel(const T* __re
   }
 }
 
-// dw[c] (and db[c]) = sum over the workgroups' partial rows in a fixed order: a workgroup owns 16 columns, thread
-// (column, slice) adds the partial rows slice, slice + 16, ... and the 16 slice sums of a column are added in slice order.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void norm_bwd_reduce_kernel(const float* __restrict__ partial, int nblocks, int cols,
-                                                                  int parts, T* __restrict__ dw, T* __restrict__ db) {
-  constexpr int CPB = 16, SLICES = kBlock / CPB;
-  __shared__ float red[SLICES][CPB];
-  const int cl = threadIdx.x % CPB, slice = threadIdx.x / CPB;
-  const int c = blockIdx.x * CPB + cl;
-  for (int part = 0; part < parts; ++part) {
-    float sum = 0.f;
-    if (c < cols) {
-#pragma unroll 4
-      for (int b = slice; b < nblocks; b += SLICES) sum += partial[(static_cast<int64_t>(b) * parts + part) * cols + c];
-    }
-    __syncthreads();
-    red[slice][cl] = sum;
-    __syncthreads();
-    if (slice == 0 && c < cols) {
-      float total = 0.f;
-#pragma unroll
-      for (int sl = 0; sl < SLICES; ++sl) total += red[sl][cl];
-      T* dst = part == 0 ? dw : db;
-      if (dst != nullptr) dst[c] = static_cast<T>(total);
-    }
-  }
-}
-
-// Sum over the workgroup of up to three values at once (wavefront shuffles, then one LDS round over the wavefronts);
-// every thread gets the totals. `red` is reused by consecutive calls: the leading barrier protects the previous round.
-template <int N>
-__device__ __forceinline__ void block_sum(float (&v)[N], float (*red)[kBlock / kWave]) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = group_sum<kWave>(v[i]);
-  __syncthreads();
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) red[i][wave] = v[i];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float total = 0.f;
-#pragma unroll
-    for (int w = 0; w < kBlock / kWave; ++w) total += red[i][w];
-    v[i] = total;
-  }
-}
-
 // Backward for shapes the vector kernel does not take (columns that are not whole 128-bit vectors, unaligned bases,
 // rows longer than its register budget): one workgroup per row at a time, thread t owns columns t, t + 256, ...; the
 // row is swept four times (mean, variance, the two projections, the result), sweeps after the first come from cache.
@@ -520,8 +421,6 @@ __global__ __launch_bounds__(kBlock) void norm_bwd_rows_generic_kernel(const T* 
     }
   }
 }
-
-constexpr int kBwdMaxBlocks = 1024;
 
 template <typename T, bool LN>
 int dispatch_bwd(const void* xv, const void* wv, const void* dyv, void* dxv, void* dwv, void* dbv, float* workspace,

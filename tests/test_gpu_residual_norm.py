@@ -1,0 +1,217 @@
+"""RMSNorm of ``x + residual`` (forward, e4m3 output with a maximum per row, backward) against its formulas in 64 bits.
+
+Tolerances: an output's one rounding is at most half a step, eps / 2 relative to the value; the fp32 arithmetic before it adds a few
+2^-24 per operation, a sum of n terms at most n 2^-24 of the sum of their magnitudes."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from taac_2026_amd.api import linear_fp8, quantize_fp8, residual_rms_norm, residual_rms_norm_fp8, rms_norm
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-6
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+# vector kernel (one to eight vectors a lane), odd widths, more than 512 vectors
+COLS = [1, 7, 8, 37, 64, 256, 264, 385, 1024, 2048, 4096, 5000]
+
+
+def _draw(rows, cols, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g).to(dtype)
+    r = (2.0 * torch.randn(rows, cols, generator=g)).to(dtype)
+    w = (1.0 + 0.1 * torch.randn(cols, generator=g)).to(dtype)
+    return x, r, w
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _definition(x, r, w):
+    summed = x + r
+    h = summed.double()
+    rstd = (h.square().mean(-1, keepdim=True) + EPS).rsqrt()
+    return summed, h, rstd, h * rstd * w.double()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", COLS)
+def test_forward(device, dtype, cols):
+    for rows in (1, 3, 67):
+        x, r, w = _draw(rows, cols, dtype, seed=cols + rows)
+        summed, _, _, want = _definition(x, r, w)
+        with torch.no_grad():
+            got, got_sum = residual_rms_norm(x.to(device), r.to(device), w.to(device), EPS)
+        assert got.dtype == got_sum.dtype == dtype
+        assert torch.equal(got_sum.cpu(), summed)
+        # fp32: the sum of squares is off by at most cols 2^-24, half of it after the root, and five further roundings
+        rtol = _half_step(dtype) + (cols / 2 + 8) * 2.0**-24
+        torch.testing.assert_close(got.cpu().double(), want, rtol=rtol, atol=1e-7)
+        # the addition followed by the norm, which sums the squares of a row in the same lanes
+        with torch.no_grad():
+            two = rms_norm((x + r).to(device), w.to(device), EPS)
+        torch.testing.assert_close(got.cpu().double(), two.cpu().double(), rtol=2 * rtol, atol=2e-7)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", COLS)
+def test_e4m3_rows(device, dtype, cols):
+    x, r, w = _draw(67, cols, dtype, seed=3 * cols)
+    x[3], r[3] = 0.0, 0.0  # a row of zeros
+    x[5] *= 200.0
+    summed, _, _, want = _definition(x, r, w)
+    with torch.no_grad():
+        values, row_amax, got_sum = residual_rms_norm_fp8(x.to(device), r.to(device), w.to(device), EPS)
+    assert values.dtype == torch.float8_e4m3fn and row_amax.shape == (67,)
+    assert torch.equal(got_sum.cpu(), summed)
+    fp32 = (cols / 2 + 8) * 2.0**-24
+    amax = want.abs().amax(-1)
+    torch.testing.assert_close(row_amax.cpu().double(), amax, rtol=fp32, atol=0.0)
+    scale = amax.clamp(min=1e-12)[:, None] / 448.0
+    got = values.cpu().float().double() * scale
+    # half a step of e4m3: 2^-4 of a normal value, 2^-10 below 2^-6
+    bound = want.abs() * (2.0**-4 + 2 * fp32) + scale * 2.0**-10 * (1 + 1e-5)
+    assert ((got - want).abs() <= bound).all()
+    assert (values.cpu().float()[3] == 0).all()
+    assert (values.cpu().float().abs().amax(-1)[[0, 5]] == 448.0).all()
+
+
+def test_unaligned_and_strided_inputs(device):
+    x, r, w = _draw(33, 256, torch.bfloat16, seed=5)
+    summed, _, _, want = _definition(x, r, w)
+    flat = torch.empty(33 * 256 + 1, dtype=torch.bfloat16, device=device)
+    off = flat[1:].view(33, 256).copy_(x.to(device))  # base off the 16-byte grid
+    wide = torch.randn(33, 512, device=device).to(torch.bfloat16)
+    wide[:, ::2] = r.to(device)
+    with torch.no_grad():
+        got, got_sum = residual_rms_norm(off, wide[:, ::2], w.to(device), EPS)
+        _, amax, fp8_sum = residual_rms_norm_fp8(off, wide[:, ::2], w.to(device), EPS)
+    assert torch.equal(got_sum.cpu(), summed) and torch.equal(fp8_sum.cpu(), summed)
+    torch.testing.assert_close(got.cpu().double(), want, rtol=2.0**-8 + 1e-5, atol=1e-7)
+    torch.testing.assert_close(amax.cpu().double(), want.abs().amax(-1), rtol=1e-5, atol=0.0)
+
+
+def test_nan_and_inf_stay_in_their_rows(device):
+    x, r, w = _draw(9, 256, torch.bfloat16, seed=6)
+    clean = x.clone()
+    x[2, 17], x[4, 3] = float("nan"), float("inf")
+    with torch.no_grad():
+        values, amax, summed = residual_rms_norm_fp8(x.to(device), r.to(device), w.to(device), EPS)
+        want, want_amax, _ = residual_rms_norm_fp8(clean.to(device), r.to(device), w.to(device), EPS)
+    rest = [0, 1, 3, 5, 6, 7, 8]
+    assert torch.equal(values.float()[rest], want.float()[rest]) and torch.equal(amax[rest], want_amax[rest])
+    assert torch.isnan(amax[2]) and torch.isnan(values.float()[2]).all() and torch.isnan(amax[4])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 256), (130, 37), (300, 256), (70, 1024), (40, 2048), (5000, 128), (21, 4104)])
+def test_gradients(device, dtype, rows, cols):
+    x, r, w = _draw(rows, cols, dtype, seed=rows + cols)
+    g = torch.Generator().manual_seed(1)
+    dy, ds = (torch.randn(rows, cols, generator=g).to(dtype) for _ in range(2))
+    _, h, rstd, _ = _definition(x, r, w)
+    unit, wdy = h * rstd, w.double() * dy.double()
+    proj = (unit * wdy).mean(-1, keepdim=True)
+    want = ds.double() + rstd * (wdy - unit * proj)
+    want_w = (dy.double() * unit).sum(0)
+    leaves = [t.to(device).requires_grad_(True) for t in (x, r, w)]
+    normed, summed = residual_rms_norm(*leaves, EPS)
+    dx, dr, dw = torch.autograd.grad((normed, summed), leaves, (dy.to(device), ds.to(device)))
+    assert torch.equal(dx, dr)
+    fp32 = (cols + 16) * 2.0**-24
+    bound = _half_step(dtype) * want.abs() + fp32 * (ds.double().abs() + rstd * (wdy.abs() + unit.abs() * (unit * wdy).abs().mean(-1, keepdim=True))) + 1e-7
+    assert ((dx.cpu().double() - want).abs() <= bound).all()
+    bound_w = _half_step(dtype) * want_w.abs() + (rows + cols + 16) * 2.0**-24 * (dy.double() * unit).abs().sum(0) + 1e-7
+    assert ((dw.cpu().double() - want_w).abs() <= bound_w).all()
+
+
+def test_gradients_where_one_output_is_unused(device):
+    x, r, w = (t.to(device) for t in _draw(50, 256, torch.float32, seed=8))
+    dy = torch.randn(50, 256, device=device)
+    leaves = [t.clone().requires_grad_(True) for t in (x, r, w)]
+    normed, summed = residual_rms_norm(*leaves, EPS)
+    got = torch.autograd.grad(normed, leaves, dy)
+    ref = [(x + r).clone().requires_grad_(True), w.clone().requires_grad_(True)]
+    want = torch.autograd.grad(rms_norm(ref[0], ref[1], EPS), ref, dy)
+    torch.testing.assert_close(got[0], want[0], rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(got[2], want[1], rtol=1e-5, atol=1e-5)
+    leaves = [t.clone().requires_grad_(True) for t in (x, r, w)]
+    _, summed = residual_rms_norm(*leaves, EPS)
+    dx, dr, dw = torch.autograd.grad(summed, leaves, dy, allow_unused=True)
+    assert torch.equal(dx, dy) and torch.equal(dr, dy) and dw is None
+
+
+def test_gradient_against_differences(device):
+    x, r, w = (t.to(device) for t in _draw(4, 96, torch.float32, seed=9))
+    coef_y, coef_s, step = torch.randn(4, 96, device=device), torch.randn(4, 96, device=device), torch.randn(4, 96, device=device)
+
+    def value(t):
+        y, s = residual_rms_norm(t, r, w, EPS)
+        return (y.double() * coef_y).sum() + (s.double() * coef_s).sum()
+
+    leaf = x.clone().requires_grad_(True)
+    slope = (torch.autograd.grad(value(leaf), leaf)[0].double() * step).sum().item()
+    with torch.no_grad():
+        e = 2.0**-8
+        diff = ((value(x + e * step) - value(x - e * step)) / (2 * e)).item()
+    # fp32 values of 768 terms near 1, divided by 2 e: 768 2^-24 2^7 = 6e-3; the third derivative adds e^2 of the sum's size
+    assert abs(slope - diff) <= 2e-2 + 1e-3 * abs(slope)
+
+
+def test_empty(device):
+    w = torch.ones(64, dtype=torch.bfloat16, device=device, requires_grad=True)
+    x = torch.empty(0, 5, 64, dtype=torch.bfloat16, device=device, requires_grad=True)
+    normed, summed = residual_rms_norm(x, x.detach(), w)
+    assert normed.shape == summed.shape == (0, 5, 64)
+    dw = torch.autograd.grad(normed, w, torch.empty_like(normed))[0]
+    assert (dw == 0).all()
+    with torch.no_grad():
+        values, amax, _ = residual_rms_norm_fp8(x, x, w)
+    assert values.shape == (0, 5, 64) and amax.shape == (0, 5)
+
+
+@pytest.mark.parametrize("swiglu,with_residual", [(False, False), (False, True), (True, False)])
+def test_the_e4m3_layer_reads_rows_with_their_maxima(device, swiglu, with_residual):
+    """norm -> e4m3 rows -> dense layer, as a block runs them: against the products of the values that the 8 bits stand for."""
+    batch, tokens, width, out = 3, 41, 256, 320
+    x, r, w = _draw(batch * tokens, width, torch.bfloat16, seed=11)
+    g = torch.Generator().manual_seed(12)
+    weight = (torch.randn(out, width, generator=g) / 16).to(torch.bfloat16)
+    bias = torch.randn(out, generator=g).to(torch.bfloat16)
+    features = out // 2 if swiglu else out
+    skip = torch.randn(batch, tokens, features, generator=g).to(torch.bfloat16) if with_residual else None
+    with torch.no_grad():
+        values, amax, _ = residual_rms_norm_fp8(x.view(batch, tokens, width).to(device), r.view(batch, tokens, width).to(device), w.to(device))
+        wq, wa = quantize_fp8(weight.to(device))
+        got = linear_fp8(values, wq, amax, wa, bias.to(device), swiglu=swiglu, residual=None if skip is None else skip.to(device))
+    a = values.cpu().float().double() * (amax.cpu().double() / 448.0)[..., None]
+    b = wq.cpu().float().double() * (wa.cpu().double() / 448.0)
+    pre = a @ b.T + bias.double()
+    if swiglu:
+        gate, value = pre.chunk(2, -1)
+        want = torch.nn.functional.silu(gate) * value
+    else:
+        want = pre if skip is None else pre + skip.double()
+    magnitude = (a.abs() @ b.abs().T + bias.double().abs()).amax()
+    # one rounding of the result; sums of 256 products in fp32; the gate's exponential and reciprocal (2^-20)
+    assert ((got.cpu().double() - want).abs() <= 2.0**-8 * want.abs() + magnitude.clamp(min=1.0) ** (2 if swiglu else 1) * 2.0**-14).all()
+
+
+def test_replayed_graph(device):
+    x, r, w = (t.to(device) for t in _draw(500, 256, torch.bfloat16, seed=13))
+    with torch.no_grad():
+        residual_rms_norm_fp8(x, r, w)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = residual_rms_norm_fp8(x, r, w)
+        for seed in range(3):
+            nx, nr, _ = _draw(500, 256, torch.bfloat16, seed=20 + seed)
+            x.copy_(nx), r.copy_(nr)
+            graph.replay()
+            want = residual_rms_norm_fp8(nx.to(device), nr.to(device), w)
+            torch.cuda.synchronize()
+            assert torch.equal(held[0].float(), want[0].float()) and torch.equal(held[1], want[1]) and torch.equal(held[2], want[2])
