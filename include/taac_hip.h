@@ -604,6 +604,48 @@ int taac_row_rstd(const float* qk_sumsq, int64_t M, int32_t d_model, float eps, 
                   const int32_t* n_rows, void* stream);
 
 /*
+ * Gated delta rule, chunked form. Per sample and value head, with a = exp(log_decay), the fp32 state S [dk, dv] follows
+ *   S <- a S,   S <- S + k (beta (v - S^T k))^T,   o = scale S^T q.
+ * q, k: bf16, logical (B, key_heads, T, dk); v, o: bf16 (B, H, T, dv), H a multiple of key_heads (value head h uses key head
+ * h / (H / key_heads)); log_decay, beta: (B, H, T) of gate_dtype (TAAC_F32 or TAAC_BF16). *_strides: ELEMENT strides of (batch, head,
+ * token); the features of a row are contiguous, q / k / v / o have strides that are multiples of 8 and 16-byte aligned bases. dk and
+ * dv: multiples of 8, at most 128. lengths: int32 [B] or NULL; tokens at or beyond a sample's length are not read, leave the
+ * state alone and get zeros in o. Keys should have at most unit length and beta lie in [0, 1], as the recurrence needs to stay
+ * bounded; log_decay is normally <= 0, values below -1e5 count as -1e5.
+ * state_in: fp32 [B, H, dk, dv] or NULL (zeros); state_out: the same shape, or NULL; it may be state_in.
+ * chunk_states (bf16 [B, H, ceil(T / 64), dk, dv]) and misses (bf16 [B, H, T, dv]): what taac_delta_rule_bwd reads, or both NULL.
+ * taac_delta_rule_bwd: gradients of q, k, v, log_decay and beta (logical shapes and dtypes of the inputs, strides of their own) for
+ * grad_o; grad_states (bf16, the size of chunk_states) is scratch. The initial state has no gradient here. Rows at or beyond a
+ * sample's length get zeros. Every sum has a fixed order.
+ * Replaces: the reference's chunked gated delta rule (accelerators/attention/kernels/gated_delta_rule).
+ */
+int taac_delta_rule_fwd(const void* q, const void* k, const void* v, const void* log_decay, const void* beta, const int32_t* lengths,
+                        void* o, const float* state_in, float* state_out, void* chunk_states, void* misses, int32_t B, int32_t H,
+                        int32_t key_heads, int32_t T, int32_t dk, int32_t dv, const int64_t q_strides[3], const int64_t k_strides[3],
+                        const int64_t v_strides[3], const int64_t o_strides[3], const int64_t decay_strides[3],
+                        const int64_t beta_strides[3], float scale, int gate_dtype, void* stream);
+int taac_delta_rule_bwd(const void* q, const void* k, const void* log_decay, const void* beta, const int32_t* lengths,
+                        const void* chunk_states, const void* misses, const void* grad_o, void* grad_q, void* grad_k, void* grad_v,
+                        void* grad_decay, void* grad_beta, void* grad_states, int32_t B, int32_t H, int32_t key_heads, int32_t T,
+                        int32_t dk, int32_t dv, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t decay_strides[3],
+                        const int64_t beta_strides[3], const int64_t go_strides[3], const int64_t gq_strides[3],
+                        const int64_t gk_strides[3], const int64_t gv_strides[3], const int64_t gdecay_strides[3],
+                        const int64_t gbeta_strides[3], float scale, int gate_dtype, void* stream);
+
+/*
+ * Gated delta rule, recurrent form: T new tokens for each of B samples, whose states live in a pool, fp32 [pool, H, dk, dv], 16-byte
+ * aligned, updated in place. slots: [B] int32 or int64 (slots_int64), or NULL (sample b has slot b, B <= pool). Samples with the same
+ * slot are one sequence, their tokens applied in the order of the batch; a slot outside the pool reads and writes no state and gets
+ * zeros in o. lengths: int32 [B] or NULL: the tokens a sample really has. q, k, v, o of dtype (fp32, bf16 or fp16), the gates of that
+ * dtype or fp32; strides as taac_delta_rule_fwd, of any value. All arithmetic is fp32.
+ */
+int taac_delta_rule_step(const void* q, const void* k, const void* v, const void* log_decay, const void* beta, float* state, int64_t pool,
+                         const void* slots, int slots_int64, const int32_t* lengths, void* o, int32_t B, int32_t H, int32_t key_heads,
+                         int32_t T, int32_t dk, int32_t dv, const int64_t q_strides[3], const int64_t k_strides[3],
+                         const int64_t v_strides[3], const int64_t o_strides[3], const int64_t decay_strides[3],
+                         const int64_t beta_strides[3], float scale, int dtype, int gate_dtype, void* stream);
+
+/*
  * Readout of the token backbone, one kernel:
  *   n(t)  = token_norm_weight ? rmsnorm(tokens[b, t], token_norm_weight, eps) : tokens[b, t]
  *   e[b]  = concat( n(cls_index), candidate_index >= 0 ? n(candidate_index) : 0, mean over the valid t of n(t) )

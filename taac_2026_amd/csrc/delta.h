@@ -1,0 +1,374 @@
+// Pieces shared by the kernels of the gated delta rule (delta_scan.hip, delta_bwd.hip).
+//
+// Per sample and value head, with a_t = exp(g_t), the state S [key_dim, value_dim] follows
+//   N_t = v_t - (a_t S)^T k_t,   S <- a_t S + k_t (beta_t N_t)^T,   o_t = scale S^T q_t.
+// Over a chunk of 64 tokens with G_i = g_1 + .. + g_i, Gam_ij = exp(G_i - G_j) and A_ij = Gam_ij (k_i . k_j) beta_j for i > j:
+//   X = V - diag(e^G) K S,   (I + A) N = X,   O = scale (diag(e^G) Q S + (Gam * Q K^T * beta) N),
+//   S' = e^{G_64} S + (beta e^{G_64 - G} K)^T N.
+// The inverse of the unit triangular I + A is written I - M; M and the score matrix P do not depend on the state.
+//
+// All products run on v_mfma_f32_16x16x32_bf16. With lane = (l16 = lane % 16, grp = lane / 16) its operands hold row (or column)
+// l16 and 8 values of the contraction, its result column l16 and rows 4 grp .. 4 grp + 3. The contraction may be walked in any
+// order that both operands share, and the order used everywhere here is: element e of group grp = index 4 grp + e of the first
+// half of a block of 32 for e < 4, of its second half for e >= 4. Two results (16 rows each) are then an operand of the next product as
+// they stand, so a chain X -> N -> S' -> next X never leaves the registers.
+//
+// Precision: q, k, v are bf16 and exact operands. The state and what it is made of (S, X, N, M) are fp32 in registers and enter a
+// product as a bf16 pair hi + lo (16 bits, 2^-17 relative), at two matrix instructions where one factor is exact and three where
+// none is; one bf16 would put 2^-9 into the state at every chunk. P enters rounded once: it only reaches the output.
+// Cumulative decays are summed in 64 bits and kept as pairs, so that G_i - G_j of a fast decaying head keeps fp32 precision.
+#pragma once
+
+#include "common.h"
+
+namespace taac {
+
+struct DeltaParams {
+  const bf16_t* q;
+  const bf16_t* k;
+  const bf16_t* v;
+  bf16_t* o;
+  const void* log_decay;
+  const void* beta;
+  const int32_t* lengths;    // [B] or null: every sample has T tokens
+  const float* state_in;     // [B, H, dk, dv] or null: zeros
+  float* state_out;          // [B, H, dk, dv] or null
+  bf16_t* chunk_states;      // [B, H, chunks, dk, dv] or null: the state in front of every chunk
+  bf16_t* misses;            // [B, H, T, dv] or null: N
+  // backward
+  const bf16_t* grad_o;
+  bf16_t* grad_q;
+  bf16_t* grad_k;
+  bf16_t* grad_v;            // also dX, which the last kernel reads
+  void* grad_decay;
+  void* grad_beta;
+  bf16_t* grad_states;       // [B, H, chunks, dk, dv]: the gradient of the state behind every chunk
+  int64_t dos[3], dqs[3], dks[3], dvs[3], dgs[3], dbs[3];
+  // element strides of (batch, head, token)
+  int64_t qs[3], ks[3], vs[3], os[3], gs[3], bs[3];
+  int32_t B, H, group, T, dk, dv, chunks;  // group: value heads per key head
+  int32_t gates_f32;
+  float scale;
+};
+
+int delta_check(const char* name, const DeltaParams& p);
+int delta_strides(const char* name, const char* what, const void* ptr, const int64_t* from, int64_t* to, bool rows);
+
+namespace {
+
+constexpr int kChunk = 64;
+constexpr int kFrag = 1024;              // bytes of one operand fragment of a wavefront
+constexpr int kBlockM = 0, kBlockLow = 6 * kFrag, kBlockP = 12 * kFrag, kBlockRows = 18 * kFrag;
+// floats behind the fragments of a block
+constexpr int kRowHi = 0, kRowLow = 64, kRowBeta = 128, kRowGrown = 192, kRowKeep = 256, kRowTotal = 320;
+constexpr int kBlockBytes = kBlockRows + 336 * 4;
+constexpr int kScratchFloats = 4 * 16 * 20;  // diagonal blocks, rows of 20 floats
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// LDS written by some lanes of a wavefront and read by others: the operations of a wavefront complete in order; this keeps the
+// compiler from reordering them.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ void split(const f32x4& a, const f32x4& b, bf16x8& hi, bf16x8& lo) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float f = e < 4 ? a[e] : b[e - 4];
+    hi[e] = static_cast<bf16_t>(f);
+    lo[e] = static_cast<bf16_t>(f - static_cast<float>(hi[e]));
+  }
+}
+__device__ __forceinline__ bf16x8 round8(const f32x4& a, const f32x4& b) {
+  bf16x8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = static_cast<bf16_t>(e < 4 ? a[e] : b[e - 4]);
+  return r;
+}
+__device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+__device__ __forceinline__ bf16x8 zero8() {
+  const u32x4 z = {0u, 0u, 0u, 0u};
+  return __builtin_bit_cast(bf16x8, z);
+}
+
+__device__ __forceinline__ float load_gate(const void* p, int64_t at, int f32) {
+  return f32 ? static_cast<const float*>(p)[at] : static_cast<float>(static_cast<const bf16_t*>(p)[at]);
+}
+
+// Operand fragment of block kb (32 features) of a row in global memory; null rows and features at or beyond width give zeros.
+__device__ __forceinline__ bf16x8 row_frag(const bf16_t* row, int kb, int grp, int width) {
+  bf16x8 r = zero8();
+  if (row != nullptr) {
+    const int at = kb * 32 + grp * 4;
+    bf16x4 lo = {}, hi = {};
+    if (at < width) lo = *reinterpret_cast<const bf16x4*>(row + at);
+    if (at + 16 < width) hi = *reinterpret_cast<const bf16x4*>(row + at + 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      r[e] = lo[e];
+      r[4 + e] = hi[e];
+    }
+  }
+  return r;
+}
+
+// Tiles in LDS. A staged tile of 64 token rows keeps each block of 32 features in operand order (group 0's 8 values, then group 1's ..), so
+// that a row fragment is one 16-byte read; rows are 16 bytes longer than their contents, which puts the 16 rows of a read on
+// different banks.
+template <int WIDTH>
+struct Tile {
+  static constexpr int STRIDE = WIDTH + 8;  // elements
+  static constexpr int BYTES = kChunk * STRIDE * 2;
+  // rows token0 .. of `src` (stride ld), n of them valid, `width` valid features from the first
+  static __device__ __forceinline__ void stage(bf16_t* dst, const bf16_t* src, int64_t ld, int n, int width, int tid, int threads) {
+    constexpr int PIECES = WIDTH / 8;
+    for (int i = tid; i < kChunk * PIECES; i += threads) {
+      const int row = i / PIECES, piece = i % PIECES;
+      bf16x8 v = zero8();
+      if (row < n && piece * 8 < width) v = *reinterpret_cast<const bf16x8*>(src + row * ld + piece * 8);
+      // pieces of 4: number 2 (piece % 4) + {0, 1} of the block; number p goes to place 2 (p % 4) + p / 4
+      bf16_t* at = dst + row * STRIDE + (piece / 4) * 32;
+      const int p0 = 2 * (piece % 4);
+      bf16x4 lo, hi;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        lo[e] = v[e];
+        hi[e] = v[4 + e];
+      }
+      *reinterpret_cast<bf16x4*>(at + ((p0 % 4) * 2 + p0 / 4) * 4) = lo;
+      *reinterpret_cast<bf16x4*>(at + (((p0 + 1) % 4) * 2 + (p0 + 1) / 4) * 4) = hi;
+    }
+  }
+  static __device__ __forceinline__ bf16x8 row(const bf16_t* tile, int row, int kb, int grp) {
+    return *reinterpret_cast<const bf16x8*>(tile + row * STRIDE + kb * 32 + grp * 8);
+  }
+  // Four tokens (token0 + 4 grp ..) of feature 16 a + l16: a transposed read. Lane 4 e + q of a group of 16 gives the address of
+  // 8 bytes of token e, lane j receives element j % 4 of what lanes 4 e + j / 4 gave.
+  static __device__ __forceinline__ bf16x4 column(const bf16_t* tile, int token0, int a, int l16, int grp) {
+    const bf16_t* at = tile + (token0 + 4 * grp + l16 / 4) * STRIDE + (a / 2) * 32 + (l16 % 4) * 8 + (a % 2) * 4;
+    typedef __attribute__((address_space(3))) bf16x4 lds_vec;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_vec*)(at));
+  }
+  // Operand fragment (feature 16 a + l16; tokens of block tk)
+  static __device__ __forceinline__ bf16x8 column_frag(const bf16_t* tile, int tk, int a, int l16, int grp) {
+    const bf16x4 lo = column(tile, 32 * tk, a, l16, grp), hi = column(tile, 32 * tk + 16, a, l16, grp);
+    bf16x8 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      r[e] = lo[e];
+      r[4 + e] = hi[e];
+    }
+    return r;
+  }
+};
+
+// 16 x 16 fp32 products on v_mfma_f32_16x16x4_f32, contraction index 4 grp + step. A matrix Y is held "by rows" (lane: row l16, columns
+// 4 grp ..) or "by columns" (lane: column l16, rows 4 grp ..).
+__device__ __forceinline__ f32x4 mul_cols(const f32x4& x_rows, const f32x4& y_cols, f32x4 acc) {  // X Y by columns
+#pragma unroll
+  for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x_rows[r], y_cols[r], acc, 0, 0, 0);
+  return acc;
+}
+__device__ __forceinline__ f32x4 mul_rows(const f32x4& x_rows, const f32x4& y_cols, f32x4 acc) {  // X Y by rows
+#pragma unroll
+  for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(y_cols[r], x_rows[r], acc, 0, 0, 0);
+  return acc;
+}
+
+// Place of a fragment in a block. By rows (forward): row tile ti, token block tk <= ti / 2. By columns (backward): column tile tj, token
+// block tk >= tj / 2.
+__host__ __device__ constexpr int frag_rows(int ti, int tk) { return ti < 2 ? ti : 2 + (ti - 2) * 2 + tk; }
+__host__ __device__ constexpr int frag_cols(int tj, int tk) { return tj < 2 ? tj * 2 + tk : 2 + tj; }
+
+// The factors of a chunk's tokens (kRow*), by one wavefront. last_minus: null, or receives e^(G_last - G) of every token.
+__device__ __forceinline__ void chunk_rows(const DeltaParams& p, int b, int h, int64_t token0, int n, float* rows,
+                                           float* last_minus = nullptr) {
+  const int lane = threadIdx.x % kWave;
+  // decays in powers of two; an exponent below -1e5 is a decay of zero, and stays finite in the sums
+  double total = 0.0;
+  float beta = 0.f;
+  if (lane < n) {
+    float g = load_gate(p.log_decay, b * p.gs[0] + h * p.gs[1] + (token0 + lane) * p.gs[2], p.gates_f32);
+    g = g < -1e5f ? -1e5f : g;
+    total = static_cast<double>(g) * 1.4426950408889634;
+    beta = load_gate(p.beta, b * p.bs[0] + h * p.bs[1] + (token0 + lane) * p.bs[2], p.gates_f32);
+  }
+#pragma unroll
+  for (int off = 1; off < kWave; off *= 2) {
+    const double up = __shfl_up(total, off, kWave);
+    if (lane >= off) total += up;
+  }
+  const double last = __shfl(total, kWave - 1, kWave);
+  const float hi = static_cast<float>(total);
+  rows[kRowHi + lane] = hi;
+  rows[kRowLow + lane] = static_cast<float>(total - static_cast<double>(hi));
+  rows[kRowBeta + lane] = beta;
+  rows[kRowGrown + lane] = __builtin_amdgcn_exp2f(hi);
+  const float left = __builtin_amdgcn_exp2f(static_cast<float>(last - total));
+  rows[kRowKeep + lane] = beta * left;
+  if (last_minus != nullptr) last_minus[lane] = left;
+  if (lane == 0) rows[kRowTotal] = __builtin_amdgcn_exp2f(static_cast<float>(last));
+}
+
+// One wavefront makes the block of one chunk (n valid tokens; rows beyond count as k = q = 0, g = 0, beta = 0): -M as hi and lo, P, and the
+// factors of its tokens. COLS: transposed fragments, for the backward. block: LDS or global; rows: LDS floats (kRow*), written for every
+// token; scratch: LDS.
+//
+// The 64 x 64 inverse: the four diagonal blocks of 16 by substitution, a column per lane, all four at once; the blocks below them by
+// products, M_21 = T_22 A_21 T_11 with T = I - M, first pairs of 16, then of 32.
+template <int DK, bool COLS>
+__device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, int64_t token0, int n, uint8_t* block, float* rows,
+                                            float* scratch) {
+  constexpr int KB = DK / 32;
+  const int lane = threadIdx.x % kWave, l16 = lane % 16, grp = lane / 16;
+
+  chunk_rows(p, b, h, token0, n, rows);
+  const int64_t hk = h / p.group;
+  const bf16_t* kbase = p.k + b * p.ks[0] + hk * p.ks[1] + token0 * p.ks[2];
+  const bf16_t* qbase = p.q + b * p.qs[0] + hk * p.qs[1] + token0 * p.qs[2];
+  bf16x8 kf[4][KB];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int row = 16 * t + l16;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) kf[t][kb] = row_frag(row < n ? kbase + row * p.ks[2] : nullptr, kb, grp, p.dk);
+  }
+  wave_sync();
+
+  f32x4 a_rows[10];  // A by rows, tile (ti, tj) at ti (ti + 1) / 2 + tj
+  bf16x8 pf[6];
+#pragma unroll
+  for (int i = 0; i < 6; ++i) pf[i] = zero8();
+#pragma unroll
+  for (int ti = 0; ti < 4; ++ti) {
+    const int row = 16 * ti + l16;
+    bf16x8 qf[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) qf[kb] = row_frag(row < n ? qbase + row * p.qs[2] : nullptr, kb, grp, p.dk);
+    const float hi_i = rows[kRowHi + row], lo_i = rows[kRowLow + row];
+#pragma unroll
+    for (int tj = 0; tj <= ti; ++tj) {
+      f32x4 kk = zero4(), qk = zero4();
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        kk = mfma16(kf[tj][kb], kf[ti][kb], kk);
+        qk = COLS ? mfma16(qf[kb], kf[tj][kb], qk) : mfma16(kf[tj][kb], qf[kb], qk);
+      }
+      const f32x4 hi_j = *reinterpret_cast<const f32x4*>(rows + kRowHi + 16 * tj + 4 * grp);
+      const f32x4 lo_j = *reinterpret_cast<const f32x4*>(rows + kRowLow + 16 * tj + 4 * grp);
+      const f32x4 beta_j = *reinterpret_cast<const f32x4*>(rows + kRowBeta + 16 * tj + 4 * grp);
+      f32x4 a, s;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float gam = __builtin_amdgcn_exp2f((hi_i - hi_j[r]) + (lo_i - lo_j[r])) * beta_j[r];
+        const int i = l16, j = 4 * grp + r;
+        a[r] = (ti > tj || i > j) ? gam * kk[r] : 0.f;
+        if (!COLS) s[r] = (ti > tj || i >= j) ? p.scale * gam * qk[r] : 0.f;
+      }
+      if (COLS) {
+        const f32x4 hi_r = *reinterpret_cast<const f32x4*>(rows + kRowHi + 16 * ti + 4 * grp);
+        const f32x4 lo_r = *reinterpret_cast<const f32x4*>(rows + kRowLow + 16 * ti + 4 * grp);
+        const float hi_c = rows[kRowHi + 16 * tj + l16], lo_c = rows[kRowLow + 16 * tj + l16], beta_c = rows[kRowBeta + 16 * tj + l16];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float gam = __builtin_amdgcn_exp2f((hi_r[r] - hi_c) + (lo_r[r] - lo_c)) * beta_c;
+          s[r] = (ti > tj || 4 * grp + r >= l16) ? p.scale * gam * qk[r] : 0.f;
+        }
+      }
+      a_rows[ti * (ti + 1) / 2 + tj] = a;
+      const int f = COLS ? frag_cols(tj, ti / 2) : frag_rows(ti, tj / 2);
+      const int half = COLS ? ti % 2 : tj % 2;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) pf[f][4 * half + r] = static_cast<bf16_t>(s[r]);
+    }
+  }
+
+  // diagonal blocks
+#pragma unroll
+  for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(scratch + (t * 16 + l16) * 20 + 4 * grp) = a_rows[t * (t + 1) / 2 + t];
+  wave_sync();
+  {
+    float* mine = scratch + grp * 16 * 20;
+    float m[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float acc = mine[i * 20 + l16];
+#pragma unroll
+      for (int j4 = 0; j4 * 4 < i; ++j4) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(mine + i * 20 + 4 * j4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * j4 + e < i) acc = fmaf(-a[e], m[4 * j4 + e], acc);
+      }
+      m[i] = acc;
+    }
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mine[i * 20 + l16] = m[i];
+  }
+  wave_sync();
+  f32x4 m_rows[4], m_cols[4], t_rows[4], t_cols[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    m_rows[t] = *reinterpret_cast<const f32x4*>(scratch + (t * 16 + l16) * 20 + 4 * grp);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      m_cols[t][r] = scratch[(t * 16 + 4 * grp + r) * 20 + l16];
+      const float one = l16 == 4 * grp + r ? 1.f : 0.f;
+      t_rows[t][r] = one - m_rows[t][r];
+      t_cols[t][r] = one - m_cols[t][r];
+    }
+  }
+  wave_sync();
+
+  const f32x4 z10 = mul_cols(a_rows[1], t_cols[0], zero4());
+  const f32x4 z32 = mul_cols(a_rows[8], t_cols[2], zero4());
+  const f32x4 m10c = mul_cols(t_rows[1], z10, zero4());
+  const f32x4 m32r = mul_rows(t_rows[3], z32, zero4());
+  f32x4 m10n, m32n;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    m10n[r] = -m10c[r];
+    m32n[r] = -m32r[r];
+  }
+  const f32x4 z20 = mul_cols(a_rows[4], m10n, mul_cols(a_rows[3], t_cols[0], zero4()));
+  const f32x4 z21 = mul_cols(a_rows[4], t_cols[1], zero4());
+  const f32x4 z30 = mul_cols(a_rows[7], m10n, mul_cols(a_rows[6], t_cols[0], zero4()));
+  const f32x4 z31 = mul_cols(a_rows[7], t_cols[1], zero4());
+
+  auto put = [&](int f, const f32x4& first, const f32x4& second) {
+    f32x4 a, c;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      a[r] = -first[r];
+      c[r] = -second[r];
+    }
+    bf16x8 hi8, lo8;
+    split(a, c, hi8, lo8);
+    *reinterpret_cast<bf16x8*>(block + kBlockM + f * kFrag + lane * 16) = hi8;
+    *reinterpret_cast<bf16x8*>(block + kBlockLow + f * kFrag + lane * 16) = lo8;
+    *reinterpret_cast<bf16x8*>(block + kBlockP + f * kFrag + lane * 16) = pf[f];
+  };
+  if (!COLS) {
+    const f32x4 m10r = mul_rows(t_rows[1], z10, zero4());
+    put(frag_rows(0, 0), m_rows[0], zero4());
+    put(frag_rows(1, 0), m10r, m_rows[1]);
+    put(frag_rows(2, 0), mul_rows(t_rows[2], z20, zero4()), mul_rows(t_rows[2], z21, zero4()));
+    put(frag_rows(2, 1), m_rows[2], zero4());
+    put(frag_rows(3, 0), mul_rows(m32n, z20, mul_rows(t_rows[3], z30, zero4())), mul_rows(m32n, z21, mul_rows(t_rows[3], z31, zero4())));
+    put(frag_rows(3, 1), m32r, m_rows[3]);
+  } else {
+    const f32x4 m32c = mul_cols(t_rows[3], z32, zero4());
+    put(frag_cols(0, 0), m_cols[0], m10c);
+    put(frag_cols(0, 1), mul_cols(t_rows[2], z20, zero4()), mul_cols(m32n, z20, mul_cols(t_rows[3], z30, zero4())));
+    put(frag_cols(1, 0), zero4(), m_cols[1]);
+    put(frag_cols(1, 1), mul_cols(t_rows[2], z21, zero4()), mul_cols(m32n, z21, mul_cols(t_rows[3], z31, zero4())));
+    put(frag_cols(2, 1), m_cols[2], m32c);
+    put(frag_cols(3, 1), zero4(), m_cols[3]);
+  }
+}
+
+}  // namespace
+}  // namespace taac

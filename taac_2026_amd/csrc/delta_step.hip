@@ -1,0 +1,250 @@
+// Gated delta rule, recurrent form: a few new tokens for states that live in a pool, updated in place (the formulas: delta.h).
+//
+// Bound by HBM: a state of dk x dv floats is read and written once for however many tokens the call brings; everything else is
+// small. A workgroup owns the state of one (sample, head): lanes hold four value columns each of some key rows, so that a row is one
+// run of memory, and the whole state stays in registers between its load and its store. A token needs one round of sums over the
+// key rows, of k S and q S and q . k at once, since o = scale (S + k u^T)^T q = scale (S^T q + (k . q) u). All arithmetic is fp32.
+//
+// Samples that name the same slot are one sequence: their tokens are applied in the order of the batch, by the workgroup of the
+// first of them. A slot outside the pool (padding) reads and writes no state and gives zeros.
+#include "common.h"
+
+namespace taac {
+namespace {
+
+struct StepParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  const void* log_decay;
+  const void* beta;
+  float* state;             // [slots, H, dk, dv]
+  const void* slots;        // [B] int32 or int64, or null: slot b
+  const int32_t* lengths;   // [B] or null
+  int64_t qs[3], ks[3], vs[3], os[3], gs[3], bs[3];
+  int64_t pool;             // number of slots
+  int32_t B, H, group, T, dk, dv;
+  int32_t gates_f32, slots_int64;
+  float scale;
+};
+
+template <typename T>
+__device__ __forceinline__ float gate_at(const void* p, int64_t at, int f32) {
+  return f32 ? static_cast<const float*>(p)[at] : static_cast<float>(static_cast<const T*>(p)[at]);
+}
+
+// NVP: lanes to a row of value columns (4 columns each); W wavefronts; RPT key rows to a lane.
+template <typename T, int NVP, int W, int RPT>
+__global__ __launch_bounds__(W * kWave) void delta_step_kernel(const StepParams p) {
+  constexpr int ROWS = W * kWave / NVP;  // rows at once
+  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+  const int vec = tid % NVP, row0 = tid / NVP;
+  const int h = static_cast<int>(blockIdx.x % p.H);
+  const int first = static_cast<int>(blockIdx.x / p.H);
+  __shared__ float red[2][W][NVP][8];
+  __shared__ float red_qk[2][W];
+  const bool col_ok = vec * 4 < p.dv;
+  const T* q = static_cast<const T*>(p.q);
+  const T* k = static_cast<const T*>(p.k);
+  const T* v = static_cast<const T*>(p.v);
+  T* o = static_cast<T*>(p.o);
+  const int hk = h / p.group;
+
+  auto slot_of = [&](int b) -> int64_t {
+    return p.slots_int64 ? static_cast<const int64_t*>(p.slots)[b] : static_cast<const int32_t*>(p.slots)[b];
+  };
+  const int64_t slot = p.slots != nullptr ? slot_of(first) : first;
+  auto length_of = [&](int b) -> int {
+    if (p.lengths == nullptr) return p.T;
+    const int n = p.lengths[b];
+    return n < 0 ? 0 : (n > p.T ? p.T : n);
+  };
+  auto clear = [&](int b, int from) {
+    for (int64_t i = tid; i < static_cast<int64_t>(p.T - from) * p.dv; i += W * kWave)
+      o[b * p.os[0] + h * p.os[1] + (from + i / p.dv) * p.os[2] + i % p.dv] = static_cast<T>(0.f);
+  };
+  if (slot < 0 || slot >= p.pool) {
+    clear(first, 0);
+    return;
+  }
+  f32x4 s[RPT];
+  float* base = p.state + (slot * p.H + h) * static_cast<int64_t>(p.dk) * p.dv;
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int row = row0 + i * ROWS;
+    s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (col_ok && row < p.dk) s[i] = *reinterpret_cast<const f32x4*>(base + static_cast<int64_t>(row) * p.dv + vec * 4);
+  }
+  bool again = false;  // a later sample has the slot too
+  if (p.slots != nullptr && p.B > 1) {
+    bool before = false, after = false;
+    for (int j = tid; j < p.B; j += W * kWave)
+      if (j != first && slot_of(j) == slot) (j < first ? before : after) = true;
+    if (__syncthreads_or(before)) return;  // that sample's workgroup applies these tokens
+    again = __syncthreads_or(after);
+  }
+  bool touched = false;
+  int round = 0;
+  for (int b = first; b < p.B;) {
+    const int n = length_of(b);
+    for (int t = 0; t < n; ++t) {
+      const float a = expf(gate_at<T>(p.log_decay, b * p.gs[0] + h * p.gs[1] + t * p.gs[2], p.gates_f32));
+      const float beta = gate_at<T>(p.beta, b * p.bs[0] + h * p.bs[1] + t * p.bs[2], p.gates_f32);
+      const T* qt = q + b * p.qs[0] + hk * p.qs[1] + t * p.qs[2];
+      const T* kt = k + b * p.ks[0] + hk * p.ks[1] + t * p.ks[2];
+      const T* vt = v + b * p.vs[0] + h * p.vs[1] + t * p.vs[2];
+      float kr[RPT], vf[4] = {0.f, 0.f, 0.f, 0.f};
+      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, qk = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col_ok) vf[e] = static_cast<float>(vt[vec * 4 + e]);
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const int row = row0 + i * ROWS;
+        kr[i] = row < p.dk ? static_cast<float>(kt[row]) : 0.f;
+        const float qr = row < p.dk ? static_cast<float>(qt[row]) : 0.f;
+        qk = fmaf(qr, kr[i], qk);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[i][e] *= a;
+          sum[e] = fmaf(kr[i], s[i][e], sum[e]);
+          sum[4 + e] = fmaf(qr, s[i][e], sum[4 + e]);
+        }
+      }
+#pragma unroll
+      for (int off = NVP; off < kWave; off *= 2) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor(sum[e], off, kWave);
+        qk += __shfl_xor(qk, off, kWave);
+      }
+      if (W > 1) {  // two sets of partial sums in turn: a token's are read while the next token's are written
+        const int buf = round++ & 1;
+        if (lane < NVP) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) red[buf][wave][lane][e] = sum[e];
+          if (lane == 0) red_qk[buf][wave] = qk;
+        }
+        __syncthreads();
+        qk = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[e] += red[buf][w][vec][e];
+          qk += red_qk[buf][w];
+        }
+      }
+      float u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = beta * (vf[e] - sum[e]);
+#pragma unroll
+      for (int i = 0; i < RPT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][e] = fmaf(kr[i], u[e], s[i][e]);
+      if (row0 == 0 && col_ok) {
+        T* ot = o + b * p.os[0] + h * p.os[1] + t * p.os[2] + vec * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ot[e] = static_cast<T>(p.scale * fmaf(qk, u[e], sum[4 + e]));
+      }
+    }
+    touched |= n > 0;
+    clear(b, n);
+    if (!again) break;
+    for (++b; b < p.B && slot_of(b) != slot; ++b) {
+    }
+  }
+  if (!touched) return;
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int row = row0 + i * ROWS;
+    if (col_ok && row < p.dk) *reinterpret_cast<f32x4*>(base + static_cast<int64_t>(row) * p.dv + vec * 4) = s[i];
+  }
+}
+
+template <typename T, int NVP, int W, int RPT>
+void launch_step(const StepParams& p, hipStream_t s) {
+  hipLaunchKernelGGL((delta_step_kernel<T, NVP, W, RPT>), dim3(static_cast<uint32_t>(p.B) * p.H), dim3(W * kWave), 0, s, p);
+}
+
+template <typename T>
+void dispatch_step(const StepParams& p, hipStream_t s) {
+  // one wavefront while a lane's share is at most four rows of four columns, else four wavefronts
+#define TAAC_STEP_ROWS(NVP, W)                                                        \
+  {                                                                                   \
+    constexpr int ROWS = W * kWave / NVP;                                             \
+    if (p.dk <= ROWS) return launch_step<T, NVP, W, 1>(p, s);                         \
+    if (p.dk <= 2 * ROWS) return launch_step<T, NVP, W, 2>(p, s);                     \
+    if (p.dk <= 4 * ROWS) return launch_step<T, NVP, W, 4>(p, s);                     \
+    if constexpr (ROWS <= 16) {                                                       \
+      if (W > 1 && p.dk <= 8 * ROWS) return launch_step<T, NVP, W, 8>(p, s);          \
+      if constexpr (ROWS <= 8) {                                                      \
+        if (W > 1) return launch_step<T, NVP, W, 16>(p, s);                           \
+      }                                                                               \
+    }                                                                                 \
+  }
+  if (p.dv <= 16) {
+    TAAC_STEP_ROWS(4, 1)
+    TAAC_STEP_ROWS(4, 4)
+  } else if (p.dv <= 32) {
+    TAAC_STEP_ROWS(8, 1)
+    TAAC_STEP_ROWS(8, 4)
+  } else if (p.dv <= 64) {
+    TAAC_STEP_ROWS(16, 1)
+    TAAC_STEP_ROWS(16, 4)
+  } else {
+    TAAC_STEP_ROWS(32, 1)
+    TAAC_STEP_ROWS(32, 4)
+  }
+#undef TAAC_STEP_ROWS
+}
+
+int step_strides(const char* name, const char* what, const int64_t* from, int64_t* to) {
+  if (from == nullptr) return set_error(TAAC_ERR_INVALID_VALUE, "%s: null strides of %s", name, what);
+  for (int i = 0; i < 3; ++i) {
+    to[i] = from[i];
+    if (from[i] < 0) return set_error(TAAC_ERR_INVALID_VALUE, "%s: negative stride of %s", name, what);
+  }
+  return TAAC_OK;
+}
+
+}  // namespace
+}  // namespace taac
+
+extern "C" int taac_delta_rule_step(const void* q, const void* k, const void* v, const void* log_decay, const void* beta, float* state,
+                                    int64_t pool, const void* slots, int slots_int64, const int32_t* lengths, void* o, int32_t B, int32_t H,
+                                    int32_t key_heads, int32_t T, int32_t dk, int32_t dv, const int64_t q_strides[3],
+                                    const int64_t k_strides[3], const int64_t v_strides[3], const int64_t o_strides[3],
+                                    const int64_t decay_strides[3], const int64_t beta_strides[3], float scale, int dtype, int gate_dtype,
+                                    void* stream) {
+  using namespace taac;
+  const char* name = "taac_delta_rule_step";
+  if (B < 0 || T < 0 || H <= 0 || key_heads <= 0 || H % key_heads != 0 || pool < 0)
+    return set_error(TAAC_ERR_INVALID_VALUE, "%s: value heads must be a multiple of the key heads, sizes not negative", name);
+  if (dk <= 0 || dv <= 0 || dk % 8 != 0 || dv % 8 != 0 || dk > 128 || dv > 128)
+    return set_error(TAAC_ERR_UNSUPPORTED, "%s: key and value widths must be multiples of 8, at most 128 (got %d, %d)", name, dk, dv);
+  if (dtype != TAAC_F32 && dtype != TAAC_BF16 && dtype != TAAC_F16) return set_error(TAAC_ERR_INVALID_VALUE, "%s: unknown dtype %d", name, dtype);
+  if (gate_dtype != dtype && gate_dtype != TAAC_F32)
+    return set_error(TAAC_ERR_INVALID_VALUE, "%s: gates must be fp32 or of the tokens' dtype", name);
+  if (slots == nullptr && B > pool) return set_error(TAAC_ERR_INVALID_VALUE, "%s: %d samples without slots and a pool of %lld", name, B, (long long)pool);
+  if (static_cast<int64_t>(B) * H > 0x7fffffffLL) return set_error(TAAC_ERR_UNSUPPORTED, "%s: too many workgroups", name);
+  if (B == 0 || T == 0) return TAAC_OK;
+  if (!q || !k || !v || !log_decay || !beta || !o || (pool > 0 && !state)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: null tensor pointer", name);
+  if (!aligned16(state)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: the state must be 16-byte aligned", name);
+  StepParams p{};
+  p.q = q, p.k = k, p.v = v, p.o = o, p.log_decay = log_decay, p.beta = beta, p.state = state, p.slots = slots, p.lengths = lengths;
+  p.pool = pool, p.B = B, p.H = H, p.group = H / key_heads, p.T = T, p.dk = dk, p.dv = dv, p.scale = scale;
+  p.gates_f32 = gate_dtype == TAAC_F32, p.slots_int64 = slots_int64 != 0;
+  if (int rc = step_strides(name, "q", q_strides, p.qs)) return rc;
+  if (int rc = step_strides(name, "k", k_strides, p.ks)) return rc;
+  if (int rc = step_strides(name, "v", v_strides, p.vs)) return rc;
+  if (int rc = step_strides(name, "o", o_strides, p.os)) return rc;
+  if (int rc = step_strides(name, "log_decay", decay_strides, p.gs)) return rc;
+  if (int rc = step_strides(name, "beta", beta_strides, p.bs)) return rc;
+  hipStream_t s = as_stream(stream);
+  if (dtype == TAAC_F32) dispatch_step<float>(p, s);
+  if (dtype == TAAC_BF16) dispatch_step<bf16_t>(p, s);
+  if (dtype == TAAC_F16) dispatch_step<f16_t>(p, s);
+  return check_launch(name);
+}

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from taac_2026_amd import _native
-from taac_2026_amd.api import residual_rms_norm, residual_rms_norm_fp8
+from taac_2026_amd.api import gated_delta_rule, gated_delta_rule_step, residual_rms_norm, residual_rms_norm_fp8
 
 
 @pytest.mark.parametrize("operator", [residual_rms_norm, residual_rms_norm_fp8])
@@ -43,3 +43,82 @@ def test_residual_norm_entry_points_check_on_the_host():
     assert library.taac_linear_fp8_rows(fake, 16, fake, None, fake, None, None, fake, 16, 4, 16, 16, 0, 1, None) == invalid
     assert library.taac_linear_fp8_rows(fake, 24, fake, fake, fake, None, None, fake, 16, 4, 16, 16, 0, 1, None) == \
         _native.TAAC_ERR_UNSUPPORTED
+
+
+def _delta_inputs(batch=1, key_heads=1, heads=2, tokens=5, key_width=16, value_width=8):
+    q, k = (torch.zeros(batch, key_heads, tokens, key_width, dtype=torch.bfloat16) for _ in range(2))
+    v = torch.zeros(batch, heads, tokens, value_width, dtype=torch.bfloat16)
+    return [q, k, v, torch.zeros(batch, heads, tokens), torch.zeros(batch, heads, tokens)]
+
+
+@pytest.mark.parametrize("operator", [gated_delta_rule, lambda *a, **kw: gated_delta_rule_step(*a, torch.zeros(1, 2, 16, 8), **kw)])
+def test_delta_rule_refuses(operator):
+    q, k, v, g, b = _delta_inputs()
+    with pytest.raises(ValueError, match="shape \\(batch, heads"):
+        operator(q[0], k, v, g, b)
+    with pytest.raises(ValueError, match="same shape"):
+        operator(q[..., :8], k, v, g, b)
+    with pytest.raises(ValueError, match="token dimensions"):
+        operator(q, k, v[:, :, :4], g, b)
+    with pytest.raises(ValueError, match="multiple of the key heads"):
+        operator(q.expand(1, 3, 5, 16), k.expand(1, 3, 5, 16), v, g, b)
+    with pytest.raises(ValueError, match="log_decay and beta"):
+        operator(q, k, v, g[..., :4], b)
+    with pytest.raises(ValueError, match="same dtype"):
+        operator(q, k.float(), v, g, b)
+    with pytest.raises(ValueError, match="same dtype"):
+        operator(q, k, v, g, b.bfloat16())
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        operator(q, k, v, g, b)
+
+
+def test_delta_step_refuses():
+    inputs = _delta_inputs()
+    with pytest.raises(ValueError, match="expects a state"):
+        gated_delta_rule_step(*inputs, torch.zeros(1, 2, 8, 16))
+    with pytest.raises(ValueError, match="in place"):
+        gated_delta_rule_step(*inputs, torch.zeros(1, 2, 16, 8, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="in place"):
+        gated_delta_rule_step(*inputs, torch.zeros(1, 2, 8, 16).transpose(2, 3))
+    with pytest.raises(ValueError, match="without state_index"):
+        gated_delta_rule_step(*inputs, torch.zeros(0, 2, 16, 8))
+    for index in (torch.zeros(2, dtype=torch.int32), torch.zeros(1), torch.zeros(1, 1, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="state_index"):
+            gated_delta_rule_step(*inputs, torch.zeros(1, 2, 16, 8), state_index=index)
+
+
+def test_delta_entry_points_check_on_the_host():
+    library = _native.load_library()
+    fake, odd = ctypes.c_void_p(256), ctypes.c_void_p(258)
+    strides = (ctypes.c_int64 * 3)
+    invalid, unsupported, ok = _native.TAAC_ERR_INVALID_VALUE, _native.TAAC_ERR_UNSUPPORTED, _native.TAAC_OK
+    f32, bf16, f16 = _native.TAAC_F32, _native.TAAC_BF16, _native.TAAC_F16
+
+    def forward(**kw):
+        a = dict(q=fake, lengths=None, final=None, states=None, misses=None, B=1, H=2, Hk=1, T=5, dk=16, dv=8, qs=strides(80, 80, 16), gs=strides(10, 5, 1), gate=f32)
+        a.update(kw)
+        s = strides(80, 40, 8)
+        return library.taac_delta_rule_fwd(a["q"], fake, fake, fake, fake, a["lengths"], fake, None, a["final"], a["states"], a["misses"], a["B"], a["H"],
+                                           a["Hk"], a["T"], a["dk"], a["dv"], a["qs"], strides(80, 80, 16), s, s, a["gs"], a["gs"], 1.0, a["gate"], None)
+
+    assert forward(Hk=3) == invalid and b"multiple of the key heads" in library.taac_last_error()
+    assert forward(H=0) == invalid and forward(B=-1) == invalid and forward(T=-1) == invalid
+    assert forward(dk=12) == unsupported and forward(dv=136) == unsupported and b"multiples of 8" in library.taac_last_error()
+    assert forward(gate=f16) == invalid and b"gates" in library.taac_last_error()
+    assert forward(states=fake) == invalid and b"come together" in library.taac_last_error()
+    assert forward(q=None) == invalid and forward(q=odd) == invalid
+    assert forward(qs=strides(80, 80, 12)) == invalid and forward(gs=strides(10, 5, -1)) == invalid and forward(qs=None) == invalid
+    assert forward(B=0) == ok and forward(T=0) == ok
+
+    def step(**kw):
+        a = dict(state=fake, pool=4, slots=fake, B=1, H=2, Hk=1, T=1, dk=16, dv=8, dtype=bf16, gate=f32, qs=strides(16, 16, 16))
+        a.update(kw)
+        s = strides(16, 8, 8)
+        return library.taac_delta_rule_step(fake, fake, fake, fake, fake, a["state"], a["pool"], a["slots"], 0, None, fake, a["B"], a["H"], a["Hk"], a["T"],
+                                            a["dk"], a["dv"], a["qs"], s, s, s, s, s, 1.0, a["dtype"], a["gate"], None)
+
+    assert step(Hk=4) == invalid and step(pool=-1) == invalid and step(state=None) == invalid and step(state=odd) == invalid
+    assert step(dk=4) == unsupported and step(dtype=7) == invalid and step(gate=f16) == invalid
+    assert step(slots=None, B=5) == invalid and b"without slots" in library.taac_last_error()
+    assert step(qs=strides(16, -16, 16)) == invalid and step(qs=None) == invalid
+    assert step(B=0) == ok and step(T=0) == ok
