@@ -617,16 +617,21 @@ int taac_row_rstd(const float* qk_sumsq, int64_t M, int32_t d_model, float eps, 
  * taac_delta_rule_bwd: gradients of q, k, v, log_decay and beta (logical shapes and dtypes of the inputs, strides of their own) for
  * grad_o; grad_states (bf16, the size of chunk_states) is scratch. The initial state has no gradient here. Rows at or beyond a
  * sample's length get zeros. Every sum has a fixed order.
+ * workspace: taac_delta_rule_workspace_bytes(B, H, T, dk, dv) bytes, 16-byte aligned, for either call (0 with many heads, whose
+ * workgroups need none; -1: bad sizes). Calls in flight together must not share one.
  * Replaces: the reference's chunked gated delta rule (accelerators/attention/kernels/gated_delta_rule).
  */
+int64_t taac_delta_rule_workspace_bytes(int32_t B, int32_t H, int32_t T, int32_t dk, int32_t dv);
 int taac_delta_rule_fwd(const void* q, const void* k, const void* v, const void* log_decay, const void* beta, const int32_t* lengths,
-                        void* o, const float* state_in, float* state_out, void* chunk_states, void* misses, int32_t B, int32_t H,
+                        void* o, const float* state_in, float* state_out, void* chunk_states, void* misses, void* workspace,
+                        int64_t workspace_bytes, int32_t B, int32_t H,
                         int32_t key_heads, int32_t T, int32_t dk, int32_t dv, const int64_t q_strides[3], const int64_t k_strides[3],
                         const int64_t v_strides[3], const int64_t o_strides[3], const int64_t decay_strides[3],
                         const int64_t beta_strides[3], float scale, int gate_dtype, void* stream);
 int taac_delta_rule_bwd(const void* q, const void* k, const void* log_decay, const void* beta, const int32_t* lengths,
                         const void* chunk_states, const void* misses, const void* grad_o, void* grad_q, void* grad_k, void* grad_v,
-                        void* grad_decay, void* grad_beta, void* grad_states, int32_t B, int32_t H, int32_t key_heads, int32_t T,
+                        void* grad_decay, void* grad_beta, void* grad_states, void* workspace, int64_t workspace_bytes, int32_t B,
+                        int32_t H, int32_t key_heads, int32_t T,
                         int32_t dk, int32_t dv, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t decay_strides[3],
                         const int64_t beta_strides[3], const int64_t go_strides[3], const int64_t gq_strides[3],
                         const int64_t gk_strides[3], const int64_t gv_strides[3], const int64_t gdecay_strides[3],

@@ -269,9 +269,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_int, c_int, c_void_p],
     ),
     "taac_delta_rule_fwd": (
-        c_int, [c_void_p] * 11 + [c_int32] * 6 + [ctypes.POINTER(c_int64)] * 6 + [c_float, c_int, c_void_p]),
+        c_int, [c_void_p] * 12 + [c_int64] + [c_int32] * 6 + [ctypes.POINTER(c_int64)] * 6 + [c_float, c_int, c_void_p]),
+    "taac_delta_rule_workspace_bytes": (c_int64, [c_int32] * 5),
     "taac_delta_rule_bwd": (
-        c_int, [c_void_p] * 14 + [c_int32] * 6 + [ctypes.POINTER(c_int64)] * 10 + [c_float, c_int, c_void_p]),
+        c_int, [c_void_p] * 15 + [c_int64] + [c_int32] * 6 + [ctypes.POINTER(c_int64)] * 10 + [c_float, c_int, c_void_p]),
     "taac_delta_rule_step": (
         c_int,
         [c_void_p] * 6 + [c_int64, c_void_p, c_int, c_void_p, c_void_p] + [c_int32] * 6 + [ctypes.POINTER(c_int64)] * 6

@@ -60,9 +60,9 @@ def _strides(t: torch.Tensor) -> ctypes.Array:
 
 
 def _rows_view(t: torch.Tensor) -> torch.Tensor:
-    """``t`` where the chunk kernels can read it in place (contiguous rows at 16-byte addresses), else a copy."""
+    """``t`` where the chunk kernels can read it in place (contiguous rows at 16-byte addresses, not too far apart), else a copy."""
     strides = t.stride()
-    if strides[3] == 1 and strides[0] % 8 == strides[1] % 8 == strides[2] % 8 == 0 and t.data_ptr() % 16 == 0:
+    if strides[3] == 1 and strides[0] % 8 == strides[1] % 8 == strides[2] % 8 == 0 and strides[2] < 1 << 24 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -70,6 +70,11 @@ def _rows_view(t: torch.Tensor) -> torch.Tensor:
 def _token_major(batch: int, heads: int, tokens: int, width: int, like: torch.Tensor) -> torch.Tensor:
     """(batch, heads, tokens, width) whose memory order is (batch, tokens, heads, width): the rows of the layers around it."""
     return torch.empty(batch, tokens, heads, width, dtype=like.dtype, device=like.device).transpose(1, 2)
+
+
+def _workspace(k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+    nbytes = _native.load_library().taac_delta_rule_workspace_bytes(v.shape[0], v.shape[1], v.shape[2], k.shape[3], v.shape[3])
+    return torch.empty(nbytes, dtype=torch.uint8, device=v.device)
 
 
 def _forward(q, k, v, log_decay, beta, scale, lengths, initial_state, return_state, keep):
@@ -82,10 +87,12 @@ def _forward(q, k, v, log_decay, beta, scale, lengths, initial_state, return_sta
         states = v.new_empty(batch, heads, (tokens + CHUNK - 1) // CHUNK, key_width, value_width)
         misses = v.new_empty(batch, heads, tokens, value_width)
     library = _native.load_library()
+    workspace = _workspace(k, v)
     with _native.on_device(v.device):
         status = library.taac_delta_rule_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), _native.ptr(lengths), out.data_ptr(),
-            _native.ptr(initial_state), _native.ptr(final), _native.ptr(states), _native.ptr(misses), batch, heads, key_heads, tokens,
+            _native.ptr(initial_state), _native.ptr(final), _native.ptr(states), _native.ptr(misses), _native.ptr(workspace),
+            workspace.numel(), batch, heads, key_heads, tokens,
             key_width, value_width, _strides(q), _strides(k), _strides(v), _strides(out), _strides(log_decay), _strides(beta),
             float(scale), _native.dtype_code(beta.dtype), _native.current_stream(v.device))
     _native.check(status, "gated_delta_rule")
@@ -116,11 +123,12 @@ class _GatedDeltaRuleFunction(torch.autograd.Function):
             grad_q, grad_k = (_token_major(batch, key_heads, tokens, key_width, k) for _ in range(2))
             grad_v = _token_major(batch, heads, tokens, value_width, k)
             grad_decay, grad_beta = (torch.empty(batch, tokens, heads, dtype=beta.dtype, device=k.device).transpose(1, 2) for _ in range(2))
-            grad_states = torch.empty_like(states)
+            grad_states, workspace = torch.empty_like(states), _workspace(k, misses)
             status = library.taac_delta_rule_bwd(
                 q.data_ptr(), k.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), _native.ptr(lengths), states.data_ptr(),
                 misses.data_ptr(), grad_out.data_ptr(), grad_q.data_ptr(), grad_k.data_ptr(), grad_v.data_ptr(), grad_decay.data_ptr(),
-                grad_beta.data_ptr(), grad_states.data_ptr(), batch, heads, key_heads, tokens, key_width, value_width, _strides(q),
+                grad_beta.data_ptr(), grad_states.data_ptr(), workspace.data_ptr(), workspace.numel(), batch, heads, key_heads, tokens,
+                key_width, value_width, _strides(q),
                 _strides(k), _strides(log_decay), _strides(beta), _strides(grad_out), _strides(grad_q), _strides(grad_k),
                 _strides(grad_v), _strides(grad_decay), _strides(grad_beta), ctx.scale, _native.dtype_code(beta.dtype),
                 _native.current_stream(k.device))

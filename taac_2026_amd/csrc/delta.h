@@ -9,9 +9,11 @@
 //
 // All products run on v_mfma_f32_16x16x32_bf16. With lane = (l16 = lane % 16, grp = lane / 16) its operands hold row (or column)
 // l16 and 8 values of the contraction, its result column l16 and rows 4 grp .. 4 grp + 3. The contraction may be walked in any
-// order that both operands share, and the order used everywhere here is: element e of group grp = index 4 grp + e of the first
-// half of a block of 32 for e < 4, of its second half for e >= 4. Two results (16 rows each) are then an operand of the next product as
-// they stand, so a chain X -> N -> S' -> next X never leaves the registers.
+// order that both operands share, and two results (16 rows each) are an operand of the next product as they stand if element e of
+// group grp stands for row 4 grp + e of the first result for e < 4, of the second for e >= 4: a chain X -> N -> S' -> next X never
+// leaves the registers. Over tokens the two results are tokens 0 .. 15 and 16 .. 31 of a block of 32. Over key features an operand
+// holds 8 neighbours of a row of memory, feature 8 grp + e of a block of 32, so row 4 g + r of result a of the state is feature
+// 32 (a / 2) + 8 g + 4 (a % 2) + r (state_row).
 //
 // Precision: q, k, v are bf16 and exact operands. The state and what it is made of (S, X, N, M) are fp32 in registers and enter a
 // product as a bf16 pair hi + lo (16 bits, 2^-17 relative), at two matrix instructions where one factor is exact and three where
@@ -35,6 +37,7 @@ struct DeltaParams {
   float* state_out;          // [B, H, dk, dv] or null
   bf16_t* chunk_states;      // [B, H, chunks, dk, dv] or null: the state in front of every chunk
   bf16_t* misses;            // [B, H, T, dv] or null: N
+  uint8_t* blocks;           // [B, H, chunks] blocks in memory (the form for few heads)
   // backward
   const bf16_t* grad_o;
   bf16_t* grad_q;
@@ -52,6 +55,10 @@ struct DeltaParams {
 };
 
 int delta_check(const char* name, const DeltaParams& p);
+// The form for few heads (delta_team.hip): bytes of its blocks, 0 where the other form is the faster one.
+int64_t delta_team_bytes(int64_t heads, int32_t T, int32_t dv);
+int delta_team_fwd(const char* name, const DeltaParams& p, hipStream_t s);
+int delta_team_back(const char* name, const DeltaParams& p, hipStream_t s);
 int delta_strides(const char* name, const char* what, const void* ptr, const int64_t* from, int64_t* to, bool rows);
 
 namespace {
@@ -97,26 +104,16 @@ __device__ __forceinline__ float load_gate(const void* p, int64_t at, int f32) {
   return f32 ? static_cast<const float*>(p)[at] : static_cast<float>(static_cast<const bf16_t*>(p)[at]);
 }
 
+__device__ __forceinline__ int state_row(int a, int m) { return 32 * (a / 2) + 8 * (m / 4) + 4 * (a % 2) + m % 4; }
+
 // Operand fragment of block kb (32 features) of a row in global memory; null rows and features at or beyond width give zeros.
 __device__ __forceinline__ bf16x8 row_frag(const bf16_t* row, int kb, int grp, int width) {
   bf16x8 r = zero8();
-  if (row != nullptr) {
-    const int at = kb * 32 + grp * 4;
-    bf16x4 lo = {}, hi = {};
-    if (at < width) lo = *reinterpret_cast<const bf16x4*>(row + at);
-    if (at + 16 < width) hi = *reinterpret_cast<const bf16x4*>(row + at + 16);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      r[e] = lo[e];
-      r[4 + e] = hi[e];
-    }
-  }
+  if (row != nullptr && kb * 32 + grp * 8 < width) r = *reinterpret_cast<const bf16x8*>(row + kb * 32 + grp * 8);
   return r;
 }
 
-// Tiles in LDS. A staged tile of 64 token rows keeps each block of 32 features in operand order (group 0's 8 values, then group 1's ..), so
-// that a row fragment is one 16-byte read; rows are 16 bytes longer than their contents, which puts the 16 rows of a read on
-// different banks.
+// Tiles of 64 token rows in LDS. Rows are 16 bytes longer than their contents, which puts the 16 rows of a read on different banks.
 template <int WIDTH>
 struct Tile {
   static constexpr int STRIDE = WIDTH + 8;  // elements
@@ -128,32 +125,25 @@ struct Tile {
       const int row = i / PIECES, piece = i % PIECES;
       bf16x8 v = zero8();
       if (row < n && piece * 8 < width) v = *reinterpret_cast<const bf16x8*>(src + row * ld + piece * 8);
-      // pieces of 4: number 2 (piece % 4) + {0, 1} of the block; number p goes to place 2 (p % 4) + p / 4
-      bf16_t* at = dst + row * STRIDE + (piece / 4) * 32;
-      const int p0 = 2 * (piece % 4);
-      bf16x4 lo, hi;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        lo[e] = v[e];
-        hi[e] = v[4 + e];
-      }
-      *reinterpret_cast<bf16x4*>(at + ((p0 % 4) * 2 + p0 / 4) * 4) = lo;
-      *reinterpret_cast<bf16x4*>(at + (((p0 + 1) % 4) * 2 + (p0 + 1) / 4) * 4) = hi;
+      *reinterpret_cast<bf16x8*>(dst + row * STRIDE + piece * 8) = v;
     }
   }
   static __device__ __forceinline__ bf16x8 row(const bf16_t* tile, int row, int kb, int grp) {
     return *reinterpret_cast<const bf16x8*>(tile + row * STRIDE + kb * 32 + grp * 8);
   }
-  // Four tokens (token0 + 4 grp ..) of feature 16 a + l16: a transposed read. Lane 4 e + q of a group of 16 gives the address of
-  // 8 bytes of token e, lane j receives element j % 4 of what lanes 4 e + j / 4 gave.
-  static __device__ __forceinline__ bf16x4 column(const bf16_t* tile, int token0, int a, int l16, int grp) {
-    const bf16_t* at = tile + (token0 + 4 * grp + l16 / 4) * STRIDE + (a / 2) * 32 + (l16 % 4) * 8 + (a % 2) * 4;
+  // Transposed reads: lane 4 e + q of a group of 16 gives the address of 8 bytes (four features) of token e, lane j receives element j % 4 of
+  // what lanes 4 e + j / 4 gave. Tokens token0 + 4 grp .. of feature 16 a + l16 (values), of feature state_row(a, l16) (key features).
+  static __device__ __forceinline__ bf16x4 read_tr(const bf16_t* at) {
     typedef __attribute__((address_space(3))) bf16x4 lds_vec;
     return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_vec*)(at));
   }
-  // Operand fragment (feature 16 a + l16; tokens of block tk)
-  static __device__ __forceinline__ bf16x8 column_frag(const bf16_t* tile, int tk, int a, int l16, int grp) {
-    const bf16x4 lo = column(tile, 32 * tk, a, l16, grp), hi = column(tile, 32 * tk + 16, a, l16, grp);
+  static __device__ __forceinline__ bf16x4 values(const bf16_t* tile, int token0, int a, int l16, int grp) {
+    return read_tr(tile + (token0 + 4 * grp + l16 / 4) * STRIDE + a * 16 + (l16 % 4) * 4);
+  }
+  static __device__ __forceinline__ bf16x4 keys(const bf16_t* tile, int token0, int a, int l16, int grp) {
+    return read_tr(tile + (token0 + 4 * grp + l16 / 4) * STRIDE + (a / 2) * 32 + (l16 % 4) * 8 + (a % 2) * 4);
+  }
+  static __device__ __forceinline__ bf16x8 join(const bf16x4& lo, const bf16x4& hi) {
     bf16x8 r;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -161,6 +151,13 @@ struct Tile {
       r[4 + e] = hi[e];
     }
     return r;
+  }
+  // operand fragments over the tokens of block tk
+  static __device__ __forceinline__ bf16x8 values_frag(const bf16_t* tile, int tk, int a, int l16, int grp) {
+    return join(values(tile, 32 * tk, a, l16, grp), values(tile, 32 * tk + 16, a, l16, grp));
+  }
+  static __device__ __forceinline__ bf16x8 keys_frag(const bf16_t* tile, int tk, int a, int l16, int grp) {
+    return join(keys(tile, 32 * tk, a, l16, grp), keys(tile, 32 * tk + 16, a, l16, grp));
   }
 };
 

@@ -104,7 +104,7 @@ __global__ __launch_bounds__(NW * kWave) void delta_back_kernel(const DeltaParam
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int row = 16 * a + 4 * grp + r;
+            const int row = state_row(a, 4 * grp + r);
             if (col_ok[n] && row < p.dk) dst[row * p.dv + col[n] + l16] = static_cast<bf16_t>(s[a][n][r]);
           }
       bf16x8 sh[KB][NT], sl[KB][NT];
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(NW * kWave) void delta_back_kernel(const DeltaParam
 #pragma unroll
       for (int tk = 0; tk < 2; ++tk)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) of[tk][n] = TV::column_frag(tile_o, tk, wave * NT + n, l16, grp);
+        for (int n = 0; n < NT; ++n) of[tk][n] = TV::values_frag(tile_o, tk, wave * NT + n, l16, grp);
       f32x4 z[4][NT];
 #pragma unroll
       for (int tj = 0; tj < 4; ++tj) {
@@ -198,8 +198,8 @@ __global__ __launch_bounds__(NW * kWave) void delta_back_kernel(const DeltaParam
           for (int r = 0; r < 4; ++r) s[a][n][r] *= total;
 #pragma unroll
         for (int tk = 0; tk < 2; ++tk) {
-          const bf16x8 kt = TK::column_frag(tile_k, tk, a, l16, grp);
-          const bf16x8 qt = TK::column_frag(tile_q, tk, a, l16, grp);
+          const bf16x8 kt = TK::keys_frag(tile_k, tk, a, l16, grp);
+          const bf16x8 qt = TK::keys_frag(tile_q, tk, a, l16, grp);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             s[a][n] = mfma16(kt, zl[tk][n], mfma16(kt, zh[tk][n], s[a][n]));
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_grads_kernel(const DeltaParam
 #pragma unroll
     for (int a = 0; a < KA; ++a) {
       f32x4 dq = zero4(), dr = zero4(), dc = zero4();
-      const int feature = 16 * a + l16;
+      const int feature = state_row(a, l16);
 #pragma unroll
       for (int vb = 0; vb < VB; ++vb) {
         const bf16x8 sf = row_frag(feature < p.dk ? state + feature * p.dv : nullptr, vb, grp, p.dv);
@@ -414,8 +414,8 @@ __global__ __launch_bounds__(4 * kWave) void delta_grads_kernel(const DeltaParam
       }
 #pragma unroll
       for (int tk = 0; tk < 2; ++tk) {
-        const bf16x8 kt = TK::column_frag(tile_k, tk, a, l16, grp);
-        const bf16x8 qt = TK::column_frag(tile_q, tk, a, l16, grp);
+        const bf16x8 kt = TK::keys_frag(tile_k, tk, a, l16, grp);
+        const bf16x8 qt = TK::keys_frag(tile_q, tk, a, l16, grp);
         dq = mfma16(kt, bil[tk], mfma16(kt, bif[tk], dq));
         dr = mfma16(kt, eil[tk], mfma16(kt, eif[tk], dr));
         dc = mfma16(qt, bjl[tk], mfma16(qt, bjf[tk], dc));
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_grads_kernel(const DeltaParam
     bf16_t* dk_row = p.grad_k + b * p.dks[0] + hk * p.dks[1] + (token0 + row) * p.dks[2];
 #pragma unroll
     for (int a = 0; a < KA; ++a) {
-      const int at = 16 * a + 4 * grp;
+      const int at = state_row(a, 4 * grp);
       if (at >= p.dk) continue;
       bf16x4 dq, dk;
 #pragma unroll
@@ -502,7 +502,8 @@ int launch_grads(const char* name, const DeltaParams& p, hipStream_t s) {
 template <int DK>
 int dispatch_back(const char* name, const DeltaParams& p, hipStream_t s) {
   int rc;
-  if (p.dv <= 32) rc = launch_back<DK, 2, 1>(name, p, s);
+  if (p.blocks != nullptr) rc = delta_team_back(name, p, s);
+  else if (p.dv <= 32) rc = launch_back<DK, 2, 1>(name, p, s);
   else if (p.dv <= 64) rc = launch_back<DK, 2, 2>(name, p, s);
   else rc = launch_back<DK, 2, 4>(name, p, s);
   if (rc != TAAC_OK) return rc;
@@ -516,7 +517,8 @@ int dispatch_back(const char* name, const DeltaParams& p, hipStream_t s) {
 
 extern "C" int taac_delta_rule_bwd(const void* q, const void* k, const void* log_decay, const void* beta, const int32_t* lengths,
                                    const void* chunk_states, const void* misses, const void* grad_o, void* grad_q, void* grad_k,
-                                   void* grad_v, void* grad_decay, void* grad_beta, void* grad_states, int32_t B, int32_t H,
+                                   void* grad_v, void* grad_decay, void* grad_beta, void* grad_states, void* workspace,
+                                   int64_t workspace_bytes, int32_t B, int32_t H,
                                    int32_t key_heads, int32_t T, int32_t dk, int32_t dv, const int64_t q_strides[3],
                                    const int64_t k_strides[3], const int64_t decay_strides[3], const int64_t beta_strides[3],
                                    const int64_t go_strides[3], const int64_t gq_strides[3], const int64_t gk_strides[3],
@@ -554,6 +556,11 @@ extern "C" int taac_delta_rule_bwd(const void* q, const void* k, const void* log
   p.grad_q = static_cast<bf16_t*>(grad_q), p.grad_k = static_cast<bf16_t*>(grad_k), p.grad_v = static_cast<bf16_t*>(grad_v);
   p.grad_decay = grad_decay, p.grad_beta = grad_beta, p.grad_states = static_cast<bf16_t*>(grad_states);
   hipStream_t s = as_stream(stream);
+  if (const int64_t bytes = delta_team_bytes(static_cast<int64_t>(B) * H, T, dv)) {
+    if (workspace == nullptr || workspace_bytes < bytes || !aligned16(workspace))
+      return set_error(TAAC_ERR_INVALID_VALUE, "%s: workspace must hold %lld bytes, 16-byte aligned", name, (long long)bytes);
+    p.blocks = static_cast<uint8_t*>(workspace);
+  }
   if (dk <= 32) return dispatch_back<32>(name, p, s);
   if (dk <= 64) return dispatch_back<64>(name, p, s);
   return dispatch_back<128>(name, p, s);

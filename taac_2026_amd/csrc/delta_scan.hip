@@ -61,7 +61,7 @@ __global__ __launch_bounds__(NW * kWave) void delta_scan_kernel(const DeltaParam
       if (p.state_in != nullptr && col_ok[n]) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = 16 * a + 4 * grp + r;
+          const int row = state_row(a, 4 * grp + r);
           if (row < p.dk) s[a][n][r] = p.state_in[(unit * p.dk + row) * p.dv + col[n] + l16];
         }
       }
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(NW * kWave) void delta_scan_kernel(const DeltaParam
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int row = 16 * a + 4 * grp + r;
+              const int row = state_row(a, 4 * grp + r);
               if (col_ok[n] && row < p.dk) dst[row * p.dv + col[n] + l16] = static_cast<bf16_t>(s[a][n][r]);
             }
       }
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(NW * kWave) void delta_scan_kernel(const DeltaParam
         const f32x4 grown = *reinterpret_cast<const f32x4*>(rows + kRowGrown + 16 * ti + 4 * grp);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const bf16x4 v = TV::column(tile_v, 16 * ti, wave * NT + n, l16, grp);
+          const bf16x4 v = TV::values(tile_v, 16 * ti, wave * NT + n, l16, grp);
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[ti][n][r] = fmaf(-grown[r], y[n][r], static_cast<float>(v[r]));
         }
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(NW * kWave) void delta_scan_kernel(const DeltaParam
           for (int r = 0; r < 4; ++r) s[a][n][r] *= total;
 #pragma unroll
         for (int tk = 0; tk < 2; ++tk) {
-          const bf16x8 kt = TK::column_frag(tile_k, tk, a, l16, grp);
+          const bf16x8 kt = TK::keys_frag(tile_k, tk, a, l16, grp);
 #pragma unroll
           for (int n = 0; n < NT; ++n) s[a][n] = mfma16(kt, xl[tk][n], mfma16(kt, xh[tk][n], s[a][n]));
         }
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(NW * kWave) void delta_scan_kernel(const DeltaParam
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = 16 * a + 4 * grp + r;
+          const int row = state_row(a, 4 * grp + r);
           if (col_ok[n] && row < p.dk) p.state_out[(unit * p.dk + row) * p.dv + col[n] + l16] = s[a][n][r];
         }
   }
@@ -283,6 +283,7 @@ int delta_strides(const char* name, const char* what, const void* ptr, const int
     if (from[i] < 0 || (rows && from[i] % 8 != 0))
       return set_error(TAAC_ERR_INVALID_VALUE, "%s: strides of %s must be multiples of 8, not negative", name, what);
   }
+  if (rows && from[2] >= (1 << 24)) return set_error(TAAC_ERR_UNSUPPORTED, "%s: the token stride of %s must be below 2^24", name, what);
   if (rows && !aligned16(ptr)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: %s must be 16-byte aligned", name, what);
   return TAAC_OK;
 }
@@ -291,7 +292,7 @@ int delta_strides(const char* name, const char* what, const void* ptr, const int
 
 extern "C" int taac_delta_rule_fwd(const void* q, const void* k, const void* v, const void* log_decay, const void* beta,
                                    const int32_t* lengths, void* o, const float* state_in, float* state_out, void* chunk_states,
-                                   void* misses, int32_t B, int32_t H, int32_t key_heads, int32_t T, int32_t dk, int32_t dv,
+                                   void* misses, void* workspace, int64_t workspace_bytes, int32_t B, int32_t H, int32_t key_heads, int32_t T, int32_t dk, int32_t dv,
                                    const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
                                    const int64_t o_strides[3], const int64_t decay_strides[3], const int64_t beta_strides[3], float scale,
                                    int gate_dtype, void* stream) {
@@ -321,6 +322,12 @@ extern "C" int taac_delta_rule_fwd(const void* q, const void* k, const void* v, 
   p.state_in = state_in, p.state_out = state_out;
   p.chunk_states = static_cast<bf16_t*>(chunk_states), p.misses = static_cast<bf16_t*>(misses);
   hipStream_t s = as_stream(stream);
+  if (const int64_t bytes = delta_team_bytes(static_cast<int64_t>(B) * H, T, dv)) {
+    if (workspace == nullptr || workspace_bytes < bytes || !aligned16(workspace))
+      return set_error(TAAC_ERR_INVALID_VALUE, "%s: workspace must hold %lld bytes, 16-byte aligned", name, (long long)bytes);
+    p.blocks = static_cast<uint8_t*>(workspace);
+    return delta_team_fwd(name, p, s);
+  }
   if (chunk_states != nullptr) {
     if (dk <= 32) return dispatch_scan<32, true>(name, p, s);
     if (dk <= 64) return dispatch_scan<64, true>(name, p, s);

@@ -1,0 +1,501 @@
+// Gated delta rule, chunked form, for few heads and long histories (the mathematics, operand order and precision: delta.h).
+//
+// With few (sample, head) pairs the time is the chain of chunks, not the work: what does not depend on the state is made for all
+// chunks at once (one wavefront each) and left in memory, and a chunk's step of the state is spread over four wavefronts to make it
+// short. A workgroup has 16 value columns; wavefront w owns tokens 16 w .. 16 w + 15 of every chunk and a quarter of the key rows
+// of the state. A step is three stages with a barrier behind each,
+//   X (own tokens) from the state | N (own tokens) from X | the state (own rows) from N; the output beside them,
+// whose results meet in LDS as operand fragments. Everything a chunk reads from memory is requested one chunk ahead.
+#include "delta.h"
+
+namespace taac {
+namespace {
+
+template <int DK, bool COLS>
+__global__ __launch_bounds__(kWave) void delta_blocks_kernel(const DeltaParams p) {
+  __shared__ __attribute__((aligned(16))) float rows[336];
+  __shared__ __attribute__((aligned(16))) float scratch[kScratchFloats];
+  const int chunk = static_cast<int>(blockIdx.x % p.chunks);
+  const int64_t unit = blockIdx.x / p.chunks;
+  const int h = static_cast<int>(unit % p.H);
+  const int b = static_cast<int>(unit / p.H);
+  int len = p.T;
+  if (p.lengths != nullptr) len = p.lengths[b] < p.T ? p.lengths[b] : p.T;
+  const int64_t token0 = static_cast<int64_t>(chunk) * kChunk;
+  const int64_t left = len - token0;
+  if (left <= 0) return;
+  uint8_t* block = p.blocks + (unit * p.chunks + chunk) * kBlockBytes;
+  chunk_block<DK, COLS>(p, b, h, token0, left < kChunk ? static_cast<int>(left) : kChunk, block, rows, scratch);
+  float* out = reinterpret_cast<float*>(block + kBlockRows);
+  for (int i = threadIdx.x; i < 336; i += kWave) out[i] = rows[i];
+}
+
+// Half fragments: the four values of one 16-row result, as the first or second half of a fragment of 32 rows in LDS.
+__device__ __forceinline__ void put_half(uint8_t* frags, int tile, int lane, const f32x4& v, int low_at) {
+  bf16x4 hi, lo;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    hi[r] = static_cast<bf16_t>(v[r]);
+    lo[r] = static_cast<bf16_t>(v[r] - static_cast<float>(hi[r]));
+  }
+  uint8_t* at = frags + (tile / 2) * kFrag + lane * 16 + (tile % 2) * 8;
+  *reinterpret_cast<bf16x4*>(at) = hi;
+  *reinterpret_cast<bf16x4*>(at + low_at) = lo;
+}
+__device__ __forceinline__ bf16x8 get_frag(const uint8_t* frags, int f, int lane) {
+  return *reinterpret_cast<const bf16x8*>(frags + f * kFrag + lane * 16);
+}
+
+template <int DK>
+struct TeamLds {  // fragments hi, then lo, of each
+  static constexpr int KB = DK / 32;
+  static constexpr int kState = 0;                      // KB fragments
+  static constexpr int kX = kState + 2 * KB * kFrag;    // 2
+  static constexpr int kN = kX + 4 * kFrag;
+  static constexpr int kW = kN + 4 * kFrag;
+  static constexpr int kTileK = kW + 4 * kFrag;
+  static constexpr int kForward = kTileK + Tile<DK>::BYTES;
+  static constexpr int kTileQ = kForward;               // backward only
+  static constexpr int kBackward = kTileQ + Tile<DK>::BYTES;
+};
+
+// What wavefront w needs of a chunk. Two of them take turns, so that nothing is copied.
+template <int KB>
+struct TeamChunk {
+  bf16x8 kf[KB], qf[KB];
+  bf16x8 mh[2], ml[2], pf[2];
+  f32x4 grown, keep;
+  float grown_row, total;
+  bf16x8 x[2];  // forward: four values of this lane's column in x[0]; backward: dO of the column, fragments over the tokens
+};
+
+// Reads through a uniform base and a 32-bit offset of the lane, which stays the same for every chunk (token strides are below 2^24
+// elements).
+template <typename V, typename T>
+__device__ __forceinline__ V at_offset(const T* base, uint32_t bytes) {
+  return *reinterpret_cast<const V*>(reinterpret_cast<const uint8_t*>(base) + bytes);
+}
+template <typename T, typename V>
+__device__ __forceinline__ void put_offset(T* base, uint32_t bytes, const V& v) {
+  *reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(base) + bytes) = v;
+}
+
+template <int DK, bool COLS>
+struct Team {
+  static constexpr int KB = DK / 32, KA = DK / 16, OWN = KA >= 4 ? KA / 4 : 1;  // OWN: state tiles of a wavefront
+  const DeltaParams& p;
+  int wave, lane, l16, grp, col0, h, b, len, chunks;
+  int64_t unit;
+  bool col_ok, owner;
+  const bf16_t *k0, *q0, *x0;
+  const uint8_t* blocks;
+  uint32_t k_off, q_off, x_off, row_off;
+
+  __device__ __forceinline__ Team(const DeltaParams& params) : p(params) {
+    const int tid = threadIdx.x;
+    wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    lane = tid % kWave, l16 = lane % 16, grp = lane / 16;
+    const int col_groups = (p.dv + 15) / 16;
+    unit = blockIdx.x / col_groups;
+    col0 = static_cast<int>(blockIdx.x % col_groups) * 16;
+    col_ok = col0 + l16 < p.dv;
+    h = static_cast<int>(unit % p.H);
+    b = static_cast<int>(unit / p.H);
+    len = p.T;
+    if (p.lengths != nullptr) {
+      len = p.lengths[b];
+      len = len < 0 ? 0 : (len > p.T ? p.T : len);
+    }
+    chunks = (len + kChunk - 1) / kChunk;
+    const int64_t hk = h / p.group;
+    const int64_t* xs = COLS ? p.dos : p.vs;
+    k0 = p.k + b * p.ks[0] + hk * p.ks[1];
+    q0 = p.q + b * p.qs[0] + hk * p.qs[1];
+    x0 = (COLS ? p.grad_o : p.v) + b * xs[0] + h * xs[1] + col0;
+    blocks = p.blocks + unit * p.chunks * kBlockBytes;
+    owner = wave * OWN < KA;
+    const int row = 16 * wave + l16;
+    k_off = static_cast<uint32_t>(row * p.ks[2] + grp * 8) * 2;
+    q_off = static_cast<uint32_t>(row * p.qs[2] + grp * 8) * 2;
+    // columns behind the last read the last one: they are not stored and meet no other column
+    const int col = col_ok ? l16 : p.dv - 1 - col0;
+    x_off = static_cast<uint32_t>((COLS ? 0 : 16 * wave + 4 * grp) * xs[2] + (COLS ? 4 * grp * xs[2] : 0) + col) * 2;
+    row_off = static_cast<uint32_t>(16 * wave + 4 * grp) * 4;
+  }
+  __device__ __forceinline__ int tokens_of(int chunk) const {
+    const int left = len - chunk * kChunk;
+    return left < kChunk ? left : kChunk;
+  }
+
+  __device__ __forceinline__ void fetch(int chunk, TeamChunk<KB>& c) const {
+    const int64_t token0 = static_cast<int64_t>(chunk) * kChunk;
+    const int n_tok = tokens_of(chunk);
+    const bf16_t *k = k0 + token0 * p.ks[2], *q = q0 + token0 * p.qs[2];
+    const int64_t x_ld = COLS ? p.dos[2] : p.vs[2];
+    const bf16_t* x = x0 + token0 * x_ld;
+    const uint8_t* block = blocks + static_cast<int64_t>(chunk) * kBlockBytes;
+    if (n_tok == kChunk && p.dk == DK) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        c.kf[kb] = at_offset<bf16x8>(k + kb * 32, k_off);
+        c.qf[kb] = at_offset<bf16x8>(q + kb * 32, q_off);
+      }
+      if (COLS) {
+#pragma unroll
+        for (int tk = 0; tk < 2; ++tk)
+          if (tk >= wave / 2) {  // the own tile and those behind it
+#pragma unroll
+            for (int e = 0; e < 8; ++e) c.x[tk][e] = at_offset<bf16_t>(x + (32 * tk + (e / 4) * 16 + e % 4) * x_ld, x_off);
+          }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c.x[0][r] = at_offset<bf16_t>(x + r * x_ld, x_off);
+      }
+    } else {
+      const bool live = 16 * wave + l16 < n_tok;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        c.kf[kb] = c.qf[kb] = zero8();
+        if (live && kb * 32 + grp * 8 < p.dk) {
+          c.kf[kb] = at_offset<bf16x8>(k + kb * 32, k_off);
+          c.qf[kb] = at_offset<bf16x8>(q + kb * 32, q_off);
+        }
+      }
+#pragma unroll
+      for (int tk = 0; tk < (COLS ? 2 : 1); ++tk) {
+        c.x[tk] = zero8();
+#pragma unroll
+        for (int e = 0; e < (COLS ? 8 : 4); ++e) {
+          const int at = COLS ? 32 * tk + (e / 4) * 16 + e % 4 : e;
+          if (at + (COLS ? 0 : 16 * wave) + 4 * grp < n_tok) c.x[tk][e] = at_offset<bf16_t>(x + at * x_ld, x_off);
+        }
+      }
+    }
+#pragma unroll
+    for (int tk = 0; tk < 2; ++tk)
+      if (COLS ? tk >= wave / 2 : tk <= wave / 2) {
+        const int f = COLS ? frag_cols(wave, tk) : frag_rows(wave, tk);
+        c.mh[tk] = at_offset<bf16x8>(block + kBlockM + f * kFrag, lane * 16);
+        c.ml[tk] = at_offset<bf16x8>(block + kBlockLow + f * kFrag, lane * 16);
+        c.pf[tk] = at_offset<bf16x8>(block + kBlockP + f * kFrag, lane * 16);
+      }
+    const uint8_t* rows = block + kBlockRows;
+    c.grown = at_offset<f32x4>(rows + kRowGrown * 4, row_off);
+    c.keep = at_offset<f32x4>(rows + kRowKeep * 4, row_off);
+    if (!COLS) c.grown_row = at_offset<float>(rows + kRowGrown * 4 + wave * 64, l16 * 4);
+    c.total = *reinterpret_cast<const float*>(rows + kRowTotal * 4);
+  }
+
+  // The own rows of the state: register r of tile a, bf16, at dst [dk][dv]
+  __device__ __forceinline__ void store_state(bf16_t* dst, const f32x4 (&s)[OWN]) const {
+    if (!owner || !col_ok) return;
+    const uint32_t off = static_cast<uint32_t>(state_row(0, 4 * grp) * p.dv + col0 + l16) * 2;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const int a = wave * OWN + i;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (p.dk == DK || state_row(a, 4 * grp + r) < p.dk)
+          put_offset(dst + (32 * (a / 2) + 4 * (a % 2) + r) * p.dv, off, static_cast<bf16_t>(s[i][r]));
+    }
+  }
+};
+
+template <int DK, bool TRAIN>
+__global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams p) {
+  typedef Team<DK, false> M;
+  typedef TeamLds<DK> L;
+  typedef Tile<DK> TK;
+  constexpr int KB = M::KB, OWN = M::OWN;
+  __shared__ __attribute__((aligned(64))) uint8_t smem[L::kForward];
+  bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK);
+  uint8_t *s_frags = smem + L::kState, *x_frags = smem + L::kX, *n_frags = smem + L::kN, *w_frags = smem + L::kW;
+  const M m(p);
+  const int wave = m.wave, lane = m.lane, l16 = m.l16, grp = m.grp, col0 = m.col0;
+  bf16_t* o0 = p.o + m.b * p.os[0] + m.h * p.os[1] + col0;
+  const uint32_t o_off = static_cast<uint32_t>((16 * wave + l16) * p.os[2] + 4 * grp) * 2;
+  const uint32_t n_off = static_cast<uint32_t>((16 * wave + 4 * grp) * p.dv + col0 + l16) * 2;
+  const bool quad_ok = col0 + 4 * grp < p.dv;
+
+  f32x4 s[OWN];
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    s[i] = zero4();
+    const int a = wave * OWN + i;
+    if (p.state_in != nullptr && m.col_ok && m.owner) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = state_row(a, 4 * grp + r);
+        if (row < p.dk) s[i][r] = p.state_in[(m.unit * p.dk + row) * p.dv + col0 + l16];
+      }
+    }
+    if (m.owner) put_half(s_frags, a, lane, s[i], KB * kFrag);
+  }
+
+  auto step = [&](int chunk, const TeamChunk<KB>& cur, TeamChunk<KB>& next) __attribute__((always_inline)) {
+    const int64_t token0 = static_cast<int64_t>(chunk) * kChunk;
+    const int n_tok = m.tokens_of(chunk);
+    if (chunk + 1 < m.chunks) m.fetch(chunk + 1, next);
+    if (TRAIN) m.store_state(p.chunk_states + (m.unit * p.chunks + chunk) * static_cast<int64_t>(p.dk) * p.dv, s);
+    // X of the own tokens; K's rows on their way into LDS
+    bf16x8 sh[KB], sl[KB];
+    f32x4 y = zero4(), y2 = zero4();
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      sh[kb] = get_frag(s_frags, kb, lane);
+      sl[kb] = get_frag(s_frags + KB * kFrag, kb, lane);
+      y = mfma16(cur.kf[kb], sh[kb], y);
+      y2 = mfma16(cur.kf[kb], sl[kb], y2);
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+      *reinterpret_cast<bf16x8*>(tile_k + (16 * wave + l16) * TK::STRIDE + kb * 32 + grp * 8) = cur.kf[kb];
+    f32x4 x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = fmaf(-cur.grown[r], y[r] + y2[r], static_cast<float>(cur.x[0][r]));
+    put_half(x_frags, wave, lane, x, 2 * kFrag);
+    __syncthreads();
+
+    // N of the own tokens
+    f32x4 x2 = zero4(), x3 = zero4();
+#pragma unroll
+    for (int tk = 0; tk < 2; ++tk)
+      if (tk <= wave / 2) {
+        const bf16x8 xh = get_frag(x_frags, tk, lane), xl = get_frag(x_frags + 2 * kFrag, tk, lane);
+        x = mfma16(cur.mh[tk], xh, x);
+        x2 = mfma16(cur.mh[tk], xl, x2);
+        x3 = mfma16(cur.ml[tk], xh, x3);
+      }
+    f32x4 out = zero4(), out2 = zero4();  // the state's part of the output: lane = token, four columns each
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      out = mfma16(sh[kb], cur.qf[kb], out);
+      out2 = mfma16(sl[kb], cur.qf[kb], out2);
+    }
+    f32x4 w;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[r] += x2[r] + x3[r];
+      w[r] = x[r] * cur.keep[r];
+    }
+    put_half(w_frags, wave, lane, w, 2 * kFrag);
+    put_half(n_frags, wave, lane, x, 2 * kFrag);
+    if (TRAIN && m.col_ok) {
+      bf16_t* dst = p.misses + (m.unit * p.T + token0) * p.dv;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (16 * wave + 4 * grp + r < n_tok) put_offset(dst + r * p.dv, n_off, static_cast<bf16_t>(x[r]));
+    }
+    const float grown = cur.grown_row * p.scale;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) out[r] = (out[r] + out2[r]) * grown;
+    __syncthreads();
+
+    // the own rows of the state
+    if (m.owner) {
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        const int a = wave * OWN + i;
+        f32x4 s2 = zero4();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[i][r] *= cur.total;
+#pragma unroll
+        for (int tk = 0; tk < 2; ++tk) {
+          const bf16x8 kt = TK::keys_frag(tile_k, tk, a, l16, grp);
+          s[i] = mfma16(kt, get_frag(w_frags, tk, lane), s[i]);
+          s2 = mfma16(kt, get_frag(w_frags + 2 * kFrag, tk, lane), s2);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[i][r] += s2[r];
+        put_half(s_frags, a, lane, s[i], KB * kFrag);
+      }
+    }
+    // the output of the own tokens
+    out2 = zero4();
+#pragma unroll
+    for (int tk = 0; tk < 2; ++tk)
+      if (tk <= wave / 2) {
+        out = mfma16(get_frag(n_frags, tk, lane), cur.pf[tk], out);
+        out2 = mfma16(get_frag(n_frags + 2 * kFrag, tk, lane), cur.pf[tk], out2);
+      }
+    if (16 * wave + l16 < n_tok && quad_ok) {
+      bf16x4 o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = static_cast<bf16_t>(out[r] + out2[r]);
+      put_offset(o0 + token0 * p.os[2], o_off, o);
+    }
+    __syncthreads();
+  };
+  TeamChunk<KB> even, odd;
+  if (m.chunks > 0) m.fetch(0, even);
+  __syncthreads();
+  for (int chunk = 0; chunk < m.chunks; chunk += 2) {
+    step(chunk, even, odd);
+    if (chunk + 1 < m.chunks) step(chunk + 1, odd, even);
+  }
+
+  if (p.state_out != nullptr && m.col_ok && m.owner) {
+#pragma unroll
+    for (int i = 0; i < OWN; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = state_row(wave * OWN + i, 4 * grp + r);
+        if (row < p.dk) p.state_out[(m.unit * p.dk + row) * p.dv + col0 + l16] = s[i][r];
+      }
+  }
+  const bf16x4 none = {};
+  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.T - m.len) * 4; i += 4 * kWave) {
+    const int at = static_cast<int>(i % 4) * 4;
+    if (col0 + at < p.dv) *reinterpret_cast<bf16x4*>(o0 + (m.len + i / 4) * p.os[2] + at) = none;
+  }
+}
+
+// The gradient of the state, chunks last to first (the formulas: delta_bwd.hip). Stages: beta dU (own tokens) | dX (own tokens) | dS (own
+// rows). dO is read as fragments by every wavefront.
+template <int DK>
+__global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaParams p) {
+  typedef Team<DK, true> M;
+  typedef TeamLds<DK> L;
+  typedef Tile<DK> TK;
+  constexpr int KB = M::KB, OWN = M::OWN;
+  __shared__ __attribute__((aligned(64))) uint8_t smem[L::kBackward];
+  bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK);
+  bf16_t* tile_q = reinterpret_cast<bf16_t*>(smem + L::kTileQ);
+  uint8_t *s_frags = smem + L::kState, *z_frags = smem + L::kX, *x_frags = smem + L::kN, *o_frags = smem + L::kW;
+  const M m(p);
+  const int wave = m.wave, lane = m.lane, l16 = m.l16, grp = m.grp, col0 = m.col0;
+  bf16_t* v0 = p.grad_v + m.b * p.dvs[0] + m.h * p.dvs[1] + col0;
+  const uint32_t v_off = static_cast<uint32_t>((16 * wave + 4 * grp) * p.dvs[2] + l16) * 2;
+
+  f32x4 s[OWN];
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    s[i] = zero4();
+    if (m.owner) put_half(s_frags, wave * OWN + i, lane, s[i], KB * kFrag);
+  }
+
+  auto step = [&](int chunk, const TeamChunk<KB>& cur, TeamChunk<KB>& next) __attribute__((always_inline)) {
+    const int64_t token0 = static_cast<int64_t>(chunk) * kChunk;
+    const int n_tok = m.tokens_of(chunk);
+    if (chunk > 0) m.fetch(chunk - 1, next);
+    m.store_state(p.grad_states + (m.unit * p.chunks + chunk) * static_cast<int64_t>(p.dk) * p.dv, s);
+    // beta dU of the own tokens
+    f32x4 z = zero4(), z2 = zero4(), z3 = zero4();
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      z = mfma16(cur.kf[kb], get_frag(s_frags, kb, lane), z);
+      z2 = mfma16(cur.kf[kb], get_frag(s_frags + KB * kFrag, kb, lane), z2);
+    }
+#pragma unroll
+    for (int tk = 0; tk < 2; ++tk)
+      if (tk >= wave / 2) z3 = mfma16(cur.pf[tk], cur.x[tk], z3);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int at = (16 * wave + l16) * TK::STRIDE + kb * 32 + grp * 8;
+      *reinterpret_cast<bf16x8*>(tile_k + at) = cur.kf[kb];
+      *reinterpret_cast<bf16x8*>(tile_q + at) = cur.qf[kb];
+    }
+    f32x4 w;
+    const bf16x8 own = wave < 2 ? cur.x[0] : cur.x[1];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      z[r] = fmaf(cur.keep[r], z[r] + z2[r], z3[r]);
+      w[r] = p.scale * cur.grown[r] * static_cast<float>(wave % 2 == 0 ? own[r] : own[4 + r]);
+    }
+    put_half(z_frags, wave, lane, z, 2 * kFrag);
+    put_half(o_frags, wave, lane, w, 2 * kFrag);
+    __syncthreads();
+
+    // dX of the own tokens
+    z2 = z3 = zero4();
+#pragma unroll
+    for (int tk = 0; tk < 2; ++tk)
+      if (tk >= wave / 2) {
+        const bf16x8 zh = get_frag(z_frags, tk, lane), zl = get_frag(z_frags + 2 * kFrag, tk, lane);
+        z = mfma16(cur.mh[tk], zh, z);
+        z2 = mfma16(cur.mh[tk], zl, z2);
+        z3 = mfma16(cur.ml[tk], zh, z3);
+      }
+    bf16_t* v = v0 + token0 * p.dvs[2];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      z[r] += z2[r] + z3[r];
+      if (m.col_ok && 16 * wave + 4 * grp + r < n_tok) put_offset(v + r * p.dvs[2], v_off, static_cast<bf16_t>(z[r]));
+      w[r] = -cur.grown[r] * z[r];
+    }
+    put_half(x_frags, wave, lane, w, 2 * kFrag);
+    __syncthreads();
+
+    // dS of the own rows
+    if (m.owner) {
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        const int a = wave * OWN + i;
+        f32x4 s2 = zero4(), s3 = zero4(), s4 = zero4();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[i][r] *= cur.total;
+#pragma unroll
+        for (int tk = 0; tk < 2; ++tk) {
+          const bf16x8 kt = TK::keys_frag(tile_k, tk, a, l16, grp), qt = TK::keys_frag(tile_q, tk, a, l16, grp);
+          s[i] = mfma16(kt, get_frag(x_frags, tk, lane), s[i]);
+          s2 = mfma16(kt, get_frag(x_frags + 2 * kFrag, tk, lane), s2);
+          s3 = mfma16(qt, get_frag(o_frags, tk, lane), s3);
+          s4 = mfma16(qt, get_frag(o_frags + 2 * kFrag, tk, lane), s4);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[i][r] += (s2[r] + s4[r]) + s3[r];
+        put_half(s_frags, a, lane, s[i], KB * kFrag);
+      }
+    }
+    __syncthreads();
+  };
+  TeamChunk<KB> even, odd;
+  if (m.chunks > 0) m.fetch(m.chunks - 1, even);
+  __syncthreads();
+  for (int chunk = m.chunks - 1; chunk >= 0; chunk -= 2) {
+    step(chunk, even, odd);
+    if (chunk > 0) step(chunk - 1, odd, even);
+  }
+  const bf16_t none = static_cast<bf16_t>(0.f);
+  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.T - m.len) * 16; i += 4 * kWave) {
+    const int at = static_cast<int>(i % 16);
+    if (col0 + at < p.dv) v0[(m.len + i / 16) * p.dvs[2] + at] = none;
+  }
+}
+
+template <int DK, bool COLS>
+int launch_team(const char* name, const DeltaParams& p, hipStream_t s) {
+  const int64_t heads = static_cast<int64_t>(p.B) * p.H, teams = heads * ((p.dv + 15) / 16);
+  if (heads * p.chunks > 0x7fffffffLL || teams > 0x7fffffffLL) return set_error(TAAC_ERR_UNSUPPORTED, "%s: too many workgroups", name);
+  if (p.chunks > 0) hipLaunchKernelGGL((delta_blocks_kernel<DK, COLS>), dim3(static_cast<uint32_t>(heads * p.chunks)), dim3(kWave), 0, s, p);
+  const dim3 grid(static_cast<uint32_t>(teams)), threads(4 * kWave);
+  if constexpr (COLS) hipLaunchKernelGGL((delta_team_back_kernel<DK>), grid, threads, 0, s, p);
+  else if (p.chunk_states != nullptr) hipLaunchKernelGGL((delta_team_kernel<DK, true>), grid, threads, 0, s, p);
+  else hipLaunchKernelGGL((delta_team_kernel<DK, false>), grid, threads, 0, s, p);
+  return check_launch(name);
+}
+
+}  // namespace
+
+int delta_team_fwd(const char* name, const DeltaParams& p, hipStream_t s) {
+  if (p.dk <= 32) return launch_team<32, false>(name, p, s);
+  if (p.dk <= 64) return launch_team<64, false>(name, p, s);
+  return launch_team<128, false>(name, p, s);
+}
+int delta_team_back(const char* name, const DeltaParams& p, hipStream_t s) {
+  if (p.dk <= 32) return launch_team<32, true>(name, p, s);
+  if (p.dk <= 64) return launch_team<64, true>(name, p, s);
+  return launch_team<128, true>(name, p, s);
+}
+
+int64_t delta_team_bytes(int64_t heads, int32_t T, int32_t dv) {
+  if (heads * ((dv + 15) / 16) > 2048) return 0;
+  return heads * ((T + kChunk - 1) / kChunk) * kBlockBytes;
+}
+
+}  // namespace taac
+
+extern "C" int64_t taac_delta_rule_workspace_bytes(int32_t B, int32_t H, int32_t T, int32_t dk, int32_t dv) {
+  if (B < 0 || H <= 0 || T < 0 || dk <= 0 || dv <= 0) return -1;
+  return taac::delta_team_bytes(static_cast<int64_t>(B) * H, T, dv);
+}

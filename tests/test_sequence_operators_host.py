@@ -95,10 +95,11 @@ def test_delta_entry_points_check_on_the_host():
     f32, bf16, f16 = _native.TAAC_F32, _native.TAAC_BF16, _native.TAAC_F16
 
     def forward(**kw):
-        a = dict(q=fake, lengths=None, final=None, states=None, misses=None, B=1, H=2, Hk=1, T=5, dk=16, dv=8, qs=strides(80, 80, 16), gs=strides(10, 5, 1), gate=f32)
+        a = dict(q=fake, lengths=None, final=None, states=None, misses=None, B=1, H=2, Hk=1, T=5, dk=16, dv=8, qs=strides(80, 80, 16), gs=strides(10, 5, 1), gate=f32,
+                 ws=fake, bytes=1 << 20)
         a.update(kw)
         s = strides(80, 40, 8)
-        return library.taac_delta_rule_fwd(a["q"], fake, fake, fake, fake, a["lengths"], fake, None, a["final"], a["states"], a["misses"], a["B"], a["H"],
+        return library.taac_delta_rule_fwd(a["q"], fake, fake, fake, fake, a["lengths"], fake, None, a["final"], a["states"], a["misses"], a["ws"], a["bytes"], a["B"], a["H"],
                                            a["Hk"], a["T"], a["dk"], a["dv"], a["qs"], strides(80, 80, 16), s, s, a["gs"], a["gs"], 1.0, a["gate"], None)
 
     assert forward(Hk=3) == invalid and b"multiple of the key heads" in library.taac_last_error()
@@ -109,6 +110,11 @@ def test_delta_entry_points_check_on_the_host():
     assert forward(q=None) == invalid and forward(q=odd) == invalid
     assert forward(qs=strides(80, 80, 12)) == invalid and forward(gs=strides(10, 5, -1)) == invalid and forward(qs=None) == invalid
     assert forward(B=0) == ok and forward(T=0) == ok
+    need = library.taac_delta_rule_workspace_bytes(1, 2, 5, 16, 8)
+    assert need > 0 and library.taac_delta_rule_workspace_bytes(1, 0, 5, 16, 8) == -1
+    assert library.taac_delta_rule_workspace_bytes(4096, 8, 512, 32, 32) == 0  # many heads
+    assert forward(bytes=need - 1) == invalid and b"workspace" in library.taac_last_error()
+    assert forward(ws=None) == invalid and forward(ws=odd) == invalid
 
     def step(**kw):
         a = dict(state=fake, pool=4, slots=fake, B=1, H=2, Hk=1, T=1, dk=16, dv=8, dtype=bf16, gate=f32, qs=strides(16, 16, 16))
