@@ -1,4 +1,4 @@
-// Pieces shared by the kernels of the gated delta rule (delta_scan.hip, delta_bwd.hip).
+// Pieces shared by the kernels of the gated delta rule (delta_scan.hip, delta_team.hip, delta_bwd.hip, delta_grads.hip).
 //
 // Per sample and value head, with a_t = exp(g_t), the state S [key_dim, value_dim] follows
 //   N_t = v_t - (a_t S)^T k_t,   S <- a_t S + k_t (beta_t N_t)^T,   o_t = scale S^T q_t.
@@ -59,6 +59,8 @@ int delta_check(const char* name, const DeltaParams& p);
 int64_t delta_team_bytes(int64_t heads, int32_t T, int32_t dv);
 int delta_team_fwd(const char* name, const DeltaParams& p, hipStream_t s);
 int delta_team_back(const char* name, const DeltaParams& p, hipStream_t s);
+// The second half of the backward (delta_grads.hip).
+int delta_grads(const char* name, const DeltaParams& p, hipStream_t s);
 int delta_strides(const char* name, const char* what, const void* ptr, const int64_t* from, int64_t* to, bool rows);
 
 namespace {
@@ -66,9 +68,11 @@ namespace {
 constexpr int kChunk = 64;
 constexpr int kFrag = 1024;              // bytes of one operand fragment of a wavefront
 constexpr int kBlockM = 0, kBlockLow = 6 * kFrag, kBlockP = 12 * kFrag, kBlockRows = 18 * kFrag;
-// floats behind the fragments of a block
-constexpr int kRowHi = 0, kRowLow = 64, kRowBeta = 128, kRowGrown = 192, kRowKeep = 256, kRowTotal = 320;
-constexpr int kBlockBytes = kBlockRows + 336 * 4;
+// floats behind the fragments of a block: e^G, beta e^(G_64 - G), e^G_64 (then e^ of the second and third tile's own decays)
+constexpr int kRowGrown = 0, kRowKeep = 64, kRowTotal = 128, kRowFloats = 144;
+constexpr int kBlockBytes = kBlockRows + kRowFloats * 4;
+// floats that only the maker of a block needs: G as a pair, beta; e^(G - G in front of the tile of 16), e^(G behind the tile - G), that times beta
+constexpr int kTempHi = 0, kTempLow = 64, kTempBeta = 128, kTempIn = 192, kTempOut = 256, kTempOutBeta = 320, kTempFloats = 384;
 constexpr int kScratchFloats = 4 * 16 * 20;  // diagonal blocks, rows of 20 floats
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -128,6 +132,27 @@ struct Tile {
       *reinterpret_cast<bf16x8*>(dst + row * STRIDE + piece * 8) = v;
     }
   }
+  // the two halves of stage() for ROWS rows, so that the loads of several tiles are in flight together
+  template <int ROWS, int THREADS>
+  struct Piece {
+    static constexpr int PIECES = WIDTH / 8, COUNT = (ROWS * PIECES + THREADS - 1) / THREADS;
+    bf16x8 v[COUNT];
+    __device__ __forceinline__ void load(const bf16_t* src, int64_t ld, int n, int width, int tid) {
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i) {
+        const int row = (tid + i * THREADS) / PIECES, piece = (tid + i * THREADS) % PIECES;
+        v[i] = zero8();
+        if (row < n && row < ROWS && piece * 8 < width) v[i] = *reinterpret_cast<const bf16x8*>(src + row * ld + piece * 8);
+      }
+    }
+    __device__ __forceinline__ void store(bf16_t* dst, int tid) const {
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i) {
+        const int row = (tid + i * THREADS) / PIECES, piece = (tid + i * THREADS) % PIECES;
+        if (row < ROWS) *reinterpret_cast<bf16x8*>(dst + row * STRIDE + piece * 8) = v[i];
+      }
+    }
+  };
   static __device__ __forceinline__ bf16x8 row(const bf16_t* tile, int row, int kb, int grp) {
     return *reinterpret_cast<const bf16x8*>(tile + row * STRIDE + kb * 32 + grp * 8);
   }
@@ -179,8 +204,8 @@ __device__ __forceinline__ f32x4 mul_rows(const f32x4& x_rows, const f32x4& y_co
 __host__ __device__ constexpr int frag_rows(int ti, int tk) { return ti < 2 ? ti : 2 + (ti - 2) * 2 + tk; }
 __host__ __device__ constexpr int frag_cols(int tj, int tk) { return tj < 2 ? tj * 2 + tk : 2 + tj; }
 
-// The factors of a chunk's tokens (kRow*), by one wavefront. last_minus: null, or receives e^(G_last - G) of every token.
-__device__ __forceinline__ void chunk_rows(const DeltaParams& p, int b, int h, int64_t token0, int n, float* rows,
+// The factors of a chunk's tokens, by one wavefront. last_minus: null, or receives e^(G_64 - G) of every token.
+__device__ __forceinline__ void chunk_rows(const DeltaParams& p, int b, int h, int64_t token0, int n, float* rows, float* temp,
                                            float* last_minus = nullptr) {
   const int lane = threadIdx.x % kWave;
   // decays in powers of two; an exponent below -1e5 is a decay of zero, and stays finite in the sums
@@ -198,30 +223,44 @@ __device__ __forceinline__ void chunk_rows(const DeltaParams& p, int b, int h, i
     if (lane >= off) total += up;
   }
   const double last = __shfl(total, kWave - 1, kWave);
+  const double behind = __shfl(total, lane | 15, kWave);
+  const double before = __shfl(total, lane < 16 ? 0 : (lane & ~15) - 1, kWave);
   const float hi = static_cast<float>(total);
-  rows[kRowHi + lane] = hi;
-  rows[kRowLow + lane] = static_cast<float>(total - static_cast<double>(hi));
-  rows[kRowBeta + lane] = beta;
+  temp[kTempHi + lane] = hi;
+  temp[kTempLow + lane] = static_cast<float>(total - static_cast<double>(hi));
+  temp[kTempBeta + lane] = beta;
+  temp[kTempIn + lane] = __builtin_amdgcn_exp2f(static_cast<float>(lane < 16 ? total : total - before));
+  const float out = __builtin_amdgcn_exp2f(static_cast<float>(behind - total));
+  temp[kTempOut + lane] = out;
+  temp[kTempOutBeta + lane] = out * beta;
   rows[kRowGrown + lane] = __builtin_amdgcn_exp2f(hi);
   const float left = __builtin_amdgcn_exp2f(static_cast<float>(last - total));
   rows[kRowKeep + lane] = beta * left;
   if (last_minus != nullptr) last_minus[lane] = left;
-  if (lane == 0) rows[kRowTotal] = __builtin_amdgcn_exp2f(static_cast<float>(last));
+  if (lane == 63) rows[kRowTotal] = __builtin_amdgcn_exp2f(hi);
+  if (lane == 31 || lane == 47) rows[kRowTotal + lane / 16] = __builtin_amdgcn_exp2f(static_cast<float>(total - before));
+}
+
+// e^(G in front of tile ti - G behind tile tj), ti > tj: the decay of the whole tiles between them. Gam of a token i of tile ti and a token
+// j of tile tj is this times In_i times Out_j: three factors of at most one, one exponential per token instead of one per pair.
+__device__ __forceinline__ float tiles_between(const float* rows, int ti, int tj) {
+  const float second = rows[kRowTotal + 1], third = rows[kRowTotal + 2];
+  return ti - tj < 2 ? 1.f : (ti - tj == 3 ? second * third : (tj == 0 ? second : third));
 }
 
 // One wavefront makes the block of one chunk (n valid tokens; rows beyond count as k = q = 0, g = 0, beta = 0): -M as hi and lo, P, and the
-// factors of its tokens. COLS: transposed fragments, for the backward. block: LDS or global; rows: LDS floats (kRow*), written for every
-// token; scratch: LDS.
+// factors of its tokens. COLS: transposed fragments, for the backward. block: LDS or global; rows, temp, scratch: LDS; scratch may be
+// the M part of the block, temp its P part.
 //
 // The 64 x 64 inverse: the four diagonal blocks of 16 by substitution, a column per lane, all four at once; the blocks below them by
 // products, M_21 = T_22 A_21 T_11 with T = I - M, first pairs of 16, then of 32.
 template <int DK, bool COLS>
 __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, int64_t token0, int n, uint8_t* block, float* rows,
-                                            float* scratch) {
+                                            float* temp, float* scratch) {
   constexpr int KB = DK / 32;
   const int lane = threadIdx.x % kWave, l16 = lane % 16, grp = lane / 16;
 
-  chunk_rows(p, b, h, token0, n, rows);
+  chunk_rows(p, b, h, token0, n, rows, temp);
   const int64_t hk = h / p.group;
   const bf16_t* kbase = p.k + b * p.ks[0] + hk * p.ks[1] + token0 * p.ks[2];
   const bf16_t* qbase = p.q + b * p.qs[0] + hk * p.qs[1] + token0 * p.qs[2];
@@ -244,7 +283,7 @@ __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, 
     bf16x8 qf[KB];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) qf[kb] = row_frag(row < n ? qbase + row * p.qs[2] : nullptr, kb, grp, p.dk);
-    const float hi_i = rows[kRowHi + row], lo_i = rows[kRowLow + row];
+    const float hi_i = temp[kTempHi + row], lo_i = temp[kTempLow + row], in_i = temp[kTempIn + row];
 #pragma unroll
     for (int tj = 0; tj <= ti; ++tj) {
       f32x4 kk = zero4(), qk = zero4();
@@ -253,25 +292,35 @@ __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, 
         kk = mfma16(kf[tj][kb], kf[ti][kb], kk);
         qk = COLS ? mfma16(qf[kb], kf[tj][kb], qk) : mfma16(kf[tj][kb], qf[kb], qk);
       }
-      const f32x4 hi_j = *reinterpret_cast<const f32x4*>(rows + kRowHi + 16 * tj + 4 * grp);
-      const f32x4 lo_j = *reinterpret_cast<const f32x4*>(rows + kRowLow + 16 * tj + 4 * grp);
-      const f32x4 beta_j = *reinterpret_cast<const f32x4*>(rows + kRowBeta + 16 * tj + 4 * grp);
       f32x4 a, s;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float gam = __builtin_amdgcn_exp2f((hi_i - hi_j[r]) + (lo_i - lo_j[r])) * beta_j[r];
-        const int i = l16, j = 4 * grp + r;
-        a[r] = (ti > tj || i > j) ? gam * kk[r] : 0.f;
-        if (!COLS) s[r] = (ti > tj || i >= j) ? p.scale * gam * qk[r] : 0.f;
-      }
-      if (COLS) {
-        const f32x4 hi_r = *reinterpret_cast<const f32x4*>(rows + kRowHi + 16 * ti + 4 * grp);
-        const f32x4 lo_r = *reinterpret_cast<const f32x4*>(rows + kRowLow + 16 * ti + 4 * grp);
-        const float hi_c = rows[kRowHi + 16 * tj + l16], lo_c = rows[kRowLow + 16 * tj + l16], beta_c = rows[kRowBeta + 16 * tj + l16];
+      if (ti > tj) {
+        const float between = tiles_between(rows, ti, tj);
+        const float a_i = in_i * between, s_i = a_i * p.scale;
+        const f32x4 out_j = *reinterpret_cast<const f32x4*>(temp + kTempOutBeta + 16 * tj + 4 * grp);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float gam = __builtin_amdgcn_exp2f((hi_r[r] - hi_c) + (lo_r[r] - lo_c)) * beta_c;
-          s[r] = (ti > tj || 4 * grp + r >= l16) ? p.scale * gam * qk[r] : 0.f;
+          a[r] = a_i * out_j[r] * kk[r];
+          if (!COLS) s[r] = s_i * out_j[r] * qk[r];
+        }
+        if (COLS) {
+          const float s_j = temp[kTempOutBeta + 16 * tj + l16] * between * p.scale;
+          const f32x4 in_r = *reinterpret_cast<const f32x4*>(temp + kTempIn + 16 * ti + 4 * grp);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[r] = s_j * in_r[r] * qk[r];
+        }
+      } else {
+        const f32x4 hi_j = *reinterpret_cast<const f32x4*>(temp + kTempHi + 16 * tj + 4 * grp);
+        const f32x4 lo_j = *reinterpret_cast<const f32x4*>(temp + kTempLow + 16 * tj + 4 * grp);
+        const f32x4 beta_j = *reinterpret_cast<const f32x4*>(temp + kTempBeta + 16 * tj + 4 * grp);
+        const float beta_i = temp[kTempBeta + row];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int m = 4 * grp + r;
+          const float diff = (hi_i - hi_j[r]) + (lo_i - lo_j[r]);  // of tokens l16 and m of the tile
+          const float gam = __builtin_amdgcn_exp2f(diff) * beta_j[r];
+          a[r] = l16 > m ? gam * kk[r] : 0.f;
+          if (COLS) s[r] = m >= l16 ? p.scale * __builtin_amdgcn_exp2f(-diff) * beta_i * qk[r] : 0.f;
+          else s[r] = l16 >= m ? p.scale * gam * qk[r] : 0.f;
         }
       }
       a_rows[ti * (ti + 1) / 2 + tj] = a;

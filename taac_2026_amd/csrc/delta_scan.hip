@@ -27,7 +27,7 @@ __global__ __launch_bounds__(NW * kWave) void delta_scan_kernel(const DeltaParam
   bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK);
   bf16_t* tile_v = reinterpret_cast<bf16_t*>(smem + L::kTileV);
 
-  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, l16 = lane % 16, grp = lane / 16;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, l16 = lane % 16, grp = lane / 16;
   const int col_groups = (p.dv + L::COLS - 1) / L::COLS;
   const int64_t unit = blockIdx.x / col_groups;
   const int col0 = static_cast<int>(blockIdx.x % col_groups) * L::COLS;  // of the workgroup
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(NW * kWave) void delta_scan_kernel(const DeltaParam
       const int64_t token0 = static_cast<int64_t>(base + wave) * kChunk;
       const int left = len - static_cast<int>(token0);
       chunk_block<DK, false>(p, b, h, token0, left < kChunk ? left : kChunk, block, reinterpret_cast<float*>(block + kBlockRows),
-                             reinterpret_cast<float*>(block));
+                             reinterpret_cast<float*>(block + kBlockP), reinterpret_cast<float*>(block));
     }
     const int here = chunks - base < NW ? chunks - base : NW;
     for (int c = 0; c < here; ++c) {

@@ -13,7 +13,8 @@ namespace {
 
 template <int DK, bool COLS>
 __global__ __launch_bounds__(kWave) void delta_blocks_kernel(const DeltaParams p) {
-  __shared__ __attribute__((aligned(16))) float rows[336];
+  __shared__ __attribute__((aligned(16))) float rows[kRowFloats];
+  __shared__ __attribute__((aligned(16))) float temp[kTempFloats];
   __shared__ __attribute__((aligned(16))) float scratch[kScratchFloats];
   const int chunk = static_cast<int>(blockIdx.x % p.chunks);
   const int64_t unit = blockIdx.x / p.chunks;
@@ -25,9 +26,9 @@ __global__ __launch_bounds__(kWave) void delta_blocks_kernel(const DeltaParams p
   const int64_t left = len - token0;
   if (left <= 0) return;
   uint8_t* block = p.blocks + (unit * p.chunks + chunk) * kBlockBytes;
-  chunk_block<DK, COLS>(p, b, h, token0, left < kChunk ? static_cast<int>(left) : kChunk, block, rows, scratch);
+  chunk_block<DK, COLS>(p, b, h, token0, left < kChunk ? static_cast<int>(left) : kChunk, block, rows, temp, scratch);
   float* out = reinterpret_cast<float*>(block + kBlockRows);
-  for (int i = threadIdx.x; i < 336; i += kWave) out[i] = rows[i];
+  for (int i = threadIdx.x; i < kRowFloats; i += kWave) out[i] = rows[i];
 }
 
 // Half fragments: the four values of one 16-row result, as the first or second half of a fragment of 32 rows in LDS.
