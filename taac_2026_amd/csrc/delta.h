@@ -1,4 +1,5 @@
-// Pieces shared by the kernels of the gated delta rule (delta_scan.hip, delta_team.hip, delta_bwd.hip, delta_grads.hip).
+// Pieces shared by the kernels of the gated delta rule (delta_solo.hip, delta_team.hip, delta_scan.hip, delta_bwd.hip,
+// delta_grads.hip).
 //
 // Per sample and value head, with a_t = exp(g_t), the state S [key_dim, value_dim] follows
 //   N_t = v_t - (a_t S)^T k_t,   S <- a_t S + k_t (beta_t N_t)^T,   o_t = scale S^T q_t.
@@ -59,6 +60,8 @@ int delta_check(const char* name, const DeltaParams& p);
 int64_t delta_team_bytes(int64_t heads, int32_t T, int32_t dv);
 int delta_team_fwd(const char* name, const DeltaParams& p, hipStream_t s);
 int delta_team_back(const char* name, const DeltaParams& p, hipStream_t s);
+// The form for many heads of at most 64 key features (delta_solo.hip).
+int delta_solo(const char* name, const DeltaParams& p, bool back, hipStream_t s);
 // The second half of the backward (delta_grads.hip).
 int delta_grads(const char* name, const DeltaParams& p, hipStream_t s);
 int delta_strides(const char* name, const char* what, const void* ptr, const int64_t* from, int64_t* to, bool rows);
@@ -106,6 +109,17 @@ __device__ __forceinline__ bf16x8 zero8() {
 
 __device__ __forceinline__ float load_gate(const void* p, int64_t at, int f32) {
   return f32 ? static_cast<const float*>(p)[at] : static_cast<float>(static_cast<const bf16_t*>(p)[at]);
+}
+
+// Reads through a uniform base and a 32-bit offset of the lane, which stays the same for every chunk (token strides are below 2^24
+// elements).
+template <typename V, typename T>
+__device__ __forceinline__ V at_offset(const T* base, uint32_t bytes) {
+  return *reinterpret_cast<const V*>(reinterpret_cast<const uint8_t*>(base) + bytes);
+}
+template <typename T, typename V>
+__device__ __forceinline__ void put_offset(T* base, uint32_t bytes, const V& v) {
+  *reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(base) + bytes) = v;
 }
 
 __device__ __forceinline__ int state_row(int a, int m) { return 32 * (a / 2) + 8 * (m / 4) + 4 * (a % 2) + m % 4; }
@@ -197,6 +211,30 @@ __device__ __forceinline__ f32x4 mul_rows(const f32x4& x_rows, const f32x4& y_co
 #pragma unroll
   for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(y_cols[r], x_rows[r], acc, 0, 0, 0);
   return acc;
+}
+
+// M of the four diagonal blocks of 16 in scratch, in the place of A, all four at once: M_ic = A_ic - sum over c < j < i of A_ij M_jc, a column
+// c per lane. Every lane of the wavefront has written its part of A before a wave_sync().
+__device__ __forceinline__ void solve_diagonal(float* scratch, int lane) {
+  float* mine = scratch + lane / 16 * 16 * 20;
+  const int l16 = lane % 16;
+  float m[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float acc = mine[i * 20 + l16];
+#pragma unroll
+    for (int j4 = 0; j4 * 4 < i; ++j4) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(mine + i * 20 + 4 * j4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (4 * j4 + e < i) acc = fmaf(-a[e], m[4 * j4 + e], acc);
+    }
+    m[i] = acc;
+  }
+  wave_sync();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) mine[i * 20 + l16] = m[i];
+  wave_sync();
 }
 
 // Place of a fragment in a block. By rows (forward): row tile ti, token block tk <= ti / 2. By columns (backward): column tile tj, token
@@ -335,26 +373,7 @@ __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, 
 #pragma unroll
   for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(scratch + (t * 16 + l16) * 20 + 4 * grp) = a_rows[t * (t + 1) / 2 + t];
   wave_sync();
-  {
-    float* mine = scratch + grp * 16 * 20;
-    float m[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float acc = mine[i * 20 + l16];
-#pragma unroll
-      for (int j4 = 0; j4 * 4 < i; ++j4) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(mine + i * 20 + 4 * j4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (4 * j4 + e < i) acc = fmaf(-a[e], m[4 * j4 + e], acc);
-      }
-      m[i] = acc;
-    }
-    wave_sync();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mine[i * 20 + l16] = m[i];
-  }
-  wave_sync();
+  solve_diagonal(scratch, lane);
   f32x4 m_rows[4], m_cols[4], t_rows[4], t_cols[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {

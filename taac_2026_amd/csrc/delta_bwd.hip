@@ -225,6 +225,7 @@ template <int DK>
 int dispatch_back(const char* name, const DeltaParams& p, hipStream_t s) {
   int rc;
   if (p.blocks != nullptr) rc = delta_team_back(name, p, s);
+  else if (p.dk <= 64) rc = delta_solo(name, p, true, s);
   else if (p.dv <= 32) rc = launch_back<DK, 2, 1>(name, p, s);
   else if (p.dv <= 64) rc = launch_back<DK, 2, 2>(name, p, s);
   else rc = launch_back<DK, 2, 4>(name, p, s);
@@ -280,7 +281,5 @@ extern "C" int taac_delta_rule_bwd(const void* q, const void* k, const void* log
       return set_error(TAAC_ERR_INVALID_VALUE, "%s: workspace must hold %lld bytes, 16-byte aligned", name, (long long)bytes);
     p.blocks = static_cast<uint8_t*>(workspace);
   }
-  if (dk <= 32) return dispatch_back<32>(name, p, s);
-  if (dk <= 64) return dispatch_back<64>(name, p, s);
   return dispatch_back<128>(name, p, s);
 }

@@ -328,12 +328,6 @@ extern "C" int taac_delta_rule_fwd(const void* q, const void* k, const void* v, 
     p.blocks = static_cast<uint8_t*>(workspace);
     return delta_team_fwd(name, p, s);
   }
-  if (chunk_states != nullptr) {
-    if (dk <= 32) return dispatch_scan<32, true>(name, p, s);
-    if (dk <= 64) return dispatch_scan<64, true>(name, p, s);
-    return dispatch_scan<128, true>(name, p, s);
-  }
-  if (dk <= 32) return dispatch_scan<32, false>(name, p, s);
-  if (dk <= 64) return dispatch_scan<64, false>(name, p, s);
-  return dispatch_scan<128, false>(name, p, s);
+  if (dk <= 64) return delta_solo(name, p, false, s);
+  return chunk_states != nullptr ? dispatch_scan<128, true>(name, p, s) : dispatch_scan<128, false>(name, p, s);
 }

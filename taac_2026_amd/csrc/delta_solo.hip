@@ -1,0 +1,601 @@
+// Gated delta rule, chunked form, for many heads of at most 64 key features (the mathematics, operand order and precision: delta.h).
+//
+// With many (sample, head) pairs the time is work and memory traffic, not the chain of chunks: a wavefront walks the tokens of one head
+// and 32 value columns on its own, without a barrier, and everything it makes for a chunk stays in its registers. It takes 64 tokens
+// at a time from memory and walks them as two chunks of 32, which need a third of the fp32 products of one chunk of 64: the four
+// diagonal blocks of 16 are still solved at once, a column per lane, but only one block below the diagonal is left per chunk
+// instead of six per 64 tokens. Scores are made where they are used.
+#include "delta.h"
+
+namespace taac {
+namespace {
+
+constexpr int kHalf = 32, kSoloCols = 32, kNT = 2;
+
+template <int DK, bool BACK>
+struct SoloLds {
+  typedef Tile<DK> TK;
+  typedef Tile<kSoloCols> TV;
+  static constexpr int kTileV = TK::BYTES * (BACK ? 2 : 1);
+  static constexpr int kScratch = kTileV + TV::BYTES;
+  static constexpr int kTotal = kScratch + kScratchFloats * 4;
+};
+
+// Floats of the 64 tokens in LDS: G as a pair, beta; e^(G - G in front of the tile of 16), e^(G behind the tile - G) beta; and over the chunk of 32:
+// e^(G - G in front of it), beta e^(G behind it - G). Behind them the decay of each chunk.
+constexpr int kSoloHi = 0, kSoloLow = 64, kSoloBeta = 128, kSoloIn = 192, kSoloOut = 256, kSoloGrown = 320, kSoloKeep = 384, kSoloTotal = 448,
+              kSoloFloats = 452;
+
+template <int DK>
+struct SoloTokens {
+  bf16x8 kf[4][DK / 32], qf[4][DK / 32], x[4];  // x: pieces of the values (backward: of dO)
+  float g, beta;
+};
+
+template <int DK, bool BACK>
+struct Solo {
+  static constexpr int KB = DK / 32, KA = DK / 16;
+  typedef Tile<DK> TK;
+  typedef Tile<kSoloCols> TV;
+  const DeltaParams& p;
+  int lane, l16, grp, col0, h, b, len, groups;
+  int64_t unit;
+  const bf16_t *k0, *q0, *x0;
+  uint32_t k_off, q_off, x_off;
+  int64_t x_ld;
+
+  __device__ __forceinline__ Solo(const DeltaParams& params) : p(params) {
+    lane = threadIdx.x, l16 = lane % 16, grp = lane / 16;
+    const int col_groups = (p.dv + kSoloCols - 1) / kSoloCols;
+    unit = blockIdx.x / col_groups;
+    col0 = static_cast<int>(blockIdx.x % col_groups) * kSoloCols;
+    h = static_cast<int>(unit % p.H);
+    b = static_cast<int>(unit / p.H);
+    len = p.T;
+    if (p.lengths != nullptr) {
+      len = p.lengths[b];
+      len = len < 0 ? 0 : (len > p.T ? p.T : len);
+    }
+    groups = (len + kChunk - 1) / kChunk;
+    const int64_t hk = h / p.group;
+    const int64_t* xs = BACK ? p.dos : p.vs;
+    x_ld = xs[2];
+    k0 = p.k + b * p.ks[0] + hk * p.ks[1];
+    q0 = p.q + b * p.qs[0] + hk * p.qs[1];
+    x0 = (BACK ? p.grad_o : p.v) + b * xs[0] + h * xs[1] + col0;
+    k_off = static_cast<uint32_t>(l16 * p.ks[2] + grp * 8) * 2;
+    q_off = static_cast<uint32_t>(l16 * p.qs[2] + grp * 8) * 2;
+    // pieces behind the last read the last one: their columns are not stored and meet no other column
+    const int last = (p.dv - col0) / 8 - 1, piece = lane % 4;
+    x_off = static_cast<uint32_t>(lane / 4 * x_ld + (piece < last ? piece : last) * 8) * 2;
+  }
+  __device__ __forceinline__ int tokens_of(int group) const {
+    const int left = len - group * kChunk;
+    return left < kChunk ? left : kChunk;
+  }
+
+  __device__ __forceinline__ void fetch(int group, SoloTokens<DK>& c) const {
+    const int64_t token0 = static_cast<int64_t>(group) * kChunk;
+    const int n_tok = tokens_of(group);
+    const bf16_t *k = k0 + token0 * p.ks[2], *q = q0 + token0 * p.qs[2], *x = x0 + token0 * x_ld;
+    c.g = c.beta = 0.f;
+    if (lane < n_tok) {
+      c.g = load_gate(p.log_decay, b * p.gs[0] + h * p.gs[1] + (token0 + lane) * p.gs[2], p.gates_f32);
+      c.beta = load_gate(p.beta, b * p.bs[0] + h * p.bs[1] + (token0 + lane) * p.bs[2], p.gates_f32);
+    }
+    if (n_tok == kChunk && p.dk == DK) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          c.kf[t][kb] = at_offset<bf16x8>(k + t * 16 * p.ks[2] + kb * 32, k_off);
+          c.qf[t][kb] = at_offset<bf16x8>(q + t * 16 * p.qs[2] + kb * 32, q_off);
+        }
+        c.x[t] = at_offset<bf16x8>(x + t * 16 * x_ld, x_off);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          c.kf[t][kb] = c.qf[t][kb] = zero8();
+          if (16 * t + l16 < n_tok && kb * 32 + grp * 8 < p.dk) {
+            c.kf[t][kb] = at_offset<bf16x8>(k + t * 16 * p.ks[2] + kb * 32, k_off);
+            c.qf[t][kb] = at_offset<bf16x8>(q + t * 16 * p.qs[2] + kb * 32, q_off);
+          }
+        }
+        c.x[t] = zero8();
+        if (16 * t + lane / 4 < n_tok) c.x[t] = at_offset<bf16x8>(x + t * 16 * x_ld, x_off);
+      }
+    }
+  }
+
+  // The tokens' factors and rows into LDS.
+  __device__ __forceinline__ void place(const SoloTokens<DK>& c, float* rows, bf16_t* tile_k, bf16_t* tile_q, bf16_t* tile_x) const {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int at = (16 * t + l16) * TK::STRIDE + kb * 32 + grp * 8;
+        *reinterpret_cast<bf16x8*>(tile_k + at) = c.kf[t][kb];
+        if (BACK) *reinterpret_cast<bf16x8*>(tile_q + at) = c.qf[t][kb];
+      }
+      *reinterpret_cast<bf16x8*>(tile_x + (16 * t + lane / 4) * TV::STRIDE + (lane % 4) * 8) = c.x[t];
+    }
+    const float g = c.g < -1e5f ? -1e5f : c.g;  // a decay of zero, finite in the sums
+    double total = static_cast<double>(g) * 1.4426950408889634;
+#pragma unroll
+    for (int off = 1; off < kWave; off *= 2) {
+      const double up = __shfl_up(total, off, kWave);
+      if (lane >= off) total += up;
+    }
+    const double tile_end = __shfl(total, lane | 15, kWave), half_end = __shfl(total, lane | 31, kWave);
+    double tile_start = __shfl(total, lane < 16 ? 0 : (lane & ~15) - 1, kWave), half_start = __shfl(total, 31, kWave);
+    if (lane < 16) tile_start = 0.0;
+    if (lane < 32) half_start = 0.0;
+    const float hi = static_cast<float>(total - half_start);
+    const float grown = __builtin_amdgcn_exp2f(hi);
+    rows[kSoloHi + lane] = hi;
+    rows[kSoloLow + lane] = static_cast<float>(total - half_start - static_cast<double>(hi));
+    rows[kSoloBeta + lane] = c.beta;
+    rows[kSoloIn + lane] = __builtin_amdgcn_exp2f(static_cast<float>(total - tile_start));
+    rows[kSoloOut + lane] = __builtin_amdgcn_exp2f(static_cast<float>(tile_end - total)) * c.beta;
+    rows[kSoloGrown + lane] = grown;
+    rows[kSoloKeep + lane] = __builtin_amdgcn_exp2f(static_cast<float>(half_end - total)) * c.beta;
+    if ((lane & 31) == 31) rows[kSoloTotal + lane / 32] = grown;
+    wave_sync();
+  }
+
+  // Gam_ij beta_j of a tile of 16 x 16, by rows (lane: token i = l16 of tile ti, tokens j = 4 grp .. of tile tj), 0 for j > i; strict: for j >= i.
+  __device__ __forceinline__ f32x4 decays_by_rows(const float* rows, int ti, int tj, bool strict) const {
+    f32x4 gam;
+    if (ti > tj) {
+      const float in_i = rows[kSoloIn + 16 * ti + l16];
+      const f32x4 out_j = *reinterpret_cast<const f32x4*>(rows + kSoloOut + 16 * tj + 4 * grp);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) gam[r] = in_i * out_j[r];
+    } else {
+      const float hi_i = rows[kSoloHi + 16 * ti + l16], lo_i = rows[kSoloLow + 16 * ti + l16];
+      const f32x4 hi_j = *reinterpret_cast<const f32x4*>(rows + kSoloHi + 16 * tj + 4 * grp);
+      const f32x4 lo_j = *reinterpret_cast<const f32x4*>(rows + kSoloLow + 16 * tj + 4 * grp);
+      const f32x4 beta_j = *reinterpret_cast<const f32x4*>(rows + kSoloBeta + 16 * tj + 4 * grp);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = 4 * grp + r;
+        const float e = __builtin_amdgcn_exp2f((hi_i - hi_j[r]) + (lo_i - lo_j[r])) * beta_j[r];
+        gam[r] = (strict ? l16 > j : l16 >= j) ? e : 0.f;
+      }
+    }
+    return gam;
+  }
+  // The same by columns (lane: token j = l16 of tile tj, tokens i = 4 grp .. of tile ti).
+  __device__ __forceinline__ f32x4 decays_by_cols(const float* rows, int ti, int tj) const {
+    f32x4 gam;
+    if (ti > tj) {
+      const float out_j = rows[kSoloOut + 16 * tj + l16];
+      const f32x4 in_i = *reinterpret_cast<const f32x4*>(rows + kSoloIn + 16 * ti + 4 * grp);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) gam[r] = out_j * in_i[r];
+    } else {
+      const float hi_j = rows[kSoloHi + 16 * tj + l16], lo_j = rows[kSoloLow + 16 * tj + l16], beta_j = rows[kSoloBeta + 16 * tj + l16];
+      const f32x4 hi_i = *reinterpret_cast<const f32x4*>(rows + kSoloHi + 16 * ti + 4 * grp);
+      const f32x4 lo_i = *reinterpret_cast<const f32x4*>(rows + kSoloLow + 16 * ti + 4 * grp);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float e = __builtin_amdgcn_exp2f((hi_i[r] - hi_j) + (lo_i[r] - lo_j)) * beta_j;
+        gam[r] = 4 * grp + r >= l16 ? e : 0.f;
+      }
+    }
+    return gam;
+  }
+
+  // -M of both chunks as operand fragments, hi and lo: by rows (forward), fragment t = row tile t; by columns (backward), column tile t.
+  __device__ __forceinline__ void solve(const SoloTokens<DK>& c, const float* rows, float* scratch, bf16x8 (&mh)[4], bf16x8 (&ml)[4]) const {
+    f32x4 low[2];  // the blocks below the diagonal, by rows
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      f32x4 kk = zero4();
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) kk = mfma16(c.kf[t][kb], c.kf[t][kb], kk);
+      const f32x4 gam = decays_by_rows(rows, t, t, true);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) kk[r] *= gam[r];
+      *reinterpret_cast<f32x4*>(scratch + (t * 16 + l16) * 20 + 4 * grp) = kk;
+    }
+    wave_sync();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      low[s] = zero4();
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) low[s] = mfma16(c.kf[2 * s][kb], c.kf[2 * s + 1][kb], low[s]);
+      const f32x4 gam = decays_by_rows(rows, 2 * s + 1, 2 * s, true);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) low[s][r] *= gam[r];
+    }
+    solve_diagonal(scratch, lane);
+    f32x4 m_rows[4], m_cols[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      m_rows[t] = *reinterpret_cast<const f32x4*>(scratch + (t * 16 + l16) * 20 + 4 * grp);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) m_cols[t][r] = scratch[(t * 16 + 4 * grp + r) * 20 + l16];
+    }
+    wave_sync();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      f32x4 t0, t1;  // T of the first block by columns, of the second by rows
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float one = l16 == 4 * grp + r ? 1.f : 0.f;
+        t0[r] = one - m_cols[2 * s][r];
+        t1[r] = m_rows[2 * s + 1][r] - one;  // negative: gives -M below
+      }
+      const f32x4 z = mul_cols(low[s], t0, zero4());
+      const f32x4 below = BACK ? mul_cols(t1, z, zero4()) : mul_rows(t1, z, zero4());
+      f32x4 d0, d1;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        d0[r] = BACK ? -m_cols[2 * s][r] : -m_rows[2 * s][r];
+        d1[r] = BACK ? -m_cols[2 * s + 1][r] : -m_rows[2 * s + 1][r];
+      }
+      if (BACK) {
+        split(d0, below, mh[2 * s], ml[2 * s]);
+        split(zero4(), d1, mh[2 * s + 1], ml[2 * s + 1]);
+      } else {
+        split(d0, zero4(), mh[2 * s], ml[2 * s]);
+        split(below, d1, mh[2 * s + 1], ml[2 * s + 1]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void split_state(const f32x4 (&s)[KA][kNT], bf16x8 (&sh)[KB][kNT], bf16x8 (&sl)[KB][kNT]) const {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) split(s[2 * kb][n], s[2 * kb + 1][n], sh[kb][n], sl[kb][n]);
+  }
+  // 16-bit copies of the state at dst [dk][dv]
+  __device__ __forceinline__ void store_state(bf16_t* dst, const f32x4 (&s)[KA][kNT]) const {
+    const uint32_t off = static_cast<uint32_t>(8 * grp * p.dv + col0 + l16) * 2;
+#pragma unroll
+    for (int a = 0; a < KA; ++a)
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        if (col0 + 16 * n + l16 >= p.dv) continue;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (p.dk == DK || state_row(a, 4 * grp + r) < p.dk)
+            put_offset(dst + (32 * (a / 2) + 4 * (a % 2) + r) * p.dv + 16 * n, off, static_cast<bf16_t>(s[a][n][r]));
+      }
+  }
+};
+
+template <int DK, bool TRAIN>
+__global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(const DeltaParams p) {
+  typedef Solo<DK, false> W;
+  typedef SoloLds<DK, false> L;
+  typedef Tile<DK> TK;
+  typedef Tile<kSoloCols> TV;
+  constexpr int KB = W::KB, KA = W::KA;
+  __shared__ __attribute__((aligned(64))) uint8_t smem[L::kTotal];
+  __shared__ __attribute__((aligned(16))) float rows[kSoloFloats];
+  bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem);
+  bf16_t* tile_v = reinterpret_cast<bf16_t*>(smem + L::kTileV);
+  float* scratch = reinterpret_cast<float*>(smem + L::kScratch);
+  const W w(p);
+  const int lane = w.lane, l16 = w.l16, grp = w.grp, col0 = w.col0;
+  bf16_t* o0 = p.o + w.b * p.os[0] + w.h * p.os[1] + col0;
+  const uint32_t o_off = static_cast<uint32_t>(l16 * p.os[2] + 4 * grp) * 2;
+  const uint32_t n_off = static_cast<uint32_t>(4 * grp * p.dv + col0 + l16) * 2;
+
+  f32x4 s[KA][kNT];
+#pragma unroll
+  for (int a = 0; a < KA; ++a)
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) {
+      s[a][n] = zero4();
+      if (p.state_in != nullptr && col0 + 16 * n + l16 < p.dv) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = state_row(a, 4 * grp + r);
+          if (row < p.dk) s[a][n][r] = p.state_in[(w.unit * p.dk + row) * p.dv + col0 + 16 * n + l16];
+        }
+      }
+    }
+
+  SoloTokens<DK> c;
+  if (w.groups > 0) w.fetch(0, c);
+  for (int group = 0; group < w.groups; ++group) {
+    const int64_t token0 = static_cast<int64_t>(group) * kChunk;
+    const int n_tok = w.tokens_of(group);
+    wave_sync();  // the previous tokens' tiles are read
+    w.place(c, rows, tile_k, nullptr, tile_v);
+    if (TRAIN) w.store_state(p.chunk_states + (w.unit * p.chunks + group) * static_cast<int64_t>(p.dk) * p.dv, s);
+    bf16x8 mh[4], ml[4];
+    w.solve(c, rows, scratch, mh, ml);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half == 1 && n_tok <= kHalf) break;
+      bf16x8 sh[KB][kNT], sl[KB][kNT];
+      w.split_state(s, sh, sl);
+      // X = V - e^G K S
+      f32x4 x[2][kNT];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int ti = 2 * half + t;
+        f32x4 y[kNT];
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) y[n] = zero4();
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) y[n] = mfma16(c.kf[ti][kb], sl[kb][n], mfma16(c.kf[ti][kb], sh[kb][n], y[n]));
+        const f32x4 grown = *reinterpret_cast<const f32x4*>(rows + kSoloGrown + 16 * ti + 4 * grp);
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          const bf16x4 v = TV::values(tile_v, 16 * ti, n, l16, grp);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[t][n][r] = fmaf(-grown[r], y[n][r], static_cast<float>(v[r]));
+        }
+      }
+      // N = X - M X
+      bf16x8 xh[kNT], xl[kNT];
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) split(x[0][n], x[1][n], xh[n], xl[n]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+          x[t][n] = mfma16(ml[2 * half + t], xh[n], mfma16(mh[2 * half + t], xl[n], mfma16(mh[2 * half + t], xh[n], x[t][n])));
+      if (TRAIN) {
+        bf16_t* dst = p.misses + (w.unit * p.T + token0) * p.dv;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) {
+            if (col0 + 16 * n + l16 >= p.dv) continue;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int row = 32 * half + 16 * t + r;
+              if (row + 4 * grp < n_tok) put_offset(dst + row * p.dv + 16 * n, n_off, static_cast<bf16_t>(x[t][n][r]));
+            }
+          }
+      }
+      // the output by columns of tokens: lane = token, four value columns each
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) split(x[0][n], x[1][n], xh[n], xl[n]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int ti = 2 * half + t;
+        f32x4 score[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          score[u] = zero4();
+          if (u > t) continue;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) score[u] = mfma16(c.kf[2 * half + u][kb], c.qf[ti][kb], score[u]);
+          const f32x4 gam = w.decays_by_rows(rows, ti, 2 * half + u, false);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) score[u][r] *= p.scale * gam[r];
+        }
+        const bf16x8 pf = round8(score[0], score[1]);
+        f32x4 out[kNT];
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) out[n] = zero4();
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) out[n] = mfma16(sl[kb][n], c.qf[ti][kb], mfma16(sh[kb][n], c.qf[ti][kb], out[n]));
+        const float grown = rows[kSoloGrown + 16 * ti + l16] * p.scale;
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) out[n][r] *= grown;
+          out[n] = mfma16(xl[n], pf, mfma16(xh[n], pf, out[n]));
+          if (16 * ti + l16 < n_tok && col0 + 16 * n + 4 * grp < p.dv) {
+            bf16x4 o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = static_cast<bf16_t>(out[n][r]);
+            put_offset(o0 + (token0 + 16 * ti) * p.os[2] + 16 * n, o_off, o);
+          }
+        }
+      }
+      // S' = e^G_last S + K^T (beta e^(G_last - G) N)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const f32x4 keep = *reinterpret_cast<const f32x4*>(rows + kSoloKeep + 32 * half + 16 * t + 4 * grp);
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[t][n][r] *= keep[r];
+      }
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) split(x[0][n], x[1][n], xh[n], xl[n]);
+      const float total = rows[kSoloTotal + half];
+#pragma unroll
+      for (int a = 0; a < KA; ++a) {
+        const bf16x8 kt = TK::keys_frag(tile_k, half, a, l16, grp);
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[a][n][r] *= total;
+          s[a][n] = mfma16(kt, xl[n], mfma16(kt, xh[n], s[a][n]));
+        }
+      }
+    }
+    if (group + 1 < w.groups) w.fetch(group + 1, c);
+  }
+
+  if (p.state_out != nullptr) {
+#pragma unroll
+    for (int a = 0; a < KA; ++a)
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = state_row(a, 4 * grp + r);
+          if (row < p.dk && col0 + 16 * n + l16 < p.dv) p.state_out[(w.unit * p.dk + row) * p.dv + col0 + 16 * n + l16] = s[a][n][r];
+        }
+  }
+  const bf16x8 none = zero8();
+  for (int64_t i = lane; i < static_cast<int64_t>(p.T - w.len) * 4; i += kWave) {
+    const int at = static_cast<int>(i % 4) * 8;
+    if (col0 + at < p.dv) *reinterpret_cast<bf16x8*>(o0 + (w.len + i / 4) * p.os[2] + at) = none;
+  }
+}
+
+// The gradient of the state, tokens last to first (the formulas: delta_bwd.hip).
+template <int DK>
+__global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kernel(const DeltaParams p) {
+  typedef Solo<DK, true> W;
+  typedef SoloLds<DK, true> L;
+  typedef Tile<DK> TK;
+  typedef Tile<kSoloCols> TV;
+  constexpr int KB = W::KB, KA = W::KA;
+  __shared__ __attribute__((aligned(64))) uint8_t smem[L::kTotal];
+  __shared__ __attribute__((aligned(16))) float rows[kSoloFloats];
+  bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem);
+  bf16_t* tile_q = tile_k + kChunk * TK::STRIDE;
+  bf16_t* tile_o = reinterpret_cast<bf16_t*>(smem + L::kTileV);
+  float* scratch = reinterpret_cast<float*>(smem + L::kScratch);
+  const W w(p);
+  const int lane = w.lane, l16 = w.l16, grp = w.grp, col0 = w.col0;
+  bf16_t* v0 = p.grad_v + w.b * p.dvs[0] + w.h * p.dvs[1] + col0;
+  const uint32_t v_off = static_cast<uint32_t>(4 * grp * p.dvs[2] + l16) * 2;
+
+  f32x4 s[KA][kNT];
+#pragma unroll
+  for (int a = 0; a < KA; ++a)
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) s[a][n] = zero4();
+
+  SoloTokens<DK> c;
+  if (w.groups > 0) w.fetch(w.groups - 1, c);
+  for (int group = w.groups - 1; group >= 0; --group) {
+    const int64_t token0 = static_cast<int64_t>(group) * kChunk;
+    const int n_tok = w.tokens_of(group);
+    wave_sync();
+    w.place(c, rows, tile_k, tile_q, tile_o);
+    w.store_state(p.grad_states + (w.unit * p.chunks + group) * static_cast<int64_t>(p.dk) * p.dv, s);
+    bf16x8 mh[4], ml[4];
+    w.solve(c, rows, scratch, mh, ml);
+#pragma unroll
+    for (int back = 0; back < 2; ++back) {
+      const int half = 1 - back;
+      if (half == 1 && n_tok <= kHalf) continue;
+      bf16x8 sh[KB][kNT], sl[KB][kNT], of[kNT];
+      w.split_state(s, sh, sl);
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) of[n] = TV::values_frag(tile_o, half, n, l16, grp);
+      // beta dU
+      f32x4 z[2][kNT];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int tj = 2 * half + t;
+        f32x4 score[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          score[u] = zero4();
+          if (u < t) continue;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) score[u] = mfma16(c.qf[2 * half + u][kb], c.kf[tj][kb], score[u]);
+          const f32x4 gam = w.decays_by_cols(rows, 2 * half + u, tj);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) score[u][r] *= p.scale * gam[r];
+        }
+        const bf16x8 pf = round8(score[0], score[1]);
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) z[t][n] = zero4();
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) z[t][n] = mfma16(c.kf[tj][kb], sl[kb][n], mfma16(c.kf[tj][kb], sh[kb][n], z[t][n]));
+        const f32x4 keep = *reinterpret_cast<const f32x4*>(rows + kSoloKeep + 16 * tj + 4 * grp);
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) z[t][n][r] *= keep[r];
+          z[t][n] = mfma16(pf, of[n], z[t][n]);
+        }
+      }
+      // dX
+      bf16x8 zh[kNT], zl[kNT];
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) split(z[0][n], z[1][n], zh[n], zl[n]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+          z[t][n] = mfma16(ml[2 * half + t], zh[n], mfma16(mh[2 * half + t], zl[n], mfma16(mh[2 * half + t], zh[n], z[t][n])));
+      bf16_t* v = v0 + token0 * p.dvs[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          if (col0 + 16 * n + l16 >= p.dv) continue;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = 32 * half + 16 * t + r;
+            if (row + 4 * grp < n_tok) put_offset(v + row * p.dvs[2] + 16 * n, v_off, static_cast<bf16_t>(z[t][n][r]));
+          }
+        }
+      // dS
+      bf16x8 wh[kNT], wl[kNT];
+      const f32x4 g0 = *reinterpret_cast<const f32x4*>(rows + kSoloGrown + 32 * half + 4 * grp);
+      const f32x4 g1 = *reinterpret_cast<const f32x4*>(rows + kSoloGrown + 32 * half + 16 + 4 * grp);
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        f32x4 a0, a1;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          a0[r] = -g0[r] * z[0][n][r];
+          a1[r] = -g1[r] * z[1][n][r];
+        }
+        split(a0, a1, zh[n], zl[n]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          a0[r] = p.scale * g0[r] * static_cast<float>(of[n][r]);
+          a1[r] = p.scale * g1[r] * static_cast<float>(of[n][4 + r]);
+        }
+        split(a0, a1, wh[n], wl[n]);
+      }
+      const float total = rows[kSoloTotal + half];
+#pragma unroll
+      for (int a = 0; a < KA; ++a) {
+        const bf16x8 kt = TK::keys_frag(tile_k, half, a, l16, grp), qt = TK::keys_frag(tile_q, half, a, l16, grp);
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[a][n][r] *= total;
+          s[a][n] = mfma16(kt, zl[n], mfma16(kt, zh[n], s[a][n]));
+          s[a][n] = mfma16(qt, wl[n], mfma16(qt, wh[n], s[a][n]));
+        }
+      }
+    }
+    if (group > 0) w.fetch(group - 1, c);
+  }
+  const bf16x8 none = zero8();
+  for (int64_t i = lane; i < static_cast<int64_t>(p.T - w.len) * 4; i += kWave) {
+    const int at = static_cast<int>(i % 4) * 8;
+    if (col0 + at < p.dv) *reinterpret_cast<bf16x8*>(v0 + (w.len + i / 4) * p.dvs[2] + at) = none;
+  }
+}
+
+template <int DK>
+int launch_solo(const char* name, const DeltaParams& p, bool back, hipStream_t s) {
+  const int64_t waves = static_cast<int64_t>(p.B) * p.H * ((p.dv + kSoloCols - 1) / kSoloCols);
+  if (waves > 0x7fffffffLL) return set_error(TAAC_ERR_UNSUPPORTED, "%s: too many workgroups", name);
+  const dim3 grid(static_cast<uint32_t>(waves)), threads(kWave);
+  if (back) hipLaunchKernelGGL((delta_solo_back_kernel<DK>), grid, threads, 0, s, p);
+  else if (p.chunk_states != nullptr) hipLaunchKernelGGL((delta_solo_kernel<DK, true>), grid, threads, 0, s, p);
+  else hipLaunchKernelGGL((delta_solo_kernel<DK, false>), grid, threads, 0, s, p);
+  return check_launch(name);
+}
+
+}  // namespace
+
+int delta_solo(const char* name, const DeltaParams& p, bool back, hipStream_t s) {
+  return p.dk <= 32 ? launch_solo<32>(name, p, back, s) : launch_solo<64>(name, p, back, s);
+}
+
+}  // namespace taac

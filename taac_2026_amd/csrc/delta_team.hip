@@ -70,17 +70,6 @@ struct TeamChunk {
   bf16x8 x[2];  // forward: four values of this lane's column in x[0]; backward: dO of the column, fragments over the tokens
 };
 
-// Reads through a uniform base and a 32-bit offset of the lane, which stays the same for every chunk (token strides are below 2^24
-// elements).
-template <typename V, typename T>
-__device__ __forceinline__ V at_offset(const T* base, uint32_t bytes) {
-  return *reinterpret_cast<const V*>(reinterpret_cast<const uint8_t*>(base) + bytes);
-}
-template <typename T, typename V>
-__device__ __forceinline__ void put_offset(T* base, uint32_t bytes, const V& v) {
-  *reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(base) + bytes) = v;
-}
-
 template <int DK, bool COLS>
 struct Team {
   static constexpr int KB = DK / 32, KA = DK / 16, OWN = KA >= 4 ? KA / 4 : 1;  // OWN: state tiles of a wavefront
