@@ -613,7 +613,7 @@ int taac_row_rstd(const float* qk_sumsq, int64_t M, int32_t d_model, float eps, 
  * state alone and get zeros in o. Keys should have at most unit length and beta lie in [0, 1], as the recurrence needs to stay
  * bounded; log_decay is normally <= 0, values below -1e5 count as -1e5.
  * state_in: fp32 [B, H, dk, dv] or NULL (zeros); state_out: the same shape, or NULL; it may be state_in.
- * chunk_states (bf16 [B, H, ceil(T / 64), dk, dv]) and misses (bf16 [B, H, T, dv]): what taac_delta_rule_bwd reads, or both NULL.
+ * chunk_states (bf16 [B, H, ceil(T / 64), dv, dk]) and misses (bf16 [B, H, T, dv]): what taac_delta_rule_bwd reads, or both NULL.
  * taac_delta_rule_bwd: gradients of q, k, v, log_decay and beta (logical shapes and dtypes of the inputs, strides of their own) for
  * grad_o; grad_states (bf16, the size of chunk_states) is scratch. The initial state has no gradient here. Rows at or beyond a
  * sample's length get zeros. Every sum has a fixed order.

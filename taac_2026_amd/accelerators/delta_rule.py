@@ -84,7 +84,7 @@ def _forward(q, k, v, log_decay, beta, scale, lengths, initial_state, return_sta
     final = v.new_empty(batch, heads, key_width, value_width, dtype=torch.float32) if return_state else None
     states = misses = None
     if keep:
-        states = v.new_empty(batch, heads, (tokens + CHUNK - 1) // CHUNK, key_width, value_width)
+        states = v.new_empty(batch, heads, (tokens + CHUNK - 1) // CHUNK, value_width, key_width)
         misses = v.new_empty(batch, heads, tokens, value_width)
     library = _native.load_library()
     workspace = _workspace(k, v)

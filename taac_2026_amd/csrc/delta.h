@@ -36,7 +36,7 @@ struct DeltaParams {
   const int32_t* lengths;    // [B] or null: every sample has T tokens
   const float* state_in;     // [B, H, dk, dv] or null: zeros
   float* state_out;          // [B, H, dk, dv] or null
-  bf16_t* chunk_states;      // [B, H, chunks, dk, dv] or null: the state in front of every chunk
+  bf16_t* chunk_states;      // [B, H, chunks, dv, dk] or null: the state in front of every chunk, transposed
   bf16_t* misses;            // [B, H, T, dv] or null: N
   uint8_t* blocks;           // [B, H, chunks] blocks in memory (the form for few heads)
   // backward
@@ -46,7 +46,7 @@ struct DeltaParams {
   bf16_t* grad_v;            // also dX, which the last kernel reads
   void* grad_decay;
   void* grad_beta;
-  bf16_t* grad_states;       // [B, H, chunks, dk, dv]: the gradient of the state behind every chunk
+  bf16_t* grad_states;       // [B, H, chunks, dv, dk]: the gradient of the state behind every chunk, transposed
   int64_t dos[3], dqs[3], dks[3], dvs[3], dgs[3], dbs[3];
   // element strides of (batch, head, token)
   int64_t qs[3], ks[3], vs[3], os[3], gs[3], bs[3];
@@ -87,19 +87,25 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// Two values to bf16 in one instruction; and what that left of them.
+__device__ __forceinline__ uint32_t round2(float a, float b) {
+  typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
+  typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t rounded) {
+  return round2(a - __builtin_bit_cast(float, rounded << 16), b - __builtin_bit_cast(float, rounded & 0xffff0000u));
+}
+__device__ __forceinline__ u32x2 round4(const f32x4& v) { return u32x2{round2(v[0], v[1]), round2(v[2], v[3])}; }
+__device__ __forceinline__ u32x2 rest4(const f32x4& v, const u32x2& r) { return u32x2{rest2(v[0], v[1], r[0]), rest2(v[2], v[3], r[1])}; }
 __device__ __forceinline__ void split(const f32x4& a, const f32x4& b, bf16x8& hi, bf16x8& lo) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float f = e < 4 ? a[e] : b[e - 4];
-    hi[e] = static_cast<bf16_t>(f);
-    lo[e] = static_cast<bf16_t>(f - static_cast<float>(hi[e]));
-  }
+  const u32x2 ha = round4(a), hb = round4(b), la = rest4(a, ha), lb = rest4(b, hb);
+  hi = __builtin_bit_cast(bf16x8, (u32x4{ha[0], ha[1], hb[0], hb[1]}));
+  lo = __builtin_bit_cast(bf16x8, (u32x4{la[0], la[1], lb[0], lb[1]}));
 }
 __device__ __forceinline__ bf16x8 round8(const f32x4& a, const f32x4& b) {
-  bf16x8 r;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = static_cast<bf16_t>(e < 4 ? a[e] : b[e - 4]);
-  return r;
+  const u32x2 ha = round4(a), hb = round4(b);
+  return __builtin_bit_cast(bf16x8, (u32x4{ha[0], ha[1], hb[0], hb[1]}));
 }
 __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 __device__ __forceinline__ bf16x8 zero8() {
@@ -159,11 +165,16 @@ struct Tile {
         if (row < n && row < ROWS && piece * 8 < width) v[i] = *reinterpret_cast<const bf16x8*>(src + row * ld + piece * 8);
       }
     }
+    // PAIRED: row 8 g + e of a block of 32 goes to row 4 g + e (e < 4) or 12 + 4 g + e, so that a keys_frag() over the rows has them in order
+    template <bool PAIRED = false>
     __device__ __forceinline__ void store(bf16_t* dst, int tid) const {
 #pragma unroll
       for (int i = 0; i < COUNT; ++i) {
-        const int row = (tid + i * THREADS) / PIECES, piece = (tid + i * THREADS) % PIECES;
-        if (row < ROWS) *reinterpret_cast<bf16x8*>(dst + row * STRIDE + piece * 8) = v[i];
+        int row = (tid + i * THREADS) / PIECES;
+        const int piece = (tid + i * THREADS) % PIECES;
+        if (row >= ROWS) continue;
+        if (PAIRED) row = (row & ~31) + (row & 4) * 4 + ((row & 24) >> 1) + (row & 3);
+        *reinterpret_cast<bf16x8*>(dst + row * STRIDE + piece * 8) = v[i];
       }
     }
   };
@@ -199,6 +210,13 @@ struct Tile {
     return join(keys(tile, 32 * tk, a, l16, grp), keys(tile, 32 * tk + 16, a, l16, grp));
   }
 };
+
+// A result (lane: column l16, rows 4 grp ..) rounded and turned (lane: row l16, columns 4 grp ..) through 16 rows of 20 elements in LDS.
+__device__ __forceinline__ u32x2 turn16(bf16_t* at, const f32x4& v, int l16, int grp) {
+  *reinterpret_cast<u32x2*>(at + l16 * 20 + grp * 4) = round4(v);
+  wave_sync();
+  return __builtin_bit_cast(u32x2, Tile<32>::read_tr(at + (4 * grp + l16 / 4) * 20 + (l16 % 4) * 4));
+}
 
 // 16 x 16 fp32 products on v_mfma_f32_16x16x4_f32, contraction index 4 grp + step. A matrix Y is held "by rows" (lane: row l16, columns
 // 4 grp ..) or "by columns" (lane: column l16, rows 4 grp ..).
@@ -312,9 +330,9 @@ __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, 
   wave_sync();
 
   f32x4 a_rows[10];  // A by rows, tile (ti, tj) at ti (ti + 1) / 2 + tj
-  bf16x8 pf[6];
+  u32x2 pf[6][2];
 #pragma unroll
-  for (int i = 0; i < 6; ++i) pf[i] = zero8();
+  for (int i = 0; i < 6; ++i) pf[i][0] = pf[i][1] = u32x2{0u, 0u};
 #pragma unroll
   for (int ti = 0; ti < 4; ++ti) {
     const int row = 16 * ti + l16;
@@ -364,8 +382,7 @@ __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, 
       a_rows[ti * (ti + 1) / 2 + tj] = a;
       const int f = COLS ? frag_cols(tj, ti / 2) : frag_rows(ti, tj / 2);
       const int half = COLS ? ti % 2 : tj % 2;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) pf[f][4 * half + r] = static_cast<bf16_t>(s[r]);
+      pf[f][half] = round4(s);
     }
   }
 
@@ -414,7 +431,7 @@ __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, 
     split(a, c, hi8, lo8);
     *reinterpret_cast<bf16x8*>(block + kBlockM + f * kFrag + lane * 16) = hi8;
     *reinterpret_cast<bf16x8*>(block + kBlockLow + f * kFrag + lane * 16) = lo8;
-    *reinterpret_cast<bf16x8*>(block + kBlockP + f * kFrag + lane * 16) = pf[f];
+    *reinterpret_cast<u32x4*>(block + kBlockP + f * kFrag + lane * 16) = u32x4{pf[f][0][0], pf[f][0][1], pf[f][1][0], pf[f][1][1]};
   };
   if (!COLS) {
     const f32x4 m10r = mul_rows(t_rows[1], z10, zero4());

@@ -23,9 +23,9 @@ struct GradLds {
   static constexpr int kTileO = kTileQ + Tile<DK>::BYTES;
   static constexpr int kTileX = kTileO + Tile<DV>::BYTES;
   static constexpr int kTileN = kTileX + Tile<DV>::BYTES;
-  static constexpr int kState = kTileN + Tile<DV>::BYTES;  // DK rows of DV
-  static constexpr int kGradState = kState + DK * Tile<DV>::STRIDE * 2;
-  static constexpr int kRows = kGradState + DK * Tile<DV>::STRIDE * 2;
+  static constexpr int kState = kTileN + Tile<DV>::BYTES;  // DV rows of DK
+  static constexpr int kGradState = kState + DV * Tile<DK>::STRIDE * 2;
+  static constexpr int kRows = kGradState + DV * Tile<DK>::STRIDE * 2;
   static constexpr int kTotal = kRows + (kRowFloats + kTempFloats + 64 + 3 * 64 + 16) * 4;
 };
 
@@ -103,20 +103,20 @@ __global__ __launch_bounds__(4 * kWave, DK <= 64 && DV <= 64 ? 2 : 1) void delta
     const int row = 16 * wave + l16;  // this lane's token
     // everything this head reads is requested before any of it is waited for
     typename TV::template Piece<kChunk, kThreads> o_in, x_in, n_in;
-    typename TV::template Piece<DK, kThreads> s_in, g_in;
+    typename TK::template Piece<DV, kThreads> s_in, g_in;
     const int64_t at_state = (unit * p.chunks + chunk) * static_cast<int64_t>(p.dk) * p.dv;
     o_in.load(p.grad_o + b * p.dos[0] + h * p.dos[1] + token0 * p.dos[2], p.dos[2], n_tok, p.dv, tid);
     x_in.load(p.grad_v + b * p.dvs[0] + h * p.dvs[1] + token0 * p.dvs[2], p.dvs[2], n_tok, p.dv, tid);
     n_in.load(p.misses + (unit * p.T + token0) * p.dv, p.dv, n_tok, p.dv, tid);
-    s_in.load(p.chunk_states + at_state, p.dv, p.dk, p.dv, tid);
-    g_in.load(p.grad_states + at_state, p.dv, p.dk, p.dv, tid);
+    s_in.load(p.chunk_states + at_state, p.dk, p.dv, p.dk, tid);
+    g_in.load(p.grad_states + at_state, p.dk, p.dv, p.dk, tid);
     __syncthreads();  // the previous head's tiles and sums are no longer read
     if (wave == 0) chunk_rows(p, b, h, token0, n_tok, rows, temp, left_over);
     o_in.store(tile_o, tid);
     x_in.store(tile_x, tid);
     n_in.store(tile_n, tid);
-    s_in.store(tile_s, tid);
-    g_in.store(tile_g, tid);
+    s_in.template store<true>(tile_s, tid);
+    g_in.template store<true>(tile_g, tid);
     __syncthreads();
 
     const float hi_t = temp[kTempHi + row], lo_t = temp[kTempLow + row], beta_t = temp[kTempBeta + row], grown = rows[kRowGrown + row];
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 64 && DV <= 64 ? 2 : 1) void delta
       f32x4 dq = zero4(), dr = zero4();
 #pragma unroll
       for (int vb = 0; vb < VB; ++vb) {
-        const bf16x8 sf = TV::row(tile_s, state_row(a, l16), vb, grp);
+        const bf16x8 sf = TK::keys_frag(tile_s, vb, a, l16, grp);
         dq = mfma16(sf, first[vb], dq);
         dr = mfma16(sf, second[vb], dr);
       }
@@ -258,10 +258,10 @@ __global__ __launch_bounds__(4 * kWave, DK <= 64 && DV <= 64 ? 2 : 1) void delta
       f32x4 dc = zero4();
 #pragma unroll
       for (int vb = 0; vb < VB; ++vb) {
-        const bf16x8 gf = TV::row(tile_g, state_row(a, l16), vb, grp);
+        const bf16x8 gf = TK::keys_frag(tile_g, vb, a, l16, grp);
         dc = mfma16(gf, first[vb], dc);
         if (a % 4 == wave) {
-          const bf16x8 sf = TV::row(tile_s, state_row(a, l16), vb, grp);
+          const bf16x8 sf = TK::keys_frag(tile_s, vb, a, l16, grp);
 #pragma unroll
           for (int e = 0; e < 8; ++e) dot_state = fmaf(static_cast<float>(sf[e]), static_cast<float>(gf[e]), dot_state);
         }
@@ -319,14 +319,8 @@ __global__ __launch_bounds__(4 * kWave, DK <= 64 && DV <= 64 ? 2 : 1) void delta
     for (int a = 0; a < KA; ++a) {
       const int at = state_row(a, 4 * grp);
       if (at >= p.dk) continue;
-      bf16x4 dq, dk;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        dq[r] = static_cast<bf16_t>(dq_sum[a][r]);
-        dk[r] = static_cast<bf16_t>(dk_sum[a][r]);
-      }
-      *reinterpret_cast<bf16x4*>(dq_row + at) = dq;
-      *reinterpret_cast<bf16x4*>(dk_row + at) = dk;
+      *reinterpret_cast<u32x2*>(dq_row + at) = round4(dq_sum[a]);
+      *reinterpret_cast<u32x2*>(dk_row + at) = round4(dk_sum[a]);
     }
   }
 }

@@ -88,23 +88,19 @@ __global__ __launch_bounds__(NW * kWave) void delta_scan_kernel(const DeltaParam
       const uint8_t* block = smem + c * kBlockBytes;
       const float* rows = reinterpret_cast<const float*>(block + kBlockRows);
 
-      if (TRAIN) {
-        bf16_t* dst = p.chunk_states + (unit * p.chunks + base + c) * static_cast<int64_t>(p.dk) * p.dv;
-#pragma unroll
-        for (int a = 0; a < KA; ++a)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int row = state_row(a, 4 * grp + r);
-              if (col_ok[n] && row < p.dk) dst[row * p.dv + col[n] + l16] = static_cast<bf16_t>(s[a][n][r]);
-            }
-      }
       bf16x8 sh[KB][NT], sl[KB][NT];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int n = 0; n < NT; ++n) split(s[2 * kb][n], s[2 * kb + 1][n], sh[kb][n], sl[kb][n]);
+      if (TRAIN) {
+        bf16_t* dst = p.chunk_states + (unit * p.chunks + base + c) * static_cast<int64_t>(p.dk) * p.dv;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            if (col_ok[n] && 32 * kb + 8 * grp < p.dk) *reinterpret_cast<bf16x8*>(dst + (col[n] + l16) * p.dk + 32 * kb + 8 * grp) = sh[kb][n];
+      }
 
       // X = V - e^G K S
       f32x4 x[4][NT];
@@ -188,10 +184,7 @@ __global__ __launch_bounds__(NW * kWave) void delta_scan_kernel(const DeltaParam
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             if (col[n] + 4 * grp >= p.dv) continue;
-            bf16x4 v;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = static_cast<bf16_t>(out[n][r]);
-            *reinterpret_cast<bf16x4*>(ob0 + (token0 + row) * p.os[2] + col[n] + 4 * grp) = v;
+            *reinterpret_cast<u32x2*>(ob0 + (token0 + row) * p.os[2] + col[n] + 4 * grp) = round4(out[n]);
           }
         }
       }

@@ -12,13 +12,13 @@ namespace {
 
 constexpr int kHalf = 32, kSoloCols = 32, kNT = 2;
 
-template <int DK, bool BACK>
+template <int DK>
 struct SoloLds {
   typedef Tile<DK> TK;
   typedef Tile<kSoloCols> TV;
-  static constexpr int kTileV = TK::BYTES * (BACK ? 2 : 1);
-  static constexpr int kScratch = kTileV + TV::BYTES;
-  static constexpr int kTotal = kScratch + kScratchFloats * 4;
+  static constexpr int kTileV = TK::BYTES;
+  static constexpr int kTileQ = kTileV + TV::BYTES;  // its first bytes are the scratch of the solution, in front of Q
+  static constexpr int kTotal = kTileQ + (TK::BYTES > kScratchFloats * 4 ? TK::BYTES : kScratchFloats * 4);
 };
 
 // Floats of the 64 tokens in LDS: G as a pair, beta; e^(G - G in front of the tile of 16), e^(G behind the tile - G) beta; and over the chunk of 32:
@@ -111,14 +111,13 @@ struct Solo {
   }
 
   // The tokens' factors and rows into LDS.
-  __device__ __forceinline__ void place(const SoloTokens<DK>& c, float* rows, bf16_t* tile_k, bf16_t* tile_q, bf16_t* tile_x) const {
+  __device__ __forceinline__ void place(const SoloTokens<DK>& c, float* rows, bf16_t* tile_k, bf16_t* tile_x) const {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         const int at = (16 * t + l16) * TK::STRIDE + kb * 32 + grp * 8;
         *reinterpret_cast<bf16x8*>(tile_k + at) = c.kf[t][kb];
-        if (BACK) *reinterpret_cast<bf16x8*>(tile_q + at) = c.qf[t][kb];
       }
       *reinterpret_cast<bf16x8*>(tile_x + (16 * t + lane / 4) * TV::STRIDE + (lane % 4) * 8) = c.x[t];
     }
@@ -143,6 +142,14 @@ struct Solo {
     rows[kSoloGrown + lane] = grown;
     rows[kSoloKeep + lane] = __builtin_amdgcn_exp2f(static_cast<float>(half_end - total)) * c.beta;
     if ((lane & 31) == 31) rows[kSoloTotal + lane / 32] = grown;
+    wave_sync();
+  }
+  // Q's rows, in the place of the solution's scratch; c holds nothing of these tokens any more.
+  __device__ __forceinline__ void place_queries(const SoloTokens<DK>& c, bf16_t* tile_q) const {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) *reinterpret_cast<bf16x8*>(tile_q + (16 * t + l16) * TK::STRIDE + kb * 32 + grp * 8) = c.qf[t][kb];
     wave_sync();
   }
 
@@ -254,26 +261,43 @@ struct Solo {
 #pragma unroll
       for (int n = 0; n < kNT; ++n) split(s[2 * kb][n], s[2 * kb + 1][n], sh[kb][n], sl[kb][n]);
   }
-  // 16-bit copies of the state at dst [dk][dv]
-  __device__ __forceinline__ void store_state(bf16_t* dst, const f32x4 (&s)[KA][kNT]) const {
-    const uint32_t off = static_cast<uint32_t>(8 * grp * p.dv + col0 + l16) * 2;
+  // the state's high parts at dst [dv][dk]
+  __device__ __forceinline__ void store_state(bf16_t* dst, const bf16x8 (&sh)[KB][kNT]) const {
+    const uint32_t off = static_cast<uint32_t>((col0 + l16) * p.dk + 8 * grp) * 2;
 #pragma unroll
-    for (int a = 0; a < KA; ++a)
+    for (int n = 0; n < kNT; ++n)
+      if (col0 + 16 * n + l16 < p.dv) {
 #pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        if (col0 + 16 * n + l16 >= p.dv) continue;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (p.dk == DK || state_row(a, 4 * grp + r) < p.dk)
-            put_offset(dst + (32 * (a / 2) + 4 * (a % 2) + r) * p.dv + 16 * n, off, static_cast<bf16_t>(s[a][n][r]));
+        for (int kb = 0; kb < KB; ++kb)
+          if (p.dk == DK || 32 * kb + 8 * grp < p.dk) put_offset(dst + 16 * n * p.dk + 32 * kb, off, sh[kb][n]);
       }
+  }
+  // Rows of one chunk of 32 tokens, held by columns, at dst (its row 0, this wavefront's first column): turned through tile's rows, which
+  // have been read.
+  __device__ __forceinline__ void store_rows(bf16_t* dst, int64_t ld, uint32_t off, bf16_t* tile, const f32x4 (&x)[2][kNT], int n_tok) const {
+    u32x2 v[2][kNT];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) *reinterpret_cast<u32x2*>(tile + (2 * t + n) * 320 + l16 * 20 + grp * 4) = round4(x[t][n]);
+    wave_sync();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+        v[t][n] = __builtin_bit_cast(u32x2, TV::read_tr(tile + (2 * t + n) * 320 + (4 * grp + l16 / 4) * 20 + (l16 % 4) * 4));
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+        if (16 * t + l16 < n_tok && col0 + 16 * n + 4 * grp < p.dv) put_offset(dst + 16 * t * ld + 16 * n, off, v[t][n]);
   }
 };
 
 template <int DK, bool TRAIN>
 __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(const DeltaParams p) {
   typedef Solo<DK, false> W;
-  typedef SoloLds<DK, false> L;
+  typedef SoloLds<DK> L;
   typedef Tile<DK> TK;
   typedef Tile<kSoloCols> TV;
   constexpr int KB = W::KB, KA = W::KA;
@@ -281,12 +305,13 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
   __shared__ __attribute__((aligned(16))) float rows[kSoloFloats];
   bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem);
   bf16_t* tile_v = reinterpret_cast<bf16_t*>(smem + L::kTileV);
-  float* scratch = reinterpret_cast<float*>(smem + L::kScratch);
+  bf16_t* tile_q = reinterpret_cast<bf16_t*>(smem + L::kTileQ);
+  float* scratch = reinterpret_cast<float*>(smem + L::kTileQ);
   const W w(p);
   const int lane = w.lane, l16 = w.l16, grp = w.grp, col0 = w.col0;
   bf16_t* o0 = p.o + w.b * p.os[0] + w.h * p.os[1] + col0;
   const uint32_t o_off = static_cast<uint32_t>(l16 * p.os[2] + 4 * grp) * 2;
-  const uint32_t n_off = static_cast<uint32_t>(4 * grp * p.dv + col0 + l16) * 2;
+  const uint32_t n_off = static_cast<uint32_t>(l16 * p.dv + 4 * grp) * 2;
 
   f32x4 s[KA][kNT];
 #pragma unroll
@@ -309,15 +334,17 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
     const int64_t token0 = static_cast<int64_t>(group) * kChunk;
     const int n_tok = w.tokens_of(group);
     wave_sync();  // the previous tokens' tiles are read
-    w.place(c, rows, tile_k, nullptr, tile_v);
-    if (TRAIN) w.store_state(p.chunk_states + (w.unit * p.chunks + group) * static_cast<int64_t>(p.dk) * p.dv, s);
+    w.place(c, rows, tile_k, tile_v);
     bf16x8 mh[4], ml[4];
     w.solve(c, rows, scratch, mh, ml);
+    w.place_queries(c, tile_q);
+    if (group + 1 < w.groups) w.fetch(group + 1, c);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (half == 1 && n_tok <= kHalf) break;
       bf16x8 sh[KB][kNT], sl[KB][kNT];
       w.split_state(s, sh, sl);
+      if (TRAIN && half == 0) w.store_state(p.chunk_states + (w.unit * p.chunks + group) * static_cast<int64_t>(p.dk) * p.dv, sh);
       // X = V - e^G K S
       f32x4 x[2][kNT];
 #pragma unroll
@@ -327,9 +354,11 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
 #pragma unroll
         for (int n = 0; n < kNT; ++n) y[n] = zero4();
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+        for (int kb = 0; kb < KB; ++kb) {
+          const bf16x8 kf = TK::row(tile_k, 16 * ti + l16, kb, grp);
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) y[n] = mfma16(c.kf[ti][kb], sl[kb][n], mfma16(c.kf[ti][kb], sh[kb][n], y[n]));
+          for (int n = 0; n < kNT; ++n) y[n] = mfma16(kf, sl[kb][n], mfma16(kf, sh[kb][n], y[n]));
+        }
         const f32x4 grown = *reinterpret_cast<const f32x4*>(rows + kSoloGrown + 16 * ti + 4 * grp);
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
@@ -347,33 +376,24 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
 #pragma unroll
         for (int n = 0; n < kNT; ++n)
           x[t][n] = mfma16(ml[2 * half + t], xh[n], mfma16(mh[2 * half + t], xl[n], mfma16(mh[2 * half + t], xh[n], x[t][n])));
-      if (TRAIN) {
-        bf16_t* dst = p.misses + (w.unit * p.T + token0) * p.dv;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int n = 0; n < kNT; ++n) {
-            if (col0 + 16 * n + l16 >= p.dv) continue;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int row = 32 * half + 16 * t + r;
-              if (row + 4 * grp < n_tok) put_offset(dst + row * p.dv + 16 * n, n_off, static_cast<bf16_t>(x[t][n][r]));
-            }
-          }
-      }
+      if (TRAIN)
+        w.store_rows(p.misses + (w.unit * p.T + token0 + 32 * half) * p.dv + col0, p.dv, n_off, tile_v + 32 * half * TV::STRIDE, x, n_tok - 32 * half);
       // the output by columns of tokens: lane = token, four value columns each
 #pragma unroll
       for (int n = 0; n < kNT; ++n) split(x[0][n], x[1][n], xh[n], xl[n]);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int ti = 2 * half + t;
+        bf16x8 qf[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) qf[kb] = TK::row(tile_q, 16 * ti + l16, kb, grp);
         f32x4 score[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           score[u] = zero4();
           if (u > t) continue;
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) score[u] = mfma16(c.kf[2 * half + u][kb], c.qf[ti][kb], score[u]);
+          for (int kb = 0; kb < KB; ++kb) score[u] = mfma16(TK::row(tile_k, 16 * (2 * half + u) + l16, kb, grp), qf[kb], score[u]);
           const f32x4 gam = w.decays_by_rows(rows, ti, 2 * half + u, false);
 #pragma unroll
           for (int r = 0; r < 4; ++r) score[u][r] *= p.scale * gam[r];
@@ -385,7 +405,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) out[n] = mfma16(sl[kb][n], c.qf[ti][kb], mfma16(sh[kb][n], c.qf[ti][kb], out[n]));
+          for (int n = 0; n < kNT; ++n) out[n] = mfma16(sl[kb][n], qf[kb], mfma16(sh[kb][n], qf[kb], out[n]));
         const float grown = rows[kSoloGrown + 16 * ti + l16] * p.scale;
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
@@ -393,10 +413,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
           for (int r = 0; r < 4; ++r) out[n][r] *= grown;
           out[n] = mfma16(xl[n], pf, mfma16(xh[n], pf, out[n]));
           if (16 * ti + l16 < n_tok && col0 + 16 * n + 4 * grp < p.dv) {
-            bf16x4 o;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = static_cast<bf16_t>(out[n][r]);
-            put_offset(o0 + (token0 + 16 * ti) * p.os[2] + 16 * n, o_off, o);
+            put_offset(o0 + (token0 + 16 * ti) * p.os[2] + 16 * n, o_off, round4(out[n]));
           }
         }
       }
@@ -423,7 +440,6 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
         }
       }
     }
-    if (group + 1 < w.groups) w.fetch(group + 1, c);
   }
 
   if (p.state_out != nullptr) {
@@ -448,20 +464,20 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
 template <int DK>
 __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kernel(const DeltaParams p) {
   typedef Solo<DK, true> W;
-  typedef SoloLds<DK, true> L;
+  typedef SoloLds<DK> L;
   typedef Tile<DK> TK;
   typedef Tile<kSoloCols> TV;
   constexpr int KB = W::KB, KA = W::KA;
   __shared__ __attribute__((aligned(64))) uint8_t smem[L::kTotal];
   __shared__ __attribute__((aligned(16))) float rows[kSoloFloats];
   bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem);
-  bf16_t* tile_q = tile_k + kChunk * TK::STRIDE;
+  bf16_t* tile_q = reinterpret_cast<bf16_t*>(smem + L::kTileQ);
   bf16_t* tile_o = reinterpret_cast<bf16_t*>(smem + L::kTileV);
-  float* scratch = reinterpret_cast<float*>(smem + L::kScratch);
+  float* scratch = reinterpret_cast<float*>(smem + L::kTileQ);
   const W w(p);
   const int lane = w.lane, l16 = w.l16, grp = w.grp, col0 = w.col0;
   bf16_t* v0 = p.grad_v + w.b * p.dvs[0] + w.h * p.dvs[1] + col0;
-  const uint32_t v_off = static_cast<uint32_t>(4 * grp * p.dvs[2] + l16) * 2;
+  const uint32_t v_off = static_cast<uint32_t>(l16 * p.dvs[2] + 4 * grp) * 2;
 
   f32x4 s[KA][kNT];
 #pragma unroll
@@ -475,16 +491,18 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
     const int64_t token0 = static_cast<int64_t>(group) * kChunk;
     const int n_tok = w.tokens_of(group);
     wave_sync();
-    w.place(c, rows, tile_k, tile_q, tile_o);
-    w.store_state(p.grad_states + (w.unit * p.chunks + group) * static_cast<int64_t>(p.dk) * p.dv, s);
+    w.place(c, rows, tile_k, tile_o);
     bf16x8 mh[4], ml[4];
     w.solve(c, rows, scratch, mh, ml);
+    w.place_queries(c, tile_q);
+    if (group > 0) w.fetch(group - 1, c);
 #pragma unroll
     for (int back = 0; back < 2; ++back) {
       const int half = 1 - back;
       if (half == 1 && n_tok <= kHalf) continue;
       bf16x8 sh[KB][kNT], sl[KB][kNT], of[kNT];
       w.split_state(s, sh, sl);
+      if (half == 1 || n_tok <= kHalf) w.store_state(p.grad_states + (w.unit * p.chunks + group) * static_cast<int64_t>(p.dk) * p.dv, sh);
 #pragma unroll
       for (int n = 0; n < kNT; ++n) of[n] = TV::values_frag(tile_o, half, n, l16, grp);
       // beta dU
@@ -492,13 +510,16 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int tj = 2 * half + t;
+        bf16x8 kf[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) kf[kb] = TK::row(tile_k, 16 * tj + l16, kb, grp);
         f32x4 score[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           score[u] = zero4();
           if (u < t) continue;
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) score[u] = mfma16(c.qf[2 * half + u][kb], c.kf[tj][kb], score[u]);
+          for (int kb = 0; kb < KB; ++kb) score[u] = mfma16(TK::row(tile_q, 16 * (2 * half + u) + l16, kb, grp), kf[kb], score[u]);
           const f32x4 gam = w.decays_by_cols(rows, 2 * half + u, tj);
 #pragma unroll
           for (int r = 0; r < 4; ++r) score[u][r] *= p.scale * gam[r];
@@ -509,7 +530,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) z[t][n] = mfma16(c.kf[tj][kb], sl[kb][n], mfma16(c.kf[tj][kb], sh[kb][n], z[t][n]));
+          for (int n = 0; n < kNT; ++n) z[t][n] = mfma16(kf[kb], sl[kb][n], mfma16(kf[kb], sh[kb][n], z[t][n]));
         const f32x4 keep = *reinterpret_cast<const f32x4*>(rows + kSoloKeep + 16 * tj + 4 * grp);
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
@@ -527,18 +548,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
 #pragma unroll
         for (int n = 0; n < kNT; ++n)
           z[t][n] = mfma16(ml[2 * half + t], zh[n], mfma16(mh[2 * half + t], zl[n], mfma16(mh[2 * half + t], zh[n], z[t][n])));
-      bf16_t* v = v0 + token0 * p.dvs[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-          if (col0 + 16 * n + l16 >= p.dv) continue;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int row = 32 * half + 16 * t + r;
-            if (row + 4 * grp < n_tok) put_offset(v + row * p.dvs[2] + 16 * n, v_off, static_cast<bf16_t>(z[t][n][r]));
-          }
-        }
+      w.store_rows(v0 + (token0 + 32 * half) * p.dvs[2], p.dvs[2], v_off, tile_o + 32 * half * TV::STRIDE, z, n_tok - 32 * half);
       // dS
       bf16x8 wh[kNT], wl[kNT];
       const f32x4 g0 = *reinterpret_cast<const f32x4*>(rows + kSoloGrown + 32 * half + 4 * grp);
@@ -572,7 +582,6 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
         }
       }
     }
-    if (group > 0) w.fetch(group - 1, c);
   }
   const bf16x8 none = zero8();
   for (int64_t i = lane; i < static_cast<int64_t>(p.T - w.len) * 4; i += kWave) {

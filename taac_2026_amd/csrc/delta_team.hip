@@ -33,15 +33,10 @@ __global__ __launch_bounds__(kWave) void delta_blocks_kernel(const DeltaParams p
 
 // Half fragments: the four values of one 16-row result, as the first or second half of a fragment of 32 rows in LDS.
 __device__ __forceinline__ void put_half(uint8_t* frags, int tile, int lane, const f32x4& v, int low_at) {
-  bf16x4 hi, lo;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    hi[r] = static_cast<bf16_t>(v[r]);
-    lo[r] = static_cast<bf16_t>(v[r] - static_cast<float>(hi[r]));
-  }
+  const u32x2 hi = round4(v);
   uint8_t* at = frags + (tile / 2) * kFrag + lane * 16 + (tile % 2) * 8;
-  *reinterpret_cast<bf16x4*>(at) = hi;
-  *reinterpret_cast<bf16x4*>(at + low_at) = lo;
+  *reinterpret_cast<u32x2*>(at) = hi;
+  *reinterpret_cast<u32x2*>(at + low_at) = rest4(v, hi);
 }
 __device__ __forceinline__ bf16x8 get_frag(const uint8_t* frags, int f, int lane) {
   return *reinterpret_cast<const bf16x8*>(frags + f * kFrag + lane * 16);
@@ -176,17 +171,14 @@ struct Team {
     c.total = *reinterpret_cast<const float*>(rows + kRowTotal * 4);
   }
 
-  // The own rows of the state: register r of tile a, bf16, at dst [dk][dv]
+  // The own rows of the state, bf16, at dst [dv][dk]
   __device__ __forceinline__ void store_state(bf16_t* dst, const f32x4 (&s)[OWN]) const {
     if (!owner || !col_ok) return;
-    const uint32_t off = static_cast<uint32_t>(state_row(0, 4 * grp) * p.dv + col0 + l16) * 2;
+    const uint32_t off = static_cast<uint32_t>((col0 + l16) * p.dk + 8 * grp) * 2;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
       const int a = wave * OWN + i;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (p.dk == DK || state_row(a, 4 * grp + r) < p.dk)
-          put_offset(dst + (32 * (a / 2) + 4 * (a % 2) + r) * p.dv, off, static_cast<bf16_t>(s[i][r]));
+      if (p.dk == DK || state_row(a, 4 * grp) < p.dk) put_offset(dst + 32 * (a / 2) + 4 * (a % 2), off, round4(s[i]));
     }
   }
 };
@@ -198,14 +190,16 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
   typedef Tile<DK> TK;
   constexpr int KB = M::KB, OWN = M::OWN;
   __shared__ __attribute__((aligned(64))) uint8_t smem[L::kForward];
+  __shared__ __attribute__((aligned(16))) bf16_t turned[TRAIN ? 4 : 1][320];
   bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK);
   uint8_t *s_frags = smem + L::kState, *x_frags = smem + L::kX, *n_frags = smem + L::kN, *w_frags = smem + L::kW;
   const M m(p);
   const int wave = m.wave, lane = m.lane, l16 = m.l16, grp = m.grp, col0 = m.col0;
   bf16_t* o0 = p.o + m.b * p.os[0] + m.h * p.os[1] + col0;
   const uint32_t o_off = static_cast<uint32_t>((16 * wave + l16) * p.os[2] + 4 * grp) * 2;
-  const uint32_t n_off = static_cast<uint32_t>((16 * wave + 4 * grp) * p.dv + col0 + l16) * 2;
+  const uint32_t n_off = static_cast<uint32_t>((16 * wave + l16) * p.dv + col0 + 4 * grp) * 2;
   const bool quad_ok = col0 + 4 * grp < p.dv;
+  bf16_t* turn = turned[TRAIN ? wave : 0];
 
   f32x4 s[OWN];
 #pragma unroll
@@ -270,11 +264,9 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
     }
     put_half(w_frags, wave, lane, w, 2 * kFrag);
     put_half(n_frags, wave, lane, x, 2 * kFrag);
-    if (TRAIN && m.col_ok) {
-      bf16_t* dst = p.misses + (m.unit * p.T + token0) * p.dv;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (16 * wave + 4 * grp + r < n_tok) put_offset(dst + r * p.dv, n_off, static_cast<bf16_t>(x[r]));
+    if (TRAIN) {
+      const u32x2 rounded = turn16(turn, x, l16, grp);
+      if (16 * wave + l16 < n_tok && quad_ok) put_offset(p.misses + (m.unit * p.T + token0) * p.dv, n_off, rounded);
     }
     const float grown = cur.grown_row * p.scale;
 #pragma unroll
@@ -309,10 +301,9 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
         out2 = mfma16(get_frag(n_frags + 2 * kFrag, tk, lane), cur.pf[tk], out2);
       }
     if (16 * wave + l16 < n_tok && quad_ok) {
-      bf16x4 o;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = static_cast<bf16_t>(out[r] + out2[r]);
-      put_offset(o0 + token0 * p.os[2], o_off, o);
+      for (int r = 0; r < 4; ++r) out[r] += out2[r];
+      put_offset(o0 + token0 * p.os[2], o_off, round4(out));
     }
     __syncthreads();
   };
@@ -349,13 +340,15 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
   typedef Tile<DK> TK;
   constexpr int KB = M::KB, OWN = M::OWN;
   __shared__ __attribute__((aligned(64))) uint8_t smem[L::kBackward];
+  __shared__ __attribute__((aligned(16))) bf16_t turned[4][320];
   bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK);
   bf16_t* tile_q = reinterpret_cast<bf16_t*>(smem + L::kTileQ);
   uint8_t *s_frags = smem + L::kState, *z_frags = smem + L::kX, *x_frags = smem + L::kN, *o_frags = smem + L::kW;
   const M m(p);
   const int wave = m.wave, lane = m.lane, l16 = m.l16, grp = m.grp, col0 = m.col0;
   bf16_t* v0 = p.grad_v + m.b * p.dvs[0] + m.h * p.dvs[1] + col0;
-  const uint32_t v_off = static_cast<uint32_t>((16 * wave + 4 * grp) * p.dvs[2] + l16) * 2;
+  const uint32_t v_off = static_cast<uint32_t>((16 * wave + l16) * p.dvs[2] + 4 * grp) * 2;
+  const bool quad_ok = col0 + 4 * grp < p.dv;
 
   f32x4 s[OWN];
 #pragma unroll
@@ -406,14 +399,14 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
         z2 = mfma16(cur.mh[tk], zl, z2);
         z3 = mfma16(cur.ml[tk], zh, z3);
       }
-    bf16_t* v = v0 + token0 * p.dvs[2];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       z[r] += z2[r] + z3[r];
-      if (m.col_ok && 16 * wave + 4 * grp + r < n_tok) put_offset(v + r * p.dvs[2], v_off, static_cast<bf16_t>(z[r]));
       w[r] = -cur.grown[r] * z[r];
     }
     put_half(x_frags, wave, lane, w, 2 * kFrag);
+    const u32x2 rounded = turn16(turned[wave], z, l16, grp);
+    if (16 * wave + l16 < n_tok && quad_ok) put_offset(v0 + token0 * p.dvs[2], v_off, rounded);
     __syncthreads();
 
     // dS of the own rows
