@@ -76,7 +76,8 @@ constexpr int kRowGrown = 0, kRowKeep = 64, kRowTotal = 128, kRowFloats = 144;
 constexpr int kBlockBytes = kBlockRows + kRowFloats * 4;
 // floats that only the maker of a block needs: G as a pair, beta; e^(G - G in front of the tile of 16), e^(G behind the tile - G), that times beta
 constexpr int kTempHi = 0, kTempLow = 64, kTempBeta = 128, kTempIn = 192, kTempOut = 256, kTempOutBeta = 320, kTempFloats = 384;
-constexpr int kScratchFloats = 4 * 16 * 20;  // diagonal blocks, rows of 20 floats
+// Scratch for the diagonal blocks: rows of 20 floats, blocks 16 banks apart.
+constexpr int kScratchRow = 20, kScratchBlock = 16 * kScratchRow + 16, kScratchFloats = 4 * kScratchBlock;
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -234,15 +235,15 @@ __device__ __forceinline__ f32x4 mul_rows(const f32x4& x_rows, const f32x4& y_co
 // M of the four diagonal blocks of 16 in scratch, in the place of A, all four at once: M_ic = A_ic - sum over c < j < i of A_ij M_jc, a column
 // c per lane. Every lane of the wavefront has written its part of A before a wave_sync().
 __device__ __forceinline__ void solve_diagonal(float* scratch, int lane) {
-  float* mine = scratch + lane / 16 * 16 * 20;
+  float* mine = scratch + lane / 16 * kScratchBlock;
   const int l16 = lane % 16;
   float m[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    float acc = mine[i * 20 + l16];
+    float acc = mine[i * kScratchRow + l16];
 #pragma unroll
     for (int j4 = 0; j4 * 4 < i; ++j4) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(mine + i * 20 + 4 * j4);
+      const f32x4 a = *reinterpret_cast<const f32x4*>(mine + i * kScratchRow + 4 * j4);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (4 * j4 + e < i) acc = fmaf(-a[e], m[4 * j4 + e], acc);
@@ -251,7 +252,7 @@ __device__ __forceinline__ void solve_diagonal(float* scratch, int lane) {
   }
   wave_sync();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) mine[i * 20 + l16] = m[i];
+  for (int i = 0; i < 16; ++i) mine[i * kScratchRow + l16] = m[i];
   wave_sync();
 }
 
@@ -388,16 +389,16 @@ __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, 
 
   // diagonal blocks
 #pragma unroll
-  for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(scratch + (t * 16 + l16) * 20 + 4 * grp) = a_rows[t * (t + 1) / 2 + t];
+  for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(scratch + t * kScratchBlock + l16 * kScratchRow + 4 * grp) = a_rows[t * (t + 1) / 2 + t];
   wave_sync();
   solve_diagonal(scratch, lane);
   f32x4 m_rows[4], m_cols[4], t_rows[4], t_cols[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    m_rows[t] = *reinterpret_cast<const f32x4*>(scratch + (t * 16 + l16) * 20 + 4 * grp);
+    m_rows[t] = *reinterpret_cast<const f32x4*>(scratch + t * kScratchBlock + l16 * kScratchRow + 4 * grp);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      m_cols[t][r] = scratch[(t * 16 + 4 * grp + r) * 20 + l16];
+      m_cols[t][r] = scratch[t * kScratchBlock + (4 * grp + r) * kScratchRow + l16];
       const float one = l16 == 4 * grp + r ? 1.f : 0.f;
       t_rows[t][r] = one - m_rows[t][r];
       t_cols[t][r] = one - m_cols[t][r];

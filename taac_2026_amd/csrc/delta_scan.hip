@@ -29,8 +29,9 @@ __global__ __launch_bounds__(NW * kWave) void delta_scan_kernel(const DeltaParam
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, l16 = lane % 16, grp = lane / 16;
   const int col_groups = (p.dv + L::COLS - 1) / L::COLS;
-  const int64_t unit = blockIdx.x / col_groups;
-  const int col0 = static_cast<int>(blockIdx.x % col_groups) * L::COLS;  // of the workgroup
+  const uint32_t block_id = xcd_remap(blockIdx.x, gridDim.x);  // the columns of a head, which read the same rows, on one die's L2
+  const int64_t unit = block_id / col_groups;
+  const int col0 = static_cast<int>(block_id % col_groups) * L::COLS;  // of the workgroup
   const int h = static_cast<int>(unit % p.H);
   const int b = static_cast<int>(unit / p.H);
   int len = p.T;

@@ -47,8 +47,9 @@ struct Solo {
   __device__ __forceinline__ Solo(const DeltaParams& params) : p(params) {
     lane = threadIdx.x, l16 = lane % 16, grp = lane / 16;
     const int col_groups = (p.dv + kSoloCols - 1) / kSoloCols;
-    unit = blockIdx.x / col_groups;
-    col0 = static_cast<int>(blockIdx.x % col_groups) * kSoloCols;
+    const uint32_t block = xcd_remap(blockIdx.x, gridDim.x);  // the columns of a head, which read the same rows, on one die's L2
+    unit = block / col_groups;
+    col0 = static_cast<int>(block % col_groups) * kSoloCols;
     h = static_cast<int>(unit % p.H);
     b = static_cast<int>(unit / p.H);
     len = p.T;
@@ -207,7 +208,7 @@ struct Solo {
       const f32x4 gam = decays_by_rows(rows, t, t, true);
 #pragma unroll
       for (int r = 0; r < 4; ++r) kk[r] *= gam[r];
-      *reinterpret_cast<f32x4*>(scratch + (t * 16 + l16) * 20 + 4 * grp) = kk;
+      *reinterpret_cast<f32x4*>(scratch + t * kScratchBlock + l16 * kScratchRow + 4 * grp) = kk;
     }
     wave_sync();
 #pragma unroll
@@ -223,9 +224,9 @@ struct Solo {
     f32x4 m_rows[4], m_cols[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      m_rows[t] = *reinterpret_cast<const f32x4*>(scratch + (t * 16 + l16) * 20 + 4 * grp);
+      m_rows[t] = *reinterpret_cast<const f32x4*>(scratch + t * kScratchBlock + l16 * kScratchRow + 4 * grp);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) m_cols[t][r] = scratch[(t * 16 + 4 * grp + r) * 20 + l16];
+      for (int r = 0; r < 4; ++r) m_cols[t][r] = scratch[t * kScratchBlock + (4 * grp + r) * kScratchRow + l16];
     }
     wave_sync();
 #pragma unroll

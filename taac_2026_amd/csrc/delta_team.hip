@@ -55,34 +55,40 @@ struct TeamLds {  // fragments hi, then lo, of each
   static constexpr int kBackward = kTileQ + Tile<DK>::BYTES;
 };
 
-// What wavefront w needs of a chunk. Two of them take turns, so that nothing is copied.
-template <int KB>
+// What wavefront w needs of a chunk. Several of them take turns, so that nothing is copied.
+template <int KB, bool COLS>
 struct TeamChunk {
   bf16x8 kf[KB], qf[KB];
   bf16x8 mh[2], ml[2], pf[2];
   f32x4 grown, keep;
   float grown_row, total;
-  bf16x8 x[2];  // forward: four values of this lane's column in x[0]; backward: dO of the column, fragments over the tokens
+  // bits of a column's values: V (backward: dO) of the four own tokens of this lane; backward, dO of eight tokens per block of 32
+  uint32_t x[4], of[COLS ? 16 : 1];
 };
 
 template <int DK, bool COLS>
 struct Team {
   static constexpr int KB = DK / 32, KA = DK / 16, OWN = KA >= 4 ? KA / 4 : 1;  // OWN: state tiles of a wavefront
+  typedef TeamChunk<KB, COLS> Chunk;
   const DeltaParams& p;
   int wave, lane, l16, grp, col0, h, b, len, chunks;
   int64_t unit;
   bool col_ok, owner;
-  const bf16_t *k0, *q0, *x0;
-  const uint8_t* blocks;
-  uint32_t k_off, q_off, x_off, row_off;
+  // The chunk that fetch() requests next: uniform pointers that move by whole chunks, and byte offsets of this lane that stay (token strides
+  // are below 2^24 elements), so that a request costs no arithmetic.
+  const uint8_t *k_at, *q_at, *x_at, *block_at;
+  int64_t k_step, q_step, x_step;
+  int at;
+  uint32_t k_ld, q_ld, x_ld, k_off[KB], q_off[KB], x_off[4], of_off[COLS ? 16 : 1], frag_off[2], low_off[2], p_off[2], row_off;
 
   __device__ __forceinline__ Team(const DeltaParams& params) : p(params) {
     const int tid = threadIdx.x;
     wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     lane = tid % kWave, l16 = lane % 16, grp = lane / 16;
     const int col_groups = (p.dv + 15) / 16;
-    unit = blockIdx.x / col_groups;
-    col0 = static_cast<int>(blockIdx.x % col_groups) * 16;
+    const uint32_t block = xcd_remap(blockIdx.x, gridDim.x);  // the columns of a head, which read the same rows, on one die's L2
+    unit = block / col_groups;
+    col0 = static_cast<int>(block % col_groups) * 16;
     col_ok = col0 + l16 < p.dv;
     h = static_cast<int>(unit % p.H);
     b = static_cast<int>(unit / p.H);
@@ -94,81 +100,95 @@ struct Team {
     chunks = (len + kChunk - 1) / kChunk;
     const int64_t hk = h / p.group;
     const int64_t* xs = COLS ? p.dos : p.vs;
-    k0 = p.k + b * p.ks[0] + hk * p.ks[1];
-    q0 = p.q + b * p.qs[0] + hk * p.qs[1];
-    x0 = (COLS ? p.grad_o : p.v) + b * xs[0] + h * xs[1] + col0;
-    blocks = p.blocks + unit * p.chunks * kBlockBytes;
+    at = COLS ? chunks - 1 : 0;
+    const int64_t first = static_cast<int64_t>(at) * kChunk;
+    k_at = reinterpret_cast<const uint8_t*>(p.k + b * p.ks[0] + hk * p.ks[1] + first * p.ks[2]);
+    q_at = reinterpret_cast<const uint8_t*>(p.q + b * p.qs[0] + hk * p.qs[1] + first * p.qs[2]);
+    x_at = reinterpret_cast<const uint8_t*>((COLS ? p.grad_o : p.v) + b * xs[0] + h * xs[1] + col0 + first * xs[2]);
+    block_at = p.blocks + (unit * p.chunks + at) * kBlockBytes;
+    constexpr int64_t kMove = COLS ? -2 * kChunk : 2 * kChunk;
+    k_step = kMove * p.ks[2], q_step = kMove * p.qs[2], x_step = kMove * xs[2];
     owner = wave * OWN < KA;
-    const int row = 16 * wave + l16;
-    k_off = static_cast<uint32_t>(row * p.ks[2] + grp * 8) * 2;
-    q_off = static_cast<uint32_t>(row * p.qs[2] + grp * 8) * 2;
-    // columns behind the last read the last one: they are not stored and meet no other column
-    const int col = col_ok ? l16 : p.dv - 1 - col0;
-    x_off = static_cast<uint32_t>((COLS ? 0 : 16 * wave + 4 * grp) * xs[2] + (COLS ? 4 * grp * xs[2] : 0) + col) * 2;
-    row_off = static_cast<uint32_t>(16 * wave + 4 * grp) * 4;
+    k_ld = static_cast<uint32_t>(p.ks[2]) * 2, q_ld = static_cast<uint32_t>(p.qs[2]) * 2, x_ld = static_cast<uint32_t>(xs[2]) * 2;
+    offsets(kChunk);
+    const int w0 = COLS ? max(0, wave / 2) : 0, w1 = COLS ? 1 : min(1, wave / 2);  // a wavefront with one fragment reads it twice
+    frag_off[0] = (COLS ? frag_cols(wave, w0) : frag_rows(wave, w0)) * kFrag + lane * 16;
+    frag_off[1] = (COLS ? frag_cols(wave, w1) : frag_rows(wave, w1)) * kFrag + lane * 16;
+#pragma unroll
+    for (int tk = 0; tk < 2; ++tk) {
+      low_off[tk] = frag_off[tk] + kBlockLow;
+      p_off[tk] = frag_off[tk] + kBlockP;
+    }
+    row_off = kBlockRows + static_cast<uint32_t>(16 * wave + 4 * grp) * 4;
+  }
+  // This lane's places in a chunk of which `rows` rows exist in the tensors. Rows, features and columns behind the last read the last ones.
+  __device__ __forceinline__ void offsets(int rows) {
+    const uint32_t last = rows - 1;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const uint32_t feature = static_cast<uint32_t>(min(32 * kb + 8 * grp, p.dk - 8)) * 2;
+      k_off[kb] = min(static_cast<uint32_t>(16 * wave + l16), last) * k_ld + feature;
+      q_off[kb] = min(static_cast<uint32_t>(16 * wave + l16), last) * q_ld + feature;
+    }
+    const uint32_t col = static_cast<uint32_t>(col_ok ? l16 : p.dv - 1 - col0) * 2;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x_off[r] = min(static_cast<uint32_t>(16 * wave + 4 * grp + r), last) * x_ld + col;
+    if (COLS) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        of_off[e] = min(static_cast<uint32_t>(32 * (e / 8) + 16 * (e / 4 % 2) + e % 4 + 4 * grp), last) * x_ld + col;
+    }
   }
   __device__ __forceinline__ int tokens_of(int chunk) const {
     const int left = len - chunk * kChunk;
     return left < kChunk ? left : kChunk;
   }
 
-  __device__ __forceinline__ void fetch(int chunk, TeamChunk<KB>& c) const {
-    const int64_t token0 = static_cast<int64_t>(chunk) * kChunk;
-    const int n_tok = tokens_of(chunk);
-    const bf16_t *k = k0 + token0 * p.ks[2], *q = q0 + token0 * p.qs[2];
-    const int64_t x_ld = COLS ? p.dos[2] : p.vs[2];
-    const bf16_t* x = x0 + token0 * x_ld;
-    const uint8_t* block = blocks + static_cast<int64_t>(chunk) * kBlockBytes;
-    if (n_tok == kChunk && p.dk == DK) {
+  // Requests a chunk (behind the last one: that one again). Without a branch around the requests, what was requested before can be awaited
+  // without awaiting this; finish() puts zeros where there are no tokens.
+  __device__ __forceinline__ void fetch(Chunk& c) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        c.kf[kb] = at_offset<bf16x8>(k + kb * 32, k_off);
-        c.qf[kb] = at_offset<bf16x8>(q + kb * 32, q_off);
-      }
-      if (COLS) {
-#pragma unroll
-        for (int tk = 0; tk < 2; ++tk)
-          if (tk >= wave / 2) {  // the own tile and those behind it
-#pragma unroll
-            for (int e = 0; e < 8; ++e) c.x[tk][e] = at_offset<bf16_t>(x + (32 * tk + (e / 4) * 16 + e % 4) * x_ld, x_off);
-          }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) c.x[0][r] = at_offset<bf16_t>(x + r * x_ld, x_off);
-      }
-    } else {
-      const bool live = 16 * wave + l16 < n_tok;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        c.kf[kb] = c.qf[kb] = zero8();
-        if (live && kb * 32 + grp * 8 < p.dk) {
-          c.kf[kb] = at_offset<bf16x8>(k + kb * 32, k_off);
-          c.qf[kb] = at_offset<bf16x8>(q + kb * 32, q_off);
-        }
-      }
-#pragma unroll
-      for (int tk = 0; tk < (COLS ? 2 : 1); ++tk) {
-        c.x[tk] = zero8();
-#pragma unroll
-        for (int e = 0; e < (COLS ? 8 : 4); ++e) {
-          const int at = COLS ? 32 * tk + (e / 4) * 16 + e % 4 : e;
-          if (at + (COLS ? 0 : 16 * wave) + 4 * grp < n_tok) c.x[tk][e] = at_offset<bf16_t>(x + at * x_ld, x_off);
-        }
-      }
+    for (int kb = 0; kb < KB; ++kb) {
+      c.kf[kb] = at_offset<bf16x8>(k_at, k_off[kb]);
+      c.qf[kb] = at_offset<bf16x8>(q_at, q_off[kb]);
     }
 #pragma unroll
-    for (int tk = 0; tk < 2; ++tk)
-      if (COLS ? tk >= wave / 2 : tk <= wave / 2) {
-        const int f = COLS ? frag_cols(wave, tk) : frag_rows(wave, tk);
-        c.mh[tk] = at_offset<bf16x8>(block + kBlockM + f * kFrag, lane * 16);
-        c.ml[tk] = at_offset<bf16x8>(block + kBlockLow + f * kFrag, lane * 16);
-        c.pf[tk] = at_offset<bf16x8>(block + kBlockP + f * kFrag, lane * 16);
-      }
-    const uint8_t* rows = block + kBlockRows;
-    c.grown = at_offset<f32x4>(rows + kRowGrown * 4, row_off);
-    c.keep = at_offset<f32x4>(rows + kRowKeep * 4, row_off);
-    if (!COLS) c.grown_row = at_offset<float>(rows + kRowGrown * 4 + wave * 64, l16 * 4);
-    c.total = *reinterpret_cast<const float*>(rows + kRowTotal * 4);
+    for (int r = 0; r < 4; ++r) c.x[r] = at_offset<uint16_t>(x_at, x_off[r]);
+    if (COLS) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) c.of[e] = at_offset<uint16_t>(x_at, of_off[e]);
+    }
+#pragma unroll
+    for (int tk = 0; tk < 2; ++tk) {
+      c.mh[tk] = at_offset<bf16x8>(block_at, frag_off[tk]);
+      c.ml[tk] = at_offset<bf16x8>(block_at, low_off[tk]);
+      c.pf[tk] = at_offset<bf16x8>(block_at, p_off[tk]);
+    }
+    c.grown = at_offset<f32x4>(block_at + kRowGrown * 4, row_off);
+    c.keep = at_offset<f32x4>(block_at + kRowKeep * 4, row_off);
+    if (!COLS) c.grown_row = at_offset<float>(block_at + kBlockRows + kRowGrown * 4 + wave * 64, l16 * 4);
+    c.total = at_offset<float>(block_at + kBlockRows + kRowTotal * 4, 0);
+  }
+  // On to the next chunk to request.
+  __device__ __forceinline__ void advance() {
+    if (COLS ? at > 0 : at + 1 < chunks) {
+      at += COLS ? -1 : 1;
+      k_at += k_step, q_at += q_step, x_at += x_step;
+      block_at += COLS ? -kBlockBytes : kBlockBytes;
+      if (!COLS && p.T - at * kChunk < kChunk) offsets(p.T - at * kChunk);  // only the last chunk can reach behind the tensors' end
+    }
+  }
+  __device__ __forceinline__ void finish(Chunk& c, int n_tok) const {
+    if (n_tok == kChunk && p.dk == DK) return;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+      if (16 * wave + l16 >= n_tok || 32 * kb + 8 * grp >= p.dk) c.kf[kb] = c.qf[kb] = zero8();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c.x[r] = 16 * wave + 4 * grp + r < n_tok ? c.x[r] : 0;
+    if (COLS) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) c.of[e] = 32 * (e / 8) + 16 * (e / 4 % 2) + e % 4 + 4 * grp < n_tok ? c.of[e] : 0;
+    }
   }
 
   // The own rows of the state, bf16, at dst [dv][dk]
@@ -193,7 +213,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
   __shared__ __attribute__((aligned(16))) bf16_t turned[TRAIN ? 4 : 1][320];
   bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK);
   uint8_t *s_frags = smem + L::kState, *x_frags = smem + L::kX, *n_frags = smem + L::kN, *w_frags = smem + L::kW;
-  const M m(p);
+  M m(p);
   const int wave = m.wave, lane = m.lane, l16 = m.l16, grp = m.grp, col0 = m.col0;
   bf16_t* o0 = p.o + m.b * p.os[0] + m.h * p.os[1] + col0;
   const uint32_t o_off = static_cast<uint32_t>((16 * wave + l16) * p.os[2] + 4 * grp) * 2;
@@ -216,11 +236,18 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
     if (m.owner) put_half(s_frags, a, lane, s[i], KB * kFrag);
   }
 
-  auto step = [&](int chunk, const TeamChunk<KB>& cur, TeamChunk<KB>& next) __attribute__((always_inline)) {
-    const int64_t token0 = static_cast<int64_t>(chunk) * kChunk;
+  bf16_t* o_at = o0;
+  bf16_t* state_at = TRAIN ? p.chunk_states + m.unit * p.chunks * static_cast<int64_t>(p.dk) * p.dv : nullptr;
+  bf16_t* miss_at = TRAIN ? p.misses + m.unit * p.T * p.dv : nullptr;
+  auto step = [&](int chunk, typename M::Chunk& cur, typename M::Chunk& next) __attribute__((always_inline)) {
     const int n_tok = m.tokens_of(chunk);
-    if (chunk + 1 < m.chunks) m.fetch(chunk + 1, next);
-    if (TRAIN) m.store_state(p.chunk_states + (m.unit * p.chunks + chunk) * static_cast<int64_t>(p.dk) * p.dv, s);
+    m.fetch(next);
+    m.advance();
+    m.finish(cur, n_tok);
+    if (TRAIN) {
+      m.store_state(state_at, s);
+      state_at += p.dk * p.dv;
+    }
     // X of the own tokens; K's rows on their way into LDS
     bf16x8 sh[KB], sl[KB];
     f32x4 y = zero4(), y2 = zero4();
@@ -236,7 +263,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
       *reinterpret_cast<bf16x8*>(tile_k + (16 * wave + l16) * TK::STRIDE + kb * 32 + grp * 8) = cur.kf[kb];
     f32x4 x;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = fmaf(-cur.grown[r], y[r] + y2[r], static_cast<float>(cur.x[0][r]));
+    for (int r = 0; r < 4; ++r) x[r] = fmaf(-cur.grown[r], y[r] + y2[r], __builtin_bit_cast(float, cur.x[r] << 16));
     put_half(x_frags, wave, lane, x, 2 * kFrag);
     __syncthreads();
 
@@ -266,7 +293,8 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
     put_half(n_frags, wave, lane, x, 2 * kFrag);
     if (TRAIN) {
       const u32x2 rounded = turn16(turn, x, l16, grp);
-      if (16 * wave + l16 < n_tok && quad_ok) put_offset(p.misses + (m.unit * p.T + token0) * p.dv, n_off, rounded);
+      if (16 * wave + l16 < n_tok && quad_ok) put_offset(miss_at, n_off, rounded);
+      miss_at += kChunk * p.dv;
     }
     const float grown = cur.grown_row * p.scale;
 #pragma unroll
@@ -303,12 +331,17 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
     if (16 * wave + l16 < n_tok && quad_ok) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) out[r] += out2[r];
-      put_offset(o0 + token0 * p.os[2], o_off, round4(out));
+      put_offset(o_at, o_off, round4(out));
     }
+    o_at += kChunk * p.os[2];
     __syncthreads();
   };
-  TeamChunk<KB> even, odd;
-  if (m.chunks > 0) m.fetch(0, even);
+  typename M::Chunk even, odd;
+  if (m.chunks > 0) {
+    if (p.T < kChunk) m.offsets(p.T);
+    m.fetch(even);
+    m.advance();
+  }
   __syncthreads();
   for (int chunk = 0; chunk < m.chunks; chunk += 2) {
     step(chunk, even, odd);
@@ -344,7 +377,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
   bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK);
   bf16_t* tile_q = reinterpret_cast<bf16_t*>(smem + L::kTileQ);
   uint8_t *s_frags = smem + L::kState, *z_frags = smem + L::kX, *x_frags = smem + L::kN, *o_frags = smem + L::kW;
-  const M m(p);
+  M m(p);
   const int wave = m.wave, lane = m.lane, l16 = m.l16, grp = m.grp, col0 = m.col0;
   bf16_t* v0 = p.grad_v + m.b * p.dvs[0] + m.h * p.dvs[1] + col0;
   const uint32_t v_off = static_cast<uint32_t>((16 * wave + l16) * p.dvs[2] + 4 * grp) * 2;
@@ -357,11 +390,15 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
     if (m.owner) put_half(s_frags, wave * OWN + i, lane, s[i], KB * kFrag);
   }
 
-  auto step = [&](int chunk, const TeamChunk<KB>& cur, TeamChunk<KB>& next) __attribute__((always_inline)) {
-    const int64_t token0 = static_cast<int64_t>(chunk) * kChunk;
+  bf16_t* v_at = v0 + (m.chunks - 1) * kChunk * p.dvs[2];
+  bf16_t* state_at = p.grad_states + (m.unit * p.chunks + m.chunks - 1) * static_cast<int64_t>(p.dk) * p.dv;
+  auto step = [&](int chunk, typename M::Chunk& cur, typename M::Chunk& next) __attribute__((always_inline)) {
     const int n_tok = m.tokens_of(chunk);
-    if (chunk > 0) m.fetch(chunk - 1, next);
-    m.store_state(p.grad_states + (m.unit * p.chunks + chunk) * static_cast<int64_t>(p.dk) * p.dv, s);
+    m.fetch(next);
+    m.advance();
+    m.finish(cur, n_tok);
+    m.store_state(state_at, s);
+    state_at -= p.dk * p.dv;
     // beta dU of the own tokens
     f32x4 z = zero4(), z2 = zero4(), z3 = zero4();
 #pragma unroll
@@ -371,7 +408,12 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
     }
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk)
-      if (tk >= wave / 2) z3 = mfma16(cur.pf[tk], cur.x[tk], z3);
+      if (tk >= wave / 2) {
+        u32x4 of;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) of[e] = cur.of[8 * tk + 2 * e] | cur.of[8 * tk + 2 * e + 1] << 16;
+        z3 = mfma16(cur.pf[tk], __builtin_bit_cast(bf16x8, of), z3);
+      }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int at = (16 * wave + l16) * TK::STRIDE + kb * 32 + grp * 8;
@@ -379,11 +421,10 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
       *reinterpret_cast<bf16x8*>(tile_q + at) = cur.qf[kb];
     }
     f32x4 w;
-    const bf16x8 own = wave < 2 ? cur.x[0] : cur.x[1];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       z[r] = fmaf(cur.keep[r], z[r] + z2[r], z3[r]);
-      w[r] = p.scale * cur.grown[r] * static_cast<float>(wave % 2 == 0 ? own[r] : own[4 + r]);
+      w[r] = p.scale * cur.grown[r] * __builtin_bit_cast(float, cur.x[r] << 16);
     }
     put_half(z_frags, wave, lane, z, 2 * kFrag);
     put_half(o_frags, wave, lane, w, 2 * kFrag);
@@ -406,7 +447,8 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
     }
     put_half(x_frags, wave, lane, w, 2 * kFrag);
     const u32x2 rounded = turn16(turned[wave], z, l16, grp);
-    if (16 * wave + l16 < n_tok && quad_ok) put_offset(v0 + token0 * p.dvs[2], v_off, rounded);
+    if (16 * wave + l16 < n_tok && quad_ok) put_offset(v_at, v_off, rounded);
+    v_at -= kChunk * p.dvs[2];
     __syncthreads();
 
     // dS of the own rows
@@ -432,8 +474,13 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
     }
     __syncthreads();
   };
-  TeamChunk<KB> even, odd;
-  if (m.chunks > 0) m.fetch(m.chunks - 1, even);
+  typename M::Chunk even, odd;
+  if (m.chunks > 0) {
+    m.offsets(min(p.T - (m.chunks - 1) * kChunk, kChunk));
+    m.fetch(even);
+    if (m.chunks > 1) m.offsets(kChunk);  // the chunks in front of the last are whole
+    m.advance();
+  }
   __syncthreads();
   for (int chunk = m.chunks - 1; chunk >= 0; chunk -= 2) {
     step(chunk, even, odd);
