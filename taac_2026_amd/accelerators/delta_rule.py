@@ -60,9 +60,10 @@ def _strides(t: torch.Tensor) -> ctypes.Array:
 
 
 def _rows_view(t: torch.Tensor) -> torch.Tensor:
-    """``t`` where the chunk kernels can read it in place (contiguous rows at 16-byte addresses, not too far apart), else a copy."""
+    """``t`` where the chunk kernels can read it in place (contiguous rows at 16-byte addresses, not overlapping and not too far apart), else a copy."""
     strides = t.stride()
-    if strides[3] == 1 and strides[0] % 8 == strides[1] % 8 == strides[2] % 8 == 0 and strides[2] < 1 << 24 and t.data_ptr() % 16 == 0:
+    apart = t.shape[3] <= strides[2] < 1 << 24
+    if strides[3] == 1 and apart and strides[0] % 8 == strides[1] % 8 == strides[2] % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -64,7 +64,7 @@ int delta_team_back(const char* name, const DeltaParams& p, hipStream_t s);
 int delta_solo(const char* name, const DeltaParams& p, bool back, hipStream_t s);
 // The second half of the backward (delta_grads.hip).
 int delta_grads(const char* name, const DeltaParams& p, hipStream_t s);
-int delta_strides(const char* name, const char* what, const void* ptr, const int64_t* from, int64_t* to, bool rows);
+int delta_strides(const char* name, const char* what, const void* ptr, const int64_t* from, int64_t* to, bool rows, int32_t width);
 
 namespace {
 
@@ -127,6 +127,25 @@ __device__ __forceinline__ V at_offset(const T* base, uint32_t bytes) {
 template <typename T, typename V>
 __device__ __forceinline__ void put_offset(T* base, uint32_t bytes, const V& v) {
   *reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(base) + bytes) = v;
+}
+
+// Reads through a buffer descriptor: bytes at or beyond its end read as zero without touching memory, so that rows behind the last token
+// need neither a branch nor a mask. kNowhere: an offset behind every end (64 rows
+// of less than 2^24 elements end below it), so also for features or columns that there are not.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+constexpr uint32_t kNowhere = 0x80000000u;
+__device__ __forceinline__ Buffer buffer_of(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes), 0x00027000);
+}
+// n rows of `width` elements, ld elements apart (at least width)
+__device__ __forceinline__ Buffer rows_buffer(const bf16_t* base, int64_t ld, int n, int width) {
+  return buffer_of(base, n > 0 ? static_cast<uint32_t>((n - 1) * ld + width) * 2 : 0);
+}
+__device__ __forceinline__ bf16x8 read8(Buffer b, uint32_t off) {
+  return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+}
+__device__ __forceinline__ uint32_t read1(Buffer b, uint32_t off) {
+  return static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(b, off, 0, 0));
 }
 
 __device__ __forceinline__ int state_row(int a, int m) { return 32 * (a / 2) + 8 * (m / 4) + 4 * (a % 2) + m % 4; }

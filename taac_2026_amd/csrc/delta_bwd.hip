@@ -258,16 +258,16 @@ extern "C" int taac_delta_rule_bwd(const void* q, const void* k, const void* log
   if (!q || !k || !log_decay || !beta || !chunk_states || !misses || !grad_o || !grad_q || !grad_k || !grad_v || !grad_decay || !grad_beta ||
       !grad_states)
     return set_error(TAAC_ERR_INVALID_VALUE, "%s: null tensor pointer", name);
-  if (int rc = delta_strides(name, "q", q, q_strides, p.qs, true)) return rc;
-  if (int rc = delta_strides(name, "k", k, k_strides, p.ks, true)) return rc;
-  if (int rc = delta_strides(name, "log_decay", log_decay, decay_strides, p.gs, false)) return rc;
-  if (int rc = delta_strides(name, "beta", beta, beta_strides, p.bs, false)) return rc;
-  if (int rc = delta_strides(name, "grad_o", grad_o, go_strides, p.dos, true)) return rc;
-  if (int rc = delta_strides(name, "grad_q", grad_q, gq_strides, p.dqs, true)) return rc;
-  if (int rc = delta_strides(name, "grad_k", grad_k, gk_strides, p.dks, true)) return rc;
-  if (int rc = delta_strides(name, "grad_v", grad_v, gv_strides, p.dvs, true)) return rc;
-  if (int rc = delta_strides(name, "grad_log_decay", grad_decay, gdecay_strides, p.dgs, false)) return rc;
-  if (int rc = delta_strides(name, "grad_beta", grad_beta, gbeta_strides, p.dbs, false)) return rc;
+  if (int rc = delta_strides(name, "q", q, q_strides, p.qs, true, dk)) return rc;
+  if (int rc = delta_strides(name, "k", k, k_strides, p.ks, true, dk)) return rc;
+  if (int rc = delta_strides(name, "log_decay", log_decay, decay_strides, p.gs, false, 1)) return rc;
+  if (int rc = delta_strides(name, "beta", beta, beta_strides, p.bs, false, 1)) return rc;
+  if (int rc = delta_strides(name, "grad_o", grad_o, go_strides, p.dos, true, dv)) return rc;
+  if (int rc = delta_strides(name, "grad_q", grad_q, gq_strides, p.dqs, true, dk)) return rc;
+  if (int rc = delta_strides(name, "grad_k", grad_k, gk_strides, p.dks, true, dk)) return rc;
+  if (int rc = delta_strides(name, "grad_v", grad_v, gv_strides, p.dvs, true, dv)) return rc;
+  if (int rc = delta_strides(name, "grad_log_decay", grad_decay, gdecay_strides, p.dgs, false, 1)) return rc;
+  if (int rc = delta_strides(name, "grad_beta", grad_beta, gbeta_strides, p.dbs, false, 1)) return rc;
   p.q = static_cast<const bf16_t*>(q), p.k = static_cast<const bf16_t*>(k), p.log_decay = log_decay, p.beta = beta, p.lengths = lengths;
   p.chunk_states = const_cast<bf16_t*>(static_cast<const bf16_t*>(chunk_states));
   p.misses = const_cast<bf16_t*>(static_cast<const bf16_t*>(misses));

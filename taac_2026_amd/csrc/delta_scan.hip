@@ -270,13 +270,15 @@ int delta_check(const char* name, const DeltaParams& p) {
 }
 
 // Strides of (batch, head, token): multiples of 8 elements for the 16-byte rows.
-int delta_strides(const char* name, const char* what, const void* ptr, const int64_t* from, int64_t* to, bool rows) {
+int delta_strides(const char* name, const char* what, const void* ptr, const int64_t* from, int64_t* to, bool rows, int32_t width) {
   if (from == nullptr) return set_error(TAAC_ERR_INVALID_VALUE, "%s: null strides of %s", name, what);
   for (int i = 0; i < 3; ++i) {
     to[i] = from[i];
     if (from[i] < 0 || (rows && from[i] % 8 != 0))
       return set_error(TAAC_ERR_INVALID_VALUE, "%s: strides of %s must be multiples of 8, not negative", name, what);
   }
+  if (rows && from[2] < width)
+    return set_error(TAAC_ERR_INVALID_VALUE, "%s: the token stride of %s must cover a row", name, what);
   if (rows && from[2] >= (1 << 24)) return set_error(TAAC_ERR_UNSUPPORTED, "%s: the token stride of %s must be below 2^24", name, what);
   if (rows && !aligned16(ptr)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: %s must be 16-byte aligned", name, what);
   return TAAC_OK;
@@ -305,12 +307,12 @@ extern "C" int taac_delta_rule_fwd(const void* q, const void* k, const void* v, 
     return set_error(TAAC_ERR_INVALID_VALUE, "%s: chunk_states and misses come together", name);
   if (B == 0 || (T == 0 && state_out == nullptr)) return TAAC_OK;
   if (T > 0 && (!q || !k || !v || !log_decay || !beta || !o)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: null tensor pointer", name);
-  if (int rc = delta_strides(name, "q", q, q_strides, p.qs, true)) return rc;
-  if (int rc = delta_strides(name, "k", k, k_strides, p.ks, true)) return rc;
-  if (int rc = delta_strides(name, "v", v, v_strides, p.vs, true)) return rc;
-  if (int rc = delta_strides(name, "o", o, o_strides, p.os, true)) return rc;
-  if (int rc = delta_strides(name, "log_decay", log_decay, decay_strides, p.gs, false)) return rc;
-  if (int rc = delta_strides(name, "beta", beta, beta_strides, p.bs, false)) return rc;
+  if (int rc = delta_strides(name, "q", q, q_strides, p.qs, true, dk)) return rc;
+  if (int rc = delta_strides(name, "k", k, k_strides, p.ks, true, dk)) return rc;
+  if (int rc = delta_strides(name, "v", v, v_strides, p.vs, true, dv)) return rc;
+  if (int rc = delta_strides(name, "o", o, o_strides, p.os, true, dv)) return rc;
+  if (int rc = delta_strides(name, "log_decay", log_decay, decay_strides, p.gs, false, 1)) return rc;
+  if (int rc = delta_strides(name, "beta", beta, beta_strides, p.bs, false, 1)) return rc;
   p.q = static_cast<const bf16_t*>(q), p.k = static_cast<const bf16_t*>(k), p.v = static_cast<const bf16_t*>(v);
   p.o = static_cast<bf16_t*>(o), p.log_decay = log_decay, p.beta = beta, p.lengths = lengths;
   p.state_in = state_in, p.state_out = state_out;

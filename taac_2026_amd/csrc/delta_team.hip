@@ -74,12 +74,13 @@ struct Team {
   int wave, lane, l16, grp, col0, h, b, len, chunks;
   int64_t unit;
   bool col_ok, owner;
-  // The chunk that fetch() requests next: uniform pointers that move by whole chunks, and byte offsets of this lane that stay (token strides
-  // are below 2^24 elements), so that a request costs no arithmetic.
-  const uint8_t *k_at, *q_at, *x_at, *block_at;
+  // The chunk that is requested next: uniform pointers that move by whole chunks, and byte offsets of this lane that stay (token strides are
+  // below 2^24 elements), so that a request costs no arithmetic.
+  const bf16_t *k_at, *q_at, *x_at;
+  const uint8_t* block_at;
   int64_t k_step, q_step, x_step;
   int at;
-  uint32_t k_ld, q_ld, x_ld, k_off[KB], q_off[KB], x_off[4], of_off[COLS ? 16 : 1], frag_off[2], low_off[2], p_off[2], row_off;
+  uint32_t k_off[KB], q_off[KB], x_off[4], of_off[COLS ? 16 : 1], frag_off[2], row_off;
 
   __device__ __forceinline__ Team(const DeltaParams& params) : p(params) {
     const int tid = threadIdx.x;
@@ -102,93 +103,78 @@ struct Team {
     const int64_t* xs = COLS ? p.dos : p.vs;
     at = COLS ? chunks - 1 : 0;
     const int64_t first = static_cast<int64_t>(at) * kChunk;
-    k_at = reinterpret_cast<const uint8_t*>(p.k + b * p.ks[0] + hk * p.ks[1] + first * p.ks[2]);
-    q_at = reinterpret_cast<const uint8_t*>(p.q + b * p.qs[0] + hk * p.qs[1] + first * p.qs[2]);
-    x_at = reinterpret_cast<const uint8_t*>((COLS ? p.grad_o : p.v) + b * xs[0] + h * xs[1] + col0 + first * xs[2]);
+    k_at = p.k + b * p.ks[0] + hk * p.ks[1] + first * p.ks[2];
+    q_at = p.q + b * p.qs[0] + hk * p.qs[1] + first * p.qs[2];
+    x_at = (COLS ? p.grad_o : p.v) + b * xs[0] + h * xs[1] + col0 + first * xs[2];
     block_at = p.blocks + (unit * p.chunks + at) * kBlockBytes;
-    constexpr int64_t kMove = COLS ? -2 * kChunk : 2 * kChunk;
+    constexpr int64_t kMove = COLS ? -kChunk : kChunk;
     k_step = kMove * p.ks[2], q_step = kMove * p.qs[2], x_step = kMove * xs[2];
     owner = wave * OWN < KA;
-    k_ld = static_cast<uint32_t>(p.ks[2]) * 2, q_ld = static_cast<uint32_t>(p.qs[2]) * 2, x_ld = static_cast<uint32_t>(xs[2]) * 2;
-    offsets(kChunk);
-    const int w0 = COLS ? max(0, wave / 2) : 0, w1 = COLS ? 1 : min(1, wave / 2);  // a wavefront with one fragment reads it twice
-    frag_off[0] = (COLS ? frag_cols(wave, w0) : frag_rows(wave, w0)) * kFrag + lane * 16;
-    frag_off[1] = (COLS ? frag_cols(wave, w1) : frag_rows(wave, w1)) * kFrag + lane * 16;
-#pragma unroll
-    for (int tk = 0; tk < 2; ++tk) {
-      low_off[tk] = frag_off[tk] + kBlockLow;
-      p_off[tk] = frag_off[tk] + kBlockP;
-    }
-    row_off = kBlockRows + static_cast<uint32_t>(16 * wave + 4 * grp) * 4;
-  }
-  // This lane's places in a chunk of which `rows` rows exist in the tensors. Rows, features and columns behind the last read the last ones.
-  __device__ __forceinline__ void offsets(int rows) {
-    const uint32_t last = rows - 1;
+    const uint32_t k_ld = static_cast<uint32_t>(p.ks[2]) * 2, q_ld = static_cast<uint32_t>(p.qs[2]) * 2, x_ld = static_cast<uint32_t>(xs[2]) * 2;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const uint32_t feature = static_cast<uint32_t>(min(32 * kb + 8 * grp, p.dk - 8)) * 2;
-      k_off[kb] = min(static_cast<uint32_t>(16 * wave + l16), last) * k_ld + feature;
-      q_off[kb] = min(static_cast<uint32_t>(16 * wave + l16), last) * q_ld + feature;
+      const uint32_t feature = static_cast<uint32_t>(32 * kb + 8 * grp);
+      k_off[kb] = feature < static_cast<uint32_t>(p.dk) ? (16 * wave + l16) * k_ld + feature * 2 : kNowhere;
+      q_off[kb] = feature < static_cast<uint32_t>(p.dk) ? (16 * wave + l16) * q_ld + feature * 2 : kNowhere;
     }
-    const uint32_t col = static_cast<uint32_t>(col_ok ? l16 : p.dv - 1 - col0) * 2;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x_off[r] = min(static_cast<uint32_t>(16 * wave + 4 * grp + r), last) * x_ld + col;
+    for (int r = 0; r < 4; ++r) x_off[r] = col_ok ? (16 * wave + 4 * grp + r) * x_ld + l16 * 2 : kNowhere;
     if (COLS) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        of_off[e] = min(static_cast<uint32_t>(32 * (e / 8) + 16 * (e / 4 % 2) + e % 4 + 4 * grp), last) * x_ld + col;
+      for (int i = 0; i < 16; ++i) {  // dO in front of the own tile is not needed
+        const int row = 32 * (i / 8) + 16 * (i / 4 % 2) + i % 4;
+        of_off[i] = col_ok && row / 16 >= wave ? (row + 4 * grp) * x_ld + l16 * 2 : kNowhere;
+      }
     }
+#pragma unroll
+    for (int tk = 0; tk < 2; ++tk)
+      frag_off[tk] = (COLS ? tk >= wave / 2 : tk <= wave / 2) ? (COLS ? frag_cols(wave, tk) : frag_rows(wave, tk)) * kFrag + lane * 16 : kNowhere;
+    row_off = static_cast<uint32_t>(16 * wave + 4 * grp) * 4;
   }
   __device__ __forceinline__ int tokens_of(int chunk) const {
     const int left = len - chunk * kChunk;
     return left < kChunk ? left : kChunk;
   }
 
-  // Requests a chunk (behind the last one: that one again). Without a branch around the requests, what was requested before can be awaited
-  // without awaiting this; finish() puts zeros where there are no tokens.
-  __device__ __forceinline__ void fetch(Chunk& c) {
+  // The requests for a chunk (behind the last one: that one again), in three parts that the stages of the chunk before it issue beside their
+  // work: in one run they would wait for each other in front of it. No branch around them, so that what was requested before can be
+  // awaited without awaiting these.
+  __device__ __forceinline__ void fetch_keys(Chunk& c) const {
+    const int n = tokens_of(at);
+    const Buffer k = rows_buffer(k_at, p.ks[2], n, p.dk), x = rows_buffer(x_at, COLS ? p.dos[2] : p.vs[2], n, p.dv - col0);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      c.kf[kb] = at_offset<bf16x8>(k_at, k_off[kb]);
-      c.qf[kb] = at_offset<bf16x8>(q_at, q_off[kb]);
-    }
+    for (int kb = 0; kb < KB; ++kb) c.kf[kb] = read8(k, k_off[kb]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) c.x[r] = at_offset<uint16_t>(x_at, x_off[r]);
+    for (int r = 0; r < 4; ++r) c.x[r] = read1(x, x_off[r]);
     if (COLS) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) c.of[e] = at_offset<uint16_t>(x_at, of_off[e]);
+      for (int i = 0; i < 16; ++i) c.of[i] = read1(x, of_off[i]);
     }
+    const uint8_t* rows = block_at + kBlockRows;
+    c.grown = at_offset<f32x4>(rows + kRowGrown * 4, row_off);
+    c.keep = at_offset<f32x4>(rows + kRowKeep * 4, row_off);
+    if (!COLS) c.grown_row = at_offset<float>(rows + kRowGrown * 4 + wave * 64, l16 * 4);
+    c.total = at_offset<float>(rows + kRowTotal * 4, 0);
+  }
+  __device__ __forceinline__ void fetch_queries(Chunk& c) const {
+    const Buffer q = rows_buffer(q_at, p.qs[2], tokens_of(at), p.dk);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) c.qf[kb] = read8(q, q_off[kb]);
+  }
+  // the last part, then on to the next chunk
+  __device__ __forceinline__ void fetch_block(Chunk& c) {
+    const Buffer high = buffer_of(block_at + kBlockM, 6 * kFrag), low = buffer_of(block_at + kBlockLow, 6 * kFrag),
+                 score = buffer_of(block_at + kBlockP, 6 * kFrag);
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk) {
-      c.mh[tk] = at_offset<bf16x8>(block_at, frag_off[tk]);
-      c.ml[tk] = at_offset<bf16x8>(block_at, low_off[tk]);
-      c.pf[tk] = at_offset<bf16x8>(block_at, p_off[tk]);
+      c.mh[tk] = read8(high, frag_off[tk]);
+      c.ml[tk] = read8(low, frag_off[tk]);
+      c.pf[tk] = read8(score, frag_off[tk]);
     }
-    c.grown = at_offset<f32x4>(block_at + kRowGrown * 4, row_off);
-    c.keep = at_offset<f32x4>(block_at + kRowKeep * 4, row_off);
-    if (!COLS) c.grown_row = at_offset<float>(block_at + kBlockRows + kRowGrown * 4 + wave * 64, l16 * 4);
-    c.total = at_offset<float>(block_at + kBlockRows + kRowTotal * 4, 0);
-  }
-  // On to the next chunk to request.
-  __device__ __forceinline__ void advance() {
-    if (COLS ? at > 0 : at + 1 < chunks) {
-      at += COLS ? -1 : 1;
-      k_at += k_step, q_at += q_step, x_at += x_step;
-      block_at += COLS ? -kBlockBytes : kBlockBytes;
-      if (!COLS && p.T - at * kChunk < kChunk) offsets(p.T - at * kChunk);  // only the last chunk can reach behind the tensors' end
-    }
-  }
-  __device__ __forceinline__ void finish(Chunk& c, int n_tok) const {
-    if (n_tok == kChunk && p.dk == DK) return;
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-      if (16 * wave + l16 >= n_tok || 32 * kb + 8 * grp >= p.dk) c.kf[kb] = c.qf[kb] = zero8();
-#pragma unroll
-    for (int r = 0; r < 4; ++r) c.x[r] = 16 * wave + 4 * grp + r < n_tok ? c.x[r] : 0;
-    if (COLS) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) c.of[e] = 32 * (e / 8) + 16 * (e / 4 % 2) + e % 4 + 4 * grp < n_tok ? c.of[e] : 0;
-    }
+    const bool more = COLS ? at > 0 : at + 1 < chunks;
+    at += more ? (COLS ? -1 : 1) : 0;
+    k_at += more ? k_step : 0, q_at += more ? q_step : 0, x_at += more ? x_step : 0;
+    block_at += more ? (COLS ? -kBlockBytes : kBlockBytes) : 0;
   }
 
   // The own rows of the state, bf16, at dst [dv][dk]
@@ -241,9 +227,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
   bf16_t* miss_at = TRAIN ? p.misses + m.unit * p.T * p.dv : nullptr;
   auto step = [&](int chunk, typename M::Chunk& cur, typename M::Chunk& next) __attribute__((always_inline)) {
     const int n_tok = m.tokens_of(chunk);
-    m.fetch(next);
-    m.advance();
-    m.finish(cur, n_tok);
+    m.fetch_keys(next);
     if (TRAIN) {
       m.store_state(state_at, s);
       state_at += p.dk * p.dv;
@@ -266,6 +250,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
     for (int r = 0; r < 4; ++r) x[r] = fmaf(-cur.grown[r], y[r] + y2[r], __builtin_bit_cast(float, cur.x[r] << 16));
     put_half(x_frags, wave, lane, x, 2 * kFrag);
     __syncthreads();
+    m.fetch_queries(next);
 
     // N of the own tokens
     f32x4 x2 = zero4(), x3 = zero4();
@@ -300,6 +285,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
 #pragma unroll
     for (int r = 0; r < 4; ++r) out[r] = (out[r] + out2[r]) * grown;
     __syncthreads();
+    m.fetch_block(next);
 
     // the own rows of the state
     if (m.owner) {
@@ -338,15 +324,18 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
   };
   typename M::Chunk even, odd;
   if (m.chunks > 0) {
-    if (p.T < kChunk) m.offsets(p.T);
-    m.fetch(even);
-    m.advance();
+    m.fetch_keys(even);
+    m.fetch_queries(even);
+    m.fetch_block(even);
   }
   __syncthreads();
-  for (int chunk = 0; chunk < m.chunks; chunk += 2) {
+  // Pairs, then the odd one: a way past the second half back to the first would have to await the requests of the wrong one.
+  int chunk = 0;
+  for (; chunk + 1 < m.chunks; chunk += 2) {
     step(chunk, even, odd);
-    if (chunk + 1 < m.chunks) step(chunk + 1, odd, even);
+    step(chunk + 1, odd, even);
   }
+  if (chunk < m.chunks) step(chunk, even, odd);
 
   if (p.state_out != nullptr && m.col_ok && m.owner) {
 #pragma unroll
@@ -394,9 +383,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
   bf16_t* state_at = p.grad_states + (m.unit * p.chunks + m.chunks - 1) * static_cast<int64_t>(p.dk) * p.dv;
   auto step = [&](int chunk, typename M::Chunk& cur, typename M::Chunk& next) __attribute__((always_inline)) {
     const int n_tok = m.tokens_of(chunk);
-    m.fetch(next);
-    m.advance();
-    m.finish(cur, n_tok);
+    m.fetch_keys(next);
     m.store_state(state_at, s);
     state_at -= p.dk * p.dv;
     // beta dU of the own tokens
@@ -429,6 +416,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
     put_half(z_frags, wave, lane, z, 2 * kFrag);
     put_half(o_frags, wave, lane, w, 2 * kFrag);
     __syncthreads();
+    m.fetch_queries(next);
 
     // dX of the own tokens
     z2 = z3 = zero4();
@@ -450,6 +438,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
     if (16 * wave + l16 < n_tok && quad_ok) put_offset(v_at, v_off, rounded);
     v_at -= kChunk * p.dvs[2];
     __syncthreads();
+    m.fetch_block(next);
 
     // dS of the own rows
     if (m.owner) {
@@ -476,16 +465,17 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
   };
   typename M::Chunk even, odd;
   if (m.chunks > 0) {
-    m.offsets(min(p.T - (m.chunks - 1) * kChunk, kChunk));
-    m.fetch(even);
-    if (m.chunks > 1) m.offsets(kChunk);  // the chunks in front of the last are whole
-    m.advance();
+    m.fetch_keys(even);
+    m.fetch_queries(even);
+    m.fetch_block(even);
   }
   __syncthreads();
-  for (int chunk = m.chunks - 1; chunk >= 0; chunk -= 2) {
+  int chunk = m.chunks - 1;  // pairs, then the odd one, as above
+  for (; chunk > 0; chunk -= 2) {
     step(chunk, even, odd);
-    if (chunk > 0) step(chunk - 1, odd, even);
+    step(chunk - 1, odd, even);
   }
+  if (chunk == 0) step(0, even, odd);
   const bf16_t none = static_cast<bf16_t>(0.f);
   for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.T - m.len) * 16; i += 4 * kWave) {
     const int at = static_cast<int>(i % 16);
