@@ -27,15 +27,16 @@ _Strides = ctypes.c_int64 * 3
 
 
 def _check_shapes(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, beta: torch.Tensor) -> None:
-    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
+    q_shape, k_shape, v_shape = q.shape, k.shape, v.shape
+    if len(q_shape) != 4 or len(k_shape) != 4 or len(v_shape) != 4:
         raise ValueError(f"{name} expects q, k, and v with shape (batch, heads, tokens, width)")
-    if q.shape != k.shape:
-        raise ValueError(f"{name} requires q and k of the same shape, got {tuple(q.shape)} and {tuple(k.shape)}")
-    if v.shape[0] != k.shape[0] or v.shape[2] != k.shape[2]:
+    if q_shape != k_shape:
+        raise ValueError(f"{name} requires q and k of the same shape, got {tuple(q_shape)} and {tuple(k_shape)}")
+    if v_shape[0] != k_shape[0] or v_shape[2] != k_shape[2]:
         raise ValueError(f"{name} requires matching batch and token dimensions of k and v")
-    if k.shape[1] == 0 or v.shape[1] == 0 or v.shape[1] % k.shape[1] != 0:
+    if k_shape[1] == 0 or v_shape[1] == 0 or v_shape[1] % k_shape[1] != 0:
         raise ValueError(f"{name} requires a number of value heads that is a multiple of the key heads")
-    if log_decay.shape != v.shape[:3] or beta.shape != v.shape[:3]:
+    if log_decay.shape != v_shape[:3] or beta.shape != v_shape[:3]:
         raise ValueError(f"{name} expects log_decay and beta with shape (batch, value heads, tokens)")
     require_same_dtype(f"{name} q, k, v", q, k, v)
     require_same_dtype(f"{name} gates", log_decay, beta)
@@ -70,7 +71,7 @@ def _rows_view(t: torch.Tensor) -> torch.Tensor:
 
 def _token_major(batch: int, heads: int, tokens: int, width: int, like: torch.Tensor) -> torch.Tensor:
     """(batch, heads, tokens, width) whose memory order is (batch, tokens, heads, width): the rows of the layers around it."""
-    return torch.empty(batch, tokens, heads, width, dtype=like.dtype, device=like.device).transpose(1, 2)
+    return like.new_empty((batch, tokens, heads, width)).transpose(1, 2)
 
 
 def _workspace(k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:

@@ -9,7 +9,10 @@ There is exactly one compute path - ``taac_rmsnorm_fwd`` / ``taac_layernorm_fwd`
 
 from __future__ import annotations
 
+import math
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from taac_2026_amd import _native
 from taac_2026_amd.accelerators.tensor_validation import require_cuda_tensors, require_inference, require_same_dtype
@@ -231,8 +234,9 @@ def layer_norm(
     return hip_layer_norm_kernel(rows, normalized_weight, normalized_bias, eps).reshape(original_shape)
 
 
-def _residual_rows(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, operator: str
-                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def _residual_inputs(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, operator: str
+                     ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Contiguous, in their own shape: a reshape there and back would cost a short call more than its kernel."""
     if x.ndim < 2:
         raise ValueError(f"{operator} expects input with at least 2 dimensions")
     if residual.shape != x.shape:
@@ -243,8 +247,11 @@ def _residual_rows(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor
         raise ValueError(f"last dimension {x.shape[-1]} does not match weight size {weight.shape[0]}")
     require_cuda_tensors(f"hip {operator}", x, residual, weight)
     require_same_dtype(operator, x, residual)
-    width = x.shape[-1]
-    return x.reshape(-1, width).contiguous(), residual.reshape(-1, width).contiguous(), weight.to(x.dtype).contiguous()
+    return x.contiguous(), residual.contiguous(), (weight if weight.dtype == x.dtype else weight.to(x.dtype)).contiguous()
+
+
+def _row_count(x: torch.Tensor) -> int:
+    return math.prod(x.shape[:-1])
 
 
 def _residual_rms_norm_forward(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float
@@ -253,7 +260,7 @@ def _residual_rms_norm_forward(x: torch.Tensor, residual: torch.Tensor, weight: 
     normed, summed = torch.empty_like(x), torch.empty_like(x)
     with _native.on_device(x.device):
         status = library.taac_residual_rmsnorm_fwd(
-            x.data_ptr(), residual.data_ptr(), weight.data_ptr(), summed.data_ptr(), normed.data_ptr(), x.shape[0], x.shape[1],
+            x.data_ptr(), residual.data_ptr(), weight.data_ptr(), summed.data_ptr(), normed.data_ptr(), _row_count(x), x.shape[-1],
             float(eps), _native.dtype_code(x.dtype), _native.current_stream(x.device))
     _native.check(status, "residual_rms_norm")
     return normed, summed
@@ -271,6 +278,7 @@ class _HipResidualRMSNormFunction(torch.autograd.Function):
         return normed, summed
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_normed, grad_summed):
         if grad_normed is None:  # only the sum was used
             return grad_summed, grad_summed, None, None
@@ -280,10 +288,10 @@ class _HipResidualRMSNormFunction(torch.autograd.Function):
         grad_summed = None if grad_summed is None else grad_summed.contiguous()
         with _native.on_device(summed.device):
             grad_x, grad_w = torch.empty_like(summed), torch.empty_like(weight)
-            workspace = _backward_workspace(summed, False)
+            workspace = _backward_workspace(summed.view(-1, summed.shape[-1]), False)
             status = library.taac_residual_rmsnorm_bwd(
                 summed.data_ptr(), weight.data_ptr(), grad_normed.data_ptr(), _native.ptr(grad_summed), grad_x.data_ptr(),
-                grad_w.data_ptr(), workspace.data_ptr(), workspace.numel(), summed.shape[0], summed.shape[1], ctx.eps,
+                grad_w.data_ptr(), workspace.data_ptr(), workspace.numel(), _row_count(summed), summed.shape[-1], ctx.eps,
                 _native.dtype_code(summed.dtype), _native.current_stream(summed.device))
         _native.check(status, "residual_rms_norm backward")
         return grad_x, grad_x, grad_w, None
@@ -295,12 +303,10 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
     to its residual stream and the norm in front of the next half. The norm is that of the sum as it is stored (rounded to
     x's dtype), so the results are those of the addition followed by :func:`rms_norm`. Differentiable in x, residual and
     weight; the gradient of the sum and that through the norm are added in the backward kernel."""
-    rows, residual_rows, normalized_weight = _residual_rows(x, residual, weight, "residual_rms_norm")
+    inputs = _residual_inputs(x, residual, weight, "residual_rms_norm")
     if _needs_grad(x, residual, weight):
-        normed, summed = _HipResidualRMSNormFunction.apply(rows, residual_rows, normalized_weight, eps)
-    else:
-        normed, summed = _residual_rms_norm_forward(rows, residual_rows, normalized_weight, eps)
-    return normed.reshape(x.shape), summed.reshape(x.shape)
+        return _HipResidualRMSNormFunction.apply(*inputs, eps)
+    return _residual_rms_norm_forward(*inputs, eps)
 
 
 def residual_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6
@@ -308,19 +314,18 @@ def residual_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch
     """``(values, row_amax, summed)``: :func:`residual_rms_norm` whose norm leaves as ``float8_e4m3fn`` with one float32
     maximum per row, ``values = e4m3(normed * 448 / row_amax)``, the activations of ``linear_fp8(values, weight, row_amax,
     amax_w)``. The norm is not rounded on its way to 8 bits. Forward only."""
-    rows, residual_rows, normalized_weight = _residual_rows(x, residual, weight, "residual_rms_norm_fp8")
+    x, residual, weight_row = _residual_inputs(x, residual, weight, "residual_rms_norm_fp8")
     require_inference("hip residual_rms_norm_fp8", x, residual, weight)
     library = _native.load_library()
-    summed = torch.empty_like(rows)
-    values = torch.empty(rows.shape, dtype=torch.uint8, device=rows.device)
-    row_amax = torch.empty(rows.shape[0], dtype=torch.float32, device=rows.device)
-    with _native.on_device(rows.device):
+    summed = torch.empty_like(x)
+    values = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    row_amax = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    with _native.on_device(x.device):
         status = library.taac_residual_rmsnorm_fp8_fwd(
-            rows.data_ptr(), residual_rows.data_ptr(), normalized_weight.data_ptr(), summed.data_ptr(), values.data_ptr(),
-            row_amax.data_ptr(), rows.shape[0], rows.shape[1], float(eps), _native.dtype_code(rows.dtype),
-            _native.current_stream(rows.device))
+            x.data_ptr(), residual.data_ptr(), weight_row.data_ptr(), summed.data_ptr(), values.data_ptr(), row_amax.data_ptr(),
+            _row_count(x), x.shape[-1], float(eps), _native.dtype_code(x.dtype), _native.current_stream(x.device))
     _native.check(status, "residual_rms_norm_fp8")
-    return values.view(torch.float8_e4m3fn).reshape(x.shape), row_amax.reshape(x.shape[:-1]), summed.reshape(x.shape)
+    return values, row_amax, summed
 
 
 __all__ = [
