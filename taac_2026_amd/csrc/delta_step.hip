@@ -7,7 +7,7 @@
 //
 // Samples that name the same slot are one sequence: their tokens are applied in the order of the batch, by the workgroup of the
 // first of them. A slot outside the pool (padding) reads and writes no state and gives zeros.
-#include "common.h"
+#include "delta.h"
 
 namespace taac {
 namespace {
@@ -29,15 +29,43 @@ struct StepParams {
   float scale;
 };
 
+// An element of a row as the bits that a read brings, for a conversion after everything is requested.
 template <typename T>
-__device__ __forceinline__ float gate_at(const void* p, int64_t at, int f32) {
-  return f32 ? static_cast<const float*>(p)[at] : static_cast<float>(static_cast<const T*>(p)[at]);
+__device__ __forceinline__ uint32_t read_bits(Buffer b, uint32_t off) {
+  if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(b, off, 0, 0);
+  else return read1(b, off);
 }
+template <typename T>
+__device__ __forceinline__ float from_bits(uint32_t bits) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, bits);
+  else return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(bits)));
+}
+// A gate is fp32 or a T, read by halves either way: a branch between two reads would await each.
+struct Gate {
+  uint32_t low, high;
+  __device__ __forceinline__ void request(const void* p, int64_t at, int f32) {
+    const Buffer b = buffer_of(static_cast<const uint8_t*>(p) + at * (f32 ? 4 : 2), f32 ? 4 : 2);
+    low = read1(b, 0);
+    high = read1(b, 2);  // zero behind a gate of two bytes
+  }
+  template <typename T>
+  __device__ __forceinline__ float value(int f32) const {
+    const float wide = __builtin_bit_cast(float, high << 16 | low);
+    return f32 ? wide : from_bits<T>(low);
+  }
+};
+
+template <int RPT>
+struct Token {
+  Gate log_decay, beta;
+  uint32_t v[4], k[RPT], q[RPT];
+};
 
 // NVP: lanes to a row of value columns (4 columns each); W wavefronts; RPT key rows to a lane.
 template <typename T, int NVP, int W, int RPT>
 __global__ __launch_bounds__(W * kWave) void delta_step_kernel(const StepParams p) {
   constexpr int ROWS = W * kWave / NVP;  // rows at once
+  constexpr int kAhead = W > 1 ? 4 : 8;
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   const int vec = tid % NVP, row0 = tid / NVP;
   const int h = static_cast<int>(blockIdx.x % p.H);
@@ -45,6 +73,9 @@ __global__ __launch_bounds__(W * kWave) void delta_step_kernel(const StepParams 
   __shared__ float red[2][W][NVP][8];
   __shared__ float red_qk[2][W];
   const bool col_ok = vec * 4 < p.dv;
+  uint32_t state_off[RPT];  // rows behind the last are behind the end of the state too
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) state_off[i] = col_ok ? ((row0 + i * ROWS) * p.dv + vec * 4) * 4 : kNowhere;
   const T* q = static_cast<const T*>(p.q);
   const T* k = static_cast<const T*>(p.k);
   const T* v = static_cast<const T*>(p.v);
@@ -61,55 +92,87 @@ __global__ __launch_bounds__(W * kWave) void delta_step_kernel(const StepParams 
     return n < 0 ? 0 : (n > p.T ? p.T : n);
   };
   auto clear = [&](int b, int from) {
-    for (int64_t i = tid; i < static_cast<int64_t>(p.T - from) * p.dv; i += W * kWave)
-      o[b * p.os[0] + h * p.os[1] + (from + i / p.dv) * p.os[2] + i % p.dv] = static_cast<T>(0.f);
+    for (int t = from; t < p.T; ++t)
+      for (int c = tid; c < p.dv; c += W * kWave) o[b * p.os[0] + h * p.os[1] + t * p.os[2] + c] = static_cast<T>(0.f);
   };
   if (slot < 0 || slot >= p.pool) {
     clear(first, 0);
     return;
   }
   f32x4 s[RPT];
-  float* base = p.state + (slot * p.H + h) * static_cast<int64_t>(p.dk) * p.dv;
+  const uint32_t state_bytes = static_cast<uint32_t>(p.dk * p.dv) * 4;
+  const Buffer state = buffer_of(p.state + (slot * p.H + h) * static_cast<int64_t>(p.dk) * p.dv, state_bytes);
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    const int row = row0 + i * ROWS;
-    s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (col_ok && row < p.dk) s[i] = *reinterpret_cast<const f32x4*>(base + static_cast<int64_t>(row) * p.dv + vec * 4);
-  }
+  for (int i = 0; i < RPT; ++i) s[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(state, state_off[i], 0, 0));
+  // A token's inputs, requested one token ahead: the first beside the state, before the search for samples of the same slot.
+  Token<RPT> next;
+  auto request = [&](int b, int t) __attribute__((always_inline)) {
+    next.log_decay.request(p.log_decay, b * p.gs[0] + h * p.gs[1] + t * p.gs[2], p.gates_f32);
+    next.beta.request(p.beta, b * p.bs[0] + h * p.bs[1] + t * p.bs[2], p.gates_f32);
+    const uint32_t key_bytes = static_cast<uint32_t>(p.dk * sizeof(T));
+    const Buffer qt = buffer_of(q + b * p.qs[0] + hk * p.qs[1] + t * p.qs[2], key_bytes);
+    const Buffer kt = buffer_of(k + b * p.ks[0] + hk * p.ks[1] + t * p.ks[2], key_bytes);
+    const Buffer vt = buffer_of(v + b * p.vs[0] + h * p.vs[1] + t * p.vs[2], static_cast<uint32_t>(p.dv * sizeof(T)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) next.v[e] = read_bits<T>(vt, (vec * 4 + e) * sizeof(T));
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      next.k[i] = read_bits<T>(kt, (row0 + i * ROWS) * sizeof(T));
+      next.q[i] = read_bits<T>(qt, (row0 + i * ROWS) * sizeof(T));
+    }
+  };
+  request(first, 0);
   bool again = false;  // a later sample has the slot too
   if (p.slots != nullptr && p.B > 1) {
     bool before = false, after = false;
-    for (int j = tid; j < p.B; j += W * kWave)
-      if (j != first && slot_of(j) == slot) (j < first ? before : after) = true;
-    if (__syncthreads_or(before)) return;  // that sample's workgroup applies these tokens
-    again = __syncthreads_or(after);
+    const uint32_t bytes = p.slots_int64 ? 8 : 4, upper = p.slots_int64 ? 4 : 0;  // of four bytes the lower half stands for both
+    const Buffer slots = buffer_of(p.slots, p.B * bytes);
+    const uint32_t low = static_cast<uint32_t>(slot), high = p.slots_int64 ? static_cast<uint32_t>(slot >> 32) : low;
+    for (int j0 = tid; j0 < p.B; j0 += kAhead * W * kWave) {  // several reads in flight: one after the other they took as long as the state
+      uint32_t at_low[kAhead], at_high[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const uint32_t off = (j0 + i * W * kWave) * bytes;
+        at_low[i] = __builtin_amdgcn_raw_buffer_load_b32(slots, off, 0, 0);
+        at_high[i] = __builtin_amdgcn_raw_buffer_load_b32(slots, off + upper, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int j = j0 + i * W * kWave;
+        const bool same = (at_low[i] == low) & (at_high[i] == high) & (j < p.B);
+        before |= same & (j < first);
+        after |= same & (j > first);
+      }
+    }
+    if (__syncthreads_or(before | after)) {
+      if (__syncthreads_or(before)) return;  // that sample's workgroup applies these tokens
+      again = true;
+    }
   }
   bool touched = false;
   int round = 0;
   for (int b = first; b < p.B;) {
     const int n = length_of(b);
     for (int t = 0; t < n; ++t) {
-      const float a = expf(gate_at<T>(p.log_decay, b * p.gs[0] + h * p.gs[1] + t * p.gs[2], p.gates_f32));
-      const float beta = gate_at<T>(p.beta, b * p.bs[0] + h * p.bs[1] + t * p.bs[2], p.gates_f32);
-      const T* qt = q + b * p.qs[0] + hk * p.qs[1] + t * p.qs[2];
-      const T* kt = k + b * p.ks[0] + hk * p.ks[1] + t * p.ks[2];
-      const T* vt = v + b * p.vs[0] + h * p.vs[1] + t * p.vs[2];
-      float kr[RPT], vf[4] = {0.f, 0.f, 0.f, 0.f};
+      const float a = expf(next.log_decay.template value<T>(p.gates_f32)), beta = next.beta.template value<T>(p.gates_f32);
+      float kr[RPT], vf[4], qr[RPT];
       float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, qk = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col_ok) vf[e] = static_cast<float>(vt[vec * 4 + e]);
+      for (int e = 0; e < 4; ++e) vf[e] = from_bits<T>(next.v[e]);
 #pragma unroll
       for (int i = 0; i < RPT; ++i) {
-        const int row = row0 + i * ROWS;
-        kr[i] = row < p.dk ? static_cast<float>(kt[row]) : 0.f;
-        const float qr = row < p.dk ? static_cast<float>(qt[row]) : 0.f;
-        qk = fmaf(qr, kr[i], qk);
+        kr[i] = from_bits<T>(next.k[i]);
+        qr[i] = from_bits<T>(next.q[i]);
+      }
+      if (t + 1 < n) request(b, t + 1);
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        qk = fmaf(qr[i], kr[i], qk);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[i][e] *= a;
           sum[e] = fmaf(kr[i], s[i][e], sum[e]);
-          sum[4 + e] = fmaf(qr, s[i][e], sum[4 + e]);
+          sum[4 + e] = fmaf(qr[i], s[i][e], sum[4 + e]);
         }
       }
 #pragma unroll
@@ -154,13 +217,11 @@ __global__ __launch_bounds__(W * kWave) void delta_step_kernel(const StepParams 
     if (!again) break;
     for (++b; b < p.B && slot_of(b) != slot; ++b) {
     }
+    if (b < p.B) request(b, 0);
   }
   if (!touched) return;
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    const int row = row0 + i * ROWS;
-    if (col_ok && row < p.dk) *reinterpret_cast<f32x4*>(base + static_cast<int64_t>(row) * p.dv + vec * 4) = s[i];
-  }
+  for (int i = 0; i < RPT; ++i) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, s[i]), state, state_off[i], 0, 0);
 }
 
 template <typename T, int NVP, int W, int RPT>
@@ -228,6 +289,7 @@ extern "C" int taac_delta_rule_step(const void* q, const void* k, const void* v,
   if (gate_dtype != dtype && gate_dtype != TAAC_F32)
     return set_error(TAAC_ERR_INVALID_VALUE, "%s: gates must be fp32 or of the tokens' dtype", name);
   if (slots == nullptr && B > pool) return set_error(TAAC_ERR_INVALID_VALUE, "%s: %d samples without slots and a pool of %lld", name, B, (long long)pool);
+  if (B > 1 << 28) return set_error(TAAC_ERR_UNSUPPORTED, "%s: at most 2^28 samples", name);  // 32-bit offsets into the slots
   if (static_cast<int64_t>(B) * H > 0x7fffffffLL) return set_error(TAAC_ERR_UNSUPPORTED, "%s: too many workgroups", name);
   if (B == 0 || T == 0) return TAAC_OK;
   if (!q || !k || !v || !log_decay || !beta || !o || (pool > 0 && !state)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: null tensor pointer", name);
