@@ -178,12 +178,21 @@ struct Tile {
     static constexpr int PIECES = WIDTH / 8, COUNT = (ROWS * PIECES + THREADS - 1) / THREADS;
     bf16x8 v[COUNT];
     __device__ __forceinline__ void load(const bf16_t* src, int64_t ld, int n, int width, int tid) {
+      static_assert(THREADS % PIECES == 0);
+      const Buffer rows = rows_buffer(src, ld, n, width);
+      const int row = tid / PIECES, piece = tid % PIECES;
+      const uint32_t pitch = static_cast<uint32_t>(ld) * 2, off = piece * 8 < width ? row * pitch + piece * 16 : kNowhere;
 #pragma unroll
-      for (int i = 0; i < COUNT; ++i) {
-        const int row = (tid + i * THREADS) / PIECES, piece = (tid + i * THREADS) % PIECES;
-        v[i] = zero8();
-        if (row < n && row < ROWS && piece * 8 < width) v[i] = *reinterpret_cast<const bf16x8*>(src + row * ld + piece * 8);
-      }
+      for (int i = 0; i < COUNT; ++i) v[i] = read8(rows, off + i * (THREADS / PIECES) * pitch);
+    }
+    // the sum of the products of this lane's elements with those of another piece
+    __device__ __forceinline__ float dot(const Piece& other) const {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(static_cast<float>(v[i][e]), static_cast<float>(other.v[i][e]), sum);
+      return sum;
     }
     // PAIRED: row 8 g + e of a block of 32 goes to row 4 g + e (e < 4) or 12 + 4 g + e, so that a keys_frag() over the rows has them in order
     template <bool PAIRED = false>

@@ -110,6 +110,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 64 && DV <= 64 ? 2 : 1) void delta
     n_in.load(p.misses + (unit * p.T + token0) * p.dv, p.dv, n_tok, p.dv, tid);
     s_in.load(p.chunk_states + at_state, p.dk, p.dv, p.dk, tid);
     g_in.load(p.grad_states + at_state, p.dk, p.dv, p.dk, tid);
+    float dot_state = s_in.dot(g_in);
     __syncthreads();  // the previous head's tiles and sums are no longer read
     if (wave == 0) chunk_rows(p, b, h, token0, n_tok, rows, temp, left_over);
     o_in.store(tile_o, tid);
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 64 && DV <= 64 ? 2 : 1) void delta
     };
     // The sums of the pairs' contributions to dG over a row and over a column are taken from the same fp32 values: pairs on one side of a
     // token then cancel in dg as they do in the formula.
-    float dot_row = 0.f, dot_col = 0.f, dot_tail = 0.f, dot_state = 0.f;
+    float dot_row = 0.f, dot_col = 0.f, dot_tail = 0.f;
     bf16x8 b_hi[2], b_lo[2], e_hi[2], e_lo[2];
     bf16x8 first[VB], second[VB], third[KA / 2], fourth[KA / 2];
     // this wavefront's tokens as i: dQ and R
@@ -260,11 +261,6 @@ __global__ __launch_bounds__(4 * kWave, DK <= 64 && DV <= 64 ? 2 : 1) void delta
       for (int vb = 0; vb < VB; ++vb) {
         const bf16x8 gf = TK::keys_frag(tile_g, vb, a, l16, grp);
         dc = mfma16(gf, first[vb], dc);
-        if (a % 4 == wave) {
-          const bf16x8 sf = TK::keys_frag(tile_s, vb, a, l16, grp);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) dot_state = fmaf(static_cast<float>(sf[e]), static_cast<float>(gf[e]), dot_state);
-        }
       }
       const bf16x4 kv = *reinterpret_cast<const bf16x4*>(tile_k + row * TK::STRIDE + state_row(a, 4 * grp));
 #pragma unroll
