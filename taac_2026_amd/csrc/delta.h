@@ -129,9 +129,9 @@ __device__ __forceinline__ void put_offset(T* base, uint32_t bytes, const V& v) 
   *reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(base) + bytes) = v;
 }
 
-// Reads through a buffer descriptor: bytes at or beyond its end read as zero without touching memory, so that rows behind the last token
-// need neither a branch nor a mask. kNowhere: an offset behind every end (64 rows
-// of less than 2^24 elements end below it), so also for features or columns that there are not.
+// Reads and writes through a buffer descriptor: bytes at or beyond its end read as zero and are not written, so that rows behind the last
+// token need neither a branch nor a mask, and a wait for one read counts everything requested since. kNowhere: an offset behind every end (64
+// rows of less than 2^24 elements end below it), so also for features or columns that there are not.
 typedef __amdgpu_buffer_rsrc_t Buffer;
 constexpr uint32_t kNowhere = 0x80000000u;
 __device__ __forceinline__ Buffer buffer_of(const void* base, uint32_t bytes) {
@@ -143,6 +143,10 @@ __device__ __forceinline__ Buffer rows_buffer(const bf16_t* base, int64_t ld, in
 }
 __device__ __forceinline__ bf16x8 read8(Buffer b, uint32_t off) {
   return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+}
+__device__ __forceinline__ void write4(Buffer b, uint32_t off, const u32x2& v) { __builtin_amdgcn_raw_buffer_store_b64(v, b, off, 0, 0); }
+__device__ __forceinline__ void write8(Buffer b, uint32_t off, const bf16x8& v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), b, off, 0, 0);
 }
 __device__ __forceinline__ uint32_t read1(Buffer b, uint32_t off) {
   return static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(b, off, 0, 0));

@@ -29,7 +29,7 @@ constexpr int kSoloHi = 0, kSoloLow = 64, kSoloBeta = 128, kSoloIn = 192, kSoloO
 template <int DK>
 struct SoloTokens {
   bf16x8 kf[4][DK / 32], qf[4][DK / 32], x[4];  // x: pieces of the values (backward: of dO)
-  float g, beta;
+  uint32_t g[2], beta[2];                       // by halves: a branch between fp32 and bf16 would await each
 };
 
 template <int DK, bool BACK>
@@ -41,7 +41,7 @@ struct Solo {
   int lane, l16, grp, col0, h, b, len, groups;
   int64_t unit;
   const bf16_t *k0, *q0, *x0;
-  uint32_t k_off, q_off, x_off;
+  uint32_t k_off[KB], q_off[KB], state_off[KB], x_off;
   int64_t x_ld;
 
   __device__ __forceinline__ Solo(const DeltaParams& params) : p(params) {
@@ -64,55 +64,54 @@ struct Solo {
     k0 = p.k + b * p.ks[0] + hk * p.ks[1];
     q0 = p.q + b * p.qs[0] + hk * p.qs[1];
     x0 = (BACK ? p.grad_o : p.v) + b * xs[0] + h * xs[1] + col0;
-    k_off = static_cast<uint32_t>(l16 * p.ks[2] + grp * 8) * 2;
-    q_off = static_cast<uint32_t>(l16 * p.qs[2] + grp * 8) * 2;
-    // pieces behind the last read the last one: their columns are not stored and meet no other column
-    const int last = (p.dv - col0) / 8 - 1, piece = lane % 4;
-    x_off = static_cast<uint32_t>(lane / 4 * x_ld + (piece < last ? piece : last) * 8) * 2;
+    const uint32_t k_ld = static_cast<uint32_t>(p.ks[2]) * 2, q_ld = static_cast<uint32_t>(p.qs[2]) * 2;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const bool there = kb * 32 + grp * 8 < p.dk;
+      k_off[kb] = there ? l16 * k_ld + kb * 64 + grp * 16 : kNowhere;
+      q_off[kb] = there ? l16 * q_ld + kb * 64 + grp * 16 : kNowhere;
+      state_off[kb] = there ? static_cast<uint32_t>(l16 * p.dk + 32 * kb + 8 * grp) * 2 : kNowhere;
+    }
+    const int piece = lane % 4;
+    x_off = col0 + piece * 8 < p.dv ? static_cast<uint32_t>(lane / 4 * x_ld) * 2 + piece * 16 : kNowhere;
   }
   __device__ __forceinline__ int tokens_of(int group) const {
     const int left = len - group * kChunk;
     return left < kChunk ? left : kChunk;
   }
 
+  // Beside the tokens of a group; of a group that there is not, nothing (zeros).
   __device__ __forceinline__ void fetch(int group, SoloTokens<DK>& c) const {
-    const int64_t token0 = static_cast<int64_t>(group) * kChunk;
-    const int n_tok = tokens_of(group);
+    const int n_tok = group >= 0 ? tokens_of(group) : 0;
+    const int64_t token0 = n_tok > 0 ? static_cast<int64_t>(group) * kChunk : 0;
     const bf16_t *k = k0 + token0 * p.ks[2], *q = q0 + token0 * p.qs[2], *x = x0 + token0 * x_ld;
-    c.g = c.beta = 0.f;
-    if (lane < n_tok) {
-      c.g = load_gate(p.log_decay, b * p.gs[0] + h * p.gs[1] + (token0 + lane) * p.gs[2], p.gates_f32);
-      c.beta = load_gate(p.beta, b * p.bs[0] + h * p.bs[1] + (token0 + lane) * p.bs[2], p.gates_f32);
+    const int64_t token = lane < n_tok ? token0 + lane : 0;
+    const int64_t at_g = b * p.gs[0] + h * p.gs[1] + token * p.gs[2], at_beta = b * p.bs[0] + h * p.bs[1] + token * p.bs[2];
+    const uint16_t *g = static_cast<const uint16_t*>(p.log_decay) + (at_g << p.gates_f32), *beta = static_cast<const uint16_t*>(p.beta) + (at_beta << p.gates_f32);
+    c.g[0] = g[0], c.g[1] = g[p.gates_f32];
+    c.beta[0] = beta[0], c.beta[1] = beta[p.gates_f32];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const Buffer kt = rows_buffer(k + t * 16 * p.ks[2], p.ks[2], n_tok - 16 * t, p.dk);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) c.kf[t][kb] = read8(kt, k_off[kb]);
     }
-    if (n_tok == kChunk && p.dk == DK) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 4; ++t) c.x[t] = read8(rows_buffer(x + t * 16 * x_ld, x_ld, n_tok - 16 * t, p.dv - col0), x_off);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          c.kf[t][kb] = at_offset<bf16x8>(k + t * 16 * p.ks[2] + kb * 32, k_off);
-          c.qf[t][kb] = at_offset<bf16x8>(q + t * 16 * p.qs[2] + kb * 32, q_off);
-        }
-        c.x[t] = at_offset<bf16x8>(x + t * 16 * x_ld, x_off);
-      }
-    } else {
+    for (int t = 0; t < 4; ++t) {
+      const Buffer qt = rows_buffer(q + t * 16 * p.qs[2], p.qs[2], n_tok - 16 * t, p.dk);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          c.kf[t][kb] = c.qf[t][kb] = zero8();
-          if (16 * t + l16 < n_tok && kb * 32 + grp * 8 < p.dk) {
-            c.kf[t][kb] = at_offset<bf16x8>(k + t * 16 * p.ks[2] + kb * 32, k_off);
-            c.qf[t][kb] = at_offset<bf16x8>(q + t * 16 * p.qs[2] + kb * 32, q_off);
-          }
-        }
-        c.x[t] = zero8();
-        if (16 * t + lane / 4 < n_tok) c.x[t] = at_offset<bf16x8>(x + t * 16 * x_ld, x_off);
-      }
+      for (int kb = 0; kb < KB; ++kb) c.qf[t][kb] = read8(qt, q_off[kb]);
     }
+  }
+  __device__ __forceinline__ float gate(const uint32_t (&bits)[2], bool live) const {
+    const float v = __builtin_bit_cast(float, bits[1] << 16 | (p.gates_f32 ? bits[0] : 0));  // a bf16 is the upper half of a float
+    return live ? v : 0.f;
   }
 
   // The tokens' factors and rows into LDS.
-  __device__ __forceinline__ void place(const SoloTokens<DK>& c, float* rows, bf16_t* tile_k, bf16_t* tile_x) const {
+  __device__ __forceinline__ void place(const SoloTokens<DK>& c, int n_tok, float* rows, bf16_t* tile_k, bf16_t* tile_x) const {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
@@ -122,7 +121,8 @@ struct Solo {
       }
       *reinterpret_cast<bf16x8*>(tile_x + (16 * t + lane / 4) * TV::STRIDE + (lane % 4) * 8) = c.x[t];
     }
-    const float g = c.g < -1e5f ? -1e5f : c.g;  // a decay of zero, finite in the sums
+    const float given = gate(c.g, lane < n_tok), beta = gate(c.beta, lane < n_tok);
+    const float g = given < -1e5f ? -1e5f : given;  // a decay of zero, finite in the sums
     double total = static_cast<double>(g) * 1.4426950408889634;
 #pragma unroll
     for (int off = 1; off < kWave; off *= 2) {
@@ -137,11 +137,11 @@ struct Solo {
     const float grown = __builtin_amdgcn_exp2f(hi);
     rows[kSoloHi + lane] = hi;
     rows[kSoloLow + lane] = static_cast<float>(total - half_start - static_cast<double>(hi));
-    rows[kSoloBeta + lane] = c.beta;
+    rows[kSoloBeta + lane] = beta;
     rows[kSoloIn + lane] = __builtin_amdgcn_exp2f(static_cast<float>(total - tile_start));
-    rows[kSoloOut + lane] = __builtin_amdgcn_exp2f(static_cast<float>(tile_end - total)) * c.beta;
+    rows[kSoloOut + lane] = __builtin_amdgcn_exp2f(static_cast<float>(tile_end - total)) * beta;
     rows[kSoloGrown + lane] = grown;
-    rows[kSoloKeep + lane] = __builtin_amdgcn_exp2f(static_cast<float>(half_end - total)) * c.beta;
+    rows[kSoloKeep + lane] = __builtin_amdgcn_exp2f(static_cast<float>(half_end - total)) * beta;
     if ((lane & 31) == 31) rows[kSoloTotal + lane / 32] = grown;
     wave_sync();
   }
@@ -264,18 +264,16 @@ struct Solo {
   }
   // the state's high parts at dst [dv][dk]
   __device__ __forceinline__ void store_state(bf16_t* dst, const bf16x8 (&sh)[KB][kNT]) const {
-    const uint32_t off = static_cast<uint32_t>((col0 + l16) * p.dk + 8 * grp) * 2;
 #pragma unroll
-    for (int n = 0; n < kNT; ++n)
-      if (col0 + 16 * n + l16 < p.dv) {
+    for (int n = 0; n < kNT; ++n) {
+      const Buffer to = rows_buffer(dst + (col0 + 16 * n) * p.dk, p.dk, p.dv - col0 - 16 * n, p.dk);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-          if (p.dk == DK || 32 * kb + 8 * grp < p.dk) put_offset(dst + 16 * n * p.dk + 32 * kb, off, sh[kb][n]);
-      }
+      for (int kb = 0; kb < KB; ++kb) write8(to, state_off[kb], sh[kb][n]);
+    }
   }
-  // Rows of one chunk of 32 tokens, held by columns, at dst (its row 0, this wavefront's first column): turned through tile's rows, which
-  // have been read.
-  __device__ __forceinline__ void store_rows(bf16_t* dst, int64_t ld, uint32_t off, bf16_t* tile, const f32x4 (&x)[2][kNT], int n_tok) const {
+  // Rows of one chunk of 32 tokens, held by columns, at dst (its row 0, this wavefront's first column; off: quads()): turned through tile's rows,
+  // which have been read.
+  __device__ __forceinline__ void store_rows(bf16_t* dst, int64_t ld, const uint32_t (&off)[kNT], bf16_t* tile, const f32x4 (&x)[2][kNT], int n_tok) const {
     u32x2 v[2][kNT];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -288,10 +286,17 @@ struct Solo {
       for (int n = 0; n < kNT; ++n)
         v[t][n] = __builtin_bit_cast(u32x2, TV::read_tr(tile + (2 * t + n) * 320 + (4 * grp + l16 / 4) * 20 + (l16 % 4) * 4));
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
+      const Buffer to = rows_buffer(dst + 16 * t * ld, ld, n_tok - 16 * t, p.dv - col0);
 #pragma unroll
-      for (int n = 0; n < kNT; ++n)
-        if (16 * t + l16 < n_tok && col0 + 16 * n + 4 * grp < p.dv) put_offset(dst + 16 * t * ld + 16 * n, off, v[t][n]);
+      for (int n = 0; n < kNT; ++n) write4(to, off[n], v[t][n]);
+    }
+  }
+  // Byte offsets of four columns of token l16 in rows ld elements apart.
+  __device__ __forceinline__ void quads(int64_t ld, uint32_t (&off)[kNT]) const {
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+      off[n] = col0 + 16 * n + 4 * grp < p.dv ? static_cast<uint32_t>(l16 * ld + 16 * n + 4 * grp) * 2 : kNowhere;
   }
 };
 
@@ -311,8 +316,9 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
   const W w(p);
   const int lane = w.lane, l16 = w.l16, grp = w.grp, col0 = w.col0;
   bf16_t* o0 = p.o + w.b * p.os[0] + w.h * p.os[1] + col0;
-  const uint32_t o_off = static_cast<uint32_t>(l16 * p.os[2] + 4 * grp) * 2;
-  const uint32_t n_off = static_cast<uint32_t>(l16 * p.dv + 4 * grp) * 2;
+  uint32_t o_off[kNT], n_off[kNT];
+  w.quads(p.os[2], o_off);
+  w.quads(p.dv, n_off);
 
   f32x4 s[KA][kNT];
 #pragma unroll
@@ -335,11 +341,11 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
     const int64_t token0 = static_cast<int64_t>(group) * kChunk;
     const int n_tok = w.tokens_of(group);
     wave_sync();  // the previous tokens' tiles are read
-    w.place(c, rows, tile_k, tile_v);
+    w.place(c, n_tok, rows, tile_k, tile_v);
     bf16x8 mh[4], ml[4];
     w.solve(c, rows, scratch, mh, ml);
     w.place_queries(c, tile_q);
-    if (group + 1 < w.groups) w.fetch(group + 1, c);
+    w.fetch(group + 1, c);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (half == 1 && n_tok <= kHalf) break;
@@ -408,14 +414,13 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
 #pragma unroll
           for (int n = 0; n < kNT; ++n) out[n] = mfma16(sl[kb][n], qf[kb], mfma16(sh[kb][n], qf[kb], out[n]));
         const float grown = rows[kSoloGrown + 16 * ti + l16] * p.scale;
+        const Buffer to = rows_buffer(o0 + (token0 + 16 * ti) * p.os[2], p.os[2], n_tok - 16 * ti, p.dv - col0);
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) out[n][r] *= grown;
           out[n] = mfma16(xl[n], pf, mfma16(xh[n], pf, out[n]));
-          if (16 * ti + l16 < n_tok && col0 + 16 * n + 4 * grp < p.dv) {
-            put_offset(o0 + (token0 + 16 * ti) * p.os[2] + 16 * n, o_off, round4(out[n]));
-          }
+          write4(to, o_off[n], round4(out[n]));
         }
       }
       // S' = e^G_last S + K^T (beta e^(G_last - G) N)
@@ -478,7 +483,8 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
   const W w(p);
   const int lane = w.lane, l16 = w.l16, grp = w.grp, col0 = w.col0;
   bf16_t* v0 = p.grad_v + w.b * p.dvs[0] + w.h * p.dvs[1] + col0;
-  const uint32_t v_off = static_cast<uint32_t>(l16 * p.dvs[2] + 4 * grp) * 2;
+  uint32_t v_off[kNT];
+  w.quads(p.dvs[2], v_off);
 
   f32x4 s[KA][kNT];
 #pragma unroll
@@ -492,11 +498,11 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
     const int64_t token0 = static_cast<int64_t>(group) * kChunk;
     const int n_tok = w.tokens_of(group);
     wave_sync();
-    w.place(c, rows, tile_k, tile_o);
+    w.place(c, n_tok, rows, tile_k, tile_o);
     bf16x8 mh[4], ml[4];
     w.solve(c, rows, scratch, mh, ml);
     w.place_queries(c, tile_q);
-    if (group > 0) w.fetch(group - 1, c);
+    w.fetch(group - 1, c);
 #pragma unroll
     for (int back = 0; back < 2; ++back) {
       const int half = 1 - back;
