@@ -141,8 +141,16 @@ __device__ __forceinline__ Buffer buffer_of(const void* base, uint32_t bytes) {
 __device__ __forceinline__ Buffer rows_buffer(const bf16_t* base, int64_t ld, int n, int width) {
   return buffer_of(base, n > 0 ? static_cast<uint32_t>((n - 1) * ld + width) * 2 : 0);
 }
-__device__ __forceinline__ bf16x8 read8(Buffer b, uint32_t off) {
-  return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+// off: of the lane; further: the same for all lanes.
+__device__ __forceinline__ bf16x8 read8(Buffer b, uint32_t off, uint32_t further = 0) {
+  return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(b, off, further, 0));
+}
+__device__ __forceinline__ f32x4 read_floats(Buffer b, uint32_t off, uint32_t further = 0) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(b, off, further, 0));
+}
+__device__ __forceinline__ u32x2 read4(Buffer b, uint32_t off) { return __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0); }
+__device__ __forceinline__ float read_float(Buffer b, uint32_t off, uint32_t further = 0) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(b, off, further, 0));
 }
 __device__ __forceinline__ void write4(Buffer b, uint32_t off, const u32x2& v) { __builtin_amdgcn_raw_buffer_store_b64(v, b, off, 0, 0); }
 __device__ __forceinline__ void write8(Buffer b, uint32_t off, const bf16x8& v) {

@@ -56,31 +56,33 @@ struct TeamLds {  // fragments hi, then lo, of each
 };
 
 // What wavefront w needs of a chunk. Several of them take turns, so that nothing is copied.
-template <int KB, bool COLS>
+constexpr int kTeamRow = 20;  // elements of a token's 16 columns in LDS
+
+template <int KB>
 struct TeamChunk {
   bf16x8 kf[KB], qf[KB];
   bf16x8 mh[2], ml[2], pf[2];
   f32x4 grown, keep;
   float grown_row, total;
-  // bits of a column's values: V (backward: dO) of the four own tokens of this lane; backward, dO of eight tokens per block of 32
-  uint32_t x[4], of[COLS ? 16 : 1];
+  u32x2 x;  // four columns of a token of V (backward: of dO), on their way into LDS
 };
 
 template <int DK, bool COLS>
 struct Team {
   static constexpr int KB = DK / 32, KA = DK / 16, OWN = KA >= 4 ? KA / 4 : 1;  // OWN: state tiles of a wavefront
-  typedef TeamChunk<KB, COLS> Chunk;
+  typedef TeamChunk<KB> Chunk;
   const DeltaParams& p;
   int wave, lane, l16, grp, col0, h, b, len, chunks;
   int64_t unit;
   bool col_ok, owner;
   // The chunk that is requested next: uniform pointers that move by whole chunks, and byte offsets of this lane that stay (token strides are
   // below 2^24 elements), so that a request costs no arithmetic.
-  const bf16_t *k_at, *q_at, *x_at;
-  const uint8_t* block_at;
+  const uint8_t *k_at, *q_at, *x_at, *block_at;
   int64_t k_step, q_step, x_step;
-  int at;
-  uint32_t k_off[KB], q_off[KB], x_off[4], of_off[COLS ? 16 : 1], frag_off[2], row_off;
+  int32_t k_ld, q_ld, x_ld, k_less, q_less, x_less;  // bytes from row to row, and what a row is short of that
+  int at, n_at;
+  Buffer block;
+  uint32_t k_off[KB], q_off[KB], x_off, frag_off[2], row_off;
 
   __device__ __forceinline__ Team(const DeltaParams& params) : p(params) {
     const int tid = threadIdx.x;
@@ -103,29 +105,22 @@ struct Team {
     const int64_t* xs = COLS ? p.dos : p.vs;
     at = COLS ? chunks - 1 : 0;
     const int64_t first = static_cast<int64_t>(at) * kChunk;
-    k_at = p.k + b * p.ks[0] + hk * p.ks[1] + first * p.ks[2];
-    q_at = p.q + b * p.qs[0] + hk * p.qs[1] + first * p.qs[2];
-    x_at = (COLS ? p.grad_o : p.v) + b * xs[0] + h * xs[1] + col0 + first * xs[2];
+    k_at = reinterpret_cast<const uint8_t*>(p.k + b * p.ks[0] + hk * p.ks[1] + first * p.ks[2]);
+    q_at = reinterpret_cast<const uint8_t*>(p.q + b * p.qs[0] + hk * p.qs[1] + first * p.qs[2]);
+    x_at = reinterpret_cast<const uint8_t*>((COLS ? p.grad_o : p.v) + b * xs[0] + h * xs[1] + col0 + first * xs[2]);
     block_at = p.blocks + (unit * p.chunks + at) * kBlockBytes;
-    constexpr int64_t kMove = COLS ? -kChunk : kChunk;
+    constexpr int64_t kMove = (COLS ? -kChunk : kChunk) * 2;
     k_step = kMove * p.ks[2], q_step = kMove * p.qs[2], x_step = kMove * xs[2];
+    k_ld = static_cast<int32_t>(p.ks[2]) * 2, q_ld = static_cast<int32_t>(p.qs[2]) * 2, x_ld = static_cast<int32_t>(xs[2]) * 2;
+    k_less = k_ld - p.dk * 2, q_less = q_ld - p.dk * 2, x_less = x_ld - (p.dv - col0) * 2;
     owner = wave * OWN < KA;
-    const uint32_t k_ld = static_cast<uint32_t>(p.ks[2]) * 2, q_ld = static_cast<uint32_t>(p.qs[2]) * 2, x_ld = static_cast<uint32_t>(xs[2]) * 2;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const uint32_t feature = static_cast<uint32_t>(32 * kb + 8 * grp);
       k_off[kb] = feature < static_cast<uint32_t>(p.dk) ? (16 * wave + l16) * k_ld + feature * 2 : kNowhere;
       q_off[kb] = feature < static_cast<uint32_t>(p.dk) ? (16 * wave + l16) * q_ld + feature * 2 : kNowhere;
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) x_off[r] = col_ok ? (16 * wave + 4 * grp + r) * x_ld + l16 * 2 : kNowhere;
-    if (COLS) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {  // dO in front of the own tile is not needed
-        const int row = 32 * (i / 8) + 16 * (i / 4 % 2) + i % 4;
-        of_off[i] = col_ok && row / 16 >= wave ? (row + 4 * grp) * x_ld + l16 * 2 : kNowhere;
-      }
-    }
+    x_off = col0 + lane % 4 * 4 < p.dv ? (16 * wave + lane / 4) * x_ld + lane % 4 * 8 : kNowhere;
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk)
       frag_off[tk] = (COLS ? tk >= wave / 2 : tk <= wave / 2) ? (COLS ? frag_cols(wave, tk) : frag_rows(wave, tk)) * kFrag + lane * 16 : kNowhere;
@@ -136,45 +131,51 @@ struct Team {
     return left < kChunk ? left : kChunk;
   }
 
-  // The requests for a chunk (behind the last one: that one again), in three parts that the stages of the chunk before it issue beside their
-  // work: in one run they would wait for each other in front of it. No branch around them, so that what was requested before can be
-  // awaited without awaiting these.
-  __device__ __forceinline__ void fetch_keys(Chunk& c) const {
-    const int n = tokens_of(at);
-    const Buffer k = rows_buffer(k_at, p.ks[2], n, p.dk), x = rows_buffer(x_at, COLS ? p.dos[2] : p.vs[2], n, p.dv - col0);
+  // The first n rows at a base; none where n is not positive.
+  static __device__ __forceinline__ Buffer rows_at(const uint8_t* base, int n, int32_t ld, int32_t less) {
+    const int32_t bytes = n * ld - less;
+    return buffer_of(base, bytes > 0 ? bytes : 0);
+  }
+
+  // The requests for a chunk (behind the last one: zeros), in three parts that the stages of the chunk before it issue beside their work:
+  // in one run they would wait for each other in front of it. No branch around them, so that what was requested before can be awaited
+  // without awaiting these.
+  __device__ __forceinline__ void fetch_keys(Chunk& c) {
+    n_at = !COLS || at >= 0 ? tokens_of(at) : 0;
+    block = buffer_of(block_at, n_at > 0 ? kBlockBytes : 0);
+    const Buffer k = rows_at(k_at, n_at, k_ld, k_less), x = rows_at(x_at, n_at, x_ld, x_less);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) c.kf[kb] = read8(k, k_off[kb]);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) c.x[r] = read1(x, x_off[r]);
-    if (COLS) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) c.of[i] = read1(x, of_off[i]);
-    }
-    const uint8_t* rows = block_at + kBlockRows;
-    c.grown = at_offset<f32x4>(rows + kRowGrown * 4, row_off);
-    c.keep = at_offset<f32x4>(rows + kRowKeep * 4, row_off);
-    if (!COLS) c.grown_row = at_offset<float>(rows + kRowGrown * 4 + wave * 64, l16 * 4);
-    c.total = at_offset<float>(rows + kRowTotal * 4, 0);
+    c.x = read4(x, x_off);
+    c.grown = read_floats(block, row_off, kBlockRows + kRowGrown * 4);
+    c.keep = read_floats(block, row_off, kBlockRows + kRowKeep * 4);
+    if (!COLS) c.grown_row = read_float(block, l16 * 4 + wave * 64, kBlockRows + kRowGrown * 4);
+    c.total = read_float(block, 0, kBlockRows + kRowTotal * 4);
   }
   __device__ __forceinline__ void fetch_queries(Chunk& c) const {
-    const Buffer q = rows_buffer(q_at, p.qs[2], tokens_of(at), p.dk);
+    const Buffer q = rows_at(q_at, n_at, q_ld, q_less);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) c.qf[kb] = read8(q, q_off[kb]);
   }
   // the last part, then on to the next chunk
   __device__ __forceinline__ void fetch_block(Chunk& c) {
-    const Buffer high = buffer_of(block_at + kBlockM, 6 * kFrag), low = buffer_of(block_at + kBlockLow, 6 * kFrag),
-                 score = buffer_of(block_at + kBlockP, 6 * kFrag);
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk) {
-      c.mh[tk] = read8(high, frag_off[tk]);
-      c.ml[tk] = read8(low, frag_off[tk]);
-      c.pf[tk] = read8(score, frag_off[tk]);
+      c.mh[tk] = read8(block, frag_off[tk], kBlockM);
+      c.ml[tk] = read8(block, frag_off[tk], kBlockLow);
+      c.pf[tk] = read8(block, frag_off[tk], kBlockP);
     }
-    const bool more = COLS ? at > 0 : at + 1 < chunks;
-    at += more ? (COLS ? -1 : 1) : 0;
-    k_at += more ? k_step : 0, q_at += more ? q_step : 0, x_at += more ? x_step : 0;
-    block_at += more ? (COLS ? -kBlockBytes : kBlockBytes) : 0;
+    at += COLS ? -1 : 1;
+    k_at += k_step, q_at += q_step, x_at += x_step;
+    block_at += COLS ? -kBlockBytes : kBlockBytes;
+  }
+
+  // The 16 columns of V (dO) in LDS, token by token: written behind a chunk's last use of them, read by columns.
+  __device__ __forceinline__ void place(const Chunk& c, bf16_t* tile_x) const {
+    *reinterpret_cast<u32x2*>(tile_x + (16 * wave + lane / 4) * kTeamRow + lane % 4 * 4) = c.x;
+  }
+  __device__ __forceinline__ bf16x4 values(const bf16_t* tile_x, int token0) const {  // tokens token0 + 4 grp .. of column l16
+    return Tile<DK>::read_tr(tile_x + (token0 + 4 * grp + l16 / 4) * kTeamRow + l16 % 4 * 4);
   }
 
   // The own rows of the state, bf16, at dst [dv][dk]
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
   typedef Tile<DK> TK;
   constexpr int KB = M::KB, OWN = M::OWN;
   __shared__ __attribute__((aligned(64))) uint8_t smem[L::kForward];
-  __shared__ __attribute__((aligned(16))) bf16_t turned[TRAIN ? 4 : 1][320];
+  __shared__ __attribute__((aligned(16))) bf16_t turned[TRAIN ? 4 : 1][320], tile_x[kChunk * kTeamRow];
   bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK);
   uint8_t *s_frags = smem + L::kState, *x_frags = smem + L::kX, *n_frags = smem + L::kN, *w_frags = smem + L::kW;
   M m(p);
@@ -246,8 +247,9 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
     for (int kb = 0; kb < KB; ++kb)
       *reinterpret_cast<bf16x8*>(tile_k + (16 * wave + l16) * TK::STRIDE + kb * 32 + grp * 8) = cur.kf[kb];
     f32x4 x;
+    const bf16x4 v = m.values(tile_x, 16 * wave);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = fmaf(-cur.grown[r], y[r] + y2[r], __builtin_bit_cast(float, cur.x[r] << 16));
+    for (int r = 0; r < 4; ++r) x[r] = fmaf(-cur.grown[r], y[r] + y2[r], static_cast<float>(v[r]));
     put_half(x_frags, wave, lane, x, 2 * kFrag);
     __syncthreads();
     m.fetch_queries(next);
@@ -320,6 +322,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
       put_offset(o_at, o_off, round4(out));
     }
     o_at += kChunk * p.os[2];
+    m.place(next, tile_x);
     __syncthreads();
   };
   typename M::Chunk even, odd;
@@ -327,6 +330,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
     m.fetch_keys(even);
     m.fetch_queries(even);
     m.fetch_block(even);
+    m.place(even, tile_x);
   }
   __syncthreads();
   // Pairs, then the odd one: a way past the second half back to the first would have to await the requests of the wrong one.
@@ -362,7 +366,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
   typedef Tile<DK> TK;
   constexpr int KB = M::KB, OWN = M::OWN;
   __shared__ __attribute__((aligned(64))) uint8_t smem[L::kBackward];
-  __shared__ __attribute__((aligned(16))) bf16_t turned[4][320];
+  __shared__ __attribute__((aligned(16))) bf16_t turned[4][320], tile_x[kChunk * kTeamRow];
   bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK);
   bf16_t* tile_q = reinterpret_cast<bf16_t*>(smem + L::kTileQ);
   uint8_t *s_frags = smem + L::kState, *z_frags = smem + L::kX, *x_frags = smem + L::kN, *o_frags = smem + L::kW;
@@ -396,10 +400,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk)
       if (tk >= wave / 2) {
-        u32x4 of;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) of[e] = cur.of[8 * tk + 2 * e] | cur.of[8 * tk + 2 * e + 1] << 16;
-        z3 = mfma16(cur.pf[tk], __builtin_bit_cast(bf16x8, of), z3);
+        z3 = mfma16(cur.pf[tk], TK::join(m.values(tile_x, 32 * tk), m.values(tile_x, 32 * tk + 16)), z3);
       }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
@@ -408,10 +409,11 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
       *reinterpret_cast<bf16x8*>(tile_q + at) = cur.qf[kb];
     }
     f32x4 w;
+    const bf16x4 own = m.values(tile_x, 16 * wave);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       z[r] = fmaf(cur.keep[r], z[r] + z2[r], z3[r]);
-      w[r] = p.scale * cur.grown[r] * __builtin_bit_cast(float, cur.x[r] << 16);
+      w[r] = p.scale * cur.grown[r] * static_cast<float>(own[r]);
     }
     put_half(z_frags, wave, lane, z, 2 * kFrag);
     put_half(o_frags, wave, lane, w, 2 * kFrag);
@@ -461,6 +463,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
         put_half(s_frags, a, lane, s[i], KB * kFrag);
       }
     }
+    m.place(next, tile_x);
     __syncthreads();
   };
   typename M::Chunk even, odd;
@@ -468,6 +471,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
     m.fetch_keys(even);
     m.fetch_queries(even);
     m.fetch_block(even);
+    m.place(even, tile_x);
   }
   __syncthreads();
   int chunk = m.chunks - 1;  // pairs, then the odd one, as above
