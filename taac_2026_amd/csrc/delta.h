@@ -57,7 +57,7 @@ struct DeltaParams {
 
 int delta_check(const char* name, const DeltaParams& p);
 // The form for few heads (delta_team.hip): bytes of its blocks, 0 where the other form is the faster one.
-int64_t delta_team_bytes(int64_t heads, int32_t T, int32_t dv);
+int64_t delta_team_bytes(int64_t heads, int32_t T, int32_t dk, int32_t dv);
 int delta_team_fwd(const char* name, const DeltaParams& p, hipStream_t s);
 int delta_team_back(const char* name, const DeltaParams& p, hipStream_t s);
 // The form for many heads of at most 64 key features (delta_solo.hip).

@@ -275,7 +275,7 @@ extern "C" int taac_delta_rule_bwd(const void* q, const void* k, const void* log
   p.grad_q = static_cast<bf16_t*>(grad_q), p.grad_k = static_cast<bf16_t*>(grad_k), p.grad_v = static_cast<bf16_t*>(grad_v);
   p.grad_decay = grad_decay, p.grad_beta = grad_beta, p.grad_states = static_cast<bf16_t*>(grad_states);
   hipStream_t s = as_stream(stream);
-  if (const int64_t bytes = delta_team_bytes(static_cast<int64_t>(B) * H, T, dv)) {
+  if (const int64_t bytes = delta_team_bytes(static_cast<int64_t>(B) * H, T, dk, dv)) {
     if (workspace == nullptr || workspace_bytes < bytes || !aligned16(workspace))
       return set_error(TAAC_ERR_INVALID_VALUE, "%s: workspace must hold %lld bytes, 16-byte aligned", name, (long long)bytes);
     p.blocks = static_cast<uint8_t*>(workspace);

@@ -318,7 +318,7 @@ extern "C" int taac_delta_rule_fwd(const void* q, const void* k, const void* v, 
   p.state_in = state_in, p.state_out = state_out;
   p.chunk_states = static_cast<bf16_t*>(chunk_states), p.misses = static_cast<bf16_t*>(misses);
   hipStream_t s = as_stream(stream);
-  if (const int64_t bytes = delta_team_bytes(static_cast<int64_t>(B) * H, T, dv)) {
+  if (const int64_t bytes = delta_team_bytes(static_cast<int64_t>(B) * H, T, dk, dv)) {
     if (workspace == nullptr || workspace_bytes < bytes || !aligned16(workspace))
       return set_error(TAAC_ERR_INVALID_VALUE, "%s: workspace must hold %lld bytes, 16-byte aligned", name, (long long)bytes);
     p.blocks = static_cast<uint8_t*>(workspace);

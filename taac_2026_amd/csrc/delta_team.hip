@@ -512,8 +512,13 @@ int delta_team_back(const char* name, const DeltaParams& p, hipStream_t s) {
   return launch_team<128, true>(name, p, s);
 }
 
-int64_t delta_team_bytes(int64_t heads, int32_t T, int32_t dv) {
-  if (heads * ((dv + 15) / 16) > 2048) return 0;
+int64_t delta_team_bytes(int64_t heads, int32_t T, int32_t dk, int32_t dv) {
+  // Two, three or six teams to a CU: beyond that the chain of chunks no longer counts, and a wavefront that walks its head alone, without the
+  // blocks in memory, is faster. 2048 tokens, forward, this form against the other, by heads times groups of 16 columns: 32 wide 119 : 163 us
+  // at 512, 192 : 171 at 768; 64 wide 152 : 194 at 768, 218 : 198 at 1024; 128 wide 340 : 418 at 1536, 445 : 428 at 2048; forward and backward
+  // together the same order (402 : 473, 617 : 561; 532 : 572, 729 : 619; 1348 : 1403, 1793 : 1593).
+  const int64_t teams = heads * ((dv + 15) / 16);
+  if (teams > (dk <= 32 ? 512 : dk <= 64 ? 768 : 1536)) return 0;
   return heads * ((T + kChunk - 1) / kChunk) * kBlockBytes;
 }
 
@@ -521,5 +526,5 @@ int64_t delta_team_bytes(int64_t heads, int32_t T, int32_t dv) {
 
 extern "C" int64_t taac_delta_rule_workspace_bytes(int32_t B, int32_t H, int32_t T, int32_t dk, int32_t dv) {
   if (B < 0 || H <= 0 || T < 0 || dk <= 0 || dv <= 0) return -1;
-  return taac::delta_team_bytes(static_cast<int64_t>(B) * H, T, dv);
+  return taac::delta_team_bytes(static_cast<int64_t>(B) * H, T, dk, dv);
 }
