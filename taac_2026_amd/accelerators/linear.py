@@ -1191,11 +1191,13 @@ def linear_fp8(
     if amax_x.numel() != 1 and amax_x.shape == shape[:-1]:
         if x.dtype != torch.float8_e4m3fn or amax_x.dtype != torch.float32:
             raise ValueError("linear_fp8 takes one float32 amax_x per row with float8_e4m3fn activations only")
-        status = library.taac_linear_fp8_rows(
-            rows.data_ptr(), rows.stride(0), weight_fp8.data_ptr(), amax_x.contiguous().data_ptr(), amax_w.data_ptr(),
-            _native.ptr(bias), _native.ptr(res_rows), out.data_ptr(), out_features, rows.shape[0], n, weight_fp8.shape[1],
-            epilogue, int(bool(gate_first)), _native.current_stream(x.device),
-        )
+        amax_rows = amax_x.contiguous()
+        with _native.on_device(x.device):
+            status = library.taac_linear_fp8_rows(
+                rows.data_ptr(), rows.stride(0), weight_fp8.data_ptr(), amax_rows.data_ptr(), amax_w.data_ptr(),
+                _native.ptr(bias), _native.ptr(res_rows), out.data_ptr(), out_features, rows.shape[0], n, weight_fp8.shape[1],
+                epilogue, int(bool(gate_first)), _native.current_stream(x.device),
+            )
         _native.check(status, "linear_fp8")
         return out.reshape(*shape[:-1], out_features)
     status = library.taac_linear_fp8(

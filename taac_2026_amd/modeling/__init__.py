@@ -25,6 +25,7 @@ from taac_2026_amd.modeling.normalization import (
     rms_norm_runtime_state,
 )
 from taac_2026_amd.modeling.readout import CandidateClsPooler, CandidateReadoutHead
+from taac_2026_amd.modeling.recurrent import GatedDeltaAttention, GatedDeltaBlock
 from taac_2026_amd.modeling.sequence import (
     causal_valid_attention_mask,
     configure_flash_attention_runtime,
@@ -41,6 +42,8 @@ __all__ = [
     "MixedFeedForward",
     "CandidateClsPooler",
     "CandidateReadoutHead",
+    "GatedDeltaAttention",
+    "GatedDeltaBlock",
     "LayerNorm",
     "MetadataAttentionMask",
     "PCVRBackbone",
