@@ -1,5 +1,4 @@
-// Pieces shared by the kernels of the gated delta rule (delta_solo.hip, delta_team.hip, delta_scan.hip, delta_bwd.hip,
-// delta_grads.hip).
+// Pieces shared by the kernels of the gated delta rule (delta_solo.hip, delta_team.hip, delta_grads.hip).
 //
 // Per sample and value head, with a_t = exp(g_t), the state S [key_dim, value_dim] follows
 //   N_t = v_t - (a_t S)^T k_t,   S <- a_t S + k_t (beta_t N_t)^T,   o_t = scale S^T q_t.
@@ -7,6 +6,11 @@
 //   X = V - diag(e^G) K S,   (I + A) N = X,   O = scale (diag(e^G) Q S + (Gam * Q K^T * beta) N),
 //   S' = e^{G_64} S + (beta e^{G_64 - G} K)^T N.
 // The inverse of the unit triangular I + A is written I - M; M and the score matrix P do not depend on the state.
+// Backward, with dS' the gradient of the state behind a chunk (P holds scale, Gam and beta of its column),
+//   beta dU = diag(beta e^{G_64 - G}) K dS' + P^T dO,   dX = beta dU - M^T (beta dU) = dV,
+//   dS = e^{G_64} dS' + Q^T (scale e^G dO) - K^T (e^G dX)
+// is a recurrence like the forward's, backwards, column by column of the values. It keeps dX and dS' of every chunk, from which the other
+// gradients are made chunk by chunk.
 //
 // All products run on v_mfma_f32_16x16x32_bf16. With lane = (l16 = lane % 16, grp = lane / 16) its operands hold row (or column)
 // l16 and 8 values of the contraction, its result column l16 and rows 4 grp .. 4 grp + 3. The contraction may be walked in any
@@ -55,16 +59,12 @@ struct DeltaParams {
   float scale;
 };
 
-int delta_check(const char* name, const DeltaParams& p);
-// The form for few heads (delta_team.hip): bytes of its blocks, 0 where the other form is the faster one.
-int64_t delta_team_bytes(int64_t heads, int32_t T, int32_t dk, int32_t dv);
-int delta_team_fwd(const char* name, const DeltaParams& p, hipStream_t s);
-int delta_team_back(const char* name, const DeltaParams& p, hipStream_t s);
-// The form for many heads of at most 64 key features (delta_solo.hip).
+// The two forms of the recurrence, forward (o, the last state; chunk_states and misses where they are wanted) and backward (grad_v,
+// grad_states): with the chunks' blocks in p.blocks (delta_team.hip), and for heads of at most 64 key features without (delta_solo.hip).
+int delta_team(const char* name, const DeltaParams& p, bool back, hipStream_t s);
 int delta_solo(const char* name, const DeltaParams& p, bool back, hipStream_t s);
 // The second half of the backward (delta_grads.hip).
 int delta_grads(const char* name, const DeltaParams& p, hipStream_t s);
-int delta_strides(const char* name, const char* what, const void* ptr, const int64_t* from, int64_t* to, bool rows, int32_t width);
 
 namespace {
 
@@ -114,16 +114,7 @@ __device__ __forceinline__ bf16x8 zero8() {
   return __builtin_bit_cast(bf16x8, z);
 }
 
-__device__ __forceinline__ float load_gate(const void* p, int64_t at, int f32) {
-  return f32 ? static_cast<const float*>(p)[at] : static_cast<float>(static_cast<const bf16_t*>(p)[at]);
-}
-
-// Reads through a uniform base and a 32-bit offset of the lane, which stays the same for every chunk (token strides are below 2^24
-// elements).
-template <typename V, typename T>
-__device__ __forceinline__ V at_offset(const T* base, uint32_t bytes) {
-  return *reinterpret_cast<const V*>(reinterpret_cast<const uint8_t*>(base) + bytes);
-}
+// Writes through a uniform base and a 32-bit offset of the lane, which stays the same for every chunk (token strides are below 2^24 elements).
 template <typename T, typename V>
 __device__ __forceinline__ void put_offset(T* base, uint32_t bytes, const V& v) {
   *reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(base) + bytes) = v;
@@ -162,29 +153,13 @@ __device__ __forceinline__ uint32_t read1(Buffer b, uint32_t off) {
 
 __device__ __forceinline__ int state_row(int a, int m) { return 32 * (a / 2) + 8 * (m / 4) + 4 * (a % 2) + m % 4; }
 
-// Operand fragment of block kb (32 features) of a row in global memory; null rows and features at or beyond width give zeros.
-__device__ __forceinline__ bf16x8 row_frag(const bf16_t* row, int kb, int grp, int width) {
-  bf16x8 r = zero8();
-  if (row != nullptr && kb * 32 + grp * 8 < width) r = *reinterpret_cast<const bf16x8*>(row + kb * 32 + grp * 8);
-  return r;
-}
-
 // Tiles of 64 token rows in LDS. Rows are 16 bytes longer than their contents, which puts the 16 rows of a read on different banks.
 template <int WIDTH>
 struct Tile {
   static constexpr int STRIDE = WIDTH + 8;  // elements
   static constexpr int BYTES = kChunk * STRIDE * 2;
-  // rows token0 .. of `src` (stride ld), n of them valid, `width` valid features from the first
-  static __device__ __forceinline__ void stage(bf16_t* dst, const bf16_t* src, int64_t ld, int n, int width, int tid, int threads) {
-    constexpr int PIECES = WIDTH / 8;
-    for (int i = tid; i < kChunk * PIECES; i += threads) {
-      const int row = i / PIECES, piece = i % PIECES;
-      bf16x8 v = zero8();
-      if (row < n && piece * 8 < width) v = *reinterpret_cast<const bf16x8*>(src + row * ld + piece * 8);
-      *reinterpret_cast<bf16x8*>(dst + row * STRIDE + piece * 8) = v;
-    }
-  }
-  // the two halves of stage() for ROWS rows, so that the loads of several tiles are in flight together
+  // ROWS rows of memory (n of them valid, `width` valid features) on their way into LDS by THREADS threads: requested for several tiles before any of
+  // them is stored
   template <int ROWS, int THREADS>
   struct Piece {
     static constexpr int PIECES = WIDTH / 8, COUNT = (ROWS * PIECES + THREADS - 1) / THREADS;
@@ -296,24 +271,36 @@ __device__ __forceinline__ void solve_diagonal(float* scratch, int lane) {
   wave_sync();
 }
 
-// Place of a fragment in a block. By rows (forward): row tile ti, token block tk <= ti / 2. By columns (backward): column tile tj, token
-// block tk >= tj / 2.
-__host__ __device__ constexpr int frag_rows(int ti, int tk) { return ti < 2 ? ti : 2 + (ti - 2) * 2 + tk; }
-__host__ __device__ constexpr int frag_cols(int tj, int tk) { return tj < 2 ? tj * 2 + tk : 2 + tj; }
+// The gates of a lane's token as the bits that the reads bring, by halves: a branch between fp32 and bf16 would await each.
+struct GateBits {
+  uint32_t g[2], beta[2];
+  // token `lane` of the n behind token0 (n may be 0: nothing is used then)
+  __device__ __forceinline__ void request(const DeltaParams& p, int b, int h, int64_t token0, int n, int lane) {
+    const int64_t token = lane < n ? token0 + lane : 0;
+    const int64_t at_g = b * p.gs[0] + h * p.gs[1] + token * p.gs[2], at_beta = b * p.bs[0] + h * p.bs[1] + token * p.bs[2];
+    const uint16_t* from_g = static_cast<const uint16_t*>(p.log_decay) + (at_g << p.gates_f32);
+    const uint16_t* from_beta = static_cast<const uint16_t*>(p.beta) + (at_beta << p.gates_f32);
+    g[0] = from_g[0], g[1] = from_g[p.gates_f32];
+    beta[0] = from_beta[0], beta[1] = from_beta[p.gates_f32];
+  }
+  static __device__ __forceinline__ float value(const uint32_t (&bits)[2], int f32, bool live) {
+    const float v = __builtin_bit_cast(float, bits[1] << 16 | (f32 ? bits[0] : 0));  // a bf16 is the upper half of a float
+    return live ? v : 0.f;
+  }
+  // A decay in powers of two; an exponent below -1e5 is a decay of zero, and stays finite in the sums.
+  __device__ __forceinline__ double decay(const DeltaParams& p, bool live) const {
+    const float v = value(g, p.gates_f32, live);
+    return static_cast<double>(v < -1e5f ? -1e5f : v) * 1.4426950408889634;
+  }
+  __device__ __forceinline__ float step(const DeltaParams& p, bool live) const { return value(beta, p.gates_f32, live); }
+};
 
-// The factors of a chunk's tokens, by one wavefront. last_minus: null, or receives e^(G_64 - G) of every token.
-__device__ __forceinline__ void chunk_rows(const DeltaParams& p, int b, int h, int64_t token0, int n, float* rows, float* temp,
+// The factors of a chunk's n tokens, by one wavefront. last_minus: null, or receives e^(G_64 - G) of every token.
+__device__ __forceinline__ void chunk_rows(const DeltaParams& p, const GateBits& gates, int n, float* rows, float* temp,
                                            float* last_minus = nullptr) {
   const int lane = threadIdx.x % kWave;
-  // decays in powers of two; an exponent below -1e5 is a decay of zero, and stays finite in the sums
-  double total = 0.0;
-  float beta = 0.f;
-  if (lane < n) {
-    float g = load_gate(p.log_decay, b * p.gs[0] + h * p.gs[1] + (token0 + lane) * p.gs[2], p.gates_f32);
-    g = g < -1e5f ? -1e5f : g;
-    total = static_cast<double>(g) * 1.4426950408889634;
-    beta = load_gate(p.beta, b * p.bs[0] + h * p.bs[1] + (token0 + lane) * p.bs[2], p.gates_f32);
-  }
+  double total = gates.decay(p, lane < n);
+  const float beta = gates.step(p, lane < n);
 #pragma unroll
   for (int off = 1; off < kWave; off *= 2) {
     const double up = __shfl_up(total, off, kWave);
@@ -343,154 +330,6 @@ __device__ __forceinline__ void chunk_rows(const DeltaParams& p, int b, int h, i
 __device__ __forceinline__ float tiles_between(const float* rows, int ti, int tj) {
   const float second = rows[kRowTotal + 1], third = rows[kRowTotal + 2];
   return ti - tj < 2 ? 1.f : (ti - tj == 3 ? second * third : (tj == 0 ? second : third));
-}
-
-// One wavefront makes the block of one chunk (n valid tokens; rows beyond count as k = q = 0, g = 0, beta = 0): -M as hi and lo, P, and the
-// factors of its tokens. COLS: transposed fragments, for the backward. block: LDS or global; rows, temp, scratch: LDS; scratch may be
-// the M part of the block, temp its P part.
-//
-// The 64 x 64 inverse: the four diagonal blocks of 16 by substitution, a column per lane, all four at once; the blocks below them by
-// products, M_21 = T_22 A_21 T_11 with T = I - M, first pairs of 16, then of 32.
-template <int DK, bool COLS>
-__device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, int64_t token0, int n, uint8_t* block, float* rows,
-                                            float* temp, float* scratch) {
-  constexpr int KB = DK / 32;
-  const int lane = threadIdx.x % kWave, l16 = lane % 16, grp = lane / 16;
-
-  chunk_rows(p, b, h, token0, n, rows, temp);
-  const int64_t hk = h / p.group;
-  const bf16_t* kbase = p.k + b * p.ks[0] + hk * p.ks[1] + token0 * p.ks[2];
-  const bf16_t* qbase = p.q + b * p.qs[0] + hk * p.qs[1] + token0 * p.qs[2];
-  bf16x8 kf[4][KB];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int row = 16 * t + l16;
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) kf[t][kb] = row_frag(row < n ? kbase + row * p.ks[2] : nullptr, kb, grp, p.dk);
-  }
-  wave_sync();
-
-  f32x4 a_rows[10];  // A by rows, tile (ti, tj) at ti (ti + 1) / 2 + tj
-  u32x2 pf[6][2];
-#pragma unroll
-  for (int i = 0; i < 6; ++i) pf[i][0] = pf[i][1] = u32x2{0u, 0u};
-#pragma unroll
-  for (int ti = 0; ti < 4; ++ti) {
-    const int row = 16 * ti + l16;
-    bf16x8 qf[KB];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) qf[kb] = row_frag(row < n ? qbase + row * p.qs[2] : nullptr, kb, grp, p.dk);
-    const float hi_i = temp[kTempHi + row], lo_i = temp[kTempLow + row], in_i = temp[kTempIn + row];
-#pragma unroll
-    for (int tj = 0; tj <= ti; ++tj) {
-      f32x4 kk = zero4(), qk = zero4();
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        kk = mfma16(kf[tj][kb], kf[ti][kb], kk);
-        qk = COLS ? mfma16(qf[kb], kf[tj][kb], qk) : mfma16(kf[tj][kb], qf[kb], qk);
-      }
-      f32x4 a, s;
-      if (ti > tj) {
-        const float between = tiles_between(rows, ti, tj);
-        const float a_i = in_i * between, s_i = a_i * p.scale;
-        const f32x4 out_j = *reinterpret_cast<const f32x4*>(temp + kTempOutBeta + 16 * tj + 4 * grp);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          a[r] = a_i * out_j[r] * kk[r];
-          if (!COLS) s[r] = s_i * out_j[r] * qk[r];
-        }
-        if (COLS) {
-          const float s_j = temp[kTempOutBeta + 16 * tj + l16] * between * p.scale;
-          const f32x4 in_r = *reinterpret_cast<const f32x4*>(temp + kTempIn + 16 * ti + 4 * grp);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[r] = s_j * in_r[r] * qk[r];
-        }
-      } else {
-        const f32x4 hi_j = *reinterpret_cast<const f32x4*>(temp + kTempHi + 16 * tj + 4 * grp);
-        const f32x4 lo_j = *reinterpret_cast<const f32x4*>(temp + kTempLow + 16 * tj + 4 * grp);
-        const f32x4 beta_j = *reinterpret_cast<const f32x4*>(temp + kTempBeta + 16 * tj + 4 * grp);
-        const float beta_i = temp[kTempBeta + row];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int m = 4 * grp + r;
-          const float diff = (hi_i - hi_j[r]) + (lo_i - lo_j[r]);  // of tokens l16 and m of the tile
-          const float gam = __builtin_amdgcn_exp2f(diff) * beta_j[r];
-          a[r] = l16 > m ? gam * kk[r] : 0.f;
-          if (COLS) s[r] = m >= l16 ? p.scale * __builtin_amdgcn_exp2f(-diff) * beta_i * qk[r] : 0.f;
-          else s[r] = l16 >= m ? p.scale * gam * qk[r] : 0.f;
-        }
-      }
-      a_rows[ti * (ti + 1) / 2 + tj] = a;
-      const int f = COLS ? frag_cols(tj, ti / 2) : frag_rows(ti, tj / 2);
-      const int half = COLS ? ti % 2 : tj % 2;
-      pf[f][half] = round4(s);
-    }
-  }
-
-  // diagonal blocks
-#pragma unroll
-  for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(scratch + t * kScratchBlock + l16 * kScratchRow + 4 * grp) = a_rows[t * (t + 1) / 2 + t];
-  wave_sync();
-  solve_diagonal(scratch, lane);
-  f32x4 m_rows[4], m_cols[4], t_rows[4], t_cols[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    m_rows[t] = *reinterpret_cast<const f32x4*>(scratch + t * kScratchBlock + l16 * kScratchRow + 4 * grp);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      m_cols[t][r] = scratch[t * kScratchBlock + (4 * grp + r) * kScratchRow + l16];
-      const float one = l16 == 4 * grp + r ? 1.f : 0.f;
-      t_rows[t][r] = one - m_rows[t][r];
-      t_cols[t][r] = one - m_cols[t][r];
-    }
-  }
-  wave_sync();
-
-  const f32x4 z10 = mul_cols(a_rows[1], t_cols[0], zero4());
-  const f32x4 z32 = mul_cols(a_rows[8], t_cols[2], zero4());
-  const f32x4 m10c = mul_cols(t_rows[1], z10, zero4());
-  const f32x4 m32r = mul_rows(t_rows[3], z32, zero4());
-  f32x4 m10n, m32n;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    m10n[r] = -m10c[r];
-    m32n[r] = -m32r[r];
-  }
-  const f32x4 z20 = mul_cols(a_rows[4], m10n, mul_cols(a_rows[3], t_cols[0], zero4()));
-  const f32x4 z21 = mul_cols(a_rows[4], t_cols[1], zero4());
-  const f32x4 z30 = mul_cols(a_rows[7], m10n, mul_cols(a_rows[6], t_cols[0], zero4()));
-  const f32x4 z31 = mul_cols(a_rows[7], t_cols[1], zero4());
-
-  auto put = [&](int f, const f32x4& first, const f32x4& second) {
-    f32x4 a, c;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      a[r] = -first[r];
-      c[r] = -second[r];
-    }
-    bf16x8 hi8, lo8;
-    split(a, c, hi8, lo8);
-    *reinterpret_cast<bf16x8*>(block + kBlockM + f * kFrag + lane * 16) = hi8;
-    *reinterpret_cast<bf16x8*>(block + kBlockLow + f * kFrag + lane * 16) = lo8;
-    *reinterpret_cast<u32x4*>(block + kBlockP + f * kFrag + lane * 16) = u32x4{pf[f][0][0], pf[f][0][1], pf[f][1][0], pf[f][1][1]};
-  };
-  if (!COLS) {
-    const f32x4 m10r = mul_rows(t_rows[1], z10, zero4());
-    put(frag_rows(0, 0), m_rows[0], zero4());
-    put(frag_rows(1, 0), m10r, m_rows[1]);
-    put(frag_rows(2, 0), mul_rows(t_rows[2], z20, zero4()), mul_rows(t_rows[2], z21, zero4()));
-    put(frag_rows(2, 1), m_rows[2], zero4());
-    put(frag_rows(3, 0), mul_rows(m32n, z20, mul_rows(t_rows[3], z30, zero4())), mul_rows(m32n, z21, mul_rows(t_rows[3], z31, zero4())));
-    put(frag_rows(3, 1), m32r, m_rows[3]);
-  } else {
-    const f32x4 m32c = mul_cols(t_rows[3], z32, zero4());
-    put(frag_cols(0, 0), m_cols[0], m10c);
-    put(frag_cols(0, 1), mul_cols(t_rows[2], z20, zero4()), mul_cols(m32n, z20, mul_cols(t_rows[3], z30, zero4())));
-    put(frag_cols(1, 0), zero4(), m_cols[1]);
-    put(frag_cols(1, 1), mul_cols(t_rows[2], z21, zero4()), mul_cols(m32n, z21, mul_cols(t_rows[3], z31, zero4())));
-    put(frag_cols(2, 1), m_cols[2], m32c);
-    put(frag_cols(3, 1), zero4(), m_cols[3]);
-  }
 }
 
 }  // namespace

@@ -1,5 +1,5 @@
 // Gated delta rule, chunked form, backward: the gradients of a chunk's tokens (notation, operand order and precision: delta.h; dS' and dX:
-// delta_bwd.hip), in parallel over the chunks. With
+// delta.h), in parallel over the chunks. With
 //   B_ij = scale Gam_ij dO_i . N_j (i >= j),   E_ij = -Gam_ij dX_i . N_j (i > j)
 //   dQ = scale e^G dO S^T + B diag(beta) K
 //   R  = E diag(beta) K - e^G dX S^T
@@ -40,7 +40,7 @@ __device__ __forceinline__ void store_gate(void* p, int64_t at, float v, int f32
 }
 
 template <int DK, int DV>
-__global__ __launch_bounds__(4 * kWave, DK <= 64 && DV <= 64 ? 2 : 1) void delta_grads_kernel(const DeltaParams p) {
+__global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && DV <= 64 ? 2 : 1) void delta_grads_kernel(const DeltaParams p) {
   constexpr int KA = DK / 16, VB = DV / 32, kThreads = 4 * kWave;
   typedef GradLds<DK, DV> L;
   typedef Tile<DK> TK;
@@ -62,9 +62,9 @@ __global__ __launch_bounds__(4 * kWave, DK <= 64 && DV <= 64 ? 2 : 1) void delta
   float* state_dot = d_tail + 64;  // per wavefront
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
-  const int key_heads = p.H / p.group;
-  const int chunk = static_cast<int>(blockIdx.x % p.chunks);
-  const int64_t pair = blockIdx.x / p.chunks;
+  const uint32_t key_heads = static_cast<uint32_t>(p.H) / p.group;
+  const int chunk = static_cast<int>(blockIdx.x % static_cast<uint32_t>(p.chunks));
+  const uint32_t pair = blockIdx.x / static_cast<uint32_t>(p.chunks);
   const int hk = static_cast<int>(pair % key_heads);
   const int b = static_cast<int>(pair / key_heads);
   int len = p.T;
@@ -105,6 +105,8 @@ __global__ __launch_bounds__(4 * kWave, DK <= 64 && DV <= 64 ? 2 : 1) void delta
     typename TV::template Piece<kChunk, kThreads> o_in, x_in, n_in;
     typename TK::template Piece<DV, kThreads> s_in, g_in;
     const int64_t at_state = (unit * p.chunks + chunk) * static_cast<int64_t>(p.dk) * p.dv;
+    GateBits gates;
+    if (wave == 0) gates.request(p, b, h, token0, n_tok, lane);
     o_in.load(p.grad_o + b * p.dos[0] + h * p.dos[1] + token0 * p.dos[2], p.dos[2], n_tok, p.dv, tid);
     x_in.load(p.grad_v + b * p.dvs[0] + h * p.dvs[1] + token0 * p.dvs[2], p.dvs[2], n_tok, p.dv, tid);
     n_in.load(p.misses + (unit * p.T + token0) * p.dv, p.dv, n_tok, p.dv, tid);
@@ -112,7 +114,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 64 && DV <= 64 ? 2 : 1) void delta
     g_in.load(p.grad_states + at_state, p.dk, p.dv, p.dk, tid);
     float dot_state = s_in.dot(g_in);
     __syncthreads();  // the previous head's tiles and sums are no longer read
-    if (wave == 0) chunk_rows(p, b, h, token0, n_tok, rows, temp, left_over);
+    if (wave == 0) chunk_rows(p, gates, n_tok, rows, temp, left_over);
     o_in.store(tile_o, tid);
     x_in.store(tile_x, tid);
     n_in.store(tile_n, tid);

@@ -29,7 +29,7 @@ constexpr int kSoloHi = 0, kSoloLow = 64, kSoloBeta = 128, kSoloIn = 192, kSoloO
 template <int DK>
 struct SoloTokens {
   bf16x8 kf[4][DK / 32], qf[4][DK / 32], x[4];  // x: pieces of the values (backward: of dO)
-  uint32_t g[2], beta[2];                       // by halves: a branch between fp32 and bf16 would await each
+  GateBits gates;
 };
 
 template <int DK, bool BACK>
@@ -46,12 +46,13 @@ struct Solo {
 
   __device__ __forceinline__ Solo(const DeltaParams& params) : p(params) {
     lane = threadIdx.x, l16 = lane % 16, grp = lane / 16;
-    const int col_groups = (p.dv + kSoloCols - 1) / kSoloCols;
+    const uint32_t col_groups = (p.dv + kSoloCols - 1) / kSoloCols;
     const uint32_t block = xcd_remap(blockIdx.x, gridDim.x);  // the columns of a head, which read the same rows, on one die's L2
-    unit = block / col_groups;
+    const uint32_t head = block / col_groups;
+    unit = head;
     col0 = static_cast<int>(block % col_groups) * kSoloCols;
-    h = static_cast<int>(unit % p.H);
-    b = static_cast<int>(unit / p.H);
+    h = static_cast<int>(head % static_cast<uint32_t>(p.H));
+    b = static_cast<int>(head / static_cast<uint32_t>(p.H));
     len = p.T;
     if (p.lengths != nullptr) {
       len = p.lengths[b];
@@ -85,11 +86,7 @@ struct Solo {
     const int n_tok = group >= 0 ? tokens_of(group) : 0;
     const int64_t token0 = n_tok > 0 ? static_cast<int64_t>(group) * kChunk : 0;
     const bf16_t *k = k0 + token0 * p.ks[2], *q = q0 + token0 * p.qs[2], *x = x0 + token0 * x_ld;
-    const int64_t token = lane < n_tok ? token0 + lane : 0;
-    const int64_t at_g = b * p.gs[0] + h * p.gs[1] + token * p.gs[2], at_beta = b * p.bs[0] + h * p.bs[1] + token * p.bs[2];
-    const uint16_t *g = static_cast<const uint16_t*>(p.log_decay) + (at_g << p.gates_f32), *beta = static_cast<const uint16_t*>(p.beta) + (at_beta << p.gates_f32);
-    c.g[0] = g[0], c.g[1] = g[p.gates_f32];
-    c.beta[0] = beta[0], c.beta[1] = beta[p.gates_f32];
+    c.gates.request(p, b, h, token0, n_tok, lane);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const Buffer kt = rows_buffer(k + t * 16 * p.ks[2], p.ks[2], n_tok - 16 * t, p.dk);
@@ -105,11 +102,6 @@ struct Solo {
       for (int kb = 0; kb < KB; ++kb) c.qf[t][kb] = read8(qt, q_off[kb]);
     }
   }
-  __device__ __forceinline__ float gate(const uint32_t (&bits)[2], bool live) const {
-    const float v = __builtin_bit_cast(float, bits[1] << 16 | (p.gates_f32 ? bits[0] : 0));  // a bf16 is the upper half of a float
-    return live ? v : 0.f;
-  }
-
   // The tokens' factors and rows into LDS.
   __device__ __forceinline__ void place(const SoloTokens<DK>& c, int n_tok, float* rows, bf16_t* tile_k, bf16_t* tile_x) const {
 #pragma unroll
@@ -121,9 +113,8 @@ struct Solo {
       }
       *reinterpret_cast<bf16x8*>(tile_x + (16 * t + lane / 4) * TV::STRIDE + (lane % 4) * 8) = c.x[t];
     }
-    const float given = gate(c.g, lane < n_tok), beta = gate(c.beta, lane < n_tok);
-    const float g = given < -1e5f ? -1e5f : given;  // a decay of zero, finite in the sums
-    double total = static_cast<double>(g) * 1.4426950408889634;
+    const float beta = c.gates.step(p, lane < n_tok);
+    double total = c.gates.decay(p, lane < n_tok);
 #pragma unroll
     for (int off = 1; off < kWave; off *= 2) {
       const double up = __shfl_up(total, off, kWave);
@@ -466,7 +457,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
   }
 }
 
-// The gradient of the state, tokens last to first (the formulas: delta_bwd.hip).
+// The gradient of the state, tokens last to first (the formulas: delta.h).
 template <int DK>
 __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kernel(const DeltaParams p) {
   typedef Solo<DK, true> W;

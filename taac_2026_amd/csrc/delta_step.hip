@@ -68,8 +68,8 @@ __global__ __launch_bounds__(W * kWave) void delta_step_kernel(const StepParams 
   constexpr int kAhead = W > 1 ? 4 : 8;
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   const int vec = tid % NVP, row0 = tid / NVP;
-  const int h = static_cast<int>(blockIdx.x % p.H);
-  const int first = static_cast<int>(blockIdx.x / p.H);
+  const int h = static_cast<int>(blockIdx.x % static_cast<uint32_t>(p.H));
+  const int first = static_cast<int>(blockIdx.x / static_cast<uint32_t>(p.H));
   __shared__ float red[2][W][NVP][8];
   __shared__ float red_qk[2][W];
   const bool col_ok = vec * 4 < p.dv;

@@ -11,21 +11,175 @@
 namespace taac {
 namespace {
 
+// Place of a fragment in a block. By rows (forward): row tile ti, token block tk <= ti / 2. By columns (backward): column tile tj, token
+// block tk >= tj / 2.
+__host__ __device__ constexpr int frag_rows(int ti, int tk) { return ti < 2 ? ti : 2 + (ti - 2) * 2 + tk; }
+__host__ __device__ constexpr int frag_cols(int tj, int tk) { return tj < 2 ? tj * 2 + tk : 2 + tj; }
+
+// One wavefront makes the block of one chunk (n valid tokens; rows beyond count as k = q = 0, g = 0, beta = 0): -M as hi and lo, P, and the
+// factors of its tokens. COLS: transposed fragments, for the backward. rows, temp, scratch: LDS.
+//
+// The 64 x 64 inverse: the four diagonal blocks of 16 by substitution, a column per lane, all four at once; the blocks below them by
+// products, M_21 = T_22 A_21 T_11 with T = I - M, first pairs of 16, then of 32.
+template <int DK, bool COLS>
+__device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, int64_t token0, int n, uint8_t* block, float* rows,
+                                            float* temp, float* scratch) {
+  constexpr int KB = DK / 32;
+  const int lane = threadIdx.x % kWave, l16 = lane % 16, grp = lane / 16;
+
+  // everything is requested before any of it is waited for
+  const int64_t hk = h / p.group;
+  const Buffer k_rows = rows_buffer(p.k + b * p.ks[0] + hk * p.ks[1] + token0 * p.ks[2], p.ks[2], n, p.dk);
+  const Buffer q_rows = rows_buffer(p.q + b * p.qs[0] + hk * p.qs[1] + token0 * p.qs[2], p.qs[2], n, p.dk);
+  GateBits gates;
+  gates.request(p, b, h, token0, n, lane);
+  bf16x8 kf[4][KB], qf[4][KB];
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+      kf[t][kb] = read8(k_rows, 32 * kb + 8 * grp < p.dk ? (16 * t + l16) * static_cast<uint32_t>(p.ks[2]) * 2 + 64 * kb + 16 * grp : kNowhere);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+      qf[t][kb] = read8(q_rows, 32 * kb + 8 * grp < p.dk ? (16 * t + l16) * static_cast<uint32_t>(p.qs[2]) * 2 + 64 * kb + 16 * grp : kNowhere);
+  chunk_rows(p, gates, n, rows, temp);
+  wave_sync();
+
+  f32x4 a_rows[10];  // A by rows, tile (ti, tj) at ti (ti + 1) / 2 + tj
+  u32x2 pf[6][2];
+#pragma unroll
+  for (int i = 0; i < 6; ++i) pf[i][0] = pf[i][1] = u32x2{0u, 0u};
+#pragma unroll
+  for (int ti = 0; ti < 4; ++ti) {
+    const int row = 16 * ti + l16;
+    const float hi_i = temp[kTempHi + row], lo_i = temp[kTempLow + row], in_i = temp[kTempIn + row];
+#pragma unroll
+    for (int tj = 0; tj <= ti; ++tj) {
+      f32x4 kk = zero4(), qk = zero4();
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        kk = mfma16(kf[tj][kb], kf[ti][kb], kk);
+        qk = COLS ? mfma16(qf[ti][kb], kf[tj][kb], qk) : mfma16(kf[tj][kb], qf[ti][kb], qk);
+      }
+      f32x4 a, s;
+      if (ti > tj) {
+        const float between = tiles_between(rows, ti, tj);
+        const float a_i = in_i * between, s_i = a_i * p.scale;
+        const f32x4 out_j = *reinterpret_cast<const f32x4*>(temp + kTempOutBeta + 16 * tj + 4 * grp);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          a[r] = a_i * out_j[r] * kk[r];
+          if (!COLS) s[r] = s_i * out_j[r] * qk[r];
+        }
+        if (COLS) {
+          const float s_j = temp[kTempOutBeta + 16 * tj + l16] * between * p.scale;
+          const f32x4 in_r = *reinterpret_cast<const f32x4*>(temp + kTempIn + 16 * ti + 4 * grp);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[r] = s_j * in_r[r] * qk[r];
+        }
+      } else {
+        const f32x4 hi_j = *reinterpret_cast<const f32x4*>(temp + kTempHi + 16 * tj + 4 * grp);
+        const f32x4 lo_j = *reinterpret_cast<const f32x4*>(temp + kTempLow + 16 * tj + 4 * grp);
+        const f32x4 beta_j = *reinterpret_cast<const f32x4*>(temp + kTempBeta + 16 * tj + 4 * grp);
+        const float beta_i = temp[kTempBeta + row];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int m = 4 * grp + r;
+          const float diff = (hi_i - hi_j[r]) + (lo_i - lo_j[r]);  // of tokens l16 and m of the tile
+          const float gam = __builtin_amdgcn_exp2f(diff) * beta_j[r];
+          a[r] = l16 > m ? gam * kk[r] : 0.f;
+          if (COLS) s[r] = m >= l16 ? p.scale * __builtin_amdgcn_exp2f(-diff) * beta_i * qk[r] : 0.f;
+          else s[r] = l16 >= m ? p.scale * gam * qk[r] : 0.f;
+        }
+      }
+      a_rows[ti * (ti + 1) / 2 + tj] = a;
+      const int f = COLS ? frag_cols(tj, ti / 2) : frag_rows(ti, tj / 2);
+      const int half = COLS ? ti % 2 : tj % 2;
+      pf[f][half] = round4(s);
+    }
+  }
+
+  // diagonal blocks
+#pragma unroll
+  for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(scratch + t * kScratchBlock + l16 * kScratchRow + 4 * grp) = a_rows[t * (t + 1) / 2 + t];
+  wave_sync();
+  solve_diagonal(scratch, lane);
+  f32x4 m_rows[4], m_cols[4], t_rows[4], t_cols[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    m_rows[t] = *reinterpret_cast<const f32x4*>(scratch + t * kScratchBlock + l16 * kScratchRow + 4 * grp);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      m_cols[t][r] = scratch[t * kScratchBlock + (4 * grp + r) * kScratchRow + l16];
+      const float one = l16 == 4 * grp + r ? 1.f : 0.f;
+      t_rows[t][r] = one - m_rows[t][r];
+      t_cols[t][r] = one - m_cols[t][r];
+    }
+  }
+  wave_sync();
+
+  const f32x4 z10 = mul_cols(a_rows[1], t_cols[0], zero4());
+  const f32x4 z32 = mul_cols(a_rows[8], t_cols[2], zero4());
+  const f32x4 m10c = mul_cols(t_rows[1], z10, zero4());
+  const f32x4 m32r = mul_rows(t_rows[3], z32, zero4());
+  f32x4 m10n, m32n;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    m10n[r] = -m10c[r];
+    m32n[r] = -m32r[r];
+  }
+  const f32x4 z20 = mul_cols(a_rows[4], m10n, mul_cols(a_rows[3], t_cols[0], zero4()));
+  const f32x4 z21 = mul_cols(a_rows[4], t_cols[1], zero4());
+  const f32x4 z30 = mul_cols(a_rows[7], m10n, mul_cols(a_rows[6], t_cols[0], zero4()));
+  const f32x4 z31 = mul_cols(a_rows[7], t_cols[1], zero4());
+
+  auto put = [&](int f, const f32x4& first, const f32x4& second) {
+    f32x4 a, c;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      a[r] = -first[r];
+      c[r] = -second[r];
+    }
+    bf16x8 hi8, lo8;
+    split(a, c, hi8, lo8);
+    *reinterpret_cast<bf16x8*>(block + kBlockM + f * kFrag + lane * 16) = hi8;
+    *reinterpret_cast<bf16x8*>(block + kBlockLow + f * kFrag + lane * 16) = lo8;
+    *reinterpret_cast<u32x4*>(block + kBlockP + f * kFrag + lane * 16) = u32x4{pf[f][0][0], pf[f][0][1], pf[f][1][0], pf[f][1][1]};
+  };
+  if (!COLS) {
+    const f32x4 m10r = mul_rows(t_rows[1], z10, zero4());
+    put(frag_rows(0, 0), m_rows[0], zero4());
+    put(frag_rows(1, 0), m10r, m_rows[1]);
+    put(frag_rows(2, 0), mul_rows(t_rows[2], z20, zero4()), mul_rows(t_rows[2], z21, zero4()));
+    put(frag_rows(2, 1), m_rows[2], zero4());
+    put(frag_rows(3, 0), mul_rows(m32n, z20, mul_rows(t_rows[3], z30, zero4())), mul_rows(m32n, z21, mul_rows(t_rows[3], z31, zero4())));
+    put(frag_rows(3, 1), m32r, m_rows[3]);
+  } else {
+    const f32x4 m32c = mul_cols(t_rows[3], z32, zero4());
+    put(frag_cols(0, 0), m_cols[0], m10c);
+    put(frag_cols(0, 1), mul_cols(t_rows[2], z20, zero4()), mul_cols(m32n, z20, mul_cols(t_rows[3], z30, zero4())));
+    put(frag_cols(1, 0), zero4(), m_cols[1]);
+    put(frag_cols(1, 1), mul_cols(t_rows[2], z21, zero4()), mul_cols(m32n, z21, mul_cols(t_rows[3], z31, zero4())));
+    put(frag_cols(2, 1), m_cols[2], m32c);
+    put(frag_cols(3, 1), zero4(), m_cols[3]);
+  }
+}
+
 template <int DK, bool COLS>
 __global__ __launch_bounds__(kWave) void delta_blocks_kernel(const DeltaParams p) {
   __shared__ __attribute__((aligned(16))) float rows[kRowFloats];
   __shared__ __attribute__((aligned(16))) float temp[kTempFloats];
   __shared__ __attribute__((aligned(16))) float scratch[kScratchFloats];
-  const int chunk = static_cast<int>(blockIdx.x % p.chunks);
-  const int64_t unit = blockIdx.x / p.chunks;
-  const int h = static_cast<int>(unit % p.H);
-  const int b = static_cast<int>(unit / p.H);
+  const uint32_t chunks = p.chunks, heads = p.H, unit = blockIdx.x / chunks;
+  const int chunk = static_cast<int>(blockIdx.x % chunks), h = static_cast<int>(unit % heads), b = static_cast<int>(unit / heads);
   int len = p.T;
   if (p.lengths != nullptr) len = p.lengths[b] < p.T ? p.lengths[b] : p.T;
   const int64_t token0 = static_cast<int64_t>(chunk) * kChunk;
   const int64_t left = len - token0;
   if (left <= 0) return;
-  uint8_t* block = p.blocks + (unit * p.chunks + chunk) * kBlockBytes;
+  uint8_t* block = p.blocks + static_cast<int64_t>(blockIdx.x) * kBlockBytes;
   chunk_block<DK, COLS>(p, b, h, token0, left < kChunk ? static_cast<int>(left) : kChunk, block, rows, temp, scratch);
   float* out = reinterpret_cast<float*>(block + kBlockRows);
   for (int i = threadIdx.x; i < kRowFloats; i += kWave) out[i] = rows[i];
@@ -88,13 +242,14 @@ struct Team {
     const int tid = threadIdx.x;
     wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     lane = tid % kWave, l16 = lane % 16, grp = lane / 16;
-    const int col_groups = (p.dv + 15) / 16;
+    const uint32_t col_groups = (p.dv + 15) / 16;
     const uint32_t block = xcd_remap(blockIdx.x, gridDim.x);  // the columns of a head, which read the same rows, on one die's L2
-    unit = block / col_groups;
+    const uint32_t head = block / col_groups;
+    unit = head;
     col0 = static_cast<int>(block % col_groups) * 16;
     col_ok = col0 + l16 < p.dv;
-    h = static_cast<int>(unit % p.H);
-    b = static_cast<int>(unit / p.H);
+    h = static_cast<int>(head % static_cast<uint32_t>(p.H));
+    b = static_cast<int>(head / static_cast<uint32_t>(p.H));
     len = p.T;
     if (p.lengths != nullptr) {
       len = p.lengths[b];
@@ -357,7 +512,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
   }
 }
 
-// The gradient of the state, chunks last to first (the formulas: delta_bwd.hip). Stages: beta dU (own tokens) | dX (own tokens) | dS (own
+// The gradient of the state, chunks last to first (the formulas: delta.h). Stages: beta dU (own tokens) | dX (own tokens) | dS (own
 // rows). dO is read as fragments by every wavefront.
 template <int DK>
 __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaParams p) {
@@ -501,30 +656,10 @@ int launch_team(const char* name, const DeltaParams& p, hipStream_t s) {
 
 }  // namespace
 
-int delta_team_fwd(const char* name, const DeltaParams& p, hipStream_t s) {
-  if (p.dk <= 32) return launch_team<32, false>(name, p, s);
-  if (p.dk <= 64) return launch_team<64, false>(name, p, s);
-  return launch_team<128, false>(name, p, s);
-}
-int delta_team_back(const char* name, const DeltaParams& p, hipStream_t s) {
-  if (p.dk <= 32) return launch_team<32, true>(name, p, s);
-  if (p.dk <= 64) return launch_team<64, true>(name, p, s);
-  return launch_team<128, true>(name, p, s);
-}
-
-int64_t delta_team_bytes(int64_t heads, int32_t T, int32_t dk, int32_t dv) {
-  // Two, three or six teams to a CU: beyond that the chain of chunks no longer counts, and a wavefront that walks its head alone, without the
-  // blocks in memory, is faster. 2048 tokens, forward, this form against the other, by heads times groups of 16 columns: 32 wide 119 : 163 us
-  // at 512, 192 : 171 at 768; 64 wide 152 : 194 at 768, 218 : 198 at 1024; 128 wide 340 : 418 at 1536, 445 : 428 at 2048; forward and backward
-  // together the same order (402 : 473, 617 : 561; 532 : 572, 729 : 619; 1348 : 1403, 1793 : 1593).
-  const int64_t teams = heads * ((dv + 15) / 16);
-  if (teams > (dk <= 32 ? 512 : dk <= 64 ? 768 : 1536)) return 0;
-  return heads * ((T + kChunk - 1) / kChunk) * kBlockBytes;
+int delta_team(const char* name, const DeltaParams& p, bool back, hipStream_t s) {
+  if (p.dk <= 32) return back ? launch_team<32, true>(name, p, s) : launch_team<32, false>(name, p, s);
+  if (p.dk <= 64) return back ? launch_team<64, true>(name, p, s) : launch_team<64, false>(name, p, s);
+  return back ? launch_team<128, true>(name, p, s) : launch_team<128, false>(name, p, s);
 }
 
 }  // namespace taac
-
-extern "C" int64_t taac_delta_rule_workspace_bytes(int32_t B, int32_t H, int32_t T, int32_t dk, int32_t dv) {
-  if (B < 0 || H <= 0 || T < 0 || dk <= 0 || dv <= 0) return -1;
-  return taac::delta_team_bytes(static_cast<int64_t>(B) * H, T, dk, dv);
-}

@@ -137,6 +137,29 @@ def test_backward_of_many_heads(device, sizes, tokens):
     _check_backward(device, _draw(sizes[0], tokens, *sizes[1:], seed=tokens), lengths=lengths)
 
 
+@pytest.mark.parametrize("sizes", MANY + [(6, *s) for s in SIZES])
+def test_state_behind_the_first_token_of_a_chunk(device, sizes):
+    """The state of one chunk as the next one takes it over. It is kept as pairs of bf16: at most 2^-16 off, three roundings (state, misses,
+    what is added) in each of two chunks, and decays of at most one."""
+    inputs = [t.to(device) for t in _draw(sizes[0], 66, *sizes[1:], seed=9)]
+    inputs[3] *= 0.02  # the first chunk's tokens still count
+    lengths = [(64, 65, 66)[i % 3] for i in range(sizes[0])]
+    _, want, _ = delta_rule(*inputs, lengths=lengths)
+    with torch.no_grad():
+        _, state = gated_delta_rule(*inputs, return_state=True, key_lengths=torch.tensor(lengths, device=device))
+    assert ((state.double() - want).flatten(2).norm(dim=-1) <= 6 * 2.0**-16 * want.flatten(2).norm(dim=-1)).all()
+
+
+def test_rows_that_overlap_are_copied(device):
+    """One key for all tokens as an expanded view, rows behind each other by less than their width."""
+    q, k, v, log_decay, beta = (t.to(device) for t in _draw(2, 70, 1, 1, 32, 32, seed=7))
+    same = k[:, :, :1].expand_as(k)
+    near = v.flatten()[: 2 * 8 * 69 + 8 * 69 + 64].as_strided(v.shape, (8 * 69, 0, 8, 1))
+    with torch.no_grad():
+        want = gated_delta_rule(q, same.contiguous(), near.contiguous(), log_decay, beta)
+        assert torch.equal(gated_delta_rule(q, same, near, log_decay, beta), want)
+
+
 @pytest.mark.parametrize("sizes", [(1100, 1, 1, 32, 32), (520, 1, 1, 64, 64), (260, 1, 1, 128, 128)])
 def test_many_heads_at_the_edges_of_the_gates(device, sizes):
     q, k, v, log_decay, beta = _draw(sizes[0], 140, *sizes[1:], seed=4)
