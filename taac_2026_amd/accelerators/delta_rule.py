@@ -14,6 +14,7 @@ them, (batch, heads, tokens, width).
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -56,8 +57,14 @@ def _lengths(name: str, key_lengths: torch.Tensor | None, batch: int, device: to
     return key_lengths.to(device=device, dtype=torch.int32).contiguous()
 
 
+@functools.lru_cache(maxsize=256)
+def _stride_array(batch: int, head: int, token: int) -> ctypes.Array:
+    return _Strides(batch, head, token)
+
+
 def _strides(t: torch.Tensor) -> ctypes.Array:
-    return _Strides(*t.stride()[:3])
+    """Of (batch, head, token), for the library to read. The arrays are kept by value: a serving program repeats a few."""
+    return _stride_array(*t.stride()[:3])
 
 
 def _rows_view(t: torch.Tensor) -> torch.Tensor:
@@ -71,12 +78,16 @@ def _rows_view(t: torch.Tensor) -> torch.Tensor:
 
 def _token_major(batch: int, heads: int, tokens: int, width: int, like: torch.Tensor) -> torch.Tensor:
     """(batch, heads, tokens, width) whose memory order is (batch, tokens, heads, width): the rows of the layers around it."""
-    return like.new_empty((batch, tokens, heads, width)).transpose(1, 2)
+    return like.new_empty_strided((batch, heads, tokens, width), (tokens * heads * width, width, heads * width, 1))
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(batch: int, heads: int, tokens: int, key_width: int, value_width: int) -> int:
+    return _native.load_library().taac_delta_rule_workspace_bytes(batch, heads, tokens, key_width, value_width)
 
 
 def _workspace(k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
-    nbytes = _native.load_library().taac_delta_rule_workspace_bytes(v.shape[0], v.shape[1], v.shape[2], k.shape[3], v.shape[3])
-    return torch.empty(nbytes, dtype=torch.uint8, device=v.device)
+    return v.new_empty(_workspace_bytes(*v.shape[:3], k.shape[3], v.shape[3]), dtype=torch.uint8)
 
 
 def _forward(q, k, v, log_decay, beta, scale, lengths, initial_state, return_state, keep):
@@ -124,7 +135,7 @@ class _GatedDeltaRuleFunction(torch.autograd.Function):
         with _native.on_device(k.device):
             grad_q, grad_k = (_token_major(batch, key_heads, tokens, key_width, k) for _ in range(2))
             grad_v = _token_major(batch, heads, tokens, value_width, k)
-            grad_decay, grad_beta = (torch.empty(batch, tokens, heads, dtype=beta.dtype, device=k.device).transpose(1, 2) for _ in range(2))
+            grad_decay, grad_beta = (beta.new_empty_strided((batch, heads, tokens), (tokens * heads, 1, heads)) for _ in range(2))
             grad_states, workspace = torch.empty_like(states), _workspace(k, misses)
             status = library.taac_delta_rule_bwd(
                 q.data_ptr(), k.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), _native.ptr(lengths), states.data_ptr(),
