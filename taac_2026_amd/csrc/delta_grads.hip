@@ -140,8 +140,9 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
       return gam;
     };
     // The sums of the pairs' contributions to dG over a row and over a column are taken from the same fp32 values: pairs on one side of a
-    // token then cancel in dg as they do in the formula.
-    float dot_row = 0.f, dot_col = 0.f, dot_tail = 0.f;
+    // token then cancel in dg as they do in the formula, and a token's pair with itself stays out of both, so that a first token's decay, which
+    // acts on nothing, has a gradient of zero.
+    float dot_row = 0.f, dot_col = 0.f, dot_own = 0.f, dot_tail = 0.f;
     bf16x8 b_hi[2], b_lo[2], e_hi[2], e_lo[2];
     bf16x8 first[VB], second[VB], third[KA / 2], fourth[KA / 2];
     // this wavefront's tokens as i: dQ and R
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
           const float g = gam[r] * beta_r[r];
           bv[half][r] = row >= j ? p.scale * g * bv[half][r] : 0.f;
           ev[half][r] = row > j ? -g * ev[half][r] : 0.f;
-          dot_row += fmaf(bv[half][r], qk[r], ev[half][r] * kk[r]);
+          if (row > j) dot_row += fmaf(bv[half][r], qk[r], ev[half][r] * kk[r]);
         }
       }
       split(bv[0], bv[1], b_hi[tk], b_lo[tk]);
@@ -248,7 +249,9 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
           const int i = 16 * t + 4 * grp + r;
           bv[half][r] = i >= row ? p.scale * gam[r] * bv[half][r] : 0.f;
           ev[half][r] = i > row ? -gam[r] * ev[half][r] : 0.f;
-          dot_col += fmaf(bv[half][r], qk[r], ev[half][r] * kk[r]);
+          const float pair = fmaf(bv[half][r], qk[r], ev[half][r] * kk[r]);
+          dot_col += i > row ? pair : 0.f;
+          dot_own += i == row ? pair : 0.f;
         }
       }
       split(bv[0], bv[1], b_hi[tk], b_lo[tk]);
@@ -282,11 +285,12 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
     }
     dot_row = group_total(dot_row);
     dot_col = group_total(dot_col);
+    dot_own = group_total(dot_own);
     dot_tail = group_total(dot_tail);
     dot_state = group_sum<kWave>(dot_state);
     if (grp == 0) {
       d_total[row] = dot_row - beta_t * dot_col;
-      d_beta[row] = dot_col + dot_tail;
+      d_beta[row] = dot_col + dot_own + dot_tail;
       d_tail[row] = beta_t * dot_tail;
     }
     if (lane == 0) state_dot[wave] = dot_state;

@@ -290,6 +290,15 @@ def test_gradients_of_broadcast_inputs(device):
     torch.testing.assert_close(got[1], want[1].sum(0, keepdim=True), rtol=2.0**-7, atol=1e-2)
 
 
+@pytest.mark.parametrize("sizes", [(3, 1, 1, 32, 32), (2, 2, 4, 64, 64), (2, 1, 2, 128, 128), (600, 1, 1, 16, 16)])
+def test_the_decay_of_a_lone_token_has_no_gradient(device, sizes):
+    """It acts on a state of zeros."""
+    leaves = [t.to(device).requires_grad_(True) for t in _draw(sizes[0], 1, *sizes[1:], seed=21)]
+    out = gated_delta_rule(*leaves)
+    grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert (grads[3] == 0).all() and (grads[4] != 0).any()
+
+
 def test_results_are_reproducible(device):
     inputs = [t.to(device).requires_grad_(True) for t in _draw(20, 190, 2, 4, 64, 64, seed=16)]
     grad_out = torch.randn(20, 4, 190, 64, device=device).bfloat16()
