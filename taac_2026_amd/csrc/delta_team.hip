@@ -196,39 +196,43 @@ __device__ __forceinline__ bf16x8 get_frag(const uint8_t* frags, int f, int lane
   return *reinterpret_cast<const bf16x8*>(frags + f * kFrag + lane * 16);
 }
 
-template <int DK>
-struct TeamLds {  // fragments hi, then lo, of each
+// NT: column tiles of 16 of a team.
+template <int DK, int NT>
+struct TeamLds {  // of every column tile: fragments hi, then lo
   static constexpr int KB = DK / 32;
-  static constexpr int kState = 0;                      // KB fragments
-  static constexpr int kX = kState + 2 * KB * kFrag;    // 2
-  static constexpr int kN = kX + 4 * kFrag;
-  static constexpr int kW = kN + 4 * kFrag;
-  static constexpr int kTileK = kW + 4 * kFrag;
+  static constexpr int kStateTile = 2 * KB * kFrag, kRowTile = 4 * kFrag;
+  static constexpr int kState = 0;
+  static constexpr int kX = kState + NT * kStateTile;
+  static constexpr int kN = kX + NT * kRowTile;
+  static constexpr int kW = kN + NT * kRowTile;
+  static constexpr int kTurned = kW + NT * kRowTile;    // 320 elements of each wavefront
+  static constexpr int kTileX = kTurned + 4 * 640;
+  static constexpr int kXRow = 16 * NT + 4;             // elements of a token's columns
+  static constexpr int kTileK = (kTileX + kChunk * kXRow * 2 + 63) / 64 * 64;
   static constexpr int kForward = kTileK + Tile<DK>::BYTES;
   static constexpr int kTileQ = kForward;               // backward only
   static constexpr int kBackward = kTileQ + Tile<DK>::BYTES;
 };
 
 // What wavefront w needs of a chunk. Several of them take turns, so that nothing is copied.
-constexpr int kTeamRow = 20;  // elements of a token's 16 columns in LDS
-
-template <int KB>
+template <int KB, int NT>
 struct TeamChunk {
   bf16x8 kf[KB], qf[KB];
   bf16x8 mh[2], ml[2], pf[2];
   f32x4 grown, keep;
   float grown_row, total;
-  u32x2 x;  // four columns of a token of V (backward: of dO), on their way into LDS
+  u32x2 x[NT];  // 4 NT columns of a token of V (backward: of dO), on their way into LDS
 };
 
-template <int DK, bool COLS>
+template <int DK, int NT, bool COLS>
 struct Team {
   static constexpr int KB = DK / 32, KA = DK / 16, OWN = KA >= 4 ? KA / 4 : 1;  // OWN: state tiles of a wavefront
-  typedef TeamChunk<KB> Chunk;
+  typedef TeamChunk<KB, NT> Chunk;
+  typedef TeamLds<DK, NT> L;
   const DeltaParams& p;
   int wave, lane, l16, grp, col0, h, b, len, chunks;
   int64_t unit;
-  bool col_ok, owner;
+  bool owner;
   // The chunk that is requested next: uniform pointers that move by whole chunks, and byte offsets of this lane that stay (token strides are
   // below 2^24 elements), so that a request costs no arithmetic.
   const uint8_t *k_at, *q_at, *x_at, *block_at;
@@ -236,18 +240,17 @@ struct Team {
   int32_t k_ld, q_ld, x_ld, k_less, q_less, x_less;  // bytes from row to row, and what a row is short of that
   int at, n_at;
   Buffer block;
-  uint32_t k_off[KB], q_off[KB], x_off, frag_off[2], row_off;
+  uint32_t k_off[KB], q_off[KB], x_off[NT], frag_off[2], row_off;
 
   __device__ __forceinline__ Team(const DeltaParams& params) : p(params) {
     const int tid = threadIdx.x;
     wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     lane = tid % kWave, l16 = lane % 16, grp = lane / 16;
-    const uint32_t col_groups = (p.dv + 15) / 16;
+    const uint32_t col_groups = (p.dv + 16 * NT - 1) / (16 * NT);
     const uint32_t block = xcd_remap(blockIdx.x, gridDim.x);  // the columns of a head, which read the same rows, on one die's L2
     const uint32_t head = block / col_groups;
     unit = head;
-    col0 = static_cast<int>(block % col_groups) * 16;
-    col_ok = col0 + l16 < p.dv;
+    col0 = static_cast<int>(block % col_groups) * 16 * NT;
     h = static_cast<int>(head % static_cast<uint32_t>(p.H));
     b = static_cast<int>(head / static_cast<uint32_t>(p.H));
     len = p.T;
@@ -275,7 +278,9 @@ struct Team {
       k_off[kb] = feature < static_cast<uint32_t>(p.dk) ? (16 * wave + l16) * k_ld + feature * 2 : kNowhere;
       q_off[kb] = feature < static_cast<uint32_t>(p.dk) ? (16 * wave + l16) * q_ld + feature * 2 : kNowhere;
     }
-    x_off = col0 + lane % 4 * 4 < p.dv ? (16 * wave + lane / 4) * x_ld + lane % 4 * 8 : kNowhere;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      x_off[n] = col0 + 16 * n + lane % 4 * 4 < p.dv ? (16 * wave + lane / 4) * x_ld + 32 * n + lane % 4 * 8 : kNowhere;
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk)
       frag_off[tk] = (COLS ? tk >= wave / 2 : tk <= wave / 2) ? (COLS ? frag_cols(wave, tk) : frag_rows(wave, tk)) * kFrag + lane * 16 : kNowhere;
@@ -301,7 +306,8 @@ struct Team {
     const Buffer k = rows_at(k_at, n_at, k_ld, k_less), x = rows_at(x_at, n_at, x_ld, x_less);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) c.kf[kb] = read8(k, k_off[kb]);
-    c.x = read4(x, x_off);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) c.x[n] = read4(x, x_off[n]);
     c.grown = read_floats(block, row_off, kBlockRows + kRowGrown * 4);
     c.keep = read_floats(block, row_off, kBlockRows + kRowKeep * 4);
     if (!COLS) c.grown_row = read_float(block, l16 * 4 + wave * 64, kBlockRows + kRowGrown * 4);
@@ -325,57 +331,65 @@ struct Team {
     block_at += COLS ? -kBlockBytes : kBlockBytes;
   }
 
-  // The 16 columns of V (dO) in LDS, token by token: written behind a chunk's last use of them, read by columns.
+  // The columns of V (dO) in LDS, token by token: written behind a chunk's last use of them, read by columns.
   __device__ __forceinline__ void place(const Chunk& c, bf16_t* tile_x) const {
-    *reinterpret_cast<u32x2*>(tile_x + (16 * wave + lane / 4) * kTeamRow + lane % 4 * 4) = c.x;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) *reinterpret_cast<u32x2*>(tile_x + (16 * wave + lane / 4) * L::kXRow + 16 * n + lane % 4 * 4) = c.x[n];
   }
-  __device__ __forceinline__ bf16x4 values(const bf16_t* tile_x, int token0) const {  // tokens token0 + 4 grp .. of column l16
-    return Tile<DK>::read_tr(tile_x + (token0 + 4 * grp + l16 / 4) * kTeamRow + l16 % 4 * 4);
+  __device__ __forceinline__ bf16x4 values(const bf16_t* tile_x, int token0, int n) const {  // tokens token0 + 4 grp .. of column 16 n + l16
+    return Tile<DK>::read_tr(tile_x + (token0 + 4 * grp + l16 / 4) * L::kXRow + 16 * n + l16 % 4 * 4);
   }
+  __device__ __forceinline__ bool col_ok(int n) const { return col0 + 16 * n + l16 < p.dv; }
+  __device__ __forceinline__ bool quad_ok(int n) const { return col0 + 16 * n + 4 * grp < p.dv; }
 
   // The own rows of the state, bf16, at dst [dv][dk]
-  __device__ __forceinline__ void store_state(bf16_t* dst, const f32x4 (&s)[OWN]) const {
-    if (!owner || !col_ok) return;
-    const uint32_t off = static_cast<uint32_t>((col0 + l16) * p.dk + 8 * grp) * 2;
+  __device__ __forceinline__ void store_state(bf16_t* dst, const f32x4 (&s)[OWN][NT]) const {
+    if (!owner) return;
 #pragma unroll
-    for (int i = 0; i < OWN; ++i) {
-      const int a = wave * OWN + i;
-      if (p.dk == DK || state_row(a, 4 * grp) < p.dk) put_offset(dst + 32 * (a / 2) + 4 * (a % 2), off, round4(s[i]));
+    for (int n = 0; n < NT; ++n) {
+      if (!col_ok(n)) continue;
+      const uint32_t off = static_cast<uint32_t>((col0 + 16 * n + l16) * p.dk + 8 * grp) * 2;
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        const int a = wave * OWN + i;
+        if (p.dk == DK || state_row(a, 4 * grp) < p.dk) put_offset(dst + 32 * (a / 2) + 4 * (a % 2), off, round4(s[i][n]));
+      }
     }
   }
 };
 
-template <int DK, bool TRAIN>
+template <int DK, int NT, bool TRAIN>
 __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams p) {
-  typedef Team<DK, false> M;
-  typedef TeamLds<DK> L;
+  typedef Team<DK, NT, false> M;
+  typedef TeamLds<DK, NT> L;
   typedef Tile<DK> TK;
   constexpr int KB = M::KB, OWN = M::OWN;
-  __shared__ __attribute__((aligned(64))) uint8_t smem[L::kForward];
-  __shared__ __attribute__((aligned(16))) bf16_t turned[TRAIN ? 4 : 1][320], tile_x[kChunk * kTeamRow];
-  bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK);
+  extern __shared__ __attribute__((aligned(64))) uint8_t smem[];
+  bf16_t *tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK), *tile_x = reinterpret_cast<bf16_t*>(smem + L::kTileX);
   uint8_t *s_frags = smem + L::kState, *x_frags = smem + L::kX, *n_frags = smem + L::kN, *w_frags = smem + L::kW;
   M m(p);
   const int wave = m.wave, lane = m.lane, l16 = m.l16, grp = m.grp, col0 = m.col0;
   bf16_t* o0 = p.o + m.b * p.os[0] + m.h * p.os[1] + col0;
   const uint32_t o_off = static_cast<uint32_t>((16 * wave + l16) * p.os[2] + 4 * grp) * 2;
   const uint32_t n_off = static_cast<uint32_t>((16 * wave + l16) * p.dv + col0 + 4 * grp) * 2;
-  const bool quad_ok = col0 + 4 * grp < p.dv;
-  bf16_t* turn = turned[TRAIN ? wave : 0];
+  bf16_t* turn = reinterpret_cast<bf16_t*>(smem + L::kTurned) + wave * 320;
 
-  f32x4 s[OWN];
+  f32x4 s[OWN][NT];
 #pragma unroll
   for (int i = 0; i < OWN; ++i) {
-    s[i] = zero4();
     const int a = wave * OWN + i;
-    if (p.state_in != nullptr && m.col_ok && m.owner) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = state_row(a, 4 * grp + r);
-        if (row < p.dk) s[i][r] = p.state_in[(m.unit * p.dk + row) * p.dv + col0 + l16];
+    for (int n = 0; n < NT; ++n) {
+      s[i][n] = zero4();
+      if (p.state_in != nullptr && m.col_ok(n) && m.owner) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = state_row(a, 4 * grp + r);
+          if (row < p.dk) s[i][n][r] = p.state_in[(m.unit * p.dk + row) * p.dv + col0 + 16 * n + l16];
+        }
       }
+      if (m.owner) put_half(s_frags + n * L::kStateTile, a, lane, s[i][n], KB * kFrag);
     }
-    if (m.owner) put_half(s_frags, a, lane, s[i], KB * kFrag);
   }
 
   bf16_t* o_at = o0;
@@ -389,58 +403,68 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
       state_at += p.dk * p.dv;
     }
     // X of the own tokens; K's rows on their way into LDS
-    bf16x8 sh[KB], sl[KB];
-    f32x4 y = zero4(), y2 = zero4();
+    f32x4 x[NT], out[NT];  // out, the state's part of the output: lane = token, four columns each
+    bf16x8 sh[NT][NT > 1 ? 1 : KB], sl[NT][NT > 1 ? 1 : KB];  // of one column tile the state's fragments stay for the output
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      sh[kb] = get_frag(s_frags, kb, lane);
-      sl[kb] = get_frag(s_frags + KB * kFrag, kb, lane);
-      y = mfma16(cur.kf[kb], sh[kb], y);
-      y2 = mfma16(cur.kf[kb], sl[kb], y2);
+    for (int n = 0; n < NT; ++n) {
+      f32x4 y = zero4(), y2 = zero4();
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const bf16x8 hi = get_frag(s_frags + n * L::kStateTile, kb, lane), lo = get_frag(s_frags + n * L::kStateTile + KB * kFrag, kb, lane);
+        y = mfma16(cur.kf[kb], hi, y);
+        y2 = mfma16(cur.kf[kb], lo, y2);
+        if (NT == 1) sh[n][NT > 1 ? 0 : kb] = hi, sl[n][NT > 1 ? 0 : kb] = lo;
+      }
+      const bf16x4 v = m.values(tile_x, 16 * wave, n);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[n][r] = fmaf(-cur.grown[r], y[r] + y2[r], static_cast<float>(v[r]));
+      put_half(x_frags + n * L::kRowTile, wave, lane, x[n], 2 * kFrag);
     }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
       *reinterpret_cast<bf16x8*>(tile_k + (16 * wave + l16) * TK::STRIDE + kb * 32 + grp * 8) = cur.kf[kb];
-    f32x4 x;
-    const bf16x4 v = m.values(tile_x, 16 * wave);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = fmaf(-cur.grown[r], y[r] + y2[r], static_cast<float>(v[r]));
-    put_half(x_frags, wave, lane, x, 2 * kFrag);
     __syncthreads();
     m.fetch_queries(next);
 
     // N of the own tokens
-    f32x4 x2 = zero4(), x3 = zero4();
-#pragma unroll
-    for (int tk = 0; tk < 2; ++tk)
-      if (tk <= wave / 2) {
-        const bf16x8 xh = get_frag(x_frags, tk, lane), xl = get_frag(x_frags + 2 * kFrag, tk, lane);
-        x = mfma16(cur.mh[tk], xh, x);
-        x2 = mfma16(cur.mh[tk], xl, x2);
-        x3 = mfma16(cur.ml[tk], xh, x3);
-      }
-    f32x4 out = zero4(), out2 = zero4();  // the state's part of the output: lane = token, four columns each
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      out = mfma16(sh[kb], cur.qf[kb], out);
-      out2 = mfma16(sl[kb], cur.qf[kb], out2);
-    }
-    f32x4 w;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      x[r] += x2[r] + x3[r];
-      w[r] = x[r] * cur.keep[r];
-    }
-    put_half(w_frags, wave, lane, w, 2 * kFrag);
-    put_half(n_frags, wave, lane, x, 2 * kFrag);
-    if (TRAIN) {
-      const u32x2 rounded = turn16(turn, x, l16, grp);
-      if (16 * wave + l16 < n_tok && quad_ok) put_offset(miss_at, n_off, rounded);
-      miss_at += kChunk * p.dv;
-    }
     const float grown = cur.grown_row * p.scale;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) out[r] = (out[r] + out2[r]) * grown;
+    for (int n = 0; n < NT; ++n) {
+      const uint8_t* from = x_frags + n * L::kRowTile;
+      f32x4 x2 = zero4(), x3 = zero4();
+#pragma unroll
+      for (int tk = 0; tk < 2; ++tk)
+        if (tk <= wave / 2) {
+          const bf16x8 xh = get_frag(from, tk, lane), xl = get_frag(from + 2 * kFrag, tk, lane);
+          x[n] = mfma16(cur.mh[tk], xh, x[n]);
+          x2 = mfma16(cur.mh[tk], xl, x2);
+          x3 = mfma16(cur.ml[tk], xh, x3);
+        }
+      f32x4 out2 = zero4();
+      out[n] = zero4();
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const uint8_t* state = s_frags + n * L::kStateTile;
+        out[n] = mfma16(NT == 1 ? sh[n][NT > 1 ? 0 : kb] : get_frag(state, kb, lane), cur.qf[kb], out[n]);
+        out2 = mfma16(NT == 1 ? sl[n][NT > 1 ? 0 : kb] : get_frag(state + KB * kFrag, kb, lane), cur.qf[kb], out2);
+      }
+      f32x4 w;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[n][r] += x2[r] + x3[r];
+        w[r] = x[n][r] * cur.keep[r];
+      }
+      put_half(w_frags + n * L::kRowTile, wave, lane, w, 2 * kFrag);
+      put_half(n_frags + n * L::kRowTile, wave, lane, x[n], 2 * kFrag);
+      if (TRAIN) {
+        const u32x2 rounded = turn16(turn, x[n], l16, grp);
+        if (16 * wave + l16 < n_tok && m.quad_ok(n)) put_offset(miss_at + 16 * n, n_off, rounded);
+        if (n + 1 < NT) wave_sync();
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) out[n][r] = (out[n][r] + out2[r]) * grown;
+    }
+    if (TRAIN) miss_at += kChunk * p.dv;
     __syncthreads();
     m.fetch_block(next);
 
@@ -449,32 +473,42 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
 #pragma unroll
       for (int i = 0; i < OWN; ++i) {
         const int a = wave * OWN + i;
-        f32x4 s2 = zero4();
+        bf16x8 kt[2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[i][r] *= cur.total;
+        for (int tk = 0; tk < 2; ++tk) kt[tk] = TK::keys_frag(tile_k, tk, a, l16, grp);
 #pragma unroll
-        for (int tk = 0; tk < 2; ++tk) {
-          const bf16x8 kt = TK::keys_frag(tile_k, tk, a, l16, grp);
-          s[i] = mfma16(kt, get_frag(w_frags, tk, lane), s[i]);
-          s2 = mfma16(kt, get_frag(w_frags + 2 * kFrag, tk, lane), s2);
+        for (int n = 0; n < NT; ++n) {
+          const uint8_t* from = w_frags + n * L::kRowTile;
+          f32x4 s2 = zero4();
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[i][n][r] *= cur.total;
+#pragma unroll
+          for (int tk = 0; tk < 2; ++tk) {
+            s[i][n] = mfma16(kt[tk], get_frag(from, tk, lane), s[i][n]);
+            s2 = mfma16(kt[tk], get_frag(from + 2 * kFrag, tk, lane), s2);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[i][n][r] += s2[r];
+          put_half(s_frags + n * L::kStateTile, a, lane, s[i][n], KB * kFrag);
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[i][r] += s2[r];
-        put_half(s_frags, a, lane, s[i], KB * kFrag);
       }
     }
     // the output of the own tokens
-    out2 = zero4();
 #pragma unroll
-    for (int tk = 0; tk < 2; ++tk)
-      if (tk <= wave / 2) {
-        out = mfma16(get_frag(n_frags, tk, lane), cur.pf[tk], out);
-        out2 = mfma16(get_frag(n_frags + 2 * kFrag, tk, lane), cur.pf[tk], out2);
+    for (int n = 0; n < NT; ++n) {
+      const uint8_t* from = n_frags + n * L::kRowTile;
+      f32x4 out2 = zero4();
+#pragma unroll
+      for (int tk = 0; tk < 2; ++tk)
+        if (tk <= wave / 2) {
+          out[n] = mfma16(get_frag(from, tk, lane), cur.pf[tk], out[n]);
+          out2 = mfma16(get_frag(from + 2 * kFrag, tk, lane), cur.pf[tk], out2);
+        }
+      if (16 * wave + l16 < n_tok && m.quad_ok(n)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) out[n][r] += out2[r];
+        put_offset(o_at + 16 * n, o_off, round4(out[n]));
       }
-    if (16 * wave + l16 < n_tok && quad_ok) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) out[r] += out2[r];
-      put_offset(o_at, o_off, round4(out));
     }
     o_at += kChunk * p.os[2];
     m.place(next, tile_x);
@@ -496,47 +530,50 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
   }
   if (chunk < m.chunks) step(chunk, even, odd);
 
-  if (p.state_out != nullptr && m.col_ok && m.owner) {
+  if (p.state_out != nullptr && m.owner) {
 #pragma unroll
     for (int i = 0; i < OWN; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = state_row(wave * OWN + i, 4 * grp + r);
-        if (row < p.dk) p.state_out[(m.unit * p.dk + row) * p.dv + col0 + l16] = s[i][r];
-      }
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = state_row(wave * OWN + i, 4 * grp + r);
+          if (row < p.dk && m.col_ok(n)) p.state_out[(m.unit * p.dk + row) * p.dv + col0 + 16 * n + l16] = s[i][n][r];
+        }
   }
   const bf16x4 none = {};
-  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.T - m.len) * 4; i += 4 * kWave) {
-    const int at = static_cast<int>(i % 4) * 4;
-    if (col0 + at < p.dv) *reinterpret_cast<bf16x4*>(o0 + (m.len + i / 4) * p.os[2] + at) = none;
+  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.T - m.len) * 4 * NT; i += 4 * kWave) {
+    const int at = static_cast<int>(i % (4 * NT)) * 4;
+    if (col0 + at < p.dv) *reinterpret_cast<bf16x4*>(o0 + (m.len + i / (4 * NT)) * p.os[2] + at) = none;
   }
 }
 
 // The gradient of the state, chunks last to first (the formulas: delta.h). Stages: beta dU (own tokens) | dX (own tokens) | dS (own
 // rows). dO is read as fragments by every wavefront.
-template <int DK>
+template <int DK, int NT>
 __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaParams p) {
-  typedef Team<DK, true> M;
-  typedef TeamLds<DK> L;
+  typedef Team<DK, NT, true> M;
+  typedef TeamLds<DK, NT> L;
   typedef Tile<DK> TK;
   constexpr int KB = M::KB, OWN = M::OWN;
-  __shared__ __attribute__((aligned(64))) uint8_t smem[L::kBackward];
-  __shared__ __attribute__((aligned(16))) bf16_t turned[4][320], tile_x[kChunk * kTeamRow];
-  bf16_t* tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK);
-  bf16_t* tile_q = reinterpret_cast<bf16_t*>(smem + L::kTileQ);
+  extern __shared__ __attribute__((aligned(64))) uint8_t smem[];
+  bf16_t *tile_k = reinterpret_cast<bf16_t*>(smem + L::kTileK), *tile_q = reinterpret_cast<bf16_t*>(smem + L::kTileQ),
+         *tile_x = reinterpret_cast<bf16_t*>(smem + L::kTileX);
   uint8_t *s_frags = smem + L::kState, *z_frags = smem + L::kX, *x_frags = smem + L::kN, *o_frags = smem + L::kW;
   M m(p);
   const int wave = m.wave, lane = m.lane, l16 = m.l16, grp = m.grp, col0 = m.col0;
+  bf16_t* turn = reinterpret_cast<bf16_t*>(smem + L::kTurned) + wave * 320;
   bf16_t* v0 = p.grad_v + m.b * p.dvs[0] + m.h * p.dvs[1] + col0;
   const uint32_t v_off = static_cast<uint32_t>((16 * wave + l16) * p.dvs[2] + 4 * grp) * 2;
-  const bool quad_ok = col0 + 4 * grp < p.dv;
 
-  f32x4 s[OWN];
+  f32x4 s[OWN][NT];
 #pragma unroll
-  for (int i = 0; i < OWN; ++i) {
-    s[i] = zero4();
-    if (m.owner) put_half(s_frags, wave * OWN + i, lane, s[i], KB * kFrag);
-  }
+  for (int i = 0; i < OWN; ++i)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      s[i][n] = zero4();
+      if (m.owner) put_half(s_frags + n * L::kStateTile, wave * OWN + i, lane, s[i][n], KB * kFrag);
+    }
 
   bf16_t* v_at = v0 + (m.chunks - 1) * kChunk * p.dvs[2];
   bf16_t* state_at = p.grad_states + (m.unit * p.chunks + m.chunks - 1) * static_cast<int64_t>(p.dk) * p.dv;
@@ -546,53 +583,61 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
     m.store_state(state_at, s);
     state_at -= p.dk * p.dv;
     // beta dU of the own tokens
-    f32x4 z = zero4(), z2 = zero4(), z3 = zero4();
+    f32x4 z[NT];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      z = mfma16(cur.kf[kb], get_frag(s_frags, kb, lane), z);
-      z2 = mfma16(cur.kf[kb], get_frag(s_frags + KB * kFrag, kb, lane), z2);
-    }
+    for (int n = 0; n < NT; ++n) {
+      f32x4 z2 = zero4(), z3 = zero4();
+      z[n] = zero4();
 #pragma unroll
-    for (int tk = 0; tk < 2; ++tk)
-      if (tk >= wave / 2) {
-        z3 = mfma16(cur.pf[tk], TK::join(m.values(tile_x, 32 * tk), m.values(tile_x, 32 * tk + 16)), z3);
+      for (int kb = 0; kb < KB; ++kb) {
+        z[n] = mfma16(cur.kf[kb], get_frag(s_frags + n * L::kStateTile, kb, lane), z[n]);
+        z2 = mfma16(cur.kf[kb], get_frag(s_frags + n * L::kStateTile + KB * kFrag, kb, lane), z2);
       }
+#pragma unroll
+      for (int tk = 0; tk < 2; ++tk)
+        if (tk >= wave / 2) z3 = mfma16(cur.pf[tk], TK::join(m.values(tile_x, 32 * tk, n), m.values(tile_x, 32 * tk + 16, n)), z3);
+      f32x4 w;
+      const bf16x4 own = m.values(tile_x, 16 * wave, n);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        z[n][r] = fmaf(cur.keep[r], z[n][r] + z2[r], z3[r]);
+        w[r] = p.scale * cur.grown[r] * static_cast<float>(own[r]);
+      }
+      put_half(z_frags + n * L::kRowTile, wave, lane, z[n], 2 * kFrag);
+      put_half(o_frags + n * L::kRowTile, wave, lane, w, 2 * kFrag);
+    }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int at = (16 * wave + l16) * TK::STRIDE + kb * 32 + grp * 8;
       *reinterpret_cast<bf16x8*>(tile_k + at) = cur.kf[kb];
       *reinterpret_cast<bf16x8*>(tile_q + at) = cur.qf[kb];
     }
-    f32x4 w;
-    const bf16x4 own = m.values(tile_x, 16 * wave);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      z[r] = fmaf(cur.keep[r], z[r] + z2[r], z3[r]);
-      w[r] = p.scale * cur.grown[r] * static_cast<float>(own[r]);
-    }
-    put_half(z_frags, wave, lane, z, 2 * kFrag);
-    put_half(o_frags, wave, lane, w, 2 * kFrag);
     __syncthreads();
     m.fetch_queries(next);
 
     // dX of the own tokens
-    z2 = z3 = zero4();
 #pragma unroll
-    for (int tk = 0; tk < 2; ++tk)
-      if (tk >= wave / 2) {
-        const bf16x8 zh = get_frag(z_frags, tk, lane), zl = get_frag(z_frags + 2 * kFrag, tk, lane);
-        z = mfma16(cur.mh[tk], zh, z);
-        z2 = mfma16(cur.mh[tk], zl, z2);
-        z3 = mfma16(cur.ml[tk], zh, z3);
+    for (int n = 0; n < NT; ++n) {
+      const uint8_t* from = z_frags + n * L::kRowTile;
+      f32x4 z2 = zero4(), z3 = zero4(), w;
+#pragma unroll
+      for (int tk = 0; tk < 2; ++tk)
+        if (tk >= wave / 2) {
+          const bf16x8 zh = get_frag(from, tk, lane), zl = get_frag(from + 2 * kFrag, tk, lane);
+          z[n] = mfma16(cur.mh[tk], zh, z[n]);
+          z2 = mfma16(cur.mh[tk], zl, z2);
+          z3 = mfma16(cur.ml[tk], zh, z3);
+        }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        z[n][r] += z2[r] + z3[r];
+        w[r] = -cur.grown[r] * z[n][r];
       }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      z[r] += z2[r] + z3[r];
-      w[r] = -cur.grown[r] * z[r];
+      put_half(x_frags + n * L::kRowTile, wave, lane, w, 2 * kFrag);
+      const u32x2 rounded = turn16(turn, z[n], l16, grp);
+      if (16 * wave + l16 < n_tok && m.quad_ok(n)) put_offset(v_at + 16 * n, v_off, rounded);
+      if (n + 1 < NT) wave_sync();
     }
-    put_half(x_frags, wave, lane, w, 2 * kFrag);
-    const u32x2 rounded = turn16(turned[wave], z, l16, grp);
-    if (16 * wave + l16 < n_tok && quad_ok) put_offset(v_at, v_off, rounded);
     v_at -= kChunk * p.dvs[2];
     __syncthreads();
     m.fetch_block(next);
@@ -602,20 +647,26 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
 #pragma unroll
       for (int i = 0; i < OWN; ++i) {
         const int a = wave * OWN + i;
-        f32x4 s2 = zero4(), s3 = zero4(), s4 = zero4();
+        bf16x8 kt[2], qt[2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[i][r] *= cur.total;
+        for (int tk = 0; tk < 2; ++tk) kt[tk] = TK::keys_frag(tile_k, tk, a, l16, grp), qt[tk] = TK::keys_frag(tile_q, tk, a, l16, grp);
 #pragma unroll
-        for (int tk = 0; tk < 2; ++tk) {
-          const bf16x8 kt = TK::keys_frag(tile_k, tk, a, l16, grp), qt = TK::keys_frag(tile_q, tk, a, l16, grp);
-          s[i] = mfma16(kt, get_frag(x_frags, tk, lane), s[i]);
-          s2 = mfma16(kt, get_frag(x_frags + 2 * kFrag, tk, lane), s2);
-          s3 = mfma16(qt, get_frag(o_frags, tk, lane), s3);
-          s4 = mfma16(qt, get_frag(o_frags + 2 * kFrag, tk, lane), s4);
+        for (int n = 0; n < NT; ++n) {
+          const uint8_t *from_x = x_frags + n * L::kRowTile, *from_o = o_frags + n * L::kRowTile;
+          f32x4 s2 = zero4(), s3 = zero4(), s4 = zero4();
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[i][n][r] *= cur.total;
+#pragma unroll
+          for (int tk = 0; tk < 2; ++tk) {
+            s[i][n] = mfma16(kt[tk], get_frag(from_x, tk, lane), s[i][n]);
+            s2 = mfma16(kt[tk], get_frag(from_x + 2 * kFrag, tk, lane), s2);
+            s3 = mfma16(qt[tk], get_frag(from_o, tk, lane), s3);
+            s4 = mfma16(qt[tk], get_frag(from_o + 2 * kFrag, tk, lane), s4);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[i][n][r] += (s2[r] + s4[r]) + s3[r];
+          put_half(s_frags + n * L::kStateTile, a, lane, s[i][n], KB * kFrag);
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[i][r] += (s2[r] + s4[r]) + s3[r];
-        put_half(s_frags, a, lane, s[i], KB * kFrag);
       }
     }
     m.place(next, tile_x);
@@ -635,31 +686,41 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
     step(chunk - 1, odd, even);
   }
   if (chunk == 0) step(0, even, odd);
-  const bf16_t none = static_cast<bf16_t>(0.f);
-  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.T - m.len) * 16; i += 4 * kWave) {
-    const int at = static_cast<int>(i % 16);
-    if (col0 + at < p.dv) v0[(m.len + i / 16) * p.dvs[2] + at] = none;
+  const bf16x4 none = {};
+  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.T - m.len) * 4 * NT; i += 4 * kWave) {
+    const int at = static_cast<int>(i % (4 * NT)) * 4;
+    if (col0 + at < p.dv) *reinterpret_cast<bf16x4*>(v0 + (m.len + i / (4 * NT)) * p.dvs[2] + at) = none;
   }
 }
 
-template <int DK, bool COLS>
+template <typename K>
+int launch_columns(const char* name, K* kernel, const DeltaParams& p, int64_t teams, int lds, hipStream_t s) {
+  if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+    return set_error(TAAC_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS", name, lds);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(teams)), dim3(4 * kWave), lds, s, p);
+  return check_launch(name);
+}
+
+template <int DK, int NT, bool COLS>
 int launch_team(const char* name, const DeltaParams& p, hipStream_t s) {
-  const int64_t heads = static_cast<int64_t>(p.B) * p.H, teams = heads * ((p.dv + 15) / 16);
+  typedef TeamLds<DK, NT> L;
+  const int64_t heads = static_cast<int64_t>(p.B) * p.H, teams = heads * ((p.dv + 16 * NT - 1) / (16 * NT));
   if (heads * p.chunks > 0x7fffffffLL || teams > 0x7fffffffLL) return set_error(TAAC_ERR_UNSUPPORTED, "%s: too many workgroups", name);
   if (p.chunks > 0) hipLaunchKernelGGL((delta_blocks_kernel<DK, COLS>), dim3(static_cast<uint32_t>(heads * p.chunks)), dim3(kWave), 0, s, p);
-  const dim3 grid(static_cast<uint32_t>(teams)), threads(4 * kWave);
-  if constexpr (COLS) hipLaunchKernelGGL((delta_team_back_kernel<DK>), grid, threads, 0, s, p);
-  else if (p.chunk_states != nullptr) hipLaunchKernelGGL((delta_team_kernel<DK, true>), grid, threads, 0, s, p);
-  else hipLaunchKernelGGL((delta_team_kernel<DK, false>), grid, threads, 0, s, p);
-  return check_launch(name);
+  if constexpr (COLS) return launch_columns(name, delta_team_back_kernel<DK, NT>, p, teams, L::kBackward, s);
+  else if (p.chunk_states != nullptr) return launch_columns(name, delta_team_kernel<DK, NT, true>, p, teams, L::kForward, s);
+  else return launch_columns(name, delta_team_kernel<DK, NT, false>, p, teams, L::kForward, s);
 }
 
 }  // namespace
 
 int delta_team(const char* name, const DeltaParams& p, bool back, hipStream_t s) {
-  if (p.dk <= 32) return back ? launch_team<32, true>(name, p, s) : launch_team<32, false>(name, p, s);
-  if (p.dk <= 64) return back ? launch_team<64, true>(name, p, s) : launch_team<64, false>(name, p, s);
-  return back ? launch_team<128, true>(name, p, s) : launch_team<128, false>(name, p, s);
+  if (p.dk <= 32) return back ? launch_team<32, 1, true>(name, p, s) : launch_team<32, 1, false>(name, p, s);
+  if (p.dk <= 64) return back ? launch_team<64, 1, true>(name, p, s) : launch_team<64, 1, false>(name, p, s);
+  // Two teams run on a CU at once: where there would be more of 16 columns, teams of 32, which read the keys and the blocks half as often.
+  if (p.dv > 16 && static_cast<int64_t>(p.B) * p.H * ((p.dv + 15) / 16) > 512)
+    return back ? launch_team<128, 2, true>(name, p, s) : launch_team<128, 2, false>(name, p, s);
+  return back ? launch_team<128, 1, true>(name, p, s) : launch_team<128, 1, false>(name, p, s);
 }
 
 }  // namespace taac
