@@ -61,7 +61,8 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
   float* d_tail = d_beta + 64;     // its share of dG_64
   float* state_dot = d_tail + 64;  // per wavefront
 
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const uint32_t key_heads = static_cast<uint32_t>(p.H) / p.group;
   const int chunk = static_cast<int>(blockIdx.x % static_cast<uint32_t>(p.chunks));
   const uint32_t pair = blockIdx.x / static_cast<uint32_t>(p.chunks);
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
     const int64_t unit = static_cast<int64_t>(b) * p.H + h;
     // opaque to the compiler, which would otherwise keep the LDS addresses of the whole loop body in registers across the heads
     int l16 = lane % 16, grp = lane / 16;
-    asm volatile("" : "+v"(l16), "+v"(grp));
+    asm volatile("" : "+v"(l16), "+v"(grp), "+v"(tid));
     const int row = 16 * wave + l16;  // this lane's token
     // everything this head reads is requested before any of it is waited for
     typename TV::template Piece<kChunk, kThreads> o_in, x_in, n_in;
@@ -209,15 +210,15 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
         dot_row = fmaf(static_cast<float>(qv[r]), dq[r], fmaf(static_cast<float>(kv[r]), dr[r], dot_row));
       }
 #pragma unroll
-      for (int tk = 0; tk < 2; ++tk) {
-        const bf16x8 kt = TK::keys_frag(tile_k, tk, a, l16, grp);
-        dq = mfma16(kt, b_lo[tk], mfma16(kt, b_hi[tk], dq));
-        dr = mfma16(kt, e_lo[tk], mfma16(kt, e_hi[tk], dr));
-      }
-#pragma unroll
       for (int r = 0; r < 4; ++r) {
         dq_sum[a][r] += dq[r];
         dk_sum[a][r] += dr[r];
+      }
+#pragma unroll
+      for (int tk = 0; tk < 2; ++tk) {
+        const bf16x8 kt = TK::keys_frag(tile_k, tk, a, l16, grp);
+        dq_sum[a] = mfma16(kt, b_lo[tk], mfma16(kt, b_hi[tk], dq_sum[a]));
+        dk_sum[a] = mfma16(kt, e_lo[tk], mfma16(kt, e_hi[tk], dk_sum[a]));
       }
       __builtin_amdgcn_sched_barrier(0);  // keeps the next round's reads, and their registers, behind this one
     }
@@ -254,6 +255,10 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
           dot_own += i == row ? pair : 0.f;
         }
       }
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bv[half][r] *= beta_t, ev[half][r] *= beta_t;
       split(bv[0], bv[1], b_hi[tk], b_lo[tk]);
       split(ev[0], ev[1], e_hi[tk], e_lo[tk]);
       __builtin_amdgcn_sched_barrier(0);
@@ -274,13 +279,13 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
         dot_tail = fmaf(static_cast<float>(kv[r]), dc[r], dot_tail);
       }
 #pragma unroll
+      for (int r = 0; r < 4; ++r) dk_sum[a][r] = fmaf(beta_t, dc[r], dk_sum[a][r]);
+#pragma unroll
       for (int tk = 0; tk < 2; ++tk) {
         const bf16x8 kt = TK::keys_frag(tile_k, tk, a, l16, grp), qt = TK::keys_frag(tile_q, tk, a, l16, grp);
-        dc = mfma16(qt, b_lo[tk], mfma16(qt, b_hi[tk], dc));
-        dc = mfma16(kt, e_lo[tk], mfma16(kt, e_hi[tk], dc));
+        dk_sum[a] = mfma16(qt, b_lo[tk], mfma16(qt, b_hi[tk], dk_sum[a]));
+        dk_sum[a] = mfma16(kt, e_lo[tk], mfma16(kt, e_hi[tk], dk_sum[a]));
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) dk_sum[a][r] = fmaf(beta_t, dc[r], dk_sum[a][r]);
       __builtin_amdgcn_sched_barrier(0);
     }
     dot_row = group_total(dot_row);
