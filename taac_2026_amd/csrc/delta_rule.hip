@@ -12,7 +12,7 @@ namespace {
 bool uses_teams(int64_t heads, int32_t dk, int32_t dv) { return dk > 64 || heads * ((dv + 15) / 16) <= (dk <= 32 ? 512 : 768); }
 
 int64_t workspace_of(int64_t heads, int32_t T, int32_t dk, int32_t dv) {
-  return uses_teams(heads, dk, dv) ? heads * ((T + kChunk - 1) / kChunk) * kBlockBytes : 0;
+  return uses_teams(heads, dk, dv) ? heads * ((static_cast<int64_t>(T) + kChunk - 1) / kChunk) * kBlockBytes : 0;
 }
 
 int take_workspace(const char* name, DeltaParams& p, void* workspace, int64_t given, bool* team) {
@@ -27,6 +27,7 @@ int take_workspace(const char* name, DeltaParams& p, void* workspace, int64_t gi
 int check_sizes(const char* name, const DeltaParams& p) {
   if (p.B < 0 || p.H <= 0 || p.T < 0 || p.dk <= 0 || p.dv <= 0 || p.group <= 0)
     return set_error(TAAC_ERR_INVALID_VALUE, "%s: batch and tokens must be >= 0, heads and widths > 0", name);
+  if (p.T > 1 << 30) return set_error(TAAC_ERR_UNSUPPORTED, "%s: at most 2^30 tokens (got %d)", name, p.T);  // 32-bit token numbers
   if (p.dk % 8 != 0 || p.dv % 8 != 0 || p.dk > 128 || p.dv > 128)
     return set_error(TAAC_ERR_UNSUPPORTED, "%s: key and value widths must be multiples of 8, at most 128 (got %d, %d)", name, p.dk, p.dv);
   return TAAC_OK;
@@ -62,8 +63,8 @@ extern "C" int taac_delta_rule_fwd(const void* q, const void* k, const void* v, 
   if (key_heads <= 0 || H <= 0 || H % key_heads != 0)
     return set_error(TAAC_ERR_INVALID_VALUE, "%s: value heads must be a multiple of the key heads", name);
   p.B = B, p.H = H, p.group = H / key_heads, p.T = T, p.dk = dk, p.dv = dv, p.scale = scale;
-  p.chunks = (T + kChunk - 1) / kChunk;
   if (int rc = check_sizes(name, p)) return rc;
+  p.chunks = (T + kChunk - 1) / kChunk;
   if (gate_dtype != TAAC_F32 && gate_dtype != TAAC_BF16)
     return set_error(TAAC_ERR_INVALID_VALUE, "%s: gates must be fp32 or bf16 (dtype %d)", name, gate_dtype);
   p.gates_f32 = gate_dtype == TAAC_F32;
@@ -102,8 +103,8 @@ extern "C" int taac_delta_rule_bwd(const void* q, const void* k, const void* log
   if (key_heads <= 0 || H <= 0 || H % key_heads != 0)
     return set_error(TAAC_ERR_INVALID_VALUE, "%s: value heads must be a multiple of the key heads", name);
   p.B = B, p.H = H, p.group = H / key_heads, p.T = T, p.dk = dk, p.dv = dv, p.scale = scale;
-  p.chunks = (T + kChunk - 1) / kChunk;
   if (int rc = check_sizes(name, p)) return rc;
+  p.chunks = (T + kChunk - 1) / kChunk;
   if (gate_dtype != TAAC_F32 && gate_dtype != TAAC_BF16)
     return set_error(TAAC_ERR_INVALID_VALUE, "%s: gates must be fp32 or bf16 (dtype %d)", name, gate_dtype);
   p.gates_f32 = gate_dtype == TAAC_F32;

@@ -362,6 +362,51 @@ def test_offsets_beyond_32_bits(device):
         assert torch.equal(gated_delta_rule_step(*views, *inputs[3:], torch.zeros(2, 1, 32, 32, device=device)), want)
 
 
+@pytest.mark.parametrize("sizes", [(70, 1, 1, 128, 128), (3, 1, 2, 96, 72), (600, 1, 1, 32, 32), (200, 1, 1, 64, 64)])
+def test_replayed_graph_of_the_other_forms(device, sizes):
+    """Wide heads, few and many, and heads that walk alone: forward and backward, replayed on new inputs with eager work in between."""
+    leaves = [t.to(device).requires_grad_(True) for t in _draw(sizes[0], 100, *sizes[1:], seed=60)]
+    lengths = torch.tensor([(i * 13) % 101 for i in range(sizes[0])], dtype=torch.int32, device=device)
+    grad_out = torch.randn(leaves[2].shape, device=device).bfloat16()
+
+    def work(inputs):
+        out = gated_delta_rule(*inputs, key_lengths=lengths)
+        return (out, *torch.autograd.grad(out, inputs, grad_out))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = work(leaves)
+    for seed in range(3):
+        new = [t.to(device) for t in _draw(sizes[0], 100, *sizes[1:], seed=61 + seed)]
+        with torch.no_grad():
+            for leaf, t in zip(leaves, new):
+                leaf.copy_(t)
+            lengths.copy_(lengths.roll(1))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = work([t.requires_grad_(True) for t in new])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(results, want))
+
+
+@pytest.mark.parametrize("sizes", [(2, 1, 2, 128, 128), (600, 1, 1, 32, 32), (90, 1, 1, 128, 128)])
+def test_states_of_empty_histories(device, sizes):
+    """No tokens at all, and samples without any."""
+    for tokens in (0, 70):
+        inputs = [t.to(device) for t in _draw(sizes[0], tokens, *sizes[1:], seed=70)]
+        state = torch.randn(sizes[0], sizes[2], *sizes[3:], device=device)
+        with torch.inference_mode():
+            out, final = gated_delta_rule(*inputs, initial_state=state, return_state=True,
+                                          key_lengths=torch.zeros(sizes[0], dtype=torch.int64, device=device))
+            assert torch.equal(final, state) and (out == 0).all()
+
+
 def test_replayed_graph(device):
     """Forward, backward and step captured together, replayed on new inputs with eager work in between."""
     def fresh(seed):

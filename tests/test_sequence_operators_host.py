@@ -109,6 +109,8 @@ def test_delta_entry_points_check_on_the_host():
     assert forward(states=fake) == invalid and b"come together" in library.taac_last_error()
     assert forward(q=None) == invalid and forward(q=odd) == invalid
     assert forward(qs=strides(80, 80, 12)) == invalid and forward(gs=strides(10, 5, -1)) == invalid and forward(qs=None) == invalid
+    assert forward(qs=strides(80, 80, 8)) == invalid and b"cover a row" in library.taac_last_error()
+    assert forward(qs=strides(80, 80, 1 << 24)) == unsupported and forward(T=(1 << 30) + 1) == unsupported
     assert forward(B=0) == ok and forward(T=0) == ok
     need = library.taac_delta_rule_workspace_bytes(1, 2, 5, 16, 8)
     assert need > 0 and library.taac_delta_rule_workspace_bytes(1, 0, 5, 16, 8) == -1
@@ -127,4 +129,5 @@ def test_delta_entry_points_check_on_the_host():
     assert step(dk=4) == unsupported and step(dtype=7) == invalid and step(gate=f16) == invalid
     assert step(slots=None, B=5) == invalid and b"without slots" in library.taac_last_error()
     assert step(qs=strides(16, -16, 16)) == invalid and step(qs=None) == invalid
+    assert step(B=(1 << 28) + 1, H=1, pool=1 << 40) == unsupported and b"2^28" in library.taac_last_error()
     assert step(B=0) == ok and step(T=0) == ok
