@@ -608,24 +608,24 @@ int taac_row_rstd(const float* qk_sumsq, int64_t M, int32_t d_model, float eps, 
  *   S <- a S,   S <- S + k (beta (v - S^T k))^T,   o = scale S^T q.
  * q, k: bf16, logical (B, key_heads, T, dk); v, o: bf16 (B, H, T, dv), H a multiple of key_heads (value head h uses key head
  * h / (H / key_heads)); log_decay, beta: (B, H, T) of gate_dtype (TAAC_F32 or TAAC_BF16). *_strides: ELEMENT strides of (batch, head,
- * token); the features of a row are contiguous, q / k / v / o have strides that are multiples of 8 and 16-byte aligned bases. dk and
- * dv: multiples of 8, at most 128. lengths: int32 [B] or NULL; tokens at or beyond a sample's length are not read, leave the
+ * token), not negative; the features of a row are contiguous, q / k / v / o have strides that are multiples of 8, token strides from a row's
+ * width to below 2^24, and 16-byte aligned bases. dk and dv: multiples of 8, at most 128; T at most 2^30. lengths: int32 [B] or NULL; tokens at or beyond a sample's length are not read, leave the
  * state alone and get zeros in o. Keys should have at most unit length and beta lie in [0, 1], as the recurrence needs to stay
- * bounded; log_decay is normally <= 0, values below -1e5 count as -1e5.
+ * bounded; log_decay is normally <= 0, values below -1e5 count as -1e5. Infinities and NaN of a valid token reach the whole chunk of 64
+ * tokens that it lies in, the tokens in front of it too, and everything behind it in its (sample, head).
  * state_in: fp32 [B, H, dk, dv] or NULL (zeros); state_out: the same shape, or NULL; it may be state_in.
  * chunk_states (bf16 [B, H, ceil(T / 64), dv, dk]) and misses (bf16 [B, H, T, dv]): what taac_delta_rule_bwd reads, or both NULL.
  * taac_delta_rule_bwd: gradients of q, k, v, log_decay and beta (logical shapes and dtypes of the inputs, strides of their own) for
  * grad_o; grad_states (bf16, the size of chunk_states) is scratch. The initial state has no gradient here. Rows at or beyond a
  * sample's length get zeros. Every sum has a fixed order.
- * workspace: taac_delta_rule_workspace_bytes(B, H, T, dk, dv) bytes, 16-byte aligned, for either call (0 with many heads, whose
- * workgroups need none; -1: bad sizes). Calls in flight together must not share one.
+ * workspace: taac_delta_rule_workspace_bytes(B, H, T, dk, dv) bytes, 16-byte aligned, for either call (0: none, as with many heads of at
+ * most 64 key features; -1: bad sizes). Calls in flight together must not share one.
  * Replaces: the reference's chunked gated delta rule (accelerators/attention/kernels/gated_delta_rule).
  */
 int64_t taac_delta_rule_workspace_bytes(int32_t B, int32_t H, int32_t T, int32_t dk, int32_t dv);
 int taac_delta_rule_fwd(const void* q, const void* k, const void* v, const void* log_decay, const void* beta, const int32_t* lengths,
                         void* o, const float* state_in, float* state_out, void* chunk_states, void* misses, void* workspace,
-                        int64_t workspace_bytes, int32_t B, int32_t H,
-                        int32_t key_heads, int32_t T, int32_t dk, int32_t dv, const int64_t q_strides[3], const int64_t k_strides[3],
+                        int64_t workspace_bytes, int32_t B, int32_t H, int32_t key_heads, int32_t T, int32_t dk, int32_t dv, const int64_t q_strides[3], const int64_t k_strides[3],
                         const int64_t v_strides[3], const int64_t o_strides[3], const int64_t decay_strides[3],
                         const int64_t beta_strides[3], float scale, int gate_dtype, void* stream);
 int taac_delta_rule_bwd(const void* q, const void* k, const void* log_decay, const void* beta, const int32_t* lengths,

@@ -5,6 +5,10 @@
 // at a time from memory and walks them as two chunks of 32, which need a third of the fp32 products of one chunk of 64: the four
 // diagonal blocks of 16 are still solved at once, a column per lane, but only one block below the diagonal is left per chunk
 // instead of six per 64 tokens. Scores are made where they are used.
+//
+// 1024 samples x 8 heads x 512 tokens, 32 wide, forward: 222 us, 4.8 TB/s, the rate of a large copy. 512 x 4 x 512, 64 wide: 202 us with the
+// states and misses of training (4.0 TB/s), 178 us backward (3.8 TB/s); there one wavefront per SIMD fills the registers, and a third of
+// its time goes to waits that no other wavefront covers. Two per SIMD spill and take 10 % longer.
 #include "delta.h"
 
 namespace taac {

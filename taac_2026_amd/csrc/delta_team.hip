@@ -1,11 +1,16 @@
-// Gated delta rule, chunked form, for few heads and long histories (the mathematics, operand order and precision: delta.h).
+// Gated delta rule, chunked form, for few or wide heads and long histories (the mathematics, operand order and precision: delta.h).
 //
 // With few (sample, head) pairs the time is the chain of chunks, not the work: what does not depend on the state is made for all
 // chunks at once (one wavefront each) and left in memory, and a chunk's step of the state is spread over four wavefronts to make it
-// short. A workgroup has 16 value columns; wavefront w owns tokens 16 w .. 16 w + 15 of every chunk and a quarter of the key rows
-// of the state. A step is three stages with a barrier behind each,
+// short. A workgroup has 16 (or 32) value columns; wavefront w owns tokens 16 w .. 16 w + 15 of every chunk and a quarter of the key
+// rows of the state. A step is three stages with a barrier behind each,
 //   X (own tokens) from the state | N (own tokens) from X | the state (own rows) from N; the output beside them,
-// whose results meet in LDS as operand fragments. Everything a chunk reads from memory is requested one chunk ahead.
+// whose results meet in LDS as operand fragments. Everything a chunk reads from memory is requested one chunk ahead, a third beside
+// each stage.
+//
+// 2 samples x 16 heads x 8192 tokens, 128 wide: 36 us for the blocks (145 MB, 4.0 TB/s) and 187 us for 128 steps of 1.5 us (305 us with masked
+// reads in one run at a step's start). A step is a chain of eight dependent matrix instructions and three exchanges through LDS, among
+// 310 instructions that every wavefront issues: bound by that chain, the matrix units are busy for a seventh of it.
 #include "delta.h"
 
 namespace taac {
