@@ -227,13 +227,6 @@ struct Tile {
   }
 };
 
-// A result (lane: column l16, rows 4 grp ..) rounded and turned (lane: row l16, columns 4 grp ..) through 16 rows of 20 elements in LDS.
-__device__ __forceinline__ u32x2 turn16(bf16_t* at, const f32x4& v, int l16, int grp) {
-  *reinterpret_cast<u32x2*>(at + l16 * 20 + grp * 4) = round4(v);
-  wave_sync();
-  return __builtin_bit_cast(u32x2, Tile<32>::read_tr(at + (4 * grp + l16 / 4) * 20 + (l16 % 4) * 4));
-}
-
 // 16 x 16 fp32 products on v_mfma_f32_16x16x4_f32, contraction index 4 grp + step. A matrix Y is held "by rows" (lane: row l16, columns
 // 4 grp ..) or "by columns" (lane: column l16, rows 4 grp ..).
 __device__ __forceinline__ f32x4 mul_cols(const f32x4& x_rows, const f32x4& y_cols, f32x4 acc) {  // X Y by columns

@@ -210,13 +210,13 @@ struct TeamLds {  // of every column tile: fragments hi, then lo
   static constexpr int kX = kState + NT * kStateTile;
   static constexpr int kN = kX + NT * kRowTile;
   static constexpr int kW = kN + NT * kRowTile;
-  static constexpr int kTurned = kW + NT * kRowTile;    // 320 elements of each wavefront
-  static constexpr int kTileX = kTurned + 4 * 640;
+  static constexpr int kTileX = kW + NT * kRowTile;
   static constexpr int kXRow = 16 * NT + 4;             // elements of a token's columns
   static constexpr int kTileK = (kTileX + kChunk * kXRow * 2 + 63) / 64 * 64;
   static constexpr int kForward = kTileK + Tile<DK>::BYTES;
   static constexpr int kTileQ = kForward;               // backward only
-  static constexpr int kBackward = kTileQ + Tile<DK>::BYTES;
+  static constexpr int kDX = kTileQ + Tile<DK>::BYTES;  // dX, high parts only
+  static constexpr int kBackward = kDX + NT * 2 * kFrag;
 };
 
 // What wavefront w needs of a chunk. Several of them take turns, so that nothing is copied.
@@ -377,7 +377,8 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
   bf16_t* o0 = p.o + m.b * p.os[0] + m.h * p.os[1] + col0;
   const uint32_t o_off = static_cast<uint32_t>((16 * wave + l16) * p.os[2] + 4 * grp) * 2;
   const uint32_t n_off = static_cast<uint32_t>((16 * wave + l16) * p.dv + col0 + 4 * grp) * 2;
-  bf16_t* turn = reinterpret_cast<bf16_t*>(smem + L::kTurned) + wave * 320;
+  // Lane (column c, tokens 4 q ..) of a half fragment holds four tokens: read_tr over the lanes c = 4 grp + l16 / 4, q = l16 % 4.
+  const uint32_t turned_at = (wave / 2) * kFrag + (l16 % 4 * 16 + 4 * grp + l16 / 4) * 16 + wave % 2 * 8;
 
   f32x4 s[OWN][NT];
 #pragma unroll
@@ -461,15 +462,9 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
       }
       put_half(w_frags + n * L::kRowTile, wave, lane, w, 2 * kFrag);
       put_half(n_frags + n * L::kRowTile, wave, lane, x[n], 2 * kFrag);
-      if (TRAIN) {
-        const u32x2 rounded = turn16(turn, x[n], l16, grp);
-        if (16 * wave + l16 < n_tok && m.quad_ok(n)) put_offset(miss_at + 16 * n, n_off, rounded);
-        if (n + 1 < NT) wave_sync();
-      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) out[n][r] = (out[n][r] + out2[r]) * grown;
     }
-    if (TRAIN) miss_at += kChunk * p.dv;
     __syncthreads();
     m.fetch_block(next);
 
@@ -514,6 +509,14 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
         for (int r = 0; r < 4; ++r) out[n][r] += out2[r];
         put_offset(o_at + 16 * n, o_off, round4(out[n]));
       }
+    }
+    if (TRAIN) {  // N of the own tokens, rounded as its fragments' high parts are, by rows
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const bf16x4 rounded = TK::read_tr(reinterpret_cast<const bf16_t*>(n_frags + n * L::kRowTile + turned_at));
+        if (16 * wave + l16 < n_tok && m.quad_ok(n)) put_offset(miss_at + 16 * n, n_off, rounded);
+      }
+      miss_at += kChunk * p.dv;
     }
     o_at += kChunk * p.os[2];
     m.place(next, tile_x);
@@ -567,7 +570,8 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
   uint8_t *s_frags = smem + L::kState, *z_frags = smem + L::kX, *x_frags = smem + L::kN, *o_frags = smem + L::kW;
   M m(p);
   const int wave = m.wave, lane = m.lane, l16 = m.l16, grp = m.grp, col0 = m.col0;
-  bf16_t* turn = reinterpret_cast<bf16_t*>(smem + L::kTurned) + wave * 320;
+  uint8_t* dx_frags = smem + L::kDX;
+  const uint32_t turned_at = (wave / 2) * kFrag + (l16 % 4 * 16 + 4 * grp + l16 / 4) * 16 + wave % 2 * 8;  // as in the forward
   bf16_t* v0 = p.grad_v + m.b * p.dvs[0] + m.h * p.dvs[1] + col0;
   const uint32_t v_off = static_cast<uint32_t>((16 * wave + l16) * p.dvs[2] + 4 * grp) * 2;
 
@@ -639,11 +643,8 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
         w[r] = -cur.grown[r] * z[n][r];
       }
       put_half(x_frags + n * L::kRowTile, wave, lane, w, 2 * kFrag);
-      const u32x2 rounded = turn16(turn, z[n], l16, grp);
-      if (16 * wave + l16 < n_tok && m.quad_ok(n)) put_offset(v_at + 16 * n, v_off, rounded);
-      if (n + 1 < NT) wave_sync();
+      *reinterpret_cast<u32x2*>(dx_frags + n * 2 * kFrag + (wave / 2) * kFrag + lane * 16 + wave % 2 * 8) = round4(z[n]);
     }
-    v_at -= kChunk * p.dvs[2];
     __syncthreads();
     m.fetch_block(next);
 
@@ -674,6 +675,12 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
         }
       }
     }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bf16x4 rounded = TK::read_tr(reinterpret_cast<const bf16_t*>(dx_frags + n * 2 * kFrag + turned_at));
+      if (16 * wave + l16 < n_tok && m.quad_ok(n)) put_offset(v_at + 16 * n, v_off, rounded);
+    }
+    v_at -= kChunk * p.dvs[2];
     m.place(next, tile_x);
     __syncthreads();
   };
