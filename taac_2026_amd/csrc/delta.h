@@ -114,12 +114,6 @@ __device__ __forceinline__ bf16x8 zero8() {
   return __builtin_bit_cast(bf16x8, z);
 }
 
-// Writes through a uniform base and a 32-bit offset of the lane, which stays the same for every chunk (token strides are below 2^24 elements).
-template <typename T, typename V>
-__device__ __forceinline__ void put_offset(T* base, uint32_t bytes, const V& v) {
-  *reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(base) + bytes) = v;
-}
-
 // Reads and writes through a buffer descriptor: bytes at or beyond its end read as zero and are not written, so that rows behind the last
 // token need neither a branch nor a mask, and a wait for one read counts everything requested since. kNowhere: an offset behind every end (64
 // rows of less than 2^24 elements end below it), so also for features or columns that there are not.

@@ -345,21 +345,29 @@ struct Team {
     return Tile<DK>::read_tr(tile_x + (token0 + 4 * grp + l16 / 4) * L::kXRow + 16 * n + l16 % 4 * 4);
   }
   __device__ __forceinline__ bool col_ok(int n) const { return col0 + 16 * n + l16 < p.dv; }
-  __device__ __forceinline__ bool quad_ok(int n) const { return col0 + 16 * n + 4 * grp < p.dv; }
 
-  // The own rows of the state, bf16, at dst [dv][dk]
-  __device__ __forceinline__ void store_state(bf16_t* dst, const f32x4 (&s)[OWN][NT]) const {
-    if (!owner) return;
+  // Writes without branches, as the reads. The own rows of the state, bf16, at dst [dv][dk]:
+  __device__ __forceinline__ void state_offsets(uint32_t (&off)[OWN][NT]) const {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if (!col_ok(n)) continue;
-      const uint32_t off = static_cast<uint32_t>((col0 + 16 * n + l16) * p.dk + 8 * grp) * 2;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < OWN; ++i) {
-        const int a = wave * OWN + i;
-        if (p.dk == DK || state_row(a, 4 * grp) < p.dk) put_offset(dst + 32 * (a / 2) + 4 * (a % 2), off, round4(s[i][n]));
+        const int row = state_row(wave * OWN + i, 4 * grp);
+        off[i][n] = owner && col_ok(n) && row < p.dk ? static_cast<uint32_t>((col0 + 16 * n + l16) * p.dk + row) * 2 : kNowhere;
       }
-    }
+  }
+  __device__ __forceinline__ void store_state(bf16_t* dst, const uint32_t (&off)[OWN][NT], const f32x4 (&s)[OWN][NT]) const {
+    const Buffer to = buffer_of(dst, static_cast<uint32_t>(p.dk * p.dv) * 2);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) write4(to, off[i][n], round4(s[i][n]));
+  }
+  // four columns of the own token in rows ld elements apart
+  __device__ __forceinline__ void quad_offsets(int64_t ld, uint32_t (&off)[NT]) const {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      off[n] = col0 + 16 * n + 4 * grp < p.dv ? static_cast<uint32_t>((16 * wave + l16) * ld + 16 * n + 4 * grp) * 2 : kNowhere;
   }
 };
 
@@ -375,8 +383,10 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
   M m(p);
   const int wave = m.wave, lane = m.lane, l16 = m.l16, grp = m.grp, col0 = m.col0;
   bf16_t* o0 = p.o + m.b * p.os[0] + m.h * p.os[1] + col0;
-  const uint32_t o_off = static_cast<uint32_t>((16 * wave + l16) * p.os[2] + 4 * grp) * 2;
-  const uint32_t n_off = static_cast<uint32_t>((16 * wave + l16) * p.dv + col0 + 4 * grp) * 2;
+  uint32_t o_off[NT], n_off[NT], s_off[OWN][NT];
+  m.quad_offsets(p.os[2], o_off);
+  m.quad_offsets(p.dv, n_off);
+  m.state_offsets(s_off);
   // Lane (column c, tokens 4 q ..) of a half fragment holds four tokens: read_tr over the lanes c = 4 grp + l16 / 4, q = l16 % 4.
   const uint32_t turned_at = (wave / 2) * kFrag + (l16 % 4 * 16 + 4 * grp + l16 / 4) * 16 + wave % 2 * 8;
 
@@ -400,12 +410,12 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
 
   bf16_t* o_at = o0;
   bf16_t* state_at = TRAIN ? p.chunk_states + m.unit * p.chunks * static_cast<int64_t>(p.dk) * p.dv : nullptr;
-  bf16_t* miss_at = TRAIN ? p.misses + m.unit * p.T * p.dv : nullptr;
+  bf16_t* miss_at = TRAIN ? p.misses + m.unit * p.T * p.dv + col0 : nullptr;
   auto step = [&](int chunk, typename M::Chunk& cur, typename M::Chunk& next) __attribute__((always_inline)) {
     const int n_tok = m.tokens_of(chunk);
     m.fetch_keys(next);
     if (TRAIN) {
-      m.store_state(state_at, s);
+      m.store_state(state_at, s_off, s);
       state_at += p.dk * p.dv;
     }
     // X of the own tokens; K's rows on their way into LDS
@@ -494,6 +504,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
       }
     }
     // the output of the own tokens
+    const Buffer to = rows_buffer(o_at, p.os[2], n_tok, p.dv - col0);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const uint8_t* from = n_frags + n * L::kRowTile;
@@ -504,17 +515,16 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
           out[n] = mfma16(get_frag(from, tk, lane), cur.pf[tk], out[n]);
           out2 = mfma16(get_frag(from + 2 * kFrag, tk, lane), cur.pf[tk], out2);
         }
-      if (16 * wave + l16 < n_tok && m.quad_ok(n)) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) out[n][r] += out2[r];
-        put_offset(o_at + 16 * n, o_off, round4(out[n]));
-      }
+      for (int r = 0; r < 4; ++r) out[n][r] += out2[r];
+      write4(to, o_off[n], round4(out[n]));
     }
     if (TRAIN) {  // N of the own tokens, rounded as its fragments' high parts are, by rows
+      const Buffer misses = rows_buffer(miss_at, p.dv, n_tok, p.dv - col0);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const bf16x4 rounded = TK::read_tr(reinterpret_cast<const bf16_t*>(n_frags + n * L::kRowTile + turned_at));
-        if (16 * wave + l16 < n_tok && m.quad_ok(n)) put_offset(miss_at + 16 * n, n_off, rounded);
+        write4(misses, n_off[n], __builtin_bit_cast(u32x2, rounded));
       }
       miss_at += kChunk * p.dv;
     }
@@ -573,7 +583,9 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
   uint8_t* dx_frags = smem + L::kDX;
   const uint32_t turned_at = (wave / 2) * kFrag + (l16 % 4 * 16 + 4 * grp + l16 / 4) * 16 + wave % 2 * 8;  // as in the forward
   bf16_t* v0 = p.grad_v + m.b * p.dvs[0] + m.h * p.dvs[1] + col0;
-  const uint32_t v_off = static_cast<uint32_t>((16 * wave + l16) * p.dvs[2] + 4 * grp) * 2;
+  uint32_t v_off[NT], s_off[OWN][NT];
+  m.quad_offsets(p.dvs[2], v_off);
+  m.state_offsets(s_off);
 
   f32x4 s[OWN][NT];
 #pragma unroll
@@ -589,7 +601,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
   auto step = [&](int chunk, typename M::Chunk& cur, typename M::Chunk& next) __attribute__((always_inline)) {
     const int n_tok = m.tokens_of(chunk);
     m.fetch_keys(next);
-    m.store_state(state_at, s);
+    m.store_state(state_at, s_off, s);
     state_at -= p.dk * p.dv;
     // beta dU of the own tokens
     f32x4 z[NT];
@@ -675,10 +687,11 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
         }
       }
     }
+    const Buffer to = rows_buffer(v_at, p.dvs[2], n_tok, p.dv - col0);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const bf16x4 rounded = TK::read_tr(reinterpret_cast<const bf16_t*>(dx_frags + n * 2 * kFrag + turned_at));
-      if (16 * wave + l16 < n_tok && m.quad_ok(n)) put_offset(v_at + 16 * n, v_off, rounded);
+      write4(to, v_off[n], __builtin_bit_cast(u32x2, rounded));
     }
     v_at -= kChunk * p.dvs[2];
     m.place(next, tile_x);
