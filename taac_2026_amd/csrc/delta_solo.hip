@@ -6,9 +6,10 @@
 // diagonal blocks of 16 are still solved at once, a column per lane, but only one block below the diagonal is left per chunk
 // instead of six per 64 tokens. Scores are made where they are used.
 //
-// 1024 samples x 8 heads x 512 tokens, 32 wide, forward: 222 us, 4.8 TB/s, the rate of a large copy. 512 x 4 x 512, 64 wide: 202 us with the
-// states and misses of training (4.0 TB/s), 178 us backward (3.8 TB/s); there one wavefront per SIMD fills the registers, and a third of
-// its time goes to waits that no other wavefront covers. Two per SIMD spill and take 10 % longer.
+// Bound by instruction issue. 1024 samples x 8 heads of up to 512 tokens (276 at the mean), 32 wide, forward: 218 us, 3.4 TB/s; two wavefronts per
+// SIMD issue in 85 % of the cycles, vector instructions in 59 %, nearly half of those for the hi and lo of fp32 operands. 512 x 4 heads of
+// up to 512, 64 wide: 198 us with the states and misses of training, 174 us backward; there one wavefront per SIMD fills the registers (two
+// spill and take 10 % longer), and 40 % of its time goes to waits that no other wavefront covers.
 #include "delta.h"
 
 namespace taac {
@@ -44,9 +45,12 @@ struct Solo {
   const DeltaParams& p;
   int lane, l16, grp, col0, h, b, len, groups;
   int64_t unit;
-  const bf16_t *k0, *q0, *x0;
+  // The 64 tokens that are requested next: uniform pointers that move by whole groups, and byte offsets of this lane.
+  const uint8_t *k_at, *q_at, *x_at;
+  int64_t k_step, q_step, x_step;
+  int32_t k_ld, q_ld, x_ld, k_less, q_less, x_less;  // bytes from row to row, and what a row is short of that
+  int at;
   uint32_t k_off[KB], q_off[KB], state_off[KB], x_off;
-  int64_t x_ld;
 
   __device__ __forceinline__ Solo(const DeltaParams& params) : p(params) {
     lane = threadIdx.x, l16 = lane % 16, grp = lane / 16;
@@ -65,11 +69,15 @@ struct Solo {
     groups = (len + kChunk - 1) / kChunk;
     const int64_t hk = h / p.group;
     const int64_t* xs = BACK ? p.dos : p.vs;
-    x_ld = xs[2];
-    k0 = p.k + b * p.ks[0] + hk * p.ks[1];
-    q0 = p.q + b * p.qs[0] + hk * p.qs[1];
-    x0 = (BACK ? p.grad_o : p.v) + b * xs[0] + h * xs[1] + col0;
-    const uint32_t k_ld = static_cast<uint32_t>(p.ks[2]) * 2, q_ld = static_cast<uint32_t>(p.qs[2]) * 2;
+    at = BACK ? groups - 1 : 0;
+    const int64_t first = static_cast<int64_t>(at) * kChunk;
+    k_at = reinterpret_cast<const uint8_t*>(p.k + b * p.ks[0] + hk * p.ks[1] + first * p.ks[2]);
+    q_at = reinterpret_cast<const uint8_t*>(p.q + b * p.qs[0] + hk * p.qs[1] + first * p.qs[2]);
+    x_at = reinterpret_cast<const uint8_t*>((BACK ? p.grad_o : p.v) + b * xs[0] + h * xs[1] + col0 + first * xs[2]);
+    constexpr int64_t kMove = (BACK ? -kChunk : kChunk) * 2;
+    k_step = kMove * p.ks[2], q_step = kMove * p.qs[2], x_step = kMove * xs[2];
+    k_ld = static_cast<int32_t>(p.ks[2]) * 2, q_ld = static_cast<int32_t>(p.qs[2]) * 2, x_ld = static_cast<int32_t>(xs[2]) * 2;
+    k_less = k_ld - p.dk * 2, q_less = q_ld - p.dk * 2, x_less = x_ld - (p.dv - col0) * 2;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const bool there = kb * 32 + grp * 8 < p.dk;
@@ -78,34 +86,37 @@ struct Solo {
       state_off[kb] = there ? static_cast<uint32_t>(l16 * p.dk + 32 * kb + 8 * grp) * 2 : kNowhere;
     }
     const int piece = lane % 4;
-    x_off = col0 + piece * 8 < p.dv ? static_cast<uint32_t>(lane / 4 * x_ld) * 2 + piece * 16 : kNowhere;
+    x_off = col0 + piece * 8 < p.dv ? static_cast<uint32_t>(lane / 4 * x_ld) + piece * 16 : kNowhere;
   }
   __device__ __forceinline__ int tokens_of(int group) const {
     const int left = len - group * kChunk;
     return left < kChunk ? left : kChunk;
   }
 
-  // Beside the tokens of a group; of a group that there is not, nothing (zeros).
-  __device__ __forceinline__ void fetch(int group, SoloTokens<DK>& c) const {
-    const int n_tok = group >= 0 ? tokens_of(group) : 0;
-    const int64_t token0 = n_tok > 0 ? static_cast<int64_t>(group) * kChunk : 0;
-    const bf16_t *k = k0 + token0 * p.ks[2], *q = q0 + token0 * p.qs[2], *x = x0 + token0 * x_ld;
-    c.gates.request(p, b, h, token0, n_tok, lane);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const Buffer kt = rows_buffer(k + t * 16 * p.ks[2], p.ks[2], n_tok - 16 * t, p.dk);
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) c.kf[t][kb] = read8(kt, k_off[kb]);
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) c.x[t] = read8(rows_buffer(x + t * 16 * x_ld, x_ld, n_tok - 16 * t, p.dv - col0), x_off);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const Buffer qt = rows_buffer(q + t * 16 * p.qs[2], p.qs[2], n_tok - 16 * t, p.dk);
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) c.qf[t][kb] = read8(qt, q_off[kb]);
-    }
+  // The first n rows at a base; none where n is not positive.
+  static __device__ __forceinline__ Buffer rows_at(const uint8_t* base, int n, int32_t ld, int32_t less) {
+    const int32_t bytes = n * ld - less;
+    return buffer_of(base, bytes > 0 ? bytes : 0);
   }
+  // The tokens of a group, then on to the next; behind the last group, zeros.
+  __device__ __forceinline__ void fetch(SoloTokens<DK>& c) {
+    const int n = at >= 0 ? tokens_of(at) : 0;
+    c.gates.request(p, b, h, static_cast<int64_t>(at) * kChunk, n, lane);
+    const Buffer k = rows_at(k_at, n, k_ld, k_less), q = rows_at(q_at, n, q_ld, q_less), x = rows_at(x_at, n, x_ld, x_less);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) c.kf[t][kb] = read8(k, k_off[kb] + t * 16 * k_ld);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c.x[t] = read8(x, x_off + t * 16 * x_ld);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) c.qf[t][kb] = read8(q, q_off[kb] + t * 16 * q_ld);
+    at += BACK ? -1 : 1;
+    k_at += k_step, q_at += q_step, x_at += x_step;
+  }
+
   // The tokens' factors and rows into LDS.
   __device__ __forceinline__ void place(const SoloTokens<DK>& c, int n_tok, float* rows, bf16_t* tile_k, bf16_t* tile_x) const {
 #pragma unroll
@@ -259,16 +270,15 @@ struct Solo {
   }
   // the state's high parts at dst [dv][dk]
   __device__ __forceinline__ void store_state(bf16_t* dst, const bf16x8 (&sh)[KB][kNT]) const {
+    const Buffer to = rows_buffer(dst + col0 * p.dk, p.dk, p.dv - col0, p.dk);
 #pragma unroll
-    for (int n = 0; n < kNT; ++n) {
-      const Buffer to = rows_buffer(dst + (col0 + 16 * n) * p.dk, p.dk, p.dv - col0 - 16 * n, p.dk);
+    for (int n = 0; n < kNT; ++n)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) write8(to, state_off[kb], sh[kb][n]);
-    }
+      for (int kb = 0; kb < KB; ++kb) write8(to, state_off[kb] + n * p.dk * 32, sh[kb][n]);
   }
-  // Rows of one chunk of 32 tokens, held by columns, at dst (its row 0, this wavefront's first column; off: quads()): turned through tile's rows,
-  // which have been read.
-  __device__ __forceinline__ void store_rows(bf16_t* dst, int64_t ld, const uint32_t (&off)[kNT], bf16_t* tile, const f32x4 (&x)[2][kNT], int n_tok) const {
+  // Rows of one chunk of 32 tokens, held by columns, to rows of a group from tile `first` on (off: quads(); pitch: bytes of 16 rows): turned through
+  // tile's rows, which have been read.
+  __device__ __forceinline__ void store_rows(Buffer to, uint32_t pitch, const uint32_t (&off)[kNT], int first, bf16_t* tile, const f32x4 (&x)[2][kNT]) const {
     u32x2 v[2][kNT];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -281,11 +291,9 @@ struct Solo {
       for (int n = 0; n < kNT; ++n)
         v[t][n] = __builtin_bit_cast(u32x2, TV::read_tr(tile + (2 * t + n) * 320 + (4 * grp + l16 / 4) * 20 + (l16 % 4) * 4));
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const Buffer to = rows_buffer(dst + 16 * t * ld, ld, n_tok - 16 * t, p.dv - col0);
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int n = 0; n < kNT; ++n) write4(to, off[n], v[t][n]);
-    }
+      for (int n = 0; n < kNT; ++n) write4(to, off[n] + (first + t) * pitch, v[t][n]);
   }
   // Byte offsets of four columns of token l16 in rows ld elements apart.
   __device__ __forceinline__ void quads(int64_t ld, uint32_t (&off)[kNT]) const {
@@ -308,9 +316,10 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
   bf16_t* tile_v = reinterpret_cast<bf16_t*>(smem + L::kTileV);
   bf16_t* tile_q = reinterpret_cast<bf16_t*>(smem + L::kTileQ);
   float* scratch = reinterpret_cast<float*>(smem + L::kTileQ);
-  const W w(p);
+  W w(p);
   const int lane = w.lane, l16 = w.l16, grp = w.grp, col0 = w.col0;
   bf16_t* o0 = p.o + w.b * p.os[0] + w.h * p.os[1] + col0;
+  const uint32_t o_pitch = static_cast<uint32_t>(p.os[2]) * 32;  // bytes of 16 rows
   uint32_t o_off[kNT], n_off[kNT];
   w.quads(p.os[2], o_off);
   w.quads(p.dv, n_off);
@@ -331,16 +340,18 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
     }
 
   SoloTokens<DK> c;
-  if (w.groups > 0) w.fetch(0, c);
+  if (w.groups > 0) w.fetch(c);
   for (int group = 0; group < w.groups; ++group) {
     const int64_t token0 = static_cast<int64_t>(group) * kChunk;
     const int n_tok = w.tokens_of(group);
+    const Buffer to = rows_buffer(o0 + token0 * p.os[2], p.os[2], n_tok, p.dv - col0);
+    const Buffer misses = rows_buffer(p.misses + (w.unit * p.T + token0) * p.dv + col0, p.dv, TRAIN ? n_tok : 0, p.dv - col0);
     wave_sync();  // the previous tokens' tiles are read
     w.place(c, n_tok, rows, tile_k, tile_v);
     bf16x8 mh[4], ml[4];
     w.solve(c, rows, scratch, mh, ml);
     w.place_queries(c, tile_q);
-    w.fetch(group + 1, c);
+    w.fetch(c);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (half == 1 && n_tok <= kHalf) break;
@@ -379,7 +390,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
         for (int n = 0; n < kNT; ++n)
           x[t][n] = mfma16(ml[2 * half + t], xh[n], mfma16(mh[2 * half + t], xl[n], mfma16(mh[2 * half + t], xh[n], x[t][n])));
       if (TRAIN)
-        w.store_rows(p.misses + (w.unit * p.T + token0 + 32 * half) * p.dv + col0, p.dv, n_off, tile_v + 32 * half * TV::STRIDE, x, n_tok - 32 * half);
+        w.store_rows(misses, p.dv * 32, n_off, 2 * half, tile_v + 32 * half * TV::STRIDE, x);
       // the output by columns of tokens: lane = token, four value columns each
 #pragma unroll
       for (int n = 0; n < kNT; ++n) split(x[0][n], x[1][n], xh[n], xl[n]);
@@ -409,13 +420,12 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
 #pragma unroll
           for (int n = 0; n < kNT; ++n) out[n] = mfma16(sl[kb][n], qf[kb], mfma16(sh[kb][n], qf[kb], out[n]));
         const float grown = rows[kSoloGrown + 16 * ti + l16] * p.scale;
-        const Buffer to = rows_buffer(o0 + (token0 + 16 * ti) * p.os[2], p.os[2], n_tok - 16 * ti, p.dv - col0);
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) out[n][r] *= grown;
           out[n] = mfma16(xl[n], pf, mfma16(xh[n], pf, out[n]));
-          write4(to, o_off[n], round4(out[n]));
+          write4(to, o_off[n] + ti * o_pitch, round4(out[n]));
         }
       }
       // S' = e^G_last S + K^T (beta e^(G_last - G) N)
@@ -475,9 +485,10 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
   bf16_t* tile_q = reinterpret_cast<bf16_t*>(smem + L::kTileQ);
   bf16_t* tile_o = reinterpret_cast<bf16_t*>(smem + L::kTileV);
   float* scratch = reinterpret_cast<float*>(smem + L::kTileQ);
-  const W w(p);
+  W w(p);
   const int lane = w.lane, l16 = w.l16, grp = w.grp, col0 = w.col0;
   bf16_t* v0 = p.grad_v + w.b * p.dvs[0] + w.h * p.dvs[1] + col0;
+  const uint32_t v_pitch = static_cast<uint32_t>(p.dvs[2]) * 32;
   uint32_t v_off[kNT];
   w.quads(p.dvs[2], v_off);
 
@@ -488,16 +499,17 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
     for (int n = 0; n < kNT; ++n) s[a][n] = zero4();
 
   SoloTokens<DK> c;
-  if (w.groups > 0) w.fetch(w.groups - 1, c);
+  if (w.groups > 0) w.fetch(c);
   for (int group = w.groups - 1; group >= 0; --group) {
     const int64_t token0 = static_cast<int64_t>(group) * kChunk;
     const int n_tok = w.tokens_of(group);
+    const Buffer to = rows_buffer(v0 + token0 * p.dvs[2], p.dvs[2], n_tok, p.dv - col0);
     wave_sync();
     w.place(c, n_tok, rows, tile_k, tile_o);
     bf16x8 mh[4], ml[4];
     w.solve(c, rows, scratch, mh, ml);
     w.place_queries(c, tile_q);
-    w.fetch(group - 1, c);
+    w.fetch(c);
 #pragma unroll
     for (int back = 0; back < 2; ++back) {
       const int half = 1 - back;
@@ -550,7 +562,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
 #pragma unroll
         for (int n = 0; n < kNT; ++n)
           z[t][n] = mfma16(ml[2 * half + t], zh[n], mfma16(mh[2 * half + t], zl[n], mfma16(mh[2 * half + t], zh[n], z[t][n])));
-      w.store_rows(v0 + (token0 + 32 * half) * p.dvs[2], p.dvs[2], v_off, tile_o + 32 * half * TV::STRIDE, z, n_tok - 32 * half);
+      w.store_rows(to, v_pitch, v_off, 2 * half, tile_o + 32 * half * TV::STRIDE, z);
       // dS
       bf16x8 wh[kNT], wl[kNT];
       const f32x4 g0 = *reinterpret_cast<const f32x4*>(rows + kSoloGrown + 32 * half + 4 * grp);
