@@ -160,8 +160,8 @@ struct Solo {
     wave_sync();
   }
 
-  // Gam_ij beta_j of a tile of 16 x 16, by rows (lane: token i = l16 of tile ti, tokens j = 4 grp .. of tile tj), 0 for j > i; strict: for j >= i.
-  __device__ __forceinline__ f32x4 decays_by_rows(const float* rows, int ti, int tj, bool strict) const {
+  // Gam_ij beta_j of a tile of 16 x 16, by rows (lane: token i = l16 of tile ti, tokens j = 4 grp .. of tile tj); of a diagonal one, whatever for j > i.
+  __device__ __forceinline__ f32x4 decays_by_rows(const float* rows, int ti, int tj) const {
     f32x4 gam;
     if (ti > tj) {
       const float in_i = rows[kSoloIn + 16 * ti + l16];
@@ -174,11 +174,7 @@ struct Solo {
       const f32x4 lo_j = *reinterpret_cast<const f32x4*>(rows + kSoloLow + 16 * tj + 4 * grp);
       const f32x4 beta_j = *reinterpret_cast<const f32x4*>(rows + kSoloBeta + 16 * tj + 4 * grp);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = 4 * grp + r;
-        const float e = __builtin_amdgcn_exp2f((hi_i - hi_j[r]) + (lo_i - lo_j[r])) * beta_j[r];
-        gam[r] = (strict ? l16 > j : l16 >= j) ? e : 0.f;
-      }
+      for (int r = 0; r < 4; ++r) gam[r] = __builtin_amdgcn_exp2f((hi_i - hi_j[r]) + (lo_i - lo_j[r])) * beta_j[r];
     }
     return gam;
   }
@@ -203,17 +199,19 @@ struct Solo {
     return gam;
   }
 
-  // -M of both chunks as operand fragments, hi and lo: by rows (forward), fragment t = row tile t; by columns (backward), column tile t.
-  __device__ __forceinline__ void solve(const SoloTokens<DK>& c, const float* rows, float* scratch, bf16x8 (&mh)[4], bf16x8 (&ml)[4]) const {
+  // -M of both chunks as operand fragments, hi and lo: by rows (forward), fragment t = row tile t; by columns (backward), column tile t. own: the
+  // diagonal tiles' decays, which the forward's scores take too.
+  __device__ __forceinline__ void solve(const SoloTokens<DK>& c, const float* rows, float* scratch, bf16x8 (&mh)[4], bf16x8 (&ml)[4],
+                                        f32x4 (&own)[4]) const {
     f32x4 low[2];  // the blocks below the diagonal, by rows
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       f32x4 kk = zero4();
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) kk = mfma16(c.kf[t][kb], c.kf[t][kb], kk);
-      const f32x4 gam = decays_by_rows(rows, t, t, true);
+      own[t] = decays_by_rows(rows, t, t);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) kk[r] *= gam[r];
+      for (int r = 0; r < 4; ++r) kk[r] = l16 > 4 * grp + r ? kk[r] * own[t][r] : 0.f;
       *reinterpret_cast<f32x4*>(scratch + t * kScratchBlock + l16 * kScratchRow + 4 * grp) = kk;
     }
     wave_sync();
@@ -222,7 +220,7 @@ struct Solo {
       low[s] = zero4();
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) low[s] = mfma16(c.kf[2 * s][kb], c.kf[2 * s + 1][kb], low[s]);
-      const f32x4 gam = decays_by_rows(rows, 2 * s + 1, 2 * s, true);
+      const f32x4 gam = decays_by_rows(rows, 2 * s + 1, 2 * s);
 #pragma unroll
       for (int r = 0; r < 4; ++r) low[s][r] *= gam[r];
     }
@@ -349,7 +347,8 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
     wave_sync();  // the previous tokens' tiles are read
     w.place(c, n_tok, rows, tile_k, tile_v);
     bf16x8 mh[4], ml[4];
-    w.solve(c, rows, scratch, mh, ml);
+    f32x4 own[4];
+    w.solve(c, rows, scratch, mh, ml, own);
     w.place_queries(c, tile_q);
     w.fetch(c);
 #pragma unroll
@@ -407,9 +406,9 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
           if (u > t) continue;
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) score[u] = mfma16(TK::row(tile_k, 16 * (2 * half + u) + l16, kb, grp), qf[kb], score[u]);
-          const f32x4 gam = w.decays_by_rows(rows, ti, 2 * half + u, false);
+          const f32x4 gam = u == t ? own[ti] : w.decays_by_rows(rows, ti, 2 * half + u);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) score[u][r] *= p.scale * gam[r];
+          for (int r = 0; r < 4; ++r) score[u][r] = u < t || l16 >= 4 * grp + r ? score[u][r] * (p.scale * gam[r]) : 0.f;
         }
         const bf16x8 pf = round8(score[0], score[1]);
         f32x4 out[kNT];
@@ -507,7 +506,8 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
     wave_sync();
     w.place(c, n_tok, rows, tile_k, tile_o);
     bf16x8 mh[4], ml[4];
-    w.solve(c, rows, scratch, mh, ml);
+    f32x4 own[4];
+    w.solve(c, rows, scratch, mh, ml, own);
     w.place_queries(c, tile_q);
     w.fetch(c);
 #pragma unroll
