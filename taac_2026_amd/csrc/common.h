@@ -78,11 +78,11 @@ int attn_out_ffn_readout(const void* attn, int64_t ld_attn, int attn_plane, cons
                          int64_t ldo, int64_t M, int32_t D, int32_t F, const int32_t* rows, const int32_t* n_rows,
                          int norm_folded, const void* head_w, float* token_dots, void* split_scratch, void* stream);
 // Token-stationary e4m3 dense layer (fp8_ts.hip): TAAC_OK after a launch, a negative status on an error, 1 when the shape
-// is not covered and the caller must use the tiled kernel.
+// is not covered and the caller must use the tiled kernel. row_amax: amax_a holds one maximum per row of an e4m3 a.
 int launch_linear_fp8_ts(const void* a, int a_is_fp8, int64_t lda, const void* w, const float* amax_a,
                          const float* amax_w, const void* bias, const void* residual, void* out, int64_t ldo,
                          int64_t M, int32_t N, int32_t K, int epilogue, int gate_first, hipStream_t s,
-                         const char* name);
+                         const char* name, bool row_amax);
 
 // taac_swiglu_ffn_fp8_fwd that also writes the dot product of every stored row with head_w [D] (16-byte aligned; no amax_next
 // then) to token_dots[row]; null: no readout.

@@ -94,9 +94,13 @@ __device__ __forceinline__ void lds_wait_halves(u32x4& a, u32x4& b) {
 // the rounded output over the steps of a tile, and from them the maximum over all tokens of |rmsnorm(out) * weight| - the
 // per-tensor scale of the layer that consumes the output - without a pass of its own over it.
 // NORM: the rows are RMS-normalised (weight p.norm_w) before they are quantised.
-template <int kK, int EPI, bool A_FP8, bool STATS, bool NORM = false>
+// ROWS: p.amax_a holds one maximum per row of a (which is e4m3 already): a lane's accumulators of a token tile belong to one token, whose scale
+// is read with its row. 131072 rows, 256 -> 768 and 256 -> 1024 gated features: 53 and 107 us, 49 and 102 with one maximum for all, 87 and 186
+// by the tiled kernel.
+template <int kK, int EPI, bool A_FP8, bool STATS, bool NORM = false, bool ROWS = false>
 __global__ __launch_bounds__(kWaves * kWave, 2) void linear_fp8_ts_kernel(const Fp8TsParams p) {
   static_assert(!NORM || (kK == 256 && !A_FP8), "the normalisation is built for bf16 rows of 256 features");
+  static_assert(!ROWS || A_FP8, "rows with scales of their own arrive quantised");
   constexpr bool RES = EPI == TAAC_EPI_RESIDUAL;
   constexpr int kTT = tiles_per_wave(kK, EPI);
   constexpr int kTokPerWg = kWaves * 32 * kTT;
@@ -161,7 +165,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void linear_fp8_ts_kernel(const 
   bf16_t* outw_lds = normw_lds + kK;            // [N]
   float* red = reinterpret_cast<float*>(outw_lds + p.N);
 
-  const float amax_a = fmaxf(*p.amax_a, 1e-12f);
+  const float amax_a = ROWS ? 448.0f : fmaxf(*p.amax_a, 1e-12f);
   const float amax_w = fmaxf(*p.amax_w, 1e-12f);
   const float inv_scale_a = 448.0f / amax_a;
   const float dq = (amax_a / 448.0f) * (amax_w / 448.0f);
@@ -207,11 +211,13 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void linear_fp8_ts_kernel(const 
   };
   // Token rows -> e4m3 B-operand fragments.
   i32x8 xq[kTT][kKS];
+  [[maybe_unused]] float row_dq[kTT];  // ROWS: of token l32 of each tile
   auto load_tile = [&](int64_t tok_base) {
 #pragma unroll
     for (int t = 0; t < kTT; ++t) {
       const int64_t tok = row_of(tok_base + t * 32 + l32);
       if (A_FP8) {
+        if constexpr (ROWS) row_dq[t] = p.amax_a[tok];
         const uint8_t* row = static_cast<const uint8_t*>(p.a) + tok * p.lda + hh * 32;
 #pragma unroll
         for (int ks = 0; ks < kKS; ++ks) {
@@ -278,6 +284,13 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void linear_fp8_ts_kernel(const 
     for (int t = 0; t < kTT; ++t)
 #pragma unroll
       for (int ks = 0; ks < kKS; ++ks) asm volatile("" : "+v"(xq[t][ks]));
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int t = 0; t < kTT; ++t) {
+        row_dq[t] = (row_dq[t] < 1e-12f ? 1e-12f : row_dq[t]) / 448.0f * dq;  // a NaN stays one
+        asm volatile("" : "+v"(row_dq[t]));
+      }
+    }
   };
 
   bf16x8 res_cur[NST], res_next[NST];
@@ -379,7 +392,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void linear_fp8_ts_kernel(const 
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[rb][e] = acc[rb][t][jq * 4 + e] * dq + static_cast<float>(bv[rb * 4 + jq][e]);
+          for (int e = 0; e < 4; ++e) v[rb][e] = acc[rb][t][jq * 4 + e] * (ROWS ? row_dq[t] : dq) + static_cast<float>(bv[rb * 4 + jq][e]);
         if constexpr (GLU) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[0][e] = silu_f(v[0][e]) * v[1][e];
@@ -481,7 +494,7 @@ bool rows_in_place(const Fp8TsParams& p, int a_bytes) {
 // K = 1024 (no SiLU-gate, weight rows a multiple of 32), 16-byte aligned rows. Returns TAAC_OK after a launch, a negative
 // status on a launch error and 1 when the shape is not covered (the caller then uses the tiled kernel).
 template <int K>
-int launch_fp8_ts_for_k(Fp8TsParams p, int a_is_fp8, int epilogue, hipStream_t s, const char* name) {
+int launch_fp8_ts_for_k(Fp8TsParams p, int a_is_fp8, bool row_amax, int epilogue, hipStream_t s, const char* name) {
   const size_t lds_bytes = static_cast<size_t>(3 * step_bytes(K)) + static_cast<size_t>(kWaves) * 32 * tile_row_bytes(K) +
                            static_cast<size_t>(p.N) * 2;
   if (lds_bytes > 160 * 1024) return 1;
@@ -494,14 +507,19 @@ int launch_fp8_ts_for_k(Fp8TsParams p, int a_is_fp8, int epilogue, hipStream_t s
   const int64_t most = p.whole_tiles ? tiles64 : tiles64 * (epilogue == TAAC_EPI_SWIGLU ? p.N / 64 : p.N / (row_blocks(K) * 32));
   int grid = static_cast<int>(most < cus ? most : cus);
   if (const int limit = test_max_workgroups(); limit > 0 && limit < grid) grid = limit;  // taac_test_hooks
-#define TAAC_FP8_TS_LAUNCH(EPI, AF8)                                                                                \
-  do {                                                                                                              \
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(linear_fp8_ts_kernel<K, EPI, AF8, false>),                       \
-                            hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds_bytes)) != hipSuccess) \
-      return set_error(TAAC_ERR_LAUNCH, "%s: cannot reserve %zu bytes of LDS", name, lds_bytes);                    \
-    hipLaunchKernelGGL((linear_fp8_ts_kernel<K, EPI, AF8, false>), dim3(grid), dim3(kWaves * kWave), lds_bytes, s, p);     \
-    return check_launch(name);                                                                                      \
+#define TAAC_FP8_TS_LAUNCH(EPI, AF8, ...)                                                                                         \
+  do {                                                                                                                            \
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(linear_fp8_ts_kernel<K, EPI, AF8, false, false, ##__VA_ARGS__>),                \
+                            hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds_bytes)) != hipSuccess)               \
+      return set_error(TAAC_ERR_LAUNCH, "%s: cannot reserve %zu bytes of LDS", name, lds_bytes);                                  \
+    hipLaunchKernelGGL((linear_fp8_ts_kernel<K, EPI, AF8, false, false, ##__VA_ARGS__>), dim3(grid), dim3(kWaves * kWave), lds_bytes, s, p); \
+    return check_launch(name);                                                                                                    \
   } while (0)
+  if constexpr (K == 256) {
+    if (row_amax && epilogue == TAAC_EPI_NONE) TAAC_FP8_TS_LAUNCH(TAAC_EPI_NONE, true, true);
+    if (row_amax && epilogue == TAAC_EPI_RESIDUAL) TAAC_FP8_TS_LAUNCH(TAAC_EPI_RESIDUAL, true, true);
+    if (row_amax) TAAC_FP8_TS_LAUNCH(TAAC_EPI_SWIGLU, true, true);
+  }
   if (epilogue == TAAC_EPI_NONE) {
     if (a_is_fp8) TAAC_FP8_TS_LAUNCH(TAAC_EPI_NONE, true);
     TAAC_FP8_TS_LAUNCH(TAAC_EPI_NONE, false);
@@ -523,8 +541,9 @@ int launch_fp8_ts_for_k(Fp8TsParams p, int a_is_fp8, int epilogue, hipStream_t s
 int launch_linear_fp8_ts(const void* a, int a_is_fp8, int64_t lda, const void* w, const float* amax_a,
                          const float* amax_w, const void* bias, const void* residual, void* out, int64_t ldo,
                          int64_t M, int32_t N, int32_t K, int epilogue, int gate_first, hipStream_t s,
-                         const char* name) {
+                         const char* name, bool row_amax) {
   if ((K != 256 && K != 1024) || M <= 0) return 1;
+  if (row_amax && K != 256) return 1;  // 1024 -> 256 features, 131072 rows: 52 us by the tiled kernel, 50 here with one maximum
   if (N % (row_blocks(K) * 32) != 0) return 1;
   if (K == 1024 && epilogue == TAAC_EPI_SWIGLU) return 1;
   if (lda % (a_is_fp8 ? 16 : 8) != 0 || ldo % 8 != 0 || (reinterpret_cast<uintptr_t>(bias) & 15u)) return 1;
@@ -543,8 +562,8 @@ int launch_linear_fp8_ts(const void* a, int a_is_fp8, int64_t lda, const void* w
   p.ldr = ldo;
   p.N = N;
   p.gate_first = gate_first ? 1 : 0;
-  if (K == 256) return launch_fp8_ts_for_k<256>(p, a_is_fp8, epilogue, s, name);
-  return launch_fp8_ts_for_k<1024>(p, a_is_fp8, epilogue, s, name);
+  if (K == 256) return launch_fp8_ts_for_k<256>(p, a_is_fp8, row_amax, epilogue, s, name);
+  return launch_fp8_ts_for_k<1024>(p, a_is_fp8, row_amax, epilogue, s, name);
 }
 
 }  // namespace taac

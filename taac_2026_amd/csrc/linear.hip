@@ -721,6 +721,9 @@ int linear_fp8_entry(const char* name, const void* a, int a_is_fp8, bool row_ama
   rc = fill_params(name, p, M, N, epilogue);
   if (rc != TAAC_OK) return rc;
   hipStream_t s = as_stream(stream);
+  rc = launch_linear_fp8_ts(a, a_is_fp8, lda, w, amax_a, amax_w, bias, residual, out, ldo, M, N, K, epilogue, gate_first,
+                            s, name, row_amax);
+  if (rc <= 0) return rc;  // launched (or failed) on the token-stationary path
   if (row_amax) {
     switch (epilogue) {
       case TAAC_EPI_NONE: hipLaunchKernelGGL((linear_fp8_kernel<TAAC_EPI_NONE, true, true>), dim3(p.total), dim3(kThreads), 0, s, p); break;
@@ -729,9 +732,6 @@ int linear_fp8_entry(const char* name, const void* a, int a_is_fp8, bool row_ama
     }
     return check_launch(name);
   }
-  rc = launch_linear_fp8_ts(a, a_is_fp8, lda, w, amax_a, amax_w, bias, residual, out, ldo, M, N, K, epilogue, gate_first,
-                            s, name);
-  if (rc <= 0) return rc;  // launched (or failed) on the token-stationary path
 #define TAAC_FP8_LAUNCH(EPI)                                                                                   \
   if (a_is_fp8)                                                                                                \
     hipLaunchKernelGGL((linear_fp8_kernel<EPI, true>), dim3(p.total), dim3(kThreads), 0, s, p);               \

@@ -200,6 +200,40 @@ def test_the_e4m3_layer_reads_rows_with_their_maxima(device, swiglu, with_residu
     assert ((got.cpu().double() - want).abs() <= 2.0**-8 * want.abs() + magnitude.clamp(min=1.0) ** (2 if swiglu else 1) * 2.0**-14).all()
 
 
+@pytest.mark.parametrize("rows,width,out", [(1, 256, 64), (777, 256, 768), (20000, 256, 128), (300, 256, 80), (130, 128, 192), (65, 1024, 256), (33, 48, 16)])
+@pytest.mark.parametrize("epilogue", ["plain", "residual", "swiglu"])
+def test_e4m3_rows_through_both_dense_kernels(device, rows, width, out, epilogue):
+    """Widths and features of the token-stationary kernel and of the tiled one; maxima over nine orders, zero and NaN among them."""
+    g = torch.Generator().manual_seed(rows + width + out)
+    x = torch.randn(rows, width, generator=g).clamp(-8, 8).to(torch.float8_e4m3fn)
+    amax = 10.0 ** (torch.rand(rows, generator=g) * 5.0 - 3.0)
+    nan = rows // 2 if rows > 2 else None
+    if nan is not None:
+        amax[0], amax[nan] = 0.0, float("nan")
+    weight = (torch.randn(out, width, generator=g) / width ** 0.5).to(torch.bfloat16)
+    skip = torch.randn(rows, out, generator=g).to(torch.bfloat16)
+    with torch.no_grad():
+        wq, wa = quantize_fp8(weight.to(device))
+        got = linear_fp8(x.to(device), wq, amax.to(device) if rows > 1 else amax.to(device).expand(1), wa, swiglu=epilogue == "swiglu",
+                         residual=skip.to(device) if epilogue == "residual" else None).cpu().double()
+    a = x.float().double() * (amax.double().clamp(min=1e-12) / 448.0)[:, None]
+    b = wq.cpu().float().double() * (wa.cpu().double() / 448.0)
+    want, size = a @ b.T, a.abs() @ b.abs().T
+    if epilogue == "swiglu":
+        gate, value = want.chunk(2, -1)
+        want = torch.nn.functional.silu(gate) * value
+        size = size.chunk(2, -1)
+        size = (1.0 + size[0]) * (1.0 + size[1])
+    elif epilogue == "residual":
+        want, size = want + skip.double(), size + skip.double().abs()
+    if nan is not None:
+        assert torch.isnan(got[nan]).all()
+        keep = torch.arange(rows) != nan
+        got, want, size = got[keep], want[keep], size[keep]
+    # one rounding; sums of up to 1024 products in fp32, the gate's exponential and reciprocal (2^-20)
+    assert ((got - want).abs() <= 2.0**-8 * want.abs() + 2.0**-13 * size + 1e-12).all()
+
+
 def test_replayed_graph(device):
     x, r, w = (t.to(device) for t in _draw(500, 256, torch.bfloat16, seed=13))
     with torch.no_grad():
