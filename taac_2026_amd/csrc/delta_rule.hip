@@ -7,8 +7,8 @@ namespace {
 // Heads of at most 64 key features walk alone (delta_solo.hip) from more than two or three teams of 16 columns to a CU on: the chain of chunks
 // no longer counts then, and nothing is left in memory between two kernels. Wider heads always take the teams of delta_team.hip: their state
 // does not fit the registers of one wavefront. 2048 tokens, team : solo, by heads times groups of 16 columns:
-//   32 wide, forward 119 : 163 us at 512, 192 : 171 at 768;  with the backward 402 : 473, 617 : 561
-//   64 wide, forward 152 : 194 us at 768, 218 : 198 at 1024; with the backward 532 : 572, 729 : 619
+//   32 wide, forward 111 : 134 us at 512, 153 : 139 at 640;  with the backward 364 : 400, 467 : 442
+//   64 wide, forward 144 : 170 us at 768, 204 : 171 at 1024; with the backward 500 : 514, 671 : 557
 bool uses_teams(int64_t heads, int32_t dk, int32_t dv) { return dk > 64 || heads * ((dv + 15) / 16) <= (dk <= 32 ? 512 : 768); }
 
 int64_t workspace_of(int64_t heads, int32_t T, int32_t dk, int32_t dv) {
