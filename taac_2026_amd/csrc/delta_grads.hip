@@ -1,5 +1,5 @@
-// Gated delta rule, chunked form, backward: the gradients of a chunk's tokens (notation, operand order and precision: delta.h; dS' and dX:
-// delta.h), in parallel over the chunks. With
+// Gated delta rule, chunked form, backward: the gradients of a chunk's tokens (notation, operand order and precision, dS' and dX: delta.h),
+// in parallel over the chunks. With
 //   B_ij = scale Gam_ij dO_i . N_j (i >= j),   E_ij = -Gam_ij dX_i . N_j (i > j)
 //   dQ = scale e^G dO S^T + B diag(beta) K
 //   R  = E diag(beta) K - e^G dX S^T
@@ -8,12 +8,15 @@
 //   dG_i = q_i . dQ_i + k_i . R_i - beta_i dbeta_i, and e^{G_64} <S, dS'> + sum_j beta_j e^{G_64 - G_j} k_j . (N dS'^T)_j for G_64
 //   dg_t = the sum of dG over t .. 64
 // where what a pair (i, j) of tokens adds to a row it takes from a column.
+//
 // All in one workgroup per chunk and key head: the tiles of K, Q, dO, dX, N, S and dS' meet in LDS, where each is read by rows and by columns.
 // 512 samples x 4 heads x 512 tokens, 64 wide: 355 us, 3.4 TB/s; two workgroups to a CU by their registers, whose wavefronts wait for 46 % of
-// their time and issue vector instructions for 25 %. 128 wide, where the tiles leave room for one: 18 us per chunk and head, 2.4 TB/s; two sets of four wavefronts on one chunk (rows
-// and columns at once) took 3 % longer.
-// N, S, dS' and dX are read back in bf16, one rounding each: they only meet the outputs. Key heads that serve several value heads sum
-// their gradients in registers, in the order of the heads.
+// their time and issue vector instructions for 25 %. 128 wide, where the tiles leave room for one: 18 us per chunk and head, 2.4 TB/s; two
+// sets of four wavefronts on one chunk (rows and columns at once) took 3 % longer.
+//
+// N, S, dS' and dX are read back in bf16, one rounding each: they only meet the outputs. Of the 2.5e-3 that a gradient is off, 1.7e-3 is its own
+// rounding, 1.7e-3 that of N, 0.5e-3 that of each of the others; N in two parts would cost a tenth of all bytes. Key heads that serve
+// several value heads sum their gradients in registers, in the order of the heads.
 #include "delta.h"
 
 namespace taac {
