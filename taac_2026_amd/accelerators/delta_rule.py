@@ -39,14 +39,15 @@ def _check_shapes(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
         raise ValueError(f"{name} requires a number of value heads that is a multiple of the key heads")
     if log_decay.shape != v_shape[:3] or beta.shape != v_shape[:3]:
         raise ValueError(f"{name} expects log_decay and beta with shape (batch, value heads, tokens)")
-    require_same_dtype(f"{name} q, k, v", q, k, v)
-    require_same_dtype(f"{name} gates", log_decay, beta)
+    if not q.dtype == k.dtype == v.dtype:
+        require_same_dtype(f"{name} q, k, v", q, k, v)
+    if log_decay.dtype != beta.dtype:
+        require_same_dtype(f"{name} gates", log_decay, beta)
 
 
 def _check_widths(name: str, key_width: int, value_width: int) -> None:
-    for width in (key_width, value_width):
-        if width <= 0 or width % 8 != 0 or width > MAX_WIDTH:
-            raise RuntimeError(f"{name} is built for key and value widths that are multiples of 8, at most {MAX_WIDTH}")
+    if key_width <= 0 or value_width <= 0 or key_width % 8 != 0 or value_width % 8 != 0 or max(key_width, value_width) > MAX_WIDTH:
+        raise RuntimeError(f"{name} is built for key and value widths that are multiples of 8, at most {MAX_WIDTH}")
 
 
 def _lengths(name: str, key_lengths: torch.Tensor | None, batch: int, device: torch.device) -> torch.Tensor | None:
@@ -190,7 +191,7 @@ def gated_delta_rule(
         require_inference(f"hip {name} initial_state", initial_state)
         initial_state = initial_state.contiguous()
     scale = k.shape[3] ** -0.5 if scale is None else float(scale)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, beta)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad or beta.requires_grad):
         if return_state:
             raise RuntimeError(f"hip {name}: the returned state has no gradient: call it under torch.no_grad() or without return_state")
         return _GatedDeltaRuleFunction.apply(q, k, v, log_decay, beta, scale, lengths, initial_state)

@@ -246,7 +246,8 @@ def _residual_inputs(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
     if x.shape[-1] != weight.shape[0]:
         raise ValueError(f"last dimension {x.shape[-1]} does not match weight size {weight.shape[0]}")
     require_cuda_tensors(f"hip {operator}", x, residual, weight)
-    require_same_dtype(operator, x, residual)
+    if x.dtype != residual.dtype:
+        require_same_dtype(operator, x, residual)
     return x.contiguous(), residual.contiguous(), (weight if weight.dtype == x.dtype else weight.to(x.dtype)).contiguous()
 
 
