@@ -150,6 +150,20 @@ def test_state_behind_the_first_token_of_a_chunk(device, sizes):
     assert ((state.double() - want).flatten(2).norm(dim=-1) <= 6 * 2.0**-16 * want.flatten(2).norm(dim=-1)).all()
 
 
+@pytest.mark.parametrize("tokens,sizes", [(4133, (1, 1, 1, 32, 32)), (2900, (1, 1, 2, 128, 64)), (1100, (600, 1, 1, 16, 24))])
+def test_long_histories(device, tokens, sizes):
+    """Dozens of chunks, an odd one at the end; slow decays, so that the first tokens still count."""
+    inputs = [t.to(device) for t in _draw(sizes[0], tokens, *sizes[1:], seed=10)]
+    inputs[3] *= 0.01
+    _check_forward(device, inputs)
+
+
+def test_backward_of_a_long_history(device):
+    inputs = list(_draw(1, 1500, 1, 2, 32, 32, seed=11))
+    inputs[3] *= 0.02
+    _check_backward(device, inputs)
+
+
 def test_rows_that_overlap_are_copied(device):
     """One key for all tokens as an expanded view, rows behind each other by less than their width."""
     q, k, v, log_decay, beta = (t.to(device) for t in _draw(2, 70, 1, 1, 32, 32, seed=7))
