@@ -611,7 +611,8 @@ int taac_row_rstd(const float* qk_sumsq, int64_t M, int32_t d_model, float eps, 
  * token), not negative; the features of a row are contiguous, q / k / v / o have strides that are multiples of 8, token strides from a row's
  * width to below 2^24, and 16-byte aligned bases. dk and dv: multiples of 8, at most 128; T at most 2^30. lengths: int32 [B] or NULL; tokens at or beyond a sample's length are not read, leave the
  * state alone and get zeros in o. Keys should have at most unit length and beta lie in [0, 1], as the recurrence needs to stay
- * bounded; log_decay is normally <= 0, values below -1e5 count as -1e5. Infinities and NaN of a valid token reach the whole chunk of 64
+ * bounded; log_decay is normally <= 0 and may have either sign as long as its sums within 64 tokens stay below 88 (exp in fp32); values below
+ * -1e5 count as -1e5. Infinities and NaN of a valid token reach the whole chunk of 64
  * tokens that it lies in, the tokens in front of it too, and everything behind it in its (sample, head).
  * state_in: fp32 [B, H, dk, dv] or NULL (zeros); state_out: the same shape, or NULL; it may be state_in.
  * chunk_states (bf16 [B, H, ceil(T / 64), dv, dk]) and misses (bf16 [B, H, T, dv]): what taac_delta_rule_bwd reads, or both NULL.

@@ -37,14 +37,20 @@ def delta_rule(q, k, v, log_decay, beta, *, scale=None, lengths=None, initial_st
     return torch.stack(outs, 2), state, torch.stack(misses, 2)
 
 
+def _pair_decays(log_decay):
+    """``exp(G_i - G_j)`` of the pairs j <= i, zero above."""
+    total = log_decay.detach().double().clamp(min=-1e5).cumsum(-1)
+    above = torch.ones(total.shape[-1], total.shape[-1], dtype=torch.bool, device=total.device).triu(1)
+    return (total[..., :, None] - total[..., None, :]).masked_fill(above, -torch.inf).exp()
+
+
 def score_magnitudes(q, k, log_decay, beta, misses, *, scale=None):
     """``|P| |N|`` with ``P_ij = scale exp(G_i - G_j) (q_i . k_j) beta_j`` over all pairs j <= i: what one rounding of every P adds up to."""
     group = misses.shape[1] // q.shape[1]
     scale = k.shape[-1] ** -0.5 if scale is None else scale
     q, k = (t.double().repeat_interleave(group, 1) for t in (q, k))
-    total = log_decay.double().clamp(min=-1e5).cumsum(-1)
-    pairs = (q @ k.transpose(-1, -2)).abs() * (total[..., :, None] - total[..., None, :]).clamp(max=0.0).exp() * beta.double().abs()[..., None, :]
-    return scale * pairs.tril() @ misses.abs()
+    pairs = (q @ k.transpose(-1, -2)).abs() * _pair_decays(log_decay) * beta.double().abs()[..., None, :]
+    return scale * pairs @ misses.abs()
 
 
 def gradient_magnitudes(q, k, log_decay, beta, misses, grad_out, grad_v, *, scale=None, initial_state=None):
@@ -60,7 +66,7 @@ def gradient_magnitudes(q, k, log_decay, beta, misses, grad_out, grad_v, *, scal
     n, do, dv, beta = (t.detach().double().abs() for t in (misses, grad_out, grad_v, beta))
     total = log_decay.detach().double().clamp(min=-1e5).cumsum(-1)
     tokens = n.shape[2]
-    decay = (total[..., :, None] - total[..., None, :]).clamp(max=0.0).exp().tril()
+    decay = _pair_decays(log_decay)
     weight = decay * beta[..., None, :]
     dx = dv + (scale * weight * (q @ k.transpose(-1, -2))).transpose(-1, -2) @ do
     from_out, from_x = scale * (do @ n.transpose(-1, -2)), (dx @ n.transpose(-1, -2)).tril(-1)

@@ -169,7 +169,8 @@ def gated_delta_rule(
     bfloat16 tokens, gates in bfloat16 or float32; widths that are multiples of 8, at most 128; value heads a multiple of the
     key heads (consecutive value heads share a key head). ``scale`` defaults to ``key width ** -0.5``. ``key_lengths`` (batch,):
     tokens at or beyond a sample's length are not read, get zeros and leave the state alone. Keys should have unit length at
-    most (an :func:`rms_norm` over the head with weight ``key width ** -0.5``) and ``beta`` lie in [0, 1]. Infinities and NaN in a
+    most (an :func:`rms_norm` over the head with weight ``key width ** -0.5``) and ``beta`` lie in [0, 1]; ``log_decay`` is normally
+    below zero, and may have either sign as long as the sums of it within 64 tokens stay below 88 (``exp`` in float32). Infinities and NaN in a
     valid token reach every token of its chunk of 64, those in front of it too, and all behind it in the same sample and head.
 
     ``initial_state`` (batch, heads, key width, value width) float32 is the state in front of the first token, ``return_state``

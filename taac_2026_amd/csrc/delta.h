@@ -313,7 +313,7 @@ __device__ __forceinline__ void chunk_rows(const DeltaParams& p, const GateBits&
 }
 
 // e^(G in front of tile ti - G behind tile tj), ti > tj: the decay of the whole tiles between them. Gam of a token i of tile ti and a token
-// j of tile tj is this times In_i times Out_j: three factors of at most one, one exponential per token instead of one per pair.
+// j of tile tj is this times In_i times Out_j, one exponential per token instead of one per pair; three factors of at most one where states decay.
 __device__ __forceinline__ float tiles_between(const float* rows, int ti, int tj) {
   const float second = rows[kRowTotal + 1], third = rows[kRowTotal + 2];
   return ti - tj < 2 ? 1.f : (ti - tj == 3 ? second * third : (tj == 0 ? second : third));

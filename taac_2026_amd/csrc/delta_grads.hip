@@ -131,14 +131,15 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
     __syncthreads();
 
     const float hi_t = temp[kTempHi + row], lo_t = temp[kTempLow + row], beta_t = temp[kTempBeta + row], grown = rows[kRowGrown + row];
-    // Gam of this lane's token and the four of tile t that its registers hold
-    auto decays = [&](int t) __attribute__((always_inline)) -> f32x4 {
+    // Gam of this lane's token and the four of tile t that its registers hold; in the own tile this token is the later of a pair (sign 1) or the
+    // earlier (sign -1), and pairs in the other order get whatever, to be masked (decays may grow: no sign of a difference says which it is)
+    auto decays = [&](int t, float sign) __attribute__((always_inline)) -> f32x4 {
       f32x4 gam;
       if (t == wave) {
         const f32x4 hi_r = *reinterpret_cast<const f32x4*>(temp + kTempHi + 16 * t + 4 * grp);
         const f32x4 lo_r = *reinterpret_cast<const f32x4*>(temp + kTempLow + 16 * t + 4 * grp);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) gam[r] = __builtin_amdgcn_exp2f(-__builtin_fabsf((hi_t - hi_r[r]) + (lo_t - lo_r[r])));
+        for (int r = 0; r < 4; ++r) gam[r] = __builtin_amdgcn_exp2f(sign * ((hi_t - hi_r[r]) + (lo_t - lo_r[r])));
       } else {
         const f32x4 other = *reinterpret_cast<const f32x4*>(temp + (t < wave ? kTempOut : kTempIn) + 16 * t + 4 * grp);
         const float own = t < wave ? temp[kTempIn + row] * tiles_between(rows, wave, t) : temp[kTempOut + row] * tiles_between(rows, t, wave);
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
           qk = mfma16(kf, third[kb], qk);
           kk = mfma16(kf, fourth[kb], kk);
         }
-        const f32x4 gam = decays(t), beta_r = *reinterpret_cast<const f32x4*>(temp + kTempBeta + 16 * t + 4 * grp);
+        const f32x4 gam = decays(t, 1.f), beta_r = *reinterpret_cast<const f32x4*>(temp + kTempBeta + 16 * t + 4 * grp);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = 16 * t + 4 * grp + r;
@@ -251,7 +252,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
           qk = mfma16(TK::row(tile_q, 16 * t + l16, kb, grp), fourth[kb], qk);
           kk = mfma16(TK::row(tile_k, 16 * t + l16, kb, grp), fourth[kb], kk);
         }
-        const f32x4 gam = decays(t);
+        const f32x4 gam = decays(t, -1.f);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int i = 16 * t + 4 * grp + r;

@@ -275,6 +275,34 @@ def test_backward_at_the_edges_of_the_gates(device, case):
     _check_backward(device, (q, k, v, log_decay, beta))
 
 
+# batch, key heads, heads, key width, value width: few heads (teams), many (wavefronts on their own), wide ones in teams of 16 and of 32 columns
+GROWING = [(3, 1, 2, 32, 32), (2, 1, 1, 64, 64), (1100, 1, 1, 32, 32), (520, 1, 1, 64, 64), (2, 1, 2, 128, 128), (70, 1, 1, 128, 128)]
+
+
+@pytest.mark.parametrize("sizes", GROWING)
+@pytest.mark.parametrize("least", [0.0, -0.1])
+def test_growing_states(device, sizes, least):
+    """Logarithms of decays up to 0.1: all above zero, and of both signs (the state grows by up to e^3.5 or stays). The bounds hold for any sign, since the
+    magnitudes that they are made of have the decays in them."""
+    q, k, v, log_decay, beta = _draw(sizes[0], 70, *sizes[1:], seed=22)
+    log_decay = least + (0.1 - least) * torch.rand(log_decay.shape, generator=torch.Generator().manual_seed(23))
+    lengths = [(70, 64, 33, 16)[i % 4] for i in range(sizes[0])]
+    _check_forward(device, (q, k, v, log_decay, beta), lengths=lengths)
+    _check_backward(device, (q, k, v, log_decay, beta), lengths=lengths)
+
+
+@pytest.mark.parametrize("sizes", [(1, 32, 32), (2, 64, 64), (1, 128, 128)])
+def test_steps_of_growing_states(device, sizes):
+    """The same tokens in one call of steps and in chunks."""
+    inputs = [t.to(device) for t in _draw(2, 20, 1, *sizes, seed=24)]
+    inputs[3] = 0.1 * torch.rand(inputs[3].shape, generator=torch.Generator().manual_seed(25)).to(device)
+    want, want_state, _ = delta_rule(*inputs)
+    pool = torch.zeros(2, *sizes, device=device)
+    with torch.no_grad():
+        out = gated_delta_rule_step(*inputs, pool)
+    _check_step(out, pool, want.cpu(), want_state.cpu(), torch.bfloat16)
+
+
 def test_gradient_against_differences(device):
     """Along one direction, on the values, which enter the outputs linearly: the difference quotient has no truncation error."""
     q, k, v, log_decay, beta = (t.to(device) for t in _draw(1, 80, 1, 1, 32, 32, seed=14))
