@@ -1159,12 +1159,20 @@ def linear_fp8(
 
     ``x`` is bf16 (quantised on load with scale ``amax_x / 448``) or already ``float8_e4m3fn``;
     ``weight_fp8`` is ``float8_e4m3fn`` ``[out, in]`` quantised with scale ``amax_w / 448``.
-    ``amax_x`` with the shape of x without its last dimension holds one maximum per row of an x that is ``float8_e4m3fn``
-    already (:func:`residual_rms_norm_fp8`); a scalar holds the tensor's.
+    ``amax_x`` (float32) with the shape of x without its last dimension holds one maximum per row of an x that is
+    ``float8_e4m3fn`` already (:func:`residual_rms_norm_fp8`); a scalar holds the tensor's. Any other shape is refused.
     ``swiglu`` selects the ``silu(gate) * value`` epilogue (output has ``out / 2`` features), ``residual`` the
     fused residual add; they are exclusive.
     """
     name = "hip linear_fp8"
+    row_amax = amax_x.numel() != 1
+    if amax_x.dtype != torch.float32:
+        raise ValueError(f"linear_fp8 amax_x must be float32, got {amax_x.dtype}")
+    if row_amax and amax_x.shape != x.shape[:-1]:
+        raise ValueError(f"linear_fp8 amax_x must hold one maximum, or one per row of x in the shape {tuple(x.shape[:-1])}, "
+                         f"got {tuple(amax_x.shape)}")
+    if row_amax and x.dtype != torch.float8_e4m3fn:
+        raise ValueError("linear_fp8 takes one amax_x per row with float8_e4m3fn activations only")
     require_cuda_tensors(name, x, weight_fp8, amax_x, amax_w, bias, residual)
     require_inference(name, x, bias, residual)
     _check_bf16(name, bias, residual)
@@ -1188,9 +1196,7 @@ def linear_fp8(
     res_rows = residual.reshape(-1, out_features).contiguous() if residual is not None else None
     epilogue = _native.EPI_SWIGLU if swiglu else (_native.EPI_RESIDUAL if res_rows is not None else _native.EPI_NONE)
     library = _native.load_library()
-    if amax_x.numel() != 1 and amax_x.shape == shape[:-1]:
-        if x.dtype != torch.float8_e4m3fn or amax_x.dtype != torch.float32:
-            raise ValueError("linear_fp8 takes one float32 amax_x per row with float8_e4m3fn activations only")
+    if row_amax:
         amax_rows = amax_x.contiguous()
         with _native.on_device(x.device):
             status = library.taac_linear_fp8_rows(

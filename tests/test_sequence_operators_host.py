@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from taac_2026_amd import _native
-from taac_2026_amd.api import gated_delta_rule, gated_delta_rule_step, residual_rms_norm, residual_rms_norm_fp8
+from taac_2026_amd.api import gated_delta_rule, gated_delta_rule_step, linear_fp8, residual_rms_norm, residual_rms_norm_fp8
 
 
 @pytest.mark.parametrize("operator", [residual_rms_norm, residual_rms_norm_fp8])
@@ -131,3 +131,20 @@ def test_delta_entry_points_check_on_the_host():
     assert step(qs=strides(16, -16, 16)) == invalid and step(qs=None) == invalid
     assert step(B=(1 << 28) + 1, H=1, pool=1 << 40) == unsupported and b"2^28" in library.taac_last_error()
     assert step(B=0) == ok and step(T=0) == ok
+
+
+def test_linear_fp8_refuses_maxima_of_another_shape():
+    """Read as one maximum, the first row's would dequantise them all."""
+    x = torch.zeros(2, 3, 16).to(torch.float8_e4m3fn)
+    weight, amax_w = torch.zeros(16, 16).to(torch.float8_e4m3fn), torch.ones(())
+    for values, amax in ((x, (6,)), (x, (2, 3, 1)), (x, (3, 2)), (x, (3,)), (x.view(6, 16), (2, 3)), (x.view(6, 16), (6, 1)), (x.view(6, 16), (5,)), (x, (0,))):
+        with pytest.raises(ValueError, match="one per row"):
+            linear_fp8(values, weight, torch.ones(amax), amax_w)
+    with pytest.raises(ValueError, match="float8_e4m3fn activations"):
+        linear_fp8(x.bfloat16(), weight, torch.ones(2, 3), amax_w)
+    for amax in ((2, 3), ()):
+        with pytest.raises(ValueError, match="float32"):
+            linear_fp8(x, weight, torch.ones(amax, dtype=torch.bfloat16), amax_w)
+    for amax in ((2, 3), (), (1,), (1, 1)):  # as they should be: only the device is wrong
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            linear_fp8(x, weight, torch.ones(amax), amax_w)
