@@ -41,8 +41,8 @@ class GatedDeltaAttention(nn.Module):
         self.out = nn.Linear(values, d_model)
 
     def empty_state(self, slots: int, device: torch.device | str) -> torch.Tensor:
-        """A pool of ``slots`` states in front of a first token."""
-        return torch.zeros(slots, self.num_heads, self.key_width, self.value_width, device=device)
+        """A pool of ``slots`` states in front of a first token, float32 as the steps take them."""
+        return torch.zeros(slots, self.num_heads, self.key_width, self.value_width, dtype=torch.float32, device=device)
 
     def _project(self, tokens: torch.Tensor) -> tuple[torch.Tensor, ...]:
         batch, count, _ = tokens.shape

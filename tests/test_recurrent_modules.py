@@ -26,6 +26,17 @@ def test_modules_refuse():
     assert block.attention.empty_state(5, "cpu").shape == (5, 2, 32, 32)
 
 
+def test_empty_state_is_float32_whatever_the_default():
+    """The type that steps take: a serving program may have set another default."""
+    mixer = GatedDeltaAttention(64, 2)
+    kept = torch.get_default_dtype()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        assert mixer.empty_state(3, "cpu").dtype == torch.float32
+    finally:
+        torch.set_default_dtype(kept)
+
+
 def _make(device, sizes, seed=0):
     torch.manual_seed(seed)
     block = GatedDeltaBlock(hidden_mult=2, **sizes).to(device)
