@@ -1239,6 +1239,8 @@ def norm_linear_fp8(
     of the layer that consumes the output: the max of ``|rmsnorm(out, out_norm_weight)|`` (of ``|out|`` without a
     weight), so that no pass of its own is needed for it."""
     name = "hip norm_linear_fp8"
+    if amax_x.dtype != torch.float32 or amax_x.numel() != 1:
+        raise ValueError("norm_linear_fp8 amax_x must be a float32 scalar tensor")
     require_cuda_tensors(name, x, weight_fp8, amax_x, amax_w, bias, norm_weight, residual, out_norm_weight)
     require_inference(name, x, bias, norm_weight, residual)
     _check_bf16(name, x, bias, norm_weight, residual, out_norm_weight)

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from taac_2026_amd import _native
-from taac_2026_amd.api import gated_delta_rule, gated_delta_rule_step, linear_fp8, residual_rms_norm, residual_rms_norm_fp8
+from taac_2026_amd.api import gated_delta_rule, gated_delta_rule_step, linear_fp8, norm_linear_fp8, residual_rms_norm, residual_rms_norm_fp8
 
 
 @pytest.mark.parametrize("operator", [residual_rms_norm, residual_rms_norm_fp8])
@@ -148,3 +148,13 @@ def test_linear_fp8_refuses_maxima_of_another_shape():
     for amax in ((2, 3), (), (1,), (1, 1)):  # as they should be: only the device is wrong
         with pytest.raises(RuntimeError, match="CUDA tensors"):
             linear_fp8(x, weight, torch.ones(amax), amax_w)
+
+
+def test_norm_linear_fp8_takes_one_maximum():
+    """It quantises its rows itself: maxima of rows would be read as the first one."""
+    x, weight = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(64, 256).to(torch.float8_e4m3fn)
+    for amax in (torch.ones(4), torch.ones(4, 1), torch.ones(0), torch.ones((), dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="float32 scalar"):
+            norm_linear_fp8(x, weight, amax, torch.ones(()))
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        norm_linear_fp8(x, weight, torch.ones(1), torch.ones(()))
