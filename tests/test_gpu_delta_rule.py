@@ -604,3 +604,32 @@ def test_prefill_then_steps(device, sizes):
     bound = 1.0625 * HALF * (want.abs() + score_magnitudes(*inputs[:2], *inputs[3:], misses)) + HALF / 16 * want.abs().amax()
     assert ((got - want).abs() <= bound).all()
     assert ((state.cpu().double() - want_state).norm() <= 2.0**-12 * want_state.norm())
+
+
+@pytest.mark.parametrize("tokens,sizes", [(4133, (1, 1, 1, 32, 32)), (2900, (1, 1, 2, 128, 64)), (1500, (3, 2, 4, 64, 64)), (1100, (600, 1, 1, 16, 24)), (700, (520, 1, 1, 64, 64))])
+def test_precision_of_the_state_behind_a_long_history(device, tokens, sizes):
+    """The state enters a chunk's products as pairs of bf16, whose error is at most 2^-16 of a value and, of random sign, 2^-16 / 3 of a vector's norm.
+    Three such roundings (state, misses, what is added) per chunk make 2^-16 / 3^0.5. What a chunk leaves behind is overwritten by the next: a token takes
+    2 b - b^2 (2 / 3 at the mean over b in [0, 1]) of the square along one of key-width directions, a chunk thus leaves exp(-64 / (3 key width)) of the
+    norm, and the errors of all chunks sum to a geometric series. Twice that."""
+    inputs = [t.to(device) for t in _draw(sizes[0], tokens, *sizes[1:], seed=26)]
+    inputs[3] *= 0.01
+    _, want, _ = delta_rule(*inputs)
+    with torch.no_grad():
+        _, state = gated_delta_rule(*inputs, return_state=True)
+    left = torch.tensor(-64.0 / (3.0 * sizes[3])).exp().item()
+    bound = 2.0 * 2.0**-16 / 3.0**0.5 / (1.0 - left)
+    error = (state.double() - want).flatten(2).norm(dim=-1) / want.flatten(2).norm(dim=-1)
+    assert (error <= bound).all(), (error.max(), bound)
+
+
+def test_step_of_a_thousand_samples_of_one_slot(device):
+    """One after the other in the order of the batch, by the workgroup of the first."""
+    inputs = _draw(1, 1000, 2, 2, 32, 32, seed=57)
+    want, final, _ = delta_rule(*inputs)
+    rows = [t.to(device).transpose(0, 2).contiguous() for t in inputs]
+    pool = torch.zeros(3, 2, 32, 32, device=device)
+    with torch.no_grad():
+        out = gated_delta_rule_step(*rows, pool, state_index=torch.full((1000,), 2, dtype=torch.int64, device=device))
+    _check_step(out.transpose(0, 2), pool[2:], want, final, torch.bfloat16)
+    assert (pool[:2] == 0).all()

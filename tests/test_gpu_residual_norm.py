@@ -249,3 +249,24 @@ def test_replayed_graph(device):
             want = residual_rms_norm_fp8(nx.to(device), nr.to(device), w)
             torch.cuda.synchronize()
             assert torch.equal(held[0].float(), want[0].float()) and torch.equal(held[1], want[1]) and torch.equal(held[2], want[2])
+
+
+@pytest.mark.parametrize("rows,width,out", [(777, 256, 768), (300, 256, 80), (65, 1024, 256)])
+@pytest.mark.parametrize("epilogue", ["plain", "residual"])
+def test_e4m3_rows_whose_maxima_span_nine_orders(device, rows, width, out, epilogue):
+    """1e-6 to 1e3, in both dense kernels: every row keeps its own scale, however small beside the others."""
+    g = torch.Generator().manual_seed(rows + width)
+    x = torch.randn(rows, width, generator=g).clamp(-8, 8).to(torch.float8_e4m3fn)
+    amax = 10.0 ** (torch.rand(rows, generator=g) * 9.0 - 6.0)
+    weight = (torch.randn(out, width, generator=g) / width ** 0.5).to(torch.bfloat16)
+    skip = torch.randn(rows, out, generator=g).to(torch.bfloat16)
+    with torch.no_grad():
+        wq, wa = quantize_fp8(weight.to(device))
+        got = linear_fp8(x.to(device), wq, amax.to(device), wa, residual=skip.to(device) if epilogue == "residual" else None).cpu().double()
+    a = x.float().double() * (amax.double() / 448.0)[:, None]
+    b = wq.cpu().float().double() * (wa.cpu().double() / 448.0)
+    want, size = a @ b.T, a.abs() @ b.abs().T
+    if epilogue == "residual":
+        want, size = want + skip.double(), size + skip.double().abs()
+    # one rounding; sums of up to 1024 products in fp32 (1024 2^-24) and four roundings of the scale and the sum behind them: 2^-13 of the magnitudes
+    assert ((got - want).abs() <= 2.0**-8 * want.abs() + 2.0**-13 * size).all()
