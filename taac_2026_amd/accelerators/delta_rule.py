@@ -175,7 +175,7 @@ def gated_delta_rule(
 
     ``initial_state`` (batch, heads, key width, value width) float32 is the state in front of the first token, ``return_state``
     returns ``(out, state behind the last)``, which :func:`gated_delta_rule_step` continues. The state is kept in float32
-    precision throughout. Differentiable in q, k, v and the gates; the states are not, so that an ``initial_state`` that
+    and everything that reaches it enters its products with 24 bits; the outputs' scores are rounded to bfloat16 once. Differentiable in q, k, v and the gates; the states are not, so that an ``initial_state`` that
     requires grad, and ``return_state`` where an input does, are refused."""
     name = "gated_delta_rule"
     _check_shapes(name, q, k, v, log_decay, beta)

@@ -20,9 +20,12 @@
 // holds 8 neighbours of a row of memory, feature 8 grp + e of a block of 32, so row 4 g + r of result a of the state is feature
 // 32 (a / 2) + 8 g + 4 (a % 2) + r (state_row).
 //
-// Precision: q, k, v are bf16 and exact operands. The state and what it is made of (S, X, N, M) are fp32 in registers and enter a
-// product as a bf16 pair hi + lo (16 bits, 2^-17 relative), at two matrix instructions where one factor is exact and three where
-// none is; one bf16 would put 2^-9 into the state at every chunk. P enters rounded once: it only reaches the output.
+// Precision: q, k, v are bf16 and exact operands. What reaches the state (S itself, X, M, and what is added to S) is fp32 and enters a product
+// with all 24 bits, as hi + mid + lo of bf16: three matrix instructions where one factor is exact, six where none is (the products whose parts
+// together stand 24 bits below the first are left out); or M and X in fp32 products. The state behind a history is then as near 64 bits as in a
+// plain fp32 evaluation, 0.8e-7 to 2.5e-7 of its norm against 0.8e-7 to 3e-7 (all four in hi + lo: 2.8e-6, S alone where decays are slow: 1.3e-6).
+// What only meets outputs enters as hi + lo (16 bits): S and N for O, and the backward's recurrence, whose results are bf16.
+// P enters rounded once: it only reaches the output.
 // Cumulative decays are summed in 64 bits and kept as pairs, so that G_i - G_j of a fast decaying head keeps fp32 precision.
 #pragma once
 
@@ -70,7 +73,7 @@ namespace {
 
 constexpr int kChunk = 64;
 constexpr int kFrag = 1024;              // bytes of one operand fragment of a wavefront
-constexpr int kBlockM = 0, kBlockLow = 6 * kFrag, kBlockP = 12 * kFrag, kBlockRows = 18 * kFrag;
+constexpr int kBlockM = 0, kBlockMid = 6 * kFrag, kBlockLow = 12 * kFrag, kBlockP = 18 * kFrag, kBlockRows = 24 * kFrag;
 // floats behind the fragments of a block: e^G, beta e^(G_64 - G), e^G_64 (then e^ of the second and third tile's own decays)
 constexpr int kRowGrown = 0, kRowKeep = 64, kRowTotal = 128, kRowFloats = 144;
 constexpr int kBlockBytes = kBlockRows + kRowFloats * 4;
@@ -102,6 +105,19 @@ __device__ __forceinline__ u32x2 rest4(const f32x4& v, const u32x2& r) { return 
 __device__ __forceinline__ void split(const f32x4& a, const f32x4& b, bf16x8& hi, bf16x8& lo) {
   const u32x2 ha = round4(a), hb = round4(b), la = rest4(a, ha), lb = rest4(b, hb);
   hi = __builtin_bit_cast(bf16x8, (u32x4{ha[0], ha[1], hb[0], hb[1]}));
+  lo = __builtin_bit_cast(bf16x8, (u32x4{la[0], la[1], lb[0], lb[1]}));
+}
+// In three parts, which are all of a float's 24 bits.
+__device__ __forceinline__ f32x4 left4(const f32x4& v, const u32x2& r) {
+  return f32x4{v[0] - __builtin_bit_cast(float, r[0] << 16), v[1] - __builtin_bit_cast(float, r[0] & 0xffff0000u),
+               v[2] - __builtin_bit_cast(float, r[1] << 16), v[3] - __builtin_bit_cast(float, r[1] & 0xffff0000u)};
+}
+__device__ __forceinline__ void split3(const f32x4& a, const f32x4& b, bf16x8& hi, bf16x8& mid, bf16x8& lo) {
+  const u32x2 ha = round4(a), hb = round4(b);
+  const f32x4 da = left4(a, ha), db = left4(b, hb);
+  const u32x2 ma = round4(da), mb = round4(db), la = rest4(da, ma), lb = rest4(db, mb);
+  hi = __builtin_bit_cast(bf16x8, (u32x4{ha[0], ha[1], hb[0], hb[1]}));
+  mid = __builtin_bit_cast(bf16x8, (u32x4{ma[0], ma[1], mb[0], mb[1]}));
   lo = __builtin_bit_cast(bf16x8, (u32x4{la[0], la[1], lb[0], lb[1]}));
 }
 __device__ __forceinline__ bf16x8 round8(const f32x4& a, const f32x4& b) {

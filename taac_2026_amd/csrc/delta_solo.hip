@@ -199,9 +199,9 @@ struct Solo {
     return gam;
   }
 
-  // -M of both chunks as operand fragments, hi and lo: by rows (forward), fragment t = row tile t; by columns (backward), column tile t. own: the
-  // diagonal tiles' decays, which the forward's scores take too.
-  __device__ __forceinline__ void solve(const SoloTokens<DK>& c, const float* rows, float* scratch, bf16x8 (&mh)[4], bf16x8 (&ml)[4],
+  // The blocks of -M of both chunks, fp32: the diagonal ones of each tile of 16, and the one below them of each chunk. By rows (forward); by columns
+  // (backward), which are the rows of its transpose. own: the diagonal tiles' decays, which the forward's scores take too.
+  __device__ __forceinline__ void solve(const SoloTokens<DK>& c, const float* rows, float* scratch, f32x4 (&diag)[4], f32x4 (&below)[2],
                                         f32x4 (&own)[4]) const {
     f32x4 low[2];  // the blocks below the diagonal, by rows
 #pragma unroll
@@ -243,20 +243,22 @@ struct Solo {
         t1[r] = m_rows[2 * s + 1][r] - one;  // negative: gives -M below
       }
       const f32x4 z = mul_cols(low[s], t0, zero4());
-      const f32x4 below = BACK ? mul_cols(t1, z, zero4()) : mul_rows(t1, z, zero4());
-      f32x4 d0, d1;
+      below[s] = BACK ? mul_cols(t1, z, zero4()) : mul_rows(t1, z, zero4());
+    }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        d0[r] = BACK ? -m_cols[2 * s][r] : -m_rows[2 * s][r];
-        d1[r] = BACK ? -m_cols[2 * s + 1][r] : -m_rows[2 * s + 1][r];
-      }
-      if (BACK) {
-        split(d0, below, mh[2 * s], ml[2 * s]);
-        split(zero4(), d1, mh[2 * s + 1], ml[2 * s + 1]);
-      } else {
-        split(d0, zero4(), mh[2 * s], ml[2 * s]);
-        split(below, d1, mh[2 * s + 1], ml[2 * s + 1]);
-      }
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) diag[t][r] = BACK ? -m_cols[t][r] : -m_rows[t][r];
+  }
+  // (I - M) X of a chunk of 32 (backward: of the transposed matrix), in place: fp32 products, since what is lost here stays in the state.
+  __device__ __forceinline__ void apply(const f32x4 (&diag)[4], const f32x4 (&below)[2], int half, f32x4 (&x)[2][kNT]) const {
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) {
+      const f32x4 x0 = x[0][n], x1 = x[1][n];
+      x[0][n] = mul_cols(diag[2 * half], x0, x0);
+      x[1][n] = mul_cols(diag[2 * half + 1], x1, x1);
+      if (BACK) x[0][n] = mul_cols(below[half], x1, x[0][n]);
+      else x[1][n] = mul_cols(below[half], x0, x[1][n]);
     }
   }
 
@@ -265,6 +267,12 @@ struct Solo {
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int n = 0; n < kNT; ++n) split(s[2 * kb][n], s[2 * kb + 1][n], sh[kb][n], sl[kb][n]);
+  }
+  __device__ __forceinline__ void split_state(const f32x4 (&s)[KA][kNT], bf16x8 (&sh)[KB][kNT], bf16x8 (&sm)[KB][kNT], bf16x8 (&sl)[KB][kNT]) const {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) split3(s[2 * kb][n], s[2 * kb + 1][n], sh[kb][n], sm[kb][n], sl[kb][n]);
   }
   // the state's high parts at dst [dv][dk]
   __device__ __forceinline__ void store_state(bf16_t* dst, const bf16x8 (&sh)[KB][kNT]) const {
@@ -346,16 +354,15 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
     const Buffer misses = rows_buffer(p.misses + (w.unit * p.T + token0) * p.dv + col0, p.dv, TRAIN ? n_tok : 0, p.dv - col0);
     wave_sync();  // the previous tokens' tiles are read
     w.place(c, n_tok, rows, tile_k, tile_v);
-    bf16x8 mh[4], ml[4];
-    f32x4 own[4];
-    w.solve(c, rows, scratch, mh, ml, own);
+    f32x4 diag[4], below[2], own[4];
+    w.solve(c, rows, scratch, diag, below, own);
     w.place_queries(c, tile_q);
     w.fetch(c);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (half == 1 && n_tok <= kHalf) break;
-      bf16x8 sh[KB][kNT], sl[KB][kNT];
-      w.split_state(s, sh, sl);
+      bf16x8 sh[KB][kNT], sm[KB][kNT], sl[KB][kNT];
+      w.split_state(s, sh, sm, sl);
       if (TRAIN && half == 0) w.store_state(p.chunk_states + (w.unit * p.chunks + group) * static_cast<int64_t>(p.dk) * p.dv, sh);
       // X = V - e^G K S
       f32x4 x[2][kNT];
@@ -369,7 +376,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
         for (int kb = 0; kb < KB; ++kb) {
           const bf16x8 kf = TK::row(tile_k, 16 * ti + l16, kb, grp);
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) y[n] = mfma16(kf, sl[kb][n], mfma16(kf, sh[kb][n], y[n]));
+          for (int n = 0; n < kNT; ++n) y[n] = mfma16(kf, sl[kb][n], mfma16(kf, sm[kb][n], mfma16(kf, sh[kb][n], y[n])));
         }
         const f32x4 grown = *reinterpret_cast<const f32x4*>(rows + kSoloGrown + 16 * ti + 4 * grp);
 #pragma unroll
@@ -380,14 +387,8 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
         }
       }
       // N = X - M X
+      w.apply(diag, below, half, x);
       bf16x8 xh[kNT], xl[kNT];
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) split(x[0][n], x[1][n], xh[n], xl[n]);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int n = 0; n < kNT; ++n)
-          x[t][n] = mfma16(ml[2 * half + t], xh[n], mfma16(mh[2 * half + t], xl[n], mfma16(mh[2 * half + t], xh[n], x[t][n])));
       if (TRAIN)
         w.store_rows(misses, p.dv * 32, n_off, 2 * half, tile_v + 32 * half * TV::STRIDE, x);
       // the output by columns of tokens: lane = token, four value columns each
@@ -417,7 +418,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) out[n] = mfma16(sl[kb][n], qf[kb], mfma16(sh[kb][n], qf[kb], out[n]));
+          for (int n = 0; n < kNT; ++n) out[n] = mfma16(sm[kb][n], qf[kb], mfma16(sh[kb][n], qf[kb], out[n]));
         const float grown = rows[kSoloGrown + 16 * ti + l16] * p.scale;
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
@@ -436,8 +437,9 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[t][n][r] *= keep[r];
       }
+      bf16x8 xm[kNT];
 #pragma unroll
-      for (int n = 0; n < kNT; ++n) split(x[0][n], x[1][n], xh[n], xl[n]);
+      for (int n = 0; n < kNT; ++n) split3(x[0][n], x[1][n], xh[n], xm[n], xl[n]);
       const float total = rows[kSoloTotal + half];
 #pragma unroll
       for (int a = 0; a < KA; ++a) {
@@ -446,7 +448,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
         for (int n = 0; n < kNT; ++n) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[a][n][r] *= total;
-          s[a][n] = mfma16(kt, xl[n], mfma16(kt, xh[n], s[a][n]));
+          s[a][n] = mfma16(kt, xl[n], mfma16(kt, xm[n], mfma16(kt, xh[n], s[a][n])));
         }
       }
     }
@@ -505,9 +507,8 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
     const Buffer to = rows_buffer(v0 + token0 * p.dvs[2], p.dvs[2], n_tok, p.dv - col0);
     wave_sync();
     w.place(c, n_tok, rows, tile_k, tile_o);
-    bf16x8 mh[4], ml[4];
-    f32x4 own[4];
-    w.solve(c, rows, scratch, mh, ml, own);
+    f32x4 diag[4], below[2], own[4];
+    w.solve(c, rows, scratch, diag, below, own);
     w.place_queries(c, tile_q);
     w.fetch(c);
 #pragma unroll
@@ -554,14 +555,8 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
         }
       }
       // dX
+      w.apply(diag, below, half, z);
       bf16x8 zh[kNT], zl[kNT];
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) split(z[0][n], z[1][n], zh[n], zl[n]);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int n = 0; n < kNT; ++n)
-          z[t][n] = mfma16(ml[2 * half + t], zh[n], mfma16(mh[2 * half + t], zl[n], mfma16(mh[2 * half + t], zh[n], z[t][n])));
       w.store_rows(to, v_pitch, v_off, 2 * half, tile_o + 32 * half * TV::STRIDE, z);
       // dS
       bf16x8 wh[kNT], wl[kNT];

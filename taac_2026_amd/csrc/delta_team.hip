@@ -21,8 +21,8 @@ namespace {
 __host__ __device__ constexpr int frag_rows(int ti, int tk) { return ti < 2 ? ti : 2 + (ti - 2) * 2 + tk; }
 __host__ __device__ constexpr int frag_cols(int tj, int tk) { return tj < 2 ? tj * 2 + tk : 2 + tj; }
 
-// One wavefront makes the block of one chunk (n valid tokens; rows beyond count as k = q = 0, g = 0, beta = 0): -M as hi and lo, P, and the
-// factors of its tokens. COLS: transposed fragments, for the backward. rows, temp, scratch: LDS.
+// One wavefront makes the block of one chunk (n valid tokens; rows beyond count as k = q = 0, g = 0, beta = 0): -M in three parts (two for the
+// backward), P, and the factors of its tokens. COLS: transposed fragments, for the backward. rows, temp, scratch: LDS.
 //
 // The 64 x 64 inverse: the four diagonal blocks of 16 by substitution, a column per lane, all four at once; the blocks below them by
 // products, M_21 = T_22 A_21 T_11 with T = I - M, first pairs of 16, then of 32.
@@ -147,10 +147,12 @@ __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, 
       a[r] = -first[r];
       c[r] = -second[r];
     }
-    bf16x8 hi8, lo8;
-    split(a, c, hi8, lo8);
+    bf16x8 hi8, mid8, lo8;
+    if (COLS) split(a, c, hi8, mid8);
+    else split3(a, c, hi8, mid8, lo8);
     *reinterpret_cast<bf16x8*>(block + kBlockM + f * kFrag + lane * 16) = hi8;
-    *reinterpret_cast<bf16x8*>(block + kBlockLow + f * kFrag + lane * 16) = lo8;
+    *reinterpret_cast<bf16x8*>(block + kBlockMid + f * kFrag + lane * 16) = mid8;
+    if (!COLS) *reinterpret_cast<bf16x8*>(block + kBlockLow + f * kFrag + lane * 16) = lo8;
     *reinterpret_cast<u32x4*>(block + kBlockP + f * kFrag + lane * 16) = u32x4{pf[f][0][0], pf[f][0][1], pf[f][1][0], pf[f][1][1]};
   };
   if (!COLS) {
@@ -190,12 +192,22 @@ __global__ __launch_bounds__(kWave) void delta_blocks_kernel(const DeltaParams p
   for (int i = threadIdx.x; i < kRowFloats; i += kWave) out[i] = rows[i];
 }
 
-// Half fragments: the four values of one 16-row result, as the first or second half of a fragment of 32 rows in LDS.
+// Half fragments: the four values of one 16-row result, as the first or second half of a fragment of 32 rows in LDS. In two parts, or in
+// three.
 __device__ __forceinline__ void put_half(uint8_t* frags, int tile, int lane, const f32x4& v, int low_at) {
   const u32x2 hi = round4(v);
   uint8_t* at = frags + (tile / 2) * kFrag + lane * 16 + (tile % 2) * 8;
   *reinterpret_cast<u32x2*>(at) = hi;
   *reinterpret_cast<u32x2*>(at + low_at) = rest4(v, hi);
+}
+__device__ __forceinline__ void put_half3(uint8_t* frags, int tile, int lane, const f32x4& v, int low_at) {
+  const u32x2 hi = round4(v);
+  const f32x4 left = left4(v, hi);
+  const u32x2 mid = round4(left);
+  uint8_t* at = frags + (tile / 2) * kFrag + lane * 16 + (tile % 2) * 8;
+  *reinterpret_cast<u32x2*>(at) = hi;
+  *reinterpret_cast<u32x2*>(at + low_at) = mid;
+  *reinterpret_cast<u32x2*>(at + 2 * low_at) = rest4(left, mid);
 }
 __device__ __forceinline__ bf16x8 get_frag(const uint8_t* frags, int f, int lane) {
   return *reinterpret_cast<const bf16x8*>(frags + f * kFrag + lane * 16);
@@ -203,14 +215,14 @@ __device__ __forceinline__ bf16x8 get_frag(const uint8_t* frags, int f, int lane
 
 // NT: column tiles of 16 of a team.
 template <int DK, int NT>
-struct TeamLds {  // of every column tile: fragments hi, then lo
+struct TeamLds {  // of every column tile: fragments of the first part, then of the second, and (not of N) of the third
   static constexpr int KB = DK / 32;
-  static constexpr int kStateTile = 2 * KB * kFrag, kRowTile = 4 * kFrag;
+  static constexpr int kStateTile = 3 * KB * kFrag, kRowTile = 4 * kFrag, kRowTile3 = 6 * kFrag;
   static constexpr int kState = 0;
   static constexpr int kX = kState + NT * kStateTile;
-  static constexpr int kN = kX + NT * kRowTile;
+  static constexpr int kN = kX + NT * kRowTile3;
   static constexpr int kW = kN + NT * kRowTile;
-  static constexpr int kTileX = kW + NT * kRowTile;
+  static constexpr int kTileX = kW + NT * kRowTile3;
   static constexpr int kXRow = 16 * NT + 4;             // elements of a token's columns
   static constexpr int kTileK = (kTileX + kChunk * kXRow * 2 + 63) / 64 * 64;
   static constexpr int kForward = kTileK + Tile<DK>::BYTES;
@@ -223,7 +235,7 @@ struct TeamLds {  // of every column tile: fragments hi, then lo
 template <int KB, int NT>
 struct TeamChunk {
   bf16x8 kf[KB], qf[KB];
-  bf16x8 mh[2], ml[2], pf[2];
+  bf16x8 mh[2], mm[2], ml[2], pf[2];
   f32x4 grown, keep;
   float grown_row, total;
   u32x2 x[NT];  // 4 NT columns of a token of V (backward: of dO), on their way into LDS
@@ -328,7 +340,8 @@ struct Team {
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk) {
       c.mh[tk] = read8(block, frag_off[tk], kBlockM);
-      c.ml[tk] = read8(block, frag_off[tk], kBlockLow);
+      c.mm[tk] = read8(block, frag_off[tk], kBlockMid);
+      if (!COLS) c.ml[tk] = read8(block, frag_off[tk], kBlockLow);
       c.pf[tk] = read8(block, frag_off[tk], kBlockP);
     }
     at += COLS ? -1 : 1;
@@ -404,7 +417,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
           if (row < p.dk) s[i][n][r] = p.state_in[(m.unit * p.dk + row) * p.dv + col0 + 16 * n + l16];
         }
       }
-      if (m.owner) put_half(s_frags + n * L::kStateTile, a, lane, s[i][n], KB * kFrag);
+      if (m.owner) put_half3(s_frags + n * L::kStateTile, a, lane, s[i][n], KB * kFrag);
     }
   }
 
@@ -426,15 +439,17 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
       f32x4 y = zero4(), y2 = zero4();
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        const bf16x8 hi = get_frag(s_frags + n * L::kStateTile, kb, lane), lo = get_frag(s_frags + n * L::kStateTile + KB * kFrag, kb, lane);
+        const uint8_t* state = s_frags + n * L::kStateTile;
+        const bf16x8 hi = get_frag(state, kb, lane), mid = get_frag(state + KB * kFrag, kb, lane);
         y = mfma16(cur.kf[kb], hi, y);
-        y2 = mfma16(cur.kf[kb], lo, y2);
-        if (NT == 1) sh[n][NT > 1 ? 0 : kb] = hi, sl[n][NT > 1 ? 0 : kb] = lo;
+        y2 = mfma16(cur.kf[kb], mid, y2);
+        y2 = mfma16(cur.kf[kb], get_frag(state + 2 * KB * kFrag, kb, lane), y2);
+        if (NT == 1) sh[n][NT > 1 ? 0 : kb] = hi, sl[n][NT > 1 ? 0 : kb] = mid;
       }
       const bf16x4 v = m.values(tile_x, 16 * wave, n);
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[n][r] = fmaf(-cur.grown[r], y[r] + y2[r], static_cast<float>(v[r]));
-      put_half(x_frags + n * L::kRowTile, wave, lane, x[n], 2 * kFrag);
+      put_half3(x_frags + n * L::kRowTile3, wave, lane, x[n], 2 * kFrag);
     }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -446,14 +461,17 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
     const float grown = cur.grown_row * p.scale;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const uint8_t* from = x_frags + n * L::kRowTile;
-      f32x4 x2 = zero4(), x3 = zero4();
+      const uint8_t* from = x_frags + n * L::kRowTile3;
+      f32x4 x2 = zero4(), x3 = zero4();  // products of parts whose sizes are 2^-8 and 2^-16 of the first ones'
 #pragma unroll
       for (int tk = 0; tk < 2; ++tk)
         if (tk <= wave / 2) {
-          const bf16x8 xh = get_frag(from, tk, lane), xl = get_frag(from + 2 * kFrag, tk, lane);
+          const bf16x8 xh = get_frag(from, tk, lane), xm = get_frag(from + 2 * kFrag, tk, lane), xl = get_frag(from + 4 * kFrag, tk, lane);
           x[n] = mfma16(cur.mh[tk], xh, x[n]);
-          x2 = mfma16(cur.mh[tk], xl, x2);
+          x2 = mfma16(cur.mh[tk], xm, x2);
+          x3 = mfma16(cur.mh[tk], xl, x3);
+          x2 = mfma16(cur.mm[tk], xh, x2);
+          x3 = mfma16(cur.mm[tk], xm, x3);
           x3 = mfma16(cur.ml[tk], xh, x3);
         }
       f32x4 out2 = zero4();
@@ -470,7 +488,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
         x[n][r] += x2[r] + x3[r];
         w[r] = x[n][r] * cur.keep[r];
       }
-      put_half(w_frags + n * L::kRowTile, wave, lane, w, 2 * kFrag);
+      put_half3(w_frags + n * L::kRowTile3, wave, lane, w, 2 * kFrag);
       put_half(n_frags + n * L::kRowTile, wave, lane, x[n], 2 * kFrag);
 #pragma unroll
       for (int r = 0; r < 4; ++r) out[n][r] = (out[n][r] + out2[r]) * grown;
@@ -488,7 +506,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
         for (int tk = 0; tk < 2; ++tk) kt[tk] = TK::keys_frag(tile_k, tk, a, l16, grp);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint8_t* from = w_frags + n * L::kRowTile;
+          const uint8_t* from = w_frags + n * L::kRowTile3;
           f32x4 s2 = zero4();
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[i][n][r] *= cur.total;
@@ -496,10 +514,11 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
           for (int tk = 0; tk < 2; ++tk) {
             s[i][n] = mfma16(kt[tk], get_frag(from, tk, lane), s[i][n]);
             s2 = mfma16(kt[tk], get_frag(from + 2 * kFrag, tk, lane), s2);
+            s2 = mfma16(kt[tk], get_frag(from + 4 * kFrag, tk, lane), s2);
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[i][n][r] += s2[r];
-          put_half(s_frags + n * L::kStateTile, a, lane, s[i][n], KB * kFrag);
+          put_half3(s_frags + n * L::kStateTile, a, lane, s[i][n], KB * kFrag);
         }
       }
     }
@@ -647,7 +666,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
           const bf16x8 zh = get_frag(from, tk, lane), zl = get_frag(from + 2 * kFrag, tk, lane);
           z[n] = mfma16(cur.mh[tk], zh, z[n]);
           z2 = mfma16(cur.mh[tk], zl, z2);
-          z3 = mfma16(cur.ml[tk], zh, z3);
+          z3 = mfma16(cur.mm[tk], zh, z3);
         }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {

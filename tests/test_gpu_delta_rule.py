@@ -633,3 +633,19 @@ def test_step_of_a_thousand_samples_of_one_slot(device):
         out = gated_delta_rule_step(*rows, pool, state_index=torch.full((1000,), 2, dtype=torch.int64, device=device))
     _check_step(out.transpose(0, 2), pool[2:], want, final, torch.bfloat16)
     assert (pool[:2] == 0).all()
+
+
+@pytest.mark.parametrize("sizes", [(4, 2, 2, 8, 16), (8, 2, 2, 16, 32), (8, 1, 2, 32, 32), (2, 2, 4, 64, 64), (8, 2, 2, 72, 32), (2, 1, 2, 128, 128), (40, 2, 2, 128, 128),
+                                   (1100, 1, 1, 16, 16), (700, 1, 1, 32, 32), (520, 1, 1, 64, 64), (70, 1, 1, 128, 128)])
+@pytest.mark.parametrize("tokens", [33, 64, 300, 1500])
+def test_the_state_has_float32_precision(device, sizes, tokens):
+    """Sixteen units of float32, 2^-20, over the whole state, with decays so slow that what a chunk adds wrongly stays. Everything that reaches the state
+    enters its products with all 24 bits; what is left are fp32 sums of at most 128 products, whose roundings of 2^-25 at random add up to 2^-21.5 of the
+    sum's size, and a chunk leaves the roundings of the chunks before it at most as they are while it overwrites what they are part of. One factor
+    in pairs of bf16 (2^-18.4 of its size at random) is more than this at once."""
+    inputs = [t.to(device) for t in _draw(sizes[0], tokens, *sizes[1:], seed=27)]
+    inputs[3] *= 0.02
+    _, want, _ = delta_rule(*inputs)
+    with torch.no_grad():
+        _, state = gated_delta_rule(*inputs, return_state=True)
+    assert (state.double() - want).norm() <= 2.0**-20 * want.norm(), (state.double() - want).norm() / want.norm()
