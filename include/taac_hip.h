@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define TAAC_ABI_VERSION 10
+#define TAAC_ABI_VERSION 11
 
 enum taac_status {
   TAAC_OK = 0,
@@ -615,7 +615,8 @@ int taac_row_rstd(const float* qk_sumsq, int64_t M, int32_t d_model, float eps, 
  * -1e5 count as -1e5. Infinities and NaN of a valid token reach the whole chunk of 64
  * tokens that it lies in, the tokens in front of it too, and everything behind it in its (sample, head).
  * state_in: fp32 [B, H, dk, dv] or NULL (zeros); state_out: the same shape, or NULL; it may be state_in.
- * chunk_states (bf16 [B, H, ceil(T / 64), dv, dk]) and misses (bf16 [B, H, T, dv]): what taac_delta_rule_bwd reads, or both NULL.
+ * chunk_states (bf16 [B, H, ceil(T / 64), dv, dk]) and misses (bf16 [2, B, H, T, dv], rounded and what the rounding left):
+ * what taac_delta_rule_bwd reads, or both NULL.
  * taac_delta_rule_bwd: gradients of q, k, v, log_decay and beta (logical shapes and dtypes of the inputs, strides of their own) for
  * grad_o; grad_states (bf16, the size of chunk_states) is scratch. The initial state has no gradient here. Rows at or beyond a
  * sample's length get zeros. Every sum has a fixed order.

@@ -87,8 +87,8 @@ def _workspace_bytes(batch: int, heads: int, tokens: int, key_width: int, value_
     return _native.load_library().taac_delta_rule_workspace_bytes(batch, heads, tokens, key_width, value_width)
 
 
-def _workspace(k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
-    return v.new_empty(_workspace_bytes(*v.shape[:3], k.shape[3], v.shape[3]), dtype=torch.uint8)
+def _workspace(like: torch.Tensor, batch: int, heads: int, tokens: int, key_width: int, value_width: int) -> torch.Tensor:
+    return like.new_empty(_workspace_bytes(batch, heads, tokens, key_width, value_width), dtype=torch.uint8)
 
 
 def _forward(q, k, v, log_decay, beta, scale, lengths, initial_state, return_state, keep):
@@ -99,9 +99,9 @@ def _forward(q, k, v, log_decay, beta, scale, lengths, initial_state, return_sta
     states = misses = None
     if keep:
         states = v.new_empty(batch, heads, (tokens + CHUNK - 1) // CHUNK, value_width, key_width)
-        misses = v.new_empty(batch, heads, tokens, value_width)
+        misses = v.new_empty(2, batch, heads, tokens, value_width)
     library = _native.load_library()
-    workspace = _workspace(k, v)
+    workspace = _workspace(v, batch, heads, tokens, key_width, value_width)
     with _native.on_device(v.device):
         status = library.taac_delta_rule_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), _native.ptr(lengths), out.data_ptr(),
@@ -114,8 +114,8 @@ def _forward(q, k, v, log_decay, beta, scale, lengths, initial_state, return_sta
 
 
 class _GatedDeltaRuleFunction(torch.autograd.Function):
-    """The forward keeps the state in front of every chunk and what the state missed of every value, in bf16; the backward makes
-    the rest again from q, k and the gates."""
+    """The forward keeps the state in front of every chunk in bf16 and what the state missed of every value in two parts of bf16;
+    the backward makes the rest again from q, k and the gates."""
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, beta, scale: float, lengths, initial_state):
@@ -130,14 +130,14 @@ class _GatedDeltaRuleFunction(torch.autograd.Function):
     def backward(ctx, grad_out):
         q, k, log_decay, beta, lengths, states, misses = ctx.saved_tensors
         batch, key_heads, tokens, key_width = k.shape
-        heads, value_width = misses.shape[1], misses.shape[3]
+        heads, value_width = misses.shape[2], misses.shape[4]
         grad_out = _rows_view(grad_out)
         library = _native.load_library()
         with _native.on_device(k.device):
             grad_q, grad_k = (_token_major(batch, key_heads, tokens, key_width, k) for _ in range(2))
             grad_v = _token_major(batch, heads, tokens, value_width, k)
             grad_decay, grad_beta = (beta.new_empty_strided((batch, heads, tokens), (tokens * heads, 1, heads)) for _ in range(2))
-            grad_states, workspace = torch.empty_like(states), _workspace(k, misses)
+            grad_states, workspace = torch.empty_like(states), _workspace(k, batch, heads, tokens, key_width, value_width)
             status = library.taac_delta_rule_bwd(
                 q.data_ptr(), k.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), _native.ptr(lengths), states.data_ptr(),
                 misses.data_ptr(), grad_out.data_ptr(), grad_q.data_ptr(), grad_k.data_ptr(), grad_v.data_ptr(), grad_decay.data_ptr(),

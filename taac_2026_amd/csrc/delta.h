@@ -45,6 +45,7 @@ struct DeltaParams {
   float* state_out;          // [B, H, dk, dv] or null
   bf16_t* chunk_states;      // [B, H, chunks, dv, dk] or null: the state in front of every chunk, transposed
   bf16_t* misses;            // [B, H, T, dv] or null: N
+  bf16_t* misses_low;        // [B, H, T, dv]: what the rounding of N left
   uint8_t* blocks;           // [B, H, chunks] blocks in memory (the form for few heads)
   // backward
   const bf16_t* grad_o;

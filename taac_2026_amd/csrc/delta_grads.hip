@@ -14,9 +14,9 @@
 // their time and issue vector instructions for 25 %. 128 wide, where the tiles leave room for one: 18 us per chunk and head, 2.4 TB/s; two
 // sets of four wavefronts on one chunk (rows and columns at once) took 3 % longer.
 //
-// N, S, dS' and dX are read back in bf16, one rounding each: they only meet the outputs. Of the 2.5e-3 that a gradient is off, 1.7e-3 is its own
-// rounding, 1.7e-3 that of N, 0.5e-3 that of each of the others; N in two parts would cost a tenth of all bytes. Key heads that serve
-// several value heads sum their gradients in registers, in the order of the heads.
+// S, dS' and dX are read back in bf16, one rounding each: they only meet the outputs, of which they are parts (0.2e-3 to 1.0e-3 of a gradient, whose
+// own rounding is 1.7e-3; together 1.8e-3 to 2.4e-3). N, which every pair of tokens has as a factor, is kept in two parts: its one rounding alone cost
+// 1.7e-3. Key heads that serve several value heads sum their gradients in registers, in the order of the heads.
 #include "delta.h"
 
 namespace taac {
@@ -30,8 +30,10 @@ struct GradLds {
   static constexpr int kTileO = kTileQ + Tile<DK>::BYTES;
   static constexpr int kTileX = kTileO + Tile<DV>::BYTES;
   static constexpr int kTileN = kTileX + Tile<DV>::BYTES;
-  static constexpr int kState = kTileN + Tile<DV>::BYTES;  // DV rows of DK
-  static constexpr int kGradState = kState + DV * Tile<DK>::STRIDE * 2;
+  static constexpr int kTileLow = kTileN + Tile<DV>::BYTES;  // what the rounding of N left
+  static constexpr int kState = kTileLow + Tile<DV>::BYTES;  // DV rows of DK
+  static constexpr bool kTurns = DK > 64 && DV > 64;         // S and dS' take turns: both do not fit
+  static constexpr int kGradState = kTurns ? kState : kState + DV * Tile<DK>::STRIDE * 2;
   static constexpr int kRows = kGradState + DV * Tile<DK>::STRIDE * 2;
   static constexpr int kTotal = kRows + (kRowFloats + kTempFloats + 64 + 3 * 64 + 16) * 4;
 };
@@ -58,6 +60,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
   bf16_t* tile_o = reinterpret_cast<bf16_t*>(smem + L::kTileO);
   bf16_t* tile_x = reinterpret_cast<bf16_t*>(smem + L::kTileX);
   bf16_t* tile_n = reinterpret_cast<bf16_t*>(smem + L::kTileN);
+  bf16_t* tile_l = reinterpret_cast<bf16_t*>(smem + L::kTileLow);
   bf16_t* tile_s = reinterpret_cast<bf16_t*>(smem + L::kState);
   bf16_t* tile_g = reinterpret_cast<bf16_t*>(smem + L::kGradState);
   float* rows = reinterpret_cast<float*>(smem + L::kRows);
@@ -110,7 +113,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
     asm volatile("" : "+v"(l16), "+v"(grp), "+v"(tid));
     const int row = 16 * wave + l16;  // this lane's token
     // everything this head reads is requested before any of it is waited for
-    typename TV::template Piece<kChunk, kThreads> o_in, x_in, n_in;
+    typename TV::template Piece<kChunk, kThreads> o_in, x_in, n_in, l_in;
     typename TK::template Piece<DV, kThreads> s_in, g_in;
     const int64_t at_state = (unit * p.chunks + chunk) * static_cast<int64_t>(p.dk) * p.dv;
     GateBits gates;
@@ -118,6 +121,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
     o_in.load(p.grad_o + b * p.dos[0] + h * p.dos[1] + token0 * p.dos[2], p.dos[2], n_tok, p.dv, tid);
     x_in.load(p.grad_v + b * p.dvs[0] + h * p.dvs[1] + token0 * p.dvs[2], p.dvs[2], n_tok, p.dv, tid);
     n_in.load(p.misses + (unit * p.T + token0) * p.dv, p.dv, n_tok, p.dv, tid);
+    l_in.load(p.misses_low + (unit * p.T + token0) * p.dv, p.dv, n_tok, p.dv, tid);
     s_in.load(p.chunk_states + at_state, p.dk, p.dv, p.dk, tid);
     g_in.load(p.grad_states + at_state, p.dk, p.dv, p.dk, tid);
     float dot_state = s_in.dot(g_in);
@@ -126,8 +130,9 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
     o_in.store(tile_o, tid);
     x_in.store(tile_x, tid);
     n_in.store(tile_n, tid);
+    l_in.store(tile_l, tid);
     s_in.template store<true>(tile_s, tid);
-    g_in.template store<true>(tile_g, tid);
+    if (!L::kTurns) g_in.template store<true>(tile_g, tid);
     __syncthreads();
 
     const float hi_t = temp[kTempHi + row], lo_t = temp[kTempLow + row], beta_t = temp[kTempBeta + row], grown = rows[kRowGrown + row];
@@ -176,9 +181,9 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
         f32x4 qk = zero4(), kk = zero4();
 #pragma unroll
         for (int vb = 0; vb < VB; ++vb) {
-          const bf16x8 nf = TV::row(tile_n, 16 * t + l16, vb, grp);
-          bv[half] = mfma16(nf, first[vb], bv[half]);
-          ev[half] = mfma16(nf, second[vb], ev[half]);
+          const bf16x8 nf = TV::row(tile_n, 16 * t + l16, vb, grp), lf = TV::row(tile_l, 16 * t + l16, vb, grp);
+          bv[half] = mfma16(lf, first[vb], mfma16(nf, first[vb], bv[half]));
+          ev[half] = mfma16(lf, second[vb], mfma16(nf, second[vb], ev[half]));
         }
 #pragma unroll
         for (int kb = 0; kb < KA / 2; ++kb) {
@@ -230,9 +235,17 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
       }
       __builtin_amdgcn_sched_barrier(0);  // keeps the next round's reads, and their registers, behind this one
     }
+    if (L::kTurns) {
+      __syncthreads();  // S is no longer read
+      g_in.template store<true>(tile_g, tid);
+      __syncthreads();
+    }
     // as j: C
 #pragma unroll
-    for (int vb = 0; vb < VB; ++vb) first[vb] = TV::row(tile_n, row, vb, grp);
+    for (int vb = 0; vb < VB; ++vb) {
+      first[vb] = TV::row(tile_n, row, vb, grp);
+      second[vb] = TV::row(tile_l, row, vb, grp);
+    }
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk) {
       f32x4 bv[2], ev[2];
@@ -244,8 +257,9 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
         f32x4 qk = zero4(), kk = zero4();
 #pragma unroll
         for (int vb = 0; vb < VB; ++vb) {
-          bv[half] = mfma16(TV::row(tile_o, 16 * t + l16, vb, grp), first[vb], bv[half]);
-          ev[half] = mfma16(TV::row(tile_x, 16 * t + l16, vb, grp), first[vb], ev[half]);
+          const bf16x8 of = TV::row(tile_o, 16 * t + l16, vb, grp), xf = TV::row(tile_x, 16 * t + l16, vb, grp);
+          bv[half] = mfma16(of, second[vb], mfma16(of, first[vb], bv[half]));
+          ev[half] = mfma16(xf, second[vb], mfma16(xf, first[vb], ev[half]));
         }
 #pragma unroll
         for (int kb = 0; kb < KA / 2; ++kb) {
@@ -278,7 +292,7 @@ __global__ __launch_bounds__(4 * kWave, DK <= 32 && DV <= 64 ? 3 : DK <= 64 && D
 #pragma unroll
       for (int vb = 0; vb < VB; ++vb) {
         const bf16x8 gf = TK::keys_frag(tile_g, vb, a, l16, grp);
-        dc = mfma16(gf, first[vb], dc);
+        dc = mfma16(gf, second[vb], mfma16(gf, first[vb], dc));
       }
       const bf16x4 kv = *reinterpret_cast<const bf16x4*>(tile_k + row * TK::STRIDE + state_row(a, 4 * grp));
 #pragma unroll

@@ -24,6 +24,12 @@ int take_workspace(const char* name, DeltaParams& p, void* workspace, int64_t gi
   return TAAC_OK;
 }
 
+// Two planes: N rounded, and the rest.
+void take_misses(DeltaParams& p, void* misses) {
+  p.misses = static_cast<bf16_t*>(misses);
+  if (misses != nullptr) p.misses_low = p.misses + static_cast<int64_t>(p.B) * p.H * p.T * p.dv;
+}
+
 int check_sizes(const char* name, const DeltaParams& p) {
   if (p.B < 0 || p.H <= 0 || p.T < 0 || p.dk <= 0 || p.dv <= 0 || p.group <= 0)
     return set_error(TAAC_ERR_INVALID_VALUE, "%s: batch and tokens must be >= 0, heads and widths > 0", name);
@@ -81,7 +87,8 @@ extern "C" int taac_delta_rule_fwd(const void* q, const void* k, const void* v, 
   p.q = static_cast<const bf16_t*>(q), p.k = static_cast<const bf16_t*>(k), p.v = static_cast<const bf16_t*>(v);
   p.o = static_cast<bf16_t*>(o), p.log_decay = log_decay, p.beta = beta, p.lengths = lengths;
   p.state_in = state_in, p.state_out = state_out;
-  p.chunk_states = static_cast<bf16_t*>(chunk_states), p.misses = static_cast<bf16_t*>(misses);
+  p.chunk_states = static_cast<bf16_t*>(chunk_states);
+  take_misses(p, misses);
   hipStream_t s = as_stream(stream);
   bool team;
   if (int rc = take_workspace(name, p, workspace, workspace_bytes, &team)) return rc;
@@ -124,7 +131,7 @@ extern "C" int taac_delta_rule_bwd(const void* q, const void* k, const void* log
   if (int rc = take_strides(name, "grad_beta", grad_beta, gbeta_strides, p.dbs, false, 1)) return rc;
   p.q = static_cast<const bf16_t*>(q), p.k = static_cast<const bf16_t*>(k), p.log_decay = log_decay, p.beta = beta, p.lengths = lengths;
   p.chunk_states = const_cast<bf16_t*>(static_cast<const bf16_t*>(chunk_states));
-  p.misses = const_cast<bf16_t*>(static_cast<const bf16_t*>(misses));
+  take_misses(p, const_cast<void*>(misses));
   p.grad_o = static_cast<const bf16_t*>(grad_o);
   p.grad_q = static_cast<bf16_t*>(grad_q), p.grad_k = static_cast<bf16_t*>(grad_k), p.grad_v = static_cast<bf16_t*>(grad_v);
   p.grad_decay = grad_decay, p.grad_beta = grad_beta, p.grad_states = static_cast<bf16_t*>(grad_states);

@@ -282,14 +282,17 @@ struct Solo {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) write8(to, state_off[kb] + n * p.dk * 32, sh[kb][n]);
   }
-  // Rows of one chunk of 32 tokens, held by columns, to rows of a group from tile `first` on (off: quads(); pitch: bytes of 16 rows): turned through
-  // tile's rows, which have been read.
-  __device__ __forceinline__ void store_rows(Buffer to, uint32_t pitch, const uint32_t (&off)[kNT], int first, bf16_t* tile, const f32x4 (&x)[2][kNT]) const {
+  // Rows of one chunk of 32 tokens, held by columns as operands over the tokens, to rows of a group from tile `first` on (off: quads(); pitch: bytes
+  // of 16 rows): turned through tile's rows, which have been read.
+  __device__ __forceinline__ void store_rows(Buffer to, uint32_t pitch, const uint32_t (&off)[kNT], int first, bf16_t* tile, const bf16x8 (&x)[kNT]) const {
     u32x2 v[2][kNT];
+    wave_sync();
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int n = 0; n < kNT; ++n) {
+      const u32x4 words = __builtin_bit_cast(u32x4, x[n]);
 #pragma unroll
-      for (int n = 0; n < kNT; ++n) *reinterpret_cast<u32x2*>(tile + (2 * t + n) * 320 + l16 * 20 + grp * 4) = round4(x[t][n]);
+      for (int t = 0; t < 2; ++t) *reinterpret_cast<u32x2*>(tile + (2 * t + n) * 320 + l16 * 20 + grp * 4) = u32x2{words[2 * t], words[2 * t + 1]};
+    }
     wave_sync();
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -351,7 +354,9 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
     const int64_t token0 = static_cast<int64_t>(group) * kChunk;
     const int n_tok = w.tokens_of(group);
     const Buffer to = rows_buffer(o0 + token0 * p.os[2], p.os[2], n_tok, p.dv - col0);
-    const Buffer misses = rows_buffer(p.misses + (w.unit * p.T + token0) * p.dv + col0, p.dv, TRAIN ? n_tok : 0, p.dv - col0);
+    const int64_t miss_at = (w.unit * p.T + token0) * p.dv + col0;
+    const Buffer misses = rows_buffer(p.misses + miss_at, p.dv, TRAIN ? n_tok : 0, p.dv - col0);
+    const Buffer misses_low = rows_buffer(p.misses_low + miss_at, p.dv, TRAIN ? n_tok : 0, p.dv - col0);
     wave_sync();  // the previous tokens' tiles are read
     w.place(c, n_tok, rows, tile_k, tile_v);
     f32x4 diag[4], below[2], own[4];
@@ -389,11 +394,13 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
       // N = X - M X
       w.apply(diag, below, half, x);
       bf16x8 xh[kNT], xl[kNT];
-      if (TRAIN)
-        w.store_rows(misses, p.dv * 32, n_off, 2 * half, tile_v + 32 * half * TV::STRIDE, x);
-      // the output by columns of tokens: lane = token, four value columns each
 #pragma unroll
       for (int n = 0; n < kNT; ++n) split(x[0][n], x[1][n], xh[n], xl[n]);
+      if (TRAIN) {
+        w.store_rows(misses, p.dv * 32, n_off, 2 * half, tile_v + 32 * half * TV::STRIDE, xh);
+        w.store_rows(misses_low, p.dv * 32, n_off, 2 * half, tile_v + 32 * half * TV::STRIDE, xl);
+      }
+      // the output by columns of tokens: lane = token, four value columns each
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int ti = 2 * half + t;
@@ -557,7 +564,9 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
       // dX
       w.apply(diag, below, half, z);
       bf16x8 zh[kNT], zl[kNT];
-      w.store_rows(to, v_pitch, v_off, 2 * half, tile_o + 32 * half * TV::STRIDE, z);
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) zh[n] = round8(z[0][n], z[1][n]);
+      w.store_rows(to, v_pitch, v_off, 2 * half, tile_o + 32 * half * TV::STRIDE, zh);
       // dS
       bf16x8 wh[kNT], wl[kNT];
       const f32x4 g0 = *reinterpret_cast<const f32x4*>(rows + kSoloGrown + 32 * half + 4 * grp);

@@ -424,6 +424,7 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
   bf16_t* o_at = o0;
   bf16_t* state_at = TRAIN ? p.chunk_states + m.unit * p.chunks * static_cast<int64_t>(p.dk) * p.dv : nullptr;
   bf16_t* miss_at = TRAIN ? p.misses + m.unit * p.T * p.dv + col0 : nullptr;
+  const int64_t low_at = TRAIN ? p.misses_low - p.misses : 0;
   auto step = [&](int chunk, typename M::Chunk& cur, typename M::Chunk& next) __attribute__((always_inline)) {
     const int n_tok = m.tokens_of(chunk);
     m.fetch_keys(next);
@@ -538,12 +539,13 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
       for (int r = 0; r < 4; ++r) out[n][r] += out2[r];
       write4(to, o_off[n], round4(out[n]));
     }
-    if (TRAIN) {  // N of the own tokens, rounded as its fragments' high parts are, by rows
-      const Buffer misses = rows_buffer(miss_at, p.dv, n_tok, p.dv - col0);
+    if (TRAIN) {  // both parts of N of the own tokens, by rows
+      const Buffer misses = rows_buffer(miss_at, p.dv, n_tok, p.dv - col0), low = rows_buffer(miss_at + low_at, p.dv, n_tok, p.dv - col0);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const bf16x4 rounded = TK::read_tr(reinterpret_cast<const bf16_t*>(n_frags + n * L::kRowTile + turned_at));
-        write4(misses, n_off[n], __builtin_bit_cast(u32x2, rounded));
+        const uint8_t* from = n_frags + n * L::kRowTile + turned_at;
+        write4(misses, n_off[n], __builtin_bit_cast(u32x2, TK::read_tr(reinterpret_cast<const bf16_t*>(from))));
+        write4(low, n_off[n], __builtin_bit_cast(u32x2, TK::read_tr(reinterpret_cast<const bf16_t*>(from + 2 * kFrag))));
       }
       miss_at += kChunk * p.dv;
     }
