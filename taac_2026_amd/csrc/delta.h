@@ -24,8 +24,8 @@
 // with all 24 bits, as hi + mid + lo of bf16: three matrix instructions where one factor is exact, six where none is (the products whose parts
 // together stand 24 bits below the first are left out); or M and X in fp32 products. The state behind a history is then as near 64 bits as in a
 // plain fp32 evaluation, 0.8e-7 to 2.5e-7 of its norm against 0.8e-7 to 3e-7 (all four in hi + lo: 2.8e-6, S alone where decays are slow: 1.3e-6).
-// What only meets outputs enters as hi + lo (16 bits): S and N for O, and the backward's recurrence, whose results are bf16.
-// P enters rounded once: it only reaches the output.
+// What only meets outputs enters as hi + lo (16 bits): S, N and P for O (of wide heads P once rounded, see the blocks below), and the backward's
+// recurrence, whose results are bf16.
 // Cumulative decays are summed in 64 bits and kept as pairs, so that G_i - G_j of a fast decaying head keeps fp32 precision.
 #pragma once
 
@@ -74,10 +74,17 @@ namespace {
 
 constexpr int kChunk = 64;
 constexpr int kFrag = 1024;              // bytes of one operand fragment of a wavefront
-constexpr int kBlockM = 0, kBlockMid = 6 * kFrag, kBlockLow = 12 * kFrag, kBlockP = 18 * kFrag, kBlockRows = 24 * kFrag;
-// floats behind the fragments of a block: e^G, beta e^(G_64 - G), e^G_64 (then e^ of the second and third tile's own decays)
+// A block in memory: the tokens' factors, M in three parts, P, and what the rounding of P left (the backward, whose M has two parts, has that in the
+// place of the third). The forward of wide heads has P rounded once: there that leaves outputs 2.3e-3 from 64 bits, of which 1.7e-3 is their own
+// rounding, and six fragments more a block take 2 x 16 heads x 8192 tokens, 128 wide, from 255 to 280 us. Of narrow heads, where pairs within a chunk
+// make more of an output, it would be up to 2.5e-3.
+constexpr int kBlockRows = 0, kBlockM = 640, kBlockMid = kBlockM + 6 * kFrag, kBlockLow = kBlockM + 12 * kFrag, kBlockP = kBlockM + 18 * kFrag,
+              kBlockPLow = kBlockM + 24 * kFrag;
+__host__ __device__ constexpr bool low_scores(int dk) { return dk <= 64; }
+__host__ __device__ constexpr int block_bytes(int dk) { return kBlockM + (low_scores(dk) ? 30 : 24) * kFrag; }
+// the floats of a block: e^G, beta e^(G_64 - G), e^G_64 (then e^ of the second and third tile's own decays)
 constexpr int kRowGrown = 0, kRowKeep = 64, kRowTotal = 128, kRowFloats = 144;
-constexpr int kBlockBytes = kBlockRows + kRowFloats * 4;
+static_assert(kRowFloats * 4 <= kBlockM);
 // floats that only the maker of a block needs: G as a pair, beta; e^(G - G in front of the tile of 16), e^(G behind the tile - G), that times beta
 constexpr int kTempHi = 0, kTempLow = 64, kTempBeta = 128, kTempIn = 192, kTempOut = 256, kTempOutBeta = 320, kTempFloats = 384;
 // Scratch for the diagonal blocks: rows of 20 floats, blocks 16 banks apart.

@@ -12,7 +12,7 @@ namespace {
 bool uses_teams(int64_t heads, int32_t dk, int32_t dv) { return dk > 64 || heads * ((dv + 15) / 16) <= (dk <= 32 ? 512 : 768); }
 
 int64_t workspace_of(int64_t heads, int32_t T, int32_t dk, int32_t dv) {
-  return uses_teams(heads, dk, dv) ? heads * ((static_cast<int64_t>(T) + kChunk - 1) / kChunk) * kBlockBytes : 0;
+  return uses_teams(heads, dk, dv) ? heads * ((static_cast<int64_t>(T) + kChunk - 1) / kChunk) * block_bytes(dk) : 0;
 }
 
 int take_workspace(const char* name, DeltaParams& p, void* workspace, int64_t given, bool* team) {

@@ -418,7 +418,8 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
 #pragma unroll
           for (int r = 0; r < 4; ++r) score[u][r] = u < t || l16 >= 4 * grp + r ? score[u][r] * (p.scale * gam[r]) : 0.f;
         }
-        const bf16x8 pf = round8(score[0], score[1]);
+        bf16x8 pf, pl;
+        split(score[0], score[1], pf, pl);
         f32x4 out[kNT];
 #pragma unroll
         for (int n = 0; n < kNT; ++n) out[n] = zero4();
@@ -431,7 +432,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_kernel(con
         for (int n = 0; n < kNT; ++n) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) out[n][r] *= grown;
-          out[n] = mfma16(xl[n], pf, mfma16(xh[n], pf, out[n]));
+          out[n] = mfma16(xh[n], pl, mfma16(xl[n], pf, mfma16(xh[n], pf, out[n])));
           write4(to, o_off[n] + ti * o_pitch, round4(out[n]));
         }
       }
@@ -546,7 +547,8 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
 #pragma unroll
           for (int r = 0; r < 4; ++r) score[u][r] *= p.scale * gam[r];
         }
-        const bf16x8 pf = round8(score[0], score[1]);
+        bf16x8 pf, pl;
+        split(score[0], score[1], pf, pl);
 #pragma unroll
         for (int n = 0; n < kNT; ++n) z[t][n] = zero4();
 #pragma unroll
@@ -558,7 +560,7 @@ __global__ __launch_bounds__(kWave, DK == 32 ? 2 : 1) void delta_solo_back_kerne
         for (int n = 0; n < kNT; ++n) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) z[t][n][r] *= keep[r];
-          z[t][n] = mfma16(pf, of[n], z[t][n]);
+          z[t][n] = mfma16(pl, of[n], mfma16(pf, of[n], z[t][n]));
         }
       }
       // dX

@@ -21,8 +21,8 @@ namespace {
 __host__ __device__ constexpr int frag_rows(int ti, int tk) { return ti < 2 ? ti : 2 + (ti - 2) * 2 + tk; }
 __host__ __device__ constexpr int frag_cols(int tj, int tk) { return tj < 2 ? tj * 2 + tk : 2 + tj; }
 
-// One wavefront makes the block of one chunk (n valid tokens; rows beyond count as k = q = 0, g = 0, beta = 0): -M in three parts (two for the
-// backward), P, and the factors of its tokens. COLS: transposed fragments, for the backward. rows, temp, scratch: LDS.
+// One wavefront makes the block of one chunk (n valid tokens; rows beyond count as k = q = 0, g = 0, beta = 0): -M and P in parts, and the
+// factors of its tokens. COLS: transposed fragments, for the backward. rows, temp, scratch: LDS.
 //
 // The 64 x 64 inverse: the four diagonal blocks of 16 by substitution, a column per lane, all four at once; the blocks below them by
 // products, M_21 = T_22 A_21 T_11 with T = I - M, first pairs of 16, then of 32.
@@ -53,9 +53,9 @@ __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, 
   wave_sync();
 
   f32x4 a_rows[10];  // A by rows, tile (ti, tj) at ti (ti + 1) / 2 + tj
-  u32x2 pf[6][2];
+  u32x2 pf[6][2], pl[6][2];
 #pragma unroll
-  for (int i = 0; i < 6; ++i) pf[i][0] = pf[i][1] = u32x2{0u, 0u};
+  for (int i = 0; i < 6; ++i) pf[i][0] = pf[i][1] = pl[i][0] = pl[i][1] = u32x2{0u, 0u};
 #pragma unroll
   for (int ti = 0; ti < 4; ++ti) {
     const int row = 16 * ti + l16;
@@ -103,6 +103,7 @@ __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, 
       const int f = COLS ? frag_cols(tj, ti / 2) : frag_rows(ti, tj / 2);
       const int half = COLS ? ti % 2 : tj % 2;
       pf[f][half] = round4(s);
+      pl[f][half] = rest4(s, pf[f][half]);
     }
   }
 
@@ -154,6 +155,8 @@ __device__ __forceinline__ void chunk_block(const DeltaParams& p, int b, int h, 
     *reinterpret_cast<bf16x8*>(block + kBlockMid + f * kFrag + lane * 16) = mid8;
     if (!COLS) *reinterpret_cast<bf16x8*>(block + kBlockLow + f * kFrag + lane * 16) = lo8;
     *reinterpret_cast<u32x4*>(block + kBlockP + f * kFrag + lane * 16) = u32x4{pf[f][0][0], pf[f][0][1], pf[f][1][0], pf[f][1][1]};
+    if (COLS || low_scores(DK))
+      *reinterpret_cast<u32x4*>(block + (COLS ? kBlockLow : kBlockPLow) + f * kFrag + lane * 16) = u32x4{pl[f][0][0], pl[f][0][1], pl[f][1][0], pl[f][1][1]};
   };
   if (!COLS) {
     const f32x4 m10r = mul_rows(t_rows[1], z10, zero4());
@@ -186,7 +189,7 @@ __global__ __launch_bounds__(kWave) void delta_blocks_kernel(const DeltaParams p
   const int64_t token0 = static_cast<int64_t>(chunk) * kChunk;
   const int64_t left = len - token0;
   if (left <= 0) return;
-  uint8_t* block = p.blocks + static_cast<int64_t>(blockIdx.x) * kBlockBytes;
+  uint8_t* block = p.blocks + static_cast<int64_t>(blockIdx.x) * block_bytes(DK);
   chunk_block<DK, COLS>(p, b, h, token0, left < kChunk ? static_cast<int>(left) : kChunk, block, rows, temp, scratch);
   float* out = reinterpret_cast<float*>(block + kBlockRows);
   for (int i = threadIdx.x; i < kRowFloats; i += kWave) out[i] = rows[i];
@@ -235,7 +238,7 @@ struct TeamLds {  // of every column tile: fragments of the first part, then of 
 template <int KB, int NT>
 struct TeamChunk {
   bf16x8 kf[KB], qf[KB];
-  bf16x8 mh[2], mm[2], ml[2], pf[2];
+  bf16x8 mh[2], mm[2], ml[2], pf[2], pl[2];
   f32x4 grown, keep;
   float grown_row, total;
   u32x2 x[NT];  // 4 NT columns of a token of V (backward: of dO), on their way into LDS
@@ -244,6 +247,7 @@ struct TeamChunk {
 template <int DK, int NT, bool COLS>
 struct Team {
   static constexpr int KB = DK / 32, KA = DK / 16, OWN = KA >= 4 ? KA / 4 : 1;  // OWN: state tiles of a wavefront
+  static constexpr int kBlockBytes = block_bytes(DK);
   typedef TeamChunk<KB, NT> Chunk;
   typedef TeamLds<DK, NT> L;
   const DeltaParams& p;
@@ -343,6 +347,7 @@ struct Team {
       c.mm[tk] = read8(block, frag_off[tk], kBlockMid);
       if (!COLS) c.ml[tk] = read8(block, frag_off[tk], kBlockLow);
       c.pf[tk] = read8(block, frag_off[tk], kBlockP);
+      if (COLS || low_scores(DK)) c.pl[tk] = read8(block, frag_off[tk], COLS ? kBlockLow : kBlockPLow);
     }
     at += COLS ? -1 : 1;
     k_at += k_step, q_at += q_step, x_at += x_step;
@@ -532,8 +537,10 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_kernel(const DeltaParams
 #pragma unroll
       for (int tk = 0; tk < 2; ++tk)
         if (tk <= wave / 2) {
-          out[n] = mfma16(get_frag(from, tk, lane), cur.pf[tk], out[n]);
+          const bf16x8 nh = get_frag(from, tk, lane);
+          out[n] = mfma16(nh, cur.pf[tk], out[n]);
           out2 = mfma16(get_frag(from + 2 * kFrag, tk, lane), cur.pf[tk], out2);
+          if (low_scores(DK)) out2 = mfma16(nh, cur.pl[tk], out2);
         }
 #pragma unroll
       for (int r = 0; r < 4; ++r) out[n][r] += out2[r];
@@ -637,7 +644,11 @@ __global__ __launch_bounds__(4 * kWave) void delta_team_back_kernel(const DeltaP
       }
 #pragma unroll
       for (int tk = 0; tk < 2; ++tk)
-        if (tk >= wave / 2) z3 = mfma16(cur.pf[tk], TK::join(m.values(tile_x, 32 * tk, n), m.values(tile_x, 32 * tk + 16, n)), z3);
+        if (tk >= wave / 2) {
+          const bf16x8 of = TK::join(m.values(tile_x, 32 * tk, n), m.values(tile_x, 32 * tk + 16, n));
+          z3 = mfma16(cur.pf[tk], of, z3);
+          z3 = mfma16(cur.pl[tk], of, z3);
+        }
       f32x4 w;
       const bf16x4 own = m.values(tile_x, 16 * wave, n);
 #pragma unroll

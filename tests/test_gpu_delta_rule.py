@@ -677,3 +677,24 @@ def test_gradients_are_nearly_as_near_as_their_type_holds(device, sizes, tokens)
     for N, a factor of every pair of tokens, would be more."""
     errors = _batch_errors(device, sizes, tokens, 0.3)
     assert all(errors[name] <= 1.5 for name in ("q", "k", "v", "beta")), errors
+
+
+@pytest.mark.parametrize("sizes,tokens", TRAINED + [((3, 8, 8, 32, 32), 300), ((2, 2, 2, 64, 64), 700), ((70, 1, 1, 128, 128), 200)])
+@pytest.mark.parametrize("slow", [1.0, 0.01])
+def test_outputs_and_gradients_of_values_are_rounded_once(device, sizes, tokens, slow):
+    """No further from 64 bits than the exact results rounded to bf16, by a fiftieth: the other roundings are pairs of bf16, 2^-18.4 of a factor at random, and fp32
+    sums, below 2^-7 of the rounding even where products cancel to a tenth. The outputs of heads of more than 64 key features have their scores rounded too,
+    parts of an output: at most 2^0.5 times as far, and a fiftieth."""
+    inputs = [t.to(device) for t in _draw(sizes[0], tokens, *sizes[1:], seed=31)]
+    inputs[3] *= slow
+    values = inputs[2].double().requires_grad_(True)
+    want, _, _ = delta_rule(*inputs[:2], values, *inputs[3:])
+    grad_out = torch.randn(want.shape, generator=torch.Generator().manual_seed(32)).bfloat16().to(device)
+    want_grad = torch.autograd.grad(want, values, grad_out.double())[0]
+    ours = inputs[2].requires_grad_(True)
+    out = gated_delta_rule(*inputs)
+    grad = torch.autograd.grad(out, ours, grad_out)[0]
+    for got, w, most in ((out, want, 2.0**0.5 if sizes[3] > 64 else 1.0), (grad, want_grad, 1.0)):
+        got, w = got.detach().double(), w.detach()
+        far = ((got - w).norm() / (w.bfloat16().double() - w).norm()).item()
+        assert far <= 1.02 * most, far
