@@ -4,12 +4,12 @@
 namespace taac {
 namespace {
 
-// Heads of at most 64 key features walk alone (delta_solo.hip) from more than two or three teams of 16 columns to a CU on: the chain of chunks
-// no longer counts then, and nothing is left in memory between two kernels. Wider heads always take the teams of delta_team.hip: their state
-// does not fit the registers of one wavefront. 2048 tokens, team : solo, by heads times groups of 16 columns:
-//   32 wide, forward 111 : 134 us at 512, 153 : 139 at 640;  with the backward 364 : 400, 467 : 442
-//   64 wide, forward 144 : 170 us at 768, 204 : 171 at 1024; with the backward 500 : 514, 671 : 557
-bool uses_teams(int64_t heads, int32_t dk, int32_t dv) { return dk > 64 || heads * ((dv + 15) / 16) <= (dk <= 32 ? 512 : 768); }
+// Heads of at most 64 key features walk alone (delta_solo.hip) from more than two teams of 16 columns to a CU on (two and a half of 64 wide ones):
+// the chain of chunks no longer counts then, and nothing is left in memory between two kernels. Wider heads always take the teams of
+// delta_team.hip: their state does not fit the registers of one wavefront. 2048 tokens, team : solo, by heads times groups of 16 columns:
+//   32 wide, forward 131 : 168 us at 384, 170 : 165 at 512, 217 : 168 at 640; with the backward 388 : 446, 463 : 468, 593 : 517
+//   64 wide, forward 182 : 205 us at 640, 204 : 205 at 768, 273 : 207 at 1024; with the backward 542 : 556, 626 : 583, 830 : 632
+bool uses_teams(int64_t heads, int32_t dk, int32_t dv) { return dk > 64 || heads * ((dv + 15) / 16) <= (dk <= 32 ? 512 : 640); }
 
 int64_t workspace_of(int64_t heads, int32_t T, int32_t dk, int32_t dv) {
   return uses_teams(heads, dk, dv) ? heads * ((static_cast<int64_t>(T) + kChunk - 1) / kChunk) * block_bytes(dk) : 0;
