@@ -10,13 +10,13 @@
 // where what a pair (i, j) of tokens adds to a row it takes from a column.
 //
 // All in one workgroup per chunk and key head: the tiles of K, Q, dO, dX, N, S and dS' meet in LDS, where each is read by rows and by columns.
-// 512 samples x 4 heads x 512 tokens, 64 wide: 355 us, 3.4 TB/s; two workgroups to a CU by their registers, whose wavefronts wait for 46 % of
-// their time and issue vector instructions for 25 %. 128 wide, where the tiles leave room for one: 18 us per chunk and head, 2.4 TB/s; two
+// 512 samples x 4 heads of up to 512 tokens, 64 wide: 389 us in a trace, 3.4 TB/s; two workgroups to a CU by their registers, whose wavefronts wait
+// for 41 % of their time and issue vector instructions for 27 %. 128 wide, where the tiles leave room for one: 20 us per chunk and head, 2.0 TB/s; two
 // sets of four wavefronts on one chunk (rows and columns at once) took 3 % longer.
 //
 // S, dS' and dX are read back in bf16, one rounding each: they only meet the outputs, of which they are parts (0.2e-3 to 1.0e-3 of a gradient, whose
-// own rounding is 1.7e-3; together 1.8e-3 to 2.4e-3). N, which every pair of tokens has as a factor, is kept in two parts: its one rounding alone cost
-// 1.7e-3. Key heads that serve several value heads sum their gradients in registers, in the order of the heads.
+// own rounding is 1.7e-3; together 1.7e-3 to 2.2e-3, where nothing is forgotten over hundreds of tokens up to 2.5e-3 and 3.0e-3 for the decays). Two parts
+// of S and dS' too would be a fifth more bytes. N, which every pair of tokens has as a factor, is kept in two parts: its one rounding alone cost 1.7e-3. Key heads that serve several value heads sum their gradients in registers, in the order of the heads.
 #include "delta.h"
 
 namespace taac {

@@ -6,10 +6,10 @@
 // diagonal blocks of 16 are still solved at once, a column per lane, but only one block below the diagonal is left per chunk
 // instead of six per 64 tokens. Scores are made where they are used.
 //
-// Bound by instruction issue. 1024 samples x 8 heads of up to 512 tokens (276 at the mean), 32 wide, forward: 218 us, 3.4 TB/s; two wavefronts per
-// SIMD issue in 85 % of the cycles, vector instructions in 59 %, nearly half of those for the hi and lo of fp32 operands. 512 x 4 heads of
-// up to 512, 64 wide: 198 us with the states and misses of training, 174 us backward; there one wavefront per SIMD fills the registers (two
-// spill and take 10 % longer), and 40 % of its time goes to waits that no other wavefront covers.
+// Bound by instruction issue. 1024 samples x 8 heads of up to 512 tokens (276 at the mean), 32 wide, forward: 246 us in a trace, 3.0 TB/s; two
+// wavefronts per SIMD issue in 73 % of the cycles, vector instructions in 55 %, many of those to take fp32 operands apart; the matrix units are busy
+// for 23 %. 512 x 4 heads of up to 512, 64 wide: 244 us with the states and misses of training, 197 us backward; there one wavefront per SIMD fills
+// the registers (two spill and take 10 % longer), which issues in half of the cycles and waits in a quarter, covered by no other wavefront.
 #include "delta.h"
 
 namespace taac {

@@ -5,11 +5,12 @@
 // run of memory, and the whole state stays in registers between its load and its store. A token needs one round of sums over the
 // key rows, of k S and q S and q . k at once, since o = scale (S + k u^T)^T q = scale (S^T q + (k . q) u). All arithmetic is fp32.
 //
-// 1024 samples of 8 heads, 64 x 64, out of 1500 slots, one token: 63 us, 4.3 TB/s (82 us with the reads of the search for
-// samples of the same slot one after the other, 90 us with the token's inputs requested behind it).
+// 1024 samples of 8 heads, 64 x 64, out of 1500 slots, one token: 58 us in a trace, 4.7 TB/s (with the reads of the search for samples of the
+// same slot one after the other 19 us more, with the token's inputs requested behind it 27).
 //
 // Samples that name the same slot are one sequence: their tokens are applied in the order of the batch, by the workgroup of the
-// first of them. A slot outside the pool (padding) reads and writes no state and gives zeros.
+// first of them. A slot outside the pool (padding) reads and writes no state and gives zeros. To find samples of the same slot every workgroup
+// reads all of them: 8 heads of 32 x 32 take 47 us for 4096 samples without slots and 104 with them, for 16384 samples 205 and 891.
 #include "delta.h"
 
 namespace taac {
@@ -235,8 +236,8 @@ void launch_step(const StepParams& p, hipStream_t s) {
 template <typename T>
 void dispatch_step(const StepParams& p, hipStream_t s) {
   // One wavefront while a lane's share is at most four rows of four columns, two while it is at most eight, else four: more wavefronts wait for
-  // each other, fewer keep less in flight. 4096 samples of 8 heads, 32 x 32: 89 us with one, 163 with four; 1024 of 64 x 64: 51 with
-  // two, 55 with four or one; 1024 of 64 x 32: 32 with two, 45 with four.
+  // each other, fewer keep less in flight. Samples of 8 heads, with slots (without), 4096 of 32 x 32: 104 (47) us with one, 170 (119) with four;
+  // 1024 of 64 x 64: 55 (44) with two, 57 (45) with one, 60 (49) with four; 1024 of 64 x 32: 32 (26) with two, 29 (24) with one, 43 (38) with four.
 #define TAAC_STEP_ROWS(NVP)                                                                                   \
   {                                                                                                           \
     constexpr int ROWS = kWave / NVP;                                                                         \

@@ -8,9 +8,9 @@
 // whose results meet in LDS as operand fragments. Everything a chunk reads from memory is requested one chunk ahead, a third beside
 // each stage.
 //
-// 2 samples x 16 heads x 8192 tokens, 128 wide: 36 us for the blocks (145 MB, 4.0 TB/s) and 187 us for 128 steps of 1.5 us (305 us with masked
-// reads in one run at a step's start). A step is a chain of eight dependent matrix instructions and three exchanges through LDS, among
-// 310 instructions that every wavefront issues: bound by that chain, the matrix units are busy for a seventh of it.
+// 2 samples x 16 heads x 8192 tokens, 128 wide: 41 us for the blocks (170 MB, 4.1 TB/s) and 239 us for 128 steps of 1.9 us (masked reads in one
+// run at a step's start took 1.6 times as long). A step is a chain of eighteen dependent matrix instructions and three exchanges through LDS, among
+// 370 instructions that every wavefront issues: bound by that chain, the matrix units are busy for a fifth of it, and a wavefront waits for 39 %.
 #include "delta.h"
 
 namespace taac {
