@@ -175,8 +175,12 @@ def gated_delta_rule(
 
     ``initial_state`` (batch, heads, key width, value width) float32 is the state in front of the first token, ``return_state``
     returns ``(out, state behind the last)``, which :func:`gated_delta_rule_step` continues. The state is kept in float32
-    and everything that reaches it enters its products with 24 bits; the outputs' scores are rounded to bfloat16 once. Differentiable in q, k, v and the gates; the states are not, so that an ``initial_state`` that
-    requires grad, and ``return_state`` where an input does, are refused."""
+    and everything that reaches it enters its products with 24 bits. Outputs and the gradient of v are rounded once, at the end
+    (the outputs of keys wider than 64 also where the scores meet the values). The gradients of q, k and the gates, float32 gates
+    among them, have the bfloat16 rounding of the states that the forward keeps in them, 1e-3 to 2.5e-3.
+
+    Differentiable in q, k, v and the gates; the states are not, so that an ``initial_state`` that requires grad, and
+    ``return_state`` where an input does, are refused."""
     name = "gated_delta_rule"
     _check_shapes(name, q, k, v, log_decay, beta)
     require_cuda_tensors(f"hip {name}", q, k, v, log_decay, beta, initial_state)
