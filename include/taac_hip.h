@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define TAAC_ABI_VERSION 11
+#define TAAC_ABI_VERSION 12
 
 enum taac_status {
   TAAC_OK = 0,
@@ -651,6 +651,67 @@ int taac_delta_rule_step(const void* q, const void* k, const void* v, const void
                          int32_t T, int32_t dk, int32_t dv, const int64_t q_strides[3], const int64_t k_strides[3],
                          const int64_t v_strides[3], const int64_t o_strides[3], const int64_t decay_strides[3],
                          const int64_t beta_strides[3], float scale, int dtype, int gate_dtype, void* stream);
+
+/*
+ * RMSNorm of every head of the queries and keys and the rotation by their positions, one pass over both.
+ * q: logical (B, H, T, d), k: (B, key_heads, T, d) of dtype (fp32, bf16 or fp16), d at most 512; *_strides: ELEMENT strides of (batch, head,
+ * token), the features of a row contiguous. With weights [d] of dtype (both or neither) every row becomes x rsqrt(mean(x^2) + eps) weight; then the
+ * pairs of the first `rotary` features (even, at most d; 0: none) turn by (c, s) = table[position][pair]: (a, b) -> (a c - b s, a s + b c), pairs (2i, 2i + 1) if
+ * interleaved, else (i, i + rotary / 2). table: fp32 [places, rotary / 2, 2], or NULL with rotary 0. positions: int32 or int64 (positions_int64) with element strides
+ * of (sample, token), the token's number added where add_token; or NULL: the token's number. A position outside the table gives NaN in the
+ * rotated features. fp32 arithmetic, one rounding. The outputs may be the inputs (with their strides).
+ * taac_head_norm_rope_bwd: grad_q, grad_k and, with weights, grad_qw and grad_kw [d], for the gradients grad_qo, grad_ko of the outputs; q and k are not
+ * read without weights (any valid pointer). workspace: taac_head_norm_rope_bwd_workspace_floats floats with weights, else NULL and 0. Every sum has a
+ * fixed order.
+ * Replaces: the rotary passes of BFTSAttention (experiments/tokenformer/model.py:165-192) for per-head norms, shared key heads and positions of any start.
+ */
+int taac_head_norm_rope_fwd(const void* q, const void* k, void* q_out, void* k_out, int32_t B, int32_t H, int32_t key_heads, int32_t T, int32_t d,
+                            int32_t rotary, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t qo_strides[3],
+                            const int64_t ko_strides[3], const void* q_weight, const void* k_weight, float eps, const float* table, int64_t places,
+                            const void* positions, int positions_int64, const int64_t position_strides[2], int add_token, int interleaved, int dtype,
+                            void* stream);
+int64_t taac_head_norm_rope_bwd_workspace_floats(int32_t B, int32_t H, int32_t key_heads, int32_t T, int32_t d);
+int taac_head_norm_rope_bwd(const void* q, const void* k, const void* grad_qo, const void* grad_ko, void* grad_q, void* grad_k, void* grad_qw,
+                            void* grad_kw, float* workspace, int64_t workspace_floats, int32_t B, int32_t H, int32_t key_heads, int32_t T, int32_t d,
+                            int32_t rotary, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t gqo_strides[3],
+                            const int64_t gko_strides[3], const int64_t gq_strides[3], const int64_t gk_strides[3], const void* q_weight,
+                            const void* k_weight, float eps, const float* table, int64_t places, const void* positions, int positions_int64,
+                            const int64_t position_strides[2], int add_token, int interleaved, int dtype, void* stream);
+
+/*
+ * A cache of keys and values in a pool of pages: taac_kv_cache_bytes(pages, ..) bytes (-1: sizes that are not covered), 16-byte aligned, filled with zeros
+ * once by the caller and written by taac_kv_cache_write only. heads key heads of d = 32, 64 or 128 features in `bits` = 4 (e2m1) or 8 (e4m3), pages of page_tokens
+ * tokens (a power of two, 16 to 65536). 32 consecutive features share a scale 2^e, the least with max |x| < 7 2^e (464 2^e), within 2^-117 .. 2^125
+ * (2^119); codes are the nearest of x 2^-e, ties to even.
+ * table: [B, table_pages] int32 or int64 (table_int64), rows table_stride elements apart: the pages of a sample's positions in order. A page outside
+ * the pool, or a position behind the table, is no place: not written, read as zeros, not attended to.
+ * write: token t of sample b, k and v logical (B, heads, T, d), goes to position starts[b] + t (starts int32, int64 (starts_int64) or NULL: 0), for t <
+ * lengths[b] (NULL: T). A token of which k or v has a NaN or an infinity in a head reads back as NaN there. Two tokens of one call must not share a place.
+ * read: the other way round, zeros for t >= lengths[b]. ELEMENT strides of (batch, head, token), multiples of 16 bytes; 16-byte aligned tensors of fp32, bf16
+ * or fp16.
+ */
+int64_t taac_kv_cache_bytes(int64_t pages, int32_t heads, int32_t page_tokens, int32_t d, int bits);
+int taac_kv_cache_write(void* cache, int64_t pages, int32_t heads, int32_t page_tokens, int32_t d, int bits, const void* table, int table_int64,
+                        int64_t table_stride, int32_t table_pages, const void* k, const void* v, const void* starts, int starts_int64,
+                        const int32_t* lengths, int32_t B, int32_t T, const int64_t k_strides[3], const int64_t v_strides[3], int dtype, void* stream);
+int taac_kv_cache_read(const void* cache, int64_t pages, int32_t heads, int32_t page_tokens, int32_t d, int bits, const void* table, int table_int64,
+                       int64_t table_stride, int32_t table_pages, void* k, void* v, const void* starts, int starts_int64, const int32_t* lengths,
+                       int32_t B, int32_t T, const int64_t k_strides[3], const int64_t v_strides[3], int dtype, void* stream);
+
+/*
+ * Attention of new tokens over such a cache: o = softmax(scale q k^T) v over the positions that a query sees. q, o: logical (B, H, T, d), bf16 or fp16, H a
+ * multiple of the cache's heads (query head h uses key head h / (H / heads)); ELEMENT strides of (batch, head, token), those of q multiples of 8, those
+ * of o of 4; q 16-byte aligned, o 8-byte. lengths: int32 [B], the sample's cached tokens, its queries among them; query_lengths: int32 [B] or NULL: T.
+ * With n = min(query_lengths[b], T) query t < n stands at position lengths[b] - n + t and sees the positions up to its own, the last `window` of them if window > 0.
+ * Other queries, and those that see nothing, get zeros. At most 2^30 positions to a table. workspace: taac_cached_attention_workspace_bytes bytes for
+ * table_tokens = table_pages * page_tokens (0 if the pool has no pages), 16-byte aligned (0: none). Calls in flight together must not share one.
+ */
+int64_t taac_cached_attention_workspace_bytes(int32_t B, int32_t H, int32_t heads, int32_t T, int32_t d, int64_t table_tokens);
+int taac_cached_attention_fwd(const void* q, void* o, const void* cache, int64_t pages, int32_t heads, int32_t page_tokens, int32_t d, int bits,
+                              const void* table, int table_int64, int64_t table_stride, int32_t table_pages, const int32_t* lengths,
+                              const int32_t* query_lengths, int32_t window, float scale, void* workspace, int64_t workspace_bytes, int32_t B, int32_t H,
+                              int32_t T, const int64_t q_strides[3], const int64_t o_strides[3], int dtype, void* stream);
+
 
 /*
  * Readout of the token backbone, one kernel:

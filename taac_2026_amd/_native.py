@@ -26,7 +26,7 @@ ATTN_CAUSAL, ATTN_REGISTER_STAGING = 1, 2
 BACKBONE_DENSE_TOKENS, BACKBONE_SPLIT_OUT_FFN, BACKBONE_FP8, BACKBONE_ROW_MAJOR_QKV = 1, 2, 4, 8
 FOLDED_NORM, FOLDED_ACTIVATION = 1, 2
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 _DTYPE_CODES = {torch.float32: TAAC_F32, torch.bfloat16: TAAC_BF16, torch.float16: TAAC_F16}
 
@@ -277,6 +277,34 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_void_p] * 6 + [c_int64, c_void_p, c_int, c_void_p, c_void_p] + [c_int32] * 6 + [ctypes.POINTER(c_int64)] * 6
         + [c_float, c_int, c_int, c_void_p],
+    ),
+    "taac_head_norm_rope_fwd": (
+        c_int,
+        [c_void_p] * 4 + [c_int32] * 6 + [ctypes.POINTER(c_int64)] * 4 + [c_void_p] * 2 + [c_float, c_void_p, c_int64, c_void_p, c_int]
+        + [ctypes.POINTER(c_int64), c_int, c_int, c_int, c_void_p],
+    ),
+    "taac_head_norm_rope_bwd_workspace_floats": (c_int64, [c_int32] * 5),
+    "taac_head_norm_rope_bwd": (
+        c_int,
+        [c_void_p] * 9 + [c_int64] + [c_int32] * 6 + [ctypes.POINTER(c_int64)] * 6 + [c_void_p] * 2 + [c_float, c_void_p, c_int64, c_void_p, c_int]
+        + [ctypes.POINTER(c_int64), c_int, c_int, c_int, c_void_p],
+    ),
+    "taac_kv_cache_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int]),
+    "taac_kv_cache_write": (
+        c_int,
+        [c_void_p, c_int64, c_int32, c_int32, c_int32, c_int, c_void_p, c_int, c_int64, c_int32] + [c_void_p] * 3 + [c_int, c_void_p, c_int32, c_int32]
+        + [ctypes.POINTER(c_int64)] * 2 + [c_int, c_void_p],
+    ),
+    "taac_kv_cache_read": (
+        c_int,
+        [c_void_p, c_int64, c_int32, c_int32, c_int32, c_int, c_void_p, c_int, c_int64, c_int32] + [c_void_p] * 3 + [c_int, c_void_p, c_int32, c_int32]
+        + [ctypes.POINTER(c_int64)] * 2 + [c_int, c_void_p],
+    ),
+    "taac_cached_attention_workspace_bytes": (c_int64, [c_int32] * 5 + [c_int64]),
+    "taac_cached_attention_fwd": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int, c_void_p, c_int, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_float]
+        + [c_void_p, c_int64, c_int32, c_int32, c_int32] + [ctypes.POINTER(c_int64)] * 2 + [c_int, c_void_p],
     ),
     "taac_embedding_bag_mean_fwd": (
         c_int,
