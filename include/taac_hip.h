@@ -706,7 +706,7 @@ int taac_kv_cache_read(const void* cache, int64_t pages, int32_t heads, int32_t 
  * Other queries, and those that see nothing, get zeros. At most 2^30 positions to a table. workspace: taac_cached_attention_workspace_bytes bytes for
  * table_tokens = table_pages * page_tokens (0 if the pool has no pages), 16-byte aligned (0: none). Calls in flight together must not share one.
  */
-int64_t taac_cached_attention_workspace_bytes(int32_t B, int32_t H, int32_t heads, int32_t T, int32_t d, int64_t table_tokens);
+int64_t taac_cached_attention_workspace_bytes(int32_t B, int32_t H, int32_t heads, int32_t T, int32_t d, int bits, int64_t table_tokens);
 int taac_cached_attention_fwd(const void* q, void* o, const void* cache, int64_t pages, int32_t heads, int32_t page_tokens, int32_t d, int bits,
                               const void* table, int table_int64, int64_t table_stride, int32_t table_pages, const int32_t* lengths,
                               const int32_t* query_lengths, int32_t window, float scale, void* workspace, int64_t workspace_bytes, int32_t B, int32_t H,

@@ -300,7 +300,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_void_p, c_int64, c_int32, c_int32, c_int32, c_int, c_void_p, c_int, c_int64, c_int32] + [c_void_p] * 3 + [c_int, c_void_p, c_int32, c_int32]
         + [ctypes.POINTER(c_int64)] * 2 + [c_int, c_void_p],
     ),
-    "taac_cached_attention_workspace_bytes": (c_int64, [c_int32] * 5 + [c_int64]),
+    "taac_cached_attention_workspace_bytes": (c_int64, [c_int32] * 5 + [c_int, c_int64]),
     "taac_cached_attention_fwd": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int, c_void_p, c_int, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_float]

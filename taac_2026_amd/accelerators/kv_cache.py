@@ -174,8 +174,8 @@ def kv_cache_read(
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(batch: int, heads: int, key_heads: int, tokens: int, width: int, table_tokens: int) -> int:
-    return _native.load_library().taac_cached_attention_workspace_bytes(batch, heads, key_heads, tokens, width, table_tokens)
+def _workspace_bytes(batch: int, heads: int, key_heads: int, tokens: int, width: int, bits: int, table_tokens: int) -> int:
+    return _native.load_library().taac_cached_attention_workspace_bytes(batch, heads, key_heads, tokens, width, bits, table_tokens)
 
 
 def cached_attention(
@@ -217,7 +217,7 @@ def cached_attention(
         raise RuntimeError(f"hip {name} does not support dtype {q.dtype}")
     q = _in_place(q, 2)
     out = token_major(batch, heads, tokens, width, q)
-    bytes_needed = _workspace_bytes(batch, heads, cache.heads, tokens, width, pages.shape[1] * cache.page_tokens if cache.pages > 0 else 0)
+    bytes_needed = _workspace_bytes(batch, heads, cache.heads, tokens, width, cache.bits, pages.shape[1] * cache.page_tokens if cache.pages > 0 else 0)
     workspace = q.new_empty(bytes_needed, dtype=torch.uint8) if bytes_needed > 0 else None
     with _native.on_device(q.device):
         status = _native.load_library().taac_cached_attention_fwd(

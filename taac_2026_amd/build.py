@@ -19,7 +19,7 @@ CSRC_DIR = PACKAGE_DIR / "csrc"
 BUILD_DIR = PACKAGE_DIR / "csrc" / "build"
 LIBRARY_PATH = PACKAGE_DIR / "libtaac_hip.so"
 
-SOURCES = ("runtime.hip", "norm.hip", "residual_norm.hip", "attention.hip", "linear.hip", "ffn.hip", "ffn_small.hip", "fp8.hip", "fp8_ts.hip", "ffn_fp8.hip", "backbone.hip", "embedding.hip", "attention_bwd.hip", "readout.hip", "delta_rule.hip", "delta_grads.hip", "delta_team.hip", "delta_solo.hip", "delta_step.hip", "head_rope.hip", "kv_cache.hip", "cached_attention.hip", "linear_bwd.hip", "ffn_bwd.hip", "train_dense.hip", "train.hip")
+SOURCES = ("runtime.hip", "norm.hip", "residual_norm.hip", "attention.hip", "linear.hip", "ffn.hip", "ffn_small.hip", "fp8.hip", "fp8_ts.hip", "ffn_fp8.hip", "backbone.hip", "embedding.hip", "attention_bwd.hip", "readout.hip", "delta_rule.hip", "delta_grads.hip", "delta_team.hip", "delta_solo.hip", "delta_step.hip", "head_rope.hip", "kv_cache.hip", "cached_attention.hip", "cached_attention_4.hip", "cached_attention_8.hip", "linear_bwd.hip", "ffn_bwd.hip", "train_dense.hip", "train.hip")
 
 # -packed-fp32-ops: keep the compiler from forming packed-fp32 VALU instructions from scalar float code.
 HIPCC_FLAGS = (
@@ -40,7 +40,8 @@ EXTRA_FLAGS = {
     "attention.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1"),
     "attention_bwd.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1"),
     "ffn_small.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1"),
-    "cached_attention.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1"),
+    "cached_attention_4.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1"),
+    "cached_attention_8.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1"),
     "delta_grads.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1"),
     "delta_solo.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1"),
     "delta_team.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1"),

@@ -1,0 +1,8 @@
+// Attention over caches of 8 bits.
+#include "cached_attention.h"
+
+namespace taac {
+
+void attend_8(const AttendParams& p, int d, bool f16, int rows, bool alone, uint32_t groups, hipStream_t s) { dispatch_attend<8>(p, d, f16, rows, alone, groups, s); }
+
+}  // namespace taac

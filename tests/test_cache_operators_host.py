@@ -214,8 +214,8 @@ def test_cache_entry_points_check_on_the_host():
     assert attend(table_pages=1 << 27) == unsupported and b"2^30" in library.taac_last_error()
     assert attend(H=1 << 21, T=32) == unsupported and attend(B=1 << 23) == unsupported
     assert attend(B=0) == ok and attend(T=0) == ok
-    need = library.taac_cached_attention_workspace_bytes(1, 4, 2, 1, 32, 1 << 16)
+    need = library.taac_cached_attention_workspace_bytes(1, 4, 2, 1, 32, 4, 1 << 16)
     assert need > 0 and attend(table_pages=1 << 12, ws=fake, bytes=need - 1) == invalid and b"workspace" in library.taac_last_error()
     assert attend(table_pages=1 << 12, ws=odd, bytes=need) == invalid
-    assert library.taac_cached_attention_workspace_bytes(1024, 8, 8, 1, 32, 512) == 0  # enough samples to fill the card
-    assert library.taac_cached_attention_workspace_bytes(1, 3, 2, 1, 32, 512) == -1
+    assert library.taac_cached_attention_workspace_bytes(1024, 8, 8, 1, 32, 4, 512) == 0  # enough samples to fill the card
+    assert library.taac_cached_attention_workspace_bytes(1, 3, 2, 1, 32, 4, 512) == -1 and library.taac_cached_attention_workspace_bytes(1, 2, 2, 1, 32, 6, 512) == -1
