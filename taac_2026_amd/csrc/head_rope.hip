@@ -7,14 +7,18 @@
 //
 // Bound by HBM: a row is read once and written once (backward: two reads and a write) and there are some ten operations to a feature. A lane holds
 // four pairs of a row, i.e. two runs of four features: with the pairs half a head apart they are the two runs that belong together, so that the
-// rotation never leaves the lane, and the sum of squares crosses d / 8 lanes. The rows of a token's heads lie next to each other in lanes, and share
-// their row of the table through the caches. All arithmetic is fp32, rounded once at the end.
+// rotation never leaves the lane, and the sum of squares crosses d / 8 lanes. A wavefront's rows are heads of the same token, next to each other in memory and
+// with one row of the table between them, or of a few tokens where a token has fewer heads. A lane keeps its head and walks the tokens: what a row costs besides
+// its features is a few additions. All arithmetic is fp32, rounded once at the end.
 #include "norm_rows.h"
 
 namespace taac {
 namespace {
 
 constexpr int kMaxHeadWidth = 512;  // 64 lanes of 8 features
+constexpr int kMaxHeads = 1 << 14;   // a wavefront each, at most, in the second dimension of a grid
+
+constexpr int kForwardBlocks = 4096;  // 16 wavefronts to a SIMD; twice or four times as many, or half, are within what runs differ by
 
 struct RopeParams {
   const void* x[2];       // queries, keys
@@ -26,20 +30,41 @@ struct RopeParams {
   const float* table;     // [places][rotary / 2][2] or null
   const void* positions;  // null: the position is the token's number
   int64_t ps[2];
-  int64_t places, rows;   // rows of queries and keys together
-  int32_t H[2], T, d, rotary;
+  int64_t places;
+  int32_t H[2], B, T, d, rotary;
   int32_t pos_int64, add_token;
-  float eps;
+  float eps, inv_d;
 };
 
-// The four pairs of lane s of a row. In vectors: two runs of four features at `at[0]` and `at[1]`; else the pairs s, s + L, ..
-template <int L, bool VEC, bool INTER>
+// How a lane reaches its features.
+//   kSingles  one by one: the pairs s, s + L, ..
+//   kRuns     two runs of four
+//   kWide     eight neighbours of 16 bits in one access. Where pairs lie half a head apart two lanes, half of the turned ones apart, exchange four features for four.
+// Eight bytes to a lane leave each access half of every line: 1024 x 512 tokens of 16 heads of 32 features take 233 us in runs, 209 wide.
+enum { kSingles, kRuns, kWide };
+
+// The four pairs of lane s of a row.
+template <int L, int VEC, bool INTER>
 struct Lane {
-  int at[VEC ? 2 : 8];  // features; -1: there is none
+  int at[VEC != kSingles ? 2 : 8];  // features; -1: there is none
   int pair[4];          // of the table, -1: not turned
+  int apart;            // kWide: lanes between the two that exchange
+  bool gives_low;       // and which of its features this one gives
+  // the lane whose runs this one has after an exchange
+  __device__ __forceinline__ int run_lane(int s) const { return INTER || pair[0] < 0 ? s : pair[0] / 4; }
   __device__ __forceinline__ Lane(int s, int d, int rotary) {
     const int half = rotary / 2;
-    if constexpr (VEC) {
+    if constexpr (VEC == kWide) {
+      const bool turned = 8 * s < rotary, there = 8 * s < d;
+      apart = rotary / 16;
+      gives_low = turned && s >= apart;
+      at[0] = there ? 8 * s : -1;
+      at[1] = !INTER && turned ? 1 : 0;  // exchanges
+      // the first of the two has the first four of its pairs, the second the last four
+      const int first = INTER ? 4 * s : gives_low ? 8 * (s - apart) + 4 : 8 * s;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pair[e] = turned ? first + e : -1;
+    } else if constexpr (VEC == kRuns) {
       const bool turned = 8 * s < rotary, there = 8 * s < d;
       at[0] = !there ? -1 : (turned && !INTER ? 4 * s : 8 * s);
       at[1] = !there ? -1 : (turned && !INTER ? half + 4 * s : 8 * s + 4);
@@ -74,33 +99,73 @@ struct Run<f16_t> {
   typedef f16x4 type;
 };
 
-// v[2 e], v[2 e + 1]: pair e.
-template <typename T, int L, bool VEC, bool INTER>
-__device__ __forceinline__ void load_row(const T* row, const Lane<L, VEC, INTER>& lane, float (&v)[8]) {
-  if constexpr (VEC) {
-    typename Run<T>::type a = {}, b = {};
-    if (lane.at[0] >= 0) {
-      a = *reinterpret_cast<const typename Run<T>::type*>(row + lane.at[0]);
-      b = *reinterpret_cast<const typename Run<T>::type*>(row + lane.at[1]);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[INTER ? e : 2 * e] = static_cast<float>(a[e]);
-      v[INTER ? 4 + e : 2 * e + 1] = static_cast<float>(b[e]);
-    }
+// Between the lanes s and s + apart, which hold features 8 s .. and half + 8 s ..: the one's last four for the other's first four, or back. Every lane of the
+// wavefront that is on its way takes part; those that are not turned keep theirs.
+template <int L, int VEC, bool INTER, typename V>
+__device__ __forceinline__ void exchange(const Lane<L, VEC, INTER>& lane, V& first, V& second) {
+  const u32x2 mine = __builtin_bit_cast(u32x2, lane.gives_low ? first : second);
+  u32x2 other;
+  if (L == 4 && lane.apart == 2) {  // heads of 32 features: within a quad
+    other[0] = __builtin_amdgcn_mov_dpp(mine[0], 0x4e, 0xf, 0xf, false), other[1] = __builtin_amdgcn_mov_dpp(mine[1], 0x4e, 0xf, 0xf, false);
   } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = lane.at[i] >= 0 ? static_cast<float>(row[lane.at[i]]) : 0.f;
+    other[0] = __shfl_xor(mine[0], lane.apart, kWave), other[1] = __shfl_xor(mine[1], lane.apart, kWave);
   }
+  if (lane.at[1] == 0) return;
+  if (lane.gives_low) first = __builtin_bit_cast(V, other);
+  else second = __builtin_bit_cast(V, other);
 }
-template <typename T, int L, bool VEC, bool INTER>
+
+// A lane's features of a row as they arrive, converted when they are needed: the next row's are on their way meanwhile.
+template <typename T, int L, int VEC, bool INTER>
+struct Raw {
+  typename Run<T>::type run[2];
+  T one[8];
+  __device__ __forceinline__ void load(const T* row, const Lane<L, VEC, INTER>& lane) {
+    if constexpr (VEC == kWide) {
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (lane.at[0] >= 0) v = *reinterpret_cast<const u32x4*>(row + lane.at[0]);
+      run[0] = __builtin_bit_cast(typename Run<T>::type, (u32x2{v[0], v[1]})), run[1] = __builtin_bit_cast(typename Run<T>::type, (u32x2{v[2], v[3]}));
+    } else if constexpr (VEC == kRuns) {
+      run[0] = typename Run<T>::type{}, run[1] = typename Run<T>::type{};
+      if (lane.at[0] >= 0) {
+        run[0] = *reinterpret_cast<const typename Run<T>::type*>(row + lane.at[0]);
+        run[1] = *reinterpret_cast<const typename Run<T>::type*>(row + lane.at[1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) one[i] = lane.at[i] >= 0 ? row[lane.at[i]] : static_cast<T>(0.f);
+    }
+  }
+  // v[2 e], v[2 e + 1]: pair e
+  __device__ __forceinline__ void get(const Lane<L, VEC, INTER>& lane, float (&v)[8]) const {
+    if constexpr (VEC != kSingles) {
+      typename Run<T>::type first = run[0], second = run[1];
+      if constexpr (VEC == kWide && !INTER) exchange(lane, first, second);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[INTER ? e : 2 * e] = static_cast<float>(first[e]);
+        v[INTER ? 4 + e : 2 * e + 1] = static_cast<float>(second[e]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(one[i]);
+    }
+  }
+};
+template <typename T, int L, int VEC, bool INTER>
 __device__ __forceinline__ void store_row(T* row, const Lane<L, VEC, INTER>& lane, const float (&v)[8]) {
-  if constexpr (VEC) {
+  if constexpr (VEC != kSingles) {
     typename Run<T>::type a, b;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       a[e] = static_cast<T>(v[INTER ? e : 2 * e]);
       b[e] = static_cast<T>(v[INTER ? 4 + e : 2 * e + 1]);
+    }
+    if constexpr (VEC == kWide) {
+      if constexpr (!INTER) exchange(lane, a, b);
+      const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
+      if (lane.at[0] >= 0) *reinterpret_cast<u32x4*>(row + lane.at[0]) = u32x4{x[0], x[1], y[0], y[1]};
+      return;
     }
     if (lane.at[0] >= 0) {
       *reinterpret_cast<typename Run<T>::type*>(row + lane.at[0]) = a;
@@ -113,26 +178,32 @@ __device__ __forceinline__ void store_row(T* row, const Lane<L, VEC, INTER>& lan
   }
 }
 
-// Where a row is: which of queries and keys, and its sample, token and head.
-struct Place {
-  int which, h, t;
-  int64_t b;
-  __device__ __forceinline__ Place(const RopeParams& p, int64_t row) {
-    const uint32_t heads = p.H[0] + p.H[1];
-    int64_t token;
-    uint32_t head;
-    if (p.rows < (int64_t{1} << 32)) {  // the same branch for all: 32-bit divisions are a third of the instructions
-      token = static_cast<uint32_t>(row) / heads;
-      head = static_cast<uint32_t>(row) - static_cast<uint32_t>(token) * heads;
-      b = static_cast<uint32_t>(token) / static_cast<uint32_t>(p.T);
+// The tokens that a lane's row slot walks: `head` heads of a token side by side in a wavefront, tokens a constant distance apart.
+struct Walk {
+  int which, h, t, step_t;
+  int64_t b, step_b;
+  bool there;
+  // slots: rows of a wavefront; chunk: of a token's heads, where they need several wavefronts
+  __device__ __forceinline__ Walk(const RopeParams& p, int slots, int slot) {
+    const int heads = p.H[0] + p.H[1], side = heads < slots ? heads : slots;  // heads of a token in a wavefront
+    const int at_once = slots / side;                                         // tokens of a wavefront
+    const int head = static_cast<int>(blockIdx.y) * slots + slot % side, of = slot / side;
+    there = of < at_once && head < heads;
+    which = head >= p.H[0];
+    h = head - (which ? p.H[0] : 0);
+    const int64_t wave = static_cast<int64_t>(blockIdx.x) * (kBlock / kWave) + threadIdx.x / kWave, token = wave * at_once + of;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kBlock / kWave) * at_once;
+    if (token < 0x7fffffff && step < 0x7fffffff) {  // for all lanes alike but behind two billion tokens: a fifth of the instructions
+      const uint32_t T = p.T;
+      b = static_cast<uint32_t>(token) / T, step_b = static_cast<uint32_t>(step) / T;
     } else {
-      token = row / heads;
-      head = static_cast<uint32_t>(row - token * heads);
-      b = token / p.T;
+      b = token / p.T, step_b = step / p.T;
     }
-    t = static_cast<int>(token - b * p.T);
-    which = head >= static_cast<uint32_t>(p.H[0]);
-    h = static_cast<int>(head) - (which ? p.H[0] : 0);
+    t = static_cast<int>(token - b * p.T), step_t = static_cast<int>(step - step_b * p.T);
+  }
+  __device__ __forceinline__ void next(const RopeParams& p) {
+    b += step_b, t += step_t;
+    if (t >= p.T) t -= p.T, ++b;
   }
   __device__ __forceinline__ int64_t offset(const int64_t (&s)[2][3]) const {
     const int64_t *q = s[0], *k = s[1];
@@ -141,122 +212,150 @@ struct Place {
 };
 
 // (c, s) of the lane's pairs; a position outside the table makes them NaN.
-template <int L, bool VEC, bool INTER>
-__device__ __forceinline__ void load_angles(const RopeParams& p, const Place& at, const Lane<L, VEC, INTER>& lane, float (&c)[4], float (&s)[4]) {
-  if (p.table == nullptr) return;
-  int64_t position = at.t;
-  if (p.positions != nullptr) {
-    const int64_t i = at.b * p.ps[0] + at.t * p.ps[1];
-    position = p.pos_int64 ? static_cast<const int64_t*>(p.positions)[i] : static_cast<const int32_t*>(p.positions)[i];
-    if (p.add_token) position += at.t;
-  }
-  const bool inside = position >= 0 && position < p.places;
-  const float* row = p.table + (inside ? position : 0) * p.rotary;
-  if constexpr (VEC) {
-    f32x4 lo = {}, hi = {};
-    if (lane.pair[0] >= 0) {
-      lo = *reinterpret_cast<const f32x4*>(row + 2 * lane.pair[0]);
-      hi = *reinterpret_cast<const f32x4*>(row + 2 * lane.pair[0] + 4);
+struct Angles {
+  float c[4], s[4];
+  bool inside;
+  template <int L, int VEC, bool INTER>
+  __device__ __forceinline__ void load(const RopeParams& p, const Walk& at, const Lane<L, VEC, INTER>& lane) {
+    if (p.table == nullptr) return;
+    int64_t position = at.t;
+    if (p.positions != nullptr) {
+      const int64_t i = at.b * p.ps[0] + at.t * p.ps[1];
+      position = p.pos_int64 ? static_cast<const int64_t*>(p.positions)[i] : static_cast<const int32_t*>(p.positions)[i];
+      if (p.add_token) position += at.t;
     }
-    c[0] = lo[0], s[0] = lo[1], c[1] = lo[2], s[1] = lo[3], c[2] = hi[0], s[2] = hi[1], c[3] = hi[2], s[3] = hi[3];
-  } else {
+    inside = position >= 0 && position < p.places;
+    const float* row = p.table + (inside ? position : 0) * p.rotary;
+    if (p.places == 0) return;
+    if constexpr (VEC != kSingles) {
+      f32x4 lo = {}, hi = {};
+      if (lane.pair[0] >= 0) {
+        lo = *reinterpret_cast<const f32x4*>(row + 2 * lane.pair[0]);
+        hi = *reinterpret_cast<const f32x4*>(row + 2 * lane.pair[0] + 4);
+      }
+      c[0] = lo[0], s[0] = lo[1], c[1] = lo[2], s[1] = lo[3], c[2] = hi[0], s[2] = hi[1], c[3] = hi[2], s[3] = hi[3];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c[e] = lane.pair[e] >= 0 ? row[2 * lane.pair[e]] : 0.f;
+        s[e] = lane.pair[e] >= 0 ? row[2 * lane.pair[e] + 1] : 0.f;
+      }
+    }
+  }
+  // sign 1: by the angles, -1: back
+  template <int L, int VEC, bool INTER>
+  __device__ __forceinline__ void turn(const RopeParams& p, const Lane<L, VEC, INTER>& lane, float sign, float (&v)[8]) const {
+    if (p.table == nullptr) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      c[e] = lane.pair[e] >= 0 ? row[2 * lane.pair[e]] : 0.f;
-      s[e] = lane.pair[e] >= 0 ? row[2 * lane.pair[e] + 1] : 0.f;
+      const float a = v[2 * e], b = v[2 * e + 1], cs = inside ? c[e] : __builtin_nanf(""), sn = inside ? sign * s[e] : __builtin_nanf("");
+      if (lane.pair[e] >= 0) {
+        v[2 * e] = fmaf(a, cs, -(b * sn));
+        v[2 * e + 1] = fmaf(a, sn, b * cs);
+      }
     }
   }
-  if (!inside) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] = s[e] = __builtin_nanf("");
-  }
-}
+};
 
-// sign 1: by the angles, -1: back.
-template <int L, bool VEC, bool INTER>
-__device__ __forceinline__ void turn(const RopeParams& p, const Lane<L, VEC, INTER>& lane, const float (&c)[4], const float (&s)[4], float sign, float (&v)[8]) {
-  if (p.table == nullptr) return;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float a = v[2 * e], b = v[2 * e + 1], sn = sign * s[e];
-    if (lane.pair[e] >= 0) {
-      v[2 * e] = fmaf(a, c[e], -(b * sn));
-      v[2 * e + 1] = fmaf(a, sn, b * c[e]);
-    }
-  }
-}
-
-template <typename T, int L, bool VEC, bool INTER>
+template <typename T, int L, int VEC, bool INTER>
 __global__ __launch_bounds__(kBlock) void head_norm_rope_kernel(const RopeParams p) {
-  constexpr int ROWS = kBlock / L;
   const Lane<L, VEC, INTER> lane(threadIdx.x % L, p.d, p.rotary);
   const bool norm = p.w[0] != nullptr;
-  float w[2][8];
+  Walk at(p, kWave / L, threadIdx.x % kWave / L);
+  float w[8];
+  Raw<T, L, VEC, INTER> next;
   if (norm) {
-    load_row<T, L, VEC, INTER>(static_cast<const T*>(p.w[0]), lane, w[0]);
-    load_row<T, L, VEC, INTER>(static_cast<const T*>(p.w[1]), lane, w[1]);
+    next.load(static_cast<const T*>(at.which ? p.w[1] : p.w[0]), lane);
+    next.get(lane, w);
   }
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / L; row < p.rows; row += static_cast<int64_t>(gridDim.x) * ROWS) {
-    const Place at(p, row);
-    float v[8], c[4], s[4];
-    load_row<T, L, VEC, INTER>(static_cast<const T*>(at.which ? p.x[1] : p.x[0]) + at.offset(p.xs), lane, v);
-    load_angles(p, at, lane, c, s);
+  const T* const x = static_cast<const T*>(at.which ? p.x[1] : p.x[0]);
+  T* const y = static_cast<T*>(at.which ? p.y[1] : p.y[0]);
+  if (!at.there) return;
+  Angles angles;
+  if (at.b < p.B) {
+    next.load(x + at.offset(p.xs), lane);
+    angles.load(p, at, lane);
+  }
+  while (at.b < p.B) {
+    float v[8];
+    next.get(lane, v);
+    const Angles now = angles;
+    T* const to = y + at.offset(p.ys);
+    at.next(p);
+    if (at.b < p.B) {
+      next.load(x + at.offset(p.xs), lane);
+      angles.load(p, at, lane);
+    }
     if (norm) {
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
-      const float rstd = 1.f / sqrtf(group_sum<L>(sum) / p.d + p.eps);
+      const float rstd = rsqrtf(fmaf(group_sum<L>(sum), p.inv_d, p.eps));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= rstd * (at.which ? w[1][i] : w[0][i]);
+      for (int i = 0; i < 8; ++i) v[i] *= rstd * w[i];
     }
-    turn(p, lane, c, s, 1.f, v);
-    store_row<T, L, VEC, INTER>(static_cast<T*>(at.which ? p.y[1] : p.y[0]) + at.offset(p.ys), lane, v);
+    now.turn(p, lane, 1.f, v);
+    store_row<T, L, VEC, INTER>(to, lane, v);
   }
 }
 
-template <typename T, int L, bool VEC, bool INTER>
+template <typename T, int L, int VEC, bool INTER>
 __global__ __launch_bounds__(kBlock) void head_norm_rope_bwd_kernel(const RopeParams p) {
-  constexpr int ROWS = kBlock / L;
   __shared__ float red[kBlock / kWave][2][kMaxHeadWidth];
   const Lane<L, VEC, INTER> lane(threadIdx.x % L, p.d, p.rotary);
   const bool norm = p.w[0] != nullptr;
-  float w[2][8], dw[2][8];
+  Walk at(p, kWave / L, threadIdx.x % kWave / L);
+  float w[8], dw[2][8];
+  Raw<T, L, VEC, INTER> next, next_g;
   if (norm) {
-    load_row<T, L, VEC, INTER>(static_cast<const T*>(p.w[0]), lane, w[0]);
-    load_row<T, L, VEC, INTER>(static_cast<const T*>(p.w[1]), lane, w[1]);
+    next.load(static_cast<const T*>(at.which ? p.w[1] : p.w[0]), lane);
+    next.get(lane, w);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) dw[0][i] = dw[1][i] = 0.f;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / L; row < p.rows; row += static_cast<int64_t>(gridDim.x) * ROWS) {
-    const Place at(p, row);
-    float g[8], c[4], s[4];
-    load_row<T, L, VEC, INTER>(static_cast<const T*>(at.which ? p.g[1] : p.g[0]) + at.offset(p.gs), lane, g);
-    load_angles(p, at, lane, c, s);
+  const T* const x = static_cast<const T*>(at.which ? p.x[1] : p.x[0]);
+  const T* const dy = static_cast<const T*>(at.which ? p.g[1] : p.g[0]);
+  T* const dx = static_cast<T*>(at.which ? p.y[1] : p.y[0]);
+  Angles angles;
+  if (at.there && at.b < p.B) {
+    next_g.load(dy + at.offset(p.gs), lane);
+    if (norm) next.load(x + at.offset(p.xs), lane);
+    angles.load(p, at, lane);
+  }
+  while (at.there && at.b < p.B) {
+    float g[8], u[8];
+    next_g.get(lane, g);
+    if (norm) next.get(lane, u);
+    const Angles now = angles;
+    T* const to = dx + at.offset(p.ys);
+    at.next(p);
+    if (at.b < p.B) {
+      next_g.load(dy + at.offset(p.gs), lane);
+      if (norm) next.load(x + at.offset(p.xs), lane);
+      angles.load(p, at, lane);
+    }
+    now.turn(p, lane, -1.f, g);
     if (norm) {
-      float x[8];
-      load_row<T, L, VEC, INTER>(static_cast<const T*>(at.which ? p.x[1] : p.x[0]) + at.offset(p.xs), lane, x);
-      turn(p, lane, c, s, -1.f, g);
       float sum = 0.f, dot = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        sum = fmaf(x[i], x[i], sum);
-        dot = fmaf(g[i] * (at.which ? w[1][i] : w[0][i]), x[i], dot);
+        sum = fmaf(u[i], u[i], sum);
+        dot = fmaf(g[i] * w[i], u[i], dot);
       }
-      const float rstd = 1.f / sqrtf(group_sum<L>(sum) / p.d + p.eps);
-      const float mean = group_sum<L>(dot) * rstd / p.d;
+      const float rstd = rsqrtf(fmaf(group_sum<L>(sum), p.inv_d, p.eps));
+      const float mean = group_sum<L>(dot) * rstd * p.inv_d;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float u = x[i] * rstd, part = g[i] * u;
-        dw[0][i] += at.which ? 0.f : part;
-        dw[1][i] += at.which ? part : 0.f;
-        g[i] = rstd * (g[i] * (at.which ? w[1][i] : w[0][i]) - u * mean);
+        u[i] *= rstd;
+        dw[0][i] = fmaf(g[i], u[i], dw[0][i]);
+        g[i] = rstd * (g[i] * w[i] - u[i] * mean);
       }
-    } else {
-      turn(p, lane, c, s, -1.f, g);
     }
-    store_row<T, L, VEC, INTER>(static_cast<T*>(at.which ? p.y[1] : p.y[0]) + at.offset(p.ys), lane, g);
+    store_row<T, L, VEC, INTER>(to, lane, g);
   }
   if (!norm) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) dw[1][i] = at.which ? dw[0][i] : 0.f, dw[0][i] = at.which ? 0.f : dw[0][i];
   // the lanes that hold the same features, then the wavefronts, in a fixed order
 #pragma unroll
   for (int off = L; off < kWave; off *= 2) {
@@ -268,8 +367,10 @@ __global__ __launch_bounds__(kBlock) void head_norm_rope_bwd_kernel(const RopePa
   }
   const int wave = threadIdx.x / kWave;
   if (threadIdx.x % kWave < L) {
-    store_row<float, L, VEC, INTER>(red[wave][0], lane, dw[0]);
-    store_row<float, L, VEC, INTER>(red[wave][1], lane, dw[1]);
+    // as singles or runs: the lanes of wide accesses hold the runs of lanes that exchanged
+    const Lane<L, VEC == kWide ? kRuns : VEC, INTER> plain(VEC == kWide ? lane.run_lane(threadIdx.x % L) : threadIdx.x % L, p.d, p.rotary);
+    store_row<float, L, VEC == kWide ? kRuns : VEC, INTER>(red[wave][0], plain, dw[0]);
+    store_row<float, L, VEC == kWide ? kRuns : VEC, INTER>(red[wave][1], plain, dw[1]);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * p.d; i += kBlock) {
@@ -277,26 +378,35 @@ __global__ __launch_bounds__(kBlock) void head_norm_rope_bwd_kernel(const RopePa
     float total = 0.f;
 #pragma unroll
     for (int v = 0; v < kBlock / kWave; ++v) total += red[v][which][c];
-    p.partial[(static_cast<int64_t>(blockIdx.x) * 2 + which) * p.d + c] = total;
+    p.partial[((static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 2 + which) * p.d + c] = total;
   }
 }
 
-// Workgroups of a backward pass with weights: one partial row of both gradients each.
-int64_t bwd_blocks(int64_t rows, int lanes) {
-  const int64_t blocks = (rows + kBlock / lanes - 1) / (kBlock / lanes);
-  return blocks < kBwdMaxBlocks ? blocks : kBwdMaxBlocks;
-}
 int lanes_of(int32_t d) {
   int lanes = 4;
   while (lanes * 8 < d) lanes *= 2;
   return lanes;
 }
+// Workgroups over the tokens, and over the heads where a token's need several wavefronts. A backward pass with weights has kBwdMaxBlocks at most, a partial row of both
+// gradients each.
+struct Grid {
+  int64_t x;
+  int32_t y;
+};
+Grid grid_of(int64_t tokens, int32_t heads, int32_t d, bool back) {
+  const int slots = kWave / lanes_of(d), side = heads < slots ? heads : slots, at_once = slots / side * (kBlock / kWave);
+  Grid grid{(tokens + at_once - 1) / at_once, (heads + slots - 1) / slots};
+  // chunks of heads that are more than that (wide heads in great number) stay: a workgroup each
+  const int64_t all = back ? kBwdMaxBlocks : kForwardBlocks, most = all > grid.y ? all / grid.y : 1;
+  if (grid.x > most) grid.x = most;
+  return grid;
+}
 
-template <typename T, bool VEC, bool INTER>
+template <typename T, int VEC, bool INTER>
 void launch_rope(const RopeParams& p, bool back, hipStream_t s) {
   const int lanes = lanes_of(p.d);
-  const int64_t blocks = (p.rows + kBlock / lanes - 1) / (kBlock / lanes);
-  const dim3 grid(static_cast<uint32_t>(back ? bwd_blocks(p.rows, lanes) : (blocks < (1 << 20) ? blocks : 1 << 20)));
+  const Grid blocks = grid_of(static_cast<int64_t>(p.B) * p.T, p.H[0] + p.H[1], p.d, back);
+  const dim3 grid(static_cast<uint32_t>(blocks.x), static_cast<uint32_t>(blocks.y));
 #define TAAC_ROPE(L)                                                                                              \
   if (lanes == L) {                                                                                               \
     if (back) hipLaunchKernelGGL((head_norm_rope_bwd_kernel<T, L, VEC, INTER>), grid, dim3(kBlock), 0, s, p);     \
@@ -308,17 +418,25 @@ void launch_rope(const RopeParams& p, bool back, hipStream_t s) {
 
 template <typename T>
 void dispatch_rope(const RopeParams& p, bool interleaved, bool back, hipStream_t s) {
-  // Runs of four features: 8 bytes, 16 of fp32, aligned.
-  bool vec = p.d % 8 == 0 && p.rotary % 8 == 0;
-  auto aligned = [&](const void* ptr) { vec &= reinterpret_cast<uintptr_t>(ptr) % (4 * sizeof(T)) == 0; };
-  auto strided = [&](const int64_t (&st)[3]) { vec &= st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0; };
+  // What strides, addresses and widths allow: eight bytes to a run (16 of fp32), sixteen to a lane where lanes that exchange are a power of two apart.
+  constexpr int WIDE = sizeof(T) == 2 ? 8 : 4;
+  int run = p.d % 8 == 0 && p.rotary % 8 == 0 ? WIDE : 1;
+  auto allow = [&](const void* ptr, const int64_t (&st)[3]) {
+    for (int64_t s : {static_cast<int64_t>(reinterpret_cast<uintptr_t>(ptr) / sizeof(T)), st[0], st[1], st[2]})
+      while (s % run != 0) run /= 2;
+  };
+  const int64_t none[3] = {0, 0, 0};
   for (int i = 0; i < 2; ++i) {
-    aligned(p.x[i]), aligned(p.y[i]), aligned(p.w[i]), strided(p.xs[i]), strided(p.ys[i]);
-    if (back) aligned(p.g[i]), strided(p.gs[i]);
+    allow(p.x[i], p.xs[i]), allow(p.y[i], p.ys[i]), allow(p.w[i], none);
+    if (back) allow(p.g[i], p.gs[i]);
   }
-  vec &= aligned16(p.table);
-  if (vec) interleaved ? launch_rope<T, true, true>(p, back, s) : launch_rope<T, true, false>(p, back, s);
-  else interleaved ? launch_rope<T, false, true>(p, back, s) : launch_rope<T, false, false>(p, back, s);
+  if (!aligned16(p.table)) run = 1;
+  const bool exchanges = interleaved || (p.rotary % 16 == 0 && (p.rotary / 16 & (p.rotary / 16 - 1)) == 0);
+  if constexpr (WIDE == 8) {
+    if (run == 8 && exchanges) return interleaved ? launch_rope<T, kWide, true>(p, back, s) : launch_rope<T, kWide, false>(p, back, s);
+  }
+  if (run >= 4) interleaved ? launch_rope<T, kRuns, true>(p, back, s) : launch_rope<T, kRuns, false>(p, back, s);
+  else interleaved ? launch_rope<T, kSingles, true>(p, back, s) : launch_rope<T, kSingles, false>(p, back, s);
 }
 
 int take_rope(const char* name, RopeParams& p, const void* q, const void* k, void* q_out, void* k_out, int32_t B, int32_t H, int32_t key_heads, int32_t T,
@@ -326,7 +444,7 @@ int take_rope(const char* name, RopeParams& p, const void* q, const void* k, voi
               float eps, const float* table, int64_t places, const void* positions, int pos_int64, const int64_t* ps, int add_token, int dtype, bool* empty) {
   if (B < 0 || T < 0 || H <= 0 || key_heads <= 0 || d <= 0) return set_error(TAAC_ERR_INVALID_VALUE, "%s: batch and tokens must be >= 0, heads and width > 0", name);
   if (d > kMaxHeadWidth) return set_error(TAAC_ERR_UNSUPPORTED, "%s: a head has at most %d features (got %d)", name, kMaxHeadWidth, d);
-  if (H > 1 << 20 || key_heads > 1 << 20) return set_error(TAAC_ERR_UNSUPPORTED, "%s: at most 2^20 heads", name);
+  if (H > kMaxHeads || key_heads > kMaxHeads) return set_error(TAAC_ERR_UNSUPPORTED, "%s: at most %d heads", name, kMaxHeads);
   if (rotary < 0 || rotary > d || rotary % 2 != 0) return set_error(TAAC_ERR_INVALID_VALUE, "%s: the rotated features must be an even number, at most the head's (got %d of %d)", name, rotary, d);
   if ((rotary > 0) != (table != nullptr) || places < 0) return set_error(TAAC_ERR_INVALID_VALUE, "%s: a table comes with rotated features, its size not negative", name);
   if ((qw == nullptr) != (kw == nullptr)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: both norm weights or neither", name);
@@ -348,8 +466,7 @@ int take_rope(const char* name, RopeParams& p, const void* q, const void* k, voi
   if (table != nullptr && reinterpret_cast<uintptr_t>(table) % 4 != 0) return set_error(TAAC_ERR_INVALID_VALUE, "%s: misaligned table", name);
   p.x[0] = q, p.x[1] = k, p.y[0] = q_out, p.y[1] = k_out, p.w[0] = qw, p.w[1] = kw;
   p.table = table, p.places = places, p.positions = positions, p.pos_int64 = pos_int64 != 0, p.add_token = add_token != 0;
-  p.rows = static_cast<int64_t>(B) * T * (static_cast<int64_t>(H) + key_heads);
-  p.H[0] = H, p.H[1] = key_heads, p.T = T, p.d = d, p.rotary = rotary, p.eps = eps;
+  p.H[0] = H, p.H[1] = key_heads, p.B = B, p.T = T, p.d = d, p.rotary = rotary, p.eps = eps, p.inv_d = 1.f / static_cast<float>(d);
   return TAAC_OK;
 }
 
@@ -359,9 +476,32 @@ void dispatch_dtype(const RopeParams& p, bool interleaved, bool back, int dtype,
   if (dtype == TAAC_F16) dispatch_rope<f16_t>(p, interleaved, back, s);
 }
 
+// dw = the workgroups' partial rows added in a fixed order: sixteen columns to a workgroup, 64 slices of the rows.
+template <typename T>
+__global__ __launch_bounds__(1024) void head_weights_kernel(const float* __restrict__ partial, int blocks, int d, T* __restrict__ dqw, T* __restrict__ dkw) {
+  __shared__ float red[64][16];
+  const int column = threadIdx.x % 16, slice = threadIdx.x / 16, c = blockIdx.x * 16 + column;
+  float sum = 0.f;
+  if (c < 2 * d) {
+#pragma unroll 4
+    for (int i = slice; i < blocks; i += 64) sum += partial[static_cast<int64_t>(i) * 2 * d + c];
+  }
+  red[slice][column] = sum;
+  __syncthreads();
+  if (slice >= 4) return;  // one wavefront
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum += red[slice + 4 * i][column];
+  sum += __shfl_xor(sum, 16, kWave);
+  sum += __shfl_xor(sum, 32, kWave);
+  if (slice > 0 || c >= 2 * d) return;
+  if (c < d) dqw[c] = static_cast<T>(sum);
+  else dkw[c - d] = static_cast<T>(sum);
+}
+
 template <typename T>
 void reduce_weights(const RopeParams& p, int blocks, void* dqw, void* dkw, hipStream_t s) {
-  hipLaunchKernelGGL(norm_bwd_reduce_kernel<T>, dim3((p.d + 15) / 16), dim3(kBlock), 0, s, p.partial, blocks, p.d, 2, static_cast<T*>(dqw), static_cast<T*>(dkw));
+  hipLaunchKernelGGL(head_weights_kernel<T>, dim3((2 * p.d + 15) / 16), dim3(1024), 0, s, p.partial, blocks, p.d, static_cast<T*>(dqw), static_cast<T*>(dkw));
 }
 
 }  // namespace
@@ -386,8 +526,9 @@ extern "C" int taac_head_norm_rope_fwd(const void* q, const void* k, void* q_out
 
 extern "C" int64_t taac_head_norm_rope_bwd_workspace_floats(int32_t B, int32_t H, int32_t key_heads, int32_t T, int32_t d) {
   using namespace taac;
-  if (B < 0 || T < 0 || H <= 0 || key_heads <= 0 || d <= 0 || d > kMaxHeadWidth) return -1;
-  return bwd_blocks(static_cast<int64_t>(B) * T * (static_cast<int64_t>(H) + key_heads), lanes_of(d)) * 2 * d;
+  if (B < 0 || T < 0 || H <= 0 || key_heads <= 0 || d <= 0 || d > kMaxHeadWidth || H > kMaxHeads || key_heads > kMaxHeads) return -1;
+  const Grid grid = grid_of(static_cast<int64_t>(B) * T, H + key_heads, d, true);
+  return grid.x * grid.y * 2 * d;
 }
 
 extern "C" int taac_head_norm_rope_bwd(const void* q, const void* k, const void* grad_qo, const void* grad_ko, void* grad_q, void* grad_k, void* grad_qw,

@@ -8,6 +8,10 @@ namespace taac {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kMostGroups = 1 << 14;  // of four chunks at a time: a wavefront asks for its next chunk's place while the rows of one are on their way
+#ifndef KCHUNKS
+#define KCHUNKS 12
+#endif
 
 struct CacheParams {
   KvPool pool;
@@ -19,7 +23,8 @@ struct CacheParams {
   const int32_t* lengths;  // [B] or null: T
   int64_t ks[3], vs[3];    // element strides of (batch, head, token)
   int64_t rows;            // B * T * heads
-  int32_t B, T, starts_int64;
+  int64_t units;           // B * chunks * heads
+  int32_t T, chunks, starts_int64;
 };
 
 template <typename T>
@@ -110,6 +115,8 @@ __device__ __forceinline__ void decode(const Codes<BITS>& c, float scale, float 
   for (int i = 0; i < 4; ++i) f[2 * i] = p[i][0], f[2 * i + 1] = p[i][1];
 }
 
+// ---- a few tokens: row by row --------------------------------------------------------------------------------------
+
 // A row (sample, token, head) and where it belongs: D / 8 lanes, eight features each.
 struct Row {
   int64_t b, position;
@@ -134,8 +141,7 @@ __global__ __launch_bounds__(kThreads) void kv_write_rows_kernel(const CachePara
   if (row >= p.rows) return;
   const int s = threadIdx.x % LANES, block = s / 4, sub = s % 4;
   const Row at(p, row);
-  if (!at.there) return;
-  const int64_t page = kv_page(p.pool, at.b, at.position >> p.pool.page_shift);
+  const int64_t page = at.there ? kv_page(p.pool, at.b, at.position >> p.pool.page_shift) : -1;
   if (page < 0) return;
   Eight<T> k, v;
   k.load(static_cast<const T*>(p.k) + at.b * p.ks[0] + at.h * p.ks[1] + at.t * p.ks[2] + 8 * s);
@@ -231,8 +237,289 @@ __global__ __launch_bounds__(kThreads) void kv_read_rows_kernel(const CacheParam
   v.store(static_cast<T*>(p.v_out) + at.b * p.vs[0] + at.h * p.vs[1] + at.t * p.vs[2] + 8 * s);
 }
 
+// ---- many tokens: chunk by chunk -----------------------------------------------------------------------------------
+//
+// A wavefront has the sixteen tokens of a record: lane = (token, sub), features 8 sub .. 8 sub + 7 of every block of 32. Keys leave as they lie. Values of four tokens and
+// two features turn into a word in two exchanges of lanes, between the sixteens of a block's features and between the tokens of a group, so that all
+// of a record is written and read in whole words, side by side.
+
+// One of a call's integers. SCALAR: by a scalar read, which counts apart from a chunk's rows and does not wait for them. For heads of 32 features, whose chunks are
+// small, that is a sixth faster (512 ragged histories of 512 tokens, 8 heads, written and read: 124 against 147 us), for wider ones a tenth slower
+// (16 x 8000 tokens of 8 heads of 128 in 8 bits: 361 against 324).
+template <bool SCALAR>
+__device__ __forceinline__ int64_t integer_at(const void* p, int64_t i, bool wide) {
+  if constexpr (SCALAR) {
+    typedef const __attribute__((address_space(4))) int32_t* Narrow;
+    typedef const __attribute__((address_space(4))) int64_t* Wide;
+    return wide ? ((Wide)(reinterpret_cast<uint64_t>(p)))[i] : ((Narrow)(reinterpret_cast<uint64_t>(p)))[i];
+  }
+  return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+}
+
+// Sample, head and chunk of a wavefront: which of the chunk's tokens are the call's, and which of them there are. The same in all
+// lanes.
+template <bool SCALAR>
+struct Chunk {
+  int64_t b;
+  int h;
+  int t0;               // the call's token that would be the chunk's first
+  int first, end;       // tokens first .. end - 1 of the chunk are written (read)
+  uint8_t* record;      // null: in no page, or nothing to do there
+  Chunk() = default;
+  __device__ __forceinline__ Chunk(const CacheParams& p, int64_t unit, int record_bytes) {
+    const uint32_t heads = p.pool.heads;
+    int64_t rest;
+    if (unit < 0x7fffffff) {
+      rest = static_cast<uint32_t>(unit) / heads;
+      b = static_cast<uint32_t>(rest) / static_cast<uint32_t>(p.chunks);
+    } else {
+      rest = unit / heads;
+      b = rest / p.chunks;
+    }
+    h = static_cast<int>(unit - rest * heads);
+    int64_t start = p.starts == nullptr ? 0 : integer_at<SCALAR>(p.starts, b, p.starts_int64);
+    int n = p.lengths == nullptr ? p.T : min(max(static_cast<int>(integer_at<SCALAR>(p.lengths, b, false)), 0), p.T);
+    if (start < 0 || start >= int64_t{1} << 40) start = 0, n = 0;
+    const int64_t chunk = (start / kKvChunk) + (rest - b * p.chunks), from = chunk * kKvChunk, behind = start + n - from;
+    t0 = static_cast<int>(from - start);
+    first = t0 < 0 ? -t0 : 0;
+    end = behind < kKvChunk ? static_cast<int>(behind) : kKvChunk;  // not above first: nothing
+    const int64_t index = from >> p.pool.page_shift;
+    record = nullptr;
+    if (first < end && index < p.pool.table_pages) {
+      const int64_t page = integer_at<SCALAR>(p.pool.table, b * p.pool.table_stride + index, p.pool.int64);
+      if (page >= 0 && page < p.pool.pages)
+        record = p.pool.data + kv_record(p.pool, page, h, static_cast<int>(chunk & ((1 << (p.pool.page_shift - 4)) - 1)), record_bytes);
+    }
+  }
+};
+
+// Lanes of four tokens (bits 2 and 3 of the lane) hold four bytes each: byte i of lane j becomes byte j of lane i. Its own inverse.
+__device__ __forceinline__ uint32_t turn_bytes(uint32_t w, int token) {
+  uint32_t other = __shfl_xor(w, 4, kWave);
+  w = __builtin_amdgcn_perm(other, w, token & 1 ? 0x03070105u : 0x06020400u);
+  other = __shfl_xor(w, 8, kWave);
+  return __builtin_amdgcn_perm(other, w, token & 2 ? 0x03020706u : 0x05040100u);
+}
+// The same of four halves of 16 bits.
+__device__ __forceinline__ void turn_halves(uint32_t (&w)[2], int token) {
+  const uint32_t a = __shfl_xor(w[0], 4, kWave), b = __shfl_xor(w[1], 4, kWave), pick = token & 1 ? 0x03020706u : 0x05040100u;
+  const uint32_t x = __builtin_amdgcn_perm(a, w[0], pick), y = __builtin_amdgcn_perm(b, w[1], pick);
+  const uint32_t other = __shfl_xor(token & 2 ? x : y, 8, kWave);
+  w[0] = token & 2 ? other : x;
+  w[1] = token & 2 ? y : other;
+}
+
+__device__ __forceinline__ uint32_t spread_nibbles(uint32_t x) {  // four in the low half, a byte each
+  x = (x | x << 8) & 0x00ff00ffu;
+  return (x | x << 4) & 0x0f0f0f0fu;
+}
+__device__ __forceinline__ uint32_t gather_nibbles(uint32_t x) {
+  x = (x | x >> 4) & 0x00ff00ffu;
+  return (x | x >> 8) & 0xffffu;
+}
+
+// Codes of eight features of a token -> the words of the record that this lane writes: features n = 8 (sub % 2) + 4 (sub / 2) + token % 4 and n + 16, tokens 4 (token / 4) ..
+template <int BITS>
+__device__ __forceinline__ Codes<BITS> to_record(const Codes<BITS>& c, int token, int sub) {
+  Codes<BITS> r;
+  if constexpr (BITS == 4) {
+    const uint32_t w = c.w[0], other = __shfl_xor(sub < 2 ? w >> 16 : w & 0xffffu, 2, kWave);
+    r.w[0] = turn_bytes(spread_nibbles(sub < 2 ? w & 0xffffu : other) | spread_nibbles(sub < 2 ? other : w >> 16) << 4, token);
+  } else {
+    const uint32_t other = __shfl_xor(sub < 2 ? c.w[1] : c.w[0], 2, kWave), low = sub < 2 ? c.w[0] : other, high = sub < 2 ? other : c.w[1];
+    r.w[0] = __builtin_amdgcn_perm(high, low, 0x05010400u), r.w[1] = __builtin_amdgcn_perm(high, low, 0x07030602u);
+    turn_halves(r.w, token);
+  }
+  return r;
+}
+template <int BITS>
+__device__ __forceinline__ Codes<BITS> from_record(const Codes<BITS>& c, int token, int sub) {
+  Codes<BITS> r;
+  if constexpr (BITS == 4) {
+    const uint32_t w = turn_bytes(c.w[0], token), low = gather_nibbles(w & 0x0f0f0f0fu), high = gather_nibbles(w >> 4 & 0x0f0f0f0fu);
+    const uint32_t other = __shfl_xor(sub < 2 ? high : low, 2, kWave);
+    r.w[0] = sub < 2 ? low | other << 16 : other | high << 16;
+  } else {
+    uint32_t w[2] = {c.w[0], c.w[1]};
+    turn_halves(w, token);
+    const uint32_t low = __builtin_amdgcn_perm(w[1], w[0], 0x06040200u), high = __builtin_amdgcn_perm(w[1], w[0], 0x07050301u);
+    const uint32_t other = __shfl_xor(sub < 2 ? high : low, 2, kWave);
+    r.w[0] = sub < 2 ? low : other, r.w[1] = sub < 2 ? other : high;
+  }
+  return r;
+}
+
+template <int N>
+__device__ __forceinline__ void store_words(uint8_t* p, const uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) reinterpret_cast<u32x4*>(p)[i] = u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+  } else if constexpr (N == 2) {
+    *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
+  } else {
+    *reinterpret_cast<uint32_t*>(p) = w[0];
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const u32x4 v = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[4 * i + j] = v[j];
+    }
+  } else if constexpr (N == 2) {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+    w[0] = v[0], w[1] = v[1];
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+template <typename T, int D, int BITS>
+__global__ __launch_bounds__(kThreads) void kv_write_chunks_kernel(const CacheParams p) {
+  constexpr int BLOCKS = D / kKvBlock, EACH = BITS / 4;
+  constexpr bool SCALAR = D == 32;
+  const int lane = threadIdx.x % kWave, token = lane / 4, sub = lane % 4;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / kWave);
+  int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + (SCALAR ? __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : threadIdx.x / kWave);
+  Chunk<SCALAR> at, next;
+  if (unit < p.units) next = Chunk<SCALAR>(p, unit, kv_record_bytes(D, BITS));
+  for (; unit < p.units; unit += step) {
+    at = next;
+    if (at.record == nullptr) {
+      if (unit + step < p.units) next = Chunk<SCALAR>(p, unit + step, kv_record_bytes(D, BITS));
+      continue;
+    }
+    const bool there = token >= at.first && token < at.end;
+    Eight<T> k[BLOCKS], v[BLOCKS];
+    const T* kp = static_cast<const T*>(p.k) + at.b * p.ks[0] + at.h * p.ks[1] + (at.t0 + token) * p.ks[2] + 8 * sub;
+    const T* vp = static_cast<const T*>(p.v) + at.b * p.vs[0] + at.h * p.vs[1] + (at.t0 + token) * p.vs[2] + 8 * sub;
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k[j].f[i] = v[j].f[i] = 0.f;
+      if (there) {
+        k[j].load(kp + kKvBlock * j);
+        v[j].load(vp + kKvBlock * j);
+      }
+    }
+    if (unit + step < p.units) next = Chunk<SCALAR>(p, unit + step, kv_record_bytes(D, BITS));
+    int k_scale[BLOCKS], v_scale[BLOCKS], bad = 0;
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j) {
+      float k_most = 0.f, v_most = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        k_most = fmaxf(k_most, fabsf(k[j].f[i]));
+        v_most = fmaxf(v_most, fabsf(v[j].f[i]));
+        bad |= !(fabsf(k[j].f[i]) <= 3.4028235e38f) | !(fabsf(v[j].f[i]) <= 3.4028235e38f);
+      }
+      k_scale[j] = scale_byte<BITS>(group_max<4>(k_most));
+      v_scale[j] = scale_byte<BITS>(group_max<4>(v_most));
+    }
+    bad |= __shfl_xor(bad, 1, kWave);
+    bad |= __shfl_xor(bad, 2, kWave);
+    uint32_t values[BLOCKS * EACH];
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j) {
+      if (bad) {
+        k_scale[j] = kKvNotFinite, v_scale[j] = 127;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[j].f[i] = v[j].f[i] = 0.f;
+      }
+      const Codes<BITS> kc = encode<BITS>(k[j].f, bad ? 127 : k_scale[j]), vc = to_record<BITS>(encode<BITS>(v[j].f, v_scale[j]), token, sub);
+      if (there) store_words(at.record + j * (kKvChunk * 4 * BITS) + token * 4 * BITS + sub * BITS, kc.w);
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) values[j * EACH + i] = vc.w[i];
+    }
+    const int n = 8 * (sub % 2) + 4 * (sub / 2) + token % 4, group = token / 4;
+    uint8_t* to = at.record + kv_value_at(D, BITS) + (n * 4 + group) * BLOCKS * BITS;
+    if (4 * group >= at.first && 4 * group + 4 <= at.end) {
+      store_words(to, values);
+    } else {
+#pragma unroll
+      for (int j = 0; j < BLOCKS; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (4 * group + e < at.first || 4 * group + e >= at.end) continue;
+          if constexpr (BITS == 4) to[j * 4 + e] = static_cast<uint8_t>(values[j] >> (8 * e));
+          else *reinterpret_cast<uint16_t*>(to + j * 8 + 2 * e) = static_cast<uint16_t>(values[2 * j + e / 2] >> (16 * (e % 2)));
+        }
+    }
+    if (there && sub == 0) {
+#pragma unroll
+      for (int j = 0; j < BLOCKS; ++j) {
+        at.record[kv_key_scale_at(D, BITS) + token * BLOCKS + j] = static_cast<uint8_t>(k_scale[j]);
+        at.record[kv_value_scale_at(D, BITS) + (group * BLOCKS + j) * 4 + token % 4] = static_cast<uint8_t>(v_scale[j]);
+      }
+    }
+  }
+}
+
+template <typename T, int D, int BITS>
+__global__ __launch_bounds__(kThreads) void kv_read_chunks_kernel(const CacheParams p) {
+  constexpr int BLOCKS = D / kKvBlock, EACH = BITS / 4;
+  constexpr bool SCALAR = D == 32;
+  const int lane = threadIdx.x % kWave, token = lane / 4, sub = lane % 4;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / kWave);
+  int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + (SCALAR ? __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : threadIdx.x / kWave);
+  Chunk<SCALAR> at, next;
+  if (unit < p.units) next = Chunk<SCALAR>(p, unit, kv_record_bytes(D, BITS));
+  for (; unit < p.units; unit += step) {
+    at = next;
+    const bool there = at.record != nullptr && token >= at.first && token < at.end;
+    Codes<BITS> keys[BLOCKS];
+    uint32_t values[BLOCKS * EACH], k_scale[BLOCKS], v_scale[BLOCKS];
+    const int n = 8 * (sub % 2) + 4 * (sub / 2) + token % 4, group = token / 4;
+    if (at.record != nullptr) {
+#pragma unroll
+      for (int j = 0; j < BLOCKS; ++j) {
+        load_words(at.record + j * (kKvChunk * 4 * BITS) + token * 4 * BITS + sub * BITS, keys[j].w);
+        k_scale[j] = at.record[kv_key_scale_at(D, BITS) + token * BLOCKS + j];
+        v_scale[j] = at.record[kv_value_scale_at(D, BITS) + (group * BLOCKS + j) * 4 + token % 4];
+      }
+      load_words(at.record + kv_value_at(D, BITS) + (n * 4 + group) * BLOCKS * BITS, values);
+    }
+    if (unit + step < p.units) next = Chunk<SCALAR>(p, unit + step, kv_record_bytes(D, BITS));
+    const int t = at.t0 + token;
+    T* kp = static_cast<T*>(p.k_out) + at.b * p.ks[0] + at.h * p.ks[1] + t * p.ks[2] + 8 * sub;
+    T* vp = static_cast<T*>(p.v_out) + at.b * p.vs[0] + at.h * p.vs[1] + t * p.vs[2] + 8 * sub;
+    const bool asked = t >= 0 && t < p.T;
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j) {
+      Eight<T> k, v;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k.f[i] = v.f[i] = 0.f;
+      if (at.record != nullptr) {
+        Codes<BITS> c;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) c.w[i] = values[j * EACH + i];
+        c = from_record<BITS>(c, token, sub);
+        if (there) {
+          decode<BITS>(keys[j], kv_scale(k_scale[j]), k.f);
+          decode<BITS>(c, kv_scale(k_scale[j] == kKvNotFinite ? kKvNotFinite : v_scale[j]), v.f);
+        }
+      }
+      if (asked) {
+        k.store(kp + kKvBlock * j);
+        v.store(vp + kKvBlock * j);
+      }
+    }
+  }
+}
+
 template <typename T, int D, int BITS>
 void launch_cache(const CacheParams& p, bool write, hipStream_t s) {
+  if (p.chunks > 0) {
+    const int64_t groups = (p.units + kThreads / kWave - 1) / (kThreads / kWave);
+    const dim3 grid(static_cast<uint32_t>(groups < kMostGroups ? groups : kMostGroups));
+    if (write) hipLaunchKernelGGL((kv_write_chunks_kernel<T, D, BITS>), grid, dim3(kThreads), 0, s, p);
+    else hipLaunchKernelGGL((kv_read_chunks_kernel<T, D, BITS>), grid, dim3(kThreads), 0, s, p);
+    return;
+  }
   constexpr int ROWS = kThreads / (D / 8);
   const dim3 grid(static_cast<uint32_t>((p.rows + ROWS - 1) / ROWS));
   if (write) hipLaunchKernelGGL((kv_write_rows_kernel<T, D, BITS>), grid, dim3(kThreads), 0, s, p);
@@ -258,9 +545,12 @@ int run_cache(const char* name, CacheParams& p, bool write, const void* k, const
   if (B == 0 || T == 0) return TAAC_OK;
   if (!k || !v) return set_error(TAAC_ERR_INVALID_VALUE, "%s: null tensor pointer", name);
   if (!aligned16(k) || !aligned16(v)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: tensors must be 16-byte aligned", name);
-  p.B = B, p.T = T;
+  p.T = T;
   p.rows = static_cast<int64_t>(B) * T * p.pool.heads;
-  if (p.rows > int64_t{0x7fffffff} * 16) return set_error(TAAC_ERR_UNSUPPORTED, "%s: too many rows for one call", name);
+  // chunks that T tokens meet at most, wherever they start
+  const int chunks = static_cast<int>((static_cast<int64_t>(T) + 2 * kKvChunk - 2) / kKvChunk);
+  if (T >= kChunksFrom || p.rows > int64_t{1} << 27) p.chunks = chunks;
+  p.units = static_cast<int64_t>(B) * chunks * p.pool.heads;
   if (dtype == TAAC_F32) dispatch_cache<float>(p, d, bits, write, s);
   if (dtype == TAAC_BF16) dispatch_cache<bf16_t>(p, d, bits, write, s);
   if (dtype == TAAC_F16) dispatch_cache<f16_t>(p, d, bits, write, s);
