@@ -9,9 +9,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int64_t kMostGroups = 1 << 14;  // of four chunks at a time: a wavefront asks for its next chunk's place while the rows of one are on their way
-#ifndef KCHUNKS
-#define KCHUNKS 12
-#endif
+// Rows of tokens one by one below, chunks from here on: 512 samples of 8 heads of 32 features in 4 bits, written and read, take 11 : 15 us with 8 tokens, 17 : 15 with 16;
+// 64 samples of 128 features in 8 bits 9 : 11 and 12 : 11.
+constexpr int kChunksFrom = 12;
 
 struct CacheParams {
   KvPool pool;
