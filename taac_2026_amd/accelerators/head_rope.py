@@ -23,18 +23,25 @@ _Strides2 = ctypes.c_int64 * 2
 
 
 @functools.lru_cache(maxsize=512)
-def _strides3(batch: int, head: int, token: int) -> ctypes.Array:
+def _strides3(batch: int, head: int, token: int, _: int) -> ctypes.Array:
     return _Strides3(batch, head, token)
 
 
 def strides_of(t: torch.Tensor) -> ctypes.Array:
-    """Of (batch, head, token), for the library to read."""
-    return _strides3(*t.stride()[:3])
+    """Of (batch, head, token), for the library to read. The arrays are kept by value: a serving program repeats a few."""
+    return _strides3(*t.stride())
 
 
-def token_major(batch: int, heads: int, tokens: int, width: int, like: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+@functools.lru_cache(maxsize=64)
+def _strides2(sample: int, token: int) -> ctypes.Array:
+    return _Strides2(sample, token)
+
+
+def token_major(shape: torch.Size, like: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
     """(batch, heads, tokens, width) whose memory order is (batch, tokens, heads, width): the rows of the layers around it."""
-    return like.new_empty_strided((batch, heads, tokens, width), (tokens * heads * width, width, heads * width, 1), dtype=dtype or like.dtype)
+    batch, heads, tokens, width = shape
+    row = heads * width
+    return torch.empty_strided(shape, (tokens * row, width, row, 1), dtype=dtype or like.dtype, device=like.device)
 
 
 def rotary_table(
@@ -72,22 +79,25 @@ def rotary_table(
     return (magnitude * torch.stack((angles.cos(), angles.sin()), -1)).float()
 
 
-def _arguments(q, k, q_out, k_out, weights, eps, table, positions, add_token, interleaved):
-    """The common arguments of both directions, from the sizes to the flags, in two halves around the strides of the gradients."""
-    position_strides = None if positions is None else _Strides2(*positions.stride())
+def _arguments(q, k, q_out, k_out, weights, eps, table, places, interleaved):
+    """The common arguments of both directions, from the sizes to the flags, in two halves around the strides of the gradients. ``places``: the positions'
+    tensor or None, its strides for (sample, token), and whether the token's number is added."""
+    positions, position_strides, add_token = places
+    batch, heads, tokens, width = q.shape
     return (
-        (q.shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[3], 0 if table is None else 2 * table.shape[1], strides_of(q), strides_of(k)),
+        (batch, heads, k.shape[1], tokens, width, 0 if table is None else 2 * table.shape[1], strides_of(q), strides_of(k)),
         (strides_of(q_out), strides_of(k_out), _native.ptr(weights[0]), _native.ptr(weights[1]), eps, _native.ptr(table),
-         0 if table is None else table.shape[0], _native.ptr(positions), int(positions is not None and positions.dtype == torch.int64), position_strides,
-         int(add_token), int(interleaved), _native.dtype_code(q.dtype), _native.current_stream(q.device)),
+         0 if table is None else table.shape[0], _native.ptr(positions), positions is not None and positions.dtype == torch.int64, position_strides,
+         add_token, interleaved, _native.dtype_code(q.dtype), _native.current_stream(q.device)),
     )
 
 
-def _forward(q, k, weights, eps, table, positions, add_token, interleaved):
-    q_out, k_out = (token_major(*t.shape[:2], *t.shape[2:], t) for t in (q, k))
-    sizes, rest = _arguments(q, k, q_out, k_out, weights, eps, table, positions, add_token, interleaved)
+def _forward(q, k, weights, eps, table, places, interleaved):
+    q_out, k_out = token_major(q.shape, q), token_major(k.shape, k)
+    sizes, rest = _arguments(q, k, q_out, k_out, weights, eps, table, places, interleaved)
+    library = _native.load_library()
     with _native.on_device(q.device):
-        status = _native.load_library().taac_head_norm_rope_fwd(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), *sizes, *rest)
+        status = library.taac_head_norm_rope_fwd(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), *sizes, *rest)
     _native.check(status, "head_norm_rope")
     return q_out, k_out
 
@@ -96,34 +106,38 @@ class _HeadNormRopeFunction(torch.autograd.Function):
     """Keeps the inputs; the backward makes each row's statistic again."""
 
     @staticmethod
-    def forward(ctx, q, k, query_weight, key_weight, eps, table, positions, add_token, interleaved):
+    def forward(ctx, q, k, query_weight, key_weight, eps, table, positions, position_strides, add_token, interleaved):
         ctx.save_for_backward(*((q, k) if query_weight is not None else (None, None)), query_weight, key_weight, table, positions)
-        ctx.options = eps, add_token, interleaved
-        return _forward(q, k, (query_weight, key_weight), eps, table, positions, add_token, interleaved)
+        ctx.options = eps, position_strides, add_token, interleaved
+        return _forward(q, k, (query_weight, key_weight), eps, table, (positions, position_strides, add_token), interleaved)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_q_out, grad_k_out):
         q, k, query_weight, key_weight, table, positions = ctx.saved_tensors
-        eps, add_token, interleaved = ctx.options
-        grad_q_out, grad_k_out = (_rows(t) for t in (grad_q_out, grad_k_out))
+        eps, position_strides, add_token, interleaved = ctx.options
+        grad_q_out, grad_k_out = _rows(grad_q_out), _rows(grad_k_out)
         if q is None:  # a rotation alone does not read them
             q, k = grad_q_out, grad_k_out
-        grad_q, grad_k = (token_major(*t.shape[:2], *t.shape[2:], t) for t in (q, k))
+        grad_q, grad_k = token_major(q.shape, q), token_major(k.shape, k)
         grad_weights, workspace, floats = (None, None), None, 0
         library = _native.load_library()
         if query_weight is not None:
             grad_weights = torch.empty_like(query_weight), torch.empty_like(key_weight)
             floats = library.taac_head_norm_rope_bwd_workspace_floats(q.shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[3])
             workspace = q.new_empty(floats, dtype=torch.float32)
-        sizes, rest = _arguments(q, k, grad_q, grad_k, (query_weight, key_weight), eps, table, positions, add_token, interleaved)
+        sizes, rest = _arguments(q, k, grad_q, grad_k, (query_weight, key_weight), eps, table, (positions, position_strides, add_token), interleaved)
         with _native.on_device(q.device):
             status = library.taac_head_norm_rope_bwd(
                 q.data_ptr(), k.data_ptr(), grad_q_out.data_ptr(), grad_k_out.data_ptr(), grad_q.data_ptr(), grad_k.data_ptr(),
                 _native.ptr(grad_weights[0]), _native.ptr(grad_weights[1]), _native.ptr(workspace), floats, *sizes,
                 strides_of(grad_q_out), strides_of(grad_k_out), *rest)
         _native.check(status, "head_norm_rope backward")
-        return grad_q, grad_k, *grad_weights, None, None, None, None, None
+        return grad_q, grad_k, *grad_weights, None, None, None, None, None, None
+
+
+def _weight(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return t if t.dtype == dtype and t.stride(0) == 1 else t.to(dtype).contiguous()
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -153,12 +167,14 @@ def head_norm_rope(
     float32, bfloat16 or float16; a head has at most 512 features. Arithmetic in float32, rounded once. Differentiable in q, k and the
     weights."""
     name = "head_norm_rope"
-    if q.ndim != 4 or k.ndim != 4:
+    q_shape, k_shape = q.shape, k.shape
+    if len(q_shape) != 4 or len(k_shape) != 4:
         raise ValueError(f"{name} expects q and k with shape (batch, heads, tokens, width)")
-    if q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:] or q.shape[1] == 0 or k.shape[1] == 0 or q.shape[3] == 0:
-        raise ValueError(f"{name} requires matching batch, tokens and width of q and k, got {tuple(q.shape)} and {tuple(k.shape)}")
-    require_same_dtype(f"{name} q, k", q, k)
-    batch, _, tokens, width = q.shape
+    batch, heads, tokens, width = q_shape
+    if batch != k_shape[0] or tokens != k_shape[2] or width != k_shape[3] or heads == 0 or k_shape[1] == 0 or width == 0:
+        raise ValueError(f"{name} requires matching batch, tokens and width of q and k, got {tuple(q_shape)} and {tuple(k_shape)}")
+    if q.dtype != k.dtype:
+        require_same_dtype(f"{name} q, k", q, k)
     if (query_weight is None) != (key_weight is None):
         raise ValueError(f"{name} takes both norm weights or neither")
     if query_weight is None and table is None:
@@ -189,15 +205,19 @@ def head_norm_rope(
         raise RuntimeError(f"hip {name} does not support dtype {q.dtype}")
     if width > MAX_HEAD_WIDTH:
         raise RuntimeError(f"hip {name} is built for heads of at most {MAX_HEAD_WIDTH} features")
-    require_inference(f"hip {name} table", table)
+    if table is not None and table.requires_grad:
+        require_inference(f"hip {name} table", table)
     if query_weight is not None:
-        query_weight, key_weight = (w.to(q.dtype).contiguous() for w in (query_weight, key_weight))
+        query_weight, key_weight = _weight(query_weight, q.dtype), _weight(key_weight, q.dtype)
+    position_strides = None
     if place is not None:
-        place = place[:, None].expand(batch, tokens) if starts is not None else place.expand(batch, tokens)
+        strides = place.stride()
+        position_strides = _strides2(strides[0], 0) if starts is not None else _strides2(*((0, *strides)[-2:]))
     q, k = _rows(q), _rows(k)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, query_weight, key_weight)):
-        return _HeadNormRopeFunction.apply(q, k, query_weight, key_weight, float(eps), table, place, starts is not None, bool(interleaved))
-    return _forward(q, k, (query_weight, key_weight), float(eps), table, place, starts is not None, bool(interleaved))
+    eps, interleaved, add_token = float(eps), bool(interleaved), starts is not None
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (query_weight is not None and (query_weight.requires_grad or key_weight.requires_grad))):
+        return _HeadNormRopeFunction.apply(q, k, query_weight, key_weight, eps, table, place, position_strides, add_token, interleaved)
+    return _forward(q, k, (query_weight, key_weight), eps, table, (place, position_strides, add_token), interleaved)
 
 
 __all__ = ["head_norm_rope", "rotary_table"]

@@ -9,7 +9,7 @@ token's head the values are stored as codes times one power of two, the least wi
 from __future__ import annotations
 
 import functools
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -22,6 +22,11 @@ _CHUNK = 16
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
+@functools.lru_cache(maxsize=64)
+def _record_bytes(head_dim: int, bits: int) -> int:
+    return _native.load_library().taac_kv_cache_bytes(1, 1, _CHUNK, head_dim, bits)
+
+
 @dataclass(frozen=True)
 class KVCache:
     """A pool of pages (:func:`empty_kv_cache`). ``data``: uint8 (pages, heads, page_tokens / 16, bytes of 16 tokens), the library's own layout."""
@@ -29,23 +34,16 @@ class KVCache:
     data: torch.Tensor
     head_dim: int
     bits: int
+    pages: int = field(init=False)
+    heads: int = field(init=False)
+    page_tokens: int = field(init=False)
 
-    @property
-    def pages(self) -> int:
-        return self.data.shape[0]
-
-    @property
-    def heads(self) -> int:
-        return self.data.shape[1]
-
-    @property
-    def page_tokens(self) -> int:
-        return self.data.shape[2] * _CHUNK
-
-
-@functools.lru_cache(maxsize=64)
-def _record_bytes(head_dim: int, bits: int) -> int:
-    return _native.load_library().taac_kv_cache_bytes(1, 1, _CHUNK, head_dim, bits)
+    def __post_init__(self) -> None:
+        data = self.data
+        if data.ndim != 4 or data.dtype != torch.uint8 or not data.is_contiguous() or data.shape[3] != _record_bytes(self.head_dim, self.bits):
+            raise ValueError("KVCache expects data as made by empty_kv_cache")
+        for name, value in (("pages", data.shape[0]), ("heads", data.shape[1]), ("page_tokens", data.shape[2] * _CHUNK)):
+            object.__setattr__(self, name, value)
 
 
 def empty_kv_cache(pages: int, heads: int, head_dim: int, *, bits: int = 4, page_tokens: int = 64, device: torch.device | str) -> KVCache:
@@ -63,12 +61,6 @@ def empty_kv_cache(pages: int, heads: int, head_dim: int, *, bits: int = 4, page
     return KVCache(data, int(head_dim), int(bits))
 
 
-def _check_cache(name: str, cache: KVCache) -> None:
-    data = cache.data
-    if data.ndim != 4 or data.dtype != torch.uint8 or not data.is_contiguous() or data.shape[3] != _record_bytes(cache.head_dim, cache.bits):
-        raise ValueError(f"{name} expects a cache as made by empty_kv_cache")
-
-
 def _check_pages(name: str, pages: torch.Tensor, batch: int) -> None:
     if pages.ndim != 2 or pages.shape[0] != batch or pages.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} expects a table of pages (batch, pages of a sample) in int32 or int64")
@@ -79,7 +71,7 @@ def _check_pages(name: str, pages: torch.Tensor, batch: int) -> None:
 def _integers(name: str, what: str, t: torch.Tensor, batch: int) -> torch.Tensor:
     if t.shape != (batch,) or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} {what} must hold one int32 or int64 per sample")
-    return t.contiguous()
+    return t if t.stride(0) == 1 else t.contiguous()
 
 
 def _lengths(name: str, what: str, t: torch.Tensor | None, batch: int) -> torch.Tensor | None:
@@ -97,8 +89,8 @@ def _pool(cache: KVCache, pages: torch.Tensor) -> tuple:
 
 def _in_place(t: torch.Tensor, size: int) -> torch.Tensor:
     """``t`` where the library can read it (contiguous rows at 16-byte addresses), else a copy."""
-    strides = t.stride()
-    if strides[3] == 1 and all(s * size % 16 == 0 for s in strides[:3]) and t.data_ptr() % 16 == 0:
+    batch, head, token, feature = t.stride()
+    if feature == 1 and (batch | head | token) * size % 16 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -118,12 +110,12 @@ def kv_cache_write(
 
     float32, bfloat16 or float16. A token whose key or value, in a head, has a NaN or an infinity is stored as NaN there. Forward only."""
     name = "kv_cache_write"
-    _check_cache(name, cache)
     if k.ndim != 4 or k.shape != v.shape:
         raise ValueError(f"{name} expects k and v of one shape (batch, heads, tokens, width)")
     if k.shape[1] != cache.heads or k.shape[3] != cache.head_dim:
         raise ValueError(f"{name} expects {cache.heads} heads of {cache.head_dim} features, got {k.shape[1]} of {k.shape[3]}")
-    require_same_dtype(f"{name} k, v", k, v)
+    if k.dtype != v.dtype:
+        require_same_dtype(f"{name} k, v", k, v)
     batch, _, tokens, _ = k.shape
     _check_pages(name, pages, batch)
     starts = None if starts is None else _integers(name, "starts", starts, batch)
@@ -132,7 +124,8 @@ def kv_cache_write(
     require_inference(f"hip {name}", k, v)
     if k.dtype not in _DTYPES:
         raise RuntimeError(f"hip {name} does not support dtype {k.dtype}")
-    k, v = (_in_place(t, t.element_size()) for t in (k, v))
+    size = k.element_size()
+    k, v = _in_place(k, size), _in_place(v, size)
     with _native.on_device(k.device):
         status = _native.load_library().taac_kv_cache_write(
             *_pool(cache, pages), k.data_ptr(), v.data_ptr(), _native.ptr(starts), int(starts is not None and starts.dtype == torch.int64),
@@ -154,7 +147,6 @@ def kv_cache_read(
     order (batch, tokens, heads, width). Positions at or beyond ``lengths[b]`` tokens, and those in no page of the pool, are zeros. Exact in bfloat16 and
     float32; in float16 where it reaches."""
     name = "kv_cache_read"
-    _check_cache(name, cache)
     batch = pages.shape[0] if pages.ndim == 2 else -1
     _check_pages(name, pages, batch)
     if int(tokens) < 0:
@@ -164,7 +156,7 @@ def kv_cache_read(
     require_cuda_tensors(f"hip {name}", cache.data, pages, starts, lengths)
     if dtype not in _DTYPES:
         raise RuntimeError(f"hip {name} does not support dtype {dtype}")
-    k, v = (token_major(batch, cache.heads, int(tokens), cache.head_dim, cache.data, dtype) for _ in range(2))
+    k, v = (token_major((batch, cache.heads, int(tokens), cache.head_dim), cache.data, dtype) for _ in range(2))
     with _native.on_device(k.device):
         status = _native.load_library().taac_kv_cache_read(
             *_pool(cache, pages), k.data_ptr(), v.data_ptr(), _native.ptr(starts), int(starts is not None and starts.dtype == torch.int64),
@@ -200,7 +192,6 @@ def cached_attention(
     output is rounded once. A NaN or an infinity in a cached token reaches the queries that see it, and no others.
     Forward only."""
     name = "cached_attention"
-    _check_cache(name, cache)
     if q.ndim != 4:
         raise ValueError(f"{name} expects q with shape (batch, heads, tokens, width)")
     batch, heads, tokens, width = q.shape
@@ -216,7 +207,7 @@ def cached_attention(
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise RuntimeError(f"hip {name} does not support dtype {q.dtype}")
     q = _in_place(q, 2)
-    out = token_major(batch, heads, tokens, width, q)
+    out = token_major(q.shape, q)
     bytes_needed = _workspace_bytes(batch, heads, cache.heads, tokens, width, cache.bits, pages.shape[1] * cache.page_tokens if cache.pages > 0 else 0)
     workspace = q.new_empty(bytes_needed, dtype=torch.uint8) if bytes_needed > 0 else None
     with _native.on_device(q.device):
