@@ -11,6 +11,7 @@ from taac_2026_amd.modeling.backbone import (
     run_interaction_blocks,
     UnifiedSelfAttention,
 )
+from taac_2026_amd.modeling.cached import CachedAttention, CachedAttentionBlock
 from taac_2026_amd.modeling.embeddings import hash_compress_ids, sparse_embedding_bag_mean
 from taac_2026_amd.modeling.masks import (
     MetadataAttentionMask,
@@ -38,6 +39,8 @@ from taac_2026_amd.modeling.sequence import (
 
 __all__ = [
     "BFTSAttention",
+    "CachedAttention",
+    "CachedAttentionBlock",
     "FeedForward",
     "MixedFeedForward",
     "CandidateClsPooler",

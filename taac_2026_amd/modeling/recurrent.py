@@ -78,15 +78,13 @@ class GatedDeltaAttention(nn.Module):
         return self._leave(mixed, tokens.dtype)
 
 
-class GatedDeltaBlock(nn.Module):
-    """Pre-norm :class:`GatedDeltaAttention` and SwiGLU feed-forward with residuals; the first residual's addition and the norm in front
-    of the feed-forward are one pass. No valid row reads a padded one; what padded rows hold is not specified."""
+class PreNormBlock(nn.Module):
+    """A token mixer and a SwiGLU feed-forward behind norms, with residuals; the first residual's addition and the norm in front of the feed-forward are one pass."""
 
-    def __init__(self, d_model: int, num_heads: int, hidden_mult: int, *, key_heads: int | None = None, key_width: int | None = None,
-                 value_width: int | None = None) -> None:
+    def __init__(self, d_model: int, attention: nn.Module, hidden_mult: int) -> None:
         super().__init__()
         self.attn_norm = RMSNorm(d_model)
-        self.attention = GatedDeltaAttention(d_model, num_heads, key_heads=key_heads, key_width=key_width, value_width=value_width)
+        self.attention = attention
         self.ffn_norm = RMSNorm(d_model)
         self.ffn = SwiGLUFeedForward(d_model, hidden_mult)
 
@@ -105,6 +103,16 @@ class GatedDeltaBlock(nn.Module):
         hidden = linear_fp8(values, fp8_weights[0], row_amax, fp8_weights[1], self.ffn.up.bias.to(dtype), swiglu=True,
                             gate_first=self.ffn.gate_first)
         return linear(hidden, self.ffn.down.weight.to(dtype), self.ffn.down.bias.to(dtype), residual=summed)
+
+
+class GatedDeltaBlock(PreNormBlock):
+    """Pre-norm :class:`GatedDeltaAttention` and SwiGLU feed-forward with residuals; the first residual's addition and the norm in front
+    of the feed-forward are one pass. No valid row reads a padded one; what padded rows hold is not specified."""
+
+    def __init__(self, d_model: int, num_heads: int, hidden_mult: int, *, key_heads: int | None = None, key_width: int | None = None,
+                 value_width: int | None = None) -> None:
+        super().__init__(d_model, GatedDeltaAttention(d_model, num_heads, key_heads=key_heads, key_width=key_width, value_width=value_width),
+                         hidden_mult)
 
     def forward(self, tokens: torch.Tensor, *, key_lengths: torch.Tensor | None = None,
                 fp8_weights: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:

@@ -1,0 +1,202 @@
+"""CachedAttention and CachedAttentionBlock: norm, rotation, cache and attention run together, whole histories and event by event, against the same layers written
+out in 64 bits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from oracle import cached_attention as oracle
+from taac_2026_amd.api import CachedAttention, CachedAttentionBlock, kv_cache_read
+
+SIZES = [dict(d_model=64, num_heads=2), dict(d_model=128, num_heads=4, key_heads=2, head_dim=64, rotary_dim=32, interleaved=True),
+         dict(d_model=96, num_heads=3, key_heads=1, head_dim=128, rotary_options=dict(factor=4.0, trained_places=64))]
+
+
+def test_modules_refuse():
+    with pytest.raises(ValueError, match="multiple of the key heads"):
+        CachedAttention(128, 4, key_heads=3)
+    with pytest.raises(ValueError, match="32, 64, 128"):
+        CachedAttention(96, 2)
+    with pytest.raises(ValueError, match="even number"):
+        CachedAttention(64, 2, rotary_dim=0)
+    block = CachedAttentionBlock(64, 2, 2, max_tokens=8)
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        block(torch.zeros(1, 3, 64))
+    cache = block.attention.empty_cache(5, "cpu", bits=8, page_tokens=16)
+    assert (cache.pages, cache.heads, cache.head_dim, cache.page_tokens, cache.bits) == (5, 2, 32, 16, 8)
+    assert "attention.table" not in block.state_dict()
+
+
+def test_the_table_keeps_its_type():
+    """A model cast to bfloat16 still turns by angles of float32, whatever torch's default type."""
+    mixer = CachedAttention(64, 2, max_tokens=300)
+    want = mixer.table.clone()
+    assert want.dtype == torch.float32 and torch.equal(mixer.bfloat16().table, want) and mixer.query_weight.dtype == torch.bfloat16
+    kept = torch.get_default_dtype()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        assert torch.equal(CachedAttention(64, 2, max_tokens=300).table, want)
+    finally:
+        torch.set_default_dtype(kept)
+
+
+def _make(device, sizes, seed=0):
+    torch.manual_seed(seed)
+    block = CachedAttentionBlock(hidden_mult=2, **sizes).to(device)
+    with torch.no_grad():
+        for t in (block.attn_norm.weight, block.ffn_norm.weight, block.attention.query_weight, block.attention.key_weight):
+            t.add_(0.2 * torch.randn_like(t))
+    return block
+
+
+def _norm(x, weight):
+    return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6) * weight
+
+
+def _project(block, weights, tokens):
+    """q, k, v in 64 bits, of tokens that begin at position 0"""
+    mixer = block.attention
+    rows = _norm(tokens, weights["attn_norm.weight"]) @ weights["attention.inputs.weight"].T + weights["attention.inputs.bias"]
+    q, k, v = (t.transpose(1, 2) for t in rows.unflatten(-1, (-1, mixer.head_dim)).split((mixer.num_heads, mixer.key_heads, mixer.key_heads), 2))
+    rotary = 2 * mixer.table.shape[1]
+    frequency = 10000.0 ** (-torch.arange(0, rotary, 2, dtype=torch.float64, device=tokens.device) / rotary)
+    options = mixer._rotary[1]
+    if options:
+        kept = ((options["trained_places"] / (2 * torch.pi) * frequency - 1.0) / 31.0).clamp(0.0, 1.0)
+        frequency = frequency * (kept + (1.0 - kept) / options["factor"])
+    angles = (torch.arange(tokens.shape[1], dtype=torch.float64, device=tokens.device)[:, None] * frequency)[None]
+    q = oracle.head_norm_rope(q, weights["attention.query_weight"], angles, interleaved=mixer.interleaved)
+    return q, oracle.head_norm_rope(k, weights["attention.key_weight"], angles, interleaved=mixer.interleaved), v
+
+
+def _finish(weights, tokens, mixed):
+    dense = lambda name, x: x @ weights[name + ".weight"].T + weights[name + ".bias"]  # noqa: E731
+    summed = tokens + dense("attention.out", mixed.transpose(1, 2).flatten(2))
+    gate, value = dense("ffn.up", _norm(summed, weights["ffn_norm.weight"])).chunk(2, -1)
+    return summed + dense("ffn.down", F.silu(gate) * value)
+
+
+def _plain(block, weights, tokens, lengths):
+    q, k, v = _project(block, weights, tokens)
+    count = tokens.shape[1]
+    seen = torch.ones(count, count, dtype=torch.bool, device=tokens.device).tril() & (torch.arange(count, device=tokens.device) < lengths[:, None, None])
+    return _finish(weights, tokens, oracle.attention(q, k, v, seen)[0])
+
+
+def _weights(block):
+    return {name: t.detach().double().requires_grad_(True) for name, t in block.named_parameters()}
+
+
+# A row passes at most sixteen roundings to bf16 on its way (tokens and normed rows, projections and their weights, queries and keys, the attention's
+# probabilities and outputs, the sum), each off by at most 2^-8 of its row, and random projections carry errors as they carry values. Scores are of order one: queries
+# and keys have unit variance, so that an error of a score of a few roundings is a relative one of a probability.
+FORWARD = 16 * 2.0**-8
+
+
+@pytest.mark.gpu
+def test_wide_heads_are_not_trained(device):
+    """The backward of attention over whole histories is built for heads of at most 64 features."""
+    block = _make(device, SIZES[2])
+    with pytest.raises(RuntimeError, match="at most 64"):
+        block(torch.randn(1, 5, 96, device=device)).float().sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", SIZES[:2] + [dict(SIZES[2], head_dim=64)])
+def test_block_forward_and_gradients(device, sizes):
+    block = _make(device, sizes)
+    generator = torch.Generator().manual_seed(1)
+    tokens = torch.randn(5, 90, sizes["d_model"], generator=generator).bfloat16().to(device)
+    lengths = torch.tensor([90, 1, 0, 64, 77], device=device)
+    live = (torch.arange(90, device=device) < lengths[:, None])[..., None]
+    grad_out = torch.randn(tokens.shape, generator=generator).bfloat16().to(device) * live
+    leaf = tokens.clone().requires_grad_(True)
+    out = block(leaf, key_lengths=lengths)
+    got = dict(zip(["tokens", *dict(block.named_parameters())], torch.autograd.grad(out, [leaf, *block.parameters()], grad_out)))
+    weights = _weights(block)
+    plain_leaf = tokens.double().requires_grad_(True)
+    want = _plain(block, weights, plain_leaf, lengths)
+    assert ((out.double() - want) * live).norm() <= FORWARD * (want * live).norm()
+    # the backward rounds as often again; a parameter's gradient adds up samples whose signs differ: errors are those of the sum of sizes
+    parts = [torch.autograd.grad((want[b] * grad_out[b]).sum(), [plain_leaf, *weights.values()], retain_graph=True) for b in range(5)]
+    for i, name in enumerate(["tokens", *weights]):
+        total, size = sum(p[i] for p in parts), sum(p[i].abs() for p in parts)
+        assert torch.isfinite(got[name]).all(), name
+        assert (got[name].double() - total).norm() <= 2 * FORWARD * size.norm(), (name, (got[name].double() - total).norm() / size.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", SIZES)
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prefill_then_steps(device, sizes, bits):
+    """Histories of their own lengths, then a few events and single ones: what the cache holds is what was projected, to half a step, and the rows of the new events
+    are attention over what it holds."""
+    block = _make(device, sizes, seed=2)
+    mixer = block.attention
+    generator = torch.Generator().manual_seed(3)
+    tokens = torch.randn(4, 75, sizes["d_model"], generator=generator).bfloat16().to(device)
+    first = torch.tensor([70, 33, 0, 16], device=device, dtype=torch.int32)
+    cache = mixer.empty_cache(30, device, bits=bits, page_tokens=16)
+    pages = torch.randperm(30, generator=generator)[:20].view(4, 5).to(device)
+    count = torch.arange(75, device=device)
+    with torch.no_grad():
+        history = block.prefill(tokens[:, :70], cache, pages, key_lengths=first)
+        new = torch.tensor([1, 3, 3, 2], device=device, dtype=torch.int32)
+        at = (first[:, None] + count[:3]).long()[..., None].expand(-1, -1, tokens.shape[2])
+        few = block.step(tokens.gather(1, at), cache, pages, first, key_lengths=new)
+        second = first + new
+        one_at = second[:, None].long()[..., None].expand(-1, -1, tokens.shape[2])
+        one = block.step(tokens.gather(1, one_at), cache, pages, second)
+        weights = {name: t.detach() for name, t in _weights(block).items()}
+        want = _plain(block, weights, tokens[:, :70].double(), first)
+        live = (count[:70] < first[:, None])[..., None]
+        assert ((history.double() - want) * live).norm() <= FORWARD * (want * live).norm()
+        q, k, v = _project(block, weights, tokens.double())
+        held_k, held_v = (t.double() for t in kv_cache_read(cache, pages, None, 75, lengths=second + 1, dtype=torch.float32))
+        there = (count < (second + 1)[:, None])[:, None, :, None]
+        for held, exact in ((held_k, k), (held_v, v)):
+            # half of a step, 1/5 or 1/17 of the block's largest (a seventh of 7, a 29th of 464 at the top of the range), behind a few roundings of the block to bf16
+            top = exact.unflatten(-1, (-1, 32)).abs().amax(-1, keepdim=True).expand(*exact.shape[:3], -1, 32).flatten(-2)
+            assert ((held - exact).abs() * there <= top * (1 / 5 if bits == 4 else 1 / 17) * (1 + FORWARD) + FORWARD * top.amax()).all()
+        for got, start, news in ((few, first, new), (one, second, torch.ones_like(new))):
+            tokens_of = at if got is few else one_at
+            mine = tokens.double().gather(1, tokens_of)
+            rows = tokens_of[:, None, :, :1].expand(-1, mixer.num_heads, -1, mixer.head_dim)
+            seen = oracle.visible(start + news, news, got.shape[1], 75)
+            expected = _finish(weights, mine, oracle.attention(q.gather(2, rows), held_k, held_v, seen)[0])
+            valid = (count[: got.shape[1]] < news[:, None])[..., None]
+            assert ((got.double() - expected) * valid).norm() <= FORWARD * (expected * valid).norm()
+
+
+@pytest.mark.gpu
+def test_step_in_a_replayed_graph(device):
+    block = _make(device, SIZES[1], seed=4)
+    mixer = block.attention
+    cache, other = (mixer.empty_cache(8, device, page_tokens=32) for _ in range(2))
+    pages = torch.tensor([[3, 1], [-1, -1], [6, 2]], device=device)  # the second sample is padding
+    tokens, starts = torch.randn(3, 1, 128, device=device).bfloat16(), torch.zeros(3, device=device, dtype=torch.int32)
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            block.step(tokens, cache, pages, starts)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = block.step(tokens, cache, pages, starts)
+        cache.data.zero_()
+        for t in range(40):
+            tokens.copy_(torch.randn(3, 1, 128, device=device))
+            starts.fill_(t)
+            graph.replay()
+            torch.cuda.synchronize()
+            want = block.step(tokens, other, pages, starts)
+            assert torch.equal(out, want) and torch.equal(cache.data, other.data)
+
+
+def test_positions_behind_the_table():
+    with pytest.raises(ValueError, match="positions for 8 tokens"):
+        CachedAttention(64, 2, max_tokens=8)._attend(torch.zeros(1, 2, 9, 32), torch.zeros(1, 2, 9, 32), torch.zeros(1, 2, 9, 32), None)
