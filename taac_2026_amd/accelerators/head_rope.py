@@ -18,6 +18,7 @@ from taac_2026_amd import _native
 from taac_2026_amd.accelerators.tensor_validation import require_cuda_tensors, require_inference, require_same_dtype
 
 MAX_HEAD_WIDTH = 512
+MAX_COUNT = 2**31 - 1  # the library counts samples and tokens in 32 bits
 _Strides3 = ctypes.c_int64 * 3
 _Strides2 = ctypes.c_int64 * 2
 
@@ -203,8 +204,8 @@ def head_norm_rope(
     require_cuda_tensors(f"hip {name}", q, k, query_weight, key_weight, table, place)
     if q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise RuntimeError(f"hip {name} does not support dtype {q.dtype}")
-    if width > MAX_HEAD_WIDTH:
-        raise RuntimeError(f"hip {name} is built for heads of at most {MAX_HEAD_WIDTH} features")
+    if width > MAX_HEAD_WIDTH or batch > MAX_COUNT or tokens > MAX_COUNT:
+        raise RuntimeError(f"hip {name} is built for heads of at most {MAX_HEAD_WIDTH} features, samples and tokens of at most 2^31 - 1")
     if table is not None and table.requires_grad:
         require_inference(f"hip {name} table", table)
     if query_weight is not None:

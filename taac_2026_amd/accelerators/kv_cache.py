@@ -14,7 +14,7 @@ from dataclasses import dataclass, field
 import torch
 
 from taac_2026_amd import _native
-from taac_2026_amd.accelerators.head_rope import strides_of, token_major
+from taac_2026_amd.accelerators.head_rope import MAX_COUNT, strides_of, token_major
 from taac_2026_amd.accelerators.tensor_validation import require_cuda_tensors, require_inference, require_same_dtype
 
 CACHED_WIDTHS = (32, 64, 128)
@@ -27,7 +27,7 @@ def _record_bytes(head_dim: int, bits: int) -> int:
     return _native.load_library().taac_kv_cache_bytes(1, 1, _CHUNK, head_dim, bits)
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class KVCache:
     """A pool of pages (:func:`empty_kv_cache`). ``data``: uint8 (pages, heads, page_tokens / 16, bytes of 16 tokens), the library's own layout."""
 
@@ -66,6 +66,11 @@ def _check_pages(name: str, pages: torch.Tensor, batch: int) -> None:
         raise ValueError(f"{name} expects a table of pages (batch, pages of a sample) in int32 or int64")
     if pages.stride(1) != 1 and pages.shape[1] > 1:
         raise ValueError(f"{name} expects a table whose rows are contiguous")
+
+
+def _check_counts(name: str, batch: int, tokens: int, pages: torch.Tensor) -> None:
+    if batch > MAX_COUNT or tokens > MAX_COUNT or pages.shape[1] > MAX_COUNT:
+        raise RuntimeError(f"hip {name} is built for samples, tokens and pages of a sample of at most 2^31 - 1")
 
 
 def _integers(name: str, what: str, t: torch.Tensor, batch: int) -> torch.Tensor:
@@ -124,6 +129,7 @@ def kv_cache_write(
     require_inference(f"hip {name}", k, v)
     if k.dtype not in _DTYPES:
         raise RuntimeError(f"hip {name} does not support dtype {k.dtype}")
+    _check_counts(name, batch, tokens, pages)
     size = k.element_size()
     k, v = _in_place(k, size), _in_place(v, size)
     with _native.on_device(k.device):
@@ -156,6 +162,7 @@ def kv_cache_read(
     require_cuda_tensors(f"hip {name}", cache.data, pages, starts, lengths)
     if dtype not in _DTYPES:
         raise RuntimeError(f"hip {name} does not support dtype {dtype}")
+    _check_counts(name, batch, int(tokens), pages)
     k, v = (token_major((batch, cache.heads, int(tokens), cache.head_dim), cache.data, dtype) for _ in range(2))
     with _native.on_device(k.device):
         status = _native.load_library().taac_kv_cache_read(
@@ -206,6 +213,7 @@ def cached_attention(
     require_inference(f"hip {name}", q)
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise RuntimeError(f"hip {name} does not support dtype {q.dtype}")
+    _check_counts(name, batch, tokens, pages)
     q = _in_place(q, 2)
     out = token_major(q.shape, q)
     bytes_needed = _workspace_bytes(batch, heads, cache.heads, tokens, width, cache.bits, pages.shape[1] * cache.page_tokens if cache.pages > 0 else 0)

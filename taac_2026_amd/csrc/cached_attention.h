@@ -4,8 +4,8 @@
 //
 // The new tokens of a sample are the last of its cached ones. Queries of the heads that share a key head are rows of one product.
 //
-// Bound by HBM: every code is read once per key head. A wavefront walks tiles of 64 tokens, one tile ahead in registers, with the running maximum and sum
-// of a softmax; the wavefronts of a workgroup take the tiles in turn and meet at its end; long histories of few heads are split over workgroups, whose parts
+// Bound by HBM: every code is read once per key head. A wavefront walks tiles of 64 tokens, which come into LDS without registers, with the running maximum and sum of a
+// softmax; the wavefronts of a workgroup take the tiles in turn and meet at its end; long histories of few heads are split over workgroups, whose parts
 // a second kernel joins. Codes become bf16 operands by the conversion instructions, two values an issue, scales included.
 //
 // Two forms, lane = (l16 = lane % 16, grp = lane / 16):
@@ -18,6 +18,11 @@
 // Precision: all operands are bf16, exact for keys and values of either size, whatever their scales, and for queries (fp16 ones in two parts); scores, statistics
 // and sums are fp32; probabilities enter as two parts (16 bits), in the first form in columns that would be empty. The maximum moves when a score exceeds it
 // by a factor of 2^8, which cancels.
+//
+// Measured: 4 samples of 65536 tokens, 32 heads over 8 of 128 features in 4 bits: 51 us and 5 for the join, 5.6 TB/s of the cache (tiles in registers, one ahead: 101, for the
+// registers left one wavefront to a SIMD, and page numbers that wait behind the rows). 1024 samples of up to 512 tokens, 8 heads of 32: 21 us, of which 9 are a launch whose
+// samples have one tile, and 2.7 every tile more, 6.7 TB/s. 64 samples of up to 2048 tokens, 24 queries of 8 heads over 4 of 128 in 8 bits: 37 us, matrix and vector
+// instructions side by side (a tile of 32 rows has 104 and 600, of which 270 convert the codes).
 #pragma once
 
 #include "kv_cache.h"
@@ -49,6 +54,7 @@ struct AttendParams {
   int64_t all_rows;              // B * heads * T
   Divisor group, splits, row_tiles, heads;
   int32_t H, T, rows, window;
+  int32_t first;                 // sample of the launch
   float scale;                   // times log2 e: powers of two; its size
   uint32_t flip, keep;           // its sign, which the queries take, of two of their elements; nothing of them where it is zero (scale is one then)
 };
@@ -230,6 +236,7 @@ struct Job {
     row0 = (id - over * p.row_tiles.d) * rows;
     b = p.heads.over(over);
     head = over - b * p.heads.d;
+    b += p.first;
   }
 };
 

@@ -67,30 +67,42 @@ __global__ __launch_bounds__(256) void cached_attention_join_kernel(const Attend
 
 // ---- the host -----------------------------------------------------------------------------------------------------
 
-#ifndef KALONE
-#define KALONE 2048
-#endif
+constexpr int64_t kMostGroups = 1 << 23;  // of a launch: below 2^31 threads
 
+// How a call is cut. A unit is a tile of rows of a key head of a sample.
 struct Plan {
-  int rows, row_tiles, splits, waves;
+  int rows;       // of a tile: 1, 2, 4, 16 or 32
+  int row_tiles;  // of a key head
+  int splits;     // of a history
+  int waves;      // of a workgroup
   bool alone;
-  uint32_t groups;
 };
+
+// From so many units on a wavefront takes one alone, without the meeting; below, four share its tokens. Medians of ragged histories, alone : shared, in us:
+//   up to 4 rows, 32 features: 9.2 : 14.0 at 4096 units of up to 256 tokens, 22.4 : 24.5 of 1024; 11.0 : 8.8 and 18.3 : 14.9 at 2048
+//   64 features: 9.3 : 15.0 at 2048 units of 256, 22.7 : 25.3 of 1024; 10.7 : 9.5 and 17.7 : 16.6 at 1024; 128 alike
+//   16 rows, 64 features: 27.9 : 36.2 at 8192 units of 256, 42.8 : 46.4 of 512; 17.7 : 21.0 of 256 and 46.6 : 38.9 of 1024 at 4096
+int64_t alone_from(int rows, int32_t d) { return rows > 4 ? 8192 : d == 32 ? 4096 : 2048; }
+
 Plan plan_of(int64_t B, int32_t heads, int32_t group, int32_t T, int32_t d, int bits, int64_t held, bool parts) {
   Plan plan{};
   const int64_t rows = static_cast<int64_t>(group) * T;
+  // up to 4 rows (2 in two parts) in the one form. In the other 16, or 32, which share the conversion of the codes: three sixteens would leave one wavefront to a SIMD, and four
+  // no registers.
   plan.rows = rows <= 2 ? static_cast<int>(rows) : rows <= 4 && !parts ? 4 : rows <= 16 ? 16 : 32;
   plan.row_tiles = static_cast<int>((rows + plan.rows - 1) / (plan.rows > 0 ? plan.rows : 1));
   const int64_t units = B * heads * plan.row_tiles;
-  plan.alone = units >= KALONE && plan.rows <= 16;
+  plan.alone = plan.rows <= 16 && units >= alone_from(plan.rows, d);
   const Shape shape = shape_of(plan.rows, d, plan.alone);
   plan.waves = shape.waves;
-  // as many as the card holds at once, by LDS and registers
+  // Histories are split until the card is full, by LDS and registers; twice as many workgroups cost more than a better balance gives back (4 x 8 key heads of 128 features,
+  // 65536 tokens: 56 us, 60 with twice as many; 64 x 4 x 2048 tokens, 24 queries: 39 and 52). A split has a tile for each of its wavefronts, and below four (six
+  // of narrower heads) the kernel that joins them takes longer than the tiles would: one sample of 768 tokens 5.7 us as a whole, of 1024 in four 7.9.
   const int by_lds = 163840 / lds_bytes(plan.rows, d, bits, plan.alone), by_registers = 4 * shape.per_simd / shape.waves;
   const int64_t resident = 256 * (by_lds < by_registers ? by_lds : by_registers), most = held / (kTile * shape.waves);
   int64_t splits = resident / (units > 0 ? units : 1);
   splits = splits < most ? splits : most;
-  plan.splits = static_cast<int>(most < 4 || splits < 1 ? 1 : splits);
+  plan.splits = static_cast<int>(most < (d == 128 ? 4 : 6) || splits < 1 ? 1 : splits);
   return plan;
 }
 
@@ -140,9 +152,8 @@ extern "C" int taac_cached_attention_fwd(const void* q, void* o, const void* cac
   if (held > int64_t{1} << 30) return set_error(TAAC_ERR_UNSUPPORTED, "%s: at most 2^30 tokens to a sample", name);
   if (static_cast<int64_t>(group) * T > 1 << 24) return set_error(TAAC_ERR_UNSUPPORTED, "%s: too many queries to a key head", name);
   Plan plan = plan_of(B, heads, group, T, d, bits, held, dtype == TAAC_F16);
-  const int64_t groups = static_cast<int64_t>(B) * heads * plan.row_tiles * plan.splits;
-  if (groups > 1 << 23) return set_error(TAAC_ERR_UNSUPPORTED, "%s: too many workgroups", name);
-  plan.groups = static_cast<uint32_t>(groups);
+  const int64_t each = static_cast<int64_t>(heads) * plan.row_tiles * plan.splits, at_once = kMostGroups / each;  // workgroups of a sample, samples of a launch
+  if (at_once < 1) return set_error(TAAC_ERR_UNSUPPORTED, "%s: too many workgroups to a sample", name);
   p.all_rows = static_cast<int64_t>(B) * H * T;
   const int64_t need = plan.splits > 1 ? p.all_rows * plan.splits * (d + 2) * 4 : 0;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
@@ -156,7 +167,11 @@ extern "C" int taac_cached_attention_fwd(const void* q, void* o, const void* cac
   p.flip = scale < 0.f ? 0x80008000u : 0u;
   const bool f16 = dtype == TAAC_F16;
   hipStream_t s = as_stream(stream);
-  bits == 4 ? attend_4(p, d, f16, plan.rows, plan.alone, plan.groups, s) : attend_8(p, d, f16, plan.rows, plan.alone, plan.groups, s);
+  for (int64_t first = 0; first < B; first += at_once) {
+    p.first = static_cast<int32_t>(first);
+    const uint32_t groups = static_cast<uint32_t>((B - first < at_once ? B - first : at_once) * each);
+    bits == 4 ? attend_4(p, d, f16, plan.rows, plan.alone, groups, s) : attend_8(p, d, f16, plan.rows, plan.alone, groups, s);
+  }
   if (plan.splits > 1) f16 ? launch_join<f16_t>(p, plan, d, s) : launch_join<bf16_t>(p, plan, d, s);
   return check_launch(name);
 }

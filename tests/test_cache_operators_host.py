@@ -137,6 +137,12 @@ def test_cached_attention_refuses():
         cached_attention(q, cache, pages, lengths)
 
 
+def test_a_cache_is_itself():
+    """Compared and hashed as one object, not by its tensor."""
+    a, b = (empty_kv_cache(1, 1, 32, device="cpu") for _ in range(2))
+    assert a == a and a != b and len({a, b, a}) == 2
+
+
 def test_rope_entry_points_check_on_the_host():
     library = _native.load_library()
     fake = ctypes.c_void_p(256)
@@ -212,7 +218,8 @@ def test_cache_entry_points_check_on_the_host():
     assert attend(qs=None) == invalid and attend(qs=strides(128, 36, 128)) == invalid and attend(os=strides(128, 34, 128)) == invalid
     assert attend(q=None) == invalid and attend(o=None) == invalid and attend(lengths=None) == invalid and attend(q=odd) == invalid and attend(o=ctypes.c_void_p(260)) == invalid
     assert attend(table_pages=1 << 27) == unsupported and b"2^30" in library.taac_last_error()
-    assert attend(H=1 << 21, T=32) == unsupported and attend(B=1 << 23) == unsupported
+    assert attend(H=1 << 21, T=32) == unsupported and b"queries" in library.taac_last_error()
+    assert attend(heads=1 << 16, H=1 << 16, T=1 << 13) == unsupported and b"workgroups" in library.taac_last_error()
     assert attend(B=0) == ok and attend(T=0) == ok
     need = library.taac_cached_attention_workspace_bytes(1, 4, 2, 1, 32, 4, 1 << 16)
     assert need > 0 and attend(table_pages=1 << 12, ws=fake, bytes=need - 1) == invalid and b"workspace" in library.taac_last_error()

@@ -234,6 +234,20 @@ def test_a_pool_beyond_32_bits(device):
         _check(got, q, oracle.cached_values(k, 8), oracle.cached_values(v, 8), [1000], [tokens])
 
 
+def test_more_workgroups_than_a_launch_has(device):
+    """2^23 + 2^12 workgroups of a row each: two launches."""
+    samples = (1 << 23) // 8 + 512
+    cache = empty_kv_cache(3, 8, 32, page_tokens=16, device=device)
+    k, v = (torch.randn(3, 8, 16, 32, generator=torch.Generator().manual_seed(seed)).bfloat16().to(device) for seed in (1, 2))
+    kv_cache_write(cache, k, v, torch.arange(3, device=device)[:, None])
+    which = torch.randint(0, 3, (samples,), generator=torch.Generator().manual_seed(3)).to(device)
+    q = torch.randn(3, 8, 1, 32, generator=torch.Generator().manual_seed(4)).bfloat16().to(device)
+    lengths = torch.tensor([16, 5, 1], device=device, dtype=torch.int32)
+    want = cached_attention(q, cache, torch.arange(3, device=device)[:, None], lengths)
+    got = cached_attention(q[which], cache, which[:, None], lengths[which])
+    assert torch.equal(got, want[which])
+
+
 def test_same_bits_again_and_on_another_stream(device):
     cache, pages, _, _ = _filled(device, [9000, 300], 2, 64, 4, 64)
     lengths = torch.tensor([9000, 300], device=device)
@@ -247,21 +261,22 @@ def test_same_bits_again_and_on_another_stream(device):
     assert all(torch.equal(want, x) for x in got)
 
 
-def test_a_history_event_by_event(device):
+@pytest.mark.parametrize("width,bits", [(64, 4), (128, 8)])
+def test_a_history_event_by_event(device, width, bits):
     """Norm and rotation, write, attention, an event at a time, in a replayed graph: the rows of causal attention over the whole history, whose keys and values are the
     cache's."""
     g = torch.Generator().manual_seed(4)
-    batch, heads, kv_heads, width, total = 3, 4, 2, 64, 70
+    batch, heads, kv_heads, total = 3, 4, 2, 70
     rows = torch.randn(batch, total, (heads + 2 * kv_heads) * width, generator=g).bfloat16().to(device)
     weights = [(1 + 0.2 * torch.randn(width, generator=g)).bfloat16().to(device) for _ in range(2)]
     table = rotary_table(128, 32, device=device)
     split = lambda x: [t.transpose(1, 2) for t in x.unflatten(-1, (-1, width)).split((heads, kv_heads, kv_heads), 2)]  # noqa: E731
     q, k, v = split(rows)
     q, k = head_norm_rope(q, k, *weights, table=table)
-    keys, values = (oracle.cached_values(x, 4).bfloat16() for x in (k, v))
+    keys, values = (oracle.cached_values(x, bits).bfloat16() for x in (k, v))
     whole = flash_attention(q, keys.repeat_interleave(2, 1), values.repeat_interleave(2, 1), is_causal=True)
 
-    cache = empty_kv_cache(12, kv_heads, width, page_tokens=32, device=device)
+    cache = empty_kv_cache(12, kv_heads, width, bits=bits, page_tokens=32, device=device)
     pages = torch.randperm(12, generator=g)[:9].view(batch, 3).to(device)
     event, starts, lengths = rows[:, :1].clone(), torch.zeros(batch, device=device, dtype=torch.int32), torch.zeros(batch, device=device, dtype=torch.int32)
 
