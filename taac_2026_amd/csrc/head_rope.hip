@@ -29,7 +29,7 @@ struct RopeParams {
   int64_t xs[2][3], gs[2][3], ys[2][3];  // element strides of (batch, head, token)
   const float* table;     // [places][rotary / 2][2] or null
   const void* positions;  // null: the position is the token's number
-  int64_t ps[2];
+  int64_t ps[2];          // of (sample, token), words of 32 bits
   int64_t places;
   int32_t H[2], B, T, d, rotary;
   int32_t pos_int64, add_token;
@@ -178,81 +178,96 @@ __device__ __forceinline__ void store_row(T* row, const Lane<L, VEC, INTER>& lan
   }
 }
 
-// The tokens that a lane's row slot walks: `head` heads of a token side by side in a wavefront, tokens a constant distance apart.
+// The tokens that a lane's row slot walks: heads of a token side by side in a wavefront, tokens a constant distance apart. Addresses move by a constant too, another one
+// where the walk passes a sample's last token: a row costs no product and no division.
 struct Walk {
-  int which, h, t, step_t;
+  int which, h, t, step_t, left;  // left: tokens that are still to come, this one among them
   int64_t b, step_b;
-  bool there;
-  // slots: rows of a wavefront; chunk: of a token's heads, where they need several wavefronts
+  // slots: rows of a wavefront, of blockIdx.y's part of a token's heads where they need several wavefronts
   __device__ __forceinline__ Walk(const RopeParams& p, int slots, int slot) {
     const int heads = p.H[0] + p.H[1], side = heads < slots ? heads : slots;  // heads of a token in a wavefront
     const int at_once = slots / side;                                         // tokens of a wavefront
     const int head = static_cast<int>(blockIdx.y) * slots + slot % side, of = slot / side;
-    there = of < at_once && head < heads;
     which = head >= p.H[0];
     h = head - (which ? p.H[0] : 0);
     const int64_t wave = static_cast<int64_t>(blockIdx.x) * (kBlock / kWave) + threadIdx.x / kWave, token = wave * at_once + of;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (kBlock / kWave) * at_once;
-    if (token < 0x7fffffff && step < 0x7fffffff) {  // for all lanes alike but behind two billion tokens: a fifth of the instructions
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kBlock / kWave) * at_once, tokens = static_cast<int64_t>(p.B) * p.T;
+    if (tokens < 0x7fffffff && step < 0x7fffffff) {  // the same for all: a fifth of the instructions
       const uint32_t T = p.T;
       b = static_cast<uint32_t>(token) / T, step_b = static_cast<uint32_t>(step) / T;
+      left = token < tokens ? static_cast<int>((static_cast<uint32_t>(tokens - token) + static_cast<uint32_t>(step) - 1) / static_cast<uint32_t>(step)) : 0;
     } else {
       b = token / p.T, step_b = step / p.T;
+      left = token < tokens ? static_cast<int>((tokens - token + step - 1) / step) : 0;
     }
+    if (of >= at_once || head >= heads) left = 0;
     t = static_cast<int>(token - b * p.T), step_t = static_cast<int>(step - step_b * p.T);
   }
-  __device__ __forceinline__ void next(const RopeParams& p) {
-    b += step_b, t += step_t;
-    if (t >= p.T) t -= p.T, ++b;
-  }
-  __device__ __forceinline__ int64_t offset(const int64_t (&s)[2][3]) const {
-    const int64_t *q = s[0], *k = s[1];
-    return b * (which ? k[0] : q[0]) + h * (which ? k[1] : q[1]) + t * (which ? k[2] : q[2]);
+  // to the next token; whether that is behind the end of a sample more than step_b behind
+  __device__ __forceinline__ bool next(const RopeParams& p) {
+    --left;
+    t += step_t;
+    const bool wraps = t >= p.T;
+    t -= wraps ? p.T : 0;
+    return wraps;
   }
 };
+// The address of a walk's token in an array with strides of (sample, token), in elements of E.
+template <typename E>
+struct Cursor {
+  E* p;
+  int64_t plain, wrapped;  // elements to the next token
+  __device__ __forceinline__ Cursor(E* base, const Walk& at, int T, int64_t sample, int64_t token) {
+    p = base + at.b * sample + at.t * token;
+    plain = at.step_b * sample + at.step_t * token;
+    wrapped = plain + sample - T * token;
+  }
+  __device__ __forceinline__ void next(bool wraps) { p += wraps ? wrapped : plain; }
+};
+#define TAAC_ROWS(E, base, st) \
+  Cursor<E>(static_cast<E*>(at.which ? base[1] : base[0]) + at.h * (at.which ? st[1][1] : st[0][1]), at, p.T, at.which ? st[1][0] : st[0][0], at.which ? st[1][2] : st[0][2])
 
 // (c, s) of the lane's pairs; a position outside the table makes them NaN.
 struct Angles {
   float c[4], s[4];
   bool inside;
+  // without a branch, which would await what was asked for before it
   template <int L, int VEC, bool INTER>
-  __device__ __forceinline__ void load(const RopeParams& p, const Walk& at, const Lane<L, VEC, INTER>& lane) {
+  __device__ __forceinline__ void load(const RopeParams& p, const Walk& at, const Cursor<const int32_t>& place, const Lane<L, VEC, INTER>& lane) {
     if (p.table == nullptr) return;
     int64_t position = at.t;
     if (p.positions != nullptr) {
-      const int64_t i = at.b * p.ps[0] + at.t * p.ps[1];
-      position = p.pos_int64 ? static_cast<const int64_t*>(p.positions)[i] : static_cast<const int32_t*>(p.positions)[i];
+      position = p.pos_int64 ? *reinterpret_cast<const int64_t*>(place.p) : *place.p;
       if (p.add_token) position += at.t;
     }
     inside = position >= 0 && position < p.places;
-    const float* row = p.table + (inside ? position : 0) * p.rotary;
     if (p.places == 0) return;
+    const float* row = p.table + static_cast<uint64_t>(inside ? static_cast<uint32_t>(position) : 0u) * static_cast<uint32_t>(p.rotary);
     if constexpr (VEC != kSingles) {
-      f32x4 lo = {}, hi = {};
-      if (lane.pair[0] >= 0) {
-        lo = *reinterpret_cast<const f32x4*>(row + 2 * lane.pair[0]);
-        hi = *reinterpret_cast<const f32x4*>(row + 2 * lane.pair[0] + 4);
-      }
+      row += 2 * max(lane.pair[0], 0);
+      const f32x4 lo = reinterpret_cast<const f32x4*>(row)[0], hi = reinterpret_cast<const f32x4*>(row)[1];
       c[0] = lo[0], s[0] = lo[1], c[1] = lo[2], s[1] = lo[3], c[2] = hi[0], s[2] = hi[1], c[3] = hi[2], s[3] = hi[3];
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        c[e] = lane.pair[e] >= 0 ? row[2 * lane.pair[e]] : 0.f;
-        s[e] = lane.pair[e] >= 0 ? row[2 * lane.pair[e] + 1] : 0.f;
+        c[e] = row[2 * max(lane.pair[e], 0)];
+        s[e] = row[2 * max(lane.pair[e], 0) + 1];
       }
     }
   }
-  // sign 1: by the angles, -1: back
-  template <int L, int VEC, bool INTER>
-  __device__ __forceinline__ void turn(const RopeParams& p, const Lane<L, VEC, INTER>& lane, float sign, float (&v)[8]) const {
-    if (p.table == nullptr) return;
+  template <bool BACK, int L, int VEC, bool INTER>
+  __device__ __forceinline__ void turn(const RopeParams& p, const Lane<L, VEC, INTER>& lane, float (&v)[8]) {
+    if (p.table == nullptr || (VEC != kSingles && lane.pair[0] < 0)) return;  // of runs all pairs are turned or none
+    if (!inside) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[e] = s[e] = __builtin_nanf("");
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float a = v[2 * e], b = v[2 * e + 1], cs = inside ? c[e] : __builtin_nanf(""), sn = inside ? sign * s[e] : __builtin_nanf("");
-      if (lane.pair[e] >= 0) {
-        v[2 * e] = fmaf(a, cs, -(b * sn));
-        v[2 * e + 1] = fmaf(a, sn, b * cs);
-      }
+      if (VEC == kSingles && lane.pair[e] < 0) continue;
+      const float a = v[2 * e], b = v[2 * e + 1];
+      v[2 * e] = BACK ? fmaf(a, c[e], b * s[e]) : fmaf(a, c[e], -(b * s[e]));
+      v[2 * e + 1] = BACK ? fmaf(b, c[e], -(a * s[e])) : fmaf(b, c[e], a * s[e]);
     }
   }
 };
@@ -268,23 +283,22 @@ __global__ __launch_bounds__(kBlock) void head_norm_rope_kernel(const RopeParams
     next.load(static_cast<const T*>(at.which ? p.w[1] : p.w[0]), lane);
     next.get(lane, w);
   }
-  const T* const x = static_cast<const T*>(at.which ? p.x[1] : p.x[0]);
-  T* const y = static_cast<T*>(at.which ? p.y[1] : p.y[0]);
-  if (!at.there) return;
+  if (at.left == 0) return;
+  Cursor<const T> x = TAAC_ROWS(const T, p.x, p.xs);
+  Cursor<T> y = TAAC_ROWS(T, p.y, p.ys);
+  Cursor<const int32_t> place(static_cast<const int32_t*>(p.positions), at, p.T, p.ps[0], p.ps[1]);
   Angles angles;
-  if (at.b < p.B) {
-    next.load(x + at.offset(p.xs), lane);
-    angles.load(p, at, lane);
-  }
-  while (at.b < p.B) {
+  next.load(x.p, lane);
+  angles.load(p, at, place, lane);
+  while (true) {
     float v[8];
     next.get(lane, v);
-    const Angles now = angles;
-    T* const to = y + at.offset(p.ys);
-    at.next(p);
-    if (at.b < p.B) {
-      next.load(x + at.offset(p.xs), lane);
-      angles.load(p, at, lane);
+    Angles now = angles;
+    const bool wraps = at.next(p);
+    if (at.left > 0) {
+      x.next(wraps), place.next(wraps);
+      next.load(x.p, lane);
+      angles.load(p, at, place, lane);
     }
     if (norm) {
       float sum = 0.f;
@@ -294,8 +308,10 @@ __global__ __launch_bounds__(kBlock) void head_norm_rope_kernel(const RopeParams
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= rstd * w[i];
     }
-    now.turn(p, lane, 1.f, v);
-    store_row<T, L, VEC, INTER>(to, lane, v);
+    now.template turn<false>(p, lane, v);
+    store_row<T, L, VEC, INTER>(y.p, lane, v);
+    if (at.left == 0) return;
+    y.next(wraps);
   }
 }
 
@@ -313,45 +329,47 @@ __global__ __launch_bounds__(kBlock) void head_norm_rope_bwd_kernel(const RopePa
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) dw[0][i] = dw[1][i] = 0.f;
-  const T* const x = static_cast<const T*>(at.which ? p.x[1] : p.x[0]);
-  const T* const dy = static_cast<const T*>(at.which ? p.g[1] : p.g[0]);
-  T* const dx = static_cast<T*>(at.which ? p.y[1] : p.y[0]);
-  Angles angles;
-  if (at.there && at.b < p.B) {
-    next_g.load(dy + at.offset(p.gs), lane);
-    if (norm) next.load(x + at.offset(p.xs), lane);
-    angles.load(p, at, lane);
-  }
-  while (at.there && at.b < p.B) {
-    float g[8], u[8];
-    next_g.get(lane, g);
-    if (norm) next.get(lane, u);
-    const Angles now = angles;
-    T* const to = dx + at.offset(p.ys);
-    at.next(p);
-    if (at.b < p.B) {
-      next_g.load(dy + at.offset(p.gs), lane);
-      if (norm) next.load(x + at.offset(p.xs), lane);
-      angles.load(p, at, lane);
-    }
-    now.turn(p, lane, -1.f, g);
-    if (norm) {
-      float sum = 0.f, dot = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sum = fmaf(u[i], u[i], sum);
-        dot = fmaf(g[i] * w[i], u[i], dot);
+  if (at.left > 0) {
+    Cursor<const T> dy = TAAC_ROWS(const T, p.g, p.gs), x = TAAC_ROWS(const T, p.x, p.xs);
+    Cursor<T> dx = TAAC_ROWS(T, p.y, p.ys);
+    Cursor<const int32_t> place(static_cast<const int32_t*>(p.positions), at, p.T, p.ps[0], p.ps[1]);
+    Angles angles;
+    next_g.load(dy.p, lane);
+    if (norm) next.load(x.p, lane);
+    angles.load(p, at, place, lane);
+    while (true) {
+      float g[8], u[8];
+      next_g.get(lane, g);
+      if (norm) next.get(lane, u);
+      Angles now = angles;
+      const bool wraps = at.next(p);
+      if (at.left > 0) {
+        dy.next(wraps), x.next(wraps), place.next(wraps);
+        next_g.load(dy.p, lane);
+        if (norm) next.load(x.p, lane);
+        angles.load(p, at, place, lane);
       }
-      const float rstd = rsqrtf(fmaf(group_sum<L>(sum), p.inv_d, p.eps));
-      const float mean = group_sum<L>(dot) * rstd * p.inv_d;
+      now.template turn<true>(p, lane, g);
+      if (norm) {
+        float sum = 0.f, dot = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        u[i] *= rstd;
-        dw[0][i] = fmaf(g[i], u[i], dw[0][i]);
-        g[i] = rstd * (g[i] * w[i] - u[i] * mean);
+        for (int i = 0; i < 8; ++i) {
+          sum = fmaf(u[i], u[i], sum);
+          dot = fmaf(g[i] * w[i], u[i], dot);
+        }
+        const float rstd = rsqrtf(fmaf(group_sum<L>(sum), p.inv_d, p.eps));
+        const float mean = group_sum<L>(dot) * rstd * p.inv_d;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          u[i] *= rstd;
+          dw[0][i] = fmaf(g[i], u[i], dw[0][i]);
+          g[i] = rstd * (g[i] * w[i] - u[i] * mean);
+        }
       }
+      store_row<T, L, VEC, INTER>(dx.p, lane, g);
+      if (at.left == 0) break;
+      dx.next(wraps);
     }
-    store_row<T, L, VEC, INTER>(to, lane, g);
   }
   if (!norm) return;
 #pragma unroll
@@ -447,6 +465,7 @@ int take_rope(const char* name, RopeParams& p, const void* q, const void* k, voi
   if (H > kMaxHeads || key_heads > kMaxHeads) return set_error(TAAC_ERR_UNSUPPORTED, "%s: at most %d heads", name, kMaxHeads);
   if (rotary < 0 || rotary > d || rotary % 2 != 0) return set_error(TAAC_ERR_INVALID_VALUE, "%s: the rotated features must be an even number, at most the head's (got %d of %d)", name, rotary, d);
   if ((rotary > 0) != (table != nullptr) || places < 0) return set_error(TAAC_ERR_INVALID_VALUE, "%s: a table comes with rotated features, its size not negative", name);
+  if (places > 0x7fffffff) return set_error(TAAC_ERR_UNSUPPORTED, "%s: a table has at most 2^31 - 1 positions", name);
   if ((qw == nullptr) != (kw == nullptr)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: both norm weights or neither", name);
   if (dtype != TAAC_F32 && dtype != TAAC_BF16 && dtype != TAAC_F16) return set_error(TAAC_ERR_INVALID_VALUE, "%s: unknown dtype %d", name, dtype);
   if (!(eps >= 0.f)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: eps must not be negative", name);
@@ -458,7 +477,8 @@ int take_rope(const char* name, RopeParams& p, const void* q, const void* k, voi
   }
   if (positions != nullptr) {
     if (ps == nullptr) return set_error(TAAC_ERR_INVALID_VALUE, "%s: null strides of the positions", name);
-    p.ps[0] = ps[0], p.ps[1] = ps[1];
+    const int64_t words = pos_int64 ? 2 : 1;  // of 32 bits
+    p.ps[0] = ps[0] * words, p.ps[1] = ps[1] * words;
   }
   *empty = B == 0 || T == 0;
   if (*empty) return TAAC_OK;
