@@ -30,19 +30,6 @@
 
 namespace taac {
 
-// n / d of n below 2^31 by a product: divisions are most of a short call's scalar instructions.
-struct Divisor {
-  uint32_t factor, shift;
-  int32_t d;
-  __device__ __forceinline__ int over(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * factor) >> shift); }
-};
-inline Divisor divisor(int32_t d) {
-  uint32_t bits = 0;
-  while ((int64_t{1} << bits) < d) ++bits;
-  // factor = ceil(2^(31 + bits) / d) is off by less than one in 2^(31 + bits) / d, i.e. n / d by less than 1 / d
-  return {static_cast<uint32_t>(((uint64_t{1} << (31 + bits)) + d - 1) / d), 31 + bits, d};
-}
-
 struct AttendParams {
   KvPool pool;
   const void* q;

@@ -24,6 +24,7 @@ struct CacheParams {
   int64_t ks[3], vs[3];    // element strides of (batch, head, token)
   int64_t rows;            // B * T * heads
   int64_t units;           // B * chunks * heads
+  Divisor by_heads, by_chunks, by_tokens;
   int32_t T, chunks, starts_int64;
 };
 
@@ -123,9 +124,15 @@ struct Row {
   int t, h;
   bool there;
   __device__ __forceinline__ Row(const CacheParams& p, int64_t row) {
-    const int64_t token = row / p.pool.heads;
+    int64_t token;
+    if (p.rows < 0x7fffffff) {
+      token = p.by_heads.over(static_cast<int>(row));
+      b = p.by_tokens.over(static_cast<int>(token));
+    } else {
+      token = row / p.pool.heads;
+      b = token / p.T;
+    }
     h = static_cast<int>(row - token * p.pool.heads);
-    b = token / p.T;
     t = static_cast<int>(token - b * p.T);
     there = p.lengths == nullptr || t < p.lengths[b];
     const int64_t start = p.starts == nullptr ? 0 : (p.starts_int64 ? static_cast<const int64_t*>(p.starts)[b] : static_cast<const int32_t*>(p.starts)[b]);
@@ -267,16 +274,15 @@ struct Chunk {
   uint8_t* record;      // null: in no page, or nothing to do there
   Chunk() = default;
   __device__ __forceinline__ Chunk(const CacheParams& p, int64_t unit, int record_bytes) {
-    const uint32_t heads = p.pool.heads;
     int64_t rest;
-    if (unit < 0x7fffffff) {
-      rest = static_cast<uint32_t>(unit) / heads;
-      b = static_cast<uint32_t>(rest) / static_cast<uint32_t>(p.chunks);
+    if (p.units < 0x7fffffff) {
+      rest = p.by_heads.over(static_cast<int>(unit));
+      b = p.by_chunks.over(static_cast<int>(rest));
     } else {
-      rest = unit / heads;
+      rest = unit / p.pool.heads;
       b = rest / p.chunks;
     }
-    h = static_cast<int>(unit - rest * heads);
+    h = static_cast<int>(unit - rest * p.pool.heads);
     int64_t start = p.starts == nullptr ? 0 : integer_at<SCALAR>(p.starts, b, p.starts_int64);
     int n = p.lengths == nullptr ? p.T : min(max(static_cast<int>(integer_at<SCALAR>(p.lengths, b, false)), 0), p.T);
     if (start < 0 || start >= int64_t{1} << 40) start = 0, n = 0;
@@ -551,6 +557,7 @@ int run_cache(const char* name, CacheParams& p, bool write, const void* k, const
   const int chunks = static_cast<int>((static_cast<int64_t>(T) + 2 * kKvChunk - 2) / kKvChunk);
   if (T >= kChunksFrom || p.rows > int64_t{1} << 27) p.chunks = chunks;
   p.units = static_cast<int64_t>(B) * chunks * p.pool.heads;
+  p.by_heads = divisor(p.pool.heads), p.by_chunks = divisor(chunks), p.by_tokens = divisor(T);
   if (dtype == TAAC_F32) dispatch_cache<float>(p, d, bits, write, s);
   if (dtype == TAAC_BF16) dispatch_cache<bf16_t>(p, d, bits, write, s);
   if (dtype == TAAC_F16) dispatch_cache<f16_t>(p, d, bits, write, s);
