@@ -120,8 +120,10 @@ void launch_join(const AttendParams& p, const Plan& plan, int d, hipStream_t s) 
 extern "C" int64_t taac_cached_attention_workspace_bytes(int32_t B, int32_t H, int32_t heads, int32_t T, int32_t d, int bits, int64_t table_tokens) {
   using namespace taac;
   if (B < 0 || T < 0 || heads <= 0 || H <= 0 || H % heads != 0 || d <= 0 || (bits != 4 && bits != 8) || table_tokens < 0) return -1;
-  const Plan plan = plan_of(B, heads, H / heads, T, d, bits, table_tokens, false);
-  return plan.splits > 1 ? static_cast<int64_t>(B) * H * T * plan.splits * (d + 2) * 4 : 0;
+  // of either type of queries: three and four rows in two parts take the other form
+  const int one = plan_of(B, heads, H / heads, T, d, bits, table_tokens, false).splits, two = plan_of(B, heads, H / heads, T, d, bits, table_tokens, true).splits;
+  const int splits = one > two ? one : two;
+  return splits > 1 ? static_cast<int64_t>(B) * H * T * splits * (d + 2) * 4 : 0;
 }
 
 extern "C" int taac_cached_attention_fwd(const void* q, void* o, const void* cache, int64_t pages, int32_t heads, int32_t page_tokens, int32_t d, int bits,

@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import ctypes
+import itertools
+import re
 
 import pytest
 import torch
@@ -224,5 +226,13 @@ def test_cache_entry_points_check_on_the_host():
     need = library.taac_cached_attention_workspace_bytes(1, 4, 2, 1, 32, 4, 1 << 16)
     assert need > 0 and attend(table_pages=1 << 12, ws=fake, bytes=need - 1) == invalid and b"workspace" in library.taac_last_error()
     assert attend(table_pages=1 << 12, ws=odd, bytes=need) == invalid
+    for d in (32, 64, 128):  # queries of either type find room in what is asked for
+        for group, bits in itertools.product((1, 2, 3, 4, 5, 16, 17), (4, 8)):
+            need = library.taac_cached_attention_workspace_bytes(1, 8 * group, 8, 1, d, bits, 1 << 16)
+            asked = []
+            for dtype in (_native.TAAC_BF16, _native.TAAC_F16):
+                assert attend(heads=8, H=8 * group, d=d, bits=bits, table_pages=1 << 12, dtype=dtype) == invalid
+                asked.append(int(re.search(rb"must hold (\d+) bytes", library.taac_last_error()).group(1)))
+            assert need == max(asked)
     assert library.taac_cached_attention_workspace_bytes(1024, 8, 8, 1, 32, 4, 512) == 0  # enough samples to fill the card
     assert library.taac_cached_attention_workspace_bytes(1, 3, 2, 1, 32, 4, 512) == -1 and library.taac_cached_attention_workspace_bytes(1, 2, 2, 1, 32, 6, 512) == -1

@@ -100,6 +100,17 @@ def test_long_histories(device, bits, dtype, width, group, tokens, window):
     _check(got, q, k, v, lengths, [tokens] * 3, window)
 
 
+@pytest.mark.parametrize("width", [64, 128])
+def test_fp16_rows_in_the_other_form(device, width):
+    """Three and four rows of fp16 are cut into more splits than those of bf16."""
+    cache, pages, k, v = _filled(device, [16000], 4, width, 4, 64)
+    table = torch.cat((pages, pages.flip(1), pages, pages), 1)  # far more places than tokens
+    for group in (3, 4):
+        q = _queries(device, 1, 4 * group, 1, width, torch.float16)
+        got = cached_attention(q, cache, table, torch.tensor([16000], device=device))
+        _check(got, q, k, v, [16000], [1])
+
+
 def test_many_samples(device):
     """More rows than split: a workgroup to a key head of a sample."""
     lengths = [int(x) for x in torch.randint(0, 300, (700,), generator=torch.Generator().manual_seed(1))]
