@@ -206,9 +206,9 @@ struct Walk {
   // to the next token; whether that is behind the end of a sample more than step_b behind
   __device__ __forceinline__ bool next(const RopeParams& p) {
     --left;
-    t += step_t;
-    const bool wraps = t >= p.T;
-    t -= wraps ? p.T : 0;
+    const uint32_t T = p.T, to = static_cast<uint32_t>(t) + static_cast<uint32_t>(step_t);  // below 2^32
+    const bool wraps = to >= T;
+    t = static_cast<int>(wraps ? to - T : to);
     return wraps;
   }
 };

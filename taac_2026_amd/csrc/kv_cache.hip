@@ -13,6 +13,8 @@ constexpr int64_t kMostGroups = 1 << 14;  // of four chunks at a time: a wavefro
 // 64 samples of 128 features in 8 bits 9 : 11 and 12 : 11.
 constexpr int kChunksFrom = 12;
 
+constexpr int64_t kMostRows = 1 << 27;  // of a launch row by row, whose numbers have 32 bits
+
 struct CacheParams {
   KvPool pool;
   const void* k;
@@ -123,17 +125,11 @@ struct Row {
   int64_t b, position;
   int t, h;
   bool there;
-  __device__ __forceinline__ Row(const CacheParams& p, int64_t row) {
-    int64_t token;
-    if (p.rows < 0x7fffffff) {
-      token = p.by_heads.over(static_cast<int>(row));
-      b = p.by_tokens.over(static_cast<int>(token));
-    } else {
-      token = row / p.pool.heads;
-      b = token / p.T;
-    }
-    h = static_cast<int>(row - token * p.pool.heads);
-    t = static_cast<int>(token - b * p.T);
+  __device__ __forceinline__ Row(const CacheParams& p, int row) {
+    const int token = p.by_heads.over(row), sample = p.by_tokens.over(token);
+    h = row - token * p.pool.heads;
+    t = token - sample * p.T;
+    b = sample;
     there = p.lengths == nullptr || t < p.lengths[b];
     const int64_t start = p.starts == nullptr ? 0 : (p.starts_int64 ? static_cast<const int64_t*>(p.starts)[b] : static_cast<const int32_t*>(p.starts)[b]);
     there &= start >= 0 && start < (int64_t{1} << 40);
@@ -144,7 +140,7 @@ struct Row {
 template <typename T, int D, int BITS>
 __global__ __launch_bounds__(kThreads) void kv_write_rows_kernel(const CacheParams p) {
   constexpr int LANES = D / 8, ROWS = kThreads / LANES, BLOCKS = D / kKvBlock;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / LANES;
+  const int row = blockIdx.x * ROWS + threadIdx.x / LANES;
   if (row >= p.rows) return;
   const int s = threadIdx.x % LANES, block = s / 4, sub = s % 4;
   const Row at(p, row);
@@ -201,7 +197,7 @@ __global__ __launch_bounds__(kThreads) void kv_write_rows_kernel(const CachePara
 template <typename T, int D, int BITS>
 __global__ __launch_bounds__(kThreads) void kv_read_rows_kernel(const CacheParams p) {
   constexpr int LANES = D / 8, ROWS = kThreads / LANES, BLOCKS = D / kKvBlock;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / LANES;
+  const int row = blockIdx.x * ROWS + threadIdx.x / LANES;
   if (row >= p.rows) return;
   const int s = threadIdx.x % LANES, block = s / 4, sub = s % 4;
   const Row at(p, row);
@@ -555,7 +551,7 @@ int run_cache(const char* name, CacheParams& p, bool write, const void* k, const
   p.rows = static_cast<int64_t>(B) * T * p.pool.heads;
   // chunks that T tokens meet at most, wherever they start
   const int chunks = static_cast<int>((static_cast<int64_t>(T) + 2 * kKvChunk - 2) / kKvChunk);
-  if (T >= kChunksFrom || p.rows > int64_t{1} << 27) p.chunks = chunks;
+  if (T >= kChunksFrom || p.rows > kMostRows) p.chunks = chunks;
   p.units = static_cast<int64_t>(B) * chunks * p.pool.heads;
   p.by_heads = divisor(p.pool.heads), p.by_chunks = divisor(chunks), p.by_tokens = divisor(T);
   if (dtype == TAAC_F32) dispatch_cache<float>(p, d, bits, write, s);

@@ -235,6 +235,15 @@ def test_many_rows(device):
             assert ((a.double() - b).abs() <= F32 * b.abs() + bound).all()
 
 
+def test_as_many_tokens_as_there_are(device):
+    """2^31 - 1 tokens, one row in memory, of which a wavefront walks sixteen thousand."""
+    tokens = 2**31 - 1
+    q, k = (torch.full((1, 1, 1, 1), x, device=device, dtype=torch.bfloat16).expand(1, 1, tokens, 1) for x in (2.0, -3.0))
+    weights = [torch.full((1,), x, device=device, dtype=torch.bfloat16) for x in (1.5, 2.5)]
+    for out, want in zip(head_norm_rope(q, k, *weights, eps=0.0), (1.5, -2.5)):
+        assert out.shape == q.shape and out.min().item() == out.max().item() == want
+
+
 def test_captured_with_attention(device):
     """Norm, rotation and attention, forward and backward, in a replayed graph, eager work between the replays."""
     q, k, weights = _inputs(device, 2, 40, 4, 4, 32, torch.bfloat16, seed=7)

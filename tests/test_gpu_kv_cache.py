@@ -191,6 +191,20 @@ def test_a_pool_beyond_32_bits(device):
         assert torch.equal(got.double(), cached_values(x, 8))
 
 
+def test_more_rows_than_32_bits(device):
+    """Samples by the hundred thousand of four thousand heads, of which the last alone has a page."""
+    batch, heads = (1 << 19) + 3, 1 << 12
+    k, v = (_rows((1, 1, 1, 32), torch.bfloat16, seed).to(device).expand(batch, heads, 1, 32) for seed in (1, 2))
+    cache = empty_kv_cache(2, heads, 32, page_tokens=16, device=device)
+    pages = torch.full((batch, 1), -1, device=device, dtype=torch.int32)
+    pages[-1] = 1
+    kv_cache_write(cache, k, v, pages)
+    got = kv_cache_read(cache, torch.tensor([[1], [0]], device=device), None, 2, dtype=torch.float32)
+    for x, y in zip(got, (k, v)):
+        assert torch.equal(x[0, :, 0].double(), cached_values(y[-1, :, 0], 4).double())
+        assert (x[0, :, 1] == 0).all() and (x[1] == 0).all()
+
+
 def test_captured(device):
     """Written and read in a replayed graph on other tokens and places, eager work between the replays; and on a stream of its own."""
     k, v = (_rows((4, 2, 3, 32), torch.bfloat16, seed).to(device) for seed in (1, 2))
