@@ -52,18 +52,19 @@ constexpr int kTile = 64;          // tokens
 // A kernel's shape, by the rows of a workgroup: 1, 2 or 4 (one form), 16 or 32 (the other). alone: a wavefront to a workgroup.
 struct Shape {
   int waves;
-  int stages;    // tiles of a wavefront in LDS
+  int stages;    // tiles of a wavefront in LDS; one: keys and values by themselves
   int per_simd;  // wavefronts that the registers leave room for
 };
 __host__ __device__ constexpr Shape shape_of(int rows, int d, bool alone) {
   if (rows <= 4) return {alone ? 1 : 4, 2, d == 32 ? 6 : d == 64 ? 4 : 2};
-  if (rows == 16) return {alone ? 1 : 4, alone ? 2 : 1, d == 32 ? 6 : d == 64 ? 4 : 3};
+  if (rows == 16) return {alone ? 1 : 4, 1, d == 32 ? 6 : d == 64 ? 4 : 3};
   return {4, 1, d == 32 ? 4 : d == 64 ? 3 : 2};
 }
 __host__ __device__ constexpr int tile_bytes(int d, int bits) { return (4 * kv_record_bytes(d, bits) + 1023) / 1024 * 1024; }
+__host__ __device__ constexpr int half_bytes(int d, int bits) { return 4 * kv_key_bytes(d, bits) + 4 * kWave; }
 __host__ __device__ constexpr int lds_bytes(int rows, int d, int bits, bool alone) {
   const Shape shape = shape_of(rows, d, alone);
-  const int tiles = shape.waves * (shape.stages * tile_bytes(d, bits) + (rows <= 4 ? 8 * (kTile + 8) * 2 : 0));
+  const int tiles = shape.waves * (rows <= 4 ? shape.stages * tile_bytes(d, bits) + 8 * (kTile + 8) * 2 : 2 * half_bytes(d, bits));
   const int meeting = shape.waves / 2 * kWave * 16 * (rows == 32 ? 2 : 1) * (d / 16 + 1);  // half of the wavefronts leave their rows for the others
   return tiles > meeting ? tiles : meeting;
 }
@@ -355,18 +356,23 @@ struct Staged {
 
   // Which chunks there are, a bit each. In the place of one that there is not: the first of the pool, whose tokens are then masked.
   template <bool WHOLE>
-  static __device__ __forceinline__ uint32_t request(const KvPool& pool, const Pages<WHOLE>& pages, int head, int tile, uint8_t* to, int lane) {
-    constexpr int N = Pages<WHOLE>::N;
+  static __device__ __forceinline__ uint32_t find(const KvPool& pool, const Pages<WHOLE>& pages, int head, int tile, const uint8_t* (&record)[Pages<WHOLE>::N]) {
     uint32_t held = 0;
-    const uint8_t* record[N];
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
+    for (int c = 0; c < Pages<WHOLE>::N; ++c) {
       const int chunk = tile * (kTile / kKvChunk) + c;
       const int64_t page = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(pages.high[c])) << 32 | static_cast<uint32_t>(pages.low[c]));
       const bool there = (chunk >> (pool.page_shift - 4)) < pool.table_pages && page >= 0 && page < pool.pages;
       held |= there ? (WHOLE ? 15u : 1u << c) : 0u;
       record[c] = pool.data + (there ? kv_record(pool, page, head, chunk & ((1 << (pool.page_shift - 4)) - 1), RECORD) : 0);
     }
+    return held;
+  }
+  template <bool WHOLE>
+  static __device__ __forceinline__ uint32_t request(const KvPool& pool, const Pages<WHOLE>& pages, int head, int tile, uint8_t* to, int lane) {
+    constexpr int N = Pages<WHOLE>::N;
+    const uint8_t* record[N];
+    const uint32_t held = find<WHOLE>(pool, pages, head, tile, record);
     if constexpr (WHOLE) {
 #pragma unroll
       for (int i = 0; i < REQUESTS; ++i)
@@ -389,18 +395,56 @@ struct Staged {
   }
 };
 
+// The same of the keys or the values alone: the codes of the four chunks, then their scales, four bytes to a lane.
+template <int D, int BITS>
+struct StagedHalf {
+  static constexpr int RECORD = kv_record_bytes(D, BITS), CODES = kv_key_bytes(D, BITS), SCALES = kKvChunk * D / kKvBlock;
+  static constexpr int PIECES = 4 * CODES / (kWave * 16), REQUESTS = PIECES + 1, BYTES = 4 * CODES + 4 * kWave;
+  template <bool WHOLE>
+  static __device__ __forceinline__ void request(const uint8_t* const (&record)[Pages<WHOLE>::N], bool values, uint8_t* to, int lane) {
+    const int codes_at = values ? kv_value_at(D, BITS) : 0, scales_at = values ? kv_value_scale_at(D, BITS) : kv_key_scale_at(D, BITS);
+    const int scale = min(lane, SCALES - 1), scale_chunk = scale / (SCALES / 4), scale_in = scale % (SCALES / 4) * 4;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      // of chunk i * 1024 / CODES, or of as many from there on as 1024 bytes hold
+      constexpr int LANES = CODES / 16 < kWave ? CODES / 16 : kWave;  // of a chunk
+      const int first = i * kWave * 16 / CODES, of = lane / LANES, in = i * kWave * 16 % CODES + lane % LANES * 16;
+      if constexpr (WHOLE) {
+        lds_dma16_offset(record[0] + first * RECORD + codes_at, of * RECORD + in, to + i * kWave * 16);
+      } else {
+        const uint8_t* from = record[first];
+        if constexpr (kWave / LANES == 2) {
+          from = of >= 1 ? record[first + 1] : from;
+        } else if constexpr (kWave / LANES == 4) {
+          const uint8_t *r1 = record[1], *r2 = record[2], *r3 = record[3];
+          from = of >= 2 ? (of == 3 ? r3 : r2) : (of == 1 ? r1 : from);
+        }
+        lds_dma16(from + codes_at + in, to + i * kWave * 16);
+      }
+    }
+    if constexpr (WHOLE) {
+      lds_dma4_offset(record[0] + scales_at, scale_chunk * RECORD + scale_in, to + 4 * CODES);
+    } else {
+      const uint8_t *r0 = record[0], *r1 = record[1], *r2 = record[2], *r3 = record[3];
+      const uint8_t* from = scale_chunk >= 2 ? (scale_chunk == 3 ? r3 : r2) : (scale_chunk == 1 ? r1 : r0);
+      lds_dma4(from + scales_at + scale_in, to + 4 * CODES);
+    }
+  }
+};
+
 // acc[rows of 16 features] += values^T p: probs[n][part][half]: of 32 tokens, group grp those of chunk 2 half at 4 grp, then those of the next chunk.
-template <int D, int BITS, int RT, int PARTS>
-__device__ __forceinline__ void times_values(const uint8_t* tile, int l16, int grp, const bf16x8 (&probs)[RT][PARTS][2], f32x4 (&acc)[RT][D / 16]) {
-  constexpr int BLOCKS = D / kKvBlock, EACH = BITS / 4, RECORD = kv_record_bytes(D, BITS);
+// code_bytes, scale_bytes: of the tile's first chunk, CODES_STEP and SCALES_STEP before the next one's.
+template <int D, int BITS, int CODES_STEP, int SCALES_STEP, int RT, int PARTS>
+__device__ __forceinline__ void times_values(const uint8_t* code_bytes, const uint8_t* scale_bytes, int l16, int grp, const bf16x8 (&probs)[RT][PARTS][2], f32x4 (&acc)[RT][D / 16]) {
+  constexpr int BLOCKS = D / kKvBlock, EACH = BITS / 4;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     Words<BLOCKS * EACH> codes[2];
     Words<BLOCKS> scales[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      codes[c].load(tile + (2 * half + c) * RECORD + kv_value_at(D, BITS) + (l16 * 4 + grp) * BLOCKS * BITS);
-      scales[c].load(tile + (2 * half + c) * RECORD + kv_value_scale_at(D, BITS) + grp * BLOCKS * 4);
+      codes[c].load(code_bytes + (2 * half + c) * CODES_STEP + (l16 * 4 + grp) * BLOCKS * BITS);
+      scales[c].load(scale_bytes + (2 * half + c) * SCALES_STEP + grp * BLOCKS * 4);
     }
 #pragma unroll
     for (int j = 0; j < BLOCKS; ++j) {
@@ -458,6 +502,47 @@ __device__ __forceinline__ void walk(const AttendParams& p, const Job& job, cons
       take(stages + i * Tile::BYTES, held[i], tile);
       tile += W;
     }
+  }
+}
+
+// A wavefront's tiles, one in LDS, keys and values by themselves: the next keys are on their way from when the scores are made, the next values from when the
+// products with these are. Two whole tiles would leave half of the wavefronts no room in LDS, and one whole tile nothing on its way while it is taken.
+template <int D, int BITS, int W, bool WHOLE, typename Scores, typename Softmax, typename Values>
+__device__ __forceinline__ void walk_halves(const AttendParams& p, const Job& job, const Span& span, int wave, int lane, uint8_t* keys, Scores&& scores, Softmax&& softmax,
+                                            Values&& take_values) {
+  typedef StagedHalf<D, BITS> Half;
+  const int64_t row = job.b * p.pool.table_stride;
+  uint8_t* const values = keys + Half::BYTES;
+  const uint8_t* record[Pages<WHOLE>::N];
+  Pages<WHOLE> pages;
+  int tile = span.first + wave;
+  if (tile >= span.end) return;
+  pages.find(p.pool, row, tile);
+  uint32_t held = Staged<D, BITS>::template find<WHOLE>(p.pool, pages, job.head, tile, record);
+  pages.find(p.pool, row, tile + W);
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // what the compiler asked for before, which it would otherwise await in every round
+  Half::template request<WHOLE>(record, false, keys, lane);
+  Half::template request<WHOLE>(record, true, values, lane);
+  while (true) {
+    vm_wait<Half::REQUESTS>();
+    scores(keys);
+    const int next = tile + W;
+    const bool more = next < span.end;
+    const uint32_t chunks = held;
+    if (more) {
+      held = Staged<D, BITS>::template find<WHOLE>(p.pool, pages, job.head, next, record);
+      pages.find(p.pool, row, next + W);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the keys that lay there
+      Half::template request<WHOLE>(record, false, keys, lane);
+    }
+    softmax(chunks, tile);
+    if (more) vm_wait<Half::REQUESTS>();
+    else vm_wait<0>();
+    take_values(values);
+    if (!more) return;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    Half::template request<WHOLE>(record, true, values, lane);
+    tile = next;
   }
 }
 
@@ -570,7 +655,7 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
     wave_sync();
     sum = mfma(ones, probs[0][0][0], sum);
     sum = mfma(ones, probs[0][0][1], sum);
-    times_values<D, BITS, 1, 1>(tile, l16, grp, probs, acc);
+    times_values<D, BITS, Tile::RECORD, Tile::RECORD>(tile + kv_value_at(D, BITS), tile + kv_value_scale_at(D, BITS), l16, grp, probs, acc);
   };
 
   p.pool.page_shift >= 6 ? walk<D, BITS, W, S, true>(p, job, span, wave, lane, stages, take) : walk<D, BITS, W, S, false>(p, job, span, wave, lane, stages, take);
@@ -592,10 +677,10 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
 
 // ---- sixteen rows at a time ---------------------------------------------------------------------------------------
 
-template <typename T, int D, int BITS, int ROWS, int W, int S>
+template <typename T, int D, int BITS, int ROWS, int W>
 __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void cached_attention_many_kernel(const AttendParams p) {
   constexpr int RT = ROWS / 16, BLOCKS = D / kKvBlock, PARTS = kParts<T>;
-  typedef Staged<D, BITS> Tile;
+  typedef StagedHalf<D, BITS> Half;
   extern __shared__ __align__(16) uint8_t memory[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, l16 = lane % 16, grp = lane / 16;
   const Job job(p, ROWS);
@@ -604,7 +689,7 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
     if (job.split == 0) clear_rows<T, D, ROWS, W * kWave>(p, job);
     return;
   }
-  uint8_t* const stages = memory + wave * (S * Tile::BYTES);
+  uint8_t* const stages = memory + wave * (2 * Half::BYTES);
   int low[RT], high[RT];
   bool empty[RT];  // rows that see nothing are taken along, and cleared at the end
   bf16x8 q[RT][PARTS][BLOCKS];
@@ -636,16 +721,16 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
 
   const int octet = grp * BLOCKS, block = octet / 4;  // of the lane's features
   const bf16x8 ones = __builtin_bit_cast(bf16x8, (u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}));
-  auto take = [&](const uint8_t* tile, uint32_t chunks, int number) __attribute__((always_inline)) {
-    f32x4 s[RT][4];
+  f32x4 s[RT][4];
+  bf16x8 probs[RT][2][2];
+  auto scores = [&](const uint8_t* keys_at) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
 #pragma unroll
       for (int n = 0; n < RT; ++n) s[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const uint8_t* record = tile + c * Tile::RECORD;
       Words<BLOCKS * BITS / 4> keys;
-      keys.load(record + block * (kKvChunk * 4 * BITS) + l16 * 4 * BITS + octet % 4 * BITS);
-      const float scale = scale_of<0>(record[kv_key_scale_at(D, BITS) + l16 * BLOCKS + block]);
+      keys.load(keys_at + c * Half::CODES + block * (kKvChunk * 4 * BITS) + l16 * 4 * BITS + octet % 4 * BITS);
+      const float scale = scale_of<0>(keys_at[4 * Half::CODES + c * Half::SCALES + l16 * BLOCKS + block]);
 #pragma unroll
       for (int j = 0; j < BLOCKS; ++j) {
         const bf16x8 key = eight<BITS>(keys.w + j * (BITS / 4), scale);
@@ -655,6 +740,8 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
           for (int part = 0; part < PARTS; ++part) s[n][c] = mfma(key, q[n][part][j], s[n][c]);
       }
     }
+  };
+  auto softmax = [&](uint32_t chunks, int number) __attribute__((always_inline)) {
     if (chunks != 15u || number * kTile < all_low || number * kTile + kTile > all_high) {
 #pragma unroll
       for (int n = 0; n < RT; ++n)
@@ -689,7 +776,6 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
           for (int e = 0; e < 4; ++e) acc[n][i][e] *= f;
       }
     }
-    bf16x8 probs[RT][2][2];
 #pragma unroll
     for (int n = 0; n < RT; ++n)
 #pragma unroll
@@ -703,10 +789,13 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
         sums[n] = mfma(ones, probs[n][0][half], sums[n]);
         sums[n] = mfma(ones, probs[n][1][half], sums[n]);
       }
-    times_values<D, BITS, RT, 2>(tile, l16, grp, probs, acc);
+  };
+  auto take_values = [&](const uint8_t* values) __attribute__((always_inline)) {
+    times_values<D, BITS, Half::CODES, Half::SCALES>(values, values + 4 * Half::CODES, l16, grp, probs, acc);
   };
 
-  p.pool.page_shift >= 6 ? walk<D, BITS, W, S, true>(p, job, span, wave, lane, stages, take) : walk<D, BITS, W, S, false>(p, job, span, wave, lane, stages, take);
+  p.pool.page_shift >= 6 ? walk_halves<D, BITS, W, true>(p, job, span, wave, lane, stages, scores, softmax, take_values)
+                         : walk_halves<D, BITS, W, false>(p, job, span, wave, lane, stages, scores, softmax, take_values);
   float sum[RT];
 #pragma unroll
   for (int n = 0; n < RT; ++n) sum[n] = sums[n][0];
@@ -732,10 +821,10 @@ void launch_with(Kernel* kernel, uint32_t groups, int threads, int bytes, const 
 template <typename T, int D, int BITS, int ROWS, bool ALONE>
 void launch_rows(const AttendParams& p, uint32_t groups, hipStream_t s) {
   constexpr Shape shape = shape_of(ROWS, D, ALONE);
-  static_assert(Staged<D, BITS>::BYTES == tile_bytes(D, BITS));
+  static_assert(Staged<D, BITS>::BYTES == tile_bytes(D, BITS) && StagedHalf<D, BITS>::BYTES == half_bytes(D, BITS));
   constexpr int bytes = lds_bytes(ROWS, D, BITS, ALONE), threads = shape.waves * kWave;
   if constexpr (ROWS <= 4) launch_with(cached_attention_few_kernel<T, D, BITS, ROWS, shape.waves, shape.stages>, groups, threads, bytes, p, s);
-  else launch_with(cached_attention_many_kernel<T, D, BITS, ROWS, shape.waves, shape.stages>, groups, threads, bytes, p, s);
+  else launch_with(cached_attention_many_kernel<T, D, BITS, ROWS, shape.waves>, groups, threads, bytes, p, s);
 }
 template <typename T, int D, int BITS>
 void launch_attend(const AttendParams& p, int rows, bool alone, uint32_t groups, hipStream_t s) {
