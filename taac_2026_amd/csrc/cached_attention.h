@@ -49,7 +49,7 @@ struct AttendParams {
 namespace {
 
 constexpr int kTile = 64;          // tokens
-// A kernel's shape, by the rows of a workgroup: 1, 2 or 4 (one form), 16 or 32 (the other). alone: a wavefront to a workgroup.
+// A kernel's shape, by the rows of a workgroup: 1, 2 or 4 (one form), 16, 32 or 48 (the other). alone: a wavefront to a workgroup.
 struct Shape {
   int waves;
   int stages;    // tiles of a wavefront in LDS; one: keys and values by themselves
@@ -58,15 +58,35 @@ struct Shape {
 __host__ __device__ constexpr Shape shape_of(int rows, int d, bool alone) {
   if (rows <= 4) return {alone ? 1 : 4, 2, d == 32 ? 6 : d == 64 ? 4 : 2};
   if (rows == 16) return {alone ? 1 : 4, 1, d == 32 ? 6 : d == 64 ? 4 : 3};
-  return {4, 1, d == 32 ? 4 : d == 64 ? 3 : 2};
+  if (rows == 32) return {4, 1, d == 32 ? 4 : d == 64 ? 3 : 2};
+  return {8, 1, 2};
 }
 __host__ __device__ constexpr int tile_bytes(int d, int bits) { return (4 * kv_record_bytes(d, bits) + 1023) / 1024 * 1024; }
 __host__ __device__ constexpr int half_bytes(int d, int bits) { return 4 * kv_key_bytes(d, bits) + 4 * kWave; }
-__host__ __device__ constexpr int lds_bytes(int rows, int d, int bits, bool alone) {
+// Queries of more than sixteen rows lie in LDS: their registers are what a second wavefront to a SIMD needs. Not those in two parts: twice the bytes are what a second
+// workgroup needs.
+__host__ __device__ constexpr bool queries_in_lds(int rows, int parts) { return rows > 16 && parts == 1; }
+// Bytes that `waves` wavefronts with n fours of features in each lane leave for each other where they meet, in the first of two places and every second time, or in
+// the second.
+__host__ __device__ constexpr int meeting_bytes(int n, int waves, bool second) {
+  int most = 0;
+  for (int half = waves / 2, level = 0; half > 0; half /= 2, ++level) {
+    const int given = n % 2 == 0 ? n / 2 : n;
+    if ((level % 2 == 1) == second && waves * given * kWave * 16 > most) most = waves * given * kWave * 16;
+    n = given;
+  }
+  return most;
+}
+__host__ __device__ constexpr int stats_bytes(int rows, int waves) { return waves > 1 ? waves * (rows <= 16 ? 16 : rows) * 8 : 0; }
+// of the tiles, or of the meeting behind them; then the queries and the statistics
+__host__ __device__ constexpr int working_bytes(int rows, int d, int bits, bool alone) {
   const Shape shape = shape_of(rows, d, alone);
   const int tiles = shape.waves * (rows <= 4 ? shape.stages * tile_bytes(d, bits) + 8 * (kTile + 8) * 2 : 2 * half_bytes(d, bits));
-  const int meeting = shape.waves / 2 * kWave * 16 * (rows == 32 ? 2 : 1) * (d / 16 + 1);  // half of the wavefronts leave their rows for the others
+  const int fours = (rows <= 16 ? 1 : rows / 16) * (d / 16), meeting = meeting_bytes(fours, shape.waves, false) + meeting_bytes(fours, shape.waves, true);
   return tiles > meeting ? tiles : meeting;
+}
+__host__ __device__ constexpr int lds_bytes(int rows, int d, int bits, int parts, bool alone) {
+  return working_bytes(rows, d, bits, alone) + (queries_in_lds(rows, parts) ? rows * d * 2 : 0) + stats_bytes(rows, shape_of(rows, d, alone).waves);
 }
 constexpr float kNothing = -3e38f; // the maximum of no scores
 constexpr float kSlack = 8.f;
@@ -239,70 +259,129 @@ struct Place {
   __device__ __forceinline__ const T* query(const AttendParams& p, const Job& job) const {
     return static_cast<const T*>(p.q) + job.b * p.qs[0] + h * p.qs[1] + t * p.qs[2];
   }
-  // four features, their sum of weights, and the maximum that both refer to
-  template <typename T, int D>
-  __device__ __forceinline__ void leave(const AttendParams& p, const Job& job, const Span& span, int c, const f32x4& total, float l, float top) const {
-    if (span.active > 1) {
-      const int64_t row = ((static_cast<int64_t>(job.b) * p.H + h) * p.T + t) * p.splits.d + job.split;
-      *reinterpret_cast<f32x4*>(p.partial + row * D + c) = total;
-      if (c == 0) {
-        float* stats = p.partial + p.all_rows * p.splits.d * D + row * 2;
-        stats[0] = top, stats[1] = l;
-      }
-      return;
-    }
-    store<T>(p, job.b, c, total, l);
-  }
   template <typename T>
-  __device__ __forceinline__ void store(const AttendParams& p, int b, int c, const f32x4& total, float l) const {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    typename Vec8<T>::half_type v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(total[e] * inv);
-    *reinterpret_cast<typename Vec8<T>::half_type*>(static_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + t * p.os[2] + c) = v;
+  __device__ __forceinline__ T* output(const AttendParams& p, int b) const {
+    return static_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + t * p.os[2];
   }
 };
+template <typename T>
+__device__ __forceinline__ void store_four(T* to, const f32x4& total, float inv) {
+  typename Vec8<T>::half_type v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(total[e] * inv);
+  *reinterpret_cast<typename Vec8<T>::half_type*>(to) = v;
+}
 
-// The wavefronts' parts of the same rows, joined in the registers of the first: half of the remaining ones leave theirs in LDS at a time. A lane's part is
-// RT columns: N / RT fours of features each, with the column's sum and the maximum that both refer to.
-template <int N, int RT, int W>
-__device__ __forceinline__ void meet(uint8_t* memory, int wave, int lane, f32x4 (&acc)[RT][N / RT], float (&sum)[RT], float (&top)[RT]) {
+// C fours of features of a lane's columns, from the `from`th of RT columns' D / 16 on: to the output, or to the split's part. sum, top: the columns' sums of weights and the
+// maxima that all refer to.
+template <typename T, int D, int RT, int C>
+__device__ __forceinline__ void leave(const AttendParams& p, const Job& job, const Span& span, int from, int l16, int grp, const f32x4* part, const float (&sum)[RT],
+                                      const float (&top)[RT]) {
+  constexpr int EACH = C < D / 16 ? C : D / 16, FOURS = D / 16 % C == 0 || C % (D / 16) == 0 ? EACH : 1;  // of the same column
 #pragma unroll
-  for (int half = W / 2; half > 0; half /= 2) {
-    __syncthreads();  // the tiles, or what lay there, are done with
-    f32x4* slot = reinterpret_cast<f32x4*>(memory) + (wave & (half - 1)) * (N + RT) * kWave + lane;
-    if (wave >= half && wave < 2 * half) {
+  for (int e = 0; e < C; e += FOURS) {
+    const int n = (from + e) / (D / 16), row = job.row0 + 16 * n + l16, c = (from + e) % (D / 16) * 16 + 4 * grp;
+    if (row >= p.rows) continue;
+    float l = sum[0], most = top[0];
 #pragma unroll
-      for (int n = 0; n < RT; ++n) {
+    for (int r = 1; r < RT; ++r) l = n == r ? sum[r] : l, most = n == r ? top[r] : most;
+    const Place place(p, job, row);
+    if (span.active > 1 && place.t < span.news) {  // rows of no query are zeros whoever writes them
+      const int64_t at = ((static_cast<int64_t>(job.b) * p.H + place.h) * p.T + place.t) * p.splits.d + job.split;
 #pragma unroll
-        for (int i = 0; i < N / RT; ++i) slot[(n * (N / RT) + i) * kWave] = acc[n][i];
-        slot[(N + n) * kWave] = f32x4{sum[n], top[n], 0.f, 0.f};
+      for (int i = 0; i < FOURS; ++i) *reinterpret_cast<f32x4*>(p.partial + at * D + c + 16 * i) = part[e + i];
+      if (c == 0) {
+        float* stats = p.partial + p.all_rows * p.splits.d * D + at * 2;
+        stats[0] = most, stats[1] = l;
       }
-    }
-    __syncthreads();
-    if (wave < half) {
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* to = place.output<T>(p, job.b) + c;
 #pragma unroll
-      for (int n = 0; n < RT; ++n) {
-        const f32x4 other = slot[(N + n) * kWave];
-        const float up = fmaxf(top[n], other[1]), f = __builtin_amdgcn_exp2f(top[n] - up), g = __builtin_amdgcn_exp2f(other[1] - up);
-        top[n] = up;
-        sum[n] = sum[n] * f + other[0] * g;
-#pragma unroll
-        for (int i = 0; i < N / RT; ++i) {
-          const f32x4 part = slot[(n * (N / RT) + i) * kWave];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[n][i][e] = acc[n][i][e] * f + part[e] * g;
-        }
-      }
+      for (int i = 0; i < FOURS; ++i) store_four<T>(to + 16 * i, part[e + i], inv);
     }
   }
 }
 
+// The wavefronts' sums of the same rows. Those HALF apart give each other the half that the other one keeps, so that each ends with a part of its own, from
+// the `from`th four on; an odd number is given as a whole, and the giver is done.
+template <int N, int HALF, int M>
+__device__ __forceinline__ void gather(f32x4* place, f32x4* other_place, int wave, int lane, f32x4 (&acc)[M], int& from, bool& there) {
+  if constexpr (HALF > 0) {
+    constexpr bool SPLIT = N % 2 == 0;
+    constexpr int GIVEN = SPLIT ? N / 2 : N;
+    const bool upper = wave & HALF;
+    if (there && (SPLIT || upper)) {
+#pragma unroll
+      for (int i = 0; i < GIVEN; ++i) {
+        const f32x4 low = acc[i], high = acc[SPLIT ? GIVEN + i : i];
+        place[(wave * GIVEN + i) * kWave + lane] = upper ? low : high;
+      }
+    }
+    __syncthreads();
+    there &= SPLIT || !upper;
+    if (there) {
+#pragma unroll
+      for (int i = 0; i < GIVEN; ++i) {
+        const f32x4 other = place[((wave ^ HALF) * GIVEN + i) * kWave + lane], low = acc[i], high = acc[SPLIT ? GIVEN + i : i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] = (upper ? high[e] : low[e]) + other[e];
+      }
+    }
+    if (SPLIT && upper) from += GIVEN;
+    gather<GIVEN, HALF / 2>(other_place, place, wave, lane, acc, from, there);
+  }
+}
+__host__ __device__ constexpr int gathered(int n, int waves) {
+  for (int half = waves / 2; half > 0; half /= 2) n = n % 2 == 0 ? n / 2 : n;
+  return n;
+}
+
+// A workgroup's end: its wavefronts' statistics, then their sums under the common maxima, then what each leaves of them.
+template <typename T, int D, int RT, int W>
+__device__ __forceinline__ void finish(const AttendParams& p, const Job& job, const Span& span, uint8_t* memory, float* stats, int wave, int lane, f32x4 (&acc)[RT * (D / 16)],
+                                       float (&sum)[RT], float (&top)[RT]) {
+  constexpr int N = RT * (D / 16), C = gathered(N, W);
+  const int l16 = lane % 16, grp = lane / 16;
+  int from = 0;
+  bool there = true;
+  if constexpr (W > 1) {
+    typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
+    f32x2* const all = reinterpret_cast<f32x2*>(stats);  // [wavefront][row]
+    if (grp == 0) {
+#pragma unroll
+      for (int n = 0; n < RT; ++n) all[wave * (RT * 16) + n * 16 + l16] = f32x2{sum[n], top[n]};
+    }
+    __syncthreads();  // all tiles are done with, too
+#pragma unroll
+    for (int n = 0; n < RT; ++n) {
+      f32x2 each[W];
+      float most = kNothing, total = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        each[w] = all[w * (RT * 16) + n * 16 + l16];
+        most = fmaxf(most, each[w][1]);
+      }
+#pragma unroll
+      for (int w = 0; w < W; ++w) total = fmaf(each[w][0], __builtin_amdgcn_exp2f(each[w][1] - most), total);
+      const float f = __builtin_amdgcn_exp2f(top[n] - most);
+      top[n] = most, sum[n] = total;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n * (D / 16) + i][e] *= f;
+    }
+    gather<N, W / 2>(reinterpret_cast<f32x4*>(memory), reinterpret_cast<f32x4*>(memory + meeting_bytes(N, W, false)), wave, lane, acc, from, there);
+  }
+  if (there) leave<T, D, RT, C>(p, job, span, from, l16, grp, acc, sum, top);
+}
+
+// Zeros for a workgroup's rows from its `from`th on.
 template <typename T, int D, int ROWS, int THREADS>
-__device__ __forceinline__ void clear_rows(const AttendParams& p, const Job& job) {
-  for (int i = threadIdx.x; i < ROWS * (D / 4); i += THREADS) {
+__device__ __forceinline__ void clear_rows(const AttendParams& p, const Job& job, int from) {
+  for (int i = from * (D / 4) + threadIdx.x; i < ROWS * (D / 4); i += THREADS) {
     const int row = job.row0 + i / (D / 4);
-    if (row < p.rows) Place(p, job, row).template store<T>(p, job.b, i % (D / 4) * 4, f32x4{0.f, 0.f, 0.f, 0.f}, 0.f);
+    if (row < p.rows) store_four<T>(Place(p, job, row).output<T>(p, job.b) + i % (D / 4) * 4, f32x4{0.f, 0.f, 0.f, 0.f}, 0.f);
   }
 }
 
@@ -435,7 +514,7 @@ struct StagedHalf {
 // acc[rows of 16 features] += values^T p: probs[n][part][half]: of 32 tokens, group grp those of chunk 2 half at 4 grp, then those of the next chunk.
 // code_bytes, scale_bytes: of the tile's first chunk, CODES_STEP and SCALES_STEP before the next one's.
 template <int D, int BITS, int CODES_STEP, int SCALES_STEP, int RT, int PARTS>
-__device__ __forceinline__ void times_values(const uint8_t* code_bytes, const uint8_t* scale_bytes, int l16, int grp, const bf16x8 (&probs)[RT][PARTS][2], f32x4 (&acc)[RT][D / 16]) {
+__device__ __forceinline__ void times_values(const uint8_t* code_bytes, const uint8_t* scale_bytes, int l16, int grp, const bf16x8 (&probs)[RT][PARTS][2], f32x4 (&acc)[RT * (D / 16)]) {
   constexpr int BLOCKS = D / kKvBlock, EACH = BITS / 4;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
@@ -457,8 +536,8 @@ __device__ __forceinline__ void times_values(const uint8_t* code_bytes, const ui
       for (int n = 0; n < RT; ++n)
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
-          acc[n][2 * j] = mfma(first, probs[n][part][half], acc[n][2 * j]);
-          acc[n][2 * j + 1] = mfma(second, probs[n][part][half], acc[n][2 * j + 1]);
+          acc[n * (D / 16) + 2 * j] = mfma(first, probs[n][part][half], acc[n * (D / 16) + 2 * j]);
+          acc[n * (D / 16) + 2 * j + 1] = mfma(second, probs[n][part][half], acc[n * (D / 16) + 2 * j + 1]);
         }
     }
   }
@@ -508,8 +587,8 @@ __device__ __forceinline__ void walk(const AttendParams& p, const Job& job, cons
 // A wavefront's tiles, one in LDS, keys and values by themselves: the next keys are on their way from when the scores are made, the next values from when the
 // products with these are. Two whole tiles would leave half of the wavefronts no room in LDS, and one whole tile nothing on its way while it is taken.
 template <int D, int BITS, int W, bool WHOLE, typename Scores, typename Softmax, typename Values>
-__device__ __forceinline__ void walk_halves(const AttendParams& p, const Job& job, const Span& span, int wave, int lane, uint8_t* keys, Scores&& scores, Softmax&& softmax,
-                                            Values&& take_values) {
+__device__ __forceinline__ void walk_halves(const AttendParams& p, const Job& job, const Span& span, int wave, int lane, uint8_t* keys, Scores&& scores,
+                                            Softmax&& softmax, Values&& take_values) {
   typedef StagedHalf<D, BITS> Half;
   const int64_t row = job.b * p.pool.table_stride;
   uint8_t* const values = keys + Half::BYTES;
@@ -563,7 +642,7 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
   const Job job(p, ROWS);
   const Span span = span_of(p, job.b, job.row0, ROWS, job.split, W);
   if (job.split >= span.active) {
-    if (job.split == 0) clear_rows<T, D, ROWS, W * kWave>(p, job);
+    if (job.split == 0) clear_rows<T, D, ROWS, W * kWave>(p, job, 0);
     return;
   }
   uint8_t* const stages = memory + wave * (S * Tile::BYTES);
@@ -587,11 +666,11 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
     }
   }
   float most[ROWS];
-  f32x4 acc[1][D / 16], sum = {0.f, 0.f, 0.f, 0.f};  // sums are products with ones: their columns are those of acc
+  f32x4 acc[D / 16], sum = {0.f, 0.f, 0.f, 0.f};  // sums are products with ones: their columns are those of acc
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) most[r] = kNothing;
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) acc[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < D / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   const bf16x8 ones = __builtin_bit_cast(bf16x8, (u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}));
   auto take = [&](const uint8_t* tile, uint32_t chunks, int number) __attribute__((always_inline)) {
@@ -637,7 +716,7 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[0][i][e] *= mine;
+        for (int e = 0; e < 4; ++e) acc[i][e] *= mine;
     }
     // token 16 grp + l16 lies in chunk grp, group l16 / 4
     bf16_t* to = &turned[0][l16 / 4 * 16 + grp * 4 + l16 % 4];
@@ -663,60 +742,56 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
 #pragma unroll
   for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[0][i][e] += from_four_on(acc[0][i][e]);
+    for (int e = 0; e < 4; ++e) acc[i][e] += from_four_on(acc[i][e]);
   sum[0] += from_four_on(sum[0]);
   float top[1] = {most[0]}, total[1] = {sum[0]};
 #pragma unroll
   for (int r = 1; r < ROWS; ++r) top[0] = l16 == r ? most[r] : top[0];
-  if constexpr (W > 1) meet<D / 16, 1, W>(memory, wave, lane, acc, total, top);
-  if (wave > 0 || l16 >= ROWS || job.row0 + l16 >= p.rows) return;
-  const Place place(p, job, job.row0 + l16);
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) place.leave<T, D>(p, job, span, 16 * i + 4 * grp, acc[0][i], total[0], top[0]);
+  finish<T, D, 1, W>(p, job, span, memory, reinterpret_cast<float*>(memory + working_bytes(ROWS, D, BITS, W == 1)), wave, lane, acc, total, top);
 }
 
 // ---- sixteen rows at a time ---------------------------------------------------------------------------------------
 
-template <typename T, int D, int BITS, int ROWS, int W>
-__global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void cached_attention_many_kernel(const AttendParams p) {
-  constexpr int RT = ROWS / 16, BLOCKS = D / kKvBlock, PARTS = kParts<T>;
+// shared_queries: their place in LDS, or null: in registers.
+template <typename T, int D, int BITS, int RT, int W, bool SHARED>
+__device__ __forceinline__ void attend_many(const AttendParams& p, const Job& job, const Span& span, int rows, uint8_t* memory, uint8_t* shared_queries, float* stats) {
+  constexpr int BLOCKS = D / kKvBlock, PARTS = kParts<T>;
   typedef StagedHalf<D, BITS> Half;
-  extern __shared__ __align__(16) uint8_t memory[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, l16 = lane % 16, grp = lane / 16;
-  const Job job(p, ROWS);
-  const Span span = span_of(p, job.b, job.row0, min(ROWS, p.rows - job.row0), job.split, W);
-  if (job.split >= span.active) {
-    if (job.split == 0) clear_rows<T, D, ROWS, W * kWave>(p, job);
-    return;
-  }
   uint8_t* const stages = memory + wave * (2 * Half::BYTES);
   int low[RT], high[RT];
   bool empty[RT];  // rows that see nothing are taken along, and cleared at the end
-  bf16x8 q[RT][PARTS][BLOCKS];
+  bf16x8 own[SHARED ? 1 : BLOCKS * RT * PARTS];  // queries: [block][sixteen][part]
+  bf16x8* const shared = reinterpret_cast<bf16x8*>(shared_queries) + lane;
+  auto query = [&](int i) __attribute__((always_inline)) {
+    const int row = job.row0 + 16 * (i / PARTS % RT) + l16;
+    const T* src = Place(p, job, min(row, p.rows - 1)).query<T>(p, job);
+    bf16x8 q = {};
+    if (row < p.rows) q = query_part<T>(src + 8 * (grp * BLOCKS + i / (PARTS * RT)), i % PARTS, p.flip, p.keep);
+    return q;
+  };
+  if constexpr (SHARED) {
+    for (int i = wave; i < BLOCKS * RT * PARTS; i += W) shared[i * kWave] = query(i);
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int i = 0; i < BLOCKS * RT * PARTS; ++i) own[i] = query(i);
+  }
 #pragma unroll
   for (int n = 0; n < RT; ++n) {
-    const int row = job.row0 + 16 * n + l16;
-    const Seen seen(p, span, row);
+    const Seen seen(p, span, job.row0 + 16 * n + l16);
     empty[n] = seen.high <= 0;
     low[n] = seen.low, high[n] = empty[n] ? 0x7fffffff : seen.high;
-    const T* src = Place(p, job, min(row, p.rows - 1)).query<T>(p, job);
-#pragma unroll
-    for (int j = 0; j < BLOCKS; ++j)
-#pragma unroll
-      for (int part = 0; part < PARTS; ++part) {
-        q[n][part][j] = bf16x8{};
-        if (row < p.rows) q[n][part][j] = query_part<T>(src + 8 * (grp * BLOCKS + j), part, p.flip, p.keep);
-      }
   }
   // the positions that all of them see
-  const int all_low = Seen(p, span, min(job.row0 + ROWS, p.rows) - 1).low, all_high = Seen(p, span, job.row0).high;
+  const int all_low = Seen(p, span, job.row0 + rows - 1).low, all_high = Seen(p, span, job.row0).high;
   float most[RT];
-  f32x4 acc[RT][D / 16], sums[RT];
+  f32x4 acc[RT * (D / 16)], sums[RT];
 #pragma unroll
   for (int n = 0; n < RT; ++n) {
     most[n] = kNothing, sums[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < D / 16; ++i) acc[n * (D / 16) + i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
   const int octet = grp * BLOCKS, block = octet / 4;  // of the lane's features
@@ -724,20 +799,25 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
   f32x4 s[RT][4];
   bf16x8 probs[RT][2][2];
   auto scores = [&](const uint8_t* keys_at) __attribute__((always_inline)) {
+    Words<BLOCKS * BITS / 4> keys[4];
+    float scale[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
+      keys[c].load(keys_at + c * Half::CODES + block * (kKvChunk * 4 * BITS) + l16 * 4 * BITS + octet % 4 * BITS);
+      scale[c] = scale_of<0>(keys_at[4 * Half::CODES + c * Half::SCALES + l16 * BLOCKS + block]);
 #pragma unroll
       for (int n = 0; n < RT; ++n) s[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-      Words<BLOCKS * BITS / 4> keys;
-      keys.load(keys_at + c * Half::CODES + block * (kKvChunk * 4 * BITS) + l16 * 4 * BITS + octet % 4 * BITS);
-      const float scale = scale_of<0>(keys_at[4 * Half::CODES + c * Half::SCALES + l16 * BLOCKS + block]);
+    }
 #pragma unroll
-      for (int j = 0; j < BLOCKS; ++j) {
-        const bf16x8 key = eight<BITS>(keys.w + j * (BITS / 4), scale);
+    for (int j = 0; j < BLOCKS; ++j) {  // sums that do not wait for each other side by side
+      bf16x8 q[RT * PARTS];
 #pragma unroll
-        for (int n = 0; n < RT; ++n)
+      for (int i = 0; i < RT * PARTS; ++i) q[i] = SHARED ? shared[(j * RT * PARTS + i) * kWave] : own[SHARED ? 0 : j * RT * PARTS + i];
 #pragma unroll
-          for (int part = 0; part < PARTS; ++part) s[n][c] = mfma(key, q[n][part][j], s[n][c]);
+      for (int c = 0; c < 4; ++c) {
+        const bf16x8 key = eight<BITS>(keys[c].w + j * (BITS / 4), scale[c]);
+#pragma unroll
+        for (int i = 0; i < RT * PARTS; ++i) s[i / PARTS][c] = mfma(key, q[i], s[i / PARTS][c]);
       }
     }
   };
@@ -773,7 +853,7 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[n][i][e] *= f;
+          for (int e = 0; e < 4; ++e) acc[n * (D / 16) + i][e] *= f;
       }
     }
 #pragma unroll
@@ -798,18 +878,33 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
                          : walk_halves<D, BITS, W, false>(p, job, span, wave, lane, stages, scores, softmax, take_values);
   float sum[RT];
 #pragma unroll
-  for (int n = 0; n < RT; ++n) sum[n] = sums[n][0];
-  if constexpr (W > 1) meet<RT * (D / 16), RT, W>(memory, wave, lane, acc, sum, most);
-  if (wave > 0) return;
-#pragma unroll
   for (int n = 0; n < RT; ++n) {
-    const int row = job.row0 + 16 * n + l16;
-    if (row >= p.rows) continue;
-    const Place place(p, job, row);
+    sum[n] = empty[n] ? 0.f : sums[n][0], most[n] = empty[n] ? kNothing : most[n];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
-      place.leave<T, D>(p, job, span, 16 * i + 4 * grp, empty[n] ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[n][i], empty[n] ? 0.f : sum[n], empty[n] ? kNothing : most[n]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n * (D / 16) + i][e] = empty[n] ? 0.f : acc[n * (D / 16) + i][e];
   }
+  finish<T, D, RT, W>(p, job, span, memory, stats, wave, lane, acc, sum, most);
+}
+
+// Rows of queries that a sample has not, whole sixteens of them, are cleared and not taken along.
+template <typename T, int D, int BITS, int ROWS, int W>
+__global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void cached_attention_many_kernel(const AttendParams p) {
+  constexpr bool SHARED = queries_in_lds(ROWS, kParts<T>);
+  extern __shared__ __align__(16) uint8_t memory[];
+  uint8_t* const queries = memory + working_bytes(ROWS, D, BITS, W == 1);
+  float* const stats = reinterpret_cast<float*>(queries + (SHARED ? ROWS * D * 2 : 0));
+  const Job job(p, ROWS);
+  const int row_end = min(job.row0 + ROWS, p.rows);
+  const Span span = span_of(p, job.b, job.row0, row_end - job.row0, job.split, W);
+  const bool mine = job.split < span.active;
+  const int rows = mine ? min(row_end, p.group.d * span.news) - job.row0 : 0, taken = (rows + 15) & ~15;  // rows that there are
+  if (job.split == 0 && taken < ROWS) clear_rows<T, D, ROWS, W * kWave>(p, job, taken);
+  if (!mine) return;
+  if (ROWS == 16 || taken == 16) attend_many<T, D, BITS, 1, W, SHARED>(p, job, span, rows, memory, queries, stats);
+  else if (ROWS == 32 || taken == 32) attend_many<T, D, BITS, 2, W, SHARED>(p, job, span, rows, memory, queries, stats);
+  else attend_many<T, D, BITS, ROWS / 16, W, SHARED>(p, job, span, rows, memory, queries, stats);
 }
 
 // More than the 64 KB of LDS that a launch may have unasked.
@@ -822,7 +917,7 @@ template <typename T, int D, int BITS, int ROWS, bool ALONE>
 void launch_rows(const AttendParams& p, uint32_t groups, hipStream_t s) {
   constexpr Shape shape = shape_of(ROWS, D, ALONE);
   static_assert(Staged<D, BITS>::BYTES == tile_bytes(D, BITS) && StagedHalf<D, BITS>::BYTES == half_bytes(D, BITS));
-  constexpr int bytes = lds_bytes(ROWS, D, BITS, ALONE), threads = shape.waves * kWave;
+  constexpr int bytes = lds_bytes(ROWS, D, BITS, kParts<T>, ALONE), threads = shape.waves * kWave;
   if constexpr (ROWS <= 4) launch_with(cached_attention_few_kernel<T, D, BITS, ROWS, shape.waves, shape.stages>, groups, threads, bytes, p, s);
   else launch_with(cached_attention_many_kernel<T, D, BITS, ROWS, shape.waves>, groups, threads, bytes, p, s);
 }
@@ -835,6 +930,9 @@ void launch_attend(const AttendParams& p, int rows, bool alone, uint32_t groups,
   }
   if (rows == 16) alone ? launch_rows<T, D, BITS, 16, true>(p, groups, s) : launch_rows<T, D, BITS, 16, false>(p, groups, s);
   if (rows == 32) launch_rows<T, D, BITS, 32, false>(p, groups, s);
+  if constexpr (kParts<T> == 1) {
+    if (rows == 48) launch_rows<T, D, BITS, 48, false>(p, groups, s);
+  }
 }
 template <int BITS>
 void dispatch_attend(const AttendParams& p, int d, bool f16, int rows, bool alone, uint32_t groups, hipStream_t s) {

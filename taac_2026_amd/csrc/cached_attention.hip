@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256) void cached_attention_join_kernel(const Attend
   const int t = static_cast<int>(out_row - token * p.T), b = static_cast<int>(token / p.H), h = static_cast<int>(token - static_cast<int64_t>(b) * p.H);
   const int head = p.group.over(h), row = t * p.group.d + h - head * p.group.d, row0 = row / tile_rows * tile_rows;
   const Span span = span_of(p, b, row0, min(tile_rows, p.rows - row0), 0, waves);
-  if (span.active <= 1) return;
+  if (span.active <= 1 || t >= span.news) return;  // whole already, or zeros
   const float* part = p.partial + out_row * p.splits.d * D + c;
   const float* stats = p.partial + p.all_rows * p.splits.d * D + out_row * p.splits.d * 2;
   float top = kNothing, l = 0.f;
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void cached_attention_join_kernel(const Attend
   }
   Job job;
   job.head = head;
-  if (group == 0) Place(p, job, row).template store<T>(p, b, c, total, l);
+  if (group == 0) store_four<T>(Place(p, job, row).output<T>(p, b) + c, total, l == 0.f ? 0.f : 1.f / l);
 }
 
 // ---- the host -----------------------------------------------------------------------------------------------------
@@ -71,7 +71,7 @@ constexpr int64_t kMostGroups = 1 << 23;  // of a launch: below 2^31 threads
 
 // How a call is cut. A unit is a tile of rows of a key head of a sample.
 struct Plan {
-  int rows;       // of a tile: 1, 2, 4, 16 or 32
+  int rows;       // of a tile: 1, 2, 4, 16, 32 or 48
   int row_tiles;  // of a key head
   int splits;     // of a history
   int waves;      // of a workgroup
@@ -87,9 +87,11 @@ int64_t alone_from(int rows, int32_t d) { return rows > 4 ? 8192 : d == 32 ? 409
 Plan plan_of(int64_t B, int32_t heads, int32_t group, int32_t T, int32_t d, int bits, int64_t held, bool parts) {
   Plan plan{};
   const int64_t rows = static_cast<int64_t>(group) * T;
+  const int64_t tiles48 = (rows + 47) / 48, parts48 = held / (kTile * 8);
+  const bool wide = !parts && tiles48 * 5 < (rows + 31) / 32 * 4 && B * heads * tiles48 * (parts48 < 4 ? 1 : parts48) >= 256;
   // up to 4 rows (2 in two parts) in the one form. In the other 16, or 32, which share the conversion of the codes: three sixteens would leave one wavefront to a SIMD, and four
   // no registers.
-  plan.rows = rows <= 2 ? static_cast<int>(rows) : rows <= 4 && !parts ? 4 : rows <= 16 ? 16 : 32;
+  plan.rows = rows <= 2 ? static_cast<int>(rows) : rows <= 4 && !parts ? 4 : rows <= 16 ? 16 : wide ? 48 : 32;
   plan.row_tiles = static_cast<int>((rows + plan.rows - 1) / (plan.rows > 0 ? plan.rows : 1));
   const int64_t units = B * heads * plan.row_tiles;
   plan.alone = plan.rows <= 16 && units >= alone_from(plan.rows, d);
@@ -98,7 +100,7 @@ Plan plan_of(int64_t B, int32_t heads, int32_t group, int32_t T, int32_t d, int 
   // Histories are split until the card is full, by LDS and registers; twice as many workgroups cost more than a better balance gives back (4 x 8 key heads of 128 features,
   // 65536 tokens: 56 us, 60 with twice as many; 64 x 4 x 2048 tokens, 24 queries: 39 and 52). A split has a tile for each of its wavefronts, and below four (six
   // of narrower heads) the kernel that joins them takes longer than the tiles would: one sample of 768 tokens 5.7 us as a whole, of 1024 in four 7.9.
-  const int by_lds = 163840 / lds_bytes(plan.rows, d, bits, plan.alone), by_registers = 4 * shape.per_simd / shape.waves;
+  const int by_lds = 163840 / lds_bytes(plan.rows, d, bits, parts ? 2 : 1, plan.alone), by_registers = 4 * shape.per_simd / shape.waves;
   const int64_t resident = 256 * (by_lds < by_registers ? by_lds : by_registers), most = held / (kTile * shape.waves);
   int64_t splits = resident / (units > 0 ? units : 1);
   splits = splits < most ? splits : most;

@@ -100,6 +100,20 @@ def test_long_histories(device, bits, dtype, width, group, tokens, window):
     _check(got, q, k, v, lengths, [tokens] * 3, window)
 
 
+@pytest.mark.parametrize("bits,dtype", [(4, torch.bfloat16), (8, torch.bfloat16), (8, torch.float16)])
+@pytest.mark.parametrize("width", [32, 64, 128])
+@pytest.mark.parametrize("batch,lengths", [(1, [5000]), (40, [900, 64, 7, 300, 0]), (3, [2100, 65, 40])])
+@pytest.mark.parametrize("group,tokens", [(2, 24), (1, 40), (3, 30)])
+def test_ragged_new_tokens(device, bits, dtype, width, batch, lengths, group, tokens):
+    """Every number of sixteens of rows that there are, of histories as a whole and in parts; the other rows are zeros."""
+    lengths = (lengths * batch)[: 5 * batch]
+    news = [(7 * i + 11) % (tokens + 1) if i else tokens // 3 for i in range(len(lengths))]
+    cache, pages, k, v = _filled(device, lengths, 2, width, bits, 64)
+    q = _queries(device, len(lengths), 2 * group, tokens, width, dtype)
+    got = cached_attention(q, cache, pages, torch.tensor(lengths, device=device), query_lengths=torch.tensor(news, device=device))
+    _check(got, q, k, v, lengths, news)
+
+
 @pytest.mark.parametrize("width", [64, 128])
 def test_fp16_rows_in_the_other_form(device, width):
     """Three and four rows of fp16 are cut into more splits than those of bf16."""
