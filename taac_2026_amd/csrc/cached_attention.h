@@ -19,10 +19,12 @@
 // and sums are fp32; probabilities enter as two parts (16 bits), in the first form in columns that would be empty. The maximum moves when a score exceeds it
 // by a factor of 2^8, which cancels.
 //
-// Measured: 4 samples of 65536 tokens, 32 heads over 8 of 128 features in 4 bits: 51 us and 5 for the join, 5.6 TB/s of the cache (tiles in registers, one ahead: 101, for the
-// registers left one wavefront to a SIMD, and page numbers that wait behind the rows). 1024 samples of up to 512 tokens, 8 heads of 32: 21 us, of which 9 are a launch whose
-// samples have one tile, and 2.7 every tile more, 6.7 TB/s. 64 samples of up to 2048 tokens, 24 queries of 8 heads over 4 of 128 in 8 bits: 37 us, matrix and vector
-// instructions side by side (a tile of 32 rows has 104 and 600, of which 270 convert the codes).
+// Measured: 4 samples of 65536 tokens, 32 heads over 8 of 128 features in 4 bits: 50 us and 5 for the join, 5.6 TB/s of the cache (tiles in registers, one ahead: 101, for the
+// registers left one wavefront to a SIMD, and page numbers that wait behind the rows). 1024 samples of up to 512 tokens, 8 heads of 32: 22 us, of which 8 are a launch whose
+// samples have one tile, and 2.7 every tile more, 6.7 TB/s. 64 samples of 2048 tokens, 24 queries of 8 heads over 4 of 128 in 8 bits: 34 us, of up to 2048 tokens and up to 24
+// queries 27. A tile of 32 rows has 104 matrix and 524 vector instructions there, of which 270 convert the codes; those of one wavefront do not overlap (six products with three
+// additions behind each take 184 cycles, the products alone 120, the additions alone 72), those of two do in part. The end of a
+// workgroup (its wavefronts' sums joined, divided, written) is shared by all of them: done by the first one it took half of a call with one tile of 48 rows, 7 of 15 us.
 #pragma once
 
 #include "kv_cache.h"
@@ -277,14 +279,13 @@ __device__ __forceinline__ void store_four(T* to, const f32x4& total, float inv)
 template <typename T, int D, int RT, int C>
 __device__ __forceinline__ void leave(const AttendParams& p, const Job& job, const Span& span, int from, int l16, int grp, const f32x4* part, const float (&sum)[RT],
                                       const float (&top)[RT]) {
+  const float sum1 = sum[RT > 1 ? 1 : 0], sum2 = sum[RT > 2 ? 2 : 0], top1 = top[RT > 1 ? 1 : 0], top2 = top[RT > 2 ? 2 : 0];
   constexpr int EACH = C < D / 16 ? C : D / 16, FOURS = D / 16 % C == 0 || C % (D / 16) == 0 ? EACH : 1;  // of the same column
 #pragma unroll
   for (int e = 0; e < C; e += FOURS) {
     const int n = (from + e) / (D / 16), row = job.row0 + 16 * n + l16, c = (from + e) % (D / 16) * 16 + 4 * grp;
     if (row >= p.rows) continue;
-    float l = sum[0], most = top[0];
-#pragma unroll
-    for (int r = 1; r < RT; ++r) l = n == r ? sum[r] : l, most = n == r ? top[r] : most;
+    const float l = n == 0 ? sum[0] : n == 1 ? sum1 : sum2, most = n == 0 ? top[0] : n == 1 ? top1 : top2;
     const Place place(p, job, row);
     if (span.active > 1 && place.t < span.news) {  // rows of no query are zeros whoever writes them
       const int64_t at = ((static_cast<int64_t>(job.b) * p.H + place.h) * p.T + place.t) * p.splits.d + job.split;

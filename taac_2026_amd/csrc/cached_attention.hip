@@ -9,20 +9,22 @@ namespace {
 
 // ---- the splits' parts --------------------------------------------------------------------------------------------
 
-// A wavefront to a row: its lanes are 64 / (D / 4) groups that take the splits in turn.
-template <typename T, int D>
+// Lanes of four features to a row. Of many splits a whole wavefront: its lanes are 64 / (D / 4) groups that take them in turn. Bound by latency: calls of two
+// splits, 64 samples of 1024 tokens, 32 rows, take 28.3 us with wavefronts, 24.9 with lanes; of eight, 4 samples of 2000 tokens, 48 rows, 13.1 and 13.7.
+template <typename T, int D, bool MANY>
 __global__ __launch_bounds__(256) void cached_attention_join_kernel(const AttendParams p, int tile_rows, int waves) {
-  constexpr int LANES = D / 4, GROUPS = kWave / LANES, AT_ONCE = 8;
-  const int64_t out_row = static_cast<int64_t>(blockIdx.x) * (256 / kWave) + threadIdx.x / kWave;
+  typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
+  constexpr int LANES = D / 4, GROUPS = MANY ? kWave / LANES : 1, AT_ONCE = MANY ? 8 : 2;
+  const int64_t out_row = static_cast<int64_t>(blockIdx.x) * (256 / (LANES * GROUPS)) + threadIdx.x / (LANES * GROUPS);
   if (out_row >= p.all_rows) return;
-  const int lane = threadIdx.x % kWave, c = lane % LANES * 4, group = lane / LANES;
+  const int c = threadIdx.x % LANES * 4, group = threadIdx.x % (LANES * GROUPS) / LANES;
   const int64_t token = out_row / p.T;
   const int t = static_cast<int>(out_row - token * p.T), b = static_cast<int>(token / p.H), h = static_cast<int>(token - static_cast<int64_t>(b) * p.H);
   const int head = p.group.over(h), row = t * p.group.d + h - head * p.group.d, row0 = row / tile_rows * tile_rows;
   const Span span = span_of(p, b, row0, min(tile_rows, p.rows - row0), 0, waves);
   if (span.active <= 1 || t >= span.news) return;  // whole already, or zeros
   const float* part = p.partial + out_row * p.splits.d * D + c;
-  const float* stats = p.partial + p.all_rows * p.splits.d * D + out_row * p.splits.d * 2;
+  const f32x2* stats = reinterpret_cast<const f32x2*>(p.partial + p.all_rows * p.splits.d * D) + out_row * p.splits.d;
   float top = kNothing, l = 0.f;
   f32x4 total = {0.f, 0.f, 0.f, 0.f};
   for (int first = group; first < span.active; first += GROUPS * AT_ONCE) {
@@ -32,7 +34,8 @@ __global__ __launch_bounds__(256) void cached_attention_join_kernel(const Attend
     for (int i = 0; i < AT_ONCE; ++i) {  // those behind the last count as the last once more, with no weight
       const int split = min(first + i * GROUPS, span.active - 1);
       v[i] = *reinterpret_cast<const f32x4*>(part + static_cast<int64_t>(split) * D);
-      most[i] = stats[2 * split], sum[i] = stats[2 * split + 1];
+      const f32x2 both = stats[split];
+      most[i] = both[0], sum[i] = both[1];
     }
 #pragma unroll
     for (int i = 0; i < AT_ONCE; ++i) up = fmaxf(up, most[i]);
@@ -50,7 +53,7 @@ __global__ __launch_bounds__(256) void cached_attention_join_kernel(const Attend
     }
   }
 #pragma unroll
-  for (int off = LANES; off < kWave; off *= 2) {
+  for (int off = LANES; off < LANES * GROUPS; off *= 2) {
     const float other = __shfl_xor(top, off, kWave), up = fmaxf(top, other), f = __builtin_amdgcn_exp2f(top - up), g = __builtin_amdgcn_exp2f(other - up);
     const float other_l = __shfl_xor(l, off, kWave);
     top = up, l = l * f + other_l * g;
@@ -84,23 +87,19 @@ struct Plan {
 //   16 rows, 64 features: 27.9 : 36.2 at 8192 units of 256, 42.8 : 46.4 of 512; 17.7 : 21.0 of 256 and 46.6 : 38.9 of 1024 at 4096
 int64_t alone_from(int rows, int32_t d) { return rows > 4 ? 8192 : d == 32 ? 4096 : 2048; }
 
-Plan plan_of(int64_t B, int32_t heads, int32_t group, int32_t T, int32_t d, int bits, int64_t held, bool parts) {
+// Tiles of so many rows.
+Plan cut(int64_t B, int32_t heads, int64_t rows, int tile, int32_t d, int bits, int64_t held, bool parts) {
   Plan plan{};
-  const int64_t rows = static_cast<int64_t>(group) * T;
-  const int64_t tiles48 = (rows + 47) / 48, parts48 = held / (kTile * 8);
-  const bool wide = !parts && tiles48 * 5 < (rows + 31) / 32 * 4 && B * heads * tiles48 * (parts48 < 4 ? 1 : parts48) >= 256;
-  // up to 4 rows (2 in two parts) in the one form. In the other 16, or 32, which share the conversion of the codes: three sixteens would leave one wavefront to a SIMD, and four
-  // no registers.
-  plan.rows = rows <= 2 ? static_cast<int>(rows) : rows <= 4 && !parts ? 4 : rows <= 16 ? 16 : wide ? 48 : 32;
-  plan.row_tiles = static_cast<int>((rows + plan.rows - 1) / (plan.rows > 0 ? plan.rows : 1));
+  plan.rows = tile;
+  plan.row_tiles = static_cast<int>((rows + tile - 1) / (tile > 0 ? tile : 1));
   const int64_t units = B * heads * plan.row_tiles;
-  plan.alone = plan.rows <= 16 && units >= alone_from(plan.rows, d);
-  const Shape shape = shape_of(plan.rows, d, plan.alone);
+  plan.alone = tile <= 16 && units >= alone_from(tile, d);
+  const Shape shape = shape_of(tile, d, plan.alone);
   plan.waves = shape.waves;
   // Histories are split until the card is full, by LDS and registers; twice as many workgroups cost more than a better balance gives back (4 x 8 key heads of 128 features,
-  // 65536 tokens: 56 us, 60 with twice as many; 64 x 4 x 2048 tokens, 24 queries: 39 and 52). A split has a tile for each of its wavefronts, and below four (six
-  // of narrower heads) the kernel that joins them takes longer than the tiles would: one sample of 768 tokens 5.7 us as a whole, of 1024 in four 7.9.
-  const int by_lds = 163840 / lds_bytes(plan.rows, d, bits, parts ? 2 : 1, plan.alone), by_registers = 4 * shape.per_simd / shape.waves;
+  // 65536 tokens: 56 us, 60 with twice as many). A split has a tile for each of its wavefronts, and below four (six of narrower heads) the kernel that joins them
+  // takes longer than the tiles would: one sample of 768 tokens 5.7 us as a whole, of 1024 in four 7.9.
+  const int by_lds = 163840 / lds_bytes(tile, d, bits, parts ? 2 : 1, plan.alone), by_registers = 4 * shape.per_simd / shape.waves;
   const int64_t resident = 256 * (by_lds < by_registers ? by_lds : by_registers), most = held / (kTile * shape.waves);
   int64_t splits = resident / (units > 0 ? units : 1);
   splits = splits < most ? splits : most;
@@ -108,12 +107,35 @@ Plan plan_of(int64_t B, int32_t heads, int32_t group, int32_t T, int32_t d, int 
   return plan;
 }
 
+Plan plan_of(int64_t B, int32_t heads, int32_t group, int32_t T, int32_t d, int bits, int64_t held, bool parts) {
+  const int64_t rows = static_cast<int64_t>(group) * T;
+  // up to 4 rows (2 in two parts) in the one form
+  if (rows <= 2 || (rows <= 4 && !parts)) return cut(B, heads, rows, rows <= 2 ? static_cast<int>(rows) : 4, d, bits, held, parts);
+  if (rows <= 16) return cut(B, heads, rows, 16, d, bits, held, parts);
+  // In the other 16, or 32, which share the conversion of the codes. Where a workgroup of eight wavefronts to a CU just fills the card, up to 48 rows in one, which need no
+  // splits and no joining; of four sixteens the sums would leave no registers. 4 key heads, 2000 tokens, 48 rows : 32: of 128 features in 8 bits, 18 rows, 48 samples 25.1 : 29.6
+  // us, 64 samples 29.8 : 32.3, 100 samples 47.8 : 43.2; 48 rows, 64 samples 32.9 : 36.8, 100 samples 56.5 : 65.9; of 64 in 4 bits, 18 rows, 64 samples 16.3 : 19.7, 100 samples
+  // 29.6 : 24.1; 48 rows 20.8 : 23.9 and 38.7 : 37.2. Of 500 tokens 16.2 : 16.3 and 29.1 : 26.6, 11.0 : 10.3 and 20.0 : 14.8.
+  if (rows <= 48 && !parts && held >= 1024 && B * heads <= 256) {
+    const Plan wide = cut(B, heads, rows, 48, d, bits, held, parts);
+    if (B * heads * wide.splits >= 192) return wide;
+  }
+  return cut(B, heads, rows, 32, d, bits, held, parts);
+}
+
+template <typename T, int D>
+void launch_join(const AttendParams& p, const Plan& plan, hipStream_t s) {
+  const bool many = plan.splits > 4;
+  const int64_t at_once = 256 / (many ? kWave : D / 4);
+  const dim3 grid(static_cast<uint32_t>((p.all_rows + at_once - 1) / at_once));
+  if (many) hipLaunchKernelGGL((cached_attention_join_kernel<T, D, true>), grid, dim3(256), 0, s, p, plan.rows, plan.waves);
+  else hipLaunchKernelGGL((cached_attention_join_kernel<T, D, false>), grid, dim3(256), 0, s, p, plan.rows, plan.waves);
+}
 template <typename T>
-void launch_join(const AttendParams& p, const Plan& plan, int d, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>((p.all_rows + 256 / kWave - 1) / (256 / kWave)));
-  if (d == 32) hipLaunchKernelGGL((cached_attention_join_kernel<T, 32>), grid, dim3(256), 0, s, p, plan.rows, plan.waves);
-  if (d == 64) hipLaunchKernelGGL((cached_attention_join_kernel<T, 64>), grid, dim3(256), 0, s, p, plan.rows, plan.waves);
-  if (d == 128) hipLaunchKernelGGL((cached_attention_join_kernel<T, 128>), grid, dim3(256), 0, s, p, plan.rows, plan.waves);
+void join(const AttendParams& p, const Plan& plan, int d, hipStream_t s) {
+  if (d == 32) launch_join<T, 32>(p, plan, s);
+  if (d == 64) launch_join<T, 64>(p, plan, s);
+  if (d == 128) launch_join<T, 128>(p, plan, s);
 }
 
 }  // namespace
@@ -176,6 +198,6 @@ extern "C" int taac_cached_attention_fwd(const void* q, void* o, const void* cac
     const uint32_t groups = static_cast<uint32_t>((B - first < at_once ? B - first : at_once) * each);
     bits == 4 ? attend_4(p, d, f16, plan.rows, plan.alone, groups, s) : attend_8(p, d, f16, plan.rows, plan.alone, groups, s);
   }
-  if (plan.splits > 1) f16 ? launch_join<f16_t>(p, plan, d, s) : launch_join<bf16_t>(p, plan, d, s);
+  if (plan.splits > 1) f16 ? join<f16_t>(p, plan, d, s) : join<bf16_t>(p, plan, d, s);
   return check_launch(name);
 }
