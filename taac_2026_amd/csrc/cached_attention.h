@@ -79,6 +79,12 @@ __host__ __device__ constexpr int meeting_bytes(int n, int waves, bool second) {
   }
   return most;
 }
+// Whether fewer columns than a workgroup's find room where all of them do.
+__host__ __device__ constexpr bool meeting_fits(int n, int waves, int each, int bytes) {
+  for (; n > 0; n -= each)
+    if (meeting_bytes(n, waves, false) + meeting_bytes(n, waves, true) > bytes) return false;
+  return true;
+}
 __host__ __device__ constexpr int stats_bytes(int rows, int waves) { return waves > 1 ? waves * (rows <= 16 ? 16 : rows) * 8 : 0; }
 // of the tiles, or of the meeting behind them; then the queries and the statistics
 __host__ __device__ constexpr int working_bytes(int rows, int d, int bits, bool alone) {
@@ -894,7 +900,9 @@ template <typename T, int D, int BITS, int ROWS, int W>
 __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void cached_attention_many_kernel(const AttendParams p) {
   constexpr bool SHARED = queries_in_lds(ROWS, kParts<T>);
   extern __shared__ __align__(16) uint8_t memory[];
-  uint8_t* const queries = memory + working_bytes(ROWS, D, BITS, W == 1);
+  constexpr int WORKING = working_bytes(ROWS, D, BITS, W == 1);
+  static_assert(meeting_fits(ROWS / 16 * (D / 16), W, D / 16, WORKING));
+  uint8_t* const queries = memory + WORKING;
   float* const stats = reinterpret_cast<float*>(queries + (SHARED ? ROWS * D * 2 : 0));
   const Job job(p, ROWS);
   const int row_end = min(job.row0 + ROWS, p.rows);
