@@ -34,40 +34,79 @@ struct CacheParams {
   int32_t T, chunks, starts_int64;
 };
 
+typedef __attribute__((__vector_size__(2 * sizeof(short)))) short s16x2;
+typedef __attribute__((__vector_size__(2 * sizeof(unsigned short)))) unsigned short u16x2;
+typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 f16x2;
+typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
+
+// Eight neighbouring features as they lie in memory.
 template <typename T>
-struct Eight {  // eight neighbouring features
-  float f[8];
+struct Eight {
+  static constexpr int WORDS = 2 * sizeof(T);
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = 0;
+  }
   __device__ __forceinline__ void load(const T* p) {
-    if constexpr (sizeof(T) == 4) {
-      const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = a[i], f[4 + i] = b[i];
-    } else {
-      const typename Vec8<T>::type a = *reinterpret_cast<const typename Vec8<T>::type*>(p);
+    for (int i = 0; i < WORDS / 4; ++i) {
+      const u32x4 v = reinterpret_cast<const u32x4*>(p)[i];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(a[i]);
+      for (int j = 0; j < 4; ++j) w[4 * i + j] = v[j];
     }
   }
-  __device__ __forceinline__ void store(T* p) const {
+  // The largest magnitude, found among the bits without the sign, whose order is that of the numbers, then infinity, then NaN. finite: none of the last two.
+  __device__ __forceinline__ float most(bool& finite) const {
     if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<f32x4*>(p)[0] = f32x4{f[0], f[1], f[2], f[3]};
-      reinterpret_cast<f32x4*>(p)[1] = f32x4{f[4], f[5], f[6], f[7]};
-    } else {
-      typename Vec8<T>::type a;
+      uint32_t m = w[0] & 0x7fffffffu;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = static_cast<T>(f[i]);
-      *reinterpret_cast<typename Vec8<T>::type*>(p) = a;
+      for (int i = 1; i < WORDS; ++i) m = max(m, w[i] & 0x7fffffffu);
+      finite &= m < 0x7f800000u;
+      return __builtin_bit_cast(float, m);
+    } else {
+      u16x2 m = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
+#pragma unroll
+      for (int i = 1; i < WORDS; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+      const uint32_t both = __builtin_bit_cast(uint32_t, m), top = max(both & 0xffffu, both >> 16);
+      if constexpr (__is_same(T, bf16_t)) {
+        finite &= top < 0x7f80u;
+        return __builtin_bit_cast(float, top << 16);
+      } else {
+        finite &= top < 0x7c00u;
+        return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(top)));
+      }
     }
+  }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, static_cast<uint32_t>(w[i]));
+    else if constexpr (__is_same(T, bf16_t)) return __builtin_bit_cast(float, i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)))));
   }
 };
+template <typename T>
+__device__ __forceinline__ void store_eight(T* p, const float (&f)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<f32x4*>(p)[0] = f32x4{f[0], f[1], f[2], f[3]};
+    reinterpret_cast<f32x4*>(p)[1] = f32x4{f[4], f[5], f[6], f[7]};
+  } else {
+    typename Vec8<T>::type a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = static_cast<T>(f[i]);
+    *reinterpret_cast<typename Vec8<T>::type*>(p) = a;
+  }
+}
 
 // The least power of two 2^e with max < 7 2^e (464 2^e), as e + 127, for a finite max. The carry out of the fraction is the step to the next power: 7 and 464
 // are 1.75 and 1.8125 of one. Kept between 2^-117, under which the smallest code would be subnormal, and what keeps the largest code finite.
 template <int BITS>
+constexpr int kMostScale = BITS == 4 ? 252 : 246;
+template <int BITS>
 __device__ __forceinline__ int scale_byte(float most) {
   const uint32_t up = BITS == 4 ? 0x200000u : 0x180000u;
   const int e = static_cast<int>((__builtin_bit_cast(uint32_t, most) + up) >> 23) - (BITS == 4 ? 2 : 8);
-  return min(max(e, 10), BITS == 4 ? 252 : 246);
+  return min(max(e, 10), kMostScale<BITS>);
 }
 
 // Codes of eight values in order: one word of 4 bits, two of 8.
@@ -75,36 +114,45 @@ template <int BITS>
 struct Codes {
   uint32_t w[BITS / 4];
 };
-template <int BITS>
-__device__ __forceinline__ Codes<BITS> encode(const float (&f)[8], int byte) {
-  typedef __attribute__((__vector_size__(2 * sizeof(short)))) short s16x2;
-  const float back = __builtin_bit_cast(float, static_cast<uint32_t>(254 - byte) << 23);  // 2^-e
-  float y[8];
-  constexpr float kMost = BITS == 4 ? 6.f : 448.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = fminf(fmaxf(f[i] * back, -kMost), kMost);
-  Codes<BITS> c;
+// Two features, x / scale, to the nearest code, in one instruction from the type that they have.
+template <int BITS, int I, typename T>
+__device__ __forceinline__ void two_codes(Codes<BITS>& c, const Eight<T>& x, float scale) {
   if constexpr (BITS == 4) {
-    uint32_t w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[0], y[1], 1.f, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], 1.f, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], 1.f, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], 1.f, 3);
-    c.w[0] = w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      s16x2 w = {0, 0};
-      w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, y[4 * i], y[4 * i + 1], 1.f, false);
-      w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, y[4 * i + 2], y[4 * i + 3], 1.f, true);
-      c.w[i] = __builtin_bit_cast(uint32_t, w);
+    if constexpr (sizeof(T) == 4) {
+      c.w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c.w[0], x.at(2 * I), x.at(2 * I + 1), scale, I);
+    } else if constexpr (__is_same(T, bf16_t)) {
+      c.w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c.w[0], __builtin_bit_cast(bf16x2, static_cast<uint32_t>(x.w[I])), scale, I);
+    } else {
+      c.w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c.w[0], __builtin_bit_cast(f16x2, static_cast<uint32_t>(x.w[I])), scale, I);
     }
+  } else {
+    s16x2 w = __builtin_bit_cast(s16x2, static_cast<uint32_t>(c.w[I / 2]));
+    if constexpr (sizeof(T) == 4) w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x.at(2 * I), x.at(2 * I + 1), scale, I % 2 != 0);
+    else if constexpr (__is_same(T, bf16_t)) w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2, static_cast<uint32_t>(x.w[I])), scale, I % 2 != 0);
+    else w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2, static_cast<uint32_t>(x.w[I])), scale, I % 2 != 0);
+    c.w[I / 2] = __builtin_bit_cast(uint32_t, w);
+  }
+}
+// Codes of eight features under the scale 2^e that they share, e + 127 = byte.
+template <int BITS, typename T>
+__device__ __forceinline__ Codes<BITS> encode(const Eight<T>& x, int byte) {
+  const float scale = kv_scale(byte);
+  Codes<BITS> c;
+#pragma unroll
+  for (int i = 0; i < BITS / 4; ++i) c.w[i] = 0;
+  if (__is_same(T, f16_t) || byte < kMostScale<BITS>) {
+    two_codes<BITS, 0>(c, x, scale), two_codes<BITS, 1>(c, x, scale), two_codes<BITS, 2>(c, x, scale), two_codes<BITS, 3>(c, x, scale);
+  } else {  // under the largest scale a number may be beyond the largest code
+    const float end = (BITS == 4 ? 6.f : 448.f) * scale;
+    Eight<float> f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.w[i] = __builtin_bit_cast(uint32_t, fminf(fmaxf(x.at(i), -end), end));
+    two_codes<BITS, 0>(c, f, scale), two_codes<BITS, 1>(c, f, scale), two_codes<BITS, 2>(c, f, scale), two_codes<BITS, 3>(c, f, scale);
   }
   return c;
 }
 template <int BITS>
 __device__ __forceinline__ void decode(const Codes<BITS>& c, float scale, float (&f)[8]) {
-  typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
   f32x2 p[4];
   if constexpr (BITS == 4) {
     p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.w[0], scale, 0);
@@ -155,26 +203,18 @@ __global__ __launch_bounds__(kThreads) void kv_write_rows_kernel(const CachePara
   v.load(static_cast<const T*>(p.v) + at.b * p.vs[0] + at.h * p.vs[1] + at.t * p.vs[2] + 8 * s);
   const int in_page = static_cast<int>(at.position & ((1 << p.pool.page_shift) - 1)), token = in_page % kKvChunk;
   uint8_t* record = p.pool.data + kv_record(p.pool, page, at.h, in_page / kKvChunk, kv_record_bytes(D, BITS));
-  float k_most = 0.f, v_most = 0.f;
   bool finite = true;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    k_most = fmaxf(k_most, fabsf(k.f[i]));
-    v_most = fmaxf(v_most, fabsf(v.f[i]));
-    finite &= fabsf(k.f[i]) <= 3.4028235e38f && fabsf(v.f[i]) <= 3.4028235e38f;
-  }
-  k_most = group_max<4>(k_most);
-  v_most = group_max<4>(v_most);
+  const float k_most = group_max<4>(k.most(finite)), v_most = group_max<4>(v.most(finite));
   int bad = !finite;
 #pragma unroll
   for (int off = LANES / 2; off > 0; off /= 2) bad |= __shfl_xor(bad, off, kWave);
   int k_scale = scale_byte<BITS>(k_most), v_scale = scale_byte<BITS>(v_most);
   if (bad) {
-    k_scale = kKvNotFinite, v_scale = 127;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) k.f[i] = v.f[i] = 0.f;
+    k_scale = v_scale = 127;
+    k.clear(), v.clear();
   }
-  const Codes<BITS> kc = encode<BITS>(k.f, bad ? 127 : k_scale), vc = encode<BITS>(v.f, v_scale);
+  const Codes<BITS> kc = encode<BITS>(k, k_scale), vc = encode<BITS>(v, v_scale);
+  if (bad) k_scale = kKvNotFinite;
   uint8_t* keys = record + block * (kKvChunk * kKvBlock * BITS / 8) + token * (kKvBlock * BITS / 8) + sub * BITS;
   if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(keys) = kc.w[0];
   else *reinterpret_cast<u32x2*>(keys) = u32x2{kc.w[0], kc.w[1]};
@@ -206,10 +246,10 @@ __global__ __launch_bounds__(kThreads) void kv_read_rows_kernel(const CacheParam
   const int s = threadIdx.x % LANES, block = s / 4, sub = s % 4;
   const Row at(p, row);
   const int64_t page = at.there ? kv_page(p.pool, at.b, at.position >> p.pool.page_shift) : -1;
-  Eight<T> k, v;
+  float k[8], v[8];
   if (page < 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) k.f[i] = v.f[i] = 0.f;
+    for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
   } else {
     const int in_page = static_cast<int>(at.position & ((1 << p.pool.page_shift) - 1)), token = in_page % kKvChunk;
     const uint8_t* record = p.pool.data + kv_record(p.pool, page, at.h, in_page / kKvChunk, kv_record_bytes(D, BITS));
@@ -237,11 +277,11 @@ __global__ __launch_bounds__(kThreads) void kv_read_rows_kernel(const CacheParam
     }
     const uint32_t k_scale = record[kv_key_scale_at(D, BITS) + token * BLOCKS + block];
     const uint32_t v_scale = k_scale == kKvNotFinite ? kKvNotFinite : record[kv_value_scale_at(D, BITS) + (group * BLOCKS + block) * 4 + of4];
-    decode<BITS>(kc, kv_scale(k_scale), k.f);
-    decode<BITS>(vc, kv_scale(v_scale), v.f);
+    decode<BITS>(kc, kv_scale(k_scale), k);
+    decode<BITS>(vc, kv_scale(v_scale), v);
   }
-  k.store(static_cast<T*>(p.k_out) + at.b * p.ks[0] + at.h * p.ks[1] + at.t * p.ks[2] + 8 * s);
-  v.store(static_cast<T*>(p.v_out) + at.b * p.vs[0] + at.h * p.vs[1] + at.t * p.vs[2] + 8 * s);
+  store_eight(static_cast<T*>(p.k_out) + at.b * p.ks[0] + at.h * p.ks[1] + at.t * p.ks[2] + 8 * s, k);
+  store_eight(static_cast<T*>(p.v_out) + at.b * p.vs[0] + at.h * p.vs[1] + at.t * p.vs[2] + 8 * s, v);
 }
 
 // ---- many tokens: chunk by chunk -----------------------------------------------------------------------------------
@@ -405,38 +445,32 @@ __global__ __launch_bounds__(kThreads) void kv_write_chunks_kernel(const CachePa
     const T* vp = static_cast<const T*>(p.v) + at.b * p.vs[0] + at.h * p.vs[1] + (at.t0 + token) * p.vs[2] + 8 * sub;
 #pragma unroll
     for (int j = 0; j < BLOCKS; ++j) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) k[j].f[i] = v[j].f[i] = 0.f;
+      k[j].clear(), v[j].clear();
       if (there) {
         k[j].load(kp + kKvBlock * j);
         v[j].load(vp + kKvBlock * j);
       }
     }
     if (unit + step < p.units) next = Chunk<SCALAR>(p, unit + step, kv_record_bytes(D, BITS));
-    int k_scale[BLOCKS], v_scale[BLOCKS], bad = 0;
+    int k_scale[BLOCKS], v_scale[BLOCKS];
+    bool finite = true;
 #pragma unroll
     for (int j = 0; j < BLOCKS; ++j) {
-      float k_most = 0.f, v_most = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        k_most = fmaxf(k_most, fabsf(k[j].f[i]));
-        v_most = fmaxf(v_most, fabsf(v[j].f[i]));
-        bad |= !(fabsf(k[j].f[i]) <= 3.4028235e38f) | !(fabsf(v[j].f[i]) <= 3.4028235e38f);
-      }
-      k_scale[j] = scale_byte<BITS>(group_max<4>(k_most));
-      v_scale[j] = scale_byte<BITS>(group_max<4>(v_most));
+      k_scale[j] = scale_byte<BITS>(group_max<4>(k[j].most(finite)));
+      v_scale[j] = scale_byte<BITS>(group_max<4>(v[j].most(finite)));
     }
+    int bad = !finite;
     bad |= __shfl_xor(bad, 1, kWave);
     bad |= __shfl_xor(bad, 2, kWave);
     uint32_t values[BLOCKS * EACH];
 #pragma unroll
     for (int j = 0; j < BLOCKS; ++j) {
       if (bad) {
-        k_scale[j] = kKvNotFinite, v_scale[j] = 127;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) k[j].f[i] = v[j].f[i] = 0.f;
+        k_scale[j] = v_scale[j] = 127;
+        k[j].clear(), v[j].clear();
       }
-      const Codes<BITS> kc = encode<BITS>(k[j].f, bad ? 127 : k_scale[j]), vc = to_record<BITS>(encode<BITS>(v[j].f, v_scale[j]), token, sub);
+      const Codes<BITS> kc = encode<BITS>(k[j], k_scale[j]), vc = to_record<BITS>(encode<BITS>(v[j], v_scale[j]), token, sub);
+      if (bad) k_scale[j] = kKvNotFinite;
       if (there) store_words(at.record + j * (kKvChunk * 4 * BITS) + token * 4 * BITS + sub * BITS, kc.w);
 #pragma unroll
       for (int i = 0; i < EACH; ++i) values[j * EACH + i] = vc.w[i];
@@ -496,22 +530,22 @@ __global__ __launch_bounds__(kThreads) void kv_read_chunks_kernel(const CachePar
     const bool asked = t >= 0 && t < p.T;
 #pragma unroll
     for (int j = 0; j < BLOCKS; ++j) {
-      Eight<T> k, v;
+      float k[8], v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) k.f[i] = v.f[i] = 0.f;
+      for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
       if (at.record != nullptr) {
         Codes<BITS> c;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) c.w[i] = values[j * EACH + i];
         c = from_record<BITS>(c, token, sub);
         if (there) {
-          decode<BITS>(keys[j], kv_scale(k_scale[j]), k.f);
-          decode<BITS>(c, kv_scale(k_scale[j] == kKvNotFinite ? kKvNotFinite : v_scale[j]), v.f);
+          decode<BITS>(keys[j], kv_scale(k_scale[j]), k);
+          decode<BITS>(c, kv_scale(k_scale[j] == kKvNotFinite ? kKvNotFinite : v_scale[j]), v);
         }
       }
       if (asked) {
-        k.store(kp + kKvBlock * j);
-        v.store(vp + kKvBlock * j);
+        store_eight(kp + kKvBlock * j, k);
+        store_eight(vp + kKvBlock * j, v);
       }
     }
   }

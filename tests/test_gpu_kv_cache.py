@@ -191,6 +191,23 @@ def test_a_pool_beyond_32_bits(device):
         assert torch.equal(got.double(), cached_values(x, 8))
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [8, 16])
+def test_every_number_of_a_type(device, bits, dtype, tokens):
+    """All finite numbers of 16 bits, beside neighbours and beside numbers some orders apart, row by row and chunk by chunk."""
+    numbers = torch.arange(-(1 << 15), 1 << 15, dtype=torch.int32).to(torch.int16).view(dtype)
+    numbers = numbers[numbers.isfinite()]
+    numbers = numbers[numbers.double().abs().argsort(stable=True)]
+    mixed = torch.cat([part[torch.randperm(len(part), generator=torch.Generator().manual_seed(len(part)))] for part in numbers.split(2048)])
+    k, v = (torch.cat((t, t.new_zeros(-len(t) % (128 * tokens)))).view(-1, 1, tokens, 128).to(device) for t in (numbers, mixed))
+    cache = empty_kv_cache(len(k), 1, 128, bits=bits, page_tokens=16, device=device)
+    pages = torch.arange(len(k), device=device)[:, None]
+    kv_cache_write(cache, k, v, pages)
+    for x, y in zip(kv_cache_read(cache, pages, None, tokens, dtype=torch.float32), (k, v)):
+        assert torch.equal(x.double(), cached_values(y, bits))
+
+
 def test_more_rows_than_32_bits(device):
     """Samples by the hundred thousand of four thousand heads, of which the last alone has a page."""
     batch, heads = (1 << 19) + 3, 1 << 12
