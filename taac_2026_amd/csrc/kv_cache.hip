@@ -98,6 +98,19 @@ __device__ __forceinline__ void store_eight(T* p, const float (&f)[8]) {
   }
 }
 
+// The value of lane l ^ XOR, by the operands' own lane patterns: quads, sixteen lanes turned by eight, and for four eight lanes mirrored, then their quads.
+template <int XOR>
+__device__ __forceinline__ uint32_t across(uint32_t v) {
+  static_assert(XOR == 1 || XOR == 2 || XOR == 4 || XOR == 8);
+  constexpr int PATTERN = XOR == 1 ? 0xb1 : XOR == 2 ? 0x4e : XOR == 4 ? 0x141 : 0x128;
+  const uint32_t r = __builtin_amdgcn_update_dpp(v, v, PATTERN, 0xf, 0xf, false);
+  return XOR == 4 ? __builtin_amdgcn_update_dpp(r, r, 0x1b, 0xf, 0xf, false) : r;
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __builtin_bit_cast(float, across<1>(__builtin_bit_cast(uint32_t, v))));
+  return fmaxf(v, __builtin_bit_cast(float, across<2>(__builtin_bit_cast(uint32_t, v))));
+}
+
 // The least power of two 2^e with max < 7 2^e (464 2^e), as e + 127, for a finite max. The carry out of the fraction is the step to the next power: 7 and 464
 // are 1.75 and 1.8125 of one. Kept between 2^-117, under which the smallest code would be subnormal, and what keeps the largest code finite.
 template <int BITS>
@@ -204,7 +217,7 @@ __global__ __launch_bounds__(kThreads) void kv_write_rows_kernel(const CachePara
   const int in_page = static_cast<int>(at.position & ((1 << p.pool.page_shift) - 1)), token = in_page % kKvChunk;
   uint8_t* record = p.pool.data + kv_record(p.pool, page, at.h, in_page / kKvChunk, kv_record_bytes(D, BITS));
   bool finite = true;
-  const float k_most = group_max<4>(k.most(finite)), v_most = group_max<4>(v.most(finite));
+  const float k_most = quad_max(k.most(finite)), v_most = quad_max(v.most(finite));
   int bad = !finite;
 #pragma unroll
   for (int off = LANES / 2; off > 0; off /= 2) bad |= __shfl_xor(bad, off, kWave);
@@ -221,7 +234,7 @@ __global__ __launch_bounds__(kThreads) void kv_write_rows_kernel(const CachePara
   uint8_t* values = record + kv_value_at(D, BITS);
   const int group = token / 4, of4 = token % 4;
   if constexpr (BITS == 4) {
-    const uint32_t mine = vc.w[0], other = __shfl_xor(mine, 2, kWave);
+    const uint32_t mine = vc.w[0], other = across<2>(mine);
     if (sub < 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -342,16 +355,16 @@ struct Chunk {
 
 // Lanes of four tokens (bits 2 and 3 of the lane) hold four bytes each: byte i of lane j becomes byte j of lane i. Its own inverse.
 __device__ __forceinline__ uint32_t turn_bytes(uint32_t w, int token) {
-  uint32_t other = __shfl_xor(w, 4, kWave);
+  uint32_t other = across<4>(w);
   w = __builtin_amdgcn_perm(other, w, token & 1 ? 0x03070105u : 0x06020400u);
-  other = __shfl_xor(w, 8, kWave);
+  other = across<8>(w);
   return __builtin_amdgcn_perm(other, w, token & 2 ? 0x03020706u : 0x05040100u);
 }
 // The same of four halves of 16 bits.
 __device__ __forceinline__ void turn_halves(uint32_t (&w)[2], int token) {
-  const uint32_t a = __shfl_xor(w[0], 4, kWave), b = __shfl_xor(w[1], 4, kWave), pick = token & 1 ? 0x03020706u : 0x05040100u;
+  const uint32_t a = across<4>(w[0]), b = across<4>(w[1]), pick = token & 1 ? 0x03020706u : 0x05040100u;
   const uint32_t x = __builtin_amdgcn_perm(a, w[0], pick), y = __builtin_amdgcn_perm(b, w[1], pick);
-  const uint32_t other = __shfl_xor(token & 2 ? x : y, 8, kWave);
+  const uint32_t other = across<8>(token & 2 ? x : y);
   w[0] = token & 2 ? other : x;
   w[1] = token & 2 ? y : other;
 }
@@ -370,10 +383,10 @@ template <int BITS>
 __device__ __forceinline__ Codes<BITS> to_record(const Codes<BITS>& c, int token, int sub) {
   Codes<BITS> r;
   if constexpr (BITS == 4) {
-    const uint32_t w = c.w[0], other = __shfl_xor(sub < 2 ? w >> 16 : w & 0xffffu, 2, kWave);
+    const uint32_t w = c.w[0], other = across<2>(sub < 2 ? w >> 16 : w & 0xffffu);
     r.w[0] = turn_bytes(spread_nibbles(sub < 2 ? w & 0xffffu : other) | spread_nibbles(sub < 2 ? other : w >> 16) << 4, token);
   } else {
-    const uint32_t other = __shfl_xor(sub < 2 ? c.w[1] : c.w[0], 2, kWave), low = sub < 2 ? c.w[0] : other, high = sub < 2 ? other : c.w[1];
+    const uint32_t other = across<2>(sub < 2 ? c.w[1] : c.w[0]), low = sub < 2 ? c.w[0] : other, high = sub < 2 ? other : c.w[1];
     r.w[0] = __builtin_amdgcn_perm(high, low, 0x05010400u), r.w[1] = __builtin_amdgcn_perm(high, low, 0x07030602u);
     turn_halves(r.w, token);
   }
@@ -384,13 +397,13 @@ __device__ __forceinline__ Codes<BITS> from_record(const Codes<BITS>& c, int tok
   Codes<BITS> r;
   if constexpr (BITS == 4) {
     const uint32_t w = turn_bytes(c.w[0], token), low = gather_nibbles(w & 0x0f0f0f0fu), high = gather_nibbles(w >> 4 & 0x0f0f0f0fu);
-    const uint32_t other = __shfl_xor(sub < 2 ? high : low, 2, kWave);
+    const uint32_t other = across<2>(sub < 2 ? high : low);
     r.w[0] = sub < 2 ? low | other << 16 : other | high << 16;
   } else {
     uint32_t w[2] = {c.w[0], c.w[1]};
     turn_halves(w, token);
     const uint32_t low = __builtin_amdgcn_perm(w[1], w[0], 0x06040200u), high = __builtin_amdgcn_perm(w[1], w[0], 0x07050301u);
-    const uint32_t other = __shfl_xor(sub < 2 ? high : low, 2, kWave);
+    const uint32_t other = across<2>(sub < 2 ? high : low);
     r.w[0] = sub < 2 ? low : other, r.w[1] = sub < 2 ? other : high;
   }
   return r;
@@ -456,12 +469,12 @@ __global__ __launch_bounds__(kThreads) void kv_write_chunks_kernel(const CachePa
     bool finite = true;
 #pragma unroll
     for (int j = 0; j < BLOCKS; ++j) {
-      k_scale[j] = scale_byte<BITS>(group_max<4>(k[j].most(finite)));
-      v_scale[j] = scale_byte<BITS>(group_max<4>(v[j].most(finite)));
+      k_scale[j] = scale_byte<BITS>(quad_max(k[j].most(finite)));
+      v_scale[j] = scale_byte<BITS>(quad_max(v[j].most(finite)));
     }
     int bad = !finite;
-    bad |= __shfl_xor(bad, 1, kWave);
-    bad |= __shfl_xor(bad, 2, kWave);
+    bad |= across<1>(bad);
+    bad |= across<2>(bad);
     uint32_t values[BLOCKS * EACH];
 #pragma unroll
     for (int j = 0; j < BLOCKS; ++j) {
