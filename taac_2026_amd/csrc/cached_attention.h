@@ -51,17 +51,17 @@ struct AttendParams {
 namespace {
 
 constexpr int kTile = 64;          // tokens
-// A kernel's shape, by the rows of a workgroup: 1, 2 or 4 (one form), 16, 32 or 48 (the other). alone: a wavefront to a workgroup.
+// A kernel's shape, by the rows of a workgroup - 1, 2 or 4 (one form), 16, 32 or 48 (the other) - and its wavefronts: 1, 4, or 8.
 struct Shape {
   int waves;
   int stages;    // tiles of a wavefront in LDS; one: keys and values by themselves
   int per_simd;  // wavefronts that the registers leave room for
 };
-__host__ __device__ constexpr Shape shape_of(int rows, int d, bool alone) {
-  if (rows <= 4) return {alone ? 1 : 4, 2, d == 32 ? 6 : d == 64 ? 4 : 2};
-  if (rows == 16) return {alone ? 1 : 4, 1, d == 32 ? 6 : d == 64 ? 4 : 3};
-  if (rows == 32) return {4, 1, d == 32 ? 4 : d == 64 ? 3 : 2};
-  return {8, 1, 2};
+__host__ __device__ constexpr Shape shape_of(int rows, int d, int waves) {
+  if (rows <= 4) return {waves, 2, d == 32 ? 6 : d == 64 ? 4 : 2};
+  if (waves == 8) return {waves, 1, 2};
+  if (rows == 16) return {waves, 1, d == 32 ? 6 : d == 64 ? 4 : 3};
+  return {waves, 1, d == 32 ? 4 : d == 64 ? 3 : 2};
 }
 __host__ __device__ constexpr int tile_bytes(int d, int bits) { return (4 * kv_record_bytes(d, bits) + 1023) / 1024 * 1024; }
 __host__ __device__ constexpr int half_bytes(int d, int bits) { return 4 * kv_key_bytes(d, bits) + 4 * kWave; }
@@ -87,14 +87,14 @@ __host__ __device__ constexpr bool meeting_fits(int n, int waves, int each, int 
 }
 __host__ __device__ constexpr int stats_bytes(int rows, int waves) { return waves > 1 ? waves * (rows <= 16 ? 16 : rows) * 8 : 0; }
 // of the tiles, or of the meeting behind them; then the queries and the statistics
-__host__ __device__ constexpr int working_bytes(int rows, int d, int bits, bool alone) {
-  const Shape shape = shape_of(rows, d, alone);
+__host__ __device__ constexpr int working_bytes(int rows, int d, int bits, int waves) {
+  const Shape shape = shape_of(rows, d, waves);
   const int tiles = shape.waves * (rows <= 4 ? shape.stages * tile_bytes(d, bits) + 8 * (kTile + 8) * 2 : 2 * half_bytes(d, bits));
   const int fours = (rows <= 16 ? 1 : rows / 16) * (d / 16), meeting = meeting_bytes(fours, shape.waves, false) + meeting_bytes(fours, shape.waves, true);
   return tiles > meeting ? tiles : meeting;
 }
-__host__ __device__ constexpr int lds_bytes(int rows, int d, int bits, int parts, bool alone) {
-  return working_bytes(rows, d, bits, alone) + (queries_in_lds(rows, parts) ? rows * d * 2 : 0) + stats_bytes(rows, shape_of(rows, d, alone).waves);
+__host__ __device__ constexpr int lds_bytes(int rows, int d, int bits, int parts, int waves) {
+  return working_bytes(rows, d, bits, waves) + (queries_in_lds(rows, parts) ? rows * d * 2 : 0) + stats_bytes(rows, shape_of(rows, d, waves).waves);
 }
 constexpr float kNothing = -3e38f; // the maximum of no scores
 constexpr float kSlack = 8.f;
@@ -641,7 +641,7 @@ __device__ __forceinline__ float from_four_on(float v) {
 // ---- up to four rows ----------------------------------------------------------------------------------------------
 
 template <typename T, int D, int BITS, int ROWS, int W, int S>
-__global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void cached_attention_few_kernel(const AttendParams p) {
+__global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W).per_simd) void cached_attention_few_kernel(const AttendParams p) {
   constexpr int BLOCKS = D / kKvBlock, SLOT = kTile + 8, PARTS = kParts<T>;
   typedef Staged<D, BITS> Tile;
   extern __shared__ __align__(16) uint8_t memory[];
@@ -754,7 +754,7 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void
   float top[1] = {most[0]}, total[1] = {sum[0]};
 #pragma unroll
   for (int r = 1; r < ROWS; ++r) top[0] = l16 == r ? most[r] : top[0];
-  finish<T, D, 1, W>(p, job, span, memory, reinterpret_cast<float*>(memory + working_bytes(ROWS, D, BITS, W == 1)), wave, lane, acc, total, top);
+  finish<T, D, 1, W>(p, job, span, memory, reinterpret_cast<float*>(memory + working_bytes(ROWS, D, BITS, W)), wave, lane, acc, total, top);
 }
 
 // ---- sixteen rows at a time ---------------------------------------------------------------------------------------
@@ -897,10 +897,10 @@ __device__ __forceinline__ void attend_many(const AttendParams& p, const Job& jo
 
 // Rows of queries that a sample has not, whole sixteens of them, are cleared and not taken along.
 template <typename T, int D, int BITS, int ROWS, int W>
-__global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W == 1).per_simd) void cached_attention_many_kernel(const AttendParams p) {
+__global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W).per_simd) void cached_attention_many_kernel(const AttendParams p) {
   constexpr bool SHARED = queries_in_lds(ROWS, kParts<T>);
   extern __shared__ __align__(16) uint8_t memory[];
-  constexpr int WORKING = working_bytes(ROWS, D, BITS, W == 1);
+  constexpr int WORKING = working_bytes(ROWS, D, BITS, W);
   static_assert(meeting_fits(ROWS / 16 * (D / 16), W, D / 16, WORKING));
   uint8_t* const queries = memory + WORKING;
   float* const stats = reinterpret_cast<float*>(queries + (SHARED ? ROWS * D * 2 : 0));
@@ -922,31 +922,31 @@ void launch_with(Kernel* kernel, uint32_t groups, int threads, int bytes, const 
   if (bytes > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   hipLaunchKernelGGL(kernel, dim3(groups), dim3(threads), bytes, s, p);
 }
-template <typename T, int D, int BITS, int ROWS, bool ALONE>
+template <typename T, int D, int BITS, int ROWS, int W>
 void launch_rows(const AttendParams& p, uint32_t groups, hipStream_t s) {
-  constexpr Shape shape = shape_of(ROWS, D, ALONE);
+  constexpr Shape shape = shape_of(ROWS, D, W);
   static_assert(Staged<D, BITS>::BYTES == tile_bytes(D, BITS) && StagedHalf<D, BITS>::BYTES == half_bytes(D, BITS));
-  constexpr int bytes = lds_bytes(ROWS, D, BITS, kParts<T>, ALONE), threads = shape.waves * kWave;
-  if constexpr (ROWS <= 4) launch_with(cached_attention_few_kernel<T, D, BITS, ROWS, shape.waves, shape.stages>, groups, threads, bytes, p, s);
-  else launch_with(cached_attention_many_kernel<T, D, BITS, ROWS, shape.waves>, groups, threads, bytes, p, s);
+  constexpr int bytes = lds_bytes(ROWS, D, BITS, kParts<T>, W), threads = W * kWave;
+  if constexpr (ROWS <= 4) launch_with(cached_attention_few_kernel<T, D, BITS, ROWS, W, shape.stages>, groups, threads, bytes, p, s);
+  else launch_with(cached_attention_many_kernel<T, D, BITS, ROWS, W>, groups, threads, bytes, p, s);
 }
 template <typename T, int D, int BITS>
-void launch_attend(const AttendParams& p, int rows, bool alone, uint32_t groups, hipStream_t s) {
-  if (rows == 1) alone ? launch_rows<T, D, BITS, 1, true>(p, groups, s) : launch_rows<T, D, BITS, 1, false>(p, groups, s);
-  if (rows == 2) alone ? launch_rows<T, D, BITS, 2, true>(p, groups, s) : launch_rows<T, D, BITS, 2, false>(p, groups, s);
+void launch_attend(const AttendParams& p, int rows, int waves, uint32_t groups, hipStream_t s) {
+  if (rows == 1) waves == 1 ? launch_rows<T, D, BITS, 1, 1>(p, groups, s) : launch_rows<T, D, BITS, 1, 4>(p, groups, s);
+  if (rows == 2) waves == 1 ? launch_rows<T, D, BITS, 2, 1>(p, groups, s) : launch_rows<T, D, BITS, 2, 4>(p, groups, s);
   if constexpr (kParts<T> == 1) {
-    if (rows == 4) alone ? launch_rows<T, D, BITS, 4, true>(p, groups, s) : launch_rows<T, D, BITS, 4, false>(p, groups, s);
+    if (rows == 4) waves == 1 ? launch_rows<T, D, BITS, 4, 1>(p, groups, s) : launch_rows<T, D, BITS, 4, 4>(p, groups, s);
   }
-  if (rows == 16) alone ? launch_rows<T, D, BITS, 16, true>(p, groups, s) : launch_rows<T, D, BITS, 16, false>(p, groups, s);
-  if (rows == 32) launch_rows<T, D, BITS, 32, false>(p, groups, s);
+  if (rows == 16) waves == 1 ? launch_rows<T, D, BITS, 16, 1>(p, groups, s) : waves == 4 ? launch_rows<T, D, BITS, 16, 4>(p, groups, s) : launch_rows<T, D, BITS, 16, 8>(p, groups, s);
+  if (rows == 32) launch_rows<T, D, BITS, 32, 4>(p, groups, s);
   if constexpr (kParts<T> == 1) {
-    if (rows == 48) launch_rows<T, D, BITS, 48, false>(p, groups, s);
+    if (rows == 48) launch_rows<T, D, BITS, 48, 8>(p, groups, s);
   }
 }
 template <int BITS>
-void dispatch_attend(const AttendParams& p, int d, bool f16, int rows, bool alone, uint32_t groups, hipStream_t s) {
+void dispatch_attend(const AttendParams& p, int d, bool f16, int rows, int waves, uint32_t groups, hipStream_t s) {
 #define TAAC_ATTEND(D) \
-  if (d == D) f16 ? launch_attend<f16_t, D, BITS>(p, rows, alone, groups, s) : launch_attend<bf16_t, D, BITS>(p, rows, alone, groups, s);
+  if (d == D) f16 ? launch_attend<f16_t, D, BITS>(p, rows, waves, groups, s) : launch_attend<bf16_t, D, BITS>(p, rows, waves, groups, s);
   TAAC_ATTEND(32) TAAC_ATTEND(64) TAAC_ATTEND(128)
 #undef TAAC_ATTEND
 }
@@ -954,7 +954,7 @@ void dispatch_attend(const AttendParams& p, int d, bool f16, int rows, bool alon
 }  // namespace
 
 // Of caches of 4 bits and of 8 (cached_attention_4.hip, cached_attention_8.hip): a unit each, which build side by side.
-void attend_4(const AttendParams& p, int d, bool f16, int rows, bool alone, uint32_t groups, hipStream_t s);
-void attend_8(const AttendParams& p, int d, bool f16, int rows, bool alone, uint32_t groups, hipStream_t s);
+void attend_4(const AttendParams& p, int d, bool f16, int rows, int waves, uint32_t groups, hipStream_t s);
+void attend_8(const AttendParams& p, int d, bool f16, int rows, int waves, uint32_t groups, hipStream_t s);
 
 }  // namespace taac

@@ -70,6 +70,7 @@ __global__ __launch_bounds__(256) void cached_attention_join_kernel(const Attend
 
 // ---- the host -----------------------------------------------------------------------------------------------------
 
+constexpr int64_t kOccupied = 192;  // units: most of 256 CUs have one
 constexpr int64_t kMostGroups = 1 << 23;  // of a launch: below 2^31 threads
 
 // How a call is cut. A unit is a tile of rows of a key head of a sample.
@@ -77,8 +78,7 @@ struct Plan {
   int rows;       // of a tile: 1, 2, 4, 16, 32 or 48
   int row_tiles;  // of a key head
   int splits;     // of a history
-  int waves;      // of a workgroup
-  bool alone;
+  int waves;      // of a workgroup: 1, 4 or 8
 };
 
 // From so many units on a wavefront takes one alone, without the meeting; below, four share its tokens. Medians of ragged histories, alone : shared, in us:
@@ -88,39 +88,43 @@ struct Plan {
 int64_t alone_from(int rows, int32_t d) { return rows > 4 ? 8192 : d == 32 ? 4096 : 2048; }
 
 // Tiles of so many rows.
-Plan cut(int64_t B, int32_t heads, int64_t rows, int tile, int32_t d, int bits, int64_t held, bool parts) {
+Plan cut(int64_t B, int32_t heads, int64_t rows, int tile, bool wide, int32_t d, int bits, int64_t held, bool parts) {
   Plan plan{};
   plan.rows = tile;
   plan.row_tiles = static_cast<int>((rows + tile - 1) / (tile > 0 ? tile : 1));
   const int64_t units = B * heads * plan.row_tiles;
-  plan.alone = tile <= 16 && units >= alone_from(tile, d);
-  const Shape shape = shape_of(tile, d, plan.alone);
-  plan.waves = shape.waves;
+  plan.waves = wide ? 8 : tile <= 16 && units >= alone_from(tile, d) ? 1 : 4;
+  const Shape shape = shape_of(tile, d, plan.waves);
   // Histories are split until the card is full, by LDS and registers; twice as many workgroups cost more than a better balance gives back (4 x 8 key heads of 128 features,
   // 65536 tokens: 56 us, 60 with twice as many). A split has a tile for each of its wavefronts, and below four (six of narrower heads) the kernel that joins them
-  // takes longer than the tiles would: one sample of 768 tokens 5.7 us as a whole, of 1024 in four 7.9.
-  const int by_lds = 163840 / lds_bytes(tile, d, bits, parts ? 2 : 1, plan.alone), by_registers = 4 * shape.per_simd / shape.waves;
+  // takes longer than the tiles would: one sample of 768 tokens 5.7 us as a whole, of 1024 in four 7.9. Where whole histories occupy three quarters of the CUs, only from 16 tiles
+  // to a wavefront on, and not of 128 features. One query of 4 key heads, split : whole, 64 samples of 2500 tokens: 32 features 11.8 : 10.4, 64 17.2 : 15.0, 128 24.8 : 20.5;
+  // of 8000: 20.8 : 26.5, 31.7 : 34.7, 53.0 : 48.2; 48 of 2500 11.5 : 9.8, 15.0 : 14.1, 22.1 : 20.0.
+  const int by_lds = 163840 / lds_bytes(tile, d, bits, parts ? 2 : 1, plan.waves), by_registers = 4 * shape.per_simd / shape.waves;
   const int64_t resident = 256 * (by_lds < by_registers ? by_lds : by_registers), most = held / (kTile * shape.waves);
   int64_t splits = resident / (units > 0 ? units : 1);
   splits = splits < most ? splits : most;
-  plan.splits = static_cast<int>(most < (d == 128 ? 4 : 6) || splits < 1 ? 1 : splits);
+  const bool long_enough = units < kOccupied ? most >= (d == 128 ? 4 : 6) : most >= 16 && d < 128;
+  plan.splits = static_cast<int>(!long_enough || splits < 1 ? 1 : splits);
   return plan;
 }
 
 Plan plan_of(int64_t B, int32_t heads, int32_t group, int32_t T, int32_t d, int bits, int64_t held, bool parts) {
   const int64_t rows = static_cast<int64_t>(group) * T;
   // up to 4 rows (2 in two parts) in the one form
-  if (rows <= 2 || (rows <= 4 && !parts)) return cut(B, heads, rows, rows <= 2 ? static_cast<int>(rows) : 4, d, bits, held, parts);
-  if (rows <= 16) return cut(B, heads, rows, 16, d, bits, held, parts);
+  if (rows <= 2 || (rows <= 4 && !parts)) return cut(B, heads, rows, rows <= 2 ? static_cast<int>(rows) : 4, false, d, bits, held, parts);
+  // 16 rows where a workgroup to a CU fills the card: eight wavefronts, and no splits. 8 rows of 4 key heads, four with splits : eight, 64 samples of 1000 and 2500 tokens: of 64
+  // features in 8 bits 10.3 : 9.9 us and 22.8 : 18.6, in 4 bits 9.0 : 8.1 and 18.5 : 14.1, of 128 in 8 bits 19.8 : 16.9 and 33.7 : 31.0; 96 samples of 128 22.7 : 25.7 and 44.0 : 46.8.
+  if (rows <= 16) return cut(B, heads, rows, 16, B * heads >= kOccupied && B * heads <= 256, d, bits, held, parts);
   // In the other 16, or 32, which share the conversion of the codes. Where a workgroup of eight wavefronts to a CU just fills the card, up to 48 rows in one, which need no
   // splits and no joining; of four sixteens the sums would leave no registers. 4 key heads, 2000 tokens, 48 rows : 32: of 128 features in 8 bits, 18 rows, 48 samples 25.1 : 29.6
   // us, 64 samples 29.8 : 32.3, 100 samples 47.8 : 43.2; 48 rows, 64 samples 32.9 : 36.8, 100 samples 56.5 : 65.9; of 64 in 4 bits, 18 rows, 64 samples 16.3 : 19.7, 100 samples
   // 29.6 : 24.1; 48 rows 20.8 : 23.9 and 38.7 : 37.2. Of 500 tokens 16.2 : 16.3 and 29.1 : 26.6, 11.0 : 10.3 and 20.0 : 14.8.
   if (rows <= 48 && !parts && held >= 1024 && B * heads <= 256) {
-    const Plan wide = cut(B, heads, rows, 48, d, bits, held, parts);
-    if (B * heads * wide.splits >= 192) return wide;
+    const Plan wide = cut(B, heads, rows, 48, true, d, bits, held, parts);
+    if (B * heads * wide.splits >= kOccupied) return wide;
   }
-  return cut(B, heads, rows, 32, d, bits, held, parts);
+  return cut(B, heads, rows, 32, false, d, bits, held, parts);
 }
 
 template <typename T, int D>
@@ -196,7 +200,7 @@ extern "C" int taac_cached_attention_fwd(const void* q, void* o, const void* cac
   for (int64_t first = 0; first < B; first += at_once) {
     p.first = static_cast<int32_t>(first);
     const uint32_t groups = static_cast<uint32_t>((B - first < at_once ? B - first : at_once) * each);
-    bits == 4 ? attend_4(p, d, f16, plan.rows, plan.alone, groups, s) : attend_8(p, d, f16, plan.rows, plan.alone, groups, s);
+    bits == 4 ? attend_4(p, d, f16, plan.rows, plan.waves, groups, s) : attend_8(p, d, f16, plan.rows, plan.waves, groups, s);
   }
   if (plan.splits > 1) f16 ? join<f16_t>(p, plan, d, s) : join<bf16_t>(p, plan, d, s);
   return check_launch(name);

@@ -3,6 +3,6 @@
 
 namespace taac {
 
-void attend_4(const AttendParams& p, int d, bool f16, int rows, bool alone, uint32_t groups, hipStream_t s) { dispatch_attend<4>(p, d, f16, rows, alone, groups, s); }
+void attend_4(const AttendParams& p, int d, bool f16, int rows, int waves, uint32_t groups, hipStream_t s) { dispatch_attend<4>(p, d, f16, rows, waves, groups, s); }
 
 }  // namespace taac
