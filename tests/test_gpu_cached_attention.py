@@ -114,6 +114,34 @@ def test_ragged_new_tokens(device, bits, dtype, width, batch, lengths, group, to
     _check(got, q, k, v, lengths, news)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("width", [32, 64, 128])
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("group,tokens,window", [(5, 1, None), (2, 8, 300), (3, 6, None), (2, 16, None), (2, 24, 500), (1, 33, None)])
+def test_a_workgroup_to_a_unit(device, bits, dtype, width, page, group, tokens, window):
+    """As many key heads of samples as the card has room for at a time, ragged: eight wavefronts to each, up to 16, 32 and 48 rows."""
+    lengths = [(37 * i + 5) % 150 if i % 9 else 1000 + i for i in range(100)]
+    lengths[1:3] = [0, 1]
+    news = [min(tokens, (5 * i + 1) % (tokens + 2)) for i in range(100)]
+    cache, pages, k, v = _filled(device, lengths, 2, width, bits, page)
+    q = _queries(device, 100, 2 * group, tokens, width, dtype)
+    got = cached_attention(q, cache, pages, torch.tensor(lengths, device=device), query_lengths=torch.tensor(news, device=device), window=window)
+    _check(got, q, k, v, lengths, news, window)
+
+
+@pytest.mark.parametrize("bits,width", [(4, 32), (8, 64), (4, 128), (8, 128)])
+@pytest.mark.parametrize("group,tokens,window", [(2, 10, None), (2, 24, None), (3, 11, 2000), (1, 48, None)])
+def test_parts_of_wide_workgroups(device, bits, width, group, tokens, window):
+    """The same workgroups over parts of long histories, beside short ones that are not split."""
+    lengths = [5000 if i % 7 == 3 else 611 * i % 1500 for i in range(20)]
+    news = [min(tokens, (5 * i + 9) % (tokens + 9)) for i in range(20)]
+    cache, pages, k, v = _filled(device, lengths, 2, width, bits, 64)
+    q = _queries(device, 20, 2 * group, tokens, width)
+    got = cached_attention(q, cache, pages, torch.tensor(lengths, device=device), query_lengths=torch.tensor(news, device=device), window=window)
+    _check(got, q, k, v, lengths, news, window)
+
+
 @pytest.mark.parametrize("width", [64, 128])
 def test_fp16_rows_in_the_other_form(device, width):
     """Three and four rows of fp16 are cut into more splits than those of bf16."""
