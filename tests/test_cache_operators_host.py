@@ -165,6 +165,7 @@ def test_rope_entry_points_check_on_the_host():
     assert both(d=513) == unsupported and both(H=(1 << 20) + 1) == unsupported
     assert both(rotary=15) == invalid and both(rotary=34) == invalid and both(rotary=-2) == invalid and b"rotated" in library.taac_last_error()
     assert both(rotary=0) == invalid and both(table=None) == invalid and both(places=-1) == invalid
+    assert both(places=1 << 31) == unsupported and b"2^31 - 1" in library.taac_last_error()
     assert both(w=None) == invalid and both(kw=None) == invalid and b"both norm weights" in library.taac_last_error()
     assert both(dtype=7) == invalid and both(eps=-1.0) == invalid and both(qs=None) == invalid and both(q=None) == invalid
     assert both(positions=fake) == invalid and b"positions" in library.taac_last_error()
