@@ -195,8 +195,8 @@ def cached_attention(
     ``window`` the last ``window`` of them, itself included. Queries at or beyond ``query_lengths[b]`` and queries that see nothing get zeros, positions in no page of
     the pool are not seen.
 
-    bfloat16 or float16 queries. They, keys and values enter exactly; scores, statistics and sums are float32, probabilities enter the product with 16 bits; the
-    output is rounded once. A NaN or an infinity in a cached token reaches the queries that see it, and no others.
+    bfloat16 or float16 queries. They, keys and values enter exactly; scores, statistics and sums are float32; probabilities enter the product with 24 bits where a
+    key head has up to four rows (query heads that share it times tokens; two of float16), else with 16; the output is rounded once. A NaN or an infinity in a cached token reaches the queries that see it, and no others.
     Forward only."""
     name = "cached_attention"
     if q.ndim != 4:

@@ -16,7 +16,8 @@
 // Values enter as their transpose: features are rows, queries columns, and a row's rescaling stays in its lanes.
 //
 // Precision: all operands are bf16, exact for keys and values of either size, whatever their scales, and for queries (fp16 ones in two parts); scores, statistics
-// and sums are fp32; probabilities enter as two parts (16 bits), in the first form in columns that would be empty. The maximum moves when a score exceeds it
+// and sums are fp32. Probabilities enter as parts of eight bits: three in the first form, in columns that would be empty, so that they keep the digits of fp32; two in the
+// other, where a third would be half as many products with the values again, and outputs of 16 bits are off by their own rounding either way. The maximum moves when a score exceeds it
 // by a factor of 2^8, which cancels.
 //
 // Measured: 4 samples of 65536 tokens, 32 heads over 8 of 128 features in 4 bits: 50 us and 5 for the join, 5.6 TB/s of the cache (tiles in registers, one ahead: 101, for the
@@ -89,7 +90,7 @@ __host__ __device__ constexpr int stats_bytes(int rows, int waves) { return wave
 // of the tiles, or of the meeting behind them; then the queries and the statistics
 __host__ __device__ constexpr int working_bytes(int rows, int d, int bits, int waves) {
   const Shape shape = shape_of(rows, d, waves);
-  const int tiles = shape.waves * (rows <= 4 ? shape.stages * tile_bytes(d, bits) + 8 * (kTile + 8) * 2 : 2 * half_bytes(d, bits));
+  const int tiles = shape.waves * (rows <= 4 ? shape.stages * tile_bytes(d, bits) + 3 * rows * (kTile + 8) * 2 : 2 * half_bytes(d, bits));
   const int fours = (rows <= 16 ? 1 : rows / 16) * (d / 16), meeting = meeting_bytes(fours, shape.waves, false) + meeting_bytes(fours, shape.waves, true);
   return tiles > meeting ? tiles : meeting;
 }
@@ -632,10 +633,11 @@ __device__ __forceinline__ void walk_halves(const AttendParams& p, const Job& jo
   }
 }
 
-// Lane l + 4's value, within a row of sixteen.
-__device__ __forceinline__ float from_four_on(float v) {
+// The sum of lanes l, l + 4 and l + 8, within a row of sixteen, for its first four.
+__device__ __forceinline__ float three_parts(float v) {
   const int bits = __builtin_bit_cast(int, v);
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(bits, bits, 0x104, 0xf, 0xf, false));
+  return v + (__builtin_bit_cast(float, __builtin_amdgcn_update_dpp(bits, bits, 0x104, 0xf, 0xf, false)) +
+              __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(bits, bits, 0x108, 0xf, 0xf, false)));
 }
 
 // ---- up to four rows ----------------------------------------------------------------------------------------------
@@ -653,7 +655,9 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W).per_simd) void cach
     return;
   }
   uint8_t* const stages = memory + wave * (S * Tile::BYTES);
-  bf16_t (*const turned)[SLOT] = reinterpret_cast<bf16_t (*)[SLOT]>(memory + W * S * Tile::BYTES) + wave * 8;
+  bf16_t (*const turned)[SLOT] = reinterpret_cast<bf16_t (*)[SLOT]>(memory + W * S * Tile::BYTES) + wave * (3 * ROWS);  // [part][row]
+  // column 4 i + r of the operand: part i of row r; the columns that are left hold one of the others', which nothing reads
+  const int column = min(l16 / 4, 2) * ROWS + min(l16 % 4, ROWS - 1);
   int low[ROWS], high[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
@@ -729,15 +733,18 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W).per_simd) void cach
     bf16_t* to = &turned[0][l16 / 4 * 16 + grp * 4 + l16 % 4];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      const float x = __builtin_amdgcn_exp2f(score[r] - most[r]);
-      const bf16_t rounded = static_cast<bf16_t>(x);
-      to[r * SLOT] = rounded;
-      to[(4 + r) * SLOT] = static_cast<bf16_t>(x - static_cast<float>(rounded));
+      float x = __builtin_amdgcn_exp2f(score[r] - most[r]);
+#pragma unroll
+      for (int part = 0; part < 3; ++part) {
+        const bf16_t rounded = static_cast<bf16_t>(x);
+        to[(part * ROWS + r) * SLOT] = rounded;
+        x -= static_cast<float>(rounded);
+      }
     }
     wave_sync();
     bf16x8 probs[1][1][2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) probs[0][0][half] = *reinterpret_cast<const bf16x8*>(&turned[l16 % 8][grp * 16 + half * 8]);
+    for (int half = 0; half < 2; ++half) probs[0][0][half] = *reinterpret_cast<const bf16x8*>(&turned[column][grp * 16 + half * 8]);
     wave_sync();
     sum = mfma(ones, probs[0][0][0], sum);
     sum = mfma(ones, probs[0][0][1], sum);
@@ -745,12 +752,11 @@ __global__ __launch_bounds__(W * kWave, shape_of(ROWS, D, W).per_simd) void cach
   };
 
   p.pool.page_shift >= 6 ? walk<D, BITS, W, S, true>(p, job, span, wave, lane, stages, take) : walk<D, BITS, W, S, false>(p, job, span, wave, lane, stages, take);
-  // the two parts of the probabilities stand in columns r and 4 + r
 #pragma unroll
   for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[i][e] += from_four_on(acc[i][e]);
-  sum[0] += from_four_on(sum[0]);
+    for (int e = 0; e < 4; ++e) acc[i][e] = three_parts(acc[i][e]);
+  sum[0] = three_parts(sum[0]);
   float top[1] = {most[0]}, total[1] = {sum[0]};
 #pragma unroll
   for (int r = 1; r < ROWS; ++r) top[0] = l16 == r ? most[r] : top[0];

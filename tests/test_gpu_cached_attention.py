@@ -362,3 +362,28 @@ def test_a_history_event_by_event(device, width, bits):
     assert ((got.double() - want).abs() <= 2.0**-8 * want.abs() + 2.0**-14 * size).all()
     # the whole history's kernel rounds its probabilities to bf16 as well: 2^-8 of p |v| in the numerator
     assert ((got.double() - whole.double()).abs() <= 2.0**-7 * want.abs() + 2.0**-7 * size).all()
+
+
+@pytest.mark.parametrize("dtype,group", [(torch.bfloat16, 1), (torch.bfloat16, 2), (torch.bfloat16, 3), (torch.bfloat16, 4), (torch.float16, 1), (torch.float16, 2)])
+@pytest.mark.parametrize("samples", [600, 4096])
+def test_probabilities_of_few_rows(device, dtype, group, samples):
+    """Two tokens, of which the first is all zeros and the second one feature: w / (1 + w) with w = exp(scale q), whose digits are the probability's own."""
+    cache = empty_kv_cache(1, 1, 32, page_tokens=16, device=device)
+    k, v = torch.zeros(1, 1, 2, 32, device=device), torch.zeros(1, 1, 2, 32, device=device)
+    k[:, :, 1, 0], v[:, :, 1] = 1.0, 1.0
+    kv_cache_write(cache, k, v, torch.zeros(1, 1, dtype=torch.int32, device=device))
+    pages, lengths = torch.zeros(samples, 1, dtype=torch.int32, device=device), torch.full((samples,), 2, device=device, dtype=torch.int32)
+    q = torch.zeros(samples, group, 1, 32, dtype=dtype)
+    q[..., 0] = -6.0 * torch.rand(samples, group, 1, generator=torch.Generator().manual_seed(group)).to(dtype)
+    q = q.to(device)
+    for scale in (1.0, 0.8125, 0.65625):  # of five bits at most: exact
+        got = cached_attention(q, cache, pages, lengths, scale=scale)[..., 0].double()
+        w = (scale * q[..., 0].double()).exp()
+        want = w / (1.0 + w)
+        # A score of one product, exact, of at most 6: log2 e, the product with it and the difference from the maximum round it by 3 x 6 steps of 2^-24 absolute, which the
+        # exponential makes relative; its own step is 2^-23. Three parts of eight bits leave 2^-24 of w, the sums, the reciprocal and the product with it 6 x 2^-24.
+        relative = (18 + 2 + 1 + 6) * F32
+        half, tiny = torch.finfo(dtype).eps / 2, torch.finfo(dtype).tiny
+        step = half * torch.exp2(want.clamp(min=tiny).log2().floor())  # half of the step at this very value
+        over = ((got - want).abs() - step) / want
+        assert (over <= relative * (1 + 2 * half)).all(), (over.max(), (over > relative * (1 + 2 * half)).sum())
