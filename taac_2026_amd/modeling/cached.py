@@ -51,9 +51,12 @@ class CachedAttention(nn.Module):
         q, k, v = (t.transpose(1, 2) for t in rows.unflatten(-1, (-1, self.head_dim)).split((self.num_heads, self.key_heads, self.key_heads), 2))
         return *head_norm_rope(q, k, self.query_weight, self.key_weight, table=self.table, starts=starts, interleaved=self.interleaved), v
 
+    def _require_positions(self, tokens: int) -> None:
+        if tokens > self.max_tokens:
+            raise ValueError(f"CachedAttention has positions for {self.max_tokens} tokens, got {tokens}")
+
     def _attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengths: torch.Tensor | None) -> torch.Tensor:
-        if q.shape[2] > self.max_tokens:
-            raise ValueError(f"CachedAttention has positions for {self.max_tokens} tokens, got {q.shape[2]}")
+        self._require_positions(q.shape[2])
         group = self.num_heads // self.key_heads
         if group > 1:
             k, v = k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)
@@ -71,6 +74,7 @@ class CachedAttention(nn.Module):
 
     def prefill(self, tokens: torch.Tensor, cache: KVCache, pages: torch.Tensor, *, key_lengths: torch.Tensor | None = None) -> torch.Tensor:
         """:meth:`forward` of histories that begin here, whose keys and values go into the cache's ``pages (B, pages of a sample)``. Forward only."""
+        self._require_positions(tokens.shape[1])  # before anything is written
         q, k, v = self._project(tokens.to(torch.bfloat16))
         kv_cache_write(cache, k, v, pages, lengths=key_lengths)
         return self._leave(self._attend(q, k, v, key_lengths), tokens.dtype)
@@ -79,9 +83,9 @@ class CachedAttention(nn.Module):
         """The next tokens (B, t, D) of sequences that have ``starts (B,)`` tokens in the cache, to which these are added. Forward only."""
         if key_lengths is not None:
             key_lengths = key_lengths.clamp(0, tokens.shape[1])
+        lengths = starts + (tokens.shape[1] if key_lengths is None else key_lengths)
         q, k, v = self._project(tokens.to(torch.bfloat16), starts)
         kv_cache_write(cache, k, v, pages, starts, lengths=key_lengths)
-        lengths = starts + (tokens.shape[1] if key_lengths is None else key_lengths)
         return self._leave(cached_attention(q, cache, pages, lengths, query_lengths=key_lengths), tokens.dtype)
 
 

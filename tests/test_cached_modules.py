@@ -200,3 +200,18 @@ def test_step_in_a_replayed_graph(device):
 def test_positions_behind_the_table():
     with pytest.raises(ValueError, match="positions for 8 tokens"):
         CachedAttention(64, 2, max_tokens=8)._attend(torch.zeros(1, 2, 9, 32), torch.zeros(1, 2, 9, 32), torch.zeros(1, 2, 9, 32), None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("whole", [False, True])
+def test_a_refused_prefill_leaves_the_cache(device, whole):
+    """More tokens than there are positions: nothing is written, whatever the samples' lengths."""
+    block = _make(device, dict(SIZES[0], max_tokens=8), seed=5)
+    cache = block.attention.empty_cache(4, device, page_tokens=16)
+    cache.data.copy_(torch.randint(0, 100, cache.data.shape, generator=torch.Generator().manual_seed(1), dtype=torch.uint8))
+    before = cache.data.clone()
+    pages = torch.arange(2, device=device)[:, None]
+    lengths = None if whole else torch.tensor([9, 3], device=device)
+    with torch.no_grad(), pytest.raises(ValueError, match="positions for 8 tokens"):
+        block.prefill(torch.randn(2, 9, 64, device=device), cache, pages, key_lengths=lengths)
+    assert torch.equal(cache.data, before)
