@@ -657,7 +657,7 @@ int taac_delta_rule_step(const void* q, const void* k, const void* v, const void
  * q: logical (B, H, T, d), k: (B, key_heads, T, d) of dtype (fp32, bf16 or fp16), d at most 512; *_strides: ELEMENT strides of (batch, head,
  * token), the features of a row contiguous. With weights [d] of dtype (both or neither) every row becomes x rsqrt(mean(x^2) + eps) weight; then the
  * pairs of the first `rotary` features (even, at most d; 0: none) turn by (c, s) = table[position][pair]: (a, b) -> (a c - b s, a s + b c), pairs (2i, 2i + 1) if
- * interleaved, else (i, i + rotary / 2). table: fp32 [places, rotary / 2, 2], at most 2^31 - 1 places, or NULL with rotary 0. positions: int32 or int64 (positions_int64) with element strides
+ * interleaved, else (i, i + rotary / 2). table: fp32 [places, rotary / 2, 2], at most 2^31 - 1 places, or NULL with rotary 0 or without places. positions: int32 or int64 (positions_int64) with element strides
  * of (sample, token), the token's number added where add_token; or NULL: the token's number. A position outside the table gives NaN in the
  * rotated features. fp32 arithmetic, one rounding. The outputs may be the inputs (with their strides).
  * taac_head_norm_rope_bwd: grad_q, grad_k and, with weights, grad_qw and grad_kw [d], for the gradients grad_qo, grad_ko of the outputs; q and k are not

@@ -30,7 +30,7 @@ struct RopeParams {
   const void* w[2];       // [d] each, or null: no norm
   float* partial;         // backward: [workgroups][2][d]
   int64_t xs[2][3], gs[2][3], ys[2][3];  // element strides of (batch, head, token)
-  const float* table;     // [places][rotary / 2][2] or null
+  const float* table;     // [places][rotary / 2][2]; null without places or rotation
   const void* positions;  // null: the position is the token's number
   int64_t ps[2];          // of (sample, token), words of 32 bits
   int64_t places;
@@ -237,7 +237,7 @@ struct Angles {
   // without a branch, which would await what was asked for before it
   template <int L, int VEC, bool INTER>
   __device__ __forceinline__ void load(const RopeParams& p, const Walk& at, const Cursor<const int32_t>& place, const Lane<L, VEC, INTER>& lane) {
-    if (p.table == nullptr) return;
+    if (p.rotary == 0) return;
     int64_t position = at.t;
     if (p.positions != nullptr) {
       position = p.pos_int64 ? *reinterpret_cast<const int64_t*>(place.p) : *place.p;
@@ -260,7 +260,7 @@ struct Angles {
   }
   template <bool BACK, int L, int VEC, bool INTER>
   __device__ __forceinline__ void turn(const RopeParams& p, const Lane<L, VEC, INTER>& lane, float (&v)[8]) {
-    if (p.table == nullptr || (VEC != kSingles && lane.pair[0] < 0)) return;  // of runs all pairs are turned or none
+    if (p.rotary == 0 || (VEC != kSingles && lane.pair[0] < 0)) return;  // of runs all pairs are turned or none
     if (!inside) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) c[e] = s[e] = __builtin_nanf("");
@@ -467,7 +467,8 @@ int take_rope(const char* name, RopeParams& p, const void* q, const void* k, voi
   if (d > kMaxHeadWidth) return set_error(TAAC_ERR_UNSUPPORTED, "%s: a head has at most %d features (got %d)", name, kMaxHeadWidth, d);
   if (H > kMaxHeads || key_heads > kMaxHeads) return set_error(TAAC_ERR_UNSUPPORTED, "%s: at most %d heads", name, kMaxHeads);
   if (rotary < 0 || rotary > d || rotary % 2 != 0) return set_error(TAAC_ERR_INVALID_VALUE, "%s: the rotated features must be an even number, at most the head's (got %d of %d)", name, rotary, d);
-  if ((rotary > 0) != (table != nullptr) || places < 0) return set_error(TAAC_ERR_INVALID_VALUE, "%s: a table comes with rotated features, its size not negative", name);
+  // a table of no places may have no address
+  if (places < 0 || (table != nullptr && rotary == 0) || (table == nullptr && rotary > 0 && places > 0)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: a table comes with rotated features, its size not negative", name);
   if (places > 0x7fffffff) return set_error(TAAC_ERR_UNSUPPORTED, "%s: a table has at most 2^31 - 1 positions", name);
   if ((qw == nullptr) != (kw == nullptr)) return set_error(TAAC_ERR_INVALID_VALUE, "%s: both norm weights or neither", name);
   if (dtype != TAAC_F32 && dtype != TAAC_BF16 && dtype != TAAC_F16) return set_error(TAAC_ERR_INVALID_VALUE, "%s: unknown dtype %d", name, dtype);

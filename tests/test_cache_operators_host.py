@@ -237,3 +237,16 @@ def test_cache_entry_points_check_on_the_host():
             assert need == max(asked)
     assert library.taac_cached_attention_workspace_bytes(1024, 8, 8, 1, 32, 4, 512) == 0  # enough samples to fill the card
     assert library.taac_cached_attention_workspace_bytes(1, 3, 2, 1, 32, 4, 512) == -1 and library.taac_cached_attention_workspace_bytes(1, 2, 2, 1, 32, 6, 512) == -1
+
+
+def test_a_table_of_no_places_is_one():
+    """Its pointer is null, and every position lies outside it."""
+    library = _native.load_library()
+    fake, s = ctypes.c_void_p(256), (ctypes.c_int64 * 3)(96, 32, 32)
+
+    def forward(tokens, rotary, table, places):
+        return library.taac_head_norm_rope_fwd(fake, fake, fake, fake, 1, 2, 1, tokens, 32, rotary, s, s, s, s, fake, fake, 1e-6, table, places, None, 0, None, 0, 0,
+                                               _native.TAAC_BF16, None)
+
+    assert forward(0, 16, None, 0) == _native.TAAC_OK
+    assert forward(0, 16, None, 1) == _native.TAAC_ERR_INVALID_VALUE and forward(0, 0, fake, 0) == _native.TAAC_ERR_INVALID_VALUE

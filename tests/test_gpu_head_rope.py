@@ -272,3 +272,22 @@ def test_captured_with_attention(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(captured, step()))
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("width,rotary", [(32, 16), (38, 18)])
+def test_a_table_without_places(device, norm, width, rotary):
+    """Every position lies outside: the rotated features and their gradients are NaN, the others as ever."""
+    q, k, weights = _inputs(device, 2, 5, 2, 1, width, torch.float32, seed=8, norm=norm)
+    leaves = [t.requires_grad_(True) for t in (q, k)]
+    out = head_norm_rope(q, k, *weights, table=rotary_table(0, rotary, device=device))
+    for x, o, w in zip((q, k), out, weights):
+        assert o[..., :rotary].isnan().all()
+        want = oracle.head_norm_rope(x.detach(), w, None)[..., rotary:]
+        assert ((o[..., rotary:].double() - want).abs() <= (width + 16) * F32 * want.abs()).all()
+    grads = [torch.randn_like(t) for t in out]
+    for got, grad in zip(torch.autograd.grad(out, leaves, grads), grads):
+        if norm:  # the mean over the head brings them all together
+            assert got.isnan().all()
+        else:
+            assert got[..., :rotary].isnan().all() and torch.equal(got[..., rotary:], grad[..., rotary:])
