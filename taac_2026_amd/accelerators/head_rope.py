@@ -15,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from taac_2026_amd import _native
-from taac_2026_amd.accelerators.tensor_validation import require_cuda_tensors, require_inference, require_same_dtype
+from taac_2026_amd.accelerators.tensor_validation import require_cuda_tensors, require_inference, require_no_tangents, require_same_dtype
 
 MAX_HEAD_WIDTH = 512
 MAX_COUNT = 2**31 - 1  # the library counts samples and tokens in 32 bits
@@ -166,7 +166,7 @@ def head_norm_rope(
     int64; the rotated features of a token at a position that the table does not have come out as NaN.
 
     float32, bfloat16 or float16; a head has at most 512 features. Arithmetic in float32, rounded once. Differentiable in q, k and the
-    weights."""
+    weights, backwards; dual tensors are refused."""
     name = "head_norm_rope"
     q_shape, k_shape = q.shape, k.shape
     if len(q_shape) != 4 or len(k_shape) != 4:
@@ -201,6 +201,7 @@ def head_norm_rope(
             raise ValueError(f"{name} expects a table of shape (places, rotated / 2, 2) with at most the head's features")
         if table.dtype != torch.float32 or not table.is_contiguous():
             raise ValueError(f"{name} table must be contiguous float32")
+    require_no_tangents(f"hip {name}", q, k, query_weight, key_weight, table)
     require_cuda_tensors(f"hip {name}", q, k, query_weight, key_weight, table, place)
     if q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise RuntimeError(f"hip {name} does not support dtype {q.dtype}")

@@ -15,7 +15,7 @@ import torch
 
 from taac_2026_amd import _native
 from taac_2026_amd.accelerators.head_rope import MAX_COUNT, strides_of, token_major
-from taac_2026_amd.accelerators.tensor_validation import require_cuda_tensors, require_inference, require_same_dtype
+from taac_2026_amd.accelerators.tensor_validation import require_cuda_tensors, require_inference, require_no_tangents, require_same_dtype
 
 CACHED_WIDTHS = (32, 64, 128)
 _CHUNK = 16
@@ -125,6 +125,7 @@ def kv_cache_write(
     _check_pages(name, pages, batch)
     starts = None if starts is None else _integers(name, "starts", starts, batch)
     lengths = _lengths(name, "lengths", lengths, batch)
+    require_no_tangents(f"hip {name}", k, v)
     require_cuda_tensors(f"hip {name}", cache.data, k, v, pages, starts, lengths)
     require_inference(f"hip {name}", k, v)
     if k.dtype not in _DTYPES:
@@ -209,6 +210,7 @@ def cached_attention(
     query_lengths = _lengths(name, "query_lengths", query_lengths, batch)
     if window is not None and (int(window) != window or window <= 0):
         raise ValueError(f"{name} window must be a number of tokens above zero")
+    require_no_tangents(f"hip {name}", q)
     require_cuda_tensors(f"hip {name}", q, cache.data, pages, lengths, query_lengths)
     require_inference(f"hip {name}", q)
     if q.dtype not in (torch.bfloat16, torch.float16):

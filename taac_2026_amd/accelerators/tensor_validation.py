@@ -10,6 +10,7 @@ from __future__ import annotations
 from collections.abc import Iterable
 
 import torch
+from torch.autograd import forward_ad
 
 
 def concrete_tensors(tensors: Iterable[torch.Tensor | None]) -> tuple[torch.Tensor, ...]:
@@ -62,10 +63,19 @@ def require_inference(operator_name: str, *tensors: torch.Tensor | None) -> None
         )
 
 
+def require_no_tangents(operator_name: str, *tensors: torch.Tensor | None) -> None:
+    """Forward-mode differentiation does not reach the HIP kernels: refuse to silently drop a tangent."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual tensors without a level: a step of a short call's host time
+        return
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in concrete_tensors(tensors)):
+        raise RuntimeError(f"{operator_name} has no forward-mode derivative: call it on tensors without tangents")
+
+
 __all__ = [
     "concrete_tensors",
     "require_cuda_tensors",
     "require_inference",
+    "require_no_tangents",
     "require_same_device",
     "require_same_dtype",
 ]

@@ -250,3 +250,23 @@ def test_a_table_of_no_places_is_one():
 
     assert forward(0, 16, None, 0) == _native.TAAC_OK
     assert forward(0, 16, None, 1) == _native.TAAC_ERR_INVALID_VALUE and forward(0, 0, fake, 0) == _native.TAAC_ERR_INVALID_VALUE
+
+
+def test_tangents_are_refused():
+    """Whatever carries one; without any, a level of forward-mode differentiation changes nothing."""
+    from torch.autograd import forward_ad
+
+    q, w, table = torch.zeros(2, 4, 3, 32), torch.ones(32), rotary_table(8, 16)
+    cache, pages, lengths = empty_kv_cache(6, 4, 32, page_tokens=16, device="cpu"), torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    calls = (
+        (lambda q, k, wq, wk, table: head_norm_rope(q, k, wq, wk, table=table), (q, q, w, w, table)),
+        (lambda k, v: kv_cache_write(cache, k, v, pages), (q, q)),
+        (lambda q: cached_attention(q, cache, pages, lengths), (q.bfloat16(),)),
+    )
+    with forward_ad.dual_level():
+        for call, arguments in calls:
+            with pytest.raises(RuntimeError, match="CUDA tensors"):
+                call(*arguments)
+            for i, t in enumerate(arguments):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*arguments[:i], forward_ad.make_dual(t, torch.ones_like(t)), *arguments[i + 1:])
