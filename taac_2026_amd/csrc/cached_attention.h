@@ -99,6 +99,7 @@ __host__ __device__ constexpr int lds_bytes(int rows, int d, int bits, int parts
 }
 constexpr float kNothing = -3e38f; // the maximum of no scores
 constexpr float kSlack = 8.f;
+constexpr float kFar = 1048576.f;  // a maximum whose own rounding, half of 2^-3, is what a product that is not rounded may differ by from it
 
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -811,6 +812,7 @@ __device__ __forceinline__ void attend_many(const AttendParams& p, const Job& jo
   const bf16x8 ones = __builtin_bit_cast(bf16x8, (u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}));
   f32x4 s[RT][4];
   bf16x8 probs[RT][2][2];
+  bool far = false;  // the same in all lanes
   auto scores = [&](const uint8_t* keys_at) __attribute__((always_inline)) {
     Words<BLOCKS * BITS / 4> keys[4];
     float scale[4];
@@ -857,18 +859,31 @@ __device__ __forceinline__ void attend_many(const AttendParams& p, const Job& jo
       above |= top[n] > most[n] + kSlack;
     }
     if (__any(above)) {
+      bool beyond = false;
 #pragma unroll
       for (int n = 0; n < RT; ++n) {
         const float t = fmaxf(most[n], max_over_rows(top[n]));
         const float f = __builtin_amdgcn_exp2f(most[n] - t);
         most[n] = t;
+        beyond |= t > kNothing && fabsf(t) > kFar;
         sums[n][0] *= f;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[n * (D / 16) + i][e] *= f;
       }
+      far = __any(beyond);
     }
+    // Product and difference are one instruction, whose product is not rounded as the maximum is. Scores in the billions would differ from their own maximum by that: such
+    // are rounded first.
+    if (far) {
+#pragma clang fp contract(off)
+#pragma unroll
+      for (int n = 0; n < RT; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i / 4][i % 4] *= p.scale;
+    }
+    const float factor = far ? 1.f : p.scale;
 #pragma unroll
     for (int n = 0; n < RT; ++n)
 #pragma unroll
@@ -877,7 +892,7 @@ __device__ __forceinline__ void attend_many(const AttendParams& p, const Job& jo
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[c][e] = __builtin_amdgcn_exp2f(fmaf(s[n][2 * half + c][e], p.scale, -most[n]));
+          for (int e = 0; e < 4; ++e) x[c][e] = __builtin_amdgcn_exp2f(fmaf(s[n][2 * half + c][e], factor, -most[n]));
         two_parts(x[0], x[1], probs[n][0][half], probs[n][1][half]);
         sums[n] = mfma(ones, probs[n][0][half], sums[n]);
         sums[n] = mfma(ones, probs[n][1][half], sums[n]);

@@ -387,3 +387,42 @@ def test_probabilities_of_few_rows(device, dtype, group, samples):
         step = half * torch.exp2(want.clamp(min=tiny).log2().floor())  # half of the step at this very value
         over = ((got - want).abs() - step) / want
         assert (over <= relative * (1 + 2 * half)).all(), (over.max(), (over > relative * (1 + 2 * half)).sum())
+
+
+def _same_scores(device, bits, group, tokens, cached, key, query, scale):
+    """All scores of a call the same number, 32 key query scale: a query that sees tokens gets their values' mean."""
+    lengths = [cached, 33, 0]
+    cache, pages, _, v = _filled(device, lengths, 1, 32, bits, 64)
+    kv_cache_write(cache, torch.full((3, 1, cached, 32), key, device=device), v.float(), pages, lengths=torch.tensor(lengths, device=device))
+    q = torch.full((3, group, tokens, 32), query, device=device, dtype=torch.bfloat16)
+    got = cached_attention(q, cache, pages, torch.tensor(lengths, device=device), scale=scale)
+    _check(got.transpose(1, 2).contiguous().transpose(1, 2), q, torch.zeros_like(v), v, lengths, [tokens] * 3)
+
+
+FORMS = [(1, 1, 40), (4, 1, 300), (9, 1, 300), (3, 12, 300), (1, 1, 9000), (2, 10, 9000)]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("group,tokens,cached", FORMS)
+def test_scores_of_any_size(device, bits, group, tokens, cached):
+    """A score in the billions and beyond is off by more than one by its rounding alone, which must not show in the weights."""
+    for power in (10, 31, 32, 33, 40, 60, 100):
+        for fraction in (1.296875, -1.1484375, 1.9921875, -1.671875):
+            _same_scores(device, bits, group, tokens, cached, 2.0 ** (power // 2), fraction * 2.0 ** (power - power // 2 - 5), 0.71)
+
+
+@pytest.mark.parametrize("group,tokens", [(1, 1), (4, 1), (9, 1), (3, 12)])
+def test_one_score_far_above(device, group, tokens):
+    """Scores in the billions, a step of float32 apart and more: the largest alone counts, wherever it stands."""
+    for top in (0, 31, 64, 170):
+        x = 2.0**20 * torch.ones(1, 1, 171, 32, device=device)
+        x[:, :, top, 7] *= 1.5
+        v = torch.randn(1, 1, 171, 32, generator=torch.Generator().manual_seed(top)).bfloat16().to(device)
+        cache, pages = empty_kv_cache(12, 1, 32, bits=8, page_tokens=16, device=device), torch.arange(12, device=device)[None]
+        kv_cache_write(cache, x, v.float(), pages)
+        q = torch.full((1, group, tokens, 32), 1.296875 * 2.0**10, device=device, dtype=torch.bfloat16)
+        for scale in (0.71, 0.3):
+            got = cached_attention(q, cache, pages, torch.tensor([171], device=device), scale=scale)
+            want = oracle.cached_values(v, 8)[0, 0, top]
+            sees = torch.arange(171 - tokens, 171, device=device) >= top
+            assert ((got[0, :, sees].double() - want).abs() <= 2.0**-8 * want.abs()).all()
