@@ -97,7 +97,7 @@ __host__ __device__ constexpr int working_bytes(int rows, int d, int bits, int w
 __host__ __device__ constexpr int lds_bytes(int rows, int d, int bits, int parts, int waves) {
   return working_bytes(rows, d, bits, waves) + (queries_in_lds(rows, parts) ? rows * d * 2 : 0) + stats_bytes(rows, shape_of(rows, d, waves).waves);
 }
-constexpr float kNothing = -3e38f; // the maximum of no scores
+constexpr float kNothing = -3.402823466e38f;  // the maximum of no scores: no finite one is below
 constexpr float kSlack = 8.f;
 constexpr float kFar = 1048576.f;  // a maximum whose own rounding, half of 2^-3, is what a product that is not rounded may differ by from it
 

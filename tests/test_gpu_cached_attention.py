@@ -426,3 +426,14 @@ def test_one_score_far_above(device, group, tokens):
             want = oracle.cached_values(v, 8)[0, 0, top]
             sees = torch.arange(171 - tokens, 171, device=device) >= top
             assert ((got[0, :, sees].double() - want).abs() <= 2.0**-8 * want.abs()).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("group,tokens,cached", FORMS)
+def test_scores_at_the_end_of_float32(device, bits, group, tokens, cached):
+    """Among the most negative numbers that there are, which are scores still: the values' mean, not the zeros of a query that sees nothing."""
+    # 32 products of 2^60 and 1.296875 2^62 are 1.296875 2^127; times log2 e 1.8710 2^127, and 1.9879 2^127 with the second scale, of the 2^128 that there are
+    for sign in (-1.0, 1.0):
+        for scale in (1.0, 1.0625):
+            _same_scores(device, bits, group, tokens, cached, 2.0**60, 1.296875 * 2.0**62, sign * scale)
+            _same_scores(device, bits, group, tokens, cached, 2.0**60, -1.296875 * 2.0**62, sign * scale)
