@@ -54,7 +54,7 @@ def rotary_table(
     trained_places: int | None = None,
     turns: tuple[float, float] = (1.0, 32.0),
     magnitude: float = 1.0,
-    device: torch.device | str = "cpu",
+    device: torch.device | str | None = None,
 ) -> torch.Tensor:
     """Float32 ``(places, rotary_dim / 2, 2)`` of ``magnitude (cos, sin)(position * frequency)`` with ``frequency_i = base ** (-2 i / rotary_dim)``, angles in 64
     bits, for :func:`head_norm_rope`.
@@ -67,7 +67,8 @@ def rotary_table(
         raise ValueError("rotary_table needs a number of places that is not negative and an even number of rotated features above zero")
     if not (base > 0.0 and factor > 0.0) or not math.isfinite(base) or not math.isfinite(factor):
         raise ValueError("rotary_table needs base and factor above zero")
-    frequencies = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    device = torch.get_default_device() if device is None else device
+    frequencies = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device="cpu") / rotary_dim)
     if trained_places is None:
         frequencies = frequencies / factor
     else:

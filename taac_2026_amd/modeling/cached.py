@@ -37,9 +37,12 @@ class CachedAttention(nn.Module):
         self.register_buffer("table", rotary_table(*self._rotary[0], **self._rotary[1]), persistent=False)
 
     def _apply(self, fn, recurse: bool = True):
+        kept = self.table
         super()._apply(fn, recurse)
-        if self.table.dtype != torch.float32:  # angles of far positions keep their digits whatever type the weights take
-            self.table = rotary_table(*self._rotary[0], **self._rotary[1], device=self.table.device)
+        # Only the device follows: angles of far positions keep their digits whatever type the weights take, and a table is no part of a state that is loaded
+        # into room without data.
+        device = self.table.device
+        self.table = rotary_table(*self._rotary[0], **self._rotary[1], device=device) if kept.is_meta and device.type != "meta" else kept.to(device)
         return self
 
     def empty_cache(self, pages: int, device: torch.device | str, *, bits: int = 4, page_tokens: int = 64) -> KVCache:

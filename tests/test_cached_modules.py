@@ -215,3 +215,29 @@ def test_a_refused_prefill_leaves_the_cache(device, whole):
     with torch.no_grad(), pytest.raises(ValueError, match="positions for 8 tokens"):
         block.prefill(torch.randn(2, 9, 64, device=device), cache, pages, key_lengths=lengths)
     assert torch.equal(cache.data, before)
+
+
+def test_the_table_follows_the_module():
+    """Made on a device by torch's default, made without data and given room later, moved: always the angles, never what lay in memory."""
+    want = CachedAttention(64, 2, max_tokens=300, rotary_options=dict(factor=2.0)).table
+    options = dict(max_tokens=300, rotary_options=dict(factor=2.0))
+    with torch.device("meta"):
+        mixer = CachedAttention(64, 2, **options)
+    assert mixer.table.is_meta and mixer.query_weight.is_meta
+    assert torch.equal(mixer.to_empty(device="cpu").table, want)
+    mixer = CachedAttention(64, 2, **options).to_empty(device="cpu")
+    assert torch.equal(mixer.table, want) and torch.equal(mixer.half().float().table, want)
+    assert torch.equal(mixer.to("meta").to_empty(device="cpu").bfloat16().table, want)
+
+
+@pytest.mark.gpu
+def test_the_table_follows_the_module_to_the_gpu(device):
+    want = CachedAttention(64, 2, max_tokens=300).table
+    with torch.device(device):
+        block = CachedAttentionBlock(64, 2, 2, max_tokens=300)
+    assert block.attention.table.device == block.attention.query_weight.device
+    with torch.no_grad():
+        assert block(torch.randn(1, 5, 64, device=device)).isfinite().all()
+    for mixer in (block.attention, CachedAttention(64, 2, max_tokens=300).to(device), CachedAttention(64, 2, max_tokens=300).to_empty(device=device)):
+        # 64-bit cosines of a GPU may be off by a step of theirs, which a rounding to float32 can show
+        assert mixer.table.is_cuda and (mixer.table.double().cpu() - want.double()).abs().max() <= 2.0**-23
