@@ -686,7 +686,8 @@ int taac_head_norm_rope_bwd(const void* q, const void* k, const void* grad_qo, c
  * table: [B, table_pages] int32 or int64 (table_int64), rows table_stride elements apart: the pages of a sample's positions in order. A page outside
  * the pool, or a position behind the table, is no place: not written, read as zeros, not attended to.
  * write: token t of sample b, k and v logical (B, heads, T, d), goes to position starts[b] + t (starts int32, int64 (starts_int64) or NULL: 0), for t <
- * lengths[b] (NULL: T). A token of which k or v has a NaN or an infinity in a head reads back as NaN there. Two tokens of one call must not share a place.
+ * lengths[b] (NULL: T); all of a sample whose start is negative, or 2^40 and more, has no place. A token of which k or v has a NaN or an infinity in a head
+ * reads back as NaN there. Two tokens of one call must not share a place.
  * read: the other way round, zeros for t >= lengths[b]. ELEMENT strides of (batch, head, token), multiples of 16 bytes; 16-byte aligned tensors of fp32, bf16
  * or fp16.
  */

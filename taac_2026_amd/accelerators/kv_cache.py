@@ -111,7 +111,7 @@ def kv_cache_write(
 ) -> None:
     """Quantises ``k, v (batch, key heads, tokens, width)`` into the cache: token t of a sample to position ``starts[b] + t`` (without starts: t), i.e. into page
     ``pages[b, position // page_tokens]``. ``lengths (batch,)``: the tokens that a sample really has; the others are not read. A token whose page is not in the
-    table or not in the pool (-1 for a padded sample) is left out. Places that two tokens of a call share hold a mixture of both afterwards.
+    table or not in the pool (-1 for a padded sample) is left out, and all of a sample whose start is negative. Places that two tokens of a call share hold a mixture of both afterwards.
 
     float32, bfloat16 or float16. A token whose key or value, in a head, has a NaN or an infinity is stored as NaN there. Forward only."""
     name = "kv_cache_write"
@@ -151,7 +151,7 @@ def kv_cache_read(
     dtype: torch.dtype = torch.bfloat16,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """``(k, v)`` of ``tokens`` positions from ``starts[b]`` on (without starts: 0), the values that the codes stand for, as (batch, key heads, tokens, width) in memory
-    order (batch, tokens, heads, width). Positions at or beyond ``lengths[b]`` tokens, and those in no page of the pool, are zeros. Exact in bfloat16 and
+    order (batch, tokens, heads, width). Positions at or beyond ``lengths[b]`` tokens, and those in no page of the pool, are zeros, as is all of a sample whose start is negative. Exact in bfloat16 and
     float32; in float16 where it reaches."""
     name = "kv_cache_read"
     batch = pages.shape[0] if pages.ndim == 2 else -1
