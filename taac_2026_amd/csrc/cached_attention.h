@@ -552,10 +552,11 @@ __device__ __forceinline__ void times_values(const uint8_t* code_bytes, const ui
   }
 }
 
-// A wavefront's tiles, S of them in LDS: S - 1 on their way while one is taken. Its only vector-memory operations are the transfers, so that their count says
-// what has arrived.
+// A wavefront's tiles, two of them in LDS: one on its way while the other is taken. Its only vector-memory operations are the transfers, so that their count says
+// what has arrived. No barrier: a wavefront reads what it brought itself, with loads of the compiler's, which the waits in front of them keep in place (ts_common.h).
 template <int D, int BITS, int W, int S, bool WHOLE, typename Take>
 __device__ __forceinline__ void walk(const AttendParams& p, const Job& job, const Span& span, int wave, int lane, uint8_t* stages, Take&& take) {
+  static_assert(S == 2, "the waits below count the requests of one tile");
   typedef Staged<D, BITS> Tile;
   const int64_t row = job.b * p.pool.table_stride;
   uint32_t held[S];
@@ -581,8 +582,6 @@ __device__ __forceinline__ void walk(const AttendParams& p, const Job& job, cons
         held[(i + S - 1) % S] = Tile::request(p.pool, pages, job.head, next, stages + (i + S - 1) % S * Tile::BYTES, lane);
         next += W;
         pages.find(p.pool, row, next);
-        vm_wait<(S - 1) * Tile::REQUESTS>();
-      } else if (S > 2 && next - tile > W) {
         vm_wait<Tile::REQUESTS>();
       } else {
         vm_wait<0>();

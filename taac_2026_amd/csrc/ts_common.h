@@ -21,8 +21,11 @@ __device__ __forceinline__ uint32_t lds_offset(const void* lds_ptr) {
 // Consequences: the compiler does not know about these transfers at all, so (1) completion is awaited by hand with
 // vm_wait<N>() - the operations of the vector-memory counter complete in issue order, N = number of vector-memory
 // instructions this wavefront issued after the transfer, and a count that is too small only waits longer - and
-// (2) the LDS bytes they write must only be read through the hand-issued lds_read_* below, after such a wait and a
-// workgroup barrier.
+// (2) the LDS bytes they write must only be read after such a wait and, where another wavefront asked for them, a
+// workgroup barrier. Reads that are scheduled by hand around later transfers are the hand-issued lds_read_* below. Loads of
+// the compiler's are right too: the wait's memory clobber keeps them behind it, and the transfers' own one, whose LDS
+// address comes from a pointer into the same array, keeps them in front of a transfer to the same place; that the reads
+// have been done by then takes a wait for lgkmcnt(0).
 __device__ __forceinline__ void lds_dma16(const void* gsrc, void* lds_wave_base) {
   const uint32_t base = __builtin_amdgcn_readfirstlane(lds_offset(lds_wave_base));
   asm volatile(
