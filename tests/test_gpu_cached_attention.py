@@ -437,3 +437,38 @@ def test_scores_at_the_end_of_float32(device, bits, group, tokens, cached):
         for scale in (1.0, 1.0625):
             _same_scores(device, bits, group, tokens, cached, 2.0**60, 1.296875 * 2.0**62, sign * scale)
             _same_scores(device, bits, group, tokens, cached, 2.0**60, -1.296875 * 2.0**62, sign * scale)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("width", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_wavefront_to_a_unit(device, bits, width, dtype):
+    """1024 samples of 8 key heads: as many units as any form needs to give each a wavefront alone. Thirty-two histories, of which every sample sees a part of its own."""
+    samples, kv_heads = 1024, 8
+    g = torch.Generator().manual_seed(width + bits)
+    lengths = torch.randint(0, 201, (samples // 2,), generator=g)
+    lengths[:10] = torch.tensor([0, 1, 63, 64, 65, 127, 128, 129, 200, 199])
+    lengths = lengths.repeat(2)
+    checked = slice(0, 48)
+    for page in (16, 64):
+        cache, pages, k, v = _filled(device, [200] * 32, kv_heads, width, bits, page, stale=False)
+        which = torch.arange(samples) % 32
+        table = pages[which.to(device)].contiguous()
+        for group, tokens, window in ((1, 1, None), (2, 1, 70), (1, 2, None), (3, 1, None), (1, 4, 65), (5, 1, None), (2, 8, None), (1, 16, 90)):
+            news = torch.randint(0, tokens + 1, (samples // 2,), generator=g).clamp(min=1 if tokens == 1 else 0).repeat(2)
+            q = _queries(device, samples // 2, kv_heads * group, tokens, width, dtype, seed=group)
+            got = cached_attention(torch.cat((q, q)), cache, table, lengths.to(device), query_lengths=news.to(device), window=window)
+            mine = which[checked].to(device)
+            _check(got[checked], q[checked], k[mine], v[mine], lengths[checked].tolist(), news[checked].tolist(), window)
+            assert torch.equal(got[: samples // 2], got[samples // 2:])  # of the same histories, other workgroups
+
+
+@pytest.mark.parametrize("bits,width,dtype", [(4, 32, torch.bfloat16), (8, 64, torch.float16), (8, 128, torch.bfloat16)])
+@pytest.mark.parametrize("group,tokens,window", [(1, 300, None), (4, 257, 333)])
+def test_hundreds_of_new_tokens(device, bits, width, dtype, group, tokens, window):
+    """A prompt continued over what is cached, and one that begins."""
+    lengths, news = [1500, 700, 257, 40, 900], [tokens, tokens - 31, tokens, 40, 0]
+    cache, pages, k, v = _filled(device, lengths, 2, width, bits, 32)
+    q = _queries(device, 5, 2 * group, tokens, width, dtype)
+    got = cached_attention(q, cache, pages, torch.tensor(lengths, device=device), query_lengths=torch.tensor(news, device=device), window=window)
+    _check(got, q, k, v, lengths, news, window)
