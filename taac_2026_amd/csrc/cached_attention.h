@@ -20,10 +20,10 @@
 // other, where a third would be half as many products with the values again, and outputs of 16 bits are off by their own rounding either way. The maximum moves when a score exceeds it
 // by a factor of 2^8, which cancels.
 //
-// Measured: 4 samples of 65536 tokens, 32 heads over 8 of 128 features in 4 bits: 50 us and 5 for the join, 5.6 TB/s of the cache (tiles in registers, one ahead: 101, for the
-// registers left one wavefront to a SIMD, and page numbers that wait behind the rows). 1024 samples of up to 512 tokens, 8 heads of 32: 22 us, of which 8 are a launch whose
-// samples have one tile, and 2.7 every tile more, 6.7 TB/s. 64 samples of 2048 tokens, 24 queries of 8 heads over 4 of 128 in 8 bits: 34 us, of up to 2048 tokens and up to 24
-// queries 27. A tile of 32 rows has 104 matrix and 524 vector instructions there, of which 270 convert the codes; those of one wavefront do not overlap (six products with three
+// Measured: 4 samples of 65536 tokens, 32 heads over 8 of 128 features in 4 bits: 51 us and 5 for the join, 5.6 TB/s of the cache (tiles in registers, one ahead: 101, for the
+// registers left one wavefront to a SIMD, and page numbers that wait behind the rows). 1024 samples of up to 512 tokens, 8 heads of 32: 23 us; of one tile each 9.5,
+// and 2.8 every tile more, 6.4 TB/s. 64 samples of 2048 tokens, 24 queries of 8 heads over 4 of 128 in 8 bits: 34 us, of up to 2048 tokens and up to 24
+// queries 27. A tile of 32 rows has 104 matrix and some 530 vector instructions there, of which 270 convert the codes; those of one wavefront do not overlap (six products with three
 // additions behind each take 184 cycles, the products alone 120, the additions alone 72), those of two do in part. The end of a
 // workgroup (its wavefronts' sums joined, divided, written) is shared by all of them: done by the first one it took half of a call with one tile of 48 rows, 7 of 15 us.
 #pragma once

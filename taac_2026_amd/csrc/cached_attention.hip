@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void cached_attention_join_kernel(const Attend
 // ---- the host -----------------------------------------------------------------------------------------------------
 
 constexpr int64_t kOccupied = 192;  // units: most of 256 CUs have one
-constexpr int64_t kMostGroups = 1 << 23;  // of a launch: below 2^31 threads
+constexpr int64_t kMostGroups = 1 << 23;  // of a launch: at most 2^31 threads in workgroups of four wavefronts, of the 2^32 - 1 that a launch may have; eight are for 256 units
 
 // How a call is cut. A unit is a tile of rows of a key head of a sample.
 struct Plan {
@@ -81,10 +81,12 @@ struct Plan {
   int waves;      // of a workgroup: 1, 4 or 8
 };
 
-// From so many units on a wavefront takes one alone, without the meeting; below, four share its tokens. Medians of ragged histories, alone : shared, in us:
-//   up to 4 rows, 32 features: 9.2 : 14.0 at 4096 units of up to 256 tokens, 22.4 : 24.5 of 1024; 11.0 : 8.8 and 18.3 : 14.9 at 2048
-//   64 features: 9.3 : 15.0 at 2048 units of 256, 22.7 : 25.3 of 1024; 10.7 : 9.5 and 17.7 : 16.6 at 1024; 128 alike
-//   16 rows, 64 features: 27.9 : 36.2 at 8192 units of 256, 42.8 : 46.4 of 512; 17.7 : 21.0 of 256 and 46.6 : 38.9 of 1024 at 4096
+// From so many units on a wavefront takes one alone, without the meeting; below, four share its tokens. Ragged histories, alone : shared, in us:
+//   up to 4 rows, 32 features: 9.9 : 14.0 at 4096 units of up to 256 tokens, 23.6 : 24.2 of 1024; 7.0 : 8.7 and 18.4 : 14.9 at 2048
+//   64 features: 9.5 : 14.9 at 2048 units of 256, 23.3 : 25.8 of 1024; 7.3 : 9.4 and 17.9 : 17.0 at 1024
+//   128 features: 16.0 : 28.5 at 2048 units of 256, 39.3 : 45.2 of 1024; 10.3 : 15.2 and 25.6 : 28.0 at 1024
+//   16 rows, 64 features: 26.0 : 37.2 at 8192 units of 256, 40.0 : 47.6 of 512; 16.6 : 21.2 of 256 and 45.0 : 39.1 of 1024 at 4096
+// Below the lines short histories are faster alone still, and with 128 features both; what long ones lose there decided.
 int64_t alone_from(int rows, int32_t d) { return rows > 4 ? 8192 : d == 32 ? 4096 : 2048; }
 
 // Tiles of so many rows.
@@ -113,8 +115,17 @@ Plan plan_of(int64_t B, int32_t heads, int32_t group, int32_t T, int32_t d, int 
   const int64_t rows = static_cast<int64_t>(group) * T;
   // up to 4 rows (2 in two parts) in the one form
   if (rows <= 2 || (rows <= 4 && !parts)) return cut(B, heads, rows, rows <= 2 ? static_cast<int>(rows) : 4, false, d, bits, held, parts);
-  // 16 rows where a workgroup to a CU fills the card: eight wavefronts, and no splits. 8 rows of 4 key heads, four with splits : eight, 64 samples of 1000 and 2500 tokens: of 64
-  // features in 8 bits 10.3 : 9.9 us and 22.8 : 18.6, in 4 bits 9.0 : 8.1 and 18.5 : 14.1, of 128 in 8 bits 19.8 : 16.9 and 33.7 : 31.0; 96 samples of 128 22.7 : 25.7 and 44.0 : 46.8.
+  // 16 rows where a workgroup to a CU fills the card: eight wavefronts, and no splits. 8 rows of 4 key heads, ragged histories, four with splits : eight, in us, at
+  //                                 128 units     192           256           288           384
+  //   32 features, 4 bits,  2500 tokens   10.5 :  9.5   12.3 :  9.7   12.4 :  9.7   13.2 : 11.5   14.8 : 13.2
+  //   64 features, 8 bits,   500           6.0 :  6.0    6.0 :  6.1    6.1 :  6.1    7.2 :  7.6    7.3 :  7.8
+  //                         1000           8.2 :  7.4    8.3 :  7.4    8.5 :  7.8    9.9 : 10.0   10.1 : 10.2
+  //                         2500          12.8 : 11.7   15.4 : 13.0   16.2 : 14.4   18.4 : 19.2   18.7 : 20.0
+  //                         8000          24.8 : 22.9   29.2 : 28.3   31.5 : 30.8   38.3 : 45.3
+  //   64 features, 4 bits,  8000          19.6 : 20.8   24.1 : 27.1   25.2 : 27.7   29.0 : 37.0
+  //   128 features, 8 bits, 1000          12.2 : 10.3   11.4 : 11.3   12.1 : 12.3   16.2 : 17.5   17.0 : 19.9
+  //                         2500          19.7 : 19.1   21.3 : 20.4   22.3 : 21.9   32.5 : 30.5   33.2 : 32.3
+  // Beyond 256 units a second round begins, which eight fill worse. Down to 128 they would be as fast or faster, but for the longest histories.
   if (rows <= 16) return cut(B, heads, rows, 16, B * heads >= kOccupied && B * heads <= 256, d, bits, held, parts);
   // In the other 16, or 32, which share the conversion of the codes. Where a workgroup of eight wavefronts to a CU just fills the card, up to 48 rows in one, which need no
   // splits and no joining; of four sixteens the sums would leave no registers. 4 key heads, 2000 tokens, 48 rows : 32: of 128 features in 8 bits, 18 rows, 48 samples 25.1 : 29.6

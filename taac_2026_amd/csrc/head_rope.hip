@@ -11,8 +11,8 @@
 // with one row of the table between them, or of a few tokens where a token has fewer heads. A lane keeps its head and walks the tokens: what a row costs besides
 // its features is a few additions. All arithmetic is fp32, rounded once at the end.
 //
-// Measured: 1024 x 512 tokens of 16 heads of 32 features in bf16, 1.07 GB, 209 to 213 us, 5.1 TB/s, where torch's copy of as much takes 200 (with a product and two divisions to a
-// row, an eighth more instructions, the same). 8 x 8192 tokens of 20 heads of 128: forward 148 us (4.5 TB/s), backward 200 (5.0), its partial rows 5.
+// Measured: 1024 x 512 tokens of 16 heads of 32 features in bf16, 1.07 GB, 211 to 215 us, 5.0 TB/s, where torch's copy of as much takes 200 (with a product and two divisions to a
+// row, an eighth more instructions, the same). 8 x 8192 tokens of 20 heads of 128: forward 146 us (4.6 TB/s), backward 200 (5.0), its partial rows 5.
 #include "norm_rows.h"
 
 namespace taac {

@@ -4,7 +4,7 @@
 // conversion.
 //
 // Measured: 512 histories of up to 512 tokens, 8 heads of 32 features in 4 bits: written in 55 us (183 MB, 3.3 TB/s), read in 54 (301 MB with the zeros, 5.6). 16 x 8000 tokens of 8
-// heads of 128 in 8 bits: 165 us (4.7 TB/s) and 149 (5.3). Writing was 58 and 180 when numbers became fp32 first and lanes exchanged through LDS: 281 and 740 vector
+// heads of 128 in 8 bits: 165 us (4.8 TB/s) and 154 (5.2). Writing was 58 and 180 when numbers became fp32 first and lanes exchanged through LDS: 281 and 740 vector
 // instructions of a wavefront, now 222 and 549. Two records of a wavefront at a time (122 us for both directions of the first, 115 then with one), the heads of a chunk in
 // turn at one address (122 to 139), more and fewer wavefronts were slower.
 #include "kv_cache.h"
