@@ -57,7 +57,7 @@ def rotary_table(
     device: torch.device | str | None = None,
 ) -> torch.Tensor:
     """Float32 ``(places, rotary_dim / 2, 2)`` of ``magnitude (cos, sin)(position * frequency)`` with ``frequency_i = base ** (-2 i / rotary_dim)``, angles in 64
-    bits, for :func:`head_norm_rope`.
+    bits, for :func:`head_norm_rope`, on ``device`` (torch's default).
 
     ``factor`` stretches positions for contexts longer than those a model was trained on: alone it divides every frequency. With ``trained_places``
     it does so by parts: frequencies that turn at most ``turns[0]`` times within them are divided, those that turn at least ``turns[1]`` times are kept, and the ones

@@ -89,7 +89,7 @@ struct Plan {
 // Below the lines short histories are faster alone still, and with 128 features both; what long ones lose there decided.
 int64_t alone_from(int rows, int32_t d) { return rows > 4 ? 8192 : d == 32 ? 4096 : 2048; }
 
-// Tiles of so many rows.
+// Tiles of so many rows. held: the table's tokens, whether a window sees them or not; splits that a window leaves without a tile end at once.
 Plan cut(int64_t B, int32_t heads, int64_t rows, int tile, bool wide, int32_t d, int bits, int64_t held, bool parts) {
   Plan plan{};
   plan.rows = tile;
